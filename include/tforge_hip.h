@@ -20,7 +20,12 @@
  * holds the message (the reference printed it and exited 1:
  * runners/gpu/tforge-gpu-bench.cu:52-70; the Python wrapper raises
  * RuntimeError with it, python/tforge_cpu.py:216-222).  Handles are not shared
- * between threads.  All tensors are row-major float32.
+ * between threads.  All tensors of compiled programs are row-major float32.
+ *
+ * Beside compiled programs the library has the operators of the residual MLP
+ * block in 16 and 8 bits, for training and serving (no counterpart in the
+ * reference): tf_rms_norm, tf_quantize_rows, tf_linear and the gradients
+ * tf_rms_norm_grad and tf_linear_grad, at the end of this file.
  */
 #ifndef TFORGE_HIP_H
 #define TFORGE_HIP_H
@@ -243,6 +248,124 @@ int tf_bench_samples(const tf_kernel_t *k, double *out_ms, int cap);
  * reference, which generates each kernel on demand. */
 int tf_registry_size(void);
 int tf_registry_entry(int i, int *family, int *cfg7, char *name, int name_cap);
+
+/* ---- operators of the residual MLP block --------------------------------------
+ *
+ * Plain calls on device pointers: no handle, no allocation, no synchronisation;
+ * everything is enqueued on `stream` (a hipStream_t, NULL for the default
+ * stream) as kernel launches alone, so a call may be captured in a HIP graph.
+ * Matrices have their rows contiguous; *_ld is the distance between two rows in
+ * elements (>= the row's length).  Any row length, distance and alignment of the
+ * elements is accepted; 16-byte aligned rows run fastest.  Sizes are at most
+ * 2^30.  A size of zero is a call without work, except that gradients summed
+ * over no rows and products over no k are written as sums of nothing.
+ * Arithmetic is float32 from the inputs on; every output is rounded once.
+ * Sums are taken in a fixed order: equal calls give equal bits.
+ * Arguments that cannot hold give TF_E_ARG before anything is enqueued. */
+
+#define TF_T_F32 0
+#define TF_T_BF16 1
+#define TF_T_F16 2
+#define TF_T_F8 3 /* OCP e4m3: 8 bits, largest value 448 */
+
+#define TF_ACT_NONE 0
+#define TF_ACT_RELU 1 /* NaN stays, as in compiled programs */
+#define TF_ACT_GELU 2 /* z * P(normal <= z) */
+#define TF_ACT_SILU 3 /* z / (1 + exp(-z)) */
+
+/* h = x + residual;  y = h / sqrt(mean(h^2) + eps) * weight, row by row, the norm
+ * taken of the sum before h is rounded.  With y_type TF_T_F8 y is in 8 bits with
+ * one scale a row: top = max(max|y|, 2^-100), scale = top/448, code = the value
+ * nearest to y * (448/top) (ties to even).  A row that holds an infinity or a
+ * NaN gives NaN. */
+typedef struct {
+  const void *x, *residual; /* rows x d of `type`; residual may be NULL          */
+  const void *weight;       /* d of weight_type                                  */
+  void *y;                  /* rows x d of y_type                                */
+  void *h;                  /* rows x d of `type`; NULL without a residual; may be
+                               x or residual itself                               */
+  float *scale;             /* rows; TF_T_F8 only                                 */
+  long long x_ld, residual_ld, y_ld, h_ld;
+  long long rows, d;
+  int type;        /* TF_T_F32, TF_T_BF16, TF_T_F16                               */
+  int weight_type; /* `type` or TF_T_F32                                          */
+  int y_type;      /* `type` or TF_T_F8                                           */
+  float eps;       /* >= 0                                                        */
+} tf_rms_norm_args_t;
+int tf_rms_norm(const tf_rms_norm_args_t *args, void *stream);
+
+/* x (rows x d of `type`) in 8 bits with one scale a row, as tf_rms_norm's. */
+int tf_quantize_rows(const void *x, long long x_ld, long long rows, long long d, int type, void *y, long long y_ld,
+                     float *scale, void *stream);
+
+/* tf_rms_norm's gradient.  r = 1/sqrt(mean(h^2) + eps), xhat = h*r:
+ *   dx = r*(dy*weight - xhat*mean(dy*weight*xhat)) + dh     (also the residual's)
+ *   dweight = sum over rows of dy*xhat */
+typedef struct {
+  const void *dy, *h; /* rows x d of `type`; h: the norm's input (x + residual)     */
+  const void *dh;     /* rows x d: the gradient that reaches h past the norm, or NULL */
+  const void *weight; /* d of weight_type                                           */
+  void *dx;           /* rows x d of `type`; may be dy or dh itself                 */
+  void *dweight;      /* d of weight_type                                           */
+  long long dy_ld, h_ld, dh_ld, dx_ld;
+  long long rows, d;
+  int type, weight_type; /* as tf_rms_norm's                                        */
+  float eps;
+  int reserved;    /* 0                                                             */
+  void *workspace; /* 16-byte aligned, tf_rms_norm_grad_workspace(rows, d) bytes    */
+  long long workspace_bytes;
+} tf_rms_norm_grad_args_t;
+int tf_rms_norm_grad_workspace(long long rows, long long d, long long *bytes);
+int tf_rms_norm_grad(const tf_rms_norm_grad_args_t *args, void *stream);
+
+/* z = x @ w + bias;  out = act(z) + residual.  x is m x k, w is k x n in either
+ * memory order.  With type TF_T_F8 x has a scale a row and w a scale a column,
+ * z = (x @ w) * x_scale[m] * w_scale[n] + bias, and w_order is 1. */
+typedef struct {
+  const void *x, *w;
+  const void *bias;     /* n of bias_type, or NULL                                  */
+  const void *residual; /* m x n of out_type, or NULL                               */
+  const float *x_scale, *w_scale; /* TF_T_F8 only: m, n                             */
+  void *out;            /* m x n of out_type                                        */
+  void *z;              /* m x n of out_type: the pre-activation kept, or NULL      */
+  void *workspace;      /* 16-byte aligned; with fewer bytes than tf_linear_workspace
+                           asks for (none: 0) the call runs unsplit along k         */
+  long long workspace_bytes;
+  long long x_ld, w_ld, residual_ld, out_ld, z_ld;
+  long long m, n, k;
+  int w_order;   /* 0: w lies as k rows of n, 1: as n rows of k                      */
+  int type;      /* TF_T_BF16, TF_T_F16, TF_T_F8                                     */
+  int out_type;  /* `type`; TF_T_BF16 or TF_T_F16 for TF_T_F8                        */
+  int bias_type; /* out_type or TF_T_F32                                             */
+  int act;       /* TF_ACT_*                                                         */
+  int tile;      /* C tile: 0 by the sizes, 1: 256x256, 2: 128x128, 3: 64x64         */
+  int splits;    /* ranges of k: 0 by the sizes, or 1..64                            */
+  int reserved;  /* 0                                                                */
+} tf_linear_args_t;
+/* Bytes of workspace for these sizes and types (pointers are not looked at). */
+int tf_linear_workspace(const tf_linear_args_t *args, long long *bytes);
+int tf_linear(const tf_linear_args_t *args, void *stream);
+
+/* tf_linear's gradient in 16 bits: dz = dy * act'(z) (rounded to `type` for the
+ * products), dx = dz @ w^T, dw = x^T @ dz in w's memory order, dbias = sum over
+ * rows of dz (before its rounding).  The residual's gradient is dy. */
+typedef struct {
+  const void *dy, *x, *w; /* m x n, m x k, k x n in either order                    */
+  const void *z;          /* m x n: the kept pre-activation; NULL with TF_ACT_NONE  */
+  void *dx, *dw;          /* each may be NULL: not wanted                           */
+  void *dbias;            /* n of bias_type, or NULL                                */
+  void *workspace;        /* 16-byte aligned, tf_linear_grad_workspace's bytes       */
+  long long workspace_bytes;
+  long long dy_ld, x_ld, w_ld, z_ld, dx_ld, dw_ld;
+  long long m, n, k;
+  int w_order;   /* of w and dw, as tf_linear's                                     */
+  int type;      /* TF_T_BF16, TF_T_F16                                             */
+  int bias_type; /* `type` or TF_T_F32                                              */
+  int act;
+  int tile, splits; /* both products', as tf_linear's                                */
+} tf_linear_grad_args_t;
+int tf_linear_grad_workspace(const tf_linear_grad_args_t *args, long long *bytes);
+int tf_linear_grad(const tf_linear_grad_args_t *args, void *stream);
 
 #ifdef __cplusplus
 }

@@ -49,6 +49,35 @@ class BenchResult(ctypes.Structure):
                 ("l2_flush", ctypes.c_int), ("padded", ctypes.c_longlong * 3)]
 
 
+class RmsNormArgs(ctypes.Structure):
+    _fields_ = [(f, ctypes.c_void_p) for f in ("x", "residual", "weight", "y", "h", "scale")] + \
+               [(f, ctypes.c_longlong) for f in ("x_ld", "residual_ld", "y_ld", "h_ld", "rows", "d")] + \
+               [(f, ctypes.c_int) for f in ("type", "weight_type", "y_type")] + [("eps", ctypes.c_float)]
+
+
+class RmsNormGradArgs(ctypes.Structure):
+    _fields_ = [(f, ctypes.c_void_p) for f in ("dy", "h", "dh", "weight", "dx", "dweight")] + \
+               [(f, ctypes.c_longlong) for f in ("dy_ld", "h_ld", "dh_ld", "dx_ld", "rows", "d")] + \
+               [("type", ctypes.c_int), ("weight_type", ctypes.c_int), ("eps", ctypes.c_float),
+                ("reserved", ctypes.c_int), ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_longlong)]
+
+
+class LinearArgs(ctypes.Structure):
+    _fields_ = [(f, ctypes.c_void_p) for f in ("x", "w", "bias", "residual", "x_scale", "w_scale", "out", "z",
+                                               "workspace")] + \
+               [(f, ctypes.c_longlong) for f in ("workspace_bytes", "x_ld", "w_ld", "residual_ld", "out_ld", "z_ld",
+                                                 "m", "n", "k")] + \
+               [(f, ctypes.c_int) for f in ("w_order", "type", "out_type", "bias_type", "act", "tile", "splits",
+                                            "reserved")]
+
+
+class LinearGradArgs(ctypes.Structure):
+    _fields_ = [(f, ctypes.c_void_p) for f in ("dy", "x", "w", "z", "dx", "dw", "dbias", "workspace")] + \
+               [(f, ctypes.c_longlong) for f in ("workspace_bytes", "dy_ld", "x_ld", "w_ld", "z_ld", "dx_ld", "dw_ld",
+                                                 "m", "n", "k")] + \
+               [(f, ctypes.c_int) for f in ("w_order", "type", "bias_type", "act", "tile", "splits")]
+
+
 # (name, restype, argtypes) of every exported function, in header order.
 P, I, LL, U = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_uint
 SIGNATURES = [
@@ -74,6 +103,16 @@ SIGNATURES = [
     ("tf_bench_samples", I, [P, ctypes.POINTER(ctypes.c_double), I]),
     ("tf_registry_size", I, []),
     ("tf_registry_entry", I, [I, ctypes.POINTER(I), ctypes.POINTER(I), ctypes.c_char_p, I]),
+    # The residual block's operators.  Their argument structs are passed as any
+    # pointer: tforge_nn packs them as bytes.
+    ("tf_rms_norm", I, [P, P]),
+    ("tf_quantize_rows", I, [P, LL, LL, LL, I, P, LL, P, P]),
+    ("tf_rms_norm_grad_workspace", I, [LL, LL, ctypes.POINTER(LL)]),
+    ("tf_rms_norm_grad", I, [P, P]),
+    ("tf_linear_workspace", I, [P, ctypes.POINTER(LL)]),
+    ("tf_linear", I, [P, P]),
+    ("tf_linear_grad_workspace", I, [P, ctypes.POINTER(LL)]),
+    ("tf_linear_grad", I, [P, P]),
 ]
 
 _lib = None

@@ -49,6 +49,7 @@ def _units():
     gen_instances.main()
     units = [CSRC / "runtime.hip", CSRC / "direct_kernels.hip", CSRC / "_gen" / "registry.hip",
              CSRC / "_gen" / "wavek.hip", CSRC / "_gen" / "forms.hip"]
+    units += sorted(CSRC.glob("nn*.hip"))
     units += sorted((CSRC / "_gen").glob("staged_*.hip"))
     return units
 

@@ -1,0 +1,130 @@
+// What the residual block's operators share: element types, rounding,
+// activations and wave reductions.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+
+#include "nn_kernels.h"
+
+namespace tfnn {
+
+typedef __bf16 bf16;
+typedef _Float16 f16;
+struct f8 {  // OCP e4m3: largest value 448, no infinities
+  uint8_t bits;
+};
+
+template <typename T, int N>
+struct Vec {
+  typedef T type __attribute__((ext_vector_type(N)));
+  // The same at the element's own alignment.  One 128-bit access all the same:
+  // global memory takes any byte address.
+  typedef T loose __attribute__((ext_vector_type(N), aligned(sizeof(T))));
+};
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+typedef short i16x4 __attribute__((ext_vector_type(4)));
+
+// f(0), f(1), ... f(N-1), each with its number as a constant.
+template <int I>
+struct Int {
+  __host__ __device__ constexpr operator int() const { return I; }
+};
+template <int N, int I = 0, typename F>
+__device__ __forceinline__ void unroll(F &&f) {
+  if constexpr (I < N) {
+    f(Int<I>{});
+    unroll<N, I + 1>(f);
+  }
+}
+
+enum Act { ACT_NONE = 0, ACT_RELU = 1, ACT_GELU = 2, ACT_SILU = 3 };
+
+// exp2 and 1/x in one instruction each (about 1 ulp).
+__device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
+__device__ __forceinline__ float fast_rcp(float x) { return __builtin_amdgcn_rcpf(x); }
+
+constexpr float kLog2e = 1.44269504088896340736f;
+
+// The normal distribution's upper tail P(Z > |x|), and its density's exp(-x^2/2).
+// erfc by Abramowitz and Stegun 7.1.26 (absolute error 1.5e-7): with
+// u = |x|/sqrt(2) and t = 1/(1 + 0.3275911 u), erfc(u) = t*poly(t)*exp(-u^2).
+// The exponential is needed for the density too, so the tail costs one
+// reciprocal and six multiply-adds beside it.
+__device__ __forceinline__ float normal_tail(float x, float &density_exp) {
+  const float a = __builtin_fabsf(x);
+  const float t = fast_rcp(__builtin_fmaf(0.3275911f * 0.70710678118654752f, a, 1.0f));
+  density_exp = fast_exp2(-0.5f * kLog2e * a * a);
+  float p = __builtin_fmaf(0.5f * 1.061405429f, t, 0.5f * -1.453152027f);
+  p = __builtin_fmaf(p, t, 0.5f * 1.421413741f);
+  p = __builtin_fmaf(p, t, 0.5f * -0.284496736f);
+  p = __builtin_fmaf(p, t, 0.5f * 0.254829592f);
+  return p * t * density_exp;
+}
+
+// 1/(1 + exp(-x)).
+__device__ __forceinline__ float sigmoid(float x) { return fast_rcp(1.0f + fast_exp2(-kLog2e * x)); }
+
+template <int ACT>
+__device__ __forceinline__ float act_value(float z) {
+  if constexpr (ACT == ACT_RELU) return (z > 0.0f || z != z) ? z : 0.0f;  // NaN stays, -0 becomes +0
+  if constexpr (ACT == ACT_GELU) {
+    // z*Phi(z): Phi is the tail itself on the left, 1 - tail on the right.
+    float e;
+    const float q = normal_tail(z, e);
+    const float v = z * (z > 0.0f ? 1.0f - q : q);
+    return z == -__builtin_inff() ? -0.0f : v;  // the limit; -inf * 0 would be NaN
+  }
+  if constexpr (ACT == ACT_SILU) return z == -__builtin_inff() ? -0.0f : z * sigmoid(z);
+  return z;
+}
+
+template <int ACT>
+__device__ __forceinline__ float act_slope(float z) {
+  if constexpr (ACT == ACT_RELU) return z > 0.0f ? 1.0f : (z != z ? z : 0.0f);
+  if constexpr (ACT == ACT_GELU) {
+    float e;
+    const float q = normal_tail(z, e);
+    const float v = __builtin_fmaf(z * 0.39894228040143267794f, e, z > 0.0f ? 1.0f - q : q);
+    return __builtin_fabsf(z) == __builtin_inff() ? (z > 0.0f ? 1.0f : 0.0f) : v;
+  }
+  if constexpr (ACT == ACT_SILU) {
+    const float s = sigmoid(z);
+    const float v = __builtin_fmaf(z * s, 1.0f - s, s);
+    return __builtin_fabsf(z) == __builtin_inff() ? (z > 0.0f ? 1.0f : 0.0f) : v;
+  }
+  return 1.0f;
+}
+
+// Rounds `v` to `type` at element `i` of `out`.
+__device__ __forceinline__ void store_as(void *out, int type, long i, float v) {
+  if (type == TYPE_F32) static_cast<float *>(out)[i] = v;
+  else if (type == TYPE_BF16) static_cast<bf16 *>(out)[i] = static_cast<bf16>(v);
+  else static_cast<f16 *>(out)[i] = static_cast<f16>(v);
+}
+
+// Sum / maximum over groups of 64 lanes; every lane gets the result.
+__device__ __forceinline__ float wave_sum(float v) {
+#pragma unroll
+  for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
+  return v;
+}
+// A NaN anywhere stays: fmaxf alone would drop it.
+__device__ __forceinline__ float max_keep_nan(float a, float b) { return (a > b || a != a) ? a : b; }
+__device__ __forceinline__ float wave_max(float v) {
+#pragma unroll
+  for (int o = 32; o; o >>= 1) v = max_keep_nan(v, __shfl_xor(v, o));
+  return v;
+}
+
+// The 8-bit code's scale: the row's largest magnitude over 448, taken as at
+// least 2^-100 so that a row of zeros keeps a finite factor.
+constexpr float kF8Max = 448.0f;
+constexpr float kF8Tiny = 0x1p-100f;
+__device__ __forceinline__ float f8_top(float top) { return top < kF8Tiny ? kF8Tiny : top; }
+
+}  // namespace tfnn

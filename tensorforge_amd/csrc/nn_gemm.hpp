@@ -1,0 +1,462 @@
+// Matrix products in 16 and 8 bits with a fused epilogue, on the matrix cores.
+//
+//   C[m][n] = sum over k of A(m, k) * B(k, n)
+//
+// Each operand lies in memory with k contiguous (rows of k) or with its own
+// dimension contiguous (columns of k: a k x n matrix row by row, or the
+// transposed left operand of a weight gradient).  Tiles go through LDS in slabs
+// of 128 bytes of k a row (64 elements of 16 bits, 128 of 8): the bytes, the
+// LDS layout and the reads are the same for all types.
+#pragma once
+
+#include "nn_common.hpp"
+#include "nn_kernels.h"
+
+namespace tfnn {
+
+typedef __attribute__((address_space(3))) char lds_char;
+
+template <typename T>
+constexpr int kSlab = 128 / sizeof(T);  // elements of k in a slab
+template <typename T>
+constexpr int kPiece = 16 / sizeof(T);  // elements in a 16-byte piece
+
+// LDS layout of one operand's slab, ROWS x 128 bytes.
+//
+// k contiguous: row after row; the 16-byte piece c of row r is at place
+// c ^ (r & 7), so that the 8 rows a quarter-wave reads at one c lie in
+// different banks.
+//
+// Own dimension contiguous: blocks of 64 rows (of the own dimension), in each
+// 64 k-lines of 128 bytes; the piece c of line k is at place c ^ (2 (k & 3)), so
+// that the four lines of a transposing read lie in different banks.
+//
+// Either way 1 KiB = 8 lines are one wave's 16-byte load, straight into LDS.
+
+// A read piece: 8 (16-bit) or 16 (8-bit) elements along k of one row.
+__device__ __forceinline__ i32x4 lds_read16(const lds_char *p) {
+  return *reinterpret_cast<const __attribute__((address_space(3))) i32x4 *>(p);
+}
+
+// ds_read_b64_tr_b16: of 16 lanes, lane 4r + q names line r, columns 4q..4q+3 of a
+// 4 x 16 block; lane j receives column j's four lines.
+__device__ __forceinline__ i16x4 lds_read_tr(const lds_char *p) {
+  return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4 *)(p));
+}
+
+// Fragment reader of one operand: read<OFF>(kk) gives, for the 16 rows from row
+// OFF (a multiple of 16) of the wave's range, this lane's row and its 16 bytes of
+// k: pieces g (kk = 0) or 4 + g (kk = 1), g = lane / 16.
+template <bool MN>
+struct FragReader {
+  uint32_t at[MN ? 4 : 2];
+  __device__ __forceinline__ void init(int row0) {
+    const int lane = threadIdx.x % 64, g = lane / 16, l = lane % 16;
+    if constexpr (!MN) {
+      at[0] = (row0 + l) * 128 + ((g ^ (l & 7)) << 4);
+      at[1] = at[0] ^ 64;
+    } else {
+      const int r = l / 4, q = l % 4;
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {
+        const int row = row0 + b * 16;  // row0: a multiple of 16
+        at[b] = row / 64 * 8192 + (8 * g + r) * 128 + (((row % 64 / 8 + q / 2) ^ (2 * r)) << 4) + (q & 1) * 8;
+      }
+    }
+  }
+  template <int OFF, int KK>
+  __device__ __forceinline__ i32x4 read(const lds_char *slab) const {
+    if constexpr (!MN) {
+      return lds_read16(slab + at[KK] + OFF * 128);
+    } else {
+      // Rows advance by whole 64-row blocks beyond the first four 16-row steps.
+      const lds_char *p = slab + at[OFF % 64 / 16] + OFF / 64 * 8192 + KK * 32 * 128;
+      union {
+        i16x4 h[2];
+        i32x4 v;
+      } u;
+      u.h[0] = lds_read_tr(p);
+      u.h[1] = lds_read_tr(p + 4 * 128);
+      return u.v;
+    }
+  }
+};
+
+// Buffer resource of `bytes` bytes from `base`; loads past it give zeros.
+__device__ __forceinline__ i32x4 buffer_resource(const void *base, uint32_t bytes) {
+  const uint64_t a = reinterpret_cast<uint64_t>(base);
+  return i32x4{__builtin_amdgcn_readfirstlane(static_cast<int>(a)),
+               __builtin_amdgcn_readfirstlane(static_cast<int>(a >> 32) & 0xffff), static_cast<int>(bytes), 0x00020000};
+}
+
+// 16 bytes a lane from resource + offset to LDS at `lds` + 16 * lane, without
+// registers in between.  The caller waits on vmcnt.  (The wait state between the
+// write of m0 and its use is the s_nop.)
+__device__ __forceinline__ void load_to_lds(i32x4 resource, uint32_t offset, uint32_t lds) {
+  asm volatile(
+      "s_mov_b32 m0, %0\n\t"
+      "s_nop 0\n\t"
+      "buffer_load_dwordx4 %1, %2, 0 offen lds"
+      :
+      : "s"(lds), "v"(offset), "s"(resource)
+      : "memory");
+}
+
+constexpr uint32_t kNowhere = 0x80000000u;  // past every resource: reads zeros
+constexpr uint32_t kResourceBytes = 0x7fffffffu;
+
+// Loads one operand's slabs.  DMA: straight into LDS; needs 16-byte aligned rows
+// and whole pieces (k, or the own dimension, a multiple of the piece), and rows'
+// offsets within a tile below 2^31 bytes.  Otherwise through registers, with any
+// alignment and any tail.
+template <typename T, bool MN, int ROWS, int NW, bool DMA>
+struct SlabLoader {
+  static constexpr int PER_WAVE = ROWS / 8 / NW;  // 1 KiB loads a wave
+  const char *base;                               // of the tile, slab 0
+  long step;                                      // bytes between slabs
+  long ld;
+  int rows, k_left;               // rows of this tile inside the matrix; elements of k from slab 0
+  uint32_t offset[DMA ? PER_WAVE : 1];
+  i32x4 held[DMA ? 1 : PER_WAVE];
+
+  // Place of this lane's piece of load i: (line, piece) of the layout above.
+  static __device__ __forceinline__ void place(int i, int &row, int &k) {
+    const int lane = threadIdx.x % 64, t = (threadIdx.x / 64) * PER_WAVE + i;
+    if constexpr (!MN) {
+      row = t * 8 + lane / 8;
+      k = ((lane % 8) ^ (lane / 8)) * kPiece<T>;
+    } else {
+      k = t % 8 * 8 + lane / 8;
+      row = t / 8 * 64 + ((lane % 8) ^ (2 * (lane / 8 & 3))) * kPiece<T>;
+    }
+  }
+
+  // matrix: element (0, 0); own0: the tile's first row; k0, k1: its range of k.
+  __device__ __forceinline__ void init(const void *matrix, long ld_, int own, int own0, int k0, int k1) {
+    const char *m = static_cast<const char *>(matrix);
+    ld = ld_ * static_cast<long>(sizeof(T));
+    rows = own - own0;
+    k_left = k1 - k0;
+    base = m + (MN ? k0 * ld + own0 * static_cast<long>(sizeof(T)) : own0 * ld + k0 * static_cast<long>(sizeof(T)));
+    step = MN ? kSlab<T> * ld : 128;
+    if constexpr (DMA) {
+#pragma unroll
+      for (int i = 0; i < PER_WAVE; ++i) {
+        int row, k;
+        place(i, row, k);
+        offset[i] = row < rows ? static_cast<uint32_t>(MN ? k * ld + row * static_cast<long>(sizeof(T))
+                                                          : row * ld + k * static_cast<long>(sizeof(T)))
+                               : kNowhere;
+      }
+    }
+  }
+
+  // DMA: starts the loads of slab s into `lds`.
+  __device__ __forceinline__ void issue(int s, uint32_t lds) {
+    const i32x4 res = buffer_resource(base + s * step, kResourceBytes);
+    const int left = k_left - s * kSlab<T>;
+    const uint32_t wave = lds + (threadIdx.x / 64) * (PER_WAVE * 1024);
+    if (left >= kSlab<T>) {
+#pragma unroll
+      for (int i = 0; i < PER_WAVE; ++i)
+        load_to_lds(res, offset[i], __builtin_amdgcn_readfirstlane(wave + i * 1024));
+    } else {
+#pragma unroll
+      for (int i = 0; i < PER_WAVE; ++i) {
+        int row, k;
+        place(i, row, k);
+        load_to_lds(res, k < left ? offset[i] : kNowhere, __builtin_amdgcn_readfirstlane(wave + i * 1024));
+      }
+    }
+  }
+
+  // Registers: reads slab s ...
+  __device__ __forceinline__ void fetch(int s) {
+    const char *from = base + s * step;
+    const int left = k_left - s * kSlab<T>;
+#pragma unroll
+    for (int i = 0; i < PER_WAVE; ++i) {
+      int row, k;
+      place(i, row, k);
+      const char *p = from + (MN ? k * ld + row * static_cast<long>(sizeof(T)) : row * ld + k * static_cast<long>(sizeof(T)));
+      int count = MN ? (k < left ? rows - row : 0) : (row < rows ? left - k : 0);
+      typedef int loose4 __attribute__((ext_vector_type(4), aligned(1)));
+      union {
+        i32x4 v;
+        T e[kPiece<T>];
+      } u;
+      u.v = i32x4{0, 0, 0, 0};
+      if (count >= kPiece<T>) {
+        u.v = *reinterpret_cast<const loose4 *>(p);
+      } else if (count > 0) {
+#pragma unroll
+        for (int e = 0; e < kPiece<T>; ++e)
+          if (e < count) u.e[e] = reinterpret_cast<const T *>(p)[e];
+      }
+      held[i] = u.v;
+    }
+  }
+  // ... and puts it into LDS.
+  __device__ __forceinline__ void put(lds_char *lds) const {
+    lds_char *wave = lds + (threadIdx.x / 64) * (PER_WAVE * 1024) + (threadIdx.x % 64) * 16;
+#pragma unroll
+    for (int i = 0; i < PER_WAVE; ++i)
+      *reinterpret_cast<__attribute__((address_space(3))) i32x4 *>(wave + i * 1024) = held[i];
+  }
+};
+
+// One 16 x 16 block's product over a slab.  The right operand goes first: the
+// block comes out with a lane's four values in one row of C, next to each other.
+__device__ __forceinline__ f32x4 block_mma(bf16, i32x4 a0, i32x4 a1, i32x4 b0, i32x4 b1, f32x4 c) {
+  typedef bf16 v8 __attribute__((ext_vector_type(8)));
+  c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8, b0), __builtin_bit_cast(v8, a0), c, 0, 0, 0);
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8, b1), __builtin_bit_cast(v8, a1), c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 block_mma(f16, i32x4 a0, i32x4 a1, i32x4 b0, i32x4 b1, f32x4 c) {
+  typedef f16 v8 __attribute__((ext_vector_type(8)));
+  c = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8, b0), __builtin_bit_cast(v8, a0), c, 0, 0, 0);
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8, b1), __builtin_bit_cast(v8, a1), c, 0, 0, 0);
+}
+// 8 bits: one instruction takes both pieces; the order of k inside it is the
+// same on both sides, so any order will do.  (Scales 0, 0: the unscaled form.)
+__device__ __forceinline__ f32x4 block_mma(f8, i32x4 a0, i32x4 a1, i32x4 b0, i32x4 b1, f32x4 c) {
+  const i32x8 a = __builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7);
+  const i32x8 b = __builtin_shufflevector(b0, b1, 0, 1, 2, 3, 4, 5, 6, 7);
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(b, a, c, 0, 0, 0, 0, 0, 0);
+}
+
+// ---- epilogue ---------------------------------------------------------------
+
+// Four consecutive values from p[0..left), zeros past them.
+template <typename T>
+__device__ __forceinline__ f32x4 load4(const T *p, int left) {
+  f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+  if (left >= 4) {
+    const typename Vec<T, 4>::loose u = *reinterpret_cast<const typename Vec<T, 4>::loose *>(p);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = static_cast<float>(u[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 3; ++i)
+      if (i < left) v[i] = static_cast<float>(p[i]);
+  }
+  return v;
+}
+template <typename T>
+__device__ __forceinline__ void store4(T *p, int left, f32x4 v) {
+  if (left >= 4) {
+    typename Vec<T, 4>::loose u;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) u[i] = static_cast<T>(v[i]);
+    *reinterpret_cast<typename Vec<T, 4>::loose *>(p) = u;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 3; ++i)
+      if (i < left) p[i] = static_cast<T>(v[i]);
+  }
+}
+
+template <typename O>
+__device__ __forceinline__ f32x4 bias4(const GemmParams &p, int n) {
+  if (!p.bias) return f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  if (p.bias_f32) return load4(static_cast<const float *>(p.bias) + n, p.n - n);
+  return load4(static_cast<const O *>(p.bias) + n, p.n - n);
+}
+
+// z = v + bias (kept if asked for); out = act(z) + residual, rounded once.
+template <typename O, int ACT>
+__device__ __forceinline__ void finish4(const GemmParams &p, int m, int n, f32x4 v, f32x4 bias) {
+  const int left = p.n - n;
+  v += bias;
+  if (p.z) store4(static_cast<O *>(p.z) + m * p.ldz + n, left, v);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = act_value<ACT>(v[i]);
+  if (p.residual) v += load4(static_cast<const O *>(p.residual) + m * p.ldr + n, left);
+  store4(static_cast<O *>(p.out) + m * p.ldo + n, left, v);
+}
+
+// A wave's accumulators: MI x NI blocks from (m0, n0).
+template <typename T, typename O, int MI, int NI, int ACT>
+__device__ __forceinline__ void finish_tile(const GemmParams &p, int m0, int n0, f32x4 (&acc)[MI][NI]) {
+  const int lane = threadIdx.x % 64;
+  float sa[MI];
+  if constexpr (sizeof(T) == 1) {
+#pragma unroll
+    for (int i = 0; i < MI; ++i) {
+      const int m = m0 + i * 16 + lane % 16;
+      sa[i] = m < p.m ? p.sa[m] : 0.0f;
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < NI; ++j) {
+    const int n = n0 + j * 16 + lane / 16 * 4;
+    if (n >= p.n) continue;
+    const f32x4 bias = bias4<O>(p, n);
+    f32x4 sb;
+    if constexpr (sizeof(T) == 1) sb = load4(p.sb + n, p.n - n);
+#pragma unroll
+    for (int i = 0; i < MI; ++i) {
+      const int m = m0 + i * 16 + lane % 16;
+      if (m >= p.m) continue;
+      f32x4 v = acc[i][j];
+      if constexpr (sizeof(T) == 1) v = v * sa[i] * sb;
+      finish4<O, ACT>(p, m, n, v, bias);
+    }
+  }
+}
+
+// One range of k of several: float partial sums, joined by gemm_join_kernel.
+template <int MI, int NI>
+__device__ __forceinline__ void store_part(const GemmParams &p, int split, int m0, int n0, f32x4 (&acc)[MI][NI]) {
+  const int lane = threadIdx.x % 64;
+  const long ld = (p.n + 3) & ~3;
+  float *part = p.parts + split * (p.m * ld);
+#pragma unroll
+  for (int j = 0; j < NI; ++j) {
+    const int n = n0 + j * 16 + lane / 16 * 4;
+#pragma unroll
+    for (int i = 0; i < MI; ++i) {
+      const int m = m0 + i * 16 + lane % 16;
+      if (m < p.m && n < p.n) *reinterpret_cast<f32x4 *>(part + m * ld + n) = acc[i][j];
+    }
+  }
+}
+
+template <typename T, typename O, int MI, int NI>
+__device__ __forceinline__ void write_tile(const GemmParams &p, int split, int m0, int n0, f32x4 (&acc)[MI][NI]) {
+  if (p.splits > 1) {
+    store_part(p, split, m0, n0, acc);
+    return;
+  }
+  switch (p.act) {
+    case ACT_RELU: finish_tile<T, O, MI, NI, ACT_RELU>(p, m0, n0, acc); break;
+    case ACT_GELU: finish_tile<T, O, MI, NI, ACT_GELU>(p, m0, n0, acc); break;
+    case ACT_SILU: finish_tile<T, O, MI, NI, ACT_SILU>(p, m0, n0, acc); break;
+    default: finish_tile<T, O, MI, NI, ACT_NONE>(p, m0, n0, acc); break;
+  }
+}
+
+// ---- tile order ---------------------------------------------------------------
+
+// Workgroups are dealt to the 8 XCDs in turn; each XCD gets one run of
+// consecutive tiles, walked in bands of 8 tile rows, so that its L2 holds the
+// rows and columns it shares.
+__device__ __forceinline__ void tile_of(const GemmParams &p, int &tm, int &tn, int &split) {
+  const int total = gridDim.x, id = blockIdx.x, xcd = id & 7, per = total >> 3, more = total & 7;
+  int t = xcd * per + min(xcd, more) + (id >> 3);
+  const int tiles = p.tiles_m * p.tiles_n;
+  split = t / tiles;
+  t -= split * tiles;
+  const int band = 8 * p.tiles_n, first = t / band * 8, rows = min(8, p.tiles_m - first);
+  t %= band;
+  tm = first + t % rows;
+  tn = t / rows;
+}
+
+__device__ __forceinline__ void wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void wait_loads() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void barrier() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+// ---- the tile kernel ----------------------------------------------------------
+
+// BM x BN of C a workgroup, WM x WN waves, ST slabs of LDS.  One barrier a slab:
+// behind it slab s has arrived for all waves and slab s-1 is used up, so slab
+// s+ST-1 may take its place while s is multiplied.
+template <typename T, typename O, bool AMN, bool BMN, int BM, int BN, int WM, int WN, int ST, bool DMA>
+__global__ __launch_bounds__(64 * WM *WN) void gemm_tile_kernel(GemmParams p) {
+  constexpr int NW = WM * WN, MI = BM / WM / 16, NI = BN / WN / 16, STAGE = (BM + BN) * 128;
+  __shared__ __align__(1024) char smem[ST * STAGE];
+  lds_char *lds = (lds_char *)smem;
+  const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(lds));
+  int tm, tn, split;
+  tile_of(p, tm, tn, split);
+  const int slabs = (p.k + kSlab<T> - 1) / kSlab<T>;
+  const int s0 = static_cast<int>(static_cast<long>(slabs) * split / p.splits);
+  const int count = static_cast<int>(static_cast<long>(slabs) * (split + 1) / p.splits) - s0;
+  const int k0 = s0 * kSlab<T>;
+  SlabLoader<T, AMN, BM, NW, DMA> la;
+  SlabLoader<T, BMN, BN, NW, DMA> lb;
+  la.init(p.a, p.lda, p.m, tm * BM, k0, p.k);
+  lb.init(p.b, p.ldb, p.n, tn * BN, k0, p.k);
+  constexpr int LOADS = decltype(la)::PER_WAVE + decltype(lb)::PER_WAVE;
+
+  const int wave = threadIdx.x / 64, wm = wave / WN, wn = wave % WN;
+  FragReader<AMN> fa;
+  FragReader<BMN> fb;
+  fa.init(wm * (BM / WM));
+  fb.init(wn * (BN / WN));
+  f32x4 acc[MI][NI];
+#pragma unroll
+  for (int i = 0; i < MI; ++i)
+#pragma unroll
+    for (int j = 0; j < NI; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+
+  const auto multiply = [&](const lds_char *slab) {
+    i32x4 a[2][MI], b[2][NI];
+    unroll<MI>([&](auto i) {
+      a[0][i] = fa.template read<16 * i, 0>(slab);
+      a[1][i] = fa.template read<16 * i, 1>(slab);
+    });
+    unroll<NI>([&](auto j) {
+      b[0][j] = fb.template read<16 * j, 0>(slab + BM * 128);
+      b[1][j] = fb.template read<16 * j, 1>(slab + BM * 128);
+    });
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
+#pragma unroll
+      for (int j = 0; j < NI; ++j) acc[i][j] = block_mma(T{}, a[0][i], a[1][i], b[0][j], b[1][j], acc[i][j]);
+  };
+
+  if constexpr (DMA) {
+#pragma unroll
+    for (int s = 0; s < ST - 1; ++s)
+      if (s < count) {
+        la.issue(s, lds0 + s * STAGE);
+        lb.issue(s, lds0 + s * STAGE + BM * 128);
+      }
+    int at = 0;
+    for (int s = 0; s < count; ++s) {
+      if (ST > 2 && s + ST - 2 < count) wait_loads<(ST - 2) * LOADS>();
+      else wait_loads<0>();
+      barrier();
+      const int into = at == 0 ? ST - 1 : at - 1;
+      if (s + ST - 1 < count) {
+        la.issue(s + ST - 1, lds0 + into * STAGE);
+        lb.issue(s + ST - 1, lds0 + into * STAGE + BM * 128);
+      }
+      multiply(lds + at * STAGE);
+      wait_lds();
+      at = at == ST - 1 ? 0 : at + 1;
+    }
+  } else {
+    if (count > 0) {
+      la.fetch(0);
+      lb.fetch(0);
+      la.put(lds);
+      lb.put(lds + BM * 128);
+    }
+    for (int s = 0; s < count; ++s) {
+      wait_lds();
+      barrier();
+      if (s + 1 < count) {
+        la.fetch(s + 1);
+        lb.fetch(s + 1);
+      }
+      multiply(lds + (s & 1) * STAGE);
+      if (s + 1 < count) {
+        la.put(lds + (~s & 1) * STAGE);
+        lb.put(lds + (~s & 1) * STAGE + BM * 128);
+      }
+    }
+  }
+  write_tile<T, O, MI, NI>(p, split, tm * BM + wm * (BM / WM), tn * BN + wn * (BN / WN), acc);
+}
+
+}  // namespace tfnn

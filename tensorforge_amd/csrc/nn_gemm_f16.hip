@@ -1,0 +1,12 @@
+// The float16 products.
+#include "nn_gemm_launch.hpp"
+
+namespace tfnn {
+
+hipError_t launch_gemm_f16(const GemmParams &p, bool amn, bool bmn, int tile, bool dma, hipStream_t stream) {
+  if (amn) return launch_layout<f16, f16, true, true>(p, tile, dma, stream);  // weight gradients: both operands by columns of k
+  if (bmn) return launch_layout<f16, f16, false, true>(p, tile, dma, stream);
+  return launch_layout<f16, f16, false, false>(p, tile, dma, stream);
+}
+
+}  // namespace tfnn

@@ -1,0 +1,72 @@
+// Parameters and launchers of the residual block's operators (norm, products,
+// gradients): what the C ABI (nn.hip) hands to the kernels' translation units.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+namespace tfnn {
+
+// The values of TF_T_* in tforge_hip.h.
+enum Type { TYPE_F32 = 0, TYPE_BF16 = 1, TYPE_F16 = 2, TYPE_F8 = 3 };
+
+// *_ld: elements between two rows.
+struct NormParams {
+  const void *x = nullptr, *residual = nullptr;
+  const void *weight = nullptr;  // null: rows are quantised as they are
+  void *y = nullptr, *h = nullptr;
+  float *scale = nullptr;  // 8-bit output only
+  long x_ld = 0, residual_ld = 0, y_ld = 0, h_ld = 0, rows = 0;
+  int d = 0, weight_type = 0;
+  float eps = 0;
+};
+
+struct NormGradParams {
+  const void *dy, *h, *dh, *weight;
+  void *dx, *dw;
+  float *shares;  // norm_grad_shares(rows, d) x d
+  long dy_ld, h_ld, dh_ld, dx_ld, rows;
+  int d, weight_type;
+  float eps;
+};
+
+struct GemmParams {
+  const void *a = nullptr, *b = nullptr;
+  const void *bias = nullptr, *residual = nullptr;
+  const float *sa = nullptr, *sb = nullptr;  // 8 bits: scales of A's rows and B's columns
+  void *out = nullptr, *z = nullptr;
+  float *parts = nullptr;  // splits > 1: splits x m x (n up to a multiple of 4)
+  long lda = 0, ldb = 0, ldr = 0, ldo = 0, ldz = 0;
+  int m = 0, n = 0, k = 0;
+  int tiles_m = 0, tiles_n = 0, splits = 1;
+  int act = 0, bias_f32 = 0;
+};
+
+// C tiles of the product kernels.  256 x 256 loads straight into LDS only.
+enum Tile { TILE_256 = 1, TILE_128 = 2, TILE_64 = 3 };
+constexpr int tile_size(int tile) { return tile == TILE_256 ? 256 : tile == TILE_128 ? 128 : 64; }
+
+// amn, bmn: the operand's own dimension (m, n) is contiguous, not k.
+hipError_t launch_gemm_bf16(const GemmParams &p, bool amn, bool bmn, int tile, bool dma, hipStream_t stream);
+hipError_t launch_gemm_f16(const GemmParams &p, bool amn, bool bmn, int tile, bool dma, hipStream_t stream);
+hipError_t launch_gemm_f8(const GemmParams &p, int out_type, int tile, bool dma, hipStream_t stream);
+// out = epilogue(sum of the splits' parts).
+hipError_t launch_gemm_join(const GemmParams &p, int out_type, hipStream_t stream);
+
+struct SlopeParams {
+  const void *dy, *z;
+  void *dz;       // m x dz_ld, columns from n on zero; null with act none
+  float *shares;  // column_shares(m) x n; null: no sums
+  long dy_ld, z_ld, dz_ld;
+  int m, n, act;
+};
+// dz = dy * act'(z), and dz's column sums in shares.
+long column_shares(long m);
+hipError_t launch_act_slope(const SlopeParams &p, int type, hipStream_t stream);
+// out[0..d) = sum of `count` shares, in order, rounded to `type`.
+hipError_t launch_share_sum(const float *shares, long count, int d, void *out, int type, hipStream_t stream);
+
+long norm_grad_shares(long rows, long d);
+hipError_t launch_rms_norm(const NormParams &p, int type, bool to_f8, hipStream_t stream);
+hipError_t launch_rms_norm_grad(const NormGradParams &p, int type, hipStream_t stream);
+
+}  // namespace tfnn

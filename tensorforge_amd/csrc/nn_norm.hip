@@ -1,0 +1,422 @@
+// Root-mean-square norm with the residual's addition, in the input's type or in
+// 8 bits with a scale a row, the row quantisation alone, and the norm's gradient.
+//
+//   h = x + residual           r = 1/sqrt(mean(h^2) + eps)
+//   y = (h*r)*w                scale = max|y| / 448, code = nearest(y * (448/max|y|))
+//   g = dy*w, xhat = h*r       dx = r*(g - xhat*mean(g*xhat)) + dh,  dw = sum over rows of dy*xhat
+//
+// All of it is bound by memory.  A row stays in its threads' registers between
+// its read and its write, so every tensor is read once and written once; both
+// sums a row needs (of squares, and the largest |h*w|, as max|y| = r*max|h*w|)
+// come from one pass and one reduction.
+#include "nn_common.hpp"
+#include "nn_kernels.h"
+
+#include <algorithm>
+
+namespace tfnn {
+namespace {
+
+template <typename T>
+__device__ __forceinline__ void load8(const T *p, int left, float (&v)[8]) {
+  if (left >= 8) {
+    const typename Vec<T, 8>::loose u = *reinterpret_cast<const typename Vec<T, 8>::loose *>(p);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = static_cast<float>(u[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = i < left ? static_cast<float>(p[i]) : 0.0f;
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void store8(T *p, int left, const float (&v)[8]) {
+  if (left >= 8) {
+    typename Vec<T, 8>::loose u;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) u[i] = static_cast<T>(v[i]);
+    *reinterpret_cast<typename Vec<T, 8>::loose *>(p) = u;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i < left) p[i] = static_cast<T>(v[i]);
+  }
+}
+
+__device__ __forceinline__ void store8(f8 *p, int left, const float (&v)[8]) {
+  int lo = __builtin_amdgcn_cvt_pk_fp8_f32(v[0], v[1], 0, false);
+  lo = __builtin_amdgcn_cvt_pk_fp8_f32(v[2], v[3], lo, true);
+  int hi = __builtin_amdgcn_cvt_pk_fp8_f32(v[4], v[5], 0, false);
+  hi = __builtin_amdgcn_cvt_pk_fp8_f32(v[6], v[7], hi, true);
+  if (left >= 8) {
+    typedef int loose2 __attribute__((ext_vector_type(2), aligned(1)));
+    *reinterpret_cast<loose2 *>(p) = loose2{lo, hi};
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i < left) p[i].bits = static_cast<uint8_t>((i < 4 ? lo : hi) >> (8 * (i & 3)));
+  }
+}
+
+__device__ __forceinline__ void load_weight8(const NormParams &p, int c, int left, float (&w)[8]) {
+  if (!p.weight) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w[i] = 1.0f;
+  } else if (p.weight_type == TYPE_F32) {
+    load8(static_cast<const float *>(p.weight) + c, left, w);
+  } else if (p.weight_type == TYPE_BF16) {
+    load8(static_cast<const bf16 *>(p.weight) + c, left, w);
+  } else {
+    load8(static_cast<const f16 *>(p.weight) + c, left, w);
+  }
+}
+
+// Sum of `sum`, and sum or maximum (MAX) of `more`, over the NT threads of a
+// row.  With NT = 256 the four waves meet in LDS; `turn` alternates between two
+// places, so one barrier a row is enough.  Every thread of the workgroup calls
+// it equally often.
+template <int NT, bool MAX>
+__device__ __forceinline__ void row_reduce(float &sum, float &more, int turn) {
+  sum = wave_sum(sum);
+  more = MAX ? wave_max(more) : wave_sum(more);
+  if constexpr (NT > 64) {
+    __shared__ float part[2][2][NT / 64];
+    const int wave = threadIdx.x / 64;
+    if (threadIdx.x % 64 == 0) {
+      part[turn][0][wave] = sum;
+      part[turn][1][wave] = more;
+    }
+    __syncthreads();
+    sum = part[turn][0][0];
+    more = part[turn][1][0];
+#pragma unroll
+    for (int i = 1; i < NT / 64; ++i) {
+      sum += part[turn][0][i];
+      more = MAX ? max_keep_nan(more, part[turn][1][i]) : more + part[turn][1][i];
+    }
+  }
+}
+
+// CH pieces of 8 elements a thread, NT threads a row, 256/NT rows a workgroup.
+// The weights stay in registers over a workgroup's rows.
+template <typename T, typename O, int NT, int CH>
+__global__ __launch_bounds__(256) void rms_norm_kernel(NormParams p) {
+  constexpr int RPB = 256 / NT;
+  const int t = threadIdx.x % NT, sub = threadIdx.x / NT;
+  float w[CH][8];
+#pragma unroll
+  for (int j = 0; j < CH; ++j) load_weight8(p, (j * NT + t) * 8, p.d - (j * NT + t) * 8, w[j]);
+  int turn = 0;
+  for (long row = static_cast<long>(blockIdx.x) * RPB + sub; row < p.rows; row += static_cast<long>(gridDim.x) * RPB) {
+    const T *x = static_cast<const T *>(p.x) + row * p.x_ld;
+    float h[CH][8];
+#pragma unroll
+    for (int j = 0; j < CH; ++j) load8(x + (j * NT + t) * 8, p.d - (j * NT + t) * 8, h[j]);
+    if (p.residual) {
+      const T *res = static_cast<const T *>(p.residual) + row * p.residual_ld;
+      T *ho = static_cast<T *>(p.h) + row * p.h_ld;
+#pragma unroll
+      for (int j = 0; j < CH; ++j) {
+        float v[8];
+        load8(res + (j * NT + t) * 8, p.d - (j * NT + t) * 8, v);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) h[j][i] += v[i];
+      }
+#pragma unroll
+      for (int j = 0; j < CH; ++j) store8(ho + (j * NT + t) * 8, p.d - (j * NT + t) * 8, h[j]);
+    }
+    float sum = 0.0f, top = 0.0f;
+#pragma unroll
+    for (int j = 0; j < CH; ++j)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        sum = __builtin_fmaf(h[j][i], h[j][i], sum);
+        if constexpr (sizeof(O) == 1) top = max_keep_nan(top, __builtin_fabsf(h[j][i] * w[j][i]));
+      }
+    row_reduce<NT, true>(sum, top, turn);
+    turn ^= 1;
+    const float r = p.weight ? rsqrtf(sum / static_cast<float>(p.d) + p.eps) : 1.0f;
+    float f = 1.0f;
+    if constexpr (sizeof(O) == 1) {
+      const float most = f8_top(top * r);
+      f = kF8Max / most;
+      if (t == 0) p.scale[row] = most / kF8Max;
+    }
+    O *y = static_cast<O *>(p.y) + row * p.y_ld;
+#pragma unroll
+    for (int j = 0; j < CH; ++j) {
+      float v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        v[i] = h[j][i] * r * w[j][i];
+        if constexpr (sizeof(O) == 1) v[i] *= f;
+      }
+      store8(y + (j * NT + t) * 8, p.d - (j * NT + t) * 8, v);
+    }
+  }
+}
+
+// Rows longer than a workgroup's registers hold: a second read of the row (from
+// the caches) in place of keeping it.
+template <typename T, typename O>
+__global__ __launch_bounds__(256) void rms_norm_long_kernel(NormParams p) {
+  constexpr int NT = 256;
+  const long row = blockIdx.x;
+  const T *x = static_cast<const T *>(p.x) + row * p.x_ld;
+  const T *res = p.residual ? static_cast<const T *>(p.residual) + row * p.residual_ld : nullptr;
+  float sum = 0.0f, top = 0.0f;
+  for (int c = threadIdx.x * 8; c < p.d; c += NT * 8) {
+    float v[8], u[8], w[8];
+    load8(x + c, p.d - c, v);
+    if (res) {
+      load8(res + c, p.d - c, u);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] += u[i];
+    }
+    load_weight8(p, c, p.d - c, w);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      sum = __builtin_fmaf(v[i], v[i], sum);
+      if constexpr (sizeof(O) == 1) top = max_keep_nan(top, __builtin_fabsf(v[i] * w[i]));
+    }
+  }
+  row_reduce<NT, true>(sum, top, 0);
+  const float r = p.weight ? rsqrtf(sum / static_cast<float>(p.d) + p.eps) : 1.0f;
+  float f = 1.0f;
+  if constexpr (sizeof(O) == 1) {
+    const float most = f8_top(top * r);
+    f = kF8Max / most;
+    if (threadIdx.x == 0) p.scale[row] = most / kF8Max;
+  }
+  for (int c = threadIdx.x * 8; c < p.d; c += NT * 8) {
+    float v[8], u[8], w[8];
+    load8(x + c, p.d - c, v);
+    if (res) {
+      load8(res + c, p.d - c, u);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] += u[i];
+      store8(static_cast<T *>(p.h) + row * p.h_ld + c, p.d - c, v);
+    }
+    load_weight8(p, c, p.d - c, w);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      v[i] = v[i] * r * w[i];
+      if constexpr (sizeof(O) == 1) v[i] *= f;
+    }
+    store8(static_cast<O *>(p.y) + row * p.y_ld + c, p.d - c, v);
+  }
+}
+
+// The gradient's dx, and this workgroup's rows' share of dw.  The shares are
+// added by share_sum_kernel, in a fixed order.
+template <typename T, int NT, int CH>
+__global__ __launch_bounds__(256) void rms_norm_grad_kernel(NormGradParams p) {
+  constexpr int RPB = 256 / NT;
+  const int t = threadIdx.x % NT, sub = threadIdx.x / NT;
+  const NormParams wp{.weight = p.weight, .weight_type = p.weight_type};
+  float w[CH][8], dw[CH][8];
+#pragma unroll
+  for (int j = 0; j < CH; ++j) {
+    load_weight8(wp, (j * NT + t) * 8, p.d - (j * NT + t) * 8, w[j]);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) dw[j][i] = 0.0f;
+  }
+  int turn = 0;
+  for (long row = static_cast<long>(blockIdx.x) * RPB + sub; row < p.rows; row += static_cast<long>(gridDim.x) * RPB) {
+    float h[CH][8], g[CH][8];
+#pragma unroll
+    for (int j = 0; j < CH; ++j)
+      load8(static_cast<const T *>(p.h) + row * p.h_ld + (j * NT + t) * 8, p.d - (j * NT + t) * 8, h[j]);
+#pragma unroll
+    for (int j = 0; j < CH; ++j)
+      load8(static_cast<const T *>(p.dy) + row * p.dy_ld + (j * NT + t) * 8, p.d - (j * NT + t) * 8, g[j]);
+    float sum = 0.0f, dot = 0.0f;
+#pragma unroll
+    for (int j = 0; j < CH; ++j)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        sum = __builtin_fmaf(h[j][i], h[j][i], sum);
+        dot = __builtin_fmaf(g[j][i] * w[j][i], h[j][i], dot);
+      }
+    row_reduce<NT, false>(sum, dot, turn);
+    turn ^= 1;
+    const float r = rsqrtf(sum / static_cast<float>(p.d) + p.eps);
+    const float c = dot * r * r / static_cast<float>(p.d);  // xhat*mean(g*xhat) = h*c
+#pragma unroll
+    for (int j = 0; j < CH; ++j) {
+      const int at = (j * NT + t) * 8;
+      float v[8], u[8];
+      if (p.dh) load8(static_cast<const T *>(p.dh) + row * p.dh_ld + at, p.d - at, u);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        v[i] = r * __builtin_fmaf(-c, h[j][i], g[j][i] * w[j][i]);
+        if (p.dh) v[i] += u[i];
+        dw[j][i] = __builtin_fmaf(g[j][i] * r, h[j][i], dw[j][i]);
+      }
+      store8(static_cast<T *>(p.dx) + row * p.dx_ld + at, p.d - at, v);
+    }
+  }
+  float *share = p.shares + static_cast<long>(blockIdx.x) * p.d;
+  if constexpr (RPB == 1) {
+#pragma unroll
+    for (int j = 0; j < CH; ++j) store8(share + (j * NT + t) * 8, p.d - (j * NT + t) * 8, dw[j]);
+  } else {
+    // The four rows' sums meet in LDS: one share a workgroup.
+    __shared__ float part[RPB][NT * CH * 8];
+#pragma unroll
+    for (int j = 0; j < CH; ++j)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) part[sub][(j * 8 + i) * NT + t] = dw[j][i];
+    __syncthreads();
+    for (int e = threadIdx.x; e < NT * CH * 8; e += 256) {
+      const int at = ((e / NT / 8) * NT + e % NT) * 8 + e / NT % 8;
+      float s = part[0][e];
+#pragma unroll
+      for (int q = 1; q < RPB; ++q) s += part[q][e];
+      if (at < p.d) share[at] = s;
+    }
+  }
+}
+
+// Rows longer than a workgroup's registers hold.  Workgroups own fixed rows; a
+// share of dw is added up in place by the threads that own its columns.
+template <typename T>
+__global__ __launch_bounds__(256) void rms_norm_grad_long_kernel(NormGradParams p) {
+  constexpr int NT = 256;
+  const NormParams wp{.weight = p.weight, .weight_type = p.weight_type};
+  float *share = p.shares + static_cast<long>(blockIdx.x) * p.d;
+  int turn = 0;
+  bool first = true;
+  for (long row = blockIdx.x; row < p.rows; row += gridDim.x) {
+    const T *hp = static_cast<const T *>(p.h) + row * p.h_ld;
+    const T *gp = static_cast<const T *>(p.dy) + row * p.dy_ld;
+    float sum = 0.0f, dot = 0.0f;
+    for (int c = threadIdx.x * 8; c < p.d; c += NT * 8) {
+      float h[8], g[8], w[8];
+      load8(hp + c, p.d - c, h);
+      load8(gp + c, p.d - c, g);
+      load_weight8(wp, c, p.d - c, w);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        sum = __builtin_fmaf(h[i], h[i], sum);
+        dot = __builtin_fmaf(g[i] * w[i], h[i], dot);
+      }
+    }
+    row_reduce<NT, false>(sum, dot, turn);
+    turn ^= 1;
+    const float r = rsqrtf(sum / static_cast<float>(p.d) + p.eps);
+    const float k = dot * r * r / static_cast<float>(p.d);
+    for (int c = threadIdx.x * 8; c < p.d; c += NT * 8) {
+      float h[8], g[8], w[8], u[8], s[8];
+      load8(hp + c, p.d - c, h);
+      load8(gp + c, p.d - c, g);
+      load_weight8(wp, c, p.d - c, w);
+      if (p.dh) load8(static_cast<const T *>(p.dh) + row * p.dh_ld + c, p.d - c, u);
+      if (!first) load8(share + c, p.d - c, s);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        s[i] = __builtin_fmaf(g[i] * r, h[i], first ? 0.0f : s[i]);
+        const float v = r * __builtin_fmaf(-k, h[i], g[i] * w[i]);
+        g[i] = p.dh ? v + u[i] : v;
+      }
+      store8(static_cast<T *>(p.dx) + row * p.dx_ld + c, p.d - c, g);
+      store8(share + c, p.d - c, s);
+    }
+    first = false;
+  }
+}
+
+// The shares' sum, in order: 32 columns a workgroup, 8 threads of four
+// columns by 32 rows of shares.
+__global__ __launch_bounds__(256) void share_sum_kernel(const float *shares, int count, int d, void *out, int type) {
+  const int c = blockIdx.x * 32 + threadIdx.x % 8 * 4, lane = threadIdx.x / 8;
+  f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
+  for (int q = lane; q < count; q += 32) {
+    const float *p = shares + static_cast<long>(q) * d + c;
+    if (c + 4 <= d) {
+      s += *reinterpret_cast<const Vec<float, 4>::loose *>(p);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (c + i < d) s[i] += p[i];
+    }
+  }
+  __shared__ float part[32][33];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) part[lane][threadIdx.x % 8 * 4 + i] = s[i];
+  __syncthreads();
+  if (threadIdx.x < 32) {
+    const int at = blockIdx.x * 32 + threadIdx.x;
+    float v = 0.0f;
+#pragma unroll
+    for (int q = 0; q < 32; ++q) v += part[q][threadIdx.x];
+    if (at < d) store_as(out, type, at, v);
+  }
+}
+
+// Workgroups beyond this many would each take few rows for the weights they load.
+constexpr long kNormGroups = 2048;
+
+// The register kernels hold up to 64 elements a thread.
+constexpr int kLongest = 16384;
+
+int pieces(long d) { return static_cast<int>((d + 7) / 8); }
+
+template <typename T, typename O>
+void norm_launch(const NormParams &p, hipStream_t stream) {
+  const int n = pieces(p.d);
+  const dim3 waves(static_cast<unsigned>(std::min<long>((p.rows + 3) / 4, kNormGroups)));
+  const dim3 groups(static_cast<unsigned>(std::min<long>(p.rows, kNormGroups)));
+  if (n <= 64) rms_norm_kernel<T, O, 64, 1><<<waves, 256, 0, stream>>>(p);
+  else if (n <= 128) rms_norm_kernel<T, O, 64, 2><<<waves, 256, 0, stream>>>(p);
+  else if (n <= 256) rms_norm_kernel<T, O, 256, 1><<<groups, 256, 0, stream>>>(p);
+  else if (n <= 512) rms_norm_kernel<T, O, 256, 2><<<groups, 256, 0, stream>>>(p);
+  else if (n <= 1024) rms_norm_kernel<T, O, 256, 4><<<groups, 256, 0, stream>>>(p);
+  else if (p.d <= kLongest) rms_norm_kernel<T, O, 256, 8><<<groups, 256, 0, stream>>>(p);
+  else rms_norm_long_kernel<T, O><<<dim3(static_cast<unsigned>(p.rows)), 256, 0, stream>>>(p);
+}
+
+template <typename T>
+void norm_grad_launch(const NormGradParams &p, hipStream_t stream) {
+  const int n = pieces(p.d);
+  const long shares = norm_grad_shares(p.rows, p.d);
+  const dim3 grid(static_cast<unsigned>(shares));
+  if (shares == 0) {
+  } else if (n <= 64) rms_norm_grad_kernel<T, 64, 1><<<grid, 256, 0, stream>>>(p);
+  else if (n <= 128) rms_norm_grad_kernel<T, 64, 2><<<grid, 256, 0, stream>>>(p);
+  else if (n <= 256) rms_norm_grad_kernel<T, 256, 1><<<grid, 256, 0, stream>>>(p);
+  else if (n <= 512) rms_norm_grad_kernel<T, 256, 2><<<grid, 256, 0, stream>>>(p);
+  else if (n <= 1024) rms_norm_grad_kernel<T, 256, 4><<<grid, 256, 0, stream>>>(p);
+  else if (p.d <= kLongest) rms_norm_grad_kernel<T, 256, 8><<<grid, 256, 0, stream>>>(p);
+  else rms_norm_grad_long_kernel<T><<<grid, 256, 0, stream>>>(p);
+  (void)launch_share_sum(p.shares, shares, p.d, p.dw, p.weight_type, stream);
+}
+
+}  // namespace
+
+long norm_grad_shares(long rows, long d) {
+  const long rpb = pieces(d) <= 128 ? 4 : 1;
+  return std::min<long>((rows + rpb - 1) / rpb, 1024);
+}
+
+hipError_t launch_share_sum(const float *shares, long count, int d, void *out, int type, hipStream_t stream) {
+  share_sum_kernel<<<dim3(static_cast<unsigned>((d + 31) / 32)), 256, 0, stream>>>(shares, static_cast<int>(count), d, out,
+                                                                                  type);
+  return hipGetLastError();
+}
+
+hipError_t launch_rms_norm(const NormParams &p, int type, bool to_f8, hipStream_t stream) {
+  if (type == TYPE_F32) to_f8 ? norm_launch<float, f8>(p, stream) : norm_launch<float, float>(p, stream);
+  else if (type == TYPE_BF16) to_f8 ? norm_launch<bf16, f8>(p, stream) : norm_launch<bf16, bf16>(p, stream);
+  else to_f8 ? norm_launch<f16, f8>(p, stream) : norm_launch<f16, f16>(p, stream);
+  return hipGetLastError();
+}
+
+hipError_t launch_rms_norm_grad(const NormGradParams &p, int type, hipStream_t stream) {
+  if (type == TYPE_F32) norm_grad_launch<float>(p, stream);
+  else if (type == TYPE_BF16) norm_grad_launch<bf16>(p, stream);
+  else norm_grad_launch<f16>(p, stream);
+  return hipGetLastError();
+}
+
+}  // namespace tfnn

@@ -19,33 +19,22 @@
 #include <string>
 #include <vector>
 
+#include "errors.h"
 #include "frontend.h"
 #include "tf_kernels.h"
 #include "tforge_hip.h"
 
-namespace {
+static thread_local std::string g_err;
 
-thread_local std::string g_err;
-
-int fail(int code, const std::string &m) {
+int tfk::fail(int code, const std::string &m) {
   g_err = m;
   return code;
 }
 
-// Runs an entry point's body; a C++ exception (an allocation failure, say)
-// becomes an error code and message instead of unwinding into the caller.
-template <typename F>
-int guarded(F &&body) {
-  try {
-    return body();
-  } catch (const std::bad_alloc &) {
-    return fail(TF_E_ARG, "out of host memory");
-  } catch (const std::exception &e) {
-    return fail(TF_E_ARG, std::string("internal error: ") + e.what());
-  } catch (...) {
-    return fail(TF_E_ARG, "internal error");
-  }
-}
+namespace {
+
+using tfk::fail;
+using tfk::guarded;
 
 #define TF_HIP(x)                                                                                  \
   do {                                                                                             \

@@ -1,0 +1,123 @@
+"""The residual block's operators without a GPU: the argument structs' layout, and
+what the C ABI and the Python functions refuse (before any device work)."""
+
+import ctypes
+import pathlib
+import subprocess
+
+import pytest
+import torch
+
+from tensorforge_amd import _lib
+from tensorforge_amd import tforge_nn as nn
+
+HEADER = pathlib.Path(__file__).resolve().parent.parent / "include" / "tforge_hip.h"
+STRUCTS = {"tf_rms_norm_args_t": _lib.RmsNormArgs, "tf_rms_norm_grad_args_t": _lib.RmsNormGradArgs,
+           "tf_linear_args_t": _lib.LinearArgs, "tf_linear_grad_args_t": _lib.LinearGradArgs}
+
+
+def test_struct_layouts_match_c(tmp_path):
+    lines = ["#include <stdio.h>", "#include <stddef.h>", f'#include "{HEADER}"', "int main(void) {"]
+    for cname, py in STRUCTS.items():
+        lines.append(f'  printf("{cname} %zu\\n", sizeof({cname}));')
+        lines += [f'  printf("{cname}.{f} %zu\\n", offsetof({cname}, {f}));' for f, _ in py._fields_]
+    (tmp_path / "sizes.c").write_text("\n".join(lines + ["  return 0;", "}"]))
+    subprocess.run(["gcc", str(tmp_path / "sizes.c"), "-o", str(tmp_path / "sizes")], check=True)
+    got = dict(l.split() for l in subprocess.run([str(tmp_path / "sizes")], capture_output=True, text=True).stdout.splitlines())
+    for cname, py in STRUCTS.items():
+        assert int(got[cname]) == ctypes.sizeof(py)
+        for f, _ in py._fields_:
+            assert int(got[f"{cname}.{f}"]) == getattr(py, f).offset, (cname, f)
+
+
+def _refused(call, args, words):
+    assert call(ctypes.byref(args), None) == -4  # TF_E_ARG
+    assert words in _lib.lib().tf_last_error().decode(), _lib.lib().tf_last_error()
+
+
+def _linear(**kw):
+    base = dict(x=256, w=256, out=256, x_ld=64, w_ld=32, out_ld=32, m=8, n=32, k=64, type=1, out_type=1)
+    return _lib.LinearArgs(**{**base, **kw})
+
+
+@pytest.mark.parametrize("change,words", [
+    (dict(type=0), "type = 0"), (dict(out_type=2), "out_type = 2"), (dict(act=4), "act = 4"), (dict(m=-1), "m = -1"),
+    (dict(k=(1 << 30) + 1), "k = 1073741825"), (dict(x=0), "x is a null pointer"), (dict(out=0), "out is a null pointer"),
+    (dict(x=257), "x is not aligned"), (dict(x_ld=63), "x: 63 elements between rows of 64"),
+    (dict(w_ld=31), "w: 31 elements between rows of 32"), (dict(w_order=1), "w: 32 elements between rows of 64"),
+    (dict(w_order=2), "w_order = 2"), (dict(out_ld=31), "out: 31"), (dict(z=256, z_ld=8), "z: 8"),
+    (dict(residual=256, residual_ld=3), "residual: 3"), (dict(bias=256, bias_type=2), "bias_type = 2"),
+    (dict(x_scale=256), "scales belong to 8-bit"), (dict(type=3), "8-bit weights"),
+    (dict(type=3, w_order=1, w_ld=64), "x_scale is a null pointer"), (dict(tile=4), "tile = 4"),
+    (dict(splits=65), "splits = 65"), (dict(workspace=8, workspace_bytes=64), "not 16-byte aligned"),
+    (dict(x_ld=1 << 41), "are too many"),
+])
+def test_linear_refusals(change, words):
+    _refused(_lib.lib().tf_linear, _linear(**change), words)
+
+
+@pytest.mark.parametrize("change,words", [
+    (dict(type=3), "type = 3"), (dict(dy=0), "dy is a null pointer"), (dict(act=1), "z is a null pointer"),
+    (dict(x=0), "x is a null pointer"), (dict(w=0), "w is a null pointer"), (dict(dx_ld=63), "dx: 63"),
+    (dict(dw_ld=31), "dw: 31"), (dict(bias_type=3), "bias_type = 3"), (dict(workspace_bytes=16), "bytes, "),
+    (dict(workspace=0), "workspace is null"), (dict(n=-2), "n = -2"),
+])
+def test_linear_grad_refusals(change, words):
+    base = dict(dy=256, x=256, w=256, dx=256, dw=256, dbias=256, workspace=256, workspace_bytes=1 << 30, dy_ld=32, x_ld=64,
+                w_ld=32, dx_ld=64, dw_ld=32, m=8, n=32, k=64, type=1, bias_type=1)
+    _refused(_lib.lib().tf_linear_grad, _lib.LinearGradArgs(**{**base, **change}), words)
+
+
+@pytest.mark.parametrize("change,words", [
+    (dict(type=3), "type = 3"), (dict(weight_type=2), "weight_type = 2"), (dict(y_type=2), "y_type = 2"),
+    (dict(rows=-1), "rows = -1"), (dict(weight=0), "weight is a null pointer"), (dict(y=0), "y is a null pointer"),
+    (dict(y_type=3), "scale is a null pointer"), (dict(residual=256, residual_ld=64), "h is a null pointer"),
+    (dict(h=256, h_ld=64), "h without a residual"), (dict(x_ld=8), "x: 8"), (dict(eps=-1.0), "eps"),
+    (dict(eps=float("nan")), "eps"), (dict(x=258, type=0, weight_type=0, y_type=0), "x is not aligned"),
+])
+def test_rms_norm_refusals(change, words):
+    base = dict(x=256, weight=256, y=256, x_ld=64, y_ld=64, rows=4, d=64, type=1, weight_type=1, y_type=1, eps=1e-6)
+    _refused(_lib.lib().tf_rms_norm, _lib.RmsNormArgs(**{**base, **change}), words)
+
+
+def test_other_refusals():
+    lib = _lib.lib()
+    assert lib.tf_quantize_rows(256, 8, 4, 64, 1, 256, 64, 256, None) == -4
+    assert lib.tf_quantize_rows(256, 64, 4, 64, 3, 256, 64, 256, None) == -4
+    assert lib.tf_rms_norm(None, None) == lib.tf_linear(None, None) == lib.tf_linear_grad(None, None) == -4
+    n = ctypes.c_longlong()
+    assert lib.tf_rms_norm_grad_workspace(-1, 8, ctypes.byref(n)) == -4
+    assert lib.tf_linear_workspace(ctypes.byref(_linear(m=-1)), ctypes.byref(n)) == -4
+    a = dict(dy=256, h=256, weight=256, dx=256, dweight=256, dy_ld=64, h_ld=64, dx_ld=64, rows=4, d=64, type=1,
+             weight_type=1, workspace=256, workspace_bytes=4)
+    _refused(lib.tf_rms_norm_grad, _lib.RmsNormGradArgs(**a), "bytes, ")
+
+
+def test_workspace_sizes():
+    lib, n = _lib.lib(), ctypes.c_longlong()
+    assert lib.tf_linear_workspace(ctypes.byref(_linear(m=8192, n=8192, k=8192)), ctypes.byref(n)) == 0 and n.value == 0
+    assert lib.tf_linear_workspace(ctypes.byref(_linear(m=5, n=7, k=512, tile=3, splits=2)), ctypes.byref(n)) == 0
+    assert n.value == 2 * 5 * 8 * 4
+    assert lib.tf_rms_norm_grad_workspace(0, 64, ctypes.byref(n)) == 0 and n.value == 0
+
+
+def test_python_refusals():
+    x = torch.zeros(4, 8, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="not on a GPU"):
+        nn.linear(x, x.t())
+    with pytest.raises(TypeError, match="float64"):
+        nn.rms_norm(x.double(), x[0])
+    with pytest.raises(TypeError, match="not a tensor"):
+        nn.quantize_rows(None)
+    with pytest.raises(ValueError, match="not next to each other"):
+        nn._rows(torch.zeros(4, 8).t(), "x")
+    with pytest.raises(ValueError, match="rows overlap"):
+        nn._rows(torch.zeros(8).expand(4, 8), "x")
+    with pytest.raises(ValueError, match="neither its rows nor its columns"):
+        nn._weights(torch.zeros(8, 8)[::2, ::2], 4, (torch.float32,), torch.device("cpu"))
+    with pytest.raises(ValueError, match="not one of"):
+        nn._act("tanh")
+    assert nn._weights(torch.zeros(8, 16), 8, (torch.float32,), torch.device("cpu")) == (0, 16)
+    assert nn._weights(torch.zeros(16, 8).t(), 8, (torch.float32,), torch.device("cpu")) == (1, 8)
+    assert nn._weights(torch.zeros(5, 1), 5, (torch.float32,), torch.device("cpu")) == (1, 5)
+    assert nn._weights(torch.zeros(1, 5), 1, (torch.float32,), torch.device("cpu")) == (1, 1)
