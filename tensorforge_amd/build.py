@@ -1,4 +1,4 @@
-"""Build libtforge_hip.so in place for gfx950.
+"""Build libtforge_hip.so (and _nn_torch.so, its operators on torch tensors) in place for gfx950.
 
 Steps: generate the staged-kernel instantiation shards (csrc/gen_instances.py),
 compile every translation unit in parallel (hipcc for HIP, g++ for the host
@@ -26,6 +26,7 @@ ROOT = PKG.parent
 CSRC = PKG / "csrc"
 OUT = CSRC / "_build"
 LIB = PKG / "libtforge_hip.so"
+TORCH_LAYER = PKG / "_nn_torch.so"
 RESOURCES = PKG / "kernel_resources.json"
 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
@@ -149,6 +150,34 @@ def _resources(logs):
     return out
 
 
+def _build_torch_layer(force):
+    """_nn_torch: the residual block's operators on torch tensors, linked against
+    libtforge_hip.so next to it.  Host code alone, so g++ builds it."""
+    import sysconfig
+    try:
+        import torch
+        from torch.utils import cpp_extension
+    except ImportError:  # the C ABI and compiled programs need no torch
+        return
+    src = CSRC / "nn_torch.cpp"
+    deps = sorted(_includes(src.resolve()))
+    if not force and TORCH_LAYER.exists() and all(TORCH_LAYER.stat().st_mtime >= d.stat().st_mtime for d in deps):
+        return
+    tmp = TORCH_LAYER.with_suffix(".so.tmp")
+    cmd = [os.environ.get("CXX", "g++"), "-shared", "-O2", "-std=c++17", "-fPIC", "-Wall", "-D__HIP_PLATFORM_AMD__=1",
+           "-DUSE_ROCM=1", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
+           "-I", str(ROOT / "include"), "-isystem", sysconfig.get_paths()["include"]]
+    cmd += [a for d in cpp_extension.include_paths("cuda") for a in ("-isystem", d)]
+    cmd += [str(src), "-o", str(tmp)]
+    cmd += [a for d in cpp_extension.library_paths() for a in ("-L", d)]
+    cmd += ["-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_hip", "-ltorch", "-ltorch_python", "-L", str(PKG),
+            "-l:libtforge_hip.so", "-Wl,-rpath,$ORIGIN"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError("compile failed: nn_torch.cpp\n" + " ".join(cmd) + "\n" + r.stdout + r.stderr)
+    os.replace(tmp, TORCH_LAYER)
+
+
 def build(force=True, jobs=None):
     OUT.mkdir(exist_ok=True)
     units = _units() + [CSRC / "frontend.cpp"]
@@ -162,6 +191,7 @@ def build(force=True, jobs=None):
     if r.returncode != 0:
         raise RuntimeError("link failed:\n" + r.stdout + r.stderr)
     os.replace(tmp, LIB)
+    _build_torch_layer(force)
     RESOURCES.write_text(json.dumps(_resources([t for _, t in results]), indent=1, sort_keys=True) + "\n")
     sys.path.insert(0, str(ROOT))
     from tensorforge_amd import provenance

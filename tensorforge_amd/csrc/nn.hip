@@ -19,35 +19,42 @@ constexpr long long kMostSize = 1LL << 30;
 
 int size_of(int type) { return type == TF_T_F32 ? 4 : type == TF_T_F8 ? 1 : 2; }
 
-// The first thing wrong with a call's arguments.
+// The first thing wrong with a call's arguments.  Messages are built only where
+// one is wanted: the checks of a good call cost some tens of nanoseconds.
 struct Checks {
   const char *call;
   std::string wrong;
 
-  void need(bool ok, const std::string &what) {
-    if (!ok && wrong.empty()) wrong = std::string(call) + ": " + what;
+  bool fine() const { return wrong.empty(); }
+  template <typename... Parts>
+  void need(bool ok, const Parts &...parts) {
+    if (ok || !wrong.empty()) return;
+    wrong = std::string(call) + ": ";
+    (void)std::initializer_list<int>{(add(parts), 0)...};
   }
+  void add(const char *s) { wrong += s; }
+  void add(long long v) { wrong += std::to_string(v); }
   void size(const char *name, long long v) {
-    need(v >= 0 && v <= kMostSize, std::string(name) + " = " + std::to_string(v) + " is not between 0 and 2^30");
+    need(v >= 0 && v <= kMostSize, name, " = ", v, " is not between 0 and 2^30");
   }
   void one_of(const char *name, int v, std::initializer_list<int> allowed) {
-    need(std::find(allowed.begin(), allowed.end(), v) != allowed.end(),
-         std::string(name) + " = " + std::to_string(v) + " is not one this call takes");
+    need(std::find(allowed.begin(), allowed.end(), v) != allowed.end(), name, " = ", static_cast<long long>(v),
+         " is not one this call takes");
   }
   // A matrix of rows x cols elements; `wanted`: it may not be missing.
   void matrix(const char *name, const void *p, long long ld, long long rows, long long cols, int type, bool wanted) {
-    if (!wrong.empty() || rows <= 0 || cols <= 0) return;
-    need(p || !wanted, std::string(name) + " is a null pointer");
+    if (!fine() || rows <= 0 || cols <= 0) return;
+    need(p || !wanted, name, " is a null pointer");
     if (!p) return;
-    need(reinterpret_cast<uintptr_t>(p) % size_of(type) == 0, std::string(name) + " is not aligned to its elements");
-    need(ld >= cols, std::string(name) + ": " + std::to_string(ld) + " elements between rows of " + std::to_string(cols));
-    need(ld <= (1LL << 40), std::string(name) + ": " + std::to_string(ld) + " elements between rows are too many");
+    need(reinterpret_cast<uintptr_t>(p) % size_of(type) == 0, name, " is not aligned to its elements");
+    need(ld >= cols, name, ": ", ld, " elements between rows of ", cols);
+    need(ld <= (1LL << 40), name, ": ", ld, " elements between rows are too many");
   }
   void vector(const char *name, const void *p, long long n, int type, bool wanted) {
     matrix(name, p, n, 1, n, type, wanted);
   }
   void workspace(const void *p, long long given, long long needed) {
-    need(given >= needed, "the workspace has " + std::to_string(given) + " bytes, " + std::to_string(needed) + " are needed");
+    need(given >= needed, "the workspace has ", given, " bytes, ", needed, " are needed");
     need(needed == 0 || (p && reinterpret_cast<uintptr_t>(p) % 16 == 0), "the workspace is null or not 16-byte aligned");
   }
 };
@@ -75,7 +82,7 @@ int rms_norm(const tf_rms_norm_args_t *a, hipStream_t stream) {
   c.vector("weight", a->weight, a->d, a->weight_type, true);
   c.matrix("y", a->y, a->y_ld, a->rows, a->d, a->y_type, true);
   c.vector("scale", a->scale, a->rows, TF_T_F32, a->y_type == TF_T_F8);
-  if (!c.wrong.empty()) return fail(TF_E_ARG, c.wrong);
+  if (!c.fine()) return fail(TF_E_ARG, c.wrong);
   if (a->rows == 0 || a->d == 0) return TF_OK;
   NormParams p;
   p.x = a->x, p.residual = a->residual, p.weight = a->weight, p.y = a->y, p.h = a->h, p.scale = a->scale;
@@ -94,7 +101,7 @@ int quantize_rows(const void *x, long long x_ld, long long rows, long long d, in
   c.matrix("x", x, x_ld, rows, d, type, true);
   c.matrix("y", y, y_ld, rows, d, TF_T_F8, true);
   c.vector("scale", scale, rows, TF_T_F32, d > 0);
-  if (!c.wrong.empty()) return fail(TF_E_ARG, c.wrong);
+  if (!c.fine()) return fail(TF_E_ARG, c.wrong);
   if (rows == 0 || d == 0) return TF_OK;
   NormParams p;
   p.x = x, p.y = y, p.scale = scale, p.x_ld = x_ld, p.y_ld = y_ld, p.rows = rows, p.d = static_cast<int>(d);
@@ -118,8 +125,8 @@ int rms_norm_grad(const tf_rms_norm_grad_args_t *a, hipStream_t stream) {
   c.vector("weight", a->weight, a->d, a->weight_type, true);
   c.matrix("dx", a->dx, a->dx_ld, a->rows, a->d, a->type, true);
   c.vector("dweight", a->dweight, a->d, a->weight_type, true);
-  if (c.wrong.empty()) c.workspace(a->workspace, a->workspace_bytes, norm_grad_shares(a->rows, a->d) * a->d * 4);
-  if (!c.wrong.empty()) return fail(TF_E_ARG, c.wrong);
+  if (c.fine()) c.workspace(a->workspace, a->workspace_bytes, norm_grad_shares(a->rows, a->d) * a->d * 4);
+  if (!c.fine()) return fail(TF_E_ARG, c.wrong);
   if (a->d == 0) return TF_OK;
   NormGradParams p;
   p.dy = a->dy, p.h = a->h, p.dh = a->dh, p.weight = a->weight, p.dx = a->dx, p.dw = a->dweight;
@@ -192,7 +199,7 @@ hipError_t run_product(Product &q, int tile, int splits, void *workspace, long l
 
 void check_choice(Checks &c, int tile, int splits) {
   c.one_of("tile", tile, {0, TILE_256, TILE_128, TILE_64});
-  c.need(splits >= 0 && splits <= 64, "splits = " + std::to_string(splits) + " is not between 0 and 64");
+  c.need(splits >= 0 && splits <= 64, "splits = ", static_cast<long long>(splits), " is not between 0 and 64");
 }
 
 void check_linear_sizes(Checks &c, const tf_linear_args_t *a) {
@@ -209,7 +216,7 @@ int linear_workspace(const tf_linear_args_t *a, long long *bytes) {
   if (!a || !bytes) return fail(TF_E_ARG, "tf_linear_workspace: null arguments");
   Checks c{"tf_linear_workspace", {}};
   check_linear_sizes(c, a);
-  if (!c.wrong.empty()) return fail(TF_E_ARG, c.wrong);
+  if (!c.fine()) return fail(TF_E_ARG, c.wrong);
   *bytes = a->m && a->n ? product_bytes(a->m, a->n, a->k, a->type, a->tile, a->splits) : 0;
   return TF_OK;
 }
@@ -235,7 +242,7 @@ int linear(const tf_linear_args_t *a, hipStream_t stream) {
   c.vector("w_scale", a->w_scale, a->n, TF_T_F32, f8);
   c.need(f8 || (!a->x_scale && !a->w_scale), "scales belong to 8-bit products");
   if (a->workspace_bytes) c.workspace(a->workspace, a->workspace_bytes, 1);
-  if (!c.wrong.empty()) return fail(TF_E_ARG, c.wrong);
+  if (!c.fine()) return fail(TF_E_ARG, c.wrong);
   if (a->m == 0 || a->n == 0) return TF_OK;
   Product q{a->type, a->out_type, false, a->w_order == 0, {}};
   GemmParams &p = q.p;
@@ -280,7 +287,7 @@ int linear_grad_workspace(const tf_linear_grad_args_t *a, long long *bytes) {
   if (!a || !bytes) return fail(TF_E_ARG, "tf_linear_grad_workspace: null arguments");
   Checks c{"tf_linear_grad_workspace", {}};
   check_grad_sizes(c, a);
-  if (!c.wrong.empty()) return fail(TF_E_ARG, c.wrong);
+  if (!c.fine()) return fail(TF_E_ARG, c.wrong);
   *bytes = grad_space(a).bytes();
   return TF_OK;
 }
@@ -299,10 +306,10 @@ int linear_grad(const tf_linear_grad_args_t *a, hipStream_t stream) {
   c.matrix("dx", a->dx, a->dx_ld, a->m, a->k, a->type, false);
   c.matrix("dw", a->dw, a->dw_ld, wr, wc, a->type, false);
   c.vector("dbias", a->dbias, a->n, a->bias_type, false);
-  if (!c.wrong.empty()) return fail(TF_E_ARG, c.wrong);
+  if (!c.fine()) return fail(TF_E_ARG, c.wrong);
   const GradSpace space = grad_space(a);
   c.workspace(a->workspace, a->workspace_bytes, space.bytes());
-  if (!c.wrong.empty()) return fail(TF_E_ARG, c.wrong);
+  if (!c.fine()) return fail(TF_E_ARG, c.wrong);
 
   char *ws = static_cast<char *>(a->workspace);
   const int m = static_cast<int>(a->m), n = static_cast<int>(a->n), k = static_cast<int>(a->k);
@@ -359,7 +366,7 @@ int tf_rms_norm_grad_workspace(long long rows, long long d, long long *bytes) {
     c.size("rows", rows);
     c.size("d", d);
     c.need(bytes != nullptr, "null arguments");
-    if (!c.wrong.empty()) return fail(TF_E_ARG, c.wrong);
+    if (!c.fine()) return fail(TF_E_ARG, c.wrong);
     *bytes = norm_grad_shares(rows, d) * d * 4;
     return TF_OK;
   });

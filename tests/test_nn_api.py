@@ -11,6 +11,7 @@ import torch
 from tensorforge_amd import _lib
 from tensorforge_amd import tforge_nn as nn
 
+F8 = torch.float8_e4m3fn
 HEADER = pathlib.Path(__file__).resolve().parent.parent / "include" / "tforge_hip.h"
 STRUCTS = {"tf_rms_norm_args_t": _lib.RmsNormArgs, "tf_rms_norm_grad_args_t": _lib.RmsNormGradArgs,
            "tf_linear_args_t": _lib.LinearArgs, "tf_linear_grad_args_t": _lib.LinearGradArgs}
@@ -102,22 +103,36 @@ def test_workspace_sizes():
 
 
 def test_python_refusals():
-    x = torch.zeros(4, 8, dtype=torch.bfloat16)
-    with pytest.raises(ValueError, match="not on a GPU"):
-        nn.linear(x, x.t())
-    with pytest.raises(TypeError, match="float64"):
-        nn.rms_norm(x.double(), x[0])
-    with pytest.raises(TypeError, match="not a tensor"):
-        nn.quantize_rows(None)
-    with pytest.raises(ValueError, match="not next to each other"):
-        nn._rows(torch.zeros(4, 8).t(), "x")
-    with pytest.raises(ValueError, match="rows overlap"):
-        nn._rows(torch.zeros(8).expand(4, 8), "x")
-    with pytest.raises(ValueError, match="neither its rows nor its columns"):
-        nn._weights(torch.zeros(8, 8)[::2, ::2], 4, (torch.float32,), torch.device("cpu"))
-    with pytest.raises(ValueError, match="not one of"):
-        nn._act("tanh")
-    assert nn._weights(torch.zeros(8, 16), 8, (torch.float32,), torch.device("cpu")) == (0, 16)
-    assert nn._weights(torch.zeros(16, 8).t(), 8, (torch.float32,), torch.device("cpu")) == (1, 8)
-    assert nn._weights(torch.zeros(5, 1), 5, (torch.float32,), torch.device("cpu")) == (1, 5)
-    assert nn._weights(torch.zeros(1, 5), 1, (torch.float32,), torch.device("cpu")) == (1, 1)
+    """On CPU tensors: what is wrong with the tensors comes first, the missing GPU last."""
+    h = torch.zeros(4, 8, dtype=torch.bfloat16)
+    w, v = torch.zeros(8, 16, dtype=torch.bfloat16), torch.zeros(16)
+    for call, error, words in [
+            (lambda: nn.linear(h, w), ValueError, "not on a GPU"),
+            (lambda: nn.rms_norm(h, h[0]), ValueError, "not on a GPU"),
+            (lambda: nn.rms_norm_grad(h, h, h[0]), ValueError, "not on a GPU"),
+            (lambda: nn.linear_grad(h[:, :1].expand(4, 16).contiguous(), h, w), ValueError, "not on a GPU"),
+            (lambda: nn.quantize_rows(h), ValueError, "not on a GPU"),
+            (lambda: nn.quantize_rows(None), TypeError, "x is not a tensor"),
+            (lambda: nn.rms_norm(h.double(), h[0]), TypeError, "x is Double"),
+            (lambda: nn.rms_norm(h, h[0].half()), TypeError, "weight is Half"),
+            (lambda: nn.rms_norm(h, w[0]), ValueError, "not a contiguous vector of 8"),
+            (lambda: nn.rms_norm(h, h[0], residual=w), ValueError, "residual is 8 x 16, not 4 x 8"),
+            (lambda: nn.rms_norm(h.requires_grad_(False).clone().requires_grad_(), h[0], quantize=True), ValueError, "gradient"),
+            (lambda: nn.linear(h.float(), w.float()), TypeError, "x is Float"),
+            (lambda: nn.linear(h, w.half()), TypeError, "w is Half"),
+            (lambda: nn.linear(h, h), ValueError, "not 8 x n"),
+            (lambda: nn.linear(h, w, h[0]), ValueError, "bias is not"),
+            (lambda: nn.linear(h, w, activation="tanh"), ValueError, "not one of none, relu, gelu, silu"),
+            (lambda: nn.linear(h, w, residual=h), ValueError, "residual is 4 x 8, not 4 x 16"),
+            (lambda: nn.linear(h, w, x_scale=v), ValueError, "scales belong"),
+            (lambda: nn.linear(h, w, out_dtype=torch.float16), TypeError, "keep x's type"),
+            (lambda: nn.linear(h.to(F8), w.to(F8), x_scale=v[:4], w_scale=v), ValueError, "column by column"),
+            (lambda: nn.linear(h.to(F8), w.to(F8).t().contiguous().t()), ValueError, "needs x_scale"),
+            (lambda: nn.linear(torch.zeros(8, 4, dtype=torch.bfloat16).t(), w), ValueError, "next to each other"),
+            (lambda: nn.linear(h[0].expand(4, 8), w), ValueError, "rows overlap"),
+            (lambda: nn.linear(h, torch.zeros(16, 32, dtype=torch.bfloat16)[::2, ::2]), ValueError, "neither its rows"),
+            (lambda: nn.linear(torch.zeros(2, 3, 9, dtype=torch.bfloat16)[:, :2, :8], w), ValueError, "one run of rows"),
+            (lambda: nn.linear_grad(w[:4], h, w, activation="gelu"), ValueError, "keep=True"),
+            (lambda: nn.linear_grad(w[:4], h, w, bias_dtype=torch.float64), TypeError, "bias_dtype is Double")]:
+        with pytest.raises(error, match=words):
+            call()
