@@ -257,7 +257,7 @@ int tf_registry_entry(int i, int *family, int *cfg7, char *name, int name_cap);
  * Matrices have their rows contiguous; *_ld is the distance between two rows in
  * elements (>= the row's length).  Any row length, distance and alignment of the
  * elements is accepted; 16-byte aligned rows run fastest.  Sizes are at most
- * 2^30.  A size of zero is a call without work, except that gradients summed
+ * 2^30.  Outputs and the workspace overlap nothing but where said.  A size of zero is a call without work, except that gradients summed
  * over no rows and products over no k are written as sums of nothing.
  * Arithmetic is float32 from the inputs on; every output is rounded once.
  * Sums are taken in a fixed order: equal calls give equal bits.
@@ -338,7 +338,9 @@ typedef struct {
   int out_type;  /* `type`; TF_T_BF16 or TF_T_F16 for TF_T_F8                        */
   int bias_type; /* out_type or TF_T_F32                                             */
   int act;       /* TF_ACT_*                                                         */
-  int tile;      /* C tile: 0 by the sizes, 1: 256x256, 2: 128x128, 3: 64x64         */
+  int tile;      /* C tile: 0 by the sizes, 1: 256x256, 2: 128x128, 3: 64x64, 4: all of
+                    up to 64 rows, k split over a workgroup's waves; one that cannot
+                    run these operands gives way to the choice by sizes              */
   int splits;    /* ranges of k: 0 by the sizes, or 1..64                            */
   int reserved;  /* 0                                                                */
 } tf_linear_args_t;

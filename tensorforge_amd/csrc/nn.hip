@@ -160,15 +160,35 @@ struct Plan {
 long ceil_div(long a, long b) { return (a + b - 1) / b; }
 
 // The C tile and the ranges of k for a product of these sizes.
-Plan plan_product(long m, long n, long k, int type, bool dma, int tile, int splits) {
-  const long slabs = ceil_div(k, 128 / size_of(type));
-  if (!tile) tile = m <= 64 || n <= 64 || ceil_div(m, 128) * ceil_div(n, 128) < 128 ? TILE_64
+//
+// Up to 64 rows a workgroup's time is what it reads, at about 35 bytes a
+// nanosecond (what a CU's misses to L2 and beyond sustain): for the few-row
+// kernel its columns' and all rows' whole k, for the 64 x 64 tile its range of
+// k, and 3.3 us for the join where k is split.  The smaller estimate runs.
+// Measured, bfloat16, us (few-row / tile), w 4096 x 4096 as n rows of k: 7.7 / 10.8
+// for 1 row, 9.8 / 11.1 for 16, 13.7 / 11.6 for 32; as k rows of n: 11.4 / 11.6, 13.4 /
+// 12.2, 16.1 / 12.5; 8192 deep and 2048 wide: 11.3 / 12.0 for 1 row, 16.6 / 12.2 for 16.
+Plan plan_product(long m, long n, long k, int type, bool amn, bool bmn, bool dma, int tile, int splits) {
+  const int size = size_of(type);
+  const long slabs = ceil_div(k, 128 / size);
+  const bool rows = m <= 64 && !amn && (!bmn || n >= 32);
+  const auto split = [&](int t) {
+    const long tiles = ceil_div(m, tile_size(t)) * ceil_div(n, tile_size(t));
+    const long s = splits ? splits : std::min<long>({256 / std::max<long>(1, tiles), slabs / 4, 16});
+    return static_cast<int>(std::max<long>(1, std::min(s, slabs)));
+  };
+  if (rows && !tile) {
+    const long cols = bmn ? 32 : 16, s = split(TILE_64);
+    const long few = ceil_div(ceil_div(n, cols), 256) * (cols + m) * k * size / 36;
+    const long many = ceil_div(ceil_div(n, 64) * s, 256) * (64 + m) * (k / s) * size / 33 * (dma ? 1 : 2) + (s > 1 ? 3300 : 0);
+    tile = few <= many ? TILE_ROWS : TILE_64;
+  }
+  if (tile == TILE_ROWS && rows) return {TILE_ROWS, 1};
+  if (!tile || tile == TILE_ROWS) tile = m <= 64 || n <= 64 || ceil_div(m, 128) * ceil_div(n, 128) < 128 ? TILE_64
                     : dma && ceil_div(m, 256) * ceil_div(n, 256) >= 192            ? TILE_256
                                                                                    : TILE_128;
   if (!dma && tile == TILE_256) tile = TILE_128;
-  const long tiles = ceil_div(m, tile_size(tile)) * ceil_div(n, tile_size(tile));
-  if (!splits) splits = static_cast<int>(std::max<long>(1, std::min<long>({256 / std::max<long>(1, tiles), slabs / 4, 16})));
-  return {tile, static_cast<int>(std::max<long>(1, std::min<long>(splits, slabs)))};
+  return {tile, split(tile)};
 }
 
 long long part_bytes(long m, long n, const Plan &plan) {
@@ -176,17 +196,17 @@ long long part_bytes(long m, long n, const Plan &plan) {
 }
 
 // The workspace that serves this product whatever the alignment of its operands.
-long long product_bytes(long m, long n, long k, int type, int tile, int splits) {
-  return std::max(part_bytes(m, n, plan_product(m, n, k, type, true, tile, splits)),
-                  part_bytes(m, n, plan_product(m, n, k, type, false, tile, splits)));
+long long product_bytes(long m, long n, long k, int type, bool amn, bool bmn, int tile, int splits) {
+  return std::max(part_bytes(m, n, plan_product(m, n, k, type, amn, bmn, true, tile, splits)),
+                  part_bytes(m, n, plan_product(m, n, k, type, amn, bmn, false, tile, splits)));
 }
 
 hipError_t run_product(Product &q, int tile, int splits, void *workspace, long long bytes, hipStream_t stream) {
   GemmParams &p = q.p;
   const int size = size_of(q.type);
   const bool dma = direct_loads(p.a, p.lda, q.amn, p.m, p.k, size) && direct_loads(p.b, p.ldb, q.bmn, p.n, p.k, size);
-  Plan plan = plan_product(p.m, p.n, p.k, q.type, dma, tile, splits);
-  if (part_bytes(p.m, p.n, plan) > bytes) plan = plan_product(p.m, p.n, p.k, q.type, dma, tile, 1);
+  Plan plan = plan_product(p.m, p.n, p.k, q.type, q.amn, q.bmn, dma, tile, splits);
+  if (part_bytes(p.m, p.n, plan) > bytes) plan = plan_product(p.m, p.n, p.k, q.type, q.amn, q.bmn, dma, tile, 1);
   p.tiles_m = static_cast<int>(ceil_div(p.m, tile_size(plan.tile)));
   p.tiles_n = static_cast<int>(ceil_div(p.n, tile_size(plan.tile)));
   p.splits = plan.splits;
@@ -198,7 +218,7 @@ hipError_t run_product(Product &q, int tile, int splits, void *workspace, long l
 }
 
 void check_choice(Checks &c, int tile, int splits) {
-  c.one_of("tile", tile, {0, TILE_256, TILE_128, TILE_64});
+  c.one_of("tile", tile, {0, TILE_256, TILE_128, TILE_64, TILE_ROWS});
   c.need(splits >= 0 && splits <= 64, "splits = ", static_cast<long long>(splits), " is not between 0 and 64");
 }
 
@@ -217,7 +237,7 @@ int linear_workspace(const tf_linear_args_t *a, long long *bytes) {
   Checks c{"tf_linear_workspace", {}};
   check_linear_sizes(c, a);
   if (!c.fine()) return fail(TF_E_ARG, c.wrong);
-  *bytes = a->m && a->n ? product_bytes(a->m, a->n, a->k, a->type, a->tile, a->splits) : 0;
+  *bytes = a->m && a->n ? product_bytes(a->m, a->n, a->k, a->type, false, a->w_order == 0, a->tile, a->splits) : 0;
   return TF_OK;
 }
 
@@ -266,9 +286,9 @@ GradSpace grad_space(const tf_linear_grad_args_t *a) {
   if (a->act != TF_ACT_NONE) s.dz = round16(2 * a->m * s.dz_ld);
   s.shares = round16(4 * column_shares(a->m) * a->n);
   if (a->k) {
-    s.parts = product_bytes(a->m, a->k, a->n, a->type, a->tile, a->splits);
-    s.parts = std::max(s.parts, a->w_order ? product_bytes(a->n, a->k, a->m, a->type, a->tile, a->splits)
-                                           : product_bytes(a->k, a->n, a->m, a->type, a->tile, a->splits));
+    s.parts = product_bytes(a->m, a->k, a->n, a->type, false, a->w_order == 1, a->tile, a->splits);
+    s.parts = std::max(s.parts, a->w_order ? product_bytes(a->n, a->k, a->m, a->type, true, true, a->tile, a->splits)
+                                           : product_bytes(a->k, a->n, a->m, a->type, true, true, a->tile, a->splits));
   }
   return s;
 }

@@ -100,6 +100,43 @@ __device__ __forceinline__ float act_slope(float z) {
   return 1.0f;
 }
 
+typedef int loose16 __attribute__((ext_vector_type(4), aligned(1)));
+
+// 16 bytes from element c >= 0 of a row of `length` elements (the same for all
+// lanes), zeros past its end; nothing outside the row is touched, at any
+// alignment.  WHOLE: length is a multiple of a piece, so a piece is inside or
+// outside.  Otherwise length is at least a piece, and the row's last 16 bytes
+// serve the pieces that reach past its end, shifted down.  Either way one load
+// and no branch: the loads of many pieces can be under way together.
+template <bool WHOLE, typename T>
+__device__ __forceinline__ i32x4 load_piece(const T *row, int c, int length) {
+  constexpr int N = 16 / sizeof(T), BITS = 8 * sizeof(T);
+  const int at = min(c, length - N), past = c - at;
+  const i32x4 v = *reinterpret_cast<const loose16 *>(row + at);
+  if constexpr (WHOLE) {
+    return past ? i32x4{0, 0, 0, 0} : v;
+  } else {
+    const auto u = __builtin_bit_cast(unsigned __int128, v) >> (min(past, N - 1) * BITS);
+    return past >= N ? i32x4{0, 0, 0, 0} : __builtin_bit_cast(i32x4, u);
+  }
+}
+
+// The same for any length, element by element where the row is shorter than a piece.
+template <typename T>
+__device__ __forceinline__ i32x4 load_piece_any(const T *row, int c, int length) {
+  constexpr int N = 16 / sizeof(T);
+  if (length >= N) return load_piece<false>(row, c, length);
+  union {
+    i32x4 v;
+    T e[N];
+  } u;
+  u.v = i32x4{0, 0, 0, 0};
+#pragma unroll
+  for (int e = 0; e < N - 1; ++e)
+    if (c + e < length) u.e[e] = row[c + e];
+  return u.v;
+}
+
 // Rounds `v` to `type` at element `i` of `out`.
 __device__ __forceinline__ void store_as(void *out, int type, long i, float v) {
   if (type == TYPE_F32) static_cast<float *>(out)[i] = v;

@@ -112,12 +112,10 @@ constexpr uint32_t kResourceBytes = 0x7fffffffu;
 template <typename T, bool MN, int ROWS, int NW, bool DMA>
 struct SlabLoader {
   static constexpr int PER_WAVE = ROWS / 8 / NW;  // 1 KiB loads a wave
-  const char *base;                               // of the tile, slab 0
-  long step;                                      // bytes between slabs
-  long ld;
-  int rows, k_left;               // rows of this tile inside the matrix; elements of k from slab 0
+  const char *matrix, *base;      // element (0, 0); the tile's first of slab 0
+  long step, ld;                  // bytes between slabs, between lines
+  int row_first, row_end, k_first, k_end;  // the tile's start and the matrix's end
   uint32_t offset[DMA ? PER_WAVE : 1];
-  i32x4 held[DMA ? 1 : PER_WAVE];
 
   // Place of this lane's piece of load i: (line, piece) of the layout above.
   static __device__ __forceinline__ void place(int i, int &row, int &k) {
@@ -131,22 +129,23 @@ struct SlabLoader {
     }
   }
 
-  // matrix: element (0, 0); own0: the tile's first row; k0, k1: its range of k.
-  __device__ __forceinline__ void init(const void *matrix, long ld_, int own, int own0, int k0, int k1) {
-    const char *m = static_cast<const char *>(matrix);
-    ld = ld_ * static_cast<long>(sizeof(T));
-    rows = own - own0;
-    k_left = k1 - k0;
-    base = m + (MN ? k0 * ld + own0 * static_cast<long>(sizeof(T)) : own0 * ld + k0 * static_cast<long>(sizeof(T)));
+  // own0: the tile's first row; k0: its first k (a whole slab's).
+  __device__ __forceinline__ void init(const void *matrix_, long ld_, int own, int own0, int k0, int k1) {
+    constexpr long E = sizeof(T);
+    matrix = static_cast<const char *>(matrix_);
+    ld = ld_ * E;
+    row_first = own0;
+    row_end = own;
+    k_first = k0;
+    k_end = k1;
+    base = matrix + (MN ? k0 * ld + own0 * E : own0 * ld + k0 * E);
     step = MN ? kSlab<T> * ld : 128;
     if constexpr (DMA) {
 #pragma unroll
       for (int i = 0; i < PER_WAVE; ++i) {
         int row, k;
         place(i, row, k);
-        offset[i] = row < rows ? static_cast<uint32_t>(MN ? k * ld + row * static_cast<long>(sizeof(T))
-                                                          : row * ld + k * static_cast<long>(sizeof(T)))
-                               : kNowhere;
+        offset[i] = row < own - own0 ? static_cast<uint32_t>(MN ? k * ld + row * E : row * ld + k * E) : kNowhere;
       }
     }
   }
@@ -154,7 +153,7 @@ struct SlabLoader {
   // DMA: starts the loads of slab s into `lds`.
   __device__ __forceinline__ void issue(int s, uint32_t lds) {
     const i32x4 res = buffer_resource(base + s * step, kResourceBytes);
-    const int left = k_left - s * kSlab<T>;
+    const int left = k_end - k_first - s * kSlab<T>;
     const uint32_t wave = lds + (threadIdx.x / 64) * (PER_WAVE * 1024);
     if (left >= kSlab<T>) {
 #pragma unroll
@@ -170,34 +169,35 @@ struct SlabLoader {
     }
   }
 
-  // Registers: reads slab s ...
-  __device__ __forceinline__ void fetch(int s) {
-    const char *from = base + s * step;
-    const int left = k_left - s * kSlab<T>;
+  // Registers: reads slab s ...  A tile that fits into the matrix starts so
+  // that it lies inside it, so only the last slab of k, and matrices smaller than a tile,
+  // have pieces to guard: those repeat a line inside and become zeros.
+  __device__ __forceinline__ void fetch(int s, i32x4 (&held)[PER_WAVE]) const {
+    const int k0 = k_first + s * kSlab<T>;
+    if (k0 + kSlab<T> <= k_end && row_first + ROWS <= row_end) {
+#pragma unroll
+      for (int i = 0; i < PER_WAVE; ++i) {
+        int row, k;
+        place(i, row, k);
+        const char *p = base + s * step + (MN ? k * ld + row * static_cast<long>(sizeof(T)) : row * ld + k * static_cast<long>(sizeof(T)));
+        held[i] = *reinterpret_cast<const loose16 *>(p);
+      }
+      return;
+    }
 #pragma unroll
     for (int i = 0; i < PER_WAVE; ++i) {
       int row, k;
       place(i, row, k);
-      const char *p = from + (MN ? k * ld + row * static_cast<long>(sizeof(T)) : row * ld + k * static_cast<long>(sizeof(T)));
-      int count = MN ? (k < left ? rows - row : 0) : (row < rows ? left - k : 0);
-      typedef int loose4 __attribute__((ext_vector_type(4), aligned(1)));
-      union {
-        i32x4 v;
-        T e[kPiece<T>];
-      } u;
-      u.v = i32x4{0, 0, 0, 0};
-      if (count >= kPiece<T>) {
-        u.v = *reinterpret_cast<const loose4 *>(p);
-      } else if (count > 0) {
-#pragma unroll
-        for (int e = 0; e < kPiece<T>; ++e)
-          if (e < count) u.e[e] = reinterpret_cast<const T *>(p)[e];
-      }
-      held[i] = u.v;
+      row += row_first;
+      k += k0;
+      const int line = MN ? k : row, lines = MN ? k_end : row_end;
+      const char *p = matrix + min(line, lines - 1) * ld;
+      held[i] = load_piece_any(reinterpret_cast<const T *>(p), MN ? row : k, MN ? row_end : k_end);
+      if (line >= lines) held[i] = i32x4{0, 0, 0, 0};
     }
   }
   // ... and puts it into LDS.
-  __device__ __forceinline__ void put(lds_char *lds) const {
+  static __device__ __forceinline__ void put(lds_char *lds, const i32x4 (&held)[PER_WAVE]) {
     lds_char *wave = lds + (threadIdx.x / 64) * (PER_WAVE * 1024) + (threadIdx.x % 64) * 16;
 #pragma unroll
     for (int i = 0; i < PER_WAVE; ++i)
@@ -276,8 +276,11 @@ __device__ __forceinline__ void finish4(const GemmParams &p, int m, int n, f32x4
 }
 
 // A wave's accumulators: MI x NI blocks from (m0, n0).
+// (mt, nt): the workgroup's own first row and column.  Where its tile was moved
+// back into the matrix, what lies before them is another's (a group of four
+// columns across nt is written by both, with the same values).
 template <typename T, typename O, int MI, int NI, int ACT>
-__device__ __forceinline__ void finish_tile(const GemmParams &p, int m0, int n0, f32x4 (&acc)[MI][NI]) {
+__device__ __forceinline__ void finish_tile(const GemmParams &p, int m0, int n0, int mt, int nt, f32x4 (&acc)[MI][NI]) {
   const int lane = threadIdx.x % 64;
   float sa[MI];
   if constexpr (sizeof(T) == 1) {
@@ -290,14 +293,14 @@ __device__ __forceinline__ void finish_tile(const GemmParams &p, int m0, int n0,
 #pragma unroll
   for (int j = 0; j < NI; ++j) {
     const int n = n0 + j * 16 + lane / 16 * 4;
-    if (n >= p.n) continue;
+    if (n >= p.n || n + 3 < nt) continue;
     const f32x4 bias = bias4<O>(p, n);
     f32x4 sb;
     if constexpr (sizeof(T) == 1) sb = load4(p.sb + n, p.n - n);
 #pragma unroll
     for (int i = 0; i < MI; ++i) {
       const int m = m0 + i * 16 + lane % 16;
-      if (m >= p.m) continue;
+      if (m >= p.m || m < mt) continue;
       f32x4 v = acc[i][j];
       if constexpr (sizeof(T) == 1) v = v * sa[i] * sb;
       finish4<O, ACT>(p, m, n, v, bias);
@@ -323,16 +326,16 @@ __device__ __forceinline__ void store_part(const GemmParams &p, int split, int m
 }
 
 template <typename T, typename O, int MI, int NI>
-__device__ __forceinline__ void write_tile(const GemmParams &p, int split, int m0, int n0, f32x4 (&acc)[MI][NI]) {
+__device__ __forceinline__ void write_tile(const GemmParams &p, int split, int m0, int n0, int mt, int nt, f32x4 (&acc)[MI][NI]) {
   if (p.splits > 1) {
     store_part(p, split, m0, n0, acc);
     return;
   }
   switch (p.act) {
-    case ACT_RELU: finish_tile<T, O, MI, NI, ACT_RELU>(p, m0, n0, acc); break;
-    case ACT_GELU: finish_tile<T, O, MI, NI, ACT_GELU>(p, m0, n0, acc); break;
-    case ACT_SILU: finish_tile<T, O, MI, NI, ACT_SILU>(p, m0, n0, acc); break;
-    default: finish_tile<T, O, MI, NI, ACT_NONE>(p, m0, n0, acc); break;
+    case ACT_RELU: finish_tile<T, O, MI, NI, ACT_RELU>(p, m0, n0, mt, nt, acc); break;
+    case ACT_GELU: finish_tile<T, O, MI, NI, ACT_GELU>(p, m0, n0, mt, nt, acc); break;
+    case ACT_SILU: finish_tile<T, O, MI, NI, ACT_SILU>(p, m0, n0, mt, nt, acc); break;
+    default: finish_tile<T, O, MI, NI, ACT_NONE>(p, m0, n0, mt, nt, acc); break;
   }
 }
 
@@ -383,8 +386,10 @@ __global__ __launch_bounds__(64 * WM *WN) void gemm_tile_kernel(GemmParams p) {
   const int k0 = s0 * kSlab<T>;
   SlabLoader<T, AMN, BM, NW, DMA> la;
   SlabLoader<T, BMN, BN, NW, DMA> lb;
-  la.init(p.a, p.lda, p.m, tm * BM, k0, p.k);
-  lb.init(p.b, p.ldb, p.n, tn * BN, k0, p.k);
+  // Loads through registers: a tile that would reach past the matrix's end starts earlier.
+  const int m0 = DMA ? tm * BM : max(0, min(tm * BM, p.m - BM)), n0 = DMA ? tn * BN : max(0, min(tn * BN, p.n - BN));
+  la.init(p.a, p.lda, p.m, m0, k0, p.k);
+  lb.init(p.b, p.ldb, p.n, n0, k0, p.k);
   constexpr int LOADS = decltype(la)::PER_WAVE + decltype(lb)::PER_WAVE;
 
   const int wave = threadIdx.x / 64, wm = wave / WN, wn = wave % WN;
@@ -436,27 +441,181 @@ __global__ __launch_bounds__(64 * WM *WN) void gemm_tile_kernel(GemmParams p) {
       at = at == ST - 1 ? 0 : at + 1;
     }
   } else {
-    if (count > 0) {
-      la.fetch(0);
-      lb.fetch(0);
-      la.put(lds);
-      lb.put(lds + BM * 128);
-    }
-    for (int s = 0; s < count; ++s) {
-      wait_lds();
-      barrier();
-      if (s + 1 < count) {
-        la.fetch(s + 1);
-        lb.fetch(s + 1);
+    // Two slabs are under way in registers while one is multiplied.
+    i32x4 ha[2][decltype(la)::PER_WAVE], hb[2][decltype(lb)::PER_WAVE];
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+      if (s < count) {
+        la.fetch(s, ha[s]);
+        lb.fetch(s, hb[s]);
       }
-      multiply(lds + (s & 1) * STAGE);
-      if (s + 1 < count) {
-        la.put(lds + (~s & 1) * STAGE);
-        lb.put(lds + (~s & 1) * STAGE + BM * 128);
+    if (count > 0) {
+      la.put(lds, ha[0]);
+      lb.put(lds + BM * 128, hb[0]);
+    }
+    for (int s = 0; s < count; s += 2) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        if (s + h >= count) break;
+        wait_lds();
+        barrier();
+        if (s + h + 2 < count) {
+          la.fetch(s + h + 2, ha[h]);
+          lb.fetch(s + h + 2, hb[h]);
+        }
+        multiply(lds + h * STAGE);
+        if (s + h + 1 < count) {
+          la.put(lds + (1 - h) * STAGE, ha[1 - h]);
+          lb.put(lds + (1 - h) * STAGE + BM * 128, hb[1 - h]);
+        }
       }
     }
   }
-  write_tile<T, O, MI, NI>(p, split, tm * BM + wm * (BM / WM), tn * BN + wn * (BN / WN), acc);
+  write_tile<T, O, MI, NI>(p, split, m0 + wm * (BM / WM), n0 + wn * (BN / WN), tm * BM, tn * BN, acc);
+}
+
+// ---- few rows -----------------------------------------------------------------
+
+// Waves of a few-row workgroup: 16, or 8 where their registers would not fit.
+constexpr int rows_waves(bool bmn, int mi) { return bmn && mi > 1 ? 8 : 16; }
+
+// Up to 16*MI rows of C: bound by the right operand's one read, so the waves of
+// a workgroup stream it side by side, each its own slabs of k, and meet in LDS
+// at the end.  No barrier on the way.  16 columns a workgroup where the right
+// operand lies along k: its pieces are fragments as they come.  32 columns where
+// it lies along n: a wave turns its slab over in LDS of its own, 64-byte lines
+// with piece c of line k at c ^ (k & 2).  The left operand's pieces come from the
+// caches.  Any alignment.  The last workgroup's columns are moved back into the
+// matrix (n >= 32 where the right operand lies along n) and a last part of a slab
+// is read apart, so the loads on the way are unguarded.
+template <typename T, typename O, bool BMN, int MI>
+__global__ __launch_bounds__(64 * rows_waves(BMN, MI)) void gemm_rows_kernel(GemmParams p) {
+  constexpr int NB = BMN ? 2 : 1, NW = rows_waves(BMN, MI), WP = BMN ? 4 : 2;  // pieces a lane of one slab of B
+  constexpr int P = kPiece<T>;
+  constexpr int TURN = BMN ? NW * 4096 : 0, JOIN = NW * MI * NB * 1024;
+  __shared__ __align__(1024) char smem[TURN > JOIN ? TURN : JOIN];
+  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, g = lane / 16, l = lane % 16;
+  // Neighbouring columns on one XCD: they share the lines of B that lie along n.
+  const int per = gridDim.x >> 3, more = gridDim.x & 7, xcd = blockIdx.x & 7;
+  const int nt = (xcd * per + min(xcd, more) + static_cast<int>(blockIdx.x >> 3)) * 16 * NB;
+  const int n0 = BMN ? min(nt, p.n - 16 * NB) : nt;
+  const int slabs = p.k / kSlab<T>;  // whole ones
+  const T *a[MI];
+#pragma unroll
+  for (int i = 0; i < MI; ++i)  // rows past the last repeat it; their results are not written
+    a[i] = static_cast<const T *>(p.a) + min(i * 16 + l, p.m - 1) * p.lda;
+  const T *b = static_cast<const T *>(p.b);
+  if constexpr (BMN) b += (lane / 4) * p.ldb + n0 + lane % 4 * 8;
+  else b += min(n0 + l, p.n - 1) * p.ldb;
+
+  struct Held {
+    i32x4 a[MI][2], b[WP];
+  };
+  const auto fetch = [&](Held &h, int s) {
+    const int k0 = s * kSlab<T>;
+#pragma unroll
+    for (int i = 0; i < WP; ++i)
+      h.b[i] = *reinterpret_cast<const loose16 *>(BMN ? b + (k0 + i * 16) * p.ldb : b + k0 + (i * 4 + g) * P);
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
+#pragma unroll
+      for (int q = 0; q < 2; ++q) h.a[i][q] = *reinterpret_cast<const loose16 *>(a[i] + k0 + (q * 4 + g) * P);
+  };
+  f32x4 acc[MI][NB];
+#pragma unroll
+  for (int i = 0; i < MI; ++i)
+#pragma unroll
+    for (int j = 0; j < NB; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  lds_char *turn = (lds_char *)smem + wave * 4096;
+  const auto multiply = [&](Held &h) {
+    i32x4 bf[NB][2];
+    if constexpr (BMN) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int k = i * 16 + lane / 4;
+        *reinterpret_cast<__attribute__((address_space(3))) i32x4 *>(turn + k * 64 + (((lane % 4) ^ (k & 2)) << 4)) = h.b[i];
+      }
+      const int r = l / 4, q = l % 4;
+#pragma unroll
+      for (int j = 0; j < NB; ++j)
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk) {
+          const lds_char *at = turn + (kk * 32 + 8 * g + r) * 64 + (((2 * j + q / 2) ^ (r & 2)) << 4) + (q & 1) * 8;
+          union {
+            i16x4 h[2];
+            i32x4 v;
+          } u;
+          u.h[0] = lds_read_tr(at);
+          u.h[1] = lds_read_tr(at + 4 * 64);
+          bf[j][kk] = u.v;
+        }
+    } else {
+      bf[0][0] = h.b[0];
+      bf[0][1] = h.b[1];
+    }
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
+#pragma unroll
+      for (int j = 0; j < NB; ++j) acc[i][j] = block_mma(T{}, h.a[i][0], h.a[i][1], bf[j][0], bf[j][1], acc[i][j]);
+  };
+  // DEEP slabs are in flight while one is multiplied.
+  constexpr int DEEP = MI == 1 && !BMN ? 4 : 2;
+  Held held[DEEP];
+  int s = wave;
+#pragma unroll
+  for (int q = 0; q < DEEP; ++q)
+    if (s + q * NW < slabs) fetch(held[q], s + q * NW);
+  for (; s < slabs; s += DEEP * NW) {
+#pragma unroll
+    for (int q = 0; q < DEEP; ++q) {
+      if (s + q * NW < slabs) {
+        multiply(held[q]);
+        if (s + (q + DEEP) * NW < slabs) fetch(held[q], s + (q + DEEP) * NW);
+      }
+    }
+  }
+  if (p.k % kSlab<T> && wave == slabs % NW) {  // what is left of k
+    const int k0 = slabs * kSlab<T>;
+    Held &h = held[0];
+#pragma unroll
+    for (int i = 0; i < WP; ++i) {
+      if constexpr (BMN) {
+        const int k = k0 + i * 16 + lane / 4;
+        h.b[i] = i32x4{0, 0, 0, 0};
+        if (k < p.k) h.b[i] = *reinterpret_cast<const loose16 *>(b + (k0 + i * 16) * p.ldb);
+      } else {
+        h.b[i] = load_piece_any(b, k0 + (i * 4 + g) * P, p.k);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
+#pragma unroll
+      for (int q = 0; q < 2; ++q) h.a[i][q] = load_piece_any(a[i], k0 + (q * 4 + g) * P, p.k);
+    multiply(h);
+  }
+  // The waves' sums, added in wave order.
+  __syncthreads();
+  f32x4 *join = reinterpret_cast<f32x4 *>(smem);
+#pragma unroll
+  for (int i = 0; i < MI; ++i)
+#pragma unroll
+    for (int j = 0; j < NB; ++j) join[(wave * MI * NB + i * NB + j) * 64 + lane] = acc[i][j];
+  __syncthreads();
+  const int block = wave;
+  if (block >= MI * NB) return;
+  f32x4 v = join[block * 64 + lane];
+#pragma unroll
+  for (int w = 1; w < NW; ++w) v += join[(w * MI * NB + block) * 64 + lane];
+  const int m = block / NB * 16 + l, n = n0 + block % NB * 16 + g * 4;
+  if (m >= p.m || n >= p.n || n + 3 < nt) return;
+  if constexpr (sizeof(T) == 1) v = v * p.sa[m] * load4(p.sb + n, p.n - n);
+  const f32x4 bias = bias4<O>(p, n);
+  switch (p.act) {
+    case ACT_RELU: finish4<O, ACT_RELU>(p, m, n, v, bias); break;
+    case ACT_GELU: finish4<O, ACT_GELU>(p, m, n, v, bias); break;
+    case ACT_SILU: finish4<O, ACT_SILU>(p, m, n, v, bias); break;
+    default: finish4<O, ACT_NONE>(p, m, n, v, bias); break;
+  }
 }
 
 }  // namespace tfnn

@@ -42,7 +42,9 @@ struct GemmParams {
 };
 
 // C tiles of the product kernels.  256 x 256 loads straight into LDS only.
-enum Tile { TILE_256 = 1, TILE_128 = 2, TILE_64 = 3 };
+// TILE_ROWS: all of up to 64 rows, the waves of a workgroup split k (the left
+// operand along k only).
+enum Tile { TILE_256 = 1, TILE_128 = 2, TILE_64 = 3, TILE_ROWS = 4 };
 constexpr int tile_size(int tile) { return tile == TILE_256 ? 256 : tile == TILE_128 ? 128 : 64; }
 
 // amn, bmn: the operand's own dimension (m, n) is contiguous, not k.

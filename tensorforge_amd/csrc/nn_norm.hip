@@ -17,15 +17,21 @@
 namespace tfnn {
 namespace {
 
-template <typename T>
-__device__ __forceinline__ void load8(const T *p, int left, float (&v)[8]) {
-  if (left >= 8) {
-    const typename Vec<T, 8>::loose u = *reinterpret_cast<const typename Vec<T, 8>::loose *>(p);
+// Row lengths: WHOLE, a multiple of 8; TAIL, at least 8; ANY (the long kernels).
+enum Length { WHOLE, TAIL, ANY };
+
+// 8 elements from c of a row of `length`; zeros past its end.
+template <Length L, typename T>
+__device__ __forceinline__ void load8(const T *row, int c, int length, float (&v)[8]) {
+  constexpr int N = 16 / sizeof(T);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = static_cast<float>(u[i]);
-  } else {
+  for (int q = 0; q < 8 / N; ++q) {
+    i32x4 raw;
+    if constexpr (L == ANY) raw = load_piece_any(row, c + q * N, length);
+    else raw = load_piece<L == WHOLE>(row, c + q * N, length);
+    const auto u = __builtin_bit_cast(typename Vec<T, N>::type, raw);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = i < left ? static_cast<float>(p[i]) : 0.0f;
+    for (int i = 0; i < N; ++i) v[q * N + i] = static_cast<float>(u[i]);
   }
 }
 
@@ -58,16 +64,17 @@ __device__ __forceinline__ void store8(f8 *p, int left, const float (&v)[8]) {
   }
 }
 
-__device__ __forceinline__ void load_weight8(const NormParams &p, int c, int left, float (&w)[8]) {
+template <Length L>
+__device__ __forceinline__ void load_weight8(const NormParams &p, int c, float (&w)[8]) {
   if (!p.weight) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) w[i] = 1.0f;
   } else if (p.weight_type == TYPE_F32) {
-    load8(static_cast<const float *>(p.weight) + c, left, w);
+    load8<L>(static_cast<const float *>(p.weight), c, p.d, w);
   } else if (p.weight_type == TYPE_BF16) {
-    load8(static_cast<const bf16 *>(p.weight) + c, left, w);
+    load8<L>(static_cast<const bf16 *>(p.weight), c, p.d, w);
   } else {
-    load8(static_cast<const f16 *>(p.weight) + c, left, w);
+    load8<L>(static_cast<const f16 *>(p.weight), c, p.d, w);
   }
 }
 
@@ -99,26 +106,26 @@ __device__ __forceinline__ void row_reduce(float &sum, float &more, int turn) {
 
 // CH pieces of 8 elements a thread, NT threads a row, 256/NT rows a workgroup.
 // The weights stay in registers over a workgroup's rows.
-template <typename T, typename O, int NT, int CH>
+template <typename T, typename O, int NT, int CH, Length L>
 __global__ __launch_bounds__(256) void rms_norm_kernel(NormParams p) {
   constexpr int RPB = 256 / NT;
   const int t = threadIdx.x % NT, sub = threadIdx.x / NT;
   float w[CH][8];
 #pragma unroll
-  for (int j = 0; j < CH; ++j) load_weight8(p, (j * NT + t) * 8, p.d - (j * NT + t) * 8, w[j]);
+  for (int j = 0; j < CH; ++j) load_weight8<L>(p, (j * NT + t) * 8, w[j]);
   int turn = 0;
   for (long row = static_cast<long>(blockIdx.x) * RPB + sub; row < p.rows; row += static_cast<long>(gridDim.x) * RPB) {
     const T *x = static_cast<const T *>(p.x) + row * p.x_ld;
     float h[CH][8];
 #pragma unroll
-    for (int j = 0; j < CH; ++j) load8(x + (j * NT + t) * 8, p.d - (j * NT + t) * 8, h[j]);
+    for (int j = 0; j < CH; ++j) load8<L>(x, (j * NT + t) * 8, p.d, h[j]);
     if (p.residual) {
       const T *res = static_cast<const T *>(p.residual) + row * p.residual_ld;
       T *ho = static_cast<T *>(p.h) + row * p.h_ld;
 #pragma unroll
       for (int j = 0; j < CH; ++j) {
         float v[8];
-        load8(res + (j * NT + t) * 8, p.d - (j * NT + t) * 8, v);
+        load8<L>(res, (j * NT + t) * 8, p.d, v);
 #pragma unroll
         for (int i = 0; i < 8; ++i) h[j][i] += v[i];
       }
@@ -167,13 +174,13 @@ __global__ __launch_bounds__(256) void rms_norm_long_kernel(NormParams p) {
   float sum = 0.0f, top = 0.0f;
   for (int c = threadIdx.x * 8; c < p.d; c += NT * 8) {
     float v[8], u[8], w[8];
-    load8(x + c, p.d - c, v);
+    load8<ANY>(x, c, p.d, v);
     if (res) {
-      load8(res + c, p.d - c, u);
+      load8<ANY>(res, c, p.d, u);
 #pragma unroll
       for (int i = 0; i < 8; ++i) v[i] += u[i];
     }
-    load_weight8(p, c, p.d - c, w);
+    load_weight8<ANY>(p, c, w);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       sum = __builtin_fmaf(v[i], v[i], sum);
@@ -190,14 +197,14 @@ __global__ __launch_bounds__(256) void rms_norm_long_kernel(NormParams p) {
   }
   for (int c = threadIdx.x * 8; c < p.d; c += NT * 8) {
     float v[8], u[8], w[8];
-    load8(x + c, p.d - c, v);
+    load8<ANY>(x, c, p.d, v);
     if (res) {
-      load8(res + c, p.d - c, u);
+      load8<ANY>(res, c, p.d, u);
 #pragma unroll
       for (int i = 0; i < 8; ++i) v[i] += u[i];
       store8(static_cast<T *>(p.h) + row * p.h_ld + c, p.d - c, v);
     }
-    load_weight8(p, c, p.d - c, w);
+    load_weight8<ANY>(p, c, w);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       v[i] = v[i] * r * w[i];
@@ -209,15 +216,15 @@ __global__ __launch_bounds__(256) void rms_norm_long_kernel(NormParams p) {
 
 // The gradient's dx, and this workgroup's rows' share of dw.  The shares are
 // added by share_sum_kernel, in a fixed order.
-template <typename T, int NT, int CH>
+template <typename T, int NT, int CH, Length L>
 __global__ __launch_bounds__(256) void rms_norm_grad_kernel(NormGradParams p) {
   constexpr int RPB = 256 / NT;
   const int t = threadIdx.x % NT, sub = threadIdx.x / NT;
-  const NormParams wp{.weight = p.weight, .weight_type = p.weight_type};
+  const NormParams wp{.weight = p.weight, .d = p.d, .weight_type = p.weight_type};
   float w[CH][8], dw[CH][8];
 #pragma unroll
   for (int j = 0; j < CH; ++j) {
-    load_weight8(wp, (j * NT + t) * 8, p.d - (j * NT + t) * 8, w[j]);
+    load_weight8<L>(wp, (j * NT + t) * 8, w[j]);
 #pragma unroll
     for (int i = 0; i < 8; ++i) dw[j][i] = 0.0f;
   }
@@ -226,10 +233,10 @@ __global__ __launch_bounds__(256) void rms_norm_grad_kernel(NormGradParams p) {
     float h[CH][8], g[CH][8];
 #pragma unroll
     for (int j = 0; j < CH; ++j)
-      load8(static_cast<const T *>(p.h) + row * p.h_ld + (j * NT + t) * 8, p.d - (j * NT + t) * 8, h[j]);
+      load8<L>(static_cast<const T *>(p.h) + row * p.h_ld, (j * NT + t) * 8, p.d, h[j]);
 #pragma unroll
     for (int j = 0; j < CH; ++j)
-      load8(static_cast<const T *>(p.dy) + row * p.dy_ld + (j * NT + t) * 8, p.d - (j * NT + t) * 8, g[j]);
+      load8<L>(static_cast<const T *>(p.dy) + row * p.dy_ld, (j * NT + t) * 8, p.d, g[j]);
     float sum = 0.0f, dot = 0.0f;
 #pragma unroll
     for (int j = 0; j < CH; ++j)
@@ -246,7 +253,7 @@ __global__ __launch_bounds__(256) void rms_norm_grad_kernel(NormGradParams p) {
     for (int j = 0; j < CH; ++j) {
       const int at = (j * NT + t) * 8;
       float v[8], u[8];
-      if (p.dh) load8(static_cast<const T *>(p.dh) + row * p.dh_ld + at, p.d - at, u);
+      if (p.dh) load8<L>(static_cast<const T *>(p.dh) + row * p.dh_ld, at, p.d, u);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         v[i] = r * __builtin_fmaf(-c, h[j][i], g[j][i] * w[j][i]);
@@ -283,7 +290,7 @@ __global__ __launch_bounds__(256) void rms_norm_grad_kernel(NormGradParams p) {
 template <typename T>
 __global__ __launch_bounds__(256) void rms_norm_grad_long_kernel(NormGradParams p) {
   constexpr int NT = 256;
-  const NormParams wp{.weight = p.weight, .weight_type = p.weight_type};
+  const NormParams wp{.weight = p.weight, .d = p.d, .weight_type = p.weight_type};
   float *share = p.shares + static_cast<long>(blockIdx.x) * p.d;
   int turn = 0;
   bool first = true;
@@ -293,9 +300,9 @@ __global__ __launch_bounds__(256) void rms_norm_grad_long_kernel(NormGradParams 
     float sum = 0.0f, dot = 0.0f;
     for (int c = threadIdx.x * 8; c < p.d; c += NT * 8) {
       float h[8], g[8], w[8];
-      load8(hp + c, p.d - c, h);
-      load8(gp + c, p.d - c, g);
-      load_weight8(wp, c, p.d - c, w);
+      load8<ANY>(hp, c, p.d, h);
+      load8<ANY>(gp, c, p.d, g);
+      load_weight8<ANY>(wp, c, w);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         sum = __builtin_fmaf(h[i], h[i], sum);
@@ -308,11 +315,11 @@ __global__ __launch_bounds__(256) void rms_norm_grad_long_kernel(NormGradParams 
     const float k = dot * r * r / static_cast<float>(p.d);
     for (int c = threadIdx.x * 8; c < p.d; c += NT * 8) {
       float h[8], g[8], w[8], u[8], s[8];
-      load8(hp + c, p.d - c, h);
-      load8(gp + c, p.d - c, g);
-      load_weight8(wp, c, p.d - c, w);
-      if (p.dh) load8(static_cast<const T *>(p.dh) + row * p.dh_ld + c, p.d - c, u);
-      if (!first) load8(share + c, p.d - c, s);
+      load8<ANY>(hp, c, p.d, h);
+      load8<ANY>(gp, c, p.d, g);
+      load_weight8<ANY>(wp, c, w);
+      if (p.dh) load8<ANY>(static_cast<const T *>(p.dh) + row * p.dh_ld, c, p.d, u);
+      if (!first) load8<ANY>(share, c, p.d, s);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         s[i] = __builtin_fmaf(g[i] * r, h[i], first ? 0.0f : s[i]);
@@ -326,31 +333,41 @@ __global__ __launch_bounds__(256) void rms_norm_grad_long_kernel(NormGradParams 
   }
 }
 
-// The shares' sum, in order: 32 columns a workgroup, 8 threads of four
-// columns by 32 rows of shares.
+// The shares' sum, in order: 16 columns a workgroup, 4 threads of four columns by
+// 64 rows of shares.  Bound by latency: 16 loads in flight a thread.
 __global__ __launch_bounds__(256) void share_sum_kernel(const float *shares, int count, int d, void *out, int type) {
-  const int c = blockIdx.x * 32 + threadIdx.x % 8 * 4, lane = threadIdx.x / 8;
+  const int c = blockIdx.x * 16 + threadIdx.x % 4 * 4, lane = threadIdx.x / 4;
   f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
-  for (int q = lane; q < count; q += 32) {
-    const float *p = shares + static_cast<long>(q) * d + c;
-    if (c + 4 <= d) {
-      s += *reinterpret_cast<const Vec<float, 4>::loose *>(p);
-    } else {
+  if (c + 4 <= d) {
+    const float *p = shares + c;
+    for (int q = lane; q < count; q += 1024) {
+      f32x4 v[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (q + i * 64 < count) v[i] = *reinterpret_cast<const Vec<float, 4>::loose *>(p + static_cast<long>(q + i * 64) * d);
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (q + i * 64 < count) s += v[i];
+    }
+  } else {
+    for (int q = lane; q < count; q += 64)
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        if (c + i < d) s[i] += p[i];
-    }
+        if (c + i < d) s[i] += shares[static_cast<long>(q) * d + c + i];
   }
-  __shared__ float part[32][33];
+  __shared__ float part[64][17];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) part[lane][threadIdx.x % 8 * 4 + i] = s[i];
+  for (int i = 0; i < 4; ++i) part[lane][threadIdx.x % 4 * 4 + i] = s[i];
   __syncthreads();
-  if (threadIdx.x < 32) {
-    const int at = blockIdx.x * 32 + threadIdx.x;
+  if (threadIdx.x < 64) {
+    // 4 threads a column, 16 rows each, joined in lane order.
+    const int col = threadIdx.x / 4, at = blockIdx.x * 16 + col;
     float v = 0.0f;
 #pragma unroll
-    for (int q = 0; q < 32; ++q) v += part[q][threadIdx.x];
-    if (at < d) store_as(out, type, at, v);
+    for (int q = 0; q < 16; ++q) v += part[threadIdx.x % 4 * 16 + q][col];
+    v += __shfl_xor(v, 1);
+    v += __shfl_xor(v, 2);
+    if (threadIdx.x % 4 == 0 && at < d) store_as(out, type, at, v);
   }
 }
 
@@ -362,45 +379,58 @@ constexpr int kLongest = 16384;
 
 int pieces(long d) { return static_cast<int>((d + 7) / 8); }
 
-template <typename T, typename O>
-void norm_launch(const NormParams &p, hipStream_t stream) {
+template <typename T, typename O, Length L>
+void norm_launch_as(const NormParams &p, hipStream_t stream) {
   const int n = pieces(p.d);
   const dim3 waves(static_cast<unsigned>(std::min<long>((p.rows + 3) / 4, kNormGroups)));
   const dim3 groups(static_cast<unsigned>(std::min<long>(p.rows, kNormGroups)));
-  if (n <= 64) rms_norm_kernel<T, O, 64, 1><<<waves, 256, 0, stream>>>(p);
-  else if (n <= 128) rms_norm_kernel<T, O, 64, 2><<<waves, 256, 0, stream>>>(p);
-  else if (n <= 256) rms_norm_kernel<T, O, 256, 1><<<groups, 256, 0, stream>>>(p);
-  else if (n <= 512) rms_norm_kernel<T, O, 256, 2><<<groups, 256, 0, stream>>>(p);
-  else if (n <= 1024) rms_norm_kernel<T, O, 256, 4><<<groups, 256, 0, stream>>>(p);
-  else if (p.d <= kLongest) rms_norm_kernel<T, O, 256, 8><<<groups, 256, 0, stream>>>(p);
-  else rms_norm_long_kernel<T, O><<<dim3(static_cast<unsigned>(p.rows)), 256, 0, stream>>>(p);
+  if (n <= 64) rms_norm_kernel<T, O, 64, 1, L><<<waves, 256, 0, stream>>>(p);
+  else if (n <= 128) rms_norm_kernel<T, O, 64, 2, L><<<waves, 256, 0, stream>>>(p);
+  else if (n <= 256) rms_norm_kernel<T, O, 256, 1, L><<<groups, 256, 0, stream>>>(p);
+  else if (n <= 512) rms_norm_kernel<T, O, 256, 2, L><<<groups, 256, 0, stream>>>(p);
+  else if (n <= 1024) rms_norm_kernel<T, O, 256, 4, L><<<groups, 256, 0, stream>>>(p);
+  else rms_norm_kernel<T, O, 256, 8, L><<<groups, 256, 0, stream>>>(p);
+}
+
+template <typename T, typename O>
+void norm_launch(const NormParams &p, hipStream_t stream) {
+  if (p.d < 8 || p.d > kLongest) rms_norm_long_kernel<T, O><<<dim3(static_cast<unsigned>(p.rows)), 256, 0, stream>>>(p);
+  else if (p.d % 8 == 0) norm_launch_as<T, O, WHOLE>(p, stream);
+  else norm_launch_as<T, O, TAIL>(p, stream);
+}
+
+template <typename T, Length L>
+void norm_grad_launch_as(const NormGradParams &p, dim3 grid, hipStream_t stream) {
+  const int n = pieces(p.d);
+  if (n <= 64) rms_norm_grad_kernel<T, 64, 1, L><<<grid, 256, 0, stream>>>(p);
+  else if (n <= 128) rms_norm_grad_kernel<T, 64, 2, L><<<grid, 256, 0, stream>>>(p);
+  else if (n <= 256) rms_norm_grad_kernel<T, 256, 1, L><<<grid, 256, 0, stream>>>(p);
+  else if (n <= 512) rms_norm_grad_kernel<T, 256, 2, L><<<grid, 256, 0, stream>>>(p);
+  else if (n <= 1024) rms_norm_grad_kernel<T, 256, 4, L><<<grid, 256, 0, stream>>>(p);
+  else rms_norm_grad_kernel<T, 256, 8, L><<<grid, 256, 0, stream>>>(p);
 }
 
 template <typename T>
 void norm_grad_launch(const NormGradParams &p, hipStream_t stream) {
-  const int n = pieces(p.d);
   const long shares = norm_grad_shares(p.rows, p.d);
   const dim3 grid(static_cast<unsigned>(shares));
-  if (shares == 0) {
-  } else if (n <= 64) rms_norm_grad_kernel<T, 64, 1><<<grid, 256, 0, stream>>>(p);
-  else if (n <= 128) rms_norm_grad_kernel<T, 64, 2><<<grid, 256, 0, stream>>>(p);
-  else if (n <= 256) rms_norm_grad_kernel<T, 256, 1><<<grid, 256, 0, stream>>>(p);
-  else if (n <= 512) rms_norm_grad_kernel<T, 256, 2><<<grid, 256, 0, stream>>>(p);
-  else if (n <= 1024) rms_norm_grad_kernel<T, 256, 4><<<grid, 256, 0, stream>>>(p);
-  else if (p.d <= kLongest) rms_norm_grad_kernel<T, 256, 8><<<grid, 256, 0, stream>>>(p);
-  else rms_norm_grad_long_kernel<T><<<grid, 256, 0, stream>>>(p);
+  if (shares) {
+    if (p.d < 8 || p.d > kLongest) rms_norm_grad_long_kernel<T><<<grid, 256, 0, stream>>>(p);
+    else if (p.d % 8 == 0) norm_grad_launch_as<T, WHOLE>(p, grid, stream);
+    else norm_grad_launch_as<T, TAIL>(p, grid, stream);
+  }
   (void)launch_share_sum(p.shares, shares, p.d, p.dw, p.weight_type, stream);
 }
 
 }  // namespace
 
 long norm_grad_shares(long rows, long d) {
-  const long rpb = pieces(d) <= 128 ? 4 : 1;
+  const long rpb = d >= 8 && pieces(d) <= 128 ? 4 : 1;  // rows a workgroup takes at a time
   return std::min<long>((rows + rpb - 1) / rpb, 1024);
 }
 
 hipError_t launch_share_sum(const float *shares, long count, int d, void *out, int type, hipStream_t stream) {
-  share_sum_kernel<<<dim3(static_cast<unsigned>((d + 31) / 32)), 256, 0, stream>>>(shares, static_cast<int>(count), d, out,
+  share_sum_kernel<<<dim3(static_cast<unsigned>((d + 15) / 16)), 256, 0, stream>>>(shares, static_cast<int>(count), d, out,
                                                                                   type);
   return hipGetLastError();
 }

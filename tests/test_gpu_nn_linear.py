@@ -87,11 +87,25 @@ def test_linear_tiles(tile, splits, order, dtype):
         _check(out, x, w, b, "gelu", r, None, dtype)
 
 
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("order", [0, 1])
+def test_linear_few_rows(order, dtype):
+    """The few-row kernel over its three heights, with fewer and more slabs of k than a workgroup's waves hold."""
+    nn = _nn()
+    for m in (1, 2, 15, 16, 17, 32, 33, 64):
+        for n, k in ((8, 64), (16, 1024), (31, 67), (33, 2200), (40, 5000), (100, 513)):
+            g = torch.Generator().manual_seed(m + n + k)
+            x, w, r = _matrix(g, m, k, dtype), _matrix(g, k, n, dtype, k ** -0.5), _matrix(g, m, n, dtype)
+            b = torch.randn(n, generator=g)
+            out, z = nn.linear(x.cuda(), _ordered(w, order), b.cuda(), "silu", r.cuda(), keep=True, tile=4)
+            _check(out, x, w, b, "silu", r, z, dtype)
+
+
 @pytest.mark.parametrize("out_dtype", HALF)
 @pytest.mark.parametrize("tile,splits", [(0, 0), (1, 1), (2, 1), (3, 1), (2, 2), (3, 3)])
 def test_linear_8bit(tile, splits, out_dtype):
     nn = _nn()
-    for m, n, k in ((1, 1, 1), (1, 64, 128), (16, 48, 256), (17, 257, 144), (64, 130, 1040), (257, 264, 272), (40, 72, 100)):
+    for m, n, k in ((1, 1, 1), (1, 64, 128), (16, 48, 256), (17, 257, 144), (30, 70, 9000), (64, 130, 1040), (257, 264, 272), (40, 72, 100)):
         g = torch.Generator().manual_seed(m + n + k)
         q, s = nn.quantize_rows(_matrix(g, m, k, torch.float32).cuda())
         wq, ws = nn.quantize_rows(_matrix(g, n, k, torch.float32, k ** -0.5).cuda())

@@ -49,7 +49,7 @@ def _linear(**kw):
     (dict(w_order=2), "w_order = 2"), (dict(out_ld=31), "out: 31"), (dict(z=256, z_ld=8), "z: 8"),
     (dict(residual=256, residual_ld=3), "residual: 3"), (dict(bias=256, bias_type=2), "bias_type = 2"),
     (dict(x_scale=256), "scales belong to 8-bit"), (dict(type=3), "8-bit weights"),
-    (dict(type=3, w_order=1, w_ld=64), "x_scale is a null pointer"), (dict(tile=4), "tile = 4"),
+    (dict(type=3, w_order=1, w_ld=64), "x_scale is a null pointer"), (dict(tile=5), "tile = 5"),
     (dict(splits=65), "splits = 65"), (dict(workspace=8, workspace_bytes=64), "not 16-byte aligned"),
     (dict(x_ld=1 << 41), "are too many"),
 ])
