@@ -33,6 +33,7 @@ typedef short i16x4 __attribute__((ext_vector_type(4)));
 template <int I>
 struct Int {
   __host__ __device__ constexpr operator int() const { return I; }
+  __host__ __device__ constexpr int operator()() const { return I; }
 };
 template <int N, int I = 0, typename F>
 __device__ __forceinline__ void unroll(F &&f) {

@@ -28,10 +28,13 @@ constexpr int kPiece = 16 / sizeof(T);  // elements in a 16-byte piece
 // different banks.
 //
 // Own dimension contiguous: blocks of 64 rows (of the own dimension), in each
-// 64 k-lines of 128 bytes; the piece c of line k is at place c ^ (2 (k & 3)), so
-// that the four lines of a transposing read lie in different banks.
+// 64 k-lines of 128 bytes; the piece c of line k is at place c ^ turn(k), so that
+// the eight lines that two transposing reads of 16 lanes touch at once (k and k + 8)
+// lie in different banks.
 //
 // Either way 1 KiB = 8 lines are one wave's 16-byte load, straight into LDS.
+
+__device__ __forceinline__ int line_turn(int k) { return 2 * ((k & 3) ^ (k >> 3 & 1)); }
 
 // A read piece: 8 (16-bit) or 16 (8-bit) elements along k of one row.
 __device__ __forceinline__ i32x4 lds_read16(const lds_char *p) {
@@ -60,7 +63,7 @@ struct FragReader {
 #pragma unroll
       for (int b = 0; b < 4; ++b) {
         const int row = row0 + b * 16;  // row0: a multiple of 16
-        at[b] = row / 64 * 8192 + (8 * g + r) * 128 + (((row % 64 / 8 + q / 2) ^ (2 * r)) << 4) + (q & 1) * 8;
+        at[b] = row / 64 * 8192 + (8 * g + r) * 128 + (((row % 64 / 8 + q / 2) ^ line_turn(8 * g + r)) << 4) + (q & 1) * 8;
       }
     }
   }
@@ -125,7 +128,7 @@ struct SlabLoader {
       k = ((lane % 8) ^ (lane / 8)) * kPiece<T>;
     } else {
       k = t % 8 * 8 + lane / 8;
-      row = t / 8 * 64 + ((lane % 8) ^ (2 * (lane / 8 & 3))) * kPiece<T>;
+      row = t / 8 * 64 + ((lane % 8) ^ line_turn(k)) * kPiece<T>;
     }
   }
 
@@ -227,116 +230,130 @@ __device__ __forceinline__ f32x4 block_mma(f8, i32x4 a0, i32x4 a1, i32x4 b0, i32
 
 // ---- epilogue ---------------------------------------------------------------
 
-// Four consecutive values from p[0..left), zeros past them.
-template <typename T>
-__device__ __forceinline__ f32x4 load4(const T *p, int left) {
-  f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
-  if (left >= 4) {
-    const typename Vec<T, 4>::loose u = *reinterpret_cast<const typename Vec<T, 4>::loose *>(p);
+// N consecutive values from p[0..left), zeros past them.
+template <int N, typename T>
+__device__ __forceinline__ void load_some(const T *p, int left, float (&v)[N]) {
+  if (left >= N) {
+    const typename Vec<T, N>::loose u = *reinterpret_cast<const typename Vec<T, N>::loose *>(p);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = static_cast<float>(u[i]);
+    for (int i = 0; i < N; ++i) v[i] = static_cast<float>(u[i]);
   } else {
 #pragma unroll
-    for (int i = 0; i < 3; ++i)
-      if (i < left) v[i] = static_cast<float>(p[i]);
+    for (int i = 0; i < N; ++i) v[i] = i < left ? static_cast<float>(p[i]) : 0.0f;
   }
-  return v;
 }
-template <typename T>
-__device__ __forceinline__ void store4(T *p, int left, f32x4 v) {
-  if (left >= 4) {
-    typename Vec<T, 4>::loose u;
+template <int N, typename T>
+__device__ __forceinline__ void store_some(T *p, int left, const float (&v)[N]) {
+  if (left >= N) {
+    typename Vec<T, N>::loose u;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) u[i] = static_cast<T>(v[i]);
-    *reinterpret_cast<typename Vec<T, 4>::loose *>(p) = u;
+    for (int i = 0; i < N; ++i) u[i] = static_cast<T>(v[i]);
+    *reinterpret_cast<typename Vec<T, N>::loose *>(p) = u;
   } else {
 #pragma unroll
-    for (int i = 0; i < 3; ++i)
+    for (int i = 0; i < N; ++i)
       if (i < left) p[i] = static_cast<T>(v[i]);
   }
 }
 
-template <typename O>
-__device__ __forceinline__ f32x4 bias4(const GemmParams &p, int n) {
-  if (!p.bias) return f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-  if (p.bias_f32) return load4(static_cast<const float *>(p.bias) + n, p.n - n);
-  return load4(static_cast<const O *>(p.bias) + n, p.n - n);
+template <typename O, int N>
+__device__ __forceinline__ void load_bias(const GemmParams &p, int n, float (&v)[N]) {
+  if (!p.bias) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = 0.0f;
+  } else if (p.bias_f32) {
+    load_some(static_cast<const float *>(p.bias) + n, p.n - n, v);
+  } else {
+    load_some(static_cast<const O *>(p.bias) + n, p.n - n, v);
+  }
 }
 
 // z = v + bias (kept if asked for); out = act(z) + residual, rounded once.
-template <typename O, int ACT>
-__device__ __forceinline__ void finish4(const GemmParams &p, int m, int n, f32x4 v, f32x4 bias) {
+template <typename O, int ACT, int N>
+__device__ __forceinline__ void finish(const GemmParams &p, int m, int n, float (&v)[N], const float (&bias)[N]) {
   const int left = p.n - n;
-  v += bias;
-  if (p.z) store4(static_cast<O *>(p.z) + m * p.ldz + n, left, v);
+  float res[N];
+  if (p.residual) load_some(static_cast<const O *>(p.residual) + m * p.ldr + n, left, res);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) v[i] = act_value<ACT>(v[i]);
-  if (p.residual) v += load4(static_cast<const O *>(p.residual) + m * p.ldr + n, left);
-  store4(static_cast<O *>(p.out) + m * p.ldo + n, left, v);
+  for (int i = 0; i < N; ++i) v[i] += bias[i];
+  if (p.z) store_some(static_cast<O *>(p.z) + m * p.ldz + n, left, v);
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = act_value<ACT>(v[i]);
+  if (p.residual) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] += res[i];
+  }
+  store_some(static_cast<O *>(p.out) + m * p.ldo + n, left, v);
 }
 
-// A wave's accumulators: MI x NI blocks from (m0, n0).
-// (mt, nt): the workgroup's own first row and column.  Where its tile was moved
-// back into the matrix, what lies before them is another's (a group of four
-// columns across nt is written by both, with the same values).
-template <typename T, typename O, int MI, int NI, int ACT>
-__device__ __forceinline__ void finish_tile(const GemmParams &p, int m0, int n0, int mt, int nt, f32x4 (&acc)[MI][NI]) {
-  const int lane = threadIdx.x % 64;
-  float sa[MI];
-  if constexpr (sizeof(T) == 1) {
-#pragma unroll
-    for (int i = 0; i < MI; ++i) {
-      const int m = m0 + i * 16 + lane % 16;
-      sa[i] = m < p.m ? p.sa[m] : 0.0f;
-    }
+// f(constant) for the product's activation.
+template <typename F>
+__device__ __forceinline__ void with_act(int act, F &&f) {
+  switch (act) {
+    case ACT_RELU: f(Int<ACT_RELU>{}); break;
+    case ACT_GELU: f(Int<ACT_GELU>{}); break;
+    case ACT_SILU: f(Int<ACT_SILU>{}); break;
+    default: f(Int<ACT_NONE>{}); break;
   }
+}
+
+// A wave's accumulators reach memory through LDS of its own: ROWS x COLS floats,
+// the four of quad c in row r at place c ^ (r mod COLS/4).  The blocks come a
+// few columns of many rows at a time; from LDS a row's lanes write whole cache
+// lines (and read the residual's).  Straight from the blocks, in 16-byte parts of
+// rows, the output's write took longer than half the product at 8192^3.
+template <int COLS>
+__device__ __forceinline__ uint32_t patch_at(int row, int quad) {
+  return row * (COLS * 4) + ((quad ^ (row & (COLS / 4 - 1))) << 4);
+}
+
+// (m0, n0): the patch's place in C.  (mt, nt): the workgroup's own first row and
+// column; where its tile was moved back into the matrix, what lies before them is
+// another's (eight columns across nt are written by both, with the same values).
+template <typename T, typename O, int ROWS, int COLS>
+__device__ __forceinline__ void write_patch(const GemmParams &p, int split, const lds_char *patch, int m0, int n0, int mt,
+                                            int nt) {
+  constexpr int LANES = COLS / 8, STEP = 64 / LANES;
+  const int lane = threadIdx.x % 64, n = n0 + lane % LANES * 8, left = p.n - n;
+  if (left <= 0 || n + 7 < nt) return;
+  const auto take = [&](int row, float (&v)[8]) {
 #pragma unroll
-  for (int j = 0; j < NI; ++j) {
-    const int n = n0 + j * 16 + lane / 16 * 4;
-    if (n >= p.n || n + 3 < nt) continue;
-    const f32x4 bias = bias4<O>(p, n);
-    f32x4 sb;
-    if constexpr (sizeof(T) == 1) sb = load4(p.sb + n, p.n - n);
+    for (int h = 0; h < 2; ++h) {
+      const f32x4 u = __builtin_bit_cast(f32x4, lds_read16(patch + patch_at<COLS>(row, lane % LANES * 2 + h)));
 #pragma unroll
-    for (int i = 0; i < MI; ++i) {
-      const int m = m0 + i * 16 + lane % 16;
+      for (int i = 0; i < 4; ++i) v[h * 4 + i] = u[i];
+    }
+  };
+  if (p.splits > 1) {  // one range of k of several: float sums, joined by gemm_join_kernel
+    const long ld = (p.n + 3) & ~3;
+    float *part = p.parts + split * (p.m * ld);
+    for (int row = lane / LANES; row < ROWS; row += STEP) {
+      const int m = m0 + row;
       if (m >= p.m || m < mt) continue;
-      f32x4 v = acc[i][j];
-      if constexpr (sizeof(T) == 1) v = v * sa[i] * sb;
-      finish4<O, ACT>(p, m, n, v, bias);
+      float v[8];
+      take(row, v);
+      store_some(part + m * ld + n, left, v);
     }
-  }
-}
-
-// One range of k of several: float partial sums, joined by gemm_join_kernel.
-template <int MI, int NI>
-__device__ __forceinline__ void store_part(const GemmParams &p, int split, int m0, int n0, f32x4 (&acc)[MI][NI]) {
-  const int lane = threadIdx.x % 64;
-  const long ld = (p.n + 3) & ~3;
-  float *part = p.parts + split * (p.m * ld);
-#pragma unroll
-  for (int j = 0; j < NI; ++j) {
-    const int n = n0 + j * 16 + lane / 16 * 4;
-#pragma unroll
-    for (int i = 0; i < MI; ++i) {
-      const int m = m0 + i * 16 + lane % 16;
-      if (m < p.m && n < p.n) *reinterpret_cast<f32x4 *>(part + m * ld + n) = acc[i][j];
-    }
-  }
-}
-
-template <typename T, typename O, int MI, int NI>
-__device__ __forceinline__ void write_tile(const GemmParams &p, int split, int m0, int n0, int mt, int nt, f32x4 (&acc)[MI][NI]) {
-  if (p.splits > 1) {
-    store_part(p, split, m0, n0, acc);
     return;
   }
-  switch (p.act) {
-    case ACT_RELU: finish_tile<T, O, MI, NI, ACT_RELU>(p, m0, n0, mt, nt, acc); break;
-    case ACT_GELU: finish_tile<T, O, MI, NI, ACT_GELU>(p, m0, n0, mt, nt, acc); break;
-    case ACT_SILU: finish_tile<T, O, MI, NI, ACT_SILU>(p, m0, n0, mt, nt, acc); break;
-    default: finish_tile<T, O, MI, NI, ACT_NONE>(p, m0, n0, mt, nt, acc); break;
-  }
+  float bias[8], sb[8];
+  load_bias<O>(p, n, bias);
+  if constexpr (sizeof(T) == 1) load_some(p.sb + n, left, sb);
+  with_act(p.act, [&](auto act) {
+#pragma unroll 4
+    for (int row = lane / LANES; row < ROWS; row += STEP) {
+      const int m = m0 + row;
+      if (m >= p.m || m < mt) continue;
+      float v[8];
+      take(row, v);
+      if constexpr (sizeof(T) == 1) {
+        const float sa = p.sa[m];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = v[i] * sa * sb[i];
+      }
+      finish<O, act()>(p, m, n, v, bias);
+    }
+  });
 }
 
 // ---- tile order ---------------------------------------------------------------
@@ -471,7 +488,24 @@ __global__ __launch_bounds__(64 * WM *WN) void gemm_tile_kernel(GemmParams p) {
       }
     }
   }
-  write_tile<T, O, MI, NI>(p, split, m0 + wm * (BM / WM), n0 + wn * (BN / WN), tm * BM, tn * BN, acc);
+  // The slabs' LDS is the patches' now: all waves have read theirs.
+  wait_lds();
+  barrier();
+  constexpr int COLS = BN / WN, ROWS = BM / WM / ((BM / WM) * COLS > 4096 ? 2 : 1);  // 16 KiB a wave at most
+  static_assert(NW * ROWS * COLS * 4 <= (DMA ? ST : 2) * STAGE, "the patches fit into the slabs' LDS");
+  lds_char *patch = lds + wave * (ROWS * COLS * 4);
+  const int lane = threadIdx.x % 64;
+#pragma unroll
+  for (int h = 0; h < BM / WM / ROWS; ++h) {
+#pragma unroll
+    for (int i = 0; i < ROWS / 16; ++i)
+#pragma unroll
+      for (int j = 0; j < NI; ++j)
+        *reinterpret_cast<__attribute__((address_space(3))) f32x4 *>(
+            patch + patch_at<COLS>(i * 16 + lane % 16, j * 4 + lane / 16)) = acc[h * (ROWS / 16) + i][j];
+    wait_lds();
+    write_patch<T, O, ROWS, COLS>(p, split, patch, m0 + wm * (BM / WM) + h * ROWS, n0 + wn * COLS, tm * BM, tn * BN);
+  }
 }
 
 // ---- few rows -----------------------------------------------------------------
@@ -608,14 +642,19 @@ __global__ __launch_bounds__(64 * rows_waves(BMN, MI)) void gemm_rows_kernel(Gem
   for (int w = 1; w < NW; ++w) v += join[(w * MI * NB + block) * 64 + lane];
   const int m = block / NB * 16 + l, n = n0 + block % NB * 16 + g * 4;
   if (m >= p.m || n >= p.n || n + 3 < nt) return;
-  if constexpr (sizeof(T) == 1) v = v * p.sa[m] * load4(p.sb + n, p.n - n);
-  const f32x4 bias = bias4<O>(p, n);
-  switch (p.act) {
-    case ACT_RELU: finish4<O, ACT_RELU>(p, m, n, v, bias); break;
-    case ACT_GELU: finish4<O, ACT_GELU>(p, m, n, v, bias); break;
-    case ACT_SILU: finish4<O, ACT_SILU>(p, m, n, v, bias); break;
-    default: finish4<O, ACT_NONE>(p, m, n, v, bias); break;
+  float out[4], bias[4];
+  load_bias<O>(p, n, bias);
+  if constexpr (sizeof(T) == 1) {
+    float sb[4];
+    load_some(p.sb + n, p.n - n, sb);
+    const float sa = p.sa[m];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) out[i] = v[i] * sa * sb[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) out[i] = v[i];
   }
+  with_act(p.act, [&](auto act) { finish<O, act()>(p, m, n, out, bias); });
 }
 
 }  // namespace tfnn

@@ -3,6 +3,7 @@
 #pragma once
 
 #include "nn_gemm.hpp"
+#include "nn_wide.hpp"
 
 namespace tfnn {
 
@@ -19,7 +20,7 @@ hipError_t launch_layout(const GemmParams &p, int tile, bool dma, hipStream_t st
   }
   const dim3 grid(static_cast<unsigned>(p.tiles_m) * p.tiles_n * p.splits);
   if (dma) {
-    if (tile == TILE_256) gemm_tile_kernel<T, O, AMN, BMN, 256, 256, 2, 4, 2, true><<<grid, 512, 0, stream>>>(p);
+    if (tile == TILE_256) gemm_wide_kernel<T, O, AMN, BMN><<<grid, 512, 0, stream>>>(p);
     else if (tile == TILE_128) gemm_tile_kernel<T, O, AMN, BMN, 128, 128, 2, 2, 2, true><<<grid, 256, 0, stream>>>(p);
     else if (grid.x <= 256) gemm_tile_kernel<T, O, AMN, BMN, 64, 64, 2, 2, 8, true><<<grid, 256, 0, stream>>>(p);
     else gemm_tile_kernel<T, O, AMN, BMN, 64, 64, 2, 2, 3, true><<<grid, 256, 0, stream>>>(p);

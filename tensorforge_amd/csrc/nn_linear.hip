@@ -14,10 +14,17 @@ __global__ __launch_bounds__(256) void gemm_join_kernel(GemmParams p) {
   const int m = static_cast<int>(id / (ld / 4)), n = static_cast<int>(id % (ld / 4)) * 4;
   if (m >= p.m) return;
   const float *part = p.parts + m * ld + n;
-  f32x4 v = *reinterpret_cast<const f32x4 *>(part);
-  for (int s = 1; s < p.splits; ++s) v += *reinterpret_cast<const f32x4 *>(part + s * (p.m * ld));
-  if (p.sa) v = v * p.sa[m] * load4(p.sb + n, p.n - n);
-  finish4<O, ACT>(p, m, n, v, bias4<O>(p, n));
+  f32x4 sum = *reinterpret_cast<const f32x4 *>(part);
+  for (int s = 1; s < p.splits; ++s) sum += *reinterpret_cast<const f32x4 *>(part + s * (p.m * ld));
+  float v[4] = {sum.x, sum.y, sum.z, sum.w}, bias[4];
+  if (p.sa) {
+    float sb[4];
+    load_some(p.sb + n, p.n - n, sb);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = v[i] * p.sa[m] * sb[i];
+  }
+  load_bias<O>(p, n, bias);
+  finish<O, ACT>(p, m, n, v, bias);
 }
 
 template <typename O>
@@ -45,23 +52,21 @@ __global__ __launch_bounds__(256) void act_slope_kernel(SlopeParams p) {
   if (left > 0) {
     for (int r = lane; r < kSlopeRows && row0 + r < p.m; r += 8) {
       const long row = row0 + r;
-      f32x4 g[2], z[2];
-#pragma unroll
-      for (int h = 0; h < 2; ++h) g[h] = load4(static_cast<const T *>(p.dy) + row * p.dy_ld + c + 4 * h, left - 4 * h);
+      float g[8], z[8];
+      load_some(static_cast<const T *>(p.dy) + row * p.dy_ld + c, left, g);
       if constexpr (ACT != ACT_NONE) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) z[h] = load4(static_cast<const T *>(p.z) + row * p.z_ld + c + 4 * h, left - 4 * h);
+        load_some(static_cast<const T *>(p.z) + row * p.z_ld + c, left, z);
         typename Vec<T, 8>::type out;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const float v = g[i / 4][i % 4] * act_slope<ACT>(z[i / 4][i % 4]);
+          const float v = g[i] * act_slope<ACT>(z[i]);
           sum[i] += v;
           out[i] = i < left ? static_cast<T>(v) : static_cast<T>(0.0f);
         }
         *reinterpret_cast<typename Vec<T, 8>::type *>(static_cast<T *>(p.dz) + row * p.dz_ld + c) = out;
       } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) sum[i] += g[i / 4][i % 4];
+        for (int i = 0; i < 8; ++i) sum[i] += g[i];
       }
     }
   }
