@@ -276,7 +276,7 @@ int tf_registry_entry(int i, int *family, int *cfg7, char *name, int name_cap);
 /* h = x + residual;  y = h / sqrt(mean(h^2) + eps) * weight, row by row, the norm
  * taken of the sum before h is rounded.  With y_type TF_T_F8 y is in 8 bits with
  * one scale a row: top = max(max|y|, 2^-100), scale = top/448, code = the value
- * nearest to y * (448/top) (ties to even).  A row that holds an infinity or a
+ * nearest to y * (448 * (1/top)) (ties to even).  A row that holds an infinity or a
  * NaN gives NaN. */
 typedef struct {
   const void *x, *residual; /* rows x d of `type`; residual may be NULL          */
@@ -329,7 +329,8 @@ typedef struct {
   void *out;            /* m x n of out_type                                        */
   void *z;              /* m x n of out_type: the pre-activation kept, or NULL      */
   void *workspace;      /* 16-byte aligned; with fewer bytes than tf_linear_workspace
-                           asks for (none: 0) the call runs unsplit along k         */
+                           asks for (none: 0) the call runs unsplit along k, without
+                           aligned copies                                           */
   long long workspace_bytes;
   long long x_ld, w_ld, residual_ld, out_ld, z_ld;
   long long m, n, k;
@@ -339,12 +340,13 @@ typedef struct {
   int bias_type; /* out_type or TF_T_F32                                             */
   int act;       /* TF_ACT_*                                                         */
   int tile;      /* C tile: 0 by the sizes, 1: 256x256, 2: 128x128, 3: 64x64, 4: all of
-                    up to 64 rows, k split over a workgroup's waves; one that cannot
-                    run these operands gives way to the choice by sizes              */
+                    up to 64 rows, k split over a workgroup's waves, 5: 64x128; one that
+                    cannot run these operands gives way to the choice by sizes       */
   int splits;    /* ranges of k: 0 by the sizes, or 1..64                            */
   int reserved;  /* 0                                                                */
 } tf_linear_args_t;
-/* Bytes of workspace for these sizes and types (pointers are not looked at). */
+/* Bytes of workspace for these arguments: sizes, types, distances and the
+ * alignment of x and w count, the memory is not touched. */
 int tf_linear_workspace(const tf_linear_args_t *args, long long *bytes);
 int tf_linear(const tf_linear_args_t *args, void *stream);
 
@@ -366,6 +368,7 @@ typedef struct {
   int act;
   int tile, splits; /* both products', as tf_linear's                                */
 } tf_linear_grad_args_t;
+/* As tf_linear_workspace; which of dx, dw and dbias are wanted counts too. */
 int tf_linear_grad_workspace(const tf_linear_grad_args_t *args, long long *bytes);
 int tf_linear_grad(const tf_linear_grad_args_t *args, void *stream);
 

@@ -2,6 +2,7 @@
 // include/tforge_hip.h): checks of arguments, the choice of tile and of ranges
 // of k, and the order of launches.
 #include <algorithm>
+#include <cmath>
 #include <cstdint>
 #include <string>
 
@@ -108,8 +109,6 @@ int quantize_rows(const void *x, long long x_ld, long long rows, long long d, in
   return hip(launch_rms_norm(p, type, true, stream), call);
 }
 
-long long round16(long long bytes) { return (bytes + 15) & ~15LL; }
-
 int rms_norm_grad(const tf_rms_norm_grad_args_t *a, hipStream_t stream) {
   const char *call = "tf_rms_norm_grad";
   if (!a) return fail(TF_E_ARG, "tf_rms_norm_grad: null arguments");
@@ -138,87 +137,185 @@ int rms_norm_grad(const tf_rms_norm_grad_args_t *a, hipStream_t stream) {
 
 // ---- products -------------------------------------------------------------------
 
-// A product's operands as the kernels see them.
-struct Product {
-  int type, out_type;
-  bool amn, bmn;
-  GemmParams p;
+// One operand as the kernels see it: `lines` lines of `length` contiguous
+// elements; mn: lines of its own dimension, not of k.  ours: in the workspace,
+// aligned, whole pieces a line, zeros in the pad.
+struct Operand {
+  const void *p = nullptr;
+  long ld = 0, lines = 0, length = 0;
+  bool mn = false, ours = false;
 };
 
-// Whether the loads may go straight into LDS: 16-byte aligned rows of whole
-// pieces, and every offset inside a tile's slab below 2^31 bytes.
-bool direct_loads(const void *base, long ld, bool mn, int own, int k, int size) {
-  const int piece = 16 / size;
-  const long span = mn ? 64 * ld * size + 1024 : 256 * ld * size + 256;
-  return reinterpret_cast<uintptr_t>(base) % 16 == 0 && ld % piece == 0 && (mn ? own : k) % piece == 0 && span < (1L << 31);
-}
-
-struct Plan {
-  int tile, splits;
+struct Product {
+  int type, out_type;
+  Operand a, b;
+  GemmParams p;  // sizes, output and epilogue
 };
 
 long ceil_div(long a, long b) { return (a + b - 1) / b; }
+long long round16(long long bytes) { return (bytes + 15) & ~15LL; }
 
-// The C tile and the ranges of k for a product of these sizes.
-//
-// Up to 64 rows a workgroup's time is what it reads, at about 35 bytes a
-// nanosecond (what a CU's misses to L2 and beyond sustain): for the few-row
-// kernel its columns' and all rows' whole k, for the 64 x 64 tile its range of
-// k, and 3.3 us for the join where k is split.  The smaller estimate runs.
-// Measured, bfloat16, us (few-row / tile), w 4096 x 4096 as n rows of k: 7.7 / 10.8
-// for 1 row, 9.8 / 11.1 for 16, 13.7 / 11.6 for 32; as k rows of n: 11.4 / 11.6, 13.4 /
-// 12.2, 16.1 / 12.5; 8192 deep and 2048 wide: 11.3 / 12.0 for 1 row, 16.6 / 12.2 for 16.
+// Whether an operand's loads may go straight into LDS: 16-byte aligned lines of
+// whole pieces, and every offset inside a tile's slab below 2^31 bytes.
+bool direct_loads(const Operand &o, int size) {
+  const int piece = 16 / size;
+  const long span = o.mn ? 64 * o.ld * size + 1024 : 256 * o.ld * size + 256;
+  if (span >= (1L << 31)) return false;
+  return o.ours || (reinterpret_cast<uintptr_t>(o.p) % 16 == 0 && o.ld % piece == 0 && o.length % piece == 0);
+}
+
+// The same operand copied to aligned lines: whole cache lines, so that no 128 bytes
+// of a tile's line lie in two.
+long packed_ld(const Operand &o, int size) { return ceil_div(o.length, 128 / size) * (128 / size); }
+long long packed_bytes(const Operand &o, int size) { return round16(o.lines * packed_ld(o, size) * size); }
+
+struct Plan {
+  int tile, splits;
+  double us;  // predicted
+};
+
+// Predicted time (us) of a product on one tile with k in `splits` ranges: start,
+// slabs (64 elements of k in 16 bits, 128 in 8) or the operands' bytes at 8 TB/s
+// (`read`, us), join.  Fitted on MI355X, the same
+// for all types in slabs: a slab takes a 64 x 64 tile 0.29 us alone on its CU, 0.38
+// for two and 0.17 for each of more, a 64 x 128 one 0.41 alone and 0.6 for two, a 128 x
+// 128 one 0.6 and 0.91, a 256 x
+// 256 one 1.1 (few CUs busy) to 1.48 (all, at the power limit).  Loads through
+// registers (64 x 64 tiles only) take 2.2 times that, 3.2 with an operand not along k.  Both sides of the choices (us, bfloat16):
+// 512 x 4096 x 4096 64/128/256-tile 28.4 / 44.3 / 80.6, 2048 x 4096 x 4096 101 / 62.8 /
+// 84, 4096^3 190 / 122 / 105; split 1/2/4 ways 256 x 4096 x 4096 64-tile 23.6 / 21.0 / 24.4,
+// 2048 x 2048 x 8192 128-tile 88.6 / 72.7 / -, 96 x 2048 x 8192 64-tile 41.6 / 25.5 / 17.5
+// (8: 15.6).
+double predicted(double m, double n, double slabs, double read, double loads, int tile, int splits) {
+  const double each = std::ceil(slabs / splits);
+  const double w = std::ceil(m / tile_rows(tile)) * std::ceil(n / tile_columns(tile)) * splits / 256;  // workgroups a CU
+  double start, slab;
+  if (tile == TILE_64) {
+    start = 4.3;
+    slab = w <= 1 ? 0.29 : std::max(0.38, 0.17 * w);
+  } else if (tile != TILE_256) {
+    const double one = tile == TILE_128 ? 0.6 : 0.41, two = tile == TILE_128 ? 0.91 : 0.6;
+    const double pairs = std::floor(w / 2), rest = w - 2 * pairs;
+    start = 4.6 + 2 * std::max(0.0, std::ceil(w / 2) - 1);
+    slab = two * pairs + (rest == 0 ? 0 : rest <= 1 ? one : two);
+  } else {
+    const double rounds = std::ceil(w);
+    start = 10 * rounds;
+    slab = 1.48 * (rounds - 1) + 1.1 + 0.38 * (w - (rounds - 1));
+  }
+  return start + std::max(each * slab * loads, read) + (splits > 1 ? 3.3 + 8 * splits * m * n / 7e6 : 0);
+}
+
+// The C tile and the ranges of k for a product of these sizes: the least
+// predicted time.  Up to 64 rows the few-row kernel stands beside the tiles; its
+// workgroups read their columns' and all rows' whole k at about 40 bytes a
+// nanosecond (what a CU's misses to L2 and beyond sustain).  Measured, bfloat16, us
+// (few-row / 64-tile), w 4096 x 4096 as n rows of k: 7.7 / 10.8 for 1 row, 9.8 / 11.1
+// for 16, 13.7 / 11.6 for 32; as k rows of n: 11.4 / 11.6, 13.4 / 12.2, 16.1 / 12.5.
 Plan plan_product(long m, long n, long k, int type, bool amn, bool bmn, bool dma, int tile, int splits) {
   const int size = size_of(type);
   const long slabs = ceil_div(k, 128 / size);
   const bool rows = m <= 64 && !amn && (!bmn || n >= 32);
-  const auto split = [&](int t) {
-    const long tiles = ceil_div(m, tile_size(t)) * ceil_div(n, tile_size(t));
-    const long s = splits ? splits : std::min<long>({256 / std::max<long>(1, tiles), slabs / 4, 16});
-    return static_cast<int>(std::max<long>(1, std::min(s, slabs)));
-  };
+  if (tile == TILE_ROWS && rows) return {TILE_ROWS, 1, 0};
+  if (tile == TILE_ROWS || (!dma && tile != TILE_64)) tile = 0;
+  splits = static_cast<int>(std::max<long>(0, std::min<long>(splits, std::max<long>(1, slabs))));
+  Plan best{TILE_64, 1, 1e30};
+  const double loads = dma ? 1 : amn || bmn ? 3.2 : 2.2;
+  const double read = (static_cast<double>(m) + n) * k * size / 8e6;
   if (rows && !tile) {
-    const long cols = bmn ? 32 : 16, s = split(TILE_64);
-    const long few = ceil_div(ceil_div(n, cols), 256) * (cols + m) * k * size / 36;
-    const long many = ceil_div(ceil_div(n, 64) * s, 256) * (64 + m) * (k / s) * size / 33 * (dma ? 1 : 2) + (s > 1 ? 3300 : 0);
-    tile = few <= many ? TILE_ROWS : TILE_64;
+    const long cols = bmn ? 32 : 16;
+    best = {TILE_ROWS, 1, 3.1 + std::max(read, ceil_div(ceil_div(n, cols), 256) * static_cast<double>(cols + m) * k * size / 40e3)};
   }
-  if (tile == TILE_ROWS && rows) return {TILE_ROWS, 1};
-  if (!tile || tile == TILE_ROWS) tile = m <= 64 || n <= 64 || ceil_div(m, 128) * ceil_div(n, 128) < 128 ? TILE_64
-                    : dma && ceil_div(m, 256) * ceil_div(n, 256) >= 192            ? TILE_256
-                                                                                   : TILE_128;
-  if (!dma && tile == TILE_256) tile = TILE_128;
-  return {tile, split(tile)};
+  for (int t : {TILE_64, TILE_64x128, TILE_128, TILE_256}) {
+    if (tile ? t != tile : t != TILE_64 && !dma) continue;
+    for (int s : {1, 2, 3, 4, 6, 8, 12, 16}) {
+      if (splits ? s != 1 : s > 1 && s * 2 > slabs) continue;
+      const int ranges = splits ? splits : s;
+      const double us = predicted(m, n, slabs, read, loads, t, ranges);
+      if (us < best.us) best = {t, ranges, us};
+    }
+  }
+  return best;
 }
 
 long long part_bytes(long m, long n, const Plan &plan) {
   return plan.splits > 1 ? round16(4LL * plan.splits * m * ((n + 3) & ~3L)) : 0;
 }
 
-// The workspace that serves this product whatever the alignment of its operands.
-long long product_bytes(long m, long n, long k, int type, bool amn, bool bmn, int tile, int splits) {
-  return std::max(part_bytes(m, n, plan_product(m, n, k, type, amn, bmn, true, tile, splits)),
-                  part_bytes(m, n, plan_product(m, n, k, type, amn, bmn, false, tile, splits)));
+// How a product runs.  Operands that cannot be loaded straight into LDS are
+// copied to aligned lines first (pack) where the faster kernels gain more than the
+// copy takes, about 4 us and its bytes at 4 TB/s: 4095 x 4097 x 1023 bfloat16 110 us
+// through registers, NNN with both copied; 777 x 1111 x 333 8.2 and NNN.
+struct Choice {
+  Plan plan;
+  bool dma = false, pack_a = false, pack_b = false;
+  long long parts = 0, copies = 0;
+  long long bytes() const { return parts + copies; }
+};
+
+Choice choose(const Product &q, int tile, int splits, bool packing = true) {
+  const GemmParams &p = q.p;
+  const int size = size_of(q.type);
+  Choice c;
+  const bool da = direct_loads(q.a, size), db = direct_loads(q.b, size);
+  c.dma = da && db;
+  c.plan = plan_product(p.m, p.n, p.k, q.type, q.a.mn, q.b.mn, c.dma, tile, splits);
+  if (!c.dma && packing && p.k > 0 && c.plan.tile != TILE_ROWS) {
+    const long long copies = (da ? 0 : packed_bytes(q.a, size)) + (db ? 0 : packed_bytes(q.b, size));
+    const auto fits = [&](const Operand &o) { return 256 * packed_ld(o, size) * size + 1024 < (1L << 31); };
+    const Plan fast = plan_product(p.m, p.n, p.k, q.type, q.a.mn, q.b.mn, true, tile, splits);
+    if (fits(q.a) && fits(q.b) && ((tile && tile != TILE_64 && tile != TILE_ROWS) || fast.us + 4 + 2 * copies / 4e6 < c.plan.us)) {
+      c.plan = fast;
+      c.dma = true;
+      c.pack_a = !da;
+      c.pack_b = !db;
+      c.copies = copies;
+    }
+  }
+  c.parts = part_bytes(p.m, p.n, c.plan);
+  return c;
+}
+
+// Fills in the kernels' view of a product that runs on this plan.
+void place(Product &q, const Plan &plan, void *parts) {
+  GemmParams &p = q.p;
+  p.a = q.a.p, p.lda = q.a.ld, p.b = q.b.p, p.ldb = q.b.ld;
+  p.tiles_m = static_cast<int>(ceil_div(p.m, tile_rows(plan.tile)));
+  p.tiles_n = static_cast<int>(ceil_div(p.n, tile_columns(plan.tile)));
+  p.splits = plan.splits;
+  p.parts = static_cast<float *>(parts);
 }
 
 hipError_t run_product(Product &q, int tile, int splits, void *workspace, long long bytes, hipStream_t stream) {
-  GemmParams &p = q.p;
   const int size = size_of(q.type);
-  const bool dma = direct_loads(p.a, p.lda, q.amn, p.m, p.k, size) && direct_loads(p.b, p.ldb, q.bmn, p.n, p.k, size);
-  Plan plan = plan_product(p.m, p.n, p.k, q.type, q.amn, q.bmn, dma, tile, splits);
-  if (part_bytes(p.m, p.n, plan) > bytes) plan = plan_product(p.m, p.n, p.k, q.type, q.amn, q.bmn, dma, tile, 1);
-  p.tiles_m = static_cast<int>(ceil_div(p.m, tile_size(plan.tile)));
-  p.tiles_n = static_cast<int>(ceil_div(p.n, tile_size(plan.tile)));
-  p.splits = plan.splits;
-  p.parts = static_cast<float *>(workspace);
-  const hipError_t e = q.type == TF_T_BF16  ? launch_gemm_bf16(p, q.amn, q.bmn, plan.tile, dma, stream)
-                       : q.type == TF_T_F16 ? launch_gemm_f16(p, q.amn, q.bmn, plan.tile, dma, stream)
-                                            : launch_gemm_f8(p, q.out_type, plan.tile, dma, stream);
-  return e == hipSuccess && plan.splits > 1 ? launch_gemm_join(p, q.out_type, stream) : e;
+  Choice c = choose(q, tile, splits);
+  if (c.bytes() > bytes) c = choose(q, tile, 1, false);
+  hipError_t e = hipSuccess;
+  if (c.pack_a || c.pack_b) {
+    char *to = static_cast<char *>(workspace) + c.parts;
+    PackParams pack{};
+    int i = 0;
+    for (Operand *o : {&q.a, &q.b}) {
+      if (!(o == &q.a ? c.pack_a : c.pack_b)) continue;
+      const long ld = packed_ld(*o, size);
+      pack.from[i] = o->p, pack.from_ld[i] = o->ld, pack.rows[i] = o->lines, pack.columns[i] = static_cast<int>(o->length);
+      pack.to[i] = to, pack.to_ld[i] = ld, pack.pieces[i] = o->lines * ld * size / 16;
+      to += packed_bytes(*o, size);
+      o->p = pack.to[i], o->ld = ld, o->ours = true;
+      ++i;
+    }
+    e = launch_pack(pack, size, stream);
+    if (e != hipSuccess) return e;
+  }
+  place(q, c.plan, workspace);
+  e = q.type == TF_T_BF16  ? launch_gemm_bf16(q.p, q.a.mn, q.b.mn, c.plan.tile, c.dma, stream)
+      : q.type == TF_T_F16 ? launch_gemm_f16(q.p, q.a.mn, q.b.mn, c.plan.tile, c.dma, stream)
+                           : launch_gemm_f8(q.p, q.out_type, c.plan.tile, c.dma, stream);
+  return e == hipSuccess && c.plan.splits > 1 ? launch_gemm_join(q.p, q.out_type, stream) : e;
 }
 
 void check_choice(Checks &c, int tile, int splits) {
-  c.one_of("tile", tile, {0, TILE_256, TILE_128, TILE_64, TILE_ROWS});
+  c.one_of("tile", tile, {0, TILE_256, TILE_128, TILE_64, TILE_ROWS, TILE_64x128});
   c.need(splits >= 0 && splits <= 64, "splits = ", static_cast<long long>(splits), " is not between 0 and 64");
 }
 
@@ -232,12 +329,24 @@ void check_linear_sizes(Checks &c, const tf_linear_args_t *a) {
   check_choice(c, a->tile, a->splits);
 }
 
+Product product_of(const tf_linear_args_t *a) {
+  Product q{a->type, a->out_type, {}, {}, {}};
+  q.a = {a->x, a->x_ld, a->m, a->k, false, false};
+  q.b = a->w_order ? Operand{a->w, a->w_ld, a->n, a->k, false, false} : Operand{a->w, a->w_ld, a->k, a->n, true, false};
+  GemmParams &p = q.p;
+  p.bias = a->bias, p.residual = a->residual, p.sa = a->x_scale, p.sb = a->w_scale, p.out = a->out, p.z = a->z;
+  p.ldr = a->residual_ld, p.ldo = a->out_ld, p.ldz = a->z_ld;
+  p.m = static_cast<int>(a->m), p.n = static_cast<int>(a->n), p.k = static_cast<int>(a->k);
+  p.act = a->act, p.bias_f32 = a->bias_type == TF_T_F32;
+  return q;
+}
+
 int linear_workspace(const tf_linear_args_t *a, long long *bytes) {
   if (!a || !bytes) return fail(TF_E_ARG, "tf_linear_workspace: null arguments");
   Checks c{"tf_linear_workspace", {}};
   check_linear_sizes(c, a);
   if (!c.fine()) return fail(TF_E_ARG, c.wrong);
-  *bytes = a->m && a->n ? product_bytes(a->m, a->n, a->k, a->type, false, a->w_order == 0, a->tile, a->splits) : 0;
+  *bytes = a->m && a->n ? choose(product_of(a), a->tile, a->splits).bytes() : 0;
   return TF_OK;
 }
 
@@ -264,33 +373,66 @@ int linear(const tf_linear_args_t *a, hipStream_t stream) {
   if (a->workspace_bytes) c.workspace(a->workspace, a->workspace_bytes, 1);
   if (!c.fine()) return fail(TF_E_ARG, c.wrong);
   if (a->m == 0 || a->n == 0) return TF_OK;
-  Product q{a->type, a->out_type, false, a->w_order == 0, {}};
-  GemmParams &p = q.p;
-  p.a = a->x, p.b = a->w, p.bias = a->bias, p.residual = a->residual, p.sa = a->x_scale, p.sb = a->w_scale;
-  p.out = a->out, p.z = a->z, p.lda = a->x_ld, p.ldb = a->w_ld, p.ldr = a->residual_ld, p.ldo = a->out_ld, p.ldz = a->z_ld;
-  p.m = static_cast<int>(a->m), p.n = static_cast<int>(a->n), p.k = static_cast<int>(a->k);
-  p.act = a->act, p.bias_f32 = a->bias_type == TF_T_F32;
+  Product q = product_of(a);
   return hip(run_product(q, a->tile, a->splits, a->workspace, a->workspace_bytes, stream), call);
 }
 
-// The gradient's workspace: dz, its column sums' shares, then one product's parts.
-struct GradSpace {
-  long long dz = 0, shares = 0, parts = 0, dz_ld = 0;
-  long long bytes() const { return dz + shares + parts; }
+// How a gradient runs: the workspace's parts and the products.
+struct GradPlan {
+  bool own_dz = false;   // dz lies in the workspace: an activation's, or an aligned copy of dy
+  bool pair = false;     // both products in one launch
+  int terms = 1;         // of dz
+  long dz_ld = 0;
+  long long dz = 0, shares = 0, product = 0;  // bytes
+  Product dx, dw;
+  long long bytes() const { return dz + shares + product; }
 };
 
-GradSpace grad_space(const tf_linear_grad_args_t *a) {
-  GradSpace s;
-  if (a->m == 0 || a->n == 0) return s;
-  s.dz_ld = (a->n + 7) & ~7LL;
-  if (a->act != TF_ACT_NONE) s.dz = round16(2 * a->m * s.dz_ld);
-  s.shares = round16(4 * column_shares(a->m) * a->n);
-  if (a->k) {
-    s.parts = product_bytes(a->m, a->k, a->n, a->type, false, a->w_order == 1, a->tile, a->splits);
-    s.parts = std::max(s.parts, a->w_order ? product_bytes(a->n, a->k, a->m, a->type, true, true, a->tile, a->splits)
-                                           : product_bytes(a->k, a->n, a->m, a->type, true, true, a->tile, a->splits));
+// Up to this many multiply-adds a product of the rounded dz is not taken alone:
+// what the rounding left goes in as a second term, into the same float sums.  A
+// small gradient then errs by its own rounding only; larger ones, where a second
+// product would show in the time, by sqrt(2) of it.
+constexpr double kTwoTerms = 1.4e8;
+
+GradPlan plan_grad(const tf_linear_grad_args_t *a) {
+  GradPlan g{};
+  const int m = static_cast<int>(a->m), n = static_cast<int>(a->n), k = static_cast<int>(a->k);
+  if (n == 0) return g;
+  const double work = static_cast<double>(m) * n * k;
+  const bool smooth = a->act == TF_ACT_GELU || a->act == TF_ACT_SILU;
+  g.dz_ld = n <= 64 ? ceil_div(n, 8) * 8 : ceil_div(n, 64) * 64;
+  const Operand dy{a->dy, a->dy_ld, m, n, false, false};
+  g.own_dz = m && (a->act != TF_ACT_NONE || (!direct_loads(dy, 2) && m > 64 && work > 1e6));
+  g.terms = smooth && work <= kTwoTerms ? 2 : 1;
+  if (g.own_dz) g.dz = round16(2 * a->m * g.dz_ld) * g.terms;
+  if (a->dbias && m && column_shares(m) > 1) g.shares = round16(4 * column_shares(m) * a->n);
+  if (k == 0) return g;
+  const bool nk = a->w_order == 1;
+  const auto dz = [&](bool mn) {
+    return g.own_dz ? Operand{nullptr, g.dz_ld, m, n, mn, true} : Operand{a->dy, a->dy_ld, m, n, mn, false};
+  };
+  g.dx = {a->type, a->type, dz(false), nk ? Operand{a->w, a->w_ld, n, k, true, false} : Operand{a->w, a->w_ld, k, n, false, false}, {}};
+  g.dx.p.m = m, g.dx.p.n = k, g.dx.p.k = n, g.dx.p.out = a->dx, g.dx.p.ldo = a->dx_ld;
+  const Operand x{a->x, a->x_ld, m, k, true, false};
+  g.dw = {a->type, a->type, nk ? dz(true) : x, nk ? x : dz(true), {}};
+  g.dw.p.m = nk ? n : k, g.dw.p.n = nk ? k : n, g.dw.p.k = m, g.dw.p.out = a->dw, g.dw.p.ldo = a->dw_ld;
+  if (g.terms == 2) {
+    g.dx.p.terms = g.dw.p.terms = 2;
+    g.dx.p.a_term = (nk ? g.dw.p.a_term : g.dw.p.b_term) = g.dz / 2;
   }
-  return s;
+  const bool free = !a->tile && !a->splits;
+  // One launch for both where neither fills the GPU and k is short on both sides.
+  if (free && a->dx && a->dw && m && direct_loads(g.dx.a, 2) && direct_loads(g.dx.b, 2) && direct_loads(g.dw.a, 2) &&
+      direct_loads(g.dw.b, 2)) {
+    const long tiles = ceil_div(m, 64) * ceil_div(k, 64) + ceil_div(g.dw.p.m, 64) * ceil_div(g.dw.p.n, 64);
+    g.pair = tiles <= 512 && m <= 512 && n <= 512;
+  }
+  if (g.pair) return g;
+  // Two terms run on the tiles that know them.
+  const int tile = g.terms == 2 ? (a->tile == TILE_128 ? TILE_128 : TILE_64) : a->tile;
+  if (a->dx && m) g.product = choose(g.dx, tile, a->splits).bytes();
+  if (a->dw) g.product = std::max(g.product, choose(g.dw, tile, a->splits).bytes());
+  return g;
 }
 
 void check_grad_sizes(Checks &c, const tf_linear_grad_args_t *a) {
@@ -308,7 +450,7 @@ int linear_grad_workspace(const tf_linear_grad_args_t *a, long long *bytes) {
   Checks c{"tf_linear_grad_workspace", {}};
   check_grad_sizes(c, a);
   if (!c.fine()) return fail(TF_E_ARG, c.wrong);
-  *bytes = grad_space(a).bytes();
+  *bytes = plan_grad(a).bytes();
   return TF_OK;
 }
 
@@ -327,43 +469,44 @@ int linear_grad(const tf_linear_grad_args_t *a, hipStream_t stream) {
   c.matrix("dw", a->dw, a->dw_ld, wr, wc, a->type, false);
   c.vector("dbias", a->dbias, a->n, a->bias_type, false);
   if (!c.fine()) return fail(TF_E_ARG, c.wrong);
-  const GradSpace space = grad_space(a);
-  c.workspace(a->workspace, a->workspace_bytes, space.bytes());
+  GradPlan g = plan_grad(a);
+  c.workspace(a->workspace, a->workspace_bytes, g.bytes());
   if (!c.fine()) return fail(TF_E_ARG, c.wrong);
 
   char *ws = static_cast<char *>(a->workspace);
+  float *shares = reinterpret_cast<float *>(ws + g.dz);
+  void *rest = ws + g.dz + g.shares;
   const int m = static_cast<int>(a->m), n = static_cast<int>(a->n), k = static_cast<int>(a->k);
-  const void *dz = a->dy;
-  long dz_ld = a->dy_ld;
   hipError_t e = hipSuccess;
-  if (m && n && (a->act != TF_ACT_NONE || a->dbias)) {
-    SlopeParams s{a->dy, a->z, nullptr, a->dbias ? reinterpret_cast<float *>(ws + space.dz) : nullptr, a->dy_ld, a->z_ld,
-                  space.dz_ld, m, n, a->act};
-    if (a->act != TF_ACT_NONE) {
-      dz = s.dz = ws;
-      dz_ld = space.dz_ld;
-    }
+  if (m && n && (g.own_dz || a->dbias)) {
+    SlopeParams s{};
+    s.dy = a->dy, s.z = a->z, s.dy_ld = a->dy_ld, s.z_ld = a->z_ld, s.m = m, s.n = n, s.act = a->act;
+    if (g.own_dz) s.dz = ws, s.dz_ld = g.dz_ld, s.lo = g.terms == 2 ? g.dz / 4 : 0;
+    if (a->dbias && g.shares) s.shares = shares;
+    if (a->dbias && !g.shares) s.sums = a->dbias, s.sums_type = a->bias_type;
     e = launch_act_slope(s, a->type, stream);
   }
-  if (e == hipSuccess && a->dbias && n)
-    e = launch_share_sum(reinterpret_cast<float *>(ws + space.dz), m ? column_shares(m) : 0, n, a->dbias, a->bias_type, stream);
-  void *parts = ws + space.dz + space.shares;
-  if (e == hipSuccess && a->dx && m && k) {
-    Product q{a->type, a->type, false, a->w_order == 1, {}};
-    GemmParams &p = q.p;
-    p.a = dz, p.lda = dz_ld, p.b = a->w, p.ldb = a->w_ld, p.out = a->dx, p.ldo = a->dx_ld;
-    p.m = m, p.n = k, p.k = n;
-    e = run_product(q, a->tile, a->splits, parts, space.parts, stream);
+  if (e == hipSuccess && a->dbias && n && (g.shares || !m))
+    e = launch_share_sum(shares, m ? column_shares(m) : 0, n, a->dbias, a->bias_type, stream);
+  if (e != hipSuccess || !k) return hip(e, call);
+  if (g.own_dz) g.dx.a.p = (a->w_order ? g.dw.a.p : g.dw.b.p) = ws;
+  if (g.pair) {
+    place(g.dx, {TILE_64, 1, 0}, nullptr);
+    place(g.dw, {TILE_64, 1, 0}, nullptr);
+    return hip(a->type == TF_T_BF16 ? launch_gemm_pair_bf16(g.dx.p, g.dx.b.mn, g.dw.p, stream)
+                                    : launch_gemm_pair_f16(g.dx.p, g.dx.b.mn, g.dw.p, stream), call);
   }
-  if (e == hipSuccess && a->dw && n && k) {
-    Product q{a->type, a->type, true, true, {}};
-    GemmParams &p = q.p;
-    const bool nk = a->w_order == 1;
-    p.a = nk ? dz : a->x, p.lda = nk ? dz_ld : a->x_ld, p.b = nk ? a->x : dz, p.ldb = nk ? a->x_ld : dz_ld;
-    p.out = a->dw, p.ldo = a->dw_ld;
-    p.m = nk ? n : k, p.n = nk ? k : n, p.k = m;
-    e = run_product(q, a->tile, a->splits, parts, space.parts, stream);
+  const int tile = g.terms == 2 ? (a->tile == TILE_128 ? TILE_128 : TILE_64) : a->tile;
+  if (a->dx && m) {
+    if (n) {
+      e = run_product(g.dx, tile, a->splits, rest, g.product, stream);
+    } else {  // a sum of nothing
+      Product q{a->type, a->type, {}, {}, {}};
+      q.p.m = m, q.p.n = k, q.p.out = a->dx, q.p.ldo = a->dx_ld;
+      e = run_product(q, 0, 1, nullptr, 0, stream);
+    }
   }
+  if (e == hipSuccess && a->dw && n) e = run_product(g.dw, tile, a->splits, rest, g.product, stream);
   return hip(e, call);
 }
 

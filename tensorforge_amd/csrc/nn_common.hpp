@@ -74,11 +74,11 @@ template <int ACT>
 __device__ __forceinline__ float act_value(float z) {
   if constexpr (ACT == ACT_RELU) return (z > 0.0f || z != z) ? z : 0.0f;  // NaN stays, -0 becomes +0
   if constexpr (ACT == ACT_GELU) {
-    // z*Phi(z): Phi is the tail itself on the left, 1 - tail on the right.
+    // z*Phi(z) = max(z, 0) - |z|*tail, which is exact where the tail is 0 (the
+    // bound keeps infinity * 0 out) and stays NaN through the tail.
     float e;
     const float q = normal_tail(z, e);
-    const float v = z * (z > 0.0f ? 1.0f - q : q);
-    return z == -__builtin_inff() ? -0.0f : v;  // the limit; -inf * 0 would be NaN
+    return __builtin_fmaf(-__builtin_fminf(__builtin_fabsf(z), 1e30f), q, __builtin_fmaxf(z, 0.0f));
   }
   if constexpr (ACT == ACT_SILU) return z == -__builtin_inff() ? -0.0f : z * sigmoid(z);
   return z;

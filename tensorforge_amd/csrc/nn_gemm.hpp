@@ -361,8 +361,8 @@ __device__ __forceinline__ void write_patch(const GemmParams &p, int split, cons
 // Workgroups are dealt to the 8 XCDs in turn; each XCD gets one run of
 // consecutive tiles, walked in bands of 8 tile rows, so that its L2 holds the
 // rows and columns it shares.
-__device__ __forceinline__ void tile_of(const GemmParams &p, int &tm, int &tn, int &split) {
-  const int total = gridDim.x, id = blockIdx.x, xcd = id & 7, per = total >> 3, more = total & 7;
+__device__ __forceinline__ void tile_of(const GemmParams &p, int id, int total, int &tm, int &tn, int &split) {
+  const int xcd = id & 7, per = total >> 3, more = total & 7;
   int t = xcd * per + min(xcd, more) + (id >> 3);
   const int tiles = p.tiles_m * p.tiles_n;
   split = t / tiles;
@@ -378,10 +378,14 @@ template <int N>
 __device__ __forceinline__ void wait_loads() {
   asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
+// A workgroup's barrier for LDS: what was written before it is read behind it.
+// (Loads and stores of memory are not waited for.)
 __device__ __forceinline__ void barrier() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
   asm volatile("" ::: "memory");
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
 }
 
 // ---- the tile kernel ----------------------------------------------------------
@@ -389,14 +393,19 @@ __device__ __forceinline__ void barrier() {
 // BM x BN of C a workgroup, WM x WN waves, ST slabs of LDS.  One barrier a slab:
 // behind it slab s has arrived for all waves and slab s-1 is used up, so slab
 // s+ST-1 may take its place while s is multiplied.
+//
+// Of `blocks` workgroups this is number `block`.  An operand of two terms (a value
+// and what its rounding left) is multiplied term after term into the same sums.
+template <int BM, int BN, int ST>
+constexpr int tile_lds() {
+  return ST * (BM + BN) * 128;
+}
 template <typename T, typename O, bool AMN, bool BMN, int BM, int BN, int WM, int WN, int ST, bool DMA>
-__global__ __launch_bounds__(64 * WM *WN) void gemm_tile_kernel(GemmParams p) {
+__device__ __forceinline__ void gemm_tile(const GemmParams &p, int block, int blocks, lds_char *lds) {
   constexpr int NW = WM * WN, MI = BM / WM / 16, NI = BN / WN / 16, STAGE = (BM + BN) * 128;
-  __shared__ __align__(1024) char smem[ST * STAGE];
-  lds_char *lds = (lds_char *)smem;
   const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(lds));
   int tm, tn, split;
-  tile_of(p, tm, tn, split);
+  tile_of(p, block, blocks, tm, tn, split);
   const int slabs = (p.k + kSlab<T> - 1) / kSlab<T>;
   const int s0 = static_cast<int>(static_cast<long>(slabs) * split / p.splits);
   const int count = static_cast<int>(static_cast<long>(slabs) * (split + 1) / p.splits) - s0;
@@ -405,8 +414,6 @@ __global__ __launch_bounds__(64 * WM *WN) void gemm_tile_kernel(GemmParams p) {
   SlabLoader<T, BMN, BN, NW, DMA> lb;
   // Loads through registers: a tile that would reach past the matrix's end starts earlier.
   const int m0 = DMA ? tm * BM : max(0, min(tm * BM, p.m - BM)), n0 = DMA ? tn * BN : max(0, min(tn * BN, p.n - BN));
-  la.init(p.a, p.lda, p.m, m0, k0, p.k);
-  lb.init(p.b, p.ldb, p.n, n0, k0, p.k);
   constexpr int LOADS = decltype(la)::PER_WAVE + decltype(lb)::PER_WAVE;
 
   const int wave = threadIdx.x / 64, wm = wave / WN, wn = wave % WN;
@@ -436,61 +443,65 @@ __global__ __launch_bounds__(64 * WM *WN) void gemm_tile_kernel(GemmParams p) {
       for (int j = 0; j < NI; ++j) acc[i][j] = block_mma(T{}, a[0][i], a[1][i], b[0][j], b[1][j], acc[i][j]);
   };
 
-  if constexpr (DMA) {
+  for (int term = 0; term < p.terms; ++term) {
+    la.init(static_cast<const char *>(p.a) + term * p.a_term, p.lda, p.m, m0, k0, p.k);
+    lb.init(static_cast<const char *>(p.b) + term * p.b_term, p.ldb, p.n, n0, k0, p.k);
+    if (term) barrier();  // the last term's slabs are used up
+    if constexpr (DMA) {
 #pragma unroll
-    for (int s = 0; s < ST - 1; ++s)
-      if (s < count) {
-        la.issue(s, lds0 + s * STAGE);
-        lb.issue(s, lds0 + s * STAGE + BM * 128);
-      }
-    int at = 0;
-    for (int s = 0; s < count; ++s) {
-      if (ST > 2 && s + ST - 2 < count) wait_loads<(ST - 2) * LOADS>();
-      else wait_loads<0>();
-      barrier();
-      const int into = at == 0 ? ST - 1 : at - 1;
-      if (s + ST - 1 < count) {
-        la.issue(s + ST - 1, lds0 + into * STAGE);
-        lb.issue(s + ST - 1, lds0 + into * STAGE + BM * 128);
-      }
-      multiply(lds + at * STAGE);
-      wait_lds();
-      at = at == ST - 1 ? 0 : at + 1;
-    }
-  } else {
-    // Two slabs are under way in registers while one is multiplied.
-    i32x4 ha[2][decltype(la)::PER_WAVE], hb[2][decltype(lb)::PER_WAVE];
-#pragma unroll
-    for (int s = 0; s < 2; ++s)
-      if (s < count) {
-        la.fetch(s, ha[s]);
-        lb.fetch(s, hb[s]);
-      }
-    if (count > 0) {
-      la.put(lds, ha[0]);
-      lb.put(lds + BM * 128, hb[0]);
-    }
-    for (int s = 0; s < count; s += 2) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        if (s + h >= count) break;
-        wait_lds();
+      for (int s = 0; s < ST - 1; ++s)
+        if (s < count) {
+          la.issue(s, lds0 + s * STAGE);
+          lb.issue(s, lds0 + s * STAGE + BM * 128);
+        }
+      int at = 0;
+      for (int s = 0; s < count; ++s) {
+        if (ST > 2 && s + ST - 2 < count) wait_loads<(ST - 2) * LOADS>();
+        else wait_loads<0>();
         barrier();
-        if (s + h + 2 < count) {
-          la.fetch(s + h + 2, ha[h]);
-          lb.fetch(s + h + 2, hb[h]);
+        const int into = at == 0 ? ST - 1 : at - 1;
+        if (s + ST - 1 < count) {
+          la.issue(s + ST - 1, lds0 + into * STAGE);
+          lb.issue(s + ST - 1, lds0 + into * STAGE + BM * 128);
         }
-        multiply(lds + h * STAGE);
-        if (s + h + 1 < count) {
-          la.put(lds + (1 - h) * STAGE, ha[1 - h]);
-          lb.put(lds + (1 - h) * STAGE + BM * 128, hb[1 - h]);
+        multiply(lds + at * STAGE);
+        wait_lds();
+        at = at == ST - 1 ? 0 : at + 1;
+      }
+    } else {
+      // Two slabs are under way in registers while one is multiplied.
+      i32x4 ha[2][decltype(la)::PER_WAVE], hb[2][decltype(lb)::PER_WAVE];
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+        if (s < count) {
+          la.fetch(s, ha[s]);
+          lb.fetch(s, hb[s]);
+        }
+      if (count > 0) {
+        la.put(lds, ha[0]);
+        lb.put(lds + BM * 128, hb[0]);
+      }
+      for (int s = 0; s < count; s += 2) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          if (s + h >= count) break;
+          wait_lds();
+          barrier();
+          if (s + h + 2 < count) {
+            la.fetch(s + h + 2, ha[h]);
+            lb.fetch(s + h + 2, hb[h]);
+          }
+          multiply(lds + h * STAGE);
+          if (s + h + 1 < count) {
+            la.put(lds + (1 - h) * STAGE, ha[1 - h]);
+            lb.put(lds + (1 - h) * STAGE + BM * 128, hb[1 - h]);
+          }
         }
       }
     }
+    wait_lds();
   }
-  // The slabs' LDS is the patches' now: all waves have read theirs.
-  wait_lds();
-  barrier();
+  barrier();  // the slabs' LDS is the patches' now
   constexpr int COLS = BN / WN, ROWS = BM / WM / ((BM / WM) * COLS > 4096 ? 2 : 1);  // 16 KiB a wave at most
   static_assert(NW * ROWS * COLS * 4 <= (DMA ? ST : 2) * STAGE, "the patches fit into the slabs' LDS");
   lds_char *patch = lds + wave * (ROWS * COLS * 4);
@@ -506,6 +517,25 @@ __global__ __launch_bounds__(64 * WM *WN) void gemm_tile_kernel(GemmParams p) {
     wait_lds();
     write_patch<T, O, ROWS, COLS>(p, split, patch, m0 + wm * (BM / WM) + h * ROWS, n0 + wn * COLS, tm * BM, tn * BN);
   }
+}
+
+template <typename T, typename O, bool AMN, bool BMN, int BM, int BN, int WM, int WN, int ST, bool DMA>
+__global__ __launch_bounds__(64 * WM *WN) void gemm_tile_kernel(GemmParams p) {
+  __shared__ __align__(1024) char smem[tile_lds<BM, BN, ST>()];
+  gemm_tile<T, O, AMN, BMN, BM, BN, WM, WN, ST, DMA>(p, blockIdx.x, gridDim.x, (lds_char *)smem);
+}
+
+// A small layer's two gradient products in one launch: dx (its left operand along
+// k) by the first `first` workgroups, dw (both along their own dimensions) by the
+// others.
+template <typename T, bool BMN>
+__global__ __launch_bounds__(256) void gemm_pair_kernel(GemmParams dx, GemmParams dw, int first) {
+  constexpr int ST = 4;
+  __shared__ __align__(1024) char smem[tile_lds<64, 64, ST>()];
+  if (static_cast<int>(blockIdx.x) < first)
+    gemm_tile<T, T, false, BMN, 64, 64, 2, 2, ST, true>(dx, blockIdx.x, first, (lds_char *)smem);
+  else
+    gemm_tile<T, T, true, true, 64, 64, 2, 2, ST, true>(dw, blockIdx.x - first, gridDim.x - first, (lds_char *)smem);
 }
 
 // ---- few rows -----------------------------------------------------------------

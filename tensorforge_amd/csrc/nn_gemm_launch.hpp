@@ -22,12 +22,24 @@ hipError_t launch_layout(const GemmParams &p, int tile, bool dma, hipStream_t st
   if (dma) {
     if (tile == TILE_256) gemm_wide_kernel<T, O, AMN, BMN><<<grid, 512, 0, stream>>>(p);
     else if (tile == TILE_128) gemm_tile_kernel<T, O, AMN, BMN, 128, 128, 2, 2, 2, true><<<grid, 256, 0, stream>>>(p);
-    else if (grid.x <= 256) gemm_tile_kernel<T, O, AMN, BMN, 64, 64, 2, 2, 8, true><<<grid, 256, 0, stream>>>(p);
-    else gemm_tile_kernel<T, O, AMN, BMN, 64, 64, 2, 2, 3, true><<<grid, 256, 0, stream>>>(p);
+    else if (tile == TILE_64x128) gemm_tile_kernel<T, O, AMN, BMN, 64, 128, 2, 2, 3, true><<<grid, 256, 0, stream>>>(p);
+    // Three slabs of LDS leave room for three workgroups on a CU, two for five: 1024 x
+    // 2048 x 4096 (512 workgroups) 28.0 us with three, 35.4 with two; 1024 x 4096 x 4096
+    // (1024) 55.7 and 48.7.
+    else if (grid.x <= 768) gemm_tile_kernel<T, O, AMN, BMN, 64, 64, 2, 2, 3, true><<<grid, 256, 0, stream>>>(p);
+    else gemm_tile_kernel<T, O, AMN, BMN, 64, 64, 2, 2, 2, true><<<grid, 256, 0, stream>>>(p);
   } else {
-    if (tile == TILE_128) gemm_tile_kernel<T, O, AMN, BMN, 128, 128, 2, 2, 2, false><<<grid, 256, 0, stream>>>(p);
-    else gemm_tile_kernel<T, O, AMN, BMN, 64, 64, 2, 2, 2, false><<<grid, 256, 0, stream>>>(p);
+    gemm_tile_kernel<T, O, AMN, BMN, 64, 64, 2, 2, 2, false><<<grid, 256, 0, stream>>>(p);
   }
+  return hipGetLastError();
+}
+
+template <typename T>
+hipError_t launch_pair(const GemmParams &dx, bool bmn, const GemmParams &dw, hipStream_t stream) {
+  const int first = dx.tiles_m * dx.tiles_n;
+  const dim3 grid(static_cast<unsigned>(first + dw.tiles_m * dw.tiles_n));
+  if (bmn) gemm_pair_kernel<T, true><<<grid, 256, 0, stream>>>(dx, dw, first);
+  else gemm_pair_kernel<T, false><<<grid, 256, 0, stream>>>(dx, dw, first);
   return hipGetLastError();
 }
 

@@ -39,29 +39,49 @@ struct GemmParams {
   int m = 0, n = 0, k = 0;
   int tiles_m = 0, tiles_n = 0, splits = 1;
   int act = 0, bias_f32 = 0;
+  int terms = 1;                // 2: a second term of A at a + a_term, or of B at b + b_term (bytes)
+  long a_term = 0, b_term = 0;  // (64 and 128 tiles)
 };
 
-// C tiles of the product kernels.  256 x 256 loads straight into LDS only.
+// C tiles of the product kernels; but for 64 x 64 they load straight into LDS only.
 // TILE_ROWS: all of up to 64 rows, the waves of a workgroup split k (the left
 // operand along k only).
-enum Tile { TILE_256 = 1, TILE_128 = 2, TILE_64 = 3, TILE_ROWS = 4 };
-constexpr int tile_size(int tile) { return tile == TILE_256 ? 256 : tile == TILE_128 ? 128 : 64; }
+enum Tile { TILE_256 = 1, TILE_128 = 2, TILE_64 = 3, TILE_ROWS = 4, TILE_64x128 = 5 };
+constexpr int tile_rows(int tile) { return tile == TILE_256 ? 256 : tile == TILE_128 ? 128 : 64; }
+constexpr int tile_columns(int tile) { return tile == TILE_64x128 ? 128 : tile_rows(tile); }
 
 // amn, bmn: the operand's own dimension (m, n) is contiguous, not k.
 hipError_t launch_gemm_bf16(const GemmParams &p, bool amn, bool bmn, int tile, bool dma, hipStream_t stream);
 hipError_t launch_gemm_f16(const GemmParams &p, bool amn, bool bmn, int tile, bool dma, hipStream_t stream);
 hipError_t launch_gemm_f8(const GemmParams &p, int out_type, int tile, bool dma, hipStream_t stream);
+// Both products of a small layer's gradient in one launch, 64 x 64 tiles, loads
+// straight into LDS: dx with amn false, dw with amn and bmn true.
+hipError_t launch_gemm_pair_bf16(const GemmParams &dx, bool bmn, const GemmParams &dw, hipStream_t stream);
+hipError_t launch_gemm_pair_f16(const GemmParams &dx, bool bmn, const GemmParams &dw, hipStream_t stream);
+
+// Up to two matrices copied to rows of whole 16-byte pieces, zeros in the pad.
+struct PackParams {
+  const void *from[2];
+  void *to[2];
+  long from_ld[2], to_ld[2], rows[2];  // elements
+  int columns[2];
+  long pieces[2];  // rows x to_ld in pieces; 0: none
+};
+hipError_t launch_pack(const PackParams &p, int size, hipStream_t stream);
+
 // out = epilogue(sum of the splits' parts).
 hipError_t launch_gemm_join(const GemmParams &p, int out_type, hipStream_t stream);
 
 struct SlopeParams {
   const void *dy, *z;
-  void *dz;       // m x dz_ld, columns from n on zero; null with act none
-  float *shares;  // column_shares(m) x n; null: no sums
+  void *dz;       // m x dz_ld, columns from n on zero; null: sums alone
+  long lo;        // not 0: what dz's rounding left, rounded, that many elements behind
+  float *shares;  // column_shares(m) x n; null with one share, or without sums
+  void *sums;     // with column_shares(m) = 1, the sums themselves, of sums_type; else null
   long dy_ld, z_ld, dz_ld;
-  int m, n, act;
+  int m, n, act, sums_type;
 };
-// dz = dy * act'(z), and dz's column sums in shares.
+// dz = dy * act'(z) (act none: dy), and dz's column sums.
 long column_shares(long m);
 hipError_t launch_act_slope(const SlopeParams &p, int type, hipStream_t stream);
 // out[0..d) = sum of `count` shares, in order, rounded to `type`.

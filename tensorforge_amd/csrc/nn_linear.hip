@@ -1,5 +1,6 @@
 // What the products need beside the matrix kernels: the join of a product split
-// along k, and the activation's slope with the bias gradient's sums.
+// along k, aligned copies of operands, and the activation's slope with the bias
+// gradient's sums.
 #include "nn_gemm.hpp"
 
 #include <algorithm>
@@ -37,63 +38,100 @@ void join(const GemmParams &p, hipStream_t stream) {
   else gemm_join_kernel<O, ACT_NONE><<<grid, 256, 0, stream>>>(p);
 }
 
-constexpr int kSlopeRows = 64;
+template <typename T>
+__global__ __launch_bounds__(256) void pack_kernel(PackParams p) {
+  constexpr int N = kPiece<T>;
+  long id = static_cast<long>(blockIdx.x) * 256 + threadIdx.x;
+  const int q = id >= p.pieces[0];
+  if (q) id -= p.pieces[0];
+  if (id >= p.pieces[q]) return;
+  const long per = p.to_ld[q] / N, row = id / per;
+  const int c = static_cast<int>(id % per) * N;
+  const i32x4 v = load_piece_any(static_cast<const T *>(p.from[q]) + row * p.from_ld[q], c, p.columns[q]);
+  *reinterpret_cast<i32x4 *>(static_cast<T *>(p.to[q]) + row * p.to_ld[q] + c) = v;
+}
 
-// 256 columns x 64 rows a workgroup: 32 threads of 8 columns by 8 rows.
-template <typename T, int ACT>
-__global__ __launch_bounds__(256) void act_slope_kernel(SlopeParams p) {
-  const int column_blocks = (p.n + 255) / 256, bc = blockIdx.x % column_blocks, br = blockIdx.x / column_blocks;
-  const int c = (bc * 32 + threadIdx.x % 32) * 8, lane = threadIdx.x / 32;
-  const long row0 = static_cast<long>(br) * kSlopeRows;
+// A workgroup of the slope takes 64 rows; with up to 512 rows, all of them, so
+// that the bias gradient needs no second launch.
+constexpr int kSlopeRows = 64, kSlopeWhole = 512;
+
+// 8 columns a thread; CT threads side by side, the others down the rows.
+template <typename T, int ACT, int CT>
+__global__ __launch_bounds__(256) void act_slope_kernel(SlopeParams p, int rows) {
+  constexpr int LANES = 256 / CT, COLS = CT * 8;
+  const int column_blocks = (p.n + COLS - 1) / COLS, bc = blockIdx.x % column_blocks, br = blockIdx.x / column_blocks;
+  const int c = bc * COLS + threadIdx.x % CT * 8, lane = threadIdx.x / CT, left = p.n - c;
+  const long row0 = static_cast<long>(br) * rows;
   float sum[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) sum[i] = 0.0f;
-  const int left = p.n - c;
   if (left > 0) {
-    for (int r = lane; r < kSlopeRows && row0 + r < p.m; r += 8) {
+    const int end = static_cast<int>(min(static_cast<long>(rows), p.m - row0));
+#pragma unroll 4
+    for (int r = lane; r < end; r += LANES) {
       const long row = row0 + r;
       float g[8], z[8];
       load_some(static_cast<const T *>(p.dy) + row * p.dy_ld + c, left, g);
       if constexpr (ACT != ACT_NONE) {
         load_some(static_cast<const T *>(p.z) + row * p.z_ld + c, left, z);
-        typename Vec<T, 8>::type out;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) g[i] *= act_slope<ACT>(z[i]);
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sum[i] += g[i];
+      if (p.dz) {
+        typename Vec<T, 8>::type hi, lo;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const float v = g[i] * act_slope<ACT>(z[i]);
-          sum[i] += v;
-          out[i] = i < left ? static_cast<T>(v) : static_cast<T>(0.0f);
+          hi[i] = i < left ? static_cast<T>(g[i]) : static_cast<T>(0.0f);
+          lo[i] = i < left ? static_cast<T>(g[i] - static_cast<float>(hi[i])) : static_cast<T>(0.0f);
         }
-        *reinterpret_cast<typename Vec<T, 8>::type *>(static_cast<T *>(p.dz) + row * p.dz_ld + c) = out;
-      } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) sum[i] += g[i];
+        T *to = static_cast<T *>(p.dz) + row * p.dz_ld + c;
+        *reinterpret_cast<typename Vec<T, 8>::type *>(to) = hi;
+        if (p.lo) *reinterpret_cast<typename Vec<T, 8>::type *>(to + p.lo) = lo;
       }
     }
   }
-  if (!p.shares) return;
-  __shared__ float part[8][8][33];
+  if (!p.shares && !p.sums) return;
+  __shared__ float part[LANES][8][CT + 1];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) part[lane][i][threadIdx.x % 32] = sum[i];
+  for (int i = 0; i < 8; ++i) part[lane][i][threadIdx.x % CT] = sum[i];
   __syncthreads();
-  const int i = threadIdx.x % 8, col = threadIdx.x / 8, at = (bc * 32 + col) * 8 + i;
+  const int e = threadIdx.x % COLS, at = bc * COLS + e;
+  if (threadIdx.x >= COLS) return;
   float v = 0.0f;
 #pragma unroll
-  for (int q = 0; q < 8; ++q) v += part[q][i][col];
-  if (at < p.n) p.shares[static_cast<long>(br) * p.n + at] = v;
+  for (int q = 0; q < LANES; ++q) v += part[q][e % 8][e / 8];
+  if (at >= p.n) return;
+  if (p.sums) store_as(p.sums, p.sums_type, at, v);
+  else p.shares[static_cast<long>(br) * p.n + at] = v;
+}
+
+template <typename T, int ACT>
+void slope(const SlopeParams &p, hipStream_t stream) {
+  const long shares = column_shares(p.m);
+  // Few rows: narrow columns, more threads down each.
+  if (shares == 1) act_slope_kernel<T, ACT, 4><<<dim3((p.n + 31) / 32), 256, 0, stream>>>(p, kSlopeWhole);
+  else act_slope_kernel<T, ACT, 32><<<dim3(static_cast<unsigned>(shares * ((p.n + 255) / 256))), 256, 0, stream>>>(p, kSlopeRows);
 }
 
 template <typename T>
 void slope(const SlopeParams &p, hipStream_t stream) {
-  const dim3 grid(static_cast<unsigned>(column_shares(p.m) * ((p.n + 255) / 256)));
-  if (p.act == ACT_RELU) act_slope_kernel<T, ACT_RELU><<<grid, 256, 0, stream>>>(p);
-  else if (p.act == ACT_GELU) act_slope_kernel<T, ACT_GELU><<<grid, 256, 0, stream>>>(p);
-  else if (p.act == ACT_SILU) act_slope_kernel<T, ACT_SILU><<<grid, 256, 0, stream>>>(p);
-  else act_slope_kernel<T, ACT_NONE><<<grid, 256, 0, stream>>>(p);
+  if (p.act == ACT_RELU) slope<T, ACT_RELU>(p, stream);
+  else if (p.act == ACT_GELU) slope<T, ACT_GELU>(p, stream);
+  else if (p.act == ACT_SILU) slope<T, ACT_SILU>(p, stream);
+  else slope<T, ACT_NONE>(p, stream);
 }
 
 }  // namespace
 
-long column_shares(long m) { return (m + kSlopeRows - 1) / kSlopeRows; }
+long column_shares(long m) { return m <= kSlopeWhole ? 1 : (m + kSlopeRows - 1) / kSlopeRows; }
+
+hipError_t launch_pack(const PackParams &p, int size, hipStream_t stream) {
+  const dim3 grid(static_cast<unsigned>((p.pieces[0] + p.pieces[1] + 255) / 256));
+  size == 1 ? pack_kernel<f8><<<grid, 256, 0, stream>>>(p) : pack_kernel<bf16><<<grid, 256, 0, stream>>>(p);
+  return hipGetLastError();
+}
 
 hipError_t launch_gemm_join(const GemmParams &p, int out_type, hipStream_t stream) {
   out_type == TYPE_BF16 ? join<bf16>(p, stream) : join<f16>(p, stream);

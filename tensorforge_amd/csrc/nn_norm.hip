@@ -2,7 +2,7 @@
 // 8 bits with a scale a row, the row quantisation alone, and the norm's gradient.
 //
 //   h = x + residual           r = 1/sqrt(mean(h^2) + eps)
-//   y = (h*r)*w                scale = max|y| / 448, code = nearest(y * (448/max|y|))
+//   y = (h*r)*w                scale = max|y| / 448, code = nearest(y * (448 * (1/max|y|)))
 //   g = dy*w, xhat = h*r       dx = r*(g - xhat*mean(g*xhat)) + dh,  dw = sum over rows of dy*xhat
 //
 // All of it is bound by memory.  A row stays in its threads' registers between
@@ -79,27 +79,27 @@ __device__ __forceinline__ void load_weight8(const NormParams &p, int c, float (
 }
 
 // Sum of `sum`, and sum or maximum (MAX) of `more`, over the NT threads of a
-// row.  With NT = 256 the four waves meet in LDS; `turn` alternates between two
-// places, so one barrier a row is enough.  Every thread of the workgroup calls
-// it equally often.
-template <int NT, bool MAX>
+// row.  With NT = 256 the four waves meet in LDS (ROWS rows a workgroup, each in a
+// place of its own); `turn` alternates between two places, so one barrier a row is
+// enough.  Every thread of the workgroup calls it equally often.
+template <int NT, bool MAX, int ROWS = 1>
 __device__ __forceinline__ void row_reduce(float &sum, float &more, int turn) {
   sum = wave_sum(sum);
   more = MAX ? wave_max(more) : wave_sum(more);
   if constexpr (NT > 64) {
-    __shared__ float part[2][2][NT / 64];
-    const int wave = threadIdx.x / 64;
+    __shared__ float part[2][2][ROWS * NT / 64];
+    const int wave = threadIdx.x / 64, first = threadIdx.x / NT * (NT / 64);
     if (threadIdx.x % 64 == 0) {
       part[turn][0][wave] = sum;
       part[turn][1][wave] = more;
     }
     __syncthreads();
-    sum = part[turn][0][0];
-    more = part[turn][1][0];
+    sum = part[turn][0][first];
+    more = part[turn][1][first];
 #pragma unroll
     for (int i = 1; i < NT / 64; ++i) {
-      sum += part[turn][0][i];
-      more = MAX ? max_keep_nan(more, part[turn][1][i]) : more + part[turn][1][i];
+      sum += part[turn][0][first + i];
+      more = MAX ? max_keep_nan(more, part[turn][1][first + i]) : more + part[turn][1][first + i];
     }
   }
 }
@@ -146,7 +146,7 @@ __global__ __launch_bounds__(256) void rms_norm_kernel(NormParams p) {
     float f = 1.0f;
     if constexpr (sizeof(O) == 1) {
       const float most = f8_top(top * r);
-      f = kF8Max / most;
+      f = kF8Max * (1.0f / most);
       if (t == 0) p.scale[row] = most / kF8Max;
     }
     O *y = static_cast<O *>(p.y) + row * p.y_ld;
@@ -192,7 +192,7 @@ __global__ __launch_bounds__(256) void rms_norm_long_kernel(NormParams p) {
   float f = 1.0f;
   if constexpr (sizeof(O) == 1) {
     const float most = f8_top(top * r);
-    f = kF8Max / most;
+    f = kF8Max * (1.0f / most);
     if (threadIdx.x == 0) p.scale[row] = most / kF8Max;
   }
   for (int c = threadIdx.x * 8; c < p.d; c += NT * 8) {
@@ -214,11 +214,18 @@ __global__ __launch_bounds__(256) void rms_norm_long_kernel(NormParams p) {
   }
 }
 
+// Rows a gradient workgroup takes at a time.  More rows leave fewer shares to add
+// up, but go in step: 777 x 1111 in float32 18.3 us a call with one, 13.7 with two
+// (shares' sum 9 to 5); 8192 x 4096 in bfloat16, where the rows' time counts, 60 us
+// with one of 256 threads, 71 with two.
+constexpr int grad_rows(int nt, int ch) { return nt == 64 ? 4 : ch == 1 ? 2 : 1; }
+constexpr long kNormGradGroups = 512;
+
 // The gradient's dx, and this workgroup's rows' share of dw.  The shares are
 // added by share_sum_kernel, in a fixed order.
 template <typename T, int NT, int CH, Length L>
-__global__ __launch_bounds__(256) void rms_norm_grad_kernel(NormGradParams p) {
-  constexpr int RPB = 256 / NT;
+__global__ __launch_bounds__(NT *grad_rows(NT, CH)) void rms_norm_grad_kernel(NormGradParams p) {
+  constexpr int RPB = grad_rows(NT, CH), THREADS = NT * RPB;
   const int t = threadIdx.x % NT, sub = threadIdx.x / NT;
   const NormParams wp{.weight = p.weight, .d = p.d, .weight_type = p.weight_type};
   float w[CH][8], dw[CH][8];
@@ -229,7 +236,12 @@ __global__ __launch_bounds__(256) void rms_norm_grad_kernel(NormGradParams p) {
     for (int i = 0; i < 8; ++i) dw[j][i] = 0.0f;
   }
   int turn = 0;
-  for (long row = static_cast<long>(blockIdx.x) * RPB + sub; row < p.rows; row += static_cast<long>(gridDim.x) * RPB) {
+  // All of a workgroup's threads go through equally many rows (the barrier); one
+  // past the end repeats the last and leaves nothing.
+  const long step = static_cast<long>(gridDim.x) * RPB;
+  for (long row0 = static_cast<long>(blockIdx.x) * RPB; row0 < p.rows; row0 += step) {
+    const bool past = row0 + sub >= p.rows;
+    const long row = past ? p.rows - 1 : row0 + sub;
     float h[CH][8], g[CH][8];
 #pragma unroll
     for (int j = 0; j < CH; ++j)
@@ -245,8 +257,9 @@ __global__ __launch_bounds__(256) void rms_norm_grad_kernel(NormGradParams p) {
         sum = __builtin_fmaf(h[j][i], h[j][i], sum);
         dot = __builtin_fmaf(g[j][i] * w[j][i], h[j][i], dot);
       }
-    row_reduce<NT, false>(sum, dot, turn);
+    row_reduce<NT, false, RPB>(sum, dot, turn);
     turn ^= 1;
+    if (past) continue;
     const float r = rsqrtf(sum / static_cast<float>(p.d) + p.eps);
     const float c = dot * r * r / static_cast<float>(p.d);  // xhat*mean(g*xhat) = h*c
 #pragma unroll
@@ -268,14 +281,14 @@ __global__ __launch_bounds__(256) void rms_norm_grad_kernel(NormGradParams p) {
 #pragma unroll
     for (int j = 0; j < CH; ++j) store8(share + (j * NT + t) * 8, p.d - (j * NT + t) * 8, dw[j]);
   } else {
-    // The four rows' sums meet in LDS: one share a workgroup.
+    // The rows' sums meet in LDS: one share a workgroup.
     __shared__ float part[RPB][NT * CH * 8];
 #pragma unroll
     for (int j = 0; j < CH; ++j)
 #pragma unroll
       for (int i = 0; i < 8; ++i) part[sub][(j * 8 + i) * NT + t] = dw[j][i];
     __syncthreads();
-    for (int e = threadIdx.x; e < NT * CH * 8; e += 256) {
+    for (int e = threadIdx.x; e < NT * CH * 8; e += THREADS) {
       const int at = ((e / NT / 8) * NT + e % NT) * 8 + e / NT % 8;
       float s = part[0][e];
 #pragma unroll
@@ -402,12 +415,12 @@ void norm_launch(const NormParams &p, hipStream_t stream) {
 template <typename T, Length L>
 void norm_grad_launch_as(const NormGradParams &p, dim3 grid, hipStream_t stream) {
   const int n = pieces(p.d);
-  if (n <= 64) rms_norm_grad_kernel<T, 64, 1, L><<<grid, 256, 0, stream>>>(p);
-  else if (n <= 128) rms_norm_grad_kernel<T, 64, 2, L><<<grid, 256, 0, stream>>>(p);
-  else if (n <= 256) rms_norm_grad_kernel<T, 256, 1, L><<<grid, 256, 0, stream>>>(p);
-  else if (n <= 512) rms_norm_grad_kernel<T, 256, 2, L><<<grid, 256, 0, stream>>>(p);
-  else if (n <= 1024) rms_norm_grad_kernel<T, 256, 4, L><<<grid, 256, 0, stream>>>(p);
-  else rms_norm_grad_kernel<T, 256, 8, L><<<grid, 256, 0, stream>>>(p);
+  if (n <= 64) rms_norm_grad_kernel<T, 64, 1, L><<<grid, 64 * grad_rows(64, 1), 0, stream>>>(p);
+  else if (n <= 128) rms_norm_grad_kernel<T, 64, 2, L><<<grid, 64 * grad_rows(64, 2), 0, stream>>>(p);
+  else if (n <= 256) rms_norm_grad_kernel<T, 256, 1, L><<<grid, 256 * grad_rows(256, 1), 0, stream>>>(p);
+  else if (n <= 512) rms_norm_grad_kernel<T, 256, 2, L><<<grid, 256 * grad_rows(256, 2), 0, stream>>>(p);
+  else if (n <= 1024) rms_norm_grad_kernel<T, 256, 4, L><<<grid, 256 * grad_rows(256, 4), 0, stream>>>(p);
+  else rms_norm_grad_kernel<T, 256, 8, L><<<grid, 256 * grad_rows(256, 8), 0, stream>>>(p);
 }
 
 template <typename T>
@@ -425,8 +438,9 @@ void norm_grad_launch(const NormGradParams &p, hipStream_t stream) {
 }  // namespace
 
 long norm_grad_shares(long rows, long d) {
-  const long rpb = d >= 8 && pieces(d) <= 128 ? 4 : 1;  // rows a workgroup takes at a time
-  return std::min<long>((rows + rpb - 1) / rpb, 1024);
+  const int n = pieces(d);
+  const long at_a_time = d < 8 || n > 256 ? 1 : n <= 128 ? 4 : 2;  // grad_rows of the kernel that runs
+  return std::min<long>((rows + at_a_time - 1) / at_a_time, at_a_time == 1 ? 2 * kNormGradGroups : kNormGradGroups);
 }
 
 hipError_t launch_share_sum(const float *shares, long count, int d, void *out, int type, hipStream_t stream) {

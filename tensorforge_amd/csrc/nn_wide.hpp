@@ -87,7 +87,7 @@ __global__ __launch_bounds__(512, 2) void gemm_wide_kernel(GemmParams p) {
   const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(lds));
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), wm = wave / 4, wn = wave % 4;
   int tm, tn, split;
-  tile_of(p, tm, tn, split);
+  tile_of(p, blockIdx.x, gridDim.x, tm, tn, split);
   const int slabs = (p.k + kSlab<T> - 1) / kSlab<T>;
   const int s0 = static_cast<int>(static_cast<long>(slabs) * split / p.splits);
   const int count = static_cast<int>(static_cast<long>(slabs) * (split + 1) / p.splits) - s0;

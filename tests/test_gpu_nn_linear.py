@@ -74,7 +74,7 @@ def test_linear(m, n, k, order, dtype):
 
 @pytest.mark.parametrize("dtype", HALF)
 @pytest.mark.parametrize("order", [0, 1])
-@pytest.mark.parametrize("tile", [1, 2, 3])
+@pytest.mark.parametrize("tile", [1, 2, 3, 5])
 @pytest.mark.parametrize("splits", [1, 3])
 def test_linear_tiles(tile, splits, order, dtype):
     """Every tile over its edges, whole and ragged k, aligned (loads straight into LDS) and not."""
@@ -102,7 +102,7 @@ def test_linear_few_rows(order, dtype):
 
 
 @pytest.mark.parametrize("out_dtype", HALF)
-@pytest.mark.parametrize("tile,splits", [(0, 0), (1, 1), (2, 1), (3, 1), (2, 2), (3, 3)])
+@pytest.mark.parametrize("tile,splits", [(0, 0), (1, 1), (2, 1), (3, 1), (5, 1), (2, 2), (3, 3)])
 def test_linear_8bit(tile, splits, out_dtype):
     nn = _nn()
     for m, n, k in ((1, 1, 1), (1, 64, 128), (16, 48, 256), (17, 257, 144), (30, 70, 9000), (64, 130, 1040), (257, 264, 272), (40, 72, 100)):
@@ -153,7 +153,7 @@ def test_linear_grad(activation, order, dtype):
 
 
 @pytest.mark.parametrize("order", [0, 1])
-@pytest.mark.parametrize("tile", [1, 2, 3])
+@pytest.mark.parametrize("tile", [1, 2, 3, 5])
 @pytest.mark.parametrize("splits", [1, 2])
 def test_linear_grad_tiles(tile, splits, order):
     nn = _nn()
@@ -163,6 +163,55 @@ def test_linear_grad_tiles(tile, splits, order):
         got = nn.linear_grad(dy.cuda(), x.cuda(), _ordered(w, order), z.cuda(), "silu", bias_dtype=torch.float32, tile=tile,
                              splits=splits)
         _check_grad(got, dy, x, w, z, "silu", torch.bfloat16, torch.float32)
+
+
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("activation", ["gelu", "silu"])
+def test_small_gradients_round_once(activation, dtype):
+    """Small gradients carry what dz's rounding leaves: their error is their own rounding's (5% for the few elements, and
+    the float sums' share)."""
+    nn = _nn()
+    for m, n, k in ((1, 300, 200), (64, 64, 64), (100, 264, 136), (130, 77, 65), (600, 128, 128), (2, 1000, 3000)):
+        for order in (0, 1):
+            g = torch.Generator().manual_seed(m + n)
+            dy, x, w, z = (_matrix(g, *s, dtype) for s in ((m, n), (m, k), (k, n), (m, n)))
+            dx, dw, _ = nn.linear_grad(dy.cuda(), x.cuda(), _ordered(w, order), z.cuda(), activation)
+            dz = dy.double() * ref.slope(z.double(), activation)
+            for got, want in ((dx, dz @ w.double().t()), (dw, x.double().t() @ dz)):
+                own = (want.to(dtype).double() - want).norm()
+                assert float((got.cpu().double() - want).norm()) <= 1.05 * float(own) + 4e-6 * float(want.norm()), (m, n, k)
+
+
+@pytest.mark.parametrize("order", [0, 1])
+def test_large_ragged(order):
+    """Sizes whose unaligned operands are copied to aligned rows first, in both directions."""
+    nn = _nn()
+    m, n, k = 1031, 1045, 1003
+    g = torch.Generator().manual_seed(1)
+    x, w, dy, z = (_matrix(g, *s, torch.bfloat16, sc) for s, sc in (((m, k), 1), ((k, n), .03), ((m, n), 1), ((m, n), 1)))
+    out = nn.linear(x.cuda(), _ordered(w, order), None, "silu", dy.cuda())
+    _check(out, x, w, None, "silu", dy, None, torch.bfloat16)
+    for activation in ("none", "gelu"):
+        got = nn.linear_grad(dy.cuda(), x.cuda(), _ordered(w, order), z.cuda(), activation, bias_dtype=torch.float32)
+        _check_grad(got, dy, x, w, z, activation, torch.bfloat16, torch.float32)
+    q, s = nn.quantize_rows(x.float().cuda())
+    wq, ws = nn.quantize_rows(w.t().contiguous().float().cuda())
+    out = nn.linear(q, wq.t(), None, "none", None, x_scale=s, w_scale=ws)
+    _check(out, q.cpu().float(), wq.cpu().float().t(), None, "none", None, None, torch.bfloat16,
+           s.cpu().double()[:, None] * ws.cpu().double())
+
+
+def test_without_workspace():
+    """Through the C ABI with no workspace: unsplit, operands as they are."""
+    from tensorforge_amd import _lib
+    g = torch.Generator().manual_seed(7)
+    for m, n, k in ((70, 64, 4096), (300, 301, 515)):
+        x, w = _matrix(g, m, k, torch.bfloat16), _matrix(g, k, n, torch.bfloat16, k ** -0.5)
+        xc, wc, out = x.cuda(), w.cuda(), torch.empty(m, n, dtype=torch.bfloat16, device="cuda")
+        a = _lib.LinearArgs(x=xc.data_ptr(), w=wc.data_ptr(), out=out.data_ptr(), x_ld=k, w_ld=n, out_ld=n, m=m, n=n, k=k,
+                            type=1, out_type=1)
+        _lib.check(_lib.lib().tf_linear(ctypes.byref(a), torch.cuda.current_stream().cuda_stream))
+        _check(out, x, w, None, "none", None, None, torch.bfloat16)
 
 
 def test_linear_grad_against_differences():
@@ -211,7 +260,7 @@ def test_strides_alignment_and_neighbours(order, dtype):
             _check_grad(got, dy, x, w, z.cpu(), "relu", dtype, dtype)
 
 
-@pytest.mark.parametrize("tile,splits", [(0, 0), (1, 1), (2, 1), (3, 1), (3, 2)])
+@pytest.mark.parametrize("tile,splits", [(0, 0), (1, 1), (2, 1), (3, 1), (5, 1), (3, 2)])
 def test_writes_stay_inside(tile, splits):
     """Through the C ABI: out and z inside wider matrices; nothing else changes."""
     from tensorforge_amd import _lib

@@ -49,7 +49,7 @@ def _linear(**kw):
     (dict(w_order=2), "w_order = 2"), (dict(out_ld=31), "out: 31"), (dict(z=256, z_ld=8), "z: 8"),
     (dict(residual=256, residual_ld=3), "residual: 3"), (dict(bias=256, bias_type=2), "bias_type = 2"),
     (dict(x_scale=256), "scales belong to 8-bit"), (dict(type=3), "8-bit weights"),
-    (dict(type=3, w_order=1, w_ld=64), "x_scale is a null pointer"), (dict(tile=5), "tile = 5"),
+    (dict(type=3, w_order=1, w_ld=64), "x_scale is a null pointer"), (dict(tile=6), "tile = 6"),
     (dict(splits=65), "splits = 65"), (dict(workspace=8, workspace_bytes=64), "not 16-byte aligned"),
     (dict(x_ld=1 << 41), "are too many"),
 ])
@@ -60,8 +60,8 @@ def test_linear_refusals(change, words):
 @pytest.mark.parametrize("change,words", [
     (dict(type=3), "type = 3"), (dict(dy=0), "dy is a null pointer"), (dict(act=1), "z is a null pointer"),
     (dict(x=0), "x is a null pointer"), (dict(w=0), "w is a null pointer"), (dict(dx_ld=63), "dx: 63"),
-    (dict(dw_ld=31), "dw: 31"), (dict(bias_type=3), "bias_type = 3"), (dict(workspace_bytes=16), "bytes, "),
-    (dict(workspace=0), "workspace is null"), (dict(n=-2), "n = -2"),
+    (dict(dw_ld=31), "dw: 31"), (dict(bias_type=3), "bias_type = 3"), (dict(act=1, z=256, z_ld=32, workspace_bytes=16), "bytes, "),
+    (dict(act=1, z=256, z_ld=32, workspace=0), "workspace is null"), (dict(n=-2), "n = -2"),
 ])
 def test_linear_grad_refusals(change, words):
     base = dict(dy=256, x=256, w=256, dx=256, dw=256, dbias=256, workspace=256, workspace_bytes=1 << 30, dy_ld=32, x_ld=64,
