@@ -242,13 +242,15 @@ __device__ __forceinline__ void load_some(const T *p, int left, float (&v)[N]) {
     for (int i = 0; i < N; ++i) v[i] = i < left ? static_cast<float>(p[i]) : 0.0f;
   }
 }
-template <int N, typename T>
+// STREAM: past the caches, for results that would push the operands out of them.
+template <bool STREAM = false, int N, typename T>
 __device__ __forceinline__ void store_some(T *p, int left, const float (&v)[N]) {
   if (left >= N) {
     typename Vec<T, N>::loose u;
 #pragma unroll
     for (int i = 0; i < N; ++i) u[i] = static_cast<T>(v[i]);
-    *reinterpret_cast<typename Vec<T, N>::loose *>(p) = u;
+    if constexpr (STREAM) __builtin_nontemporal_store(u, reinterpret_cast<typename Vec<T, N>::loose *>(p));
+    else *reinterpret_cast<typename Vec<T, N>::loose *>(p) = u;
   } else {
 #pragma unroll
     for (int i = 0; i < N; ++i)
@@ -269,21 +271,21 @@ __device__ __forceinline__ void load_bias(const GemmParams &p, int n, float (&v)
 }
 
 // z = v + bias (kept if asked for); out = act(z) + residual, rounded once.
-template <typename O, int ACT, int N>
+template <typename O, int ACT, bool STREAM = false, int N>
 __device__ __forceinline__ void finish(const GemmParams &p, int m, int n, float (&v)[N], const float (&bias)[N]) {
   const int left = p.n - n;
   float res[N];
   if (p.residual) load_some(static_cast<const O *>(p.residual) + m * p.ldr + n, left, res);
 #pragma unroll
   for (int i = 0; i < N; ++i) v[i] += bias[i];
-  if (p.z) store_some(static_cast<O *>(p.z) + m * p.ldz + n, left, v);
+  if (p.z) store_some<STREAM>(static_cast<O *>(p.z) + m * p.ldz + n, left, v);
 #pragma unroll
   for (int i = 0; i < N; ++i) v[i] = act_value<ACT>(v[i]);
   if (p.residual) {
 #pragma unroll
     for (int i = 0; i < N; ++i) v[i] += res[i];
   }
-  store_some(static_cast<O *>(p.out) + m * p.ldo + n, left, v);
+  store_some<STREAM>(static_cast<O *>(p.out) + m * p.ldo + n, left, v);
 }
 
 // f(constant) for the product's activation.
@@ -310,7 +312,7 @@ __device__ __forceinline__ uint32_t patch_at(int row, int quad) {
 // (m0, n0): the patch's place in C.  (mt, nt): the workgroup's own first row and
 // column; where its tile was moved back into the matrix, what lies before them is
 // another's (eight columns across nt are written by both, with the same values).
-template <typename T, typename O, int ROWS, int COLS>
+template <typename T, typename O, int ROWS, int COLS, bool STREAM = false>
 __device__ __forceinline__ void write_patch(const GemmParams &p, int split, const lds_char *patch, int m0, int n0, int mt,
                                             int nt) {
   constexpr int LANES = COLS / 8, STEP = 64 / LANES;
@@ -351,7 +353,7 @@ __device__ __forceinline__ void write_patch(const GemmParams &p, int split, cons
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] = v[i] * sa * sb[i];
       }
-      finish<O, act()>(p, m, n, v, bias);
+      finish<O, act(), STREAM>(p, m, n, v, bias);
     }
   });
 }

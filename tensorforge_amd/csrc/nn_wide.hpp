@@ -175,7 +175,8 @@ __global__ __launch_bounds__(512, 2) void gemm_wide_kernel(GemmParams p) {
   if (wm == 0) barrier();
   wait_loads<0>();  // the empty ones past the end
   barrier();
-  // Through LDS (nn_gemm.hpp), 64 rows at a time.
+  // Through LDS (nn_gemm.hpp), 64 rows at a time.  Results of this size stream past
+  // the caches: 8192^3 in bfloat16 1389 TFLOP/s without that, 1423 with it.
   const int lane = threadIdx.x % 64;
   lds_char *patch = lds + wave * (64 * 64 * 4);
 #pragma unroll
@@ -187,7 +188,7 @@ __global__ __launch_bounds__(512, 2) void gemm_wide_kernel(GemmParams p) {
         *reinterpret_cast<__attribute__((address_space(3))) f32x4 *>(patch + patch_at<64>(i * 16 + lane % 16, j * 4 + lane / 16)) =
             acc[4 * h + i][j];
     wait_lds();
-    write_patch<T, O, 64, 64>(p, split, patch, tm * 256 + wm * 128 + h * 64, tn * 256 + wn * 64, 0, 0);
+    write_patch<T, O, 64, 64, true>(p, split, patch, tm * 256 + wm * 128 + h * 64, tn * 256 + wn * 64, 0, 0);
   }
 }
 
