@@ -228,8 +228,11 @@ Plan plan_product(long m, long n, long k, int type, bool amn, bool bmn, bool dma
   }
   for (int t : {TILE_64, TILE_64x128, TILE_128, TILE_256}) {
     if (tile ? t != tile : t != TILE_64 && !dma) continue;
+    // Tiles mostly empty, and splits into more than four workgroups a CU, never win.
+    if (!tile && t != TILE_64 && (2 * m <= tile_rows(t) || 2 * n <= tile_columns(t))) continue;
+    const long tiles = ceil_div(m, tile_rows(t)) * ceil_div(n, tile_columns(t));
     for (int s : {1, 2, 3, 4, 6, 8, 12, 16}) {
-      if (splits ? s != 1 : s > 1 && s * 2 > slabs) continue;
+      if (s > 1 && (splits || s * 2 > slabs || tiles * s > 1024)) break;
       const int ranges = splits ? splits : s;
       const double us = predicted(m, n, slabs, read, loads, t, ranges);
       if (us < best.us) best = {t, ranges, us};
