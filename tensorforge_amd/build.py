@@ -137,7 +137,8 @@ def _resources(logs):
     dem = _demangle(list(recs))
     out = {}
     for mangled, rec in recs.items():
-        names = _entry_name(dem[mangled])
+        # The residual block's kernels are listed by their symbols.
+        names = mangled if "4tfnn" in mangled and "_kernel" in mangled else _entry_name(dem[mangled])
         if names is None:
             continue
         for name in names if isinstance(names, list) else [names]:

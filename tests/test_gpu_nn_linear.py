@@ -311,6 +311,22 @@ def test_special_values_stay_in_their_rows_and_columns():
         assert torch.allclose(db.cpu(), torch.tensor(want), atol=1e-6, equal_nan=True), activation
 
 
+def test_leading_dimensions_and_views():
+    """Leading dimensions are rows; a slice of rows, every other row and a matrix's transpose are taken where they lie."""
+    nn = _nn()
+    g = torch.Generator().manual_seed(13)
+    x, w = _matrix(g, 24, 64, torch.bfloat16).cuda(), _matrix(g, 64, 48, torch.bfloat16).cuda()
+    want = nn.linear(x, w)
+    assert torch.equal(nn.linear(x.view(2, 3, 4, 64), w), want.view(2, 3, 4, 48))
+    assert torch.equal(nn.linear(x[0], w), nn.linear(x[:1], w)[0])
+    assert torch.equal(nn.linear(x[::2], w), nn.linear(x[::2].contiguous(), w))
+    assert torch.equal(nn.linear(x.view(4, 6, 64)[1:3], w), want[6:18].view(2, 6, 48))
+    wide = _matrix(g, 64, 96, torch.bfloat16).cuda()
+    assert torch.equal(nn.linear(x, wide[:, 48:]), nn.linear(x, wide[:, 48:].contiguous()))
+    dx, _, _ = nn.linear_grad(want.view(2, 12, 48), x.view(2, 12, 64), w)
+    assert dx.shape == (2, 12, 64) and torch.equal(dx.view(24, 64), nn.linear_grad(want, x, w)[0])
+
+
 def test_empty_sizes():
     nn = _nn()
     e = lambda *s: torch.zeros(s, dtype=torch.bfloat16, device="cuda")  # noqa: E731

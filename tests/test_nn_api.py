@@ -31,6 +31,17 @@ def test_struct_layouts_match_c(tmp_path):
             assert int(got[f"{cname}.{f}"]) == getattr(py, f).offset, (cname, f)
 
 
+def test_kernels_do_not_spill():
+    import json
+    res = json.loads((_lib.PKG / "kernel_resources.json").read_text())
+    ours = {n: r for n, r in res.items() if "4tfnn" in n}
+    for kernel in ("gemm_wide_kernel", "gemm_tile_kernel", "gemm_rows_kernel", "gemm_pair_kernel", "gemm_join_kernel",
+                   "pack_kernel", "act_slope_kernel", "rms_norm_kernel", "rms_norm_grad_kernel", "share_sum_kernel"):
+        assert any(kernel in n for n in ours), kernel
+    for name, r in ours.items():
+        assert r["scratch_bytes"] == 0 and r["vgpr_spill"] == 0, name
+
+
 def _refused(call, args, words):
     assert call(ctypes.byref(args), None) == -4  # TF_E_ARG
     assert words in _lib.lib().tf_last_error().decode(), _lib.lib().tf_last_error()
