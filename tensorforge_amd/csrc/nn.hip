@@ -248,7 +248,7 @@ long long part_bytes(long m, long n, const Plan &plan) {
 // How a product runs.  Operands that cannot be loaded straight into LDS are
 // copied to aligned lines first (pack) where the faster kernels gain more than the
 // copy takes, about 4 us and its bytes at 4 TB/s: 4095 x 4097 x 1023 bfloat16 110 us
-// through registers, NNN with both copied; 777 x 1111 x 333 8.2 and NNN.
+// through registers, 63 with both copied; 777 x 1111 x 333 8.3 and 13.
 struct Choice {
   Plan plan;
   bool dma = false, pack_a = false, pack_b = false;

@@ -219,7 +219,6 @@ __global__ __launch_bounds__(256) void rms_norm_long_kernel(NormParams p) {
 // (shares' sum 9 to 5); 8192 x 4096 in bfloat16, where the rows' time counts, 60 us
 // with one of 256 threads, 71 with two.
 constexpr int grad_rows(int nt, int ch) { return nt == 64 ? 4 : ch == 1 ? 2 : 1; }
-constexpr long kNormGradGroups = 512;
 
 // The gradient's dx, and this workgroup's rows' share of dw.  The shares are
 // added by share_sum_kernel, in a fixed order.
@@ -437,10 +436,15 @@ void norm_grad_launch(const NormGradParams &p, hipStream_t stream) {
 
 }  // namespace
 
+// Workgroups, each with a share of the weight's gradient: as many as are on the GPU
+// at once, and a quarter less where that is 1024, for fewer shares to add.  us a call,
+// bfloat16, with 512 / 768 / 1024: 8192 x 4096 65.5 / 57.8 / 60.8; 8192 x 8192 83.9 / - /
+// 91.8 (256: 100); 4096 x 16384 107 / - / 130 (256: 98).
 long norm_grad_shares(long rows, long d) {
   const int n = pieces(d);
   const long at_a_time = d < 8 || n > 256 ? 1 : n <= 128 ? 4 : 2;  // grad_rows of the kernel that runs
-  return std::min<long>((rows + at_a_time - 1) / at_a_time, at_a_time == 1 ? 2 * kNormGradGroups : kNormGradGroups);
+  const long most = n <= 256 || d < 8 ? 512 : n <= 512 ? 768 : n <= 1024 ? 512 : 256;
+  return std::min<long>((rows + at_a_time - 1) / at_a_time, most);
 }
 
 hipError_t launch_share_sum(const float *shares, long count, int d, void *out, int type, hipStream_t stream) {
