@@ -174,67 +174,83 @@ struct Plan {
   double us;  // predicted
 };
 
-// Predicted time (us) of a product on one tile with k in `splits` ranges: start,
-// slabs (64 elements of k in 16 bits, 128 in 8) or the operands' bytes at 8 TB/s
-// (`read`, us), join.  Fitted on MI355X, the same
-// for all types in slabs: a slab takes a 64 x 64 tile 0.29 us alone on its CU, 0.38
-// for two and 0.17 for each of more, a 64 x 128 one 0.41 alone and 0.6 for two, a 128 x
-// 128 one 0.6 and 0.91, a 256 x
-// 256 one 1.1 (few CUs busy) to 1.48 (all, at the power limit).  Loads through
-// registers (64 x 64 tiles only) take 2.2 times that, 3.2 with an operand not along k.  Both sides of the choices (us, bfloat16):
-// 512 x 4096 x 4096 64/128/256-tile 28.4 / 44.3 / 80.6, 2048 x 4096 x 4096 101 / 62.8 /
-// 84, 4096^3 190 / 122 / 105; split 1/2/4 ways 256 x 4096 x 4096 64-tile 23.6 / 21.0 / 24.4,
+// What a product takes on one tile (us), fitted to 7444 measurements on MI355X: 500 products
+// with sizes drawn from 64 to 8192, bfloat16 and 8 bits, each tile, k in 1 to 16 ranges; it
+// errs by 6 to 9% (root mean square), and its choices take 1.8% longer than the best of
+// them (of 250 others: 3.5%).  `most` workgroups fit on a CU; one takes `end` and `slab` for each of its slabs (64
+// elements of k in 16 bits, 128 in 8) with the CU to itself, `end_most` and `slab_most` (8
+// bits: times f8) when it is full.  A last round of workgroups that leaves CUs empty takes
+// at least `rest` of a full one.  A split adds its join, start and per 1e6 results and
+// range; results that are written cost their bytes, per 1e6.  Both sides (us, bfloat16):
+// 512 x 4096 x 4096 64/128/256-tile 28.4 / 44.3 / 80.6, 2048 x 4096 x 4096 101 / 62.8 / 84,
+// 4096^3 190 / 122 / 105; split 1/2/4 ways 256 x 4096 x 4096 64-tile 23.6 / 21.0 / 24.4,
 // 2048 x 2048 x 8192 128-tile 88.6 / 72.7 / -, 96 x 2048 x 8192 64-tile 41.6 / 25.5 / 17.5
-// (8: 15.6).
-double predicted(double m, double n, double slabs, double read, double loads, int tile, int splits) {
-  const double each = std::ceil(slabs / splits);
+// (8: 15.6); 4096 x 4096 x 64 64/64 x 128/128/256-tile 15.2 / 16.6 / 14.1 / 12.4.
+struct TileCost {
+  int most;
+  double start, end, end_most, slab, slab_most, f8, rest, join, join_part, written;
+};
+constexpr TileCost kCost256{1, 7.0, 3.5, 1.3, 1.03, 1.21, 1.12, 1.0, 1.1, 1.34, 1.02};
+constexpr TileCost kCost128{2, 5.5, 0.0, 0.57, 0.58, 0.78, 1.23, 0.78, 1.8, 1.56, 0.82};
+constexpr TileCost kCost64x128{2, 2.5, 1.9, 2.9, 0.38, 0.58, 1.1, 0.49, 2.4, 1.36, 0.28};
+constexpr TileCost kCost64{3, 3.6, 0.04, 0.58, 0.27, 0.56, 1.09, 0.6, 2.5, 1.74, 0.21};
+
+// Few slabs of LDS let five 64 x 64 tiles on a CU, from 768 on: 3.5, and a workgroup 0.46
+// and 0.22 a slab.  Loads through registers (64 x 64 only) take `loads` times the slabs' time, and
+// write past the others: 1856 x 7183 x 46 32 us against 14.2.  read: the operands' bytes at 8 TB/s.
+double predicted(double m, double n, double slabs, double read, double loads, bool dma, bool f8, int tile, int splits) {
+  const TileCost &c = tile == TILE_256 ? kCost256 : tile == TILE_128 ? kCost128 : tile == TILE_64 ? kCost64 : kCost64x128;
+  const double each = std::ceil(slabs / splits) * loads, results = m * n / 1e6, most = c.most;
   const double w = std::ceil(m / tile_rows(tile)) * std::ceil(n / tile_columns(tile)) * splits / 256;  // workgroups a CU
-  double start, slab;
-  if (tile == TILE_64) {
-    start = 4.3;
-    slab = w <= 1 ? 0.29 : std::max(0.38, 0.17 * w);
-  } else if (tile != TILE_256) {
-    const double one = tile == TILE_128 ? 0.6 : 0.41, two = tile == TILE_128 ? 0.91 : 0.6;
-    const double pairs = std::floor(w / 2), rest = w - 2 * pairs;
-    start = 4.6 + 2 * std::max(0.0, std::ceil(w / 2) - 1);
-    slab = two * pairs + (rest == 0 ? 0 : rest <= 1 ? one : two);
+  const double slab_most = f8 ? c.slab_most * c.f8 : c.slab_most;
+  double us;
+  if (tile == TILE_64 && w > 3) {
+    us = 3.5 + w * (0.46 + each * (f8 ? 0.22 * c.f8 : 0.22));
   } else {
-    const double rounds = std::ceil(w);
-    start = 10 * rounds;
-    slab = 1.48 * (rounds - 1) + 1.1 + 0.38 * (w - (rounds - 1));
+    const double full = each * slab_most + c.end_most, rounds = std::floor(w / most), rest = w - rounds * most;
+    us = c.start + rounds * full;
+    if (rest > 0 && rounds > 0) us += full * (c.rest + (1 - c.rest) * rest / most);
+    if (rest > 0 && rounds == 0) {  // spread over the CUs: how full one is
+      const double of = most > 1 ? (std::ceil(rest) - 1) / (most - 1) : 0;
+      const double slab = c.slab + (slab_most - c.slab) * (most > 1 ? of : rest);  // one alone: the power limit
+      us += each * slab + c.end + (c.end_most - c.end) * of;
+    }
   }
-  return start + std::max(each * slab * loads, read) + (splits > 1 ? 3.3 + 8 * splits * m * n / 7e6 : 0);
+  us = std::max(us, 4.5 + read);
+  return splits > 1 ? us + c.join + c.join_part * splits * results : std::max(us, 4.5 + results * (dma ? c.written : 2.2));
 }
 
 // The C tile and the ranges of k for a product of these sizes: the least
-// predicted time.  Up to 64 rows the few-row kernel stands beside the tiles; its
-// workgroups read their columns' and all rows' whole k at about 40 bytes a
-// nanosecond (what a CU's misses to L2 and beyond sustain).  Measured, bfloat16, us
+// predicted time.  Up to 64 rows the few-row kernel stands beside the tiles; a workgroup
+// reads its columns' k at about 110 bytes a nanosecond and all rows' (from the caches) at
+// 45, fitted to 200 products of 1 to 64 rows.  Measured, bfloat16, us
 // (few-row / 64-tile), w 4096 x 4096 as n rows of k: 7.7 / 10.8 for 1 row, 9.8 / 11.1
 // for 16, 13.7 / 11.6 for 32; as k rows of n: 11.4 / 11.6, 13.4 / 12.2, 16.1 / 12.5.
-Plan plan_product(long m, long n, long k, int type, bool amn, bool bmn, bool dma, int tile, int splits) {
+// A left operand of two terms counts as twice the rows here, as twice the slabs on the tiles.
+Plan plan_product(long m, long n, long k, int type, int terms, bool amn, bool bmn, bool dma, int tile, int splits) {
   const int size = size_of(type);
   const long slabs = ceil_div(k, 128 / size);
-  const bool rows = m <= 64 && !amn && (!bmn || n >= 32);
+  const bool rows = m * terms <= 64 && !amn && (!bmn || n >= 32);
   if (tile == TILE_ROWS && rows) return {TILE_ROWS, 1, 0};
-  if (tile == TILE_ROWS || (!dma && tile != TILE_64)) tile = 0;
+  if (tile == TILE_ROWS || (!dma && tile != TILE_64) || (terms > 1 && tile == TILE_256)) tile = 0;
   splits = static_cast<int>(std::max<long>(0, std::min<long>(splits, std::max<long>(1, slabs))));
   Plan best{TILE_64, 1, 1e30};
   const double loads = dma ? 1 : amn || bmn ? 3.2 : 2.2;
-  const double read = (static_cast<double>(m) + n) * k * size / 8e6;
+  const double read = (static_cast<double>(m) + n) * k * terms * size / 8e6;
   if (rows && !tile) {
     const long cols = bmn ? 32 : 16;
-    best = {TILE_ROWS, 1, 3.1 + std::max(read, ceil_div(ceil_div(n, cols), 256) * static_cast<double>(cols + m) * k * size / 40e3)};
+    const double bytes = static_cast<double>(k) * size / 1e3;
+    best = {TILE_ROWS, 1, 3.4 + std::max(read, ceil_div(ceil_div(n, cols), 256) * (cols / 110.0 + m * terms / 45.0) * bytes)};
   }
   for (int t : {TILE_64, TILE_64x128, TILE_128, TILE_256}) {
-    if (tile ? t != tile : t != TILE_64 && !dma) continue;
+    if (tile ? t != tile : (t != TILE_64 && !dma) || (t == TILE_256 && terms > 1)) continue;
     // Tiles mostly empty, and splits into more than four workgroups a CU, never win.
     if (!tile && t != TILE_64 && (2 * m <= tile_rows(t) || 2 * n <= tile_columns(t))) continue;
     const long tiles = ceil_div(m, tile_rows(t)) * ceil_div(n, tile_columns(t));
     for (int s : {1, 2, 3, 4, 6, 8, 12, 16}) {
       if (s > 1 && (splits || s * 2 > slabs || tiles * s > 1024)) break;
       const int ranges = splits ? splits : s;
-      const double us = predicted(m, n, slabs, read, loads, t, ranges);
+      const double us = predicted(m, n, slabs, read, loads * terms, dma, size == 1, t, ranges);
       if (us < best.us) best = {t, ranges, us};
     }
   }
@@ -252,6 +268,7 @@ long long part_bytes(long m, long n, const Plan &plan) {
 struct Choice {
   Plan plan;
   bool dma = false, pack_a = false, pack_b = false;
+  double us = 0;  // predicted, copies and all
   long long parts = 0, copies = 0;
   long long bytes() const { return parts + copies; }
 };
@@ -262,13 +279,16 @@ Choice choose(const Product &q, int tile, int splits, bool packing = true) {
   Choice c;
   const bool da = direct_loads(q.a, size), db = direct_loads(q.b, size);
   c.dma = da && db;
-  c.plan = plan_product(p.m, p.n, p.k, q.type, q.a.mn, q.b.mn, c.dma, tile, splits);
+  c.plan = plan_product(p.m, p.n, p.k, q.type, p.terms, q.a.mn, q.b.mn, c.dma, tile, splits);
+  c.us = c.plan.us;
   if (!c.dma && packing && p.k > 0 && c.plan.tile != TILE_ROWS) {
     const long long copies = (da ? 0 : packed_bytes(q.a, size)) + (db ? 0 : packed_bytes(q.b, size));
     const auto fits = [&](const Operand &o) { return 256 * packed_ld(o, size) * size + 1024 < (1L << 31); };
-    const Plan fast = plan_product(p.m, p.n, p.k, q.type, q.a.mn, q.b.mn, true, tile, splits);
-    if (fits(q.a) && fits(q.b) && ((tile && tile != TILE_64 && tile != TILE_ROWS) || fast.us + 4 + 2 * copies / 4e6 < c.plan.us)) {
+    const Plan fast = plan_product(p.m, p.n, p.k, q.type, p.terms, q.a.mn, q.b.mn, true, tile, splits);
+    const double us = fast.us + 4 + 2 * copies / 4e6;
+    if (fits(q.a) && fits(q.b) && ((tile && tile != TILE_64 && tile != TILE_ROWS) || us < c.us)) {
       c.plan = fast;
+      c.us = us;
       c.dma = true;
       c.pack_a = !da;
       c.pack_b = !db;
@@ -289,6 +309,17 @@ void place(Product &q, const Plan &plan, void *parts) {
   p.parts = static_cast<float *>(parts);
 }
 
+// The operand becomes its aligned copy at `to`, one more of `pack`; the copy's bytes.
+long long copy_of(Operand &o, int size, char *to, PackParams &pack) {
+  const int i = pack.pieces[0] ? 1 : 0;
+  const long ld = packed_ld(o, size);
+  const long long bytes = packed_bytes(o, size);
+  pack.from[i] = o.p, pack.from_ld[i] = o.ld, pack.rows[i] = o.lines, pack.columns[i] = static_cast<int>(o.length);
+  pack.to[i] = to, pack.to_ld[i] = ld, pack.pieces[i] = o.lines * ld * size / 16;
+  o.p = to, o.ld = ld, o.ours = true;
+  return bytes;
+}
+
 hipError_t run_product(Product &q, int tile, int splits, void *workspace, long long bytes, hipStream_t stream) {
   const int size = size_of(q.type);
   Choice c = choose(q, tile, splits);
@@ -296,17 +327,9 @@ hipError_t run_product(Product &q, int tile, int splits, void *workspace, long l
   hipError_t e = hipSuccess;
   if (c.pack_a || c.pack_b) {
     char *to = static_cast<char *>(workspace) + c.parts;
-    PackParams pack{};
-    int i = 0;
-    for (Operand *o : {&q.a, &q.b}) {
-      if (!(o == &q.a ? c.pack_a : c.pack_b)) continue;
-      const long ld = packed_ld(*o, size);
-      pack.from[i] = o->p, pack.from_ld[i] = o->ld, pack.rows[i] = o->lines, pack.columns[i] = static_cast<int>(o->length);
-      pack.to[i] = to, pack.to_ld[i] = ld, pack.pieces[i] = o->lines * ld * size / 16;
-      to += packed_bytes(*o, size);
-      o->p = pack.to[i], o->ld = ld, o->ours = true;
-      ++i;
-    }
+    PackParams pack;
+    if (c.pack_a) to += copy_of(q.a, size, to, pack);
+    if (c.pack_b) copy_of(q.b, size, to, pack);
     e = launch_pack(pack, size, stream);
     if (e != hipSuccess) return e;
   }
@@ -383,13 +406,40 @@ int linear(const tf_linear_args_t *a, hipStream_t stream) {
 // How a gradient runs: the workspace's parts and the products.
 struct GradPlan {
   bool own_dz = false;   // dz lies in the workspace: an activation's, or an aligned copy of dy
-  bool pair = false;     // both products in one launch
   int terms = 1;         // of dz
-  long dz_ld = 0;
+  int rows = 0;          // of a workgroup of dz
+  long dz_ld = 0, count = 1;                  // shares of the bias gradient
   long long dz = 0, shares = 0, product = 0;  // bytes
+  bool pair = false;                          // both products in one launch, in these ranges of k,
+  int dx_splits = 1, dw_splits = 1;           // and of `product`, the bytes of
+  long long copies = 0, dx_parts = 0;         // aligned copies of w and x, and dx's parts
   Product dx, dw;
   long long bytes() const { return dz + shares + product; }
 };
+
+// Both products on 64 x 64 tiles in one launch: the aligned copies of x and w come with
+// dz, one more launch joins the ranges of k of both.  Predicted as predicted() does,
+// two workgroups on a CU; us.  The time of what it finds, and the ranges in `g`.
+double plan_pair(GradPlan &g) {
+  const GemmParams &dx = g.dx.p, &dw = g.dw.p;
+  const double t1 = static_cast<double>(ceil_div(dx.m, 64)) * ceil_div(dx.n, 64);
+  const double t2 = static_cast<double>(ceil_div(dw.m, 64)) * ceil_div(dw.n, 64);
+  double best = 1e30;
+  if (t1 + t2 > 2048) return best;
+  const double slabs1 = ceil_div(dx.k, 64), slabs2 = ceil_div(dw.k, 64), all = t1 * slabs1 + t2 * slabs2;
+  for (int s1 = 1; s1 == 1 || s1 * 2 <= slabs1; s1 *= 2) {
+    for (int s2 = 1; s2 == 1 || s2 * 2 <= slabs2; s2 *= 2) {
+      const double w = (t1 * s1 + t2 * s2) / 256;
+      if (s1 > 16 || s2 > 16 || (w > 4 && s1 * s2 > 1)) break;
+      const double longest = std::max(std::ceil(slabs1 / s1), std::ceil(slabs2 / s2));
+      double us = 4.3 + 2 * std::max(0.0, std::ceil(w / 2) - 1) + g.terms * std::max(longest * (w <= 1 ? 0.29 : 0.38), all * 0.19 / 256);
+      const double parts = (s1 > 1 ? s1 * static_cast<double>(dx.m) * dx.n : 0) + (s2 > 1 ? s2 * static_cast<double>(dw.m) * dw.n : 0);
+      if (parts > 0) us += 3.3 + 8 * parts / 7e6;
+      if (us < best) best = us, g.dx_splits = s1, g.dw_splits = s2;
+    }
+  }
+  return best;
+}
 
 // Up to this many multiply-adds a product of the rounded dz is not taken alone:
 // what the rounding left goes in as a second term, into the same float sums.  A
@@ -405,10 +455,19 @@ GradPlan plan_grad(const tf_linear_grad_args_t *a) {
   const bool smooth = a->act == TF_ACT_GELU || a->act == TF_ACT_SILU;
   g.dz_ld = n <= 64 ? ceil_div(n, 8) * 8 : ceil_div(n, 64) * 64;
   const Operand dy{a->dy, a->dy_ld, m, n, false, false};
-  g.own_dz = m && (a->act != TF_ACT_NONE || (!direct_loads(dy, 2) && m > 64 && work > 1e6));
+  const auto lay = [&](bool own, int rows) {
+    g.own_dz = own;
+    g.dz = own ? round16(2 * a->m * g.dz_ld) * g.terms : 0;
+    g.rows = rows;
+    g.count = ceil_div(m, rows);
+    g.shares = a->dbias && g.count > 1 ? round16(4 * g.count * a->n) : 0;
+  };
   g.terms = smooth && work <= kTwoTerms ? 2 : 1;
-  if (g.own_dz) g.dz = round16(2 * a->m * g.dz_ld) * g.terms;
-  if (a->dbias && m && column_shares(m) > 1) g.shares = round16(4 * column_shares(m) * a->n);
+  const bool odd = !direct_loads(dy, 2);
+  // A workgroup of dz takes all of up to 256 rows where that spares the bias gradient a
+  // second launch; else 64, or 32 where that leaves CUs without work.
+  lay(m && (a->act != TF_ACT_NONE || (odd && m > 64 && work > 1e6)),
+      a->dbias && m <= SLOPE_WHOLE ? SLOPE_WHOLE : ceil_div(m, 64) * ceil_div(n, 256) < 512 ? SLOPE_FEW : SLOPE_MANY);
   if (k == 0) return g;
   const bool nk = a->w_order == 1;
   const auto dz = [&](bool mn) {
@@ -423,18 +482,27 @@ GradPlan plan_grad(const tf_linear_grad_args_t *a) {
     g.dx.p.terms = g.dw.p.terms = 2;
     g.dx.p.a_term = (nk ? g.dw.p.a_term : g.dw.p.b_term) = g.dz / 2;
   }
-  const bool free = !a->tile && !a->splits;
-  // One launch for both where neither fills the GPU and k is short on both sides.
-  if (free && a->dx && a->dw && m && direct_loads(g.dx.a, 2) && direct_loads(g.dx.b, 2) && direct_loads(g.dw.a, 2) &&
-      direct_loads(g.dw.b, 2)) {
-    const long tiles = ceil_div(m, 64) * ceil_div(k, 64) + ceil_div(g.dw.p.m, 64) * ceil_div(g.dw.p.n, 64);
-    g.pair = tiles <= 512 && m <= 512 && n <= 512;
+  double apart = g.shares ? 5 : 1;  // the sum's launch, or a gap between two
+  if (a->dx && m) {
+    const Choice c = choose(g.dx, a->tile, a->splits);
+    g.product = c.bytes(), apart += c.us;
   }
-  if (g.pair) return g;
-  // Two terms run on the tiles that know them.
-  const int tile = g.terms == 2 ? (a->tile == TILE_128 ? TILE_128 : TILE_64) : a->tile;
-  if (a->dx && m) g.product = choose(g.dx, tile, a->splits).bytes();
-  if (a->dw) g.product = std::max(g.product, choose(g.dw, tile, a->splits).bytes());
+  if (a->dw) {
+    const Choice c = choose(g.dw, a->tile, a->splits);
+    g.product = std::max(g.product, c.bytes()), apart += c.us;
+  }
+  if (a->tile || a->splits || !a->dx || !a->dw || !m) return g;
+  // One launch for both where it takes less.
+  const long long copies = (direct_loads(g.dx.b, 2) ? 0 : packed_bytes(g.dx.b, 2)) + (direct_loads(x, 2) ? 0 : packed_bytes(x, 2));
+  const bool more = !g.own_dz && !a->dbias && (odd || copies);  // a launch for the copies alone
+  if (plan_pair(g) + (more ? 4 : 0) + 2 * copies / 4e6 > apart) return g;
+  g.pair = true;
+  lay(a->act != TF_ACT_NONE || odd, SLOPE_FEW);
+  g.dx.a = dz(false);
+  (nk ? g.dw.a : g.dw.b) = dz(true);
+  g.copies = copies;
+  g.dx_parts = part_bytes(m, k, {TILE_64, g.dx_splits, 0});
+  g.product = copies + g.dx_parts + part_bytes(g.dw.p.m, g.dw.p.n, {TILE_64, g.dw_splits, 0});
   return g;
 }
 
@@ -480,36 +548,50 @@ int linear_grad(const tf_linear_grad_args_t *a, hipStream_t stream) {
   float *shares = reinterpret_cast<float *>(ws + g.dz);
   void *rest = ws + g.dz + g.shares;
   const int m = static_cast<int>(a->m), n = static_cast<int>(a->n), k = static_cast<int>(a->k);
+  char *const parts = static_cast<char *>(rest) + g.copies;
   hipError_t e = hipSuccess;
+  PackParams pack;
+  if (g.copies) {
+    Operand &w = g.dx.b, &x = a->w_order ? g.dw.b : g.dw.a;
+    char *to = static_cast<char *>(rest);
+    if (!direct_loads(w, 2)) to += copy_of(w, 2, to, pack);
+    if (!direct_loads(x, 2)) copy_of(x, 2, to, pack);
+  }
   if (m && n && (g.own_dz || a->dbias)) {
     SlopeParams s{};
+    s.rows = g.rows;
     s.dy = a->dy, s.z = a->z, s.dy_ld = a->dy_ld, s.z_ld = a->z_ld, s.m = m, s.n = n, s.act = a->act;
     if (g.own_dz) s.dz = ws, s.dz_ld = g.dz_ld, s.lo = g.terms == 2 ? g.dz / 4 : 0;
     if (a->dbias && g.shares) s.shares = shares;
     if (a->dbias && !g.shares) s.sums = a->dbias, s.sums_type = a->bias_type;
-    e = launch_act_slope(s, a->type, stream);
+    e = launch_act_slope(s, pack, a->type, stream);
+  } else if (g.copies) {
+    e = launch_pack(pack, 2, stream);
   }
-  if (e == hipSuccess && a->dbias && n && (g.shares || !m))
-    e = launch_share_sum(shares, m ? column_shares(m) : 0, n, a->dbias, a->bias_type, stream);
+  if (e == hipSuccess && a->dbias && n && ((g.shares && !g.pair) || !m))
+    e = launch_share_sum(shares, m ? g.count : 0, n, a->dbias, a->bias_type, stream);
   if (e != hipSuccess || !k) return hip(e, call);
   if (g.own_dz) g.dx.a.p = (a->w_order ? g.dw.a.p : g.dw.b.p) = ws;
   if (g.pair) {
-    place(g.dx, {TILE_64, 1, 0}, nullptr);
-    place(g.dw, {TILE_64, 1, 0}, nullptr);
-    return hip(a->type == TF_T_BF16 ? launch_gemm_pair_bf16(g.dx.p, g.dx.b.mn, g.dw.p, stream)
-                                    : launch_gemm_pair_f16(g.dx.p, g.dx.b.mn, g.dw.p, stream), call);
+    place(g.dx, {TILE_64, g.dx_splits, 0}, parts);
+    place(g.dw, {TILE_64, g.dw_splits, 0}, parts + g.dx_parts);
+    ShareParams sum;
+    if (g.shares) sum = {shares, a->dbias, static_cast<int>(g.count), n, a->bias_type};
+    e = a->type == TF_T_BF16 ? launch_gemm_pair_bf16(g.dx.p, g.dx.b.mn, g.dw.p, sum, stream)
+                             : launch_gemm_pair_f16(g.dx.p, g.dx.b.mn, g.dw.p, sum, stream);
+    if (e == hipSuccess && g.dx_splits * g.dw_splits > 1) e = launch_gemm_join_pair(g.dx.p, g.dw.p, a->type, stream);
+    return hip(e, call);
   }
-  const int tile = g.terms == 2 ? (a->tile == TILE_128 ? TILE_128 : TILE_64) : a->tile;
   if (a->dx && m) {
     if (n) {
-      e = run_product(g.dx, tile, a->splits, rest, g.product, stream);
+      e = run_product(g.dx, a->tile, a->splits, rest, g.product, stream);
     } else {  // a sum of nothing
       Product q{a->type, a->type, {}, {}, {}};
       q.p.m = m, q.p.n = k, q.p.out = a->dx, q.p.ldo = a->dx_ld;
       e = run_product(q, 0, 1, nullptr, 0, stream);
     }
   }
-  if (e == hipSuccess && a->dw && n) e = run_product(g.dw, tile, a->splits, rest, g.product, stream);
+  if (e == hipSuccess && a->dw && n) e = run_product(g.dw, a->tile, a->splits, rest, g.product, stream);
   return hip(e, call);
 }
 

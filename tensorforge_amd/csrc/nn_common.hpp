@@ -159,6 +159,43 @@ __device__ __forceinline__ float wave_max(float v) {
   return v;
 }
 
+// The shares' sum, in order: 16 columns a workgroup of 256, 4 threads of four columns by
+// 64 rows of shares.  Bound by latency: 16 loads in flight a thread.
+__device__ __forceinline__ void share_sum(const float *shares, int count, int d, void *out, int type, int block, float (*part)[17]) {
+  const int c = block * 16 + threadIdx.x % 4 * 4, lane = threadIdx.x / 4;
+  f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
+  if (c + 4 <= d) {
+    const float *p = shares + c;
+    for (int q = lane; q < count; q += 1024) {
+      f32x4 v[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (q + i * 64 < count) v[i] = *reinterpret_cast<const Vec<float, 4>::loose *>(p + static_cast<long>(q + i * 64) * d);
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (q + i * 64 < count) s += v[i];
+    }
+  } else {
+    for (int q = lane; q < count; q += 64)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (c + i < d) s[i] += shares[static_cast<long>(q) * d + c + i];
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) part[lane][threadIdx.x % 4 * 4 + i] = s[i];
+  __syncthreads();
+  if (threadIdx.x < 64) {
+    // 4 threads a column, 16 rows each, joined in lane order.
+    const int col = threadIdx.x / 4, at = block * 16 + col;
+    float v = 0.0f;
+#pragma unroll
+    for (int q = 0; q < 16; ++q) v += part[threadIdx.x % 4 * 16 + q][col];
+    v += __shfl_xor(v, 1);
+    v += __shfl_xor(v, 2);
+    if (threadIdx.x % 4 == 0 && at < d) store_as(out, type, at, v);
+  }
+}
+
 // The 8-bit code's scale: the row's largest magnitude over 448, taken as at
 // least 2^-100 so that a row of zeros keeps a finite factor.
 constexpr float kF8Max = 448.0f;

@@ -303,7 +303,7 @@ __device__ __forceinline__ void with_act(int act, F &&f) {
 // the four of quad c in row r at place c ^ (r mod COLS/4).  The blocks come a
 // few columns of many rows at a time; from LDS a row's lanes write whole cache
 // lines (and read the residual's).  Straight from the blocks, in 16-byte parts of
-// rows, the output's write took longer than half the product at 8192^3.
+// rows, the whole product took a twelfth longer at 8192^3 (883 us, 815 this way).
 template <int COLS>
 __device__ __forceinline__ uint32_t patch_at(int row, int quad) {
   return row * (COLS * 4) + ((quad ^ (row & (COLS / 4 - 1))) << 4);
@@ -529,15 +529,18 @@ __global__ __launch_bounds__(64 * WM *WN) void gemm_tile_kernel(GemmParams p) {
 
 // A small layer's two gradient products in one launch: dx (its left operand along
 // k) by the first `first` workgroups, dw (both along their own dimensions) by the
-// others.
+// next `second`, the bias gradient's sum by the others.
 template <typename T, bool BMN>
-__global__ __launch_bounds__(256) void gemm_pair_kernel(GemmParams dx, GemmParams dw, int first) {
+__global__ __launch_bounds__(256) void gemm_pair_kernel(GemmParams dx, GemmParams dw, ShareParams sum, int first, int second) {
   constexpr int ST = 4;
   __shared__ __align__(1024) char smem[tile_lds<64, 64, ST>()];
-  if (static_cast<int>(blockIdx.x) < first)
-    gemm_tile<T, T, false, BMN, 64, 64, 2, 2, ST, true>(dx, blockIdx.x, first, (lds_char *)smem);
+  const int block = blockIdx.x;
+  if (block < first)
+    gemm_tile<T, T, false, BMN, 64, 64, 2, 2, ST, true>(dx, block, first, (lds_char *)smem);
+  else if (block < first + second)
+    gemm_tile<T, T, true, true, 64, 64, 2, 2, ST, true>(dw, block - first, second, (lds_char *)smem);
   else
-    gemm_tile<T, T, true, true, 64, 64, 2, 2, ST, true>(dw, blockIdx.x - first, gridDim.x - first, (lds_char *)smem);
+    share_sum(sum.shares, sum.count, sum.d, sum.out, sum.type, block - first - second, reinterpret_cast<float (*)[17]>(smem));
 }
 
 // ---- few rows -----------------------------------------------------------------
@@ -553,7 +556,8 @@ constexpr int rows_waves(bool bmn, int mi) { return bmn && mi > 1 ? 8 : 16; }
 // with piece c of line k at c ^ (k & 2).  The left operand's pieces come from the
 // caches.  Any alignment.  The last workgroup's columns are moved back into the
 // matrix (n >= 32 where the right operand lies along n) and a last part of a slab
-// is read apart, so the loads on the way are unguarded.
+// is read apart, so the loads on the way are unguarded.  A left operand of two
+// terms takes twice the blocks of rows, joined with the waves' sums.
 template <typename T, typename O, bool BMN, int MI>
 __global__ __launch_bounds__(64 * rows_waves(BMN, MI)) void gemm_rows_kernel(GemmParams p) {
   constexpr int NB = BMN ? 2 : 1, NW = rows_waves(BMN, MI), WP = BMN ? 4 : 2;  // pieces a lane of one slab of B
@@ -568,8 +572,10 @@ __global__ __launch_bounds__(64 * rows_waves(BMN, MI)) void gemm_rows_kernel(Gem
   const int slabs = p.k / kSlab<T>;  // whole ones
   const T *a[MI];
 #pragma unroll
-  for (int i = 0; i < MI; ++i)  // rows past the last repeat it; their results are not written
-    a[i] = static_cast<const T *>(p.a) + min(i * 16 + l, p.m - 1) * p.lda;
+  for (int i = 0; i < MI; ++i) {  // rows past the last repeat it; their results are not written
+    const int term = MI > 1 && p.terms == 2 && i >= MI / 2, row = (i - (term ? MI / 2 : 0)) * 16 + l;
+    a[i] = reinterpret_cast<const T *>(static_cast<const char *>(p.a) + term * p.a_term) + min(row, p.m - 1) * p.lda;
+  }
   const T *b = static_cast<const T *>(p.b);
   if constexpr (BMN) b += (lane / 4) * p.ldb + n0 + lane % 4 * 8;
   else b += min(n0 + l, p.n - 1) * p.ldb;
@@ -668,10 +674,15 @@ __global__ __launch_bounds__(64 * rows_waves(BMN, MI)) void gemm_rows_kernel(Gem
     for (int j = 0; j < NB; ++j) join[(wave * MI * NB + i * NB + j) * 64 + lane] = acc[i][j];
   __syncthreads();
   const int block = wave;
-  if (block >= MI * NB) return;
+  const int blocks = MI > 1 && p.terms == 2 ? MI / 2 * NB : MI * NB;
+  if (block >= blocks) return;
   f32x4 v = join[block * 64 + lane];
 #pragma unroll
   for (int w = 1; w < NW; ++w) v += join[(w * MI * NB + block) * 64 + lane];
+  if (blocks < MI * NB) {
+#pragma unroll
+    for (int w = 0; w < NW; ++w) v += join[(w * MI * NB + blocks + block) * 64 + lane];
+  }
   const int m = block / NB * 16 + l, n = n0 + block % NB * 16 + g * 4;
   if (m >= p.m || n >= p.n || n + 3 < nt) return;
   float out[4], bias[4];

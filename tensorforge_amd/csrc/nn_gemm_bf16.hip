@@ -9,8 +9,8 @@ hipError_t launch_gemm_bf16(const GemmParams &p, bool amn, bool bmn, int tile, b
   return launch_layout<bf16, bf16, false, false>(p, tile, dma, stream);
 }
 
-hipError_t launch_gemm_pair_bf16(const GemmParams &dx, bool bmn, const GemmParams &dw, hipStream_t stream) {
-  return launch_pair<bf16>(dx, bmn, dw, stream);
+hipError_t launch_gemm_pair_bf16(const GemmParams &dx, bool bmn, const GemmParams &dw, const ShareParams &sum, hipStream_t stream) {
+  return launch_pair<bf16>(dx, bmn, dw, sum, stream);
 }
 
 }  // namespace tfnn

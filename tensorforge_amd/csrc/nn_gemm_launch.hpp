@@ -12,8 +12,8 @@ hipError_t launch_layout(const GemmParams &p, int tile, bool dma, hipStream_t st
   if constexpr (!AMN) {
     if (tile == TILE_ROWS) {
       const dim3 grid(static_cast<unsigned>((p.n + (BMN ? 31 : 15)) / (BMN ? 32 : 16)));
-      if (p.m <= 16) gemm_rows_kernel<T, O, BMN, 1><<<grid, 64 * rows_waves(BMN, 1), 0, stream>>>(p);
-      else if (p.m <= 32) gemm_rows_kernel<T, O, BMN, 2><<<grid, 64 * rows_waves(BMN, 2), 0, stream>>>(p);
+      if ((p.m + 15) / 16 * p.terms <= 1) gemm_rows_kernel<T, O, BMN, 1><<<grid, 64 * rows_waves(BMN, 1), 0, stream>>>(p);
+      else if ((p.m + 15) / 16 * p.terms <= 2) gemm_rows_kernel<T, O, BMN, 2><<<grid, 64 * rows_waves(BMN, 2), 0, stream>>>(p);
       else gemm_rows_kernel<T, O, BMN, 4><<<grid, 64 * rows_waves(BMN, 4), 0, stream>>>(p);
       return hipGetLastError();
     }
@@ -35,11 +35,11 @@ hipError_t launch_layout(const GemmParams &p, int tile, bool dma, hipStream_t st
 }
 
 template <typename T>
-hipError_t launch_pair(const GemmParams &dx, bool bmn, const GemmParams &dw, hipStream_t stream) {
-  const int first = dx.tiles_m * dx.tiles_n;
-  const dim3 grid(static_cast<unsigned>(first + dw.tiles_m * dw.tiles_n));
-  if (bmn) gemm_pair_kernel<T, true><<<grid, 256, 0, stream>>>(dx, dw, first);
-  else gemm_pair_kernel<T, false><<<grid, 256, 0, stream>>>(dx, dw, first);
+hipError_t launch_pair(const GemmParams &dx, bool bmn, const GemmParams &dw, const ShareParams &sum, hipStream_t stream) {
+  const int first = dx.tiles_m * dx.tiles_n * dx.splits, second = dw.tiles_m * dw.tiles_n * dw.splits;
+  const dim3 grid(static_cast<unsigned>(first + second + (sum.d + 15) / 16));
+  if (bmn) gemm_pair_kernel<T, true><<<grid, 256, 0, stream>>>(dx, dw, sum, first, second);
+  else gemm_pair_kernel<T, false><<<grid, 256, 0, stream>>>(dx, dw, sum, first, second);
   return hipGetLastError();
 }
 

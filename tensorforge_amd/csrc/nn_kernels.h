@@ -40,7 +40,7 @@ struct GemmParams {
   int tiles_m = 0, tiles_n = 0, splits = 1;
   int act = 0, bias_f32 = 0;
   int terms = 1;                // 2: a second term of A at a + a_term, or of B at b + b_term (bytes)
-  long a_term = 0, b_term = 0;  // (64 and 128 tiles)
+  long a_term = 0, b_term = 0;  // (all tiles but 256; few rows: of A, up to 32 rows)
 };
 
 // C tiles of the product kernels; but for 64 x 64 they load straight into LDS only.
@@ -54,36 +54,45 @@ constexpr int tile_columns(int tile) { return tile == TILE_64x128 ? 128 : tile_r
 hipError_t launch_gemm_bf16(const GemmParams &p, bool amn, bool bmn, int tile, bool dma, hipStream_t stream);
 hipError_t launch_gemm_f16(const GemmParams &p, bool amn, bool bmn, int tile, bool dma, hipStream_t stream);
 hipError_t launch_gemm_f8(const GemmParams &p, int out_type, int tile, bool dma, hipStream_t stream);
+// A sum of `count` shares of d floats, rounded to `type`; d = 0: none.
+struct ShareParams {
+  const float *shares = nullptr;
+  void *out = nullptr;
+  int count = 0, d = 0, type = 0;
+};
 // Both products of a small layer's gradient in one launch, 64 x 64 tiles, loads
-// straight into LDS: dx with amn false, dw with amn and bmn true.
-hipError_t launch_gemm_pair_bf16(const GemmParams &dx, bool bmn, const GemmParams &dw, hipStream_t stream);
-hipError_t launch_gemm_pair_f16(const GemmParams &dx, bool bmn, const GemmParams &dw, hipStream_t stream);
+// straight into LDS: dx with amn false, dw with amn and bmn true; and a sum.
+hipError_t launch_gemm_pair_bf16(const GemmParams &dx, bool bmn, const GemmParams &dw, const ShareParams &sum, hipStream_t stream);
+hipError_t launch_gemm_pair_f16(const GemmParams &dx, bool bmn, const GemmParams &dw, const ShareParams &sum, hipStream_t stream);
 
 // Up to two matrices copied to rows of whole 16-byte pieces, zeros in the pad.
 struct PackParams {
-  const void *from[2];
-  void *to[2];
-  long from_ld[2], to_ld[2], rows[2];  // elements
-  int columns[2];
-  long pieces[2];  // rows x to_ld in pieces; 0: none
+  const void *from[2] = {};
+  void *to[2] = {};
+  long from_ld[2] = {}, to_ld[2] = {}, rows[2] = {};  // elements
+  int columns[2] = {};
+  long pieces[2] = {};  // rows x to_ld in pieces; 0: none
 };
 hipError_t launch_pack(const PackParams &p, int size, hipStream_t stream);
 
 // out = epilogue(sum of the splits' parts).
 hipError_t launch_gemm_join(const GemmParams &p, int out_type, hipStream_t stream);
+// The same of a pair's products, those that are split.
+hipError_t launch_gemm_join_pair(const GemmParams &dx, const GemmParams &dw, int out_type, hipStream_t stream);
 
 struct SlopeParams {
   const void *dy, *z;
   void *dz;       // m x dz_ld, columns from n on zero; null: sums alone
   long lo;        // not 0: what dz's rounding left, rounded, that many elements behind
-  float *shares;  // column_shares(m) x n; null with one share, or without sums
-  void *sums;     // with column_shares(m) = 1, the sums themselves, of sums_type; else null
+  float *shares;  // ceil(m / rows) x n; null with one share, or without sums
+  void *sums;     // with one share, the sums themselves, of sums_type; else null
   long dy_ld, z_ld, dz_ld;
   int m, n, act, sums_type;
+  int rows;  // a workgroup's: one of SlopeRows
 };
-// dz = dy * act'(z) (act none: dy), and dz's column sums.
-long column_shares(long m);
-hipError_t launch_act_slope(const SlopeParams &p, int type, hipStream_t stream);
+enum SlopeRows { SLOPE_FEW = 32, SLOPE_MANY = 64, SLOPE_WHOLE = 256 };
+// dz = dy * act'(z) (act none: dy), and dz's column sums; beside them the copies of `pack`.
+hipError_t launch_act_slope(const SlopeParams &p, const PackParams &pack, int type, hipStream_t stream);
 // out[0..d) = sum of `count` shares, in order, rounded to `type`.
 hipError_t launch_share_sum(const float *shares, long count, int d, void *out, int type, hipStream_t stream);
 

@@ -10,12 +10,13 @@ namespace {
 
 // Four columns a thread: the parts' sum in order, then the tile kernels' epilogue.
 template <typename O, int ACT>
-__global__ __launch_bounds__(256) void gemm_join_kernel(GemmParams p) {
-  const long ld = (p.n + 3) & ~3, id = static_cast<long>(blockIdx.x) * 256 + threadIdx.x;
+__device__ __forceinline__ void join_four(const GemmParams &p, int block) {
+  const long ld = (p.n + 3) & ~3, id = static_cast<long>(block) * 256 + threadIdx.x;
   const int m = static_cast<int>(id / (ld / 4)), n = static_cast<int>(id % (ld / 4)) * 4;
   if (m >= p.m) return;
   const float *part = p.parts + m * ld + n;
   f32x4 sum = *reinterpret_cast<const f32x4 *>(part);
+#pragma unroll 4
   for (int s = 1; s < p.splits; ++s) sum += *reinterpret_cast<const f32x4 *>(part + s * (p.m * ld));
   float v[4] = {sum.x, sum.y, sum.z, sum.w}, bias[4];
   if (p.sa) {
@@ -27,11 +28,24 @@ __global__ __launch_bounds__(256) void gemm_join_kernel(GemmParams p) {
   load_bias<O>(p, n, bias);
   finish<O, ACT>(p, m, n, v, bias);
 }
+template <typename O, int ACT>
+__global__ __launch_bounds__(256) void gemm_join_kernel(GemmParams p) {
+  join_four<O, ACT>(p, blockIdx.x);
+}
+template <typename O>
+__global__ __launch_bounds__(256) void gemm_join_pair_kernel(GemmParams dx, GemmParams dw, int first) {
+  const int block = blockIdx.x;
+  if (block < first) join_four<O, ACT_NONE>(dx, block);
+  else join_four<O, ACT_NONE>(dw, block - first);
+}
+
+unsigned join_blocks(const GemmParams &p) {
+  return static_cast<unsigned>((static_cast<long>(p.m) * ((p.n + 3) / 4) + 255) / 256);
+}
 
 template <typename O>
 void join(const GemmParams &p, hipStream_t stream) {
-  const long threads = static_cast<long>(p.m) * ((p.n + 3) / 4);
-  const dim3 grid(static_cast<unsigned>((threads + 255) / 256));
+  const dim3 grid(join_blocks(p));
   if (p.act == ACT_RELU) gemm_join_kernel<O, ACT_RELU><<<grid, 256, 0, stream>>>(p);
   else if (p.act == ACT_GELU) gemm_join_kernel<O, ACT_GELU><<<grid, 256, 0, stream>>>(p);
   else if (p.act == ACT_SILU) gemm_join_kernel<O, ACT_SILU><<<grid, 256, 0, stream>>>(p);
@@ -39,9 +53,9 @@ void join(const GemmParams &p, hipStream_t stream) {
 }
 
 template <typename T>
-__global__ __launch_bounds__(256) void pack_kernel(PackParams p) {
+__device__ __forceinline__ void pack_piece(const PackParams &p, int block) {
   constexpr int N = kPiece<T>;
-  long id = static_cast<long>(blockIdx.x) * 256 + threadIdx.x;
+  long id = static_cast<long>(block) * 256 + threadIdx.x;
   const int q = id >= p.pieces[0];
   if (q) id -= p.pieces[0];
   if (id >= p.pieces[q]) return;
@@ -50,17 +64,30 @@ __global__ __launch_bounds__(256) void pack_kernel(PackParams p) {
   const i32x4 v = load_piece_any(static_cast<const T *>(p.from[q]) + row * p.from_ld[q], c, p.columns[q]);
   *reinterpret_cast<i32x4 *>(static_cast<T *>(p.to[q]) + row * p.to_ld[q] + c) = v;
 }
+template <typename T>
+__global__ __launch_bounds__(256) void pack_kernel(PackParams p) {
+  pack_piece<T>(p, blockIdx.x);
+}
+unsigned pack_blocks(const PackParams &p) { return static_cast<unsigned>((p.pieces[0] + p.pieces[1] + 255) / 256); }
 
-// A workgroup of the slope takes 64 rows; with up to 512 rows, all of them, so
-// that the bias gradient needs no second launch.
-constexpr int kSlopeRows = 64, kSlopeWhole = 512;
+template <typename T>
+__device__ __forceinline__ void load_slope8(const T *row, int c, int n, float (&v)[8]) {
+  const auto u = __builtin_bit_cast(typename Vec<T, 8>::type, load_piece_any(row, c, n));
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = static_cast<float>(u[i]);
+}
 
-// 8 columns a thread; CT threads side by side, the others down the rows.
+// 8 columns a thread; CT threads side by side, the others down the workgroup's rows.
+// The workgroups from `blocks` on make copies.
 template <typename T, int ACT, int CT>
-__global__ __launch_bounds__(256) void act_slope_kernel(SlopeParams p, int rows) {
+__global__ __launch_bounds__(256) void act_slope_kernel(SlopeParams p, PackParams pack, int blocks) {
+  if (static_cast<int>(blockIdx.x) >= blocks) {
+    pack_piece<T>(pack, blockIdx.x - blocks);
+    return;
+  }
   constexpr int LANES = 256 / CT, COLS = CT * 8;
   const int column_blocks = (p.n + COLS - 1) / COLS, bc = blockIdx.x % column_blocks, br = blockIdx.x / column_blocks;
-  const int c = bc * COLS + threadIdx.x % CT * 8, lane = threadIdx.x / CT, left = p.n - c;
+  const int c = bc * COLS + threadIdx.x % CT * 8, lane = threadIdx.x / CT, left = p.n - c, rows = p.rows;
   const long row0 = static_cast<long>(br) * rows;
   float sum[8];
 #pragma unroll
@@ -71,9 +98,9 @@ __global__ __launch_bounds__(256) void act_slope_kernel(SlopeParams p, int rows)
     for (int r = lane; r < end; r += LANES) {
       const long row = row0 + r;
       float g[8], z[8];
-      load_some(static_cast<const T *>(p.dy) + row * p.dy_ld + c, left, g);
+      load_slope8(static_cast<const T *>(p.dy) + row * p.dy_ld, c, p.n, g);
       if constexpr (ACT != ACT_NONE) {
-        load_some(static_cast<const T *>(p.z) + row * p.z_ld + c, left, z);
+        load_slope8(static_cast<const T *>(p.z) + row * p.z_ld, c, p.n, z);
 #pragma unroll
         for (int i = 0; i < 8; ++i) g[i] *= act_slope<ACT>(z[i]);
       }
@@ -108,27 +135,27 @@ __global__ __launch_bounds__(256) void act_slope_kernel(SlopeParams p, int rows)
 }
 
 template <typename T, int ACT>
-void slope(const SlopeParams &p, hipStream_t stream) {
-  const long shares = column_shares(p.m);
-  // Few rows: narrow columns, more threads down each.
-  if (shares == 1) act_slope_kernel<T, ACT, 4><<<dim3((p.n + 31) / 32), 256, 0, stream>>>(p, kSlopeWhole);
-  else act_slope_kernel<T, ACT, 32><<<dim3(static_cast<unsigned>(shares * ((p.n + 255) / 256))), 256, 0, stream>>>(p, kSlopeRows);
+void slope(const SlopeParams &p, const PackParams &pack, hipStream_t stream) {
+  const int columns = p.rows == SLOPE_WHOLE ? 32 : p.rows == SLOPE_FEW ? 128 : 256;
+  const int blocks = (p.m + p.rows - 1) / p.rows * ((p.n + columns - 1) / columns);
+  const dim3 grid(blocks + pack_blocks(pack));
+  if (p.rows == SLOPE_WHOLE) act_slope_kernel<T, ACT, 4><<<grid, 256, 0, stream>>>(p, pack, blocks);
+  else if (p.rows == SLOPE_FEW) act_slope_kernel<T, ACT, 16><<<grid, 256, 0, stream>>>(p, pack, blocks);
+  else act_slope_kernel<T, ACT, 32><<<grid, 256, 0, stream>>>(p, pack, blocks);
 }
 
 template <typename T>
-void slope(const SlopeParams &p, hipStream_t stream) {
-  if (p.act == ACT_RELU) slope<T, ACT_RELU>(p, stream);
-  else if (p.act == ACT_GELU) slope<T, ACT_GELU>(p, stream);
-  else if (p.act == ACT_SILU) slope<T, ACT_SILU>(p, stream);
-  else slope<T, ACT_NONE>(p, stream);
+void slope(const SlopeParams &p, const PackParams &pack, hipStream_t stream) {
+  if (p.act == ACT_RELU) slope<T, ACT_RELU>(p, pack, stream);
+  else if (p.act == ACT_GELU) slope<T, ACT_GELU>(p, pack, stream);
+  else if (p.act == ACT_SILU) slope<T, ACT_SILU>(p, pack, stream);
+  else slope<T, ACT_NONE>(p, pack, stream);
 }
 
 }  // namespace
 
-long column_shares(long m) { return m <= kSlopeWhole ? 1 : (m + kSlopeRows - 1) / kSlopeRows; }
-
 hipError_t launch_pack(const PackParams &p, int size, hipStream_t stream) {
-  const dim3 grid(static_cast<unsigned>((p.pieces[0] + p.pieces[1] + 255) / 256));
+  const dim3 grid(pack_blocks(p));
   size == 1 ? pack_kernel<f8><<<grid, 256, 0, stream>>>(p) : pack_kernel<bf16><<<grid, 256, 0, stream>>>(p);
   return hipGetLastError();
 }
@@ -138,8 +165,15 @@ hipError_t launch_gemm_join(const GemmParams &p, int out_type, hipStream_t strea
   return hipGetLastError();
 }
 
-hipError_t launch_act_slope(const SlopeParams &p, int type, hipStream_t stream) {
-  type == TYPE_BF16 ? slope<bf16>(p, stream) : slope<f16>(p, stream);
+hipError_t launch_gemm_join_pair(const GemmParams &dx, const GemmParams &dw, int out_type, hipStream_t stream) {
+  const unsigned first = dx.splits > 1 ? join_blocks(dx) : 0, second = dw.splits > 1 ? join_blocks(dw) : 0;
+  if (out_type == TYPE_BF16) gemm_join_pair_kernel<bf16><<<dim3(first + second), 256, 0, stream>>>(dx, dw, first);
+  else gemm_join_pair_kernel<f16><<<dim3(first + second), 256, 0, stream>>>(dx, dw, first);
+  return hipGetLastError();
+}
+
+hipError_t launch_act_slope(const SlopeParams &p, const PackParams &pack, int type, hipStream_t stream) {
+  type == TYPE_BF16 ? slope<bf16>(p, pack, stream) : slope<f16>(p, pack, stream);
   return hipGetLastError();
 }
 

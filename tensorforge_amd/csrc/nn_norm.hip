@@ -345,42 +345,9 @@ __global__ __launch_bounds__(256) void rms_norm_grad_long_kernel(NormGradParams 
   }
 }
 
-// The shares' sum, in order: 16 columns a workgroup, 4 threads of four columns by
-// 64 rows of shares.  Bound by latency: 16 loads in flight a thread.
 __global__ __launch_bounds__(256) void share_sum_kernel(const float *shares, int count, int d, void *out, int type) {
-  const int c = blockIdx.x * 16 + threadIdx.x % 4 * 4, lane = threadIdx.x / 4;
-  f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
-  if (c + 4 <= d) {
-    const float *p = shares + c;
-    for (int q = lane; q < count; q += 1024) {
-      f32x4 v[16];
-#pragma unroll
-      for (int i = 0; i < 16; ++i)
-        if (q + i * 64 < count) v[i] = *reinterpret_cast<const Vec<float, 4>::loose *>(p + static_cast<long>(q + i * 64) * d);
-#pragma unroll
-      for (int i = 0; i < 16; ++i)
-        if (q + i * 64 < count) s += v[i];
-    }
-  } else {
-    for (int q = lane; q < count; q += 64)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (c + i < d) s[i] += shares[static_cast<long>(q) * d + c + i];
-  }
   __shared__ float part[64][17];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) part[lane][threadIdx.x % 4 * 4 + i] = s[i];
-  __syncthreads();
-  if (threadIdx.x < 64) {
-    // 4 threads a column, 16 rows each, joined in lane order.
-    const int col = threadIdx.x / 4, at = blockIdx.x * 16 + col;
-    float v = 0.0f;
-#pragma unroll
-    for (int q = 0; q < 16; ++q) v += part[threadIdx.x % 4 * 16 + q][col];
-    v += __shfl_xor(v, 1);
-    v += __shfl_xor(v, 2);
-    if (threadIdx.x % 4 == 0 && at < d) store_as(out, type, at, v);
-  }
+  share_sum(shares, count, d, out, type, blockIdx.x, part);
 }
 
 // Workgroups beyond this many would each take few rows for the weights they load.

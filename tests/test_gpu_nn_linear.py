@@ -182,6 +182,36 @@ def test_small_gradients_round_once(activation, dtype):
                 assert float((got.cpu().double() - want).norm()) <= 1.05 * float(own) + 4e-6 * float(want.norm()), (m, n, k)
 
 
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("order", [0, 1])
+@pytest.mark.parametrize("activation", ["none", "gelu"])
+def test_small_gradients_with_long_sums(activation, order, dtype):
+    """One side's sum is long and the other's results are few: ranges of k in the products' one launch, odd operands
+    copied beside dz, the bias gradient's shares added with the products."""
+    nn = _nn()
+    for m, n, k in ((2100, 141, 150), (17, 2071, 67), (33, 64, 1030), (1, 1216, 791), (300, 513, 72), (768, 256, 344)):
+        g = torch.Generator().manual_seed(m + n + k)
+        dy, x, w, z = (_matrix(g, *s, dtype) for s in ((m, n), (m, k), (k, n), (m, n)))
+        args = dy.cuda(), x.cuda(), _ordered(w, order), z.cuda() if activation != "none" else None, activation
+        _check_grad(nn.linear_grad(*args, bias_dtype=torch.float32), dy, x, w, z, activation, dtype, torch.float32)
+        dx, dw, _ = nn.linear_grad(*args)
+        assert torch.equal(dx, nn.linear_grad(*args)[0]) and torch.equal(dw, nn.linear_grad(*args)[1])
+
+
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("order", [0, 1])
+def test_few_rows_of_two_terms(order, dtype):
+    """dx of up to 32 rows on the few-row kernel: what dz's rounding leaves goes in as further rows."""
+    nn = _nn()
+    for m, n, k in ((1, 300, 200), (5, 1024, 96), (16, 129, 64), (17, 520, 131), (32, 264, 264), (33, 200, 64)):
+        g = torch.Generator().manual_seed(m + n)
+        dy, x, w, z = (_matrix(g, *s, dtype) for s in ((m, n), (m, k), (k, n), (m, n)))
+        dx, _, _ = nn.linear_grad(dy.cuda(), x.cuda(), _ordered(w, order), z.cuda(), "silu", want_dw=False, tile=4)
+        want = (dy.double() * ref.slope(z.double(), "silu")) @ w.double().t()
+        own = (want.to(dtype).double() - want).norm()
+        assert float((dx.cpu().double() - want).norm()) <= 1.05 * float(own) + 4e-6 * float(want.norm()), (m, n, k)
+
+
 @pytest.mark.parametrize("order", [0, 1])
 def test_large_ragged(order):
     """Sizes whose unaligned operands are copied to aligned rows first, in both directions."""
