@@ -164,6 +164,11 @@ bool direct_loads(const Operand &o, int size) {
   return o.ours || (reinterpret_cast<uintptr_t>(o.p) % 16 == 0 && o.ld % piece == 0 && o.length % piece == 0);
 }
 
+// Whether loads of these lines may start off four bytes.
+bool off_four(const Operand &o, int size) {
+  return reinterpret_cast<uintptr_t>(o.p) % 4 || o.ld * size % 4 || (o.mn && o.length * size % 4);
+}
+
 // The same operand copied to aligned lines: whole cache lines, so that no 128 bytes
 // of a tile's line lie in two.
 long packed_ld(const Operand &o, int size) { return ceil_div(o.length, 128 / size) * (128 / size); }
@@ -194,17 +199,18 @@ constexpr TileCost kCost256{1, 7.0, 3.5, 1.3, 1.03, 1.21, 1.12, 1.0, 1.1, 1.34, 
 constexpr TileCost kCost128{2, 5.5, 0.0, 0.57, 0.58, 0.78, 1.23, 0.78, 1.8, 1.56, 0.82};
 constexpr TileCost kCost64x128{2, 2.5, 1.9, 2.9, 0.38, 0.58, 1.1, 0.49, 2.4, 1.36, 0.28};
 constexpr TileCost kCost64{3, 3.6, 0.04, 0.58, 0.27, 0.56, 1.09, 0.6, 2.5, 1.74, 0.21};
+// Loads through registers (64 x 64), fitted to 200 products of odd sizes: within 6%.
+constexpr TileCost kCostAny{3, 3.9, 0.55, 3.0, 0.28, 0.92, 1.09, 0.2, 2.5, 1.74, 1.37};
 
 // Few slabs of LDS let five 64 x 64 tiles on a CU, from 768 on: 3.5, and a workgroup 0.46
-// and 0.22 a slab.  Loads through registers (64 x 64 only) take `loads` times the slabs' time, and
-// write past the others: 1856 x 7183 x 46 32 us against 14.2.  read: the operands' bytes at 8 TB/s.
-double predicted(double m, double n, double slabs, double read, double loads, bool dma, bool f8, int tile, int splits) {
-  const TileCost &c = tile == TILE_256 ? kCost256 : tile == TILE_128 ? kCost128 : tile == TILE_64 ? kCost64 : kCost64x128;
-  const double each = std::ceil(slabs / splits) * loads, results = m * n / 1e6, most = c.most;
+// and 0.22 a slab.  read: the operands' bytes at 8 TB/s.
+double predicted(double m, double n, double slabs, double read, bool dma, bool f8, int tile, int splits) {
+  const TileCost &c = !dma ? kCostAny : tile == TILE_256 ? kCost256 : tile == TILE_128 ? kCost128 : tile == TILE_64 ? kCost64 : kCost64x128;
+  const double each = std::ceil(slabs / splits), results = m * n / 1e6, most = c.most;
   const double w = std::ceil(m / tile_rows(tile)) * std::ceil(n / tile_columns(tile)) * splits / 256;  // workgroups a CU
   const double slab_most = f8 ? c.slab_most * c.f8 : c.slab_most;
   double us;
-  if (tile == TILE_64 && w > 3) {
+  if (dma && tile == TILE_64 && w > 3) {
     us = 3.5 + w * (0.46 + each * (f8 ? 0.22 * c.f8 : 0.22));
   } else {
     const double full = each * slab_most + c.end_most, rounds = std::floor(w / most), rest = w - rounds * most;
@@ -217,7 +223,7 @@ double predicted(double m, double n, double slabs, double read, double loads, bo
     }
   }
   us = std::max(us, 4.5 + read);
-  return splits > 1 ? us + c.join + c.join_part * splits * results : std::max(us, 4.5 + results * (dma ? c.written : 2.2));
+  return splits > 1 ? us + c.join + c.join_part * splits * results : std::max(us, 4.5 + results * c.written);
 }
 
 // The C tile and the ranges of k for a product of these sizes: the least
@@ -227,7 +233,12 @@ double predicted(double m, double n, double slabs, double read, double loads, bo
 // (few-row / 64-tile), w 4096 x 4096 as n rows of k: 7.7 / 10.8 for 1 row, 9.8 / 11.1
 // for 16, 13.7 / 11.6 for 32; as k rows of n: 11.4 / 11.6, 13.4 / 12.2, 16.1 / 12.5.
 // A left operand of two terms counts as twice the rows here, as twice the slabs on the tiles.
-Plan plan_product(long m, long n, long k, int type, int terms, bool amn, bool bmn, bool dma, int tile, int splits) {
+// Lines off four bytes take it longer (150 more): 5 x 4224 x 1022 5.3, x 1023 10.6 (8.1 on the
+// 64-tile); 4 x 5911 x 5281 40.8 and 21.8.
+Plan plan_product(const Product &q, bool dma, int tile, int splits) {
+  const long m = q.p.m, n = q.p.n, k = q.p.k;
+  const int type = q.type, terms = q.p.terms;
+  const bool amn = q.a.mn, bmn = q.b.mn;
   const int size = size_of(type);
   const long slabs = ceil_div(k, 128 / size);
   const bool rows = m * terms <= 64 && !amn && (!bmn || n >= 32);
@@ -235,12 +246,13 @@ Plan plan_product(long m, long n, long k, int type, int terms, bool amn, bool bm
   if (tile == TILE_ROWS || (!dma && tile != TILE_64) || (terms > 1 && tile == TILE_256)) tile = 0;
   splits = static_cast<int>(std::max<long>(0, std::min<long>(splits, std::max<long>(1, slabs))));
   Plan best{TILE_64, 1, 1e30};
-  const double loads = dma ? 1 : amn || bmn ? 3.2 : 2.2;
   const double read = (static_cast<double>(m) + n) * k * terms * size / 8e6;
   if (rows && !tile) {
     const long cols = bmn ? 32 : 16;
     const double bytes = static_cast<double>(k) * size / 1e3;
-    best = {TILE_ROWS, 1, 3.4 + std::max(read, ceil_div(ceil_div(n, cols), 256) * (cols / 110.0 + m * terms / 45.0) * bytes)};
+    const double of_b = cols / 110.0 * (!off_four(q.b, size) ? 1 : bmn ? 1.9 : 7.5);
+    const double of_a = m * terms / 45.0 * (off_four(q.a, size) ? 3.3 : 1);
+    best = {TILE_ROWS, 1, 3.4 + std::max(read, ceil_div(ceil_div(n, cols), 256) * (of_b + of_a) * bytes)};
   }
   for (int t : {TILE_64, TILE_64x128, TILE_128, TILE_256}) {
     if (tile ? t != tile : (t != TILE_64 && !dma) || (t == TILE_256 && terms > 1)) continue;
@@ -250,7 +262,7 @@ Plan plan_product(long m, long n, long k, int type, int terms, bool amn, bool bm
     for (int s : {1, 2, 3, 4, 6, 8, 12, 16}) {
       if (s > 1 && (splits || s * 2 > slabs || tiles * s > 1024)) break;
       const int ranges = splits ? splits : s;
-      const double us = predicted(m, n, slabs, read, loads * terms, dma, size == 1, t, ranges);
+      const double us = predicted(m, n, slabs * terms, read, dma, size == 1, t, ranges);
       if (us < best.us) best = {t, ranges, us};
     }
   }
@@ -263,8 +275,10 @@ long long part_bytes(long m, long n, const Plan &plan) {
 
 // How a product runs.  Operands that cannot be loaded straight into LDS are
 // copied to aligned lines first (pack) where the faster kernels gain more than the
-// copy takes, about 4 us and its bytes at 4 TB/s: 4095 x 4097 x 1023 bfloat16 110 us
-// through registers, 63 with both copied; 777 x 1111 x 333 8.3 and 13.
+// copy takes, about 3.7 us and 0.21 for its 1e6 bytes; results in rows off 16 bytes then
+// take 0.28 more for each 1e6 (fitted to the same products; the choices take 1.8% longer than
+// the best).  4095 x 4097 x 1023 bfloat16 110 us through registers, 62 with both copied; 777 x
+// 1111 x 333 6.2 and 10.4.
 struct Choice {
   Plan plan;
   bool dma = false, pack_a = false, pack_b = false;
@@ -279,13 +293,13 @@ Choice choose(const Product &q, int tile, int splits, bool packing = true) {
   Choice c;
   const bool da = direct_loads(q.a, size), db = direct_loads(q.b, size);
   c.dma = da && db;
-  c.plan = plan_product(p.m, p.n, p.k, q.type, p.terms, q.a.mn, q.b.mn, c.dma, tile, splits);
+  c.plan = plan_product(q, c.dma, tile, splits);
   c.us = c.plan.us;
   if (!c.dma && packing && p.k > 0 && c.plan.tile != TILE_ROWS) {
     const long long copies = (da ? 0 : packed_bytes(q.a, size)) + (db ? 0 : packed_bytes(q.b, size));
     const auto fits = [&](const Operand &o) { return 256 * packed_ld(o, size) * size + 1024 < (1L << 31); };
-    const Plan fast = plan_product(p.m, p.n, p.k, q.type, p.terms, q.a.mn, q.b.mn, true, tile, splits);
-    const double us = fast.us + 4 + 2 * copies / 4e6;
+    const Plan fast = plan_product(q, true, tile, splits);
+    const double us = fast.us + 3.7 + copies * 0.21e-6 + (p.n % 8 ? 0.28e-6 * p.m * p.n : 0);
     if (fits(q.a) && fits(q.b) && ((tile && tile != TILE_64 && tile != TILE_ROWS) || us < c.us)) {
       c.plan = fast;
       c.us = us;
@@ -495,7 +509,7 @@ GradPlan plan_grad(const tf_linear_grad_args_t *a) {
   // One launch for both where it takes less.
   const long long copies = (direct_loads(g.dx.b, 2) ? 0 : packed_bytes(g.dx.b, 2)) + (direct_loads(x, 2) ? 0 : packed_bytes(x, 2));
   const bool more = !g.own_dz && !a->dbias && (odd || copies);  // a launch for the copies alone
-  if (plan_pair(g) + (more ? 4 : 0) + 2 * copies / 4e6 > apart) return g;
+  if (plan_pair(g) + (more ? 4 : 0) + copies * 0.21e-6 > apart) return g;
   g.pair = true;
   lay(a->act != TF_ACT_NONE || odd, SLOPE_FEW);
   g.dx.a = dz(false);

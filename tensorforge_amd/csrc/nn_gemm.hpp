@@ -118,7 +118,8 @@ struct SlabLoader {
   const char *matrix, *base;      // element (0, 0); the tile's first of slab 0
   long step, ld;                  // bytes between slabs, between lines
   int row_first, row_end, k_first, k_end;  // the tile's start and the matrix's end
-  uint32_t offset[DMA ? PER_WAVE : 1];
+  uint32_t offset[DMA ? PER_WAVE : 1];     // of this lane's pieces from base
+  long far[DMA ? 1 : PER_WAVE];            // the same without the limit
 
   // Place of this lane's piece of load i: (line, piece) of the layout above.
   static __device__ __forceinline__ void place(int i, int &row, int &k) {
@@ -150,6 +151,16 @@ struct SlabLoader {
         place(i, row, k);
         offset[i] = row < own - own0 ? static_cast<uint32_t>(MN ? k * ld + row * E : row * ld + k * E) : kNowhere;
       }
+    } else {
+      // Rows past a matrix shorter than the tile repeat its last (their results are not
+      // written); pieces past it start earlier and are shifted.
+#pragma unroll
+      for (int i = 0; i < PER_WAVE; ++i) {
+        int row, k;
+        place(i, row, k);
+        const int at = min(row, own - own0 - (MN ? kPiece<T> : 1));
+        far[i] = MN ? k * ld + at * E : at * ld + k * E;
+      }
     }
   }
 
@@ -172,35 +183,69 @@ struct SlabLoader {
     }
   }
 
-  // Registers: reads slab s ...  A tile that fits into the matrix starts so
-  // that it lies inside it, so only the last slab of k, and matrices smaller than a tile,
-  // have pieces to guard: those repeat a line inside and become zeros.
+  // Registers: whether the matrix is too small for the unguarded loads.
+  __device__ __forceinline__ bool tiny() const { return k_end < kSlab<T> || (MN && row_end < kPiece<T>); }
+  // Where slab s is read from, in k from the first: the last starts so that it lies inside.
+  __device__ __forceinline__ int slab_at(int s) const { return min(s * kSlab<T>, k_end - kSlab<T> - k_first); }
+  // Reads slab s: no branch, so that the compiler counts exactly the loads it has to wait for.
   __device__ __forceinline__ void fetch(int s, i32x4 (&held)[PER_WAVE]) const {
-    const int k0 = k_first + s * kSlab<T>;
-    if (k0 + kSlab<T> <= k_end && row_first + ROWS <= row_end) {
+    const char *from = base + slab_at(s) * (MN ? ld : static_cast<long>(sizeof(T)));
+#pragma unroll
+    for (int i = 0; i < PER_WAVE; ++i) held[i] = *reinterpret_cast<const loose16 *>(from + far[i]);
+  }
+  // Reads any slab: what lies outside becomes zeros.
+  __device__ __forceinline__ void fetch_guarded(int s, i32x4 (&held)[PER_WAVE]) const {
+    const int length = MN ? row_end : k_end, lines = MN ? k_end : row_end;
+    const auto read = [&](auto whole) {
 #pragma unroll
       for (int i = 0; i < PER_WAVE; ++i) {
         int row, k;
         place(i, row, k);
-        const char *p = base + s * step + (MN ? k * ld + row * static_cast<long>(sizeof(T)) : row * ld + k * static_cast<long>(sizeof(T)));
-        held[i] = *reinterpret_cast<const loose16 *>(p);
+        row += row_first;
+        k += k_first + s * kSlab<T>;
+        const int line = MN ? k : row, at = MN ? row : k;
+        const T *p = reinterpret_cast<const T *>(matrix + min(line, lines - 1) * ld);
+        if constexpr (whole()) held[i] = load_piece<false>(p, at, length);
+        else held[i] = load_piece_any(p, at, length);
+        if (line >= lines) held[i] = i32x4{0, 0, 0, 0};
       }
-      return;
-    }
-#pragma unroll
-    for (int i = 0; i < PER_WAVE; ++i) {
-      int row, k;
-      place(i, row, k);
-      row += row_first;
-      k += k0;
-      const int line = MN ? k : row, lines = MN ? k_end : row_end;
-      const char *p = matrix + min(line, lines - 1) * ld;
-      held[i] = load_piece_any(reinterpret_cast<const T *>(p), MN ? row : k, MN ? row_end : k_end);
-      if (line >= lines) held[i] = i32x4{0, 0, 0, 0};
-    }
+    };
+    if (length >= kPiece<T>) read(Int<1>{});
+    else read(Int<0>{});
   }
-  // ... and puts it into LDS.
-  static __device__ __forceinline__ void put(lds_char *lds, const i32x4 (&held)[PER_WAVE]) {
+  // Puts what fetch read of slab s into LDS, without the k that the slab before had.
+  __device__ __forceinline__ void put(int s, lds_char *lds, i32x4 (&held)[PER_WAVE]) const {
+    constexpr int P = kPiece<T>, BITS = 8 * sizeof(T);
+    const int had = s * kSlab<T> - slab_at(s);
+    if (had > 0) {
+#pragma unroll
+      for (int i = 0; i < PER_WAVE; ++i) {
+        int row, k;
+        place(i, row, k);
+        if constexpr (MN) {
+          if (k < had) held[i] = i32x4{0, 0, 0, 0};
+        } else {
+          const int drop = had - k, bits = max(0, min(drop, P - 1)) * BITS;
+          const auto u = __builtin_bit_cast(unsigned __int128, held[i]) >> bits << bits;
+          held[i] = drop >= P ? i32x4{0, 0, 0, 0} : __builtin_bit_cast(i32x4, u);
+        }
+      }
+    }
+    if constexpr (MN) {
+      if (row_first + ROWS > row_end) {
+#pragma unroll
+        for (int i = 0; i < PER_WAVE; ++i) {
+          int row, k;
+          place(i, row, k);
+          const int past = max(0, row - (row_end - row_first - P));
+          const auto u = __builtin_bit_cast(unsigned __int128, held[i]) >> (min(past, P - 1) * BITS);
+          held[i] = past >= P ? i32x4{0, 0, 0, 0} : __builtin_bit_cast(i32x4, u);
+        }
+      }
+    }
+    put_as_is(lds, held);
+  }
+  static __device__ __forceinline__ void put_as_is(lds_char *lds, const i32x4 (&held)[PER_WAVE]) {
     lds_char *wave = lds + (threadIdx.x / 64) * (PER_WAVE * 1024) + (threadIdx.x % 64) * 16;
 #pragma unroll
     for (int i = 0; i < PER_WAVE; ++i)
@@ -471,33 +516,46 @@ __device__ __forceinline__ void gemm_tile(const GemmParams &p, int block, int bl
         at = at == ST - 1 ? 0 : at + 1;
       }
     } else {
-      // Two slabs are under way in registers while one is multiplied.
-      i32x4 ha[2][decltype(la)::PER_WAVE], hb[2][decltype(lb)::PER_WAVE];
+      // DEEP slabs are under way in registers while one is multiplied; past the last they
+      // repeat it.  With branches around the loads the compiler waits for all of them:
+      // 1536 x 256 x 2558 bfloat16 30.7 us, two slabs deep; 14.2 this way.
+      // (Four of lines not along k would not leave registers for three workgroups a CU.)
+      constexpr int DEEP = AMN || BMN ? 3 : 4;
+      i32x4 ha[DEEP][decltype(la)::PER_WAVE], hb[DEEP][decltype(lb)::PER_WAVE];
+      if (count > 0 && !la.tiny() && !lb.tiny()) {
 #pragma unroll
-      for (int s = 0; s < 2; ++s)
-        if (s < count) {
-          la.fetch(s, ha[s]);
-          lb.fetch(s, hb[s]);
+        for (int q = 0; q < DEEP; ++q) {
+          la.fetch(q, ha[q]);
+          lb.fetch(q, hb[q]);
         }
-      if (count > 0) {
-        la.put(lds, ha[0]);
-        lb.put(lds + BM * 128, hb[0]);
-      }
-      for (int s = 0; s < count; s += 2) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          if (s + h >= count) break;
+        la.put(0, lds, ha[0]);
+        lb.put(0, lds + BM * 128, hb[0]);
+        constexpr int TURN = DEEP % 2 ? 2 * DEEP : DEEP;  // steps until slab and LDS place come together again
+        const auto step = [&](auto h, int s) {
           wait_lds();
           barrier();
-          if (s + h + 2 < count) {
-            la.fetch(s + h + 2, ha[h]);
-            lb.fetch(s + h + 2, hb[h]);
-          }
-          multiply(lds + h * STAGE);
-          if (s + h + 1 < count) {
-            la.put(lds + (1 - h) * STAGE, ha[1 - h]);
-            lb.put(lds + (1 - h) * STAGE + BM * 128, hb[1 - h]);
-          }
+          la.fetch(s + h() + DEEP, ha[h() % DEEP]);
+          lb.fetch(s + h() + DEEP, hb[h() % DEEP]);
+          multiply(lds + h() % 2 * STAGE);
+          la.put(s + h() + 1, lds + (1 - h() % 2) * STAGE, ha[(h() + 1) % DEEP]);
+          lb.put(s + h() + 1, lds + (1 - h() % 2) * STAGE + BM * 128, hb[(h() + 1) % DEEP]);
+        };
+        int s = 0;
+        for (; s + TURN <= count; s += TURN) unroll<TURN>([&](auto h) { step(h, s); });
+        unroll<TURN - 1>([&](auto h) {
+          if (s + h() < count) step(h, s);
+        });
+      } else {
+        for (int s = 0; s < count; ++s) {
+          la.fetch_guarded(s, ha[0]);
+          lb.fetch_guarded(s, hb[0]);
+          wait_lds();
+          barrier();
+          la.put_as_is(lds, ha[0]);
+          lb.put_as_is(lds + BM * 128, hb[0]);
+          wait_lds();
+          barrier();
+          multiply(lds);
         }
       }
     }
@@ -522,7 +580,7 @@ __device__ __forceinline__ void gemm_tile(const GemmParams &p, int block, int bl
 }
 
 template <typename T, typename O, bool AMN, bool BMN, int BM, int BN, int WM, int WN, int ST, bool DMA>
-__global__ __launch_bounds__(64 * WM *WN) void gemm_tile_kernel(GemmParams p) {
+__global__ __launch_bounds__(64 * WM *WN, DMA ? 1 : 3) void gemm_tile_kernel(GemmParams p) {
   __shared__ __align__(1024) char smem[tile_lds<BM, BN, ST>()];
   gemm_tile<T, O, AMN, BMN, BM, BN, WM, WN, ST, DMA>(p, blockIdx.x, gridDim.x, (lds_char *)smem);
 }
@@ -649,20 +707,28 @@ __global__ __launch_bounds__(64 * rows_waves(BMN, MI)) void gemm_rows_kernel(Gem
   if (p.k % kSlab<T> && wave == slabs % NW) {  // what is left of k
     const int k0 = slabs * kSlab<T>;
     Held &h = held[0];
+    const auto rest = [&](auto whole) {  // whole: k is at least a piece
+      const auto piece = [&](const T *row, int at) {
+        if constexpr (whole()) return load_piece<false>(row, at, p.k);
+        else return load_piece_any(row, at, p.k);
+      };
 #pragma unroll
-    for (int i = 0; i < WP; ++i) {
-      if constexpr (BMN) {
-        const int k = k0 + i * 16 + lane / 4;
-        h.b[i] = i32x4{0, 0, 0, 0};
-        if (k < p.k) h.b[i] = *reinterpret_cast<const loose16 *>(b + (k0 + i * 16) * p.ldb);
-      } else {
-        h.b[i] = load_piece_any(b, k0 + (i * 4 + g) * P, p.k);
+      for (int i = 0; i < WP; ++i) {
+        if constexpr (BMN) {
+          const int k = k0 + i * 16 + lane / 4;
+          const i32x4 v = *reinterpret_cast<const loose16 *>(b + (min(k, p.k - 1) - lane / 4) * p.ldb);
+          h.b[i] = k < p.k ? v : i32x4{0, 0, 0, 0};
+        } else {
+          h.b[i] = piece(b, k0 + (i * 4 + g) * P);
+        }
       }
-    }
 #pragma unroll
-    for (int i = 0; i < MI; ++i)
+      for (int i = 0; i < MI; ++i)
 #pragma unroll
-      for (int q = 0; q < 2; ++q) h.a[i][q] = load_piece_any(a[i], k0 + (q * 4 + g) * P, p.k);
+        for (int q = 0; q < 2; ++q) h.a[i][q] = piece(a[i], k0 + (q * 4 + g) * P);
+    };
+    if (p.k >= P) rest(Int<1>{});
+    else rest(Int<0>{});
     multiply(h);
   }
   // The waves' sums, added in wave order.
