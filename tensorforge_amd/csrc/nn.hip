@@ -496,20 +496,26 @@ GradPlan plan_grad(const tf_linear_grad_args_t *a) {
     g.dx.p.terms = g.dw.p.terms = 2;
     g.dx.p.a_term = (nk ? g.dw.p.a_term : g.dw.p.b_term) = g.dz / 2;
   }
-  double apart = g.shares ? 5 : 1;  // the sum's launch, or a gap between two
-  if (a->dx && m) {
-    const Choice c = choose(g.dx, a->tile, a->splits);
-    g.product = c.bytes(), apart += c.us;
+  // One launch for both where it takes less; below 8 us two cannot.
+  double pair = 1e30;
+  long long copies = 0;
+  if (!a->tile && !a->splits && a->dx && a->dw && m) {
+    copies = (direct_loads(g.dx.b, 2) ? 0 : packed_bytes(g.dx.b, 2)) + (direct_loads(x, 2) ? 0 : packed_bytes(x, 2));
+    const bool more = !g.own_dz && !a->dbias && (odd || copies);  // a launch for the copies alone
+    pair = plan_pair(g) + (more ? 4 : 0) + copies * 0.21e-6;
   }
-  if (a->dw) {
-    const Choice c = choose(g.dw, a->tile, a->splits);
-    g.product = std::max(g.product, c.bytes()), apart += c.us;
+  if (pair > 8) {
+    double apart = g.shares ? 5 : 1;  // the sum's launch, or a gap between two
+    if (a->dx && m) {
+      const Choice c = choose(g.dx, a->tile, a->splits);
+      g.product = c.bytes(), apart += c.us;
+    }
+    if (a->dw) {
+      const Choice c = choose(g.dw, a->tile, a->splits);
+      g.product = std::max(g.product, c.bytes()), apart += c.us;
+    }
+    if (pair > apart) return g;
   }
-  if (a->tile || a->splits || !a->dx || !a->dw || !m) return g;
-  // One launch for both where it takes less.
-  const long long copies = (direct_loads(g.dx.b, 2) ? 0 : packed_bytes(g.dx.b, 2)) + (direct_loads(x, 2) ? 0 : packed_bytes(x, 2));
-  const bool more = !g.own_dz && !a->dbias && (odd || copies);  // a launch for the copies alone
-  if (plan_pair(g) + (more ? 4 : 0) + copies * 0.21e-6 > apart) return g;
   g.pair = true;
   lay(a->act != TF_ACT_NONE || odd, SLOPE_FEW);
   g.dx.a = dz(false);
