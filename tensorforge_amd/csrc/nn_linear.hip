@@ -70,6 +70,8 @@ __global__ __launch_bounds__(256) void pack_kernel(PackParams p) {
 }
 unsigned pack_blocks(const PackParams &p) { return static_cast<unsigned>((p.pieces[0] + p.pieces[1] + 255) / 256); }
 
+// Without a branch, also where columns end inside a piece: 4096 x 8191 bfloat16 gelu 49 us
+// against 80 with one (4096 x 8192 44 either way).
 template <typename T>
 __device__ __forceinline__ void load_slope8(const T *row, int c, int n, float (&v)[8]) {
   const auto u = __builtin_bit_cast(typename Vec<T, 8>::type, load_piece_any(row, c, n));
