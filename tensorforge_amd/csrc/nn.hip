@@ -431,7 +431,8 @@ struct GradPlan {
   long long bytes() const { return dz + shares + product; }
 };
 
-// Both products on 64 x 64 tiles in one launch: the aligned copies of x and w come with
+// Both products on 64 x 64 tiles in one launch (1148 x 848 x 209 bfloat16 silu 16.7 us, 35.8 in
+// launches apart; 4096 x 8192 x 2048 244 us against 238 apart): the aligned copies of x and w come with
 // dz, one more launch joins the ranges of k of both.  Predicted as predicted() does,
 // two workgroups on a CU; us.  The time of what it finds, and the ranges in `g`.
 double plan_pair(GradPlan &g) {

