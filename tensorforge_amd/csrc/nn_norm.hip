@@ -222,6 +222,13 @@ __global__ __launch_bounds__(256) void rms_norm_long_kernel(NormParams p) {
 // with one of 256 threads, 71 with two.
 constexpr int grad_rows(int nt, int ch) { return nt == 64 ? 4 : ch == 1 ? 2 : 1; }
 
+// A workgroup alone: its share is the sum.
+__device__ __forceinline__ void store_weight8(const NormGradParams &p, int c, const float (&v)[8]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    if (c + i < p.d) store_as(p.dw, p.weight_type, c + i, v[i]);
+}
+
 // The gradient's dx, and this workgroup's rows' share of dw, kept in registers over
 // its rows.  The shares are added by share_sum_kernel, in a fixed order.  Bound by
 // memory: 8192 x 4096 bfloat16 with dh 57 us, 51 and 5 for the sum (268 MB, 5.2 TB/s
@@ -282,7 +289,11 @@ __global__ __launch_bounds__(NT *grad_rows(NT, CH)) void rms_norm_grad_kernel(No
   float *share = p.shares + static_cast<long>(blockIdx.x) * p.d;
   if constexpr (RPB == 1) {
 #pragma unroll
-    for (int j = 0; j < CH; ++j) store8(share + (j * NT + t) * 8, p.d - (j * NT + t) * 8, dw[j]);
+    for (int j = 0; j < CH; ++j) {
+      const int c = (j * NT + t) * 8;
+      if (p.shares) store8(share + c, p.d - c, dw[j]);
+      else store_weight8(p, c, dw[j]);
+    }
   } else {
     // The rows' sums meet in LDS: one share a workgroup.
     __shared__ float part[RPB][NT * CH * 8];
@@ -296,7 +307,9 @@ __global__ __launch_bounds__(NT *grad_rows(NT, CH)) void rms_norm_grad_kernel(No
       float s = part[0][e];
 #pragma unroll
       for (int q = 1; q < RPB; ++q) s += part[q][e];
-      if (at < p.d) share[at] = s;
+      if (at >= p.d) continue;
+      if (p.shares) share[at] = s;
+      else store_as(p.dw, p.weight_type, at, s);
     }
   }
 }
@@ -395,15 +408,16 @@ void norm_grad_launch_as(const NormGradParams &p, dim3 grid, hipStream_t stream)
 }
 
 template <typename T>
-void norm_grad_launch(const NormGradParams &p, hipStream_t stream) {
+void norm_grad_launch(NormGradParams p, hipStream_t stream) {
   const long shares = norm_grad_shares(p.rows, p.d);
+  if (shares == 1 && p.d >= 8 && p.d <= kLongest) p.shares = nullptr;
   const dim3 grid(static_cast<unsigned>(shares));
   if (shares) {
     if (p.d < 8 || p.d > kLongest) rms_norm_grad_long_kernel<T><<<grid, 256, 0, stream>>>(p);
     else if (p.d % 8 == 0) norm_grad_launch_as<T, WHOLE>(p, grid, stream);
     else norm_grad_launch_as<T, TAIL>(p, grid, stream);
   }
-  (void)launch_share_sum(p.shares, shares, p.d, p.dw, p.weight_type, stream);
+  if (p.shares || !shares) (void)launch_share_sum(p.shares, shares, p.d, p.dw, p.weight_type, stream);
 }
 
 }  // namespace
@@ -411,10 +425,14 @@ void norm_grad_launch(const NormGradParams &p, hipStream_t stream) {
 // Workgroups, each with a share of the weight's gradient: as many as are on the GPU
 // at once, and a quarter less where that is 1024, for fewer shares to add.  us a call,
 // bfloat16, with 512 / 768 / 1024: 8192 x 4096 65.5 / 57.8 / 60.8; 8192 x 8192 83.9 / - /
-// 91.8 (256: 100); 4096 x 16384 107 / - / 130 (256: 98).
+// 91.8 (256: 100); 4096 x 16384 107 / - / 130 (256: 98).  Few rows go to one workgroup,
+// up to `steps` after each other, whose share is the sum: no second launch (16 x 287 8.7 us a call
+// with it, 6.0 without; 2 x 4032 8.8 and 6.1).
 long norm_grad_shares(long rows, long d) {
   const int n = pieces(d);
   const long at_a_time = d < 8 || n > 256 ? 1 : n <= 128 ? 4 : 2;  // grad_rows of the kernel that runs
+  const long steps = n <= 256 ? 5 : n <= 512 ? 4 : n <= 1024 ? 2 : 1;
+  if (d >= 8 && d <= kLongest && rows <= steps * at_a_time) return rows > 0;
   const long most = n <= 256 || d < 8 ? 512 : n <= 512 ? 768 : n <= 1024 ? 512 : 256;
   return std::min<long>((rows + at_a_time - 1) / at_a_time, most);
 }

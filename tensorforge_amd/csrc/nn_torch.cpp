@@ -243,8 +243,8 @@ PyObject *rms_norm_grad(PyObject *, PyObject *const *a, Py_ssize_t n) {
   const Tensor dx = fresh(h, h.sizes(), t), dw = fresh(h, {hr.n}, weight.scalar_type());
   g.dx = dx.data_ptr(), g.dx_ld = hr.n, g.dweight = dw.data_ptr();
   check(tf_rms_norm_grad_workspace(g.rows, g.d, &g.workspace_bytes));
-  const Tensor space = fresh(h, {static_cast<int64_t>(g.workspace_bytes)}, ScalarType::Byte);
-  g.workspace = space.data_ptr();
+  Tensor space;
+  if (g.workspace_bytes) space = fresh(h, {static_cast<int64_t>(g.workspace_bytes)}, ScalarType::Byte), g.workspace = space.data_ptr();
   check(tf_rms_norm_grad(&g, on.stream));
   return tuple({&dx, &dw});
   END_HANDLE_TH_ERRORS
@@ -347,8 +347,8 @@ PyObject *linear_grad(PyObject *, PyObject *const *a, Py_ssize_t n) {
   }
   if (want_db) db = fresh(x, {wr.n}, bt), g.dbias = db.data_ptr(), g.bias_type = type_of(bt);
   check(tf_linear_grad_workspace(&g, &g.workspace_bytes));
-  const Tensor space = fresh(x, {static_cast<int64_t>(g.workspace_bytes)}, ScalarType::Byte);
-  g.workspace = space.data_ptr();
+  Tensor space;
+  if (g.workspace_bytes) space = fresh(x, {static_cast<int64_t>(g.workspace_bytes)}, ScalarType::Byte), g.workspace = space.data_ptr();
   check(tf_linear_grad(&g, on.stream));
   return tuple({want_dx ? &dx : nullptr, want_dw ? &dw : nullptr, want_db ? &db : nullptr});
   END_HANDLE_TH_ERRORS
