@@ -459,7 +459,8 @@ double plan_pair(GradPlan &g) {
 // Up to this many multiply-adds a product of the rounded dz is not taken alone:
 // what the rounding left goes in as a second term, into the same float sums.  A
 // small gradient then errs by its own rounding only; larger ones, where a second
-// product would show in the time, by sqrt(2) of it.
+// product would cost as much again, by sqrt(2) of it.  bfloat16 gelu, two terms here and
+// one just above: 512 x 512 x 520 14.4 us, x 544 11.2; 2048 x 256 x 264 17.4, x 280 15.4.
 constexpr double kTwoTerms = 1.4e8;
 
 GradPlan plan_grad(const tf_linear_grad_args_t *a) {
