@@ -290,6 +290,31 @@ def test_strides_alignment_and_neighbours(order, dtype):
             _check_grad(got, dy, x, w, z.cpu(), "relu", dtype, dtype)
 
 
+@pytest.mark.parametrize("splits", [1, 2, 3])
+@pytest.mark.parametrize("order", [0, 1])
+def test_odd_slabs_and_edges(order, splits):
+    """Loads through registers, NaN around the operands: sums of k that end inside a slab (one slab is read back into
+    the matrix), ranges of k that are nothing but that slab, tiles wider than the matrix, rows shorter than a piece."""
+    nn = _nn()
+    g = torch.Generator().manual_seed(splits)
+    for m, n, k in ((70, 69, 129), (65, 9, 71), (200, 63, 191), (67, 65, 65), (131, 7, 330), (65, 70, 63), (66, 130, 449)):
+        x, w = _matrix(g, m, k, torch.bfloat16), _matrix(g, k, n, torch.bfloat16, k ** -0.5)
+        r, dy, z = (_matrix(g, m, n, torch.bfloat16) for _ in range(3))
+
+        def inside(t):
+            big = torch.full((t.shape[0] + 2, t.shape[1] + 4), float("nan"), dtype=t.dtype, device="cuda")
+            big[1:-1, 1:-3] = t.cuda()
+            return big[1:-1, 1:-3]
+
+        wi = inside(w) if order == 0 else inside(w.t()).t()
+        out = nn.linear(inside(x), wi, None, "silu", inside(r), tile=3, splits=splits)
+        _check(out, x, w, None, "silu", r, None, torch.bfloat16)
+        got = nn.linear_grad(inside(dy), inside(x), wi, inside(z), "relu", bias_dtype=torch.float32, tile=3, splits=splits)
+        _check_grad(got, dy, x, w, z, "relu", torch.bfloat16, torch.float32)
+        got = nn.linear_grad(inside(dy), inside(x), wi, inside(z), "relu", bias_dtype=torch.float32)
+        _check_grad(got, dy, x, w, z, "relu", torch.bfloat16, torch.float32)
+
+
 @pytest.mark.parametrize("tile,splits", [(0, 0), (1, 1), (2, 1), (3, 1), (5, 1), (3, 2)])
 def test_writes_stay_inside(tile, splits):
     """Through the C ABI: out and z inside wider matrices; nothing else changes."""
@@ -394,6 +419,35 @@ def test_streams_and_graphs():
         got = chain()
     side.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = chain()
+    for _ in range(4):
+        for t in captured:
+            t.fill_(0)
+        torch.cuda.synchronize()
+        graph.replay()
+        eager = chain()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(captured, want))
+        assert all(torch.equal(a, b) for a, b in zip(eager, want))
+
+
+def test_small_gradients_in_a_graph():
+    """The small gradients' launches (copies of odd operands, ranges of k, their join, the bias shares) and the norm's
+    one, captured once and replayed between eager calls."""
+    nn = _nn()
+    g = torch.Generator().manual_seed(8)
+    cases = [[_matrix(g, *s, torch.bfloat16).cuda() for s in ((m, n), (m, k), (k, n), (m, n))]
+             for m, n, k in ((2100, 141, 150), (17, 2071, 67), (256, 256, 128))]
+    h, nw = _matrix(g, 9, 999, torch.bfloat16).cuda(), torch.ones(999, device="cuda")
+
+    def chain():
+        out = [t for dy, x, w, z in cases for t in nn.linear_grad(dy, x, w, z, "gelu", bias_dtype=torch.float32)]
+        return out + list(nn.rms_norm_grad(h, h, nw))
+
+    want = chain()
+    torch.cuda.synchronize()
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
         captured = chain()
