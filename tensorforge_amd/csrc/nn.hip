@@ -460,7 +460,7 @@ double plan_pair(GradPlan &g) {
 // what the rounding left goes in as a second term, into the same float sums.  A
 // small gradient then errs by its own rounding only; larger ones, where a second
 // product would cost as much again, by sqrt(2) of it.  bfloat16 gelu, two terms here and
-// one just above: 512 x 512 x 520 14.4 us, x 544 11.2; 2048 x 256 x 264 17.4, x 280 15.4.
+// one just above: 512 x 512 x 520 14.0 us, x 544 11.0; 2048 x 256 x 264 17.1, x 280 15.0.
 constexpr double kTwoTerms = 1.4e8;
 
 GradPlan plan_grad(const tf_linear_grad_args_t *a) {

@@ -598,7 +598,7 @@ __global__ __launch_bounds__(64 * WM *WN, DMA ? 1 : 3) void gemm_tile_kernel(Gem
 // float16 5.1 us (one launch each: 5 + 5), 768 x 256 x 344 in ranges of k 7.0 (6.2 + 11.1).
 template <typename T, bool BMN>
 __global__ __launch_bounds__(256) void gemm_pair_kernel(GemmParams dx, GemmParams dw, ShareParams sum, int first, int second) {
-  constexpr int ST = 4;
+  constexpr int ST = 3;  // three workgroups on a CU; with four slabs, two: 100 drawn gradients took 2% longer
   __shared__ __align__(1024) char smem[tile_lds<64, 64, ST>()];
   const int block = blockIdx.x;
   if (block < first)
