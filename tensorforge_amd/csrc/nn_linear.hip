@@ -84,6 +84,9 @@ __device__ __forceinline__ void load_slope8(const T *row, int c, int n, float (&
   for (int i = 0; i < 8; ++i) v[i] = static_cast<float>(u[i]);
 }
 
+template <typename T>
+constexpr float largest = __is_same(T, f16) ? 65504.0f : 0x1.fep127f;  // finite
+
 // 8 columns a thread; CT threads side by side, the others down the workgroup's rows.
 // The workgroups from `blocks` on make copies.  Bound by memory with arithmetic close
 // behind (gelu's slope is some 50 instructions an element): 4096 x 8192 bfloat16 gelu 44 us
@@ -118,14 +121,22 @@ __global__ __launch_bounds__(256) void act_slope_kernel(SlopeParams p, PackParam
       for (int i = 0; i < 8; ++i) sum[i] += g[i];
       if (p.dz) {
         typename Vec<T, 8>::type hi, lo;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          hi[i] = i < left ? static_cast<T>(g[i]) : static_cast<T>(0.0f);
-          lo[i] = i < left ? static_cast<T>(g[i] - static_cast<float>(hi[i])) : static_cast<T>(0.0f);
-        }
         T *to = static_cast<T *>(p.dz) + row * p.dz_ld + c;
+        if (p.lo) {
+          // Two terms.  An infinity has no second one (it would be a NaN); a finite value past
+          // the type's largest is that and the rest, which the products' float sums hold.
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const bool finite = __builtin_fabsf(g[i]) < __builtin_inff();
+            hi[i] = static_cast<T>(i < left ? (finite ? __builtin_fminf(__builtin_fmaxf(g[i], -largest<T>), largest<T>) : g[i]) : 0.0f);
+            lo[i] = static_cast<T>(i < left && finite ? g[i] - static_cast<float>(hi[i]) : 0.0f);
+          }
+          *reinterpret_cast<typename Vec<T, 8>::type *>(to + p.lo) = lo;
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) hi[i] = i < left ? static_cast<T>(g[i]) : static_cast<T>(0.0f);
+        }
         *reinterpret_cast<typename Vec<T, 8>::type *>(to) = hi;
-        if (p.lo) *reinterpret_cast<typename Vec<T, 8>::type *>(to + p.lo) = lo;
       }
     }
   }

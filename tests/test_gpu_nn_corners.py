@@ -1,0 +1,77 @@
+"""Corners of the residual block's operators, each against its definition: infinities in the gradients' second term,
+rows of no elements, sizes near the limits, second-order and forward-mode gradients."""
+
+import pytest
+import torch
+
+import nn_reference as ref
+
+pytestmark = pytest.mark.gpu
+
+HALF = [torch.bfloat16, torch.float16]
+
+
+def _nn():
+    from tensorforge_amd import tforge_nn
+    return tforge_nn
+
+
+def _matrix(g, rows, cols, dtype, scale=1.0):
+    return (torch.randn(rows, cols, generator=g) * scale).to(dtype)
+
+
+def _ordered(w, order):
+    """w (k x n) on the GPU, row by row or column by column."""
+    return w.cuda() if order == 0 else w.t().contiguous().cuda().t()
+
+
+# On both sides of 1.4e8 multiply-adds: below, dz of a smooth activation goes into the products in two terms.
+GRAD_SIZES = [(4, 16, 8, 2), (40, 130, 77, 2), (300, 264, 200, 2), (528, 528, 528, 1)]
+
+
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("order", [0, 1])
+@pytest.mark.parametrize("activation", ["gelu", "silu"])
+def test_infinite_dy(activation, order, dtype):
+    """An infinity in dy: infinities of the right sign in its row of dx and its column of dw, nothing else changed."""
+    nn = _nn()
+    for m, n, k, _ in GRAD_SIZES:
+        g = torch.Generator().manual_seed(m + n)
+        x, w, dy = _matrix(g, m, k, dtype), _matrix(g, k, n, dtype), _matrix(g, m, n, dtype)
+        z = torch.ones(m, n, dtype=dtype)
+        x[x == 0], w[w == 0] = 1, 1
+        dy[1, 3], dy[2, 5] = float("inf"), -float("inf")
+        dz = dy.double() * ref.slope(z.double(), activation)
+        args = dy.cuda(), x.cuda(), _ordered(w, order), z.cuda(), activation
+        dx, dw, _ = nn.linear_grad(*args)
+        for how in ({}, {"want_dw": False, "tile": 4}, {"want_dw": False}):
+            dx = nn.linear_grad(*args, **how)[0]
+            for got, want in ((dx, dz @ w.double().t()), (dw, x.double().t() @ dz)):
+                got = got.cpu().double()
+                assert not got.isnan().any(), (m, how)
+                assert torch.equal(got[want.isinf()], want[want.isinf()])
+                assert got[want.isfinite()].isfinite().all()
+
+
+@pytest.mark.parametrize("order", [0, 1])
+def test_dz_past_float16(order):
+    """dy * act'(z) past float16's largest value.  Two terms hold it; one is rounded to an infinity."""
+    nn = _nn()
+    for m, n, k, terms in GRAD_SIZES:
+        g = torch.Generator().manual_seed(m + n)
+        x, w, dy = _matrix(g, m, k, torch.float16, 1 / 64), _matrix(g, k, n, torch.float16, 1 / 64), _matrix(g, m, n, torch.float16)
+        x[x == 0], w[w == 0] = 0.01, 0.01
+        z = torch.ones(m, n, dtype=torch.float16)
+        dy[1, 3], z[1, 3], dy[2, 5], z[2, 5] = 60000, 1.5, -65504, 1.4
+        dz = dy.double() * ref.slope(z.double(), "gelu")
+        assert dz[1, 3] > 65520 and dz[2, 5] < -65520
+        if terms == 1:
+            dz = dz.half().double()
+        dx, dw, _ = nn.linear_grad(dy.cuda(), x.cuda(), _ordered(w, order), z.cuda(), "gelu")
+        # dz is off by its slope (2e-6 of dy) and, in one term, its rounding; then float sums and the result's rounding
+        off = 2e-6 * dy.double().abs()
+        if terms == 1:
+            off = off + ref.U[torch.float16] * torch.where(dz.isinf(), torch.zeros_like(dz), dz.abs())
+        size = torch.where(dz.isinf(), torch.zeros_like(dz), dz.abs())
+        ref.close(dx, dz @ w.double().t(), (off + (2 * n + 8) * ref.u * size) @ w.double().abs().t(), torch.float16)
+        ref.close(dw, x.double().t() @ dz, x.double().abs().t() @ (off + (2 * m + 8) * ref.u * size), torch.float16)
