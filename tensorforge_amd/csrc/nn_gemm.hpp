@@ -273,6 +273,12 @@ __device__ __forceinline__ f32x4 block_mma(f8, i32x4 a0, i32x4 a1, i32x4 b0, i32
   return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(b, a, c, 0, 0, 0, 0, 0, 0);
 }
 
+__device__ __forceinline__ f32x4 finite_or_zero(f32x4 v) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = __builtin_fabsf(v[i]) < __builtin_inff() ? v[i] : 0.0f;
+  return v;
+}
+
 // ---- epilogue ---------------------------------------------------------------
 
 // N consecutive values from p[0..left), zeros past them.
@@ -448,7 +454,10 @@ __device__ __forceinline__ void barrier() {
 // 30.3 / 26.1 (658).
 //
 // Of `blocks` workgroups this is number `block`.  An operand of two terms (a value
-// and what its rounding left) is multiplied term after term into the same sums.
+// and what its rounding left) is multiplied term after term into the same sums, the
+// second term first: it is finite, so a sum of it that is not finite has met an infinity
+// or a NaN of the other operand, and is dropped.  The first term gives these elements
+// their infinity or NaN; both would give infinity - infinity or infinity * 0.
 template <int BM, int BN, int ST>
 constexpr int tile_lds() {
   return ST * (BM + BN) * 128;
@@ -496,10 +505,10 @@ __device__ __forceinline__ void gemm_tile(const GemmParams &p, int block, int bl
       for (int j = 0; j < NI; ++j) acc[i][j] = block_mma(T{}, a[0][i], a[1][i], b[0][j], b[1][j], acc[i][j]);
   };
 
-  for (int term = 0; term < p.terms; ++term) {
+  for (int term = p.terms - 1; term >= 0; --term) {
     la.init(static_cast<const char *>(p.a) + term * p.a_term, p.lda, p.m, m0, k0, p.k);
     lb.init(static_cast<const char *>(p.b) + term * p.b_term, p.ldb, p.n, n0, k0, p.k);
-    if (term) barrier();  // the last term's slabs are used up
+    if (term < p.terms - 1) barrier();  // the last term's slabs are used up
     if constexpr (DMA) {
 #pragma unroll
       for (int s = 0; s < ST - 1; ++s)
@@ -567,6 +576,12 @@ __device__ __forceinline__ void gemm_tile(const GemmParams &p, int block, int bl
       }
     }
     wait_lds();
+    if (term) {
+#pragma unroll
+      for (int i = 0; i < MI; ++i)
+#pragma unroll
+        for (int j = 0; j < NI; ++j) acc[i][j] = finite_or_zero(acc[i][j]);
+    }
   }
   barrier();  // the slabs' LDS is the patches' now
   constexpr int COLS = BN / WN, ROWS = BM / WM / ((BM / WM) * COLS > 4096 ? 2 : 1);  // 16 KiB a wave at most
@@ -755,9 +770,11 @@ __global__ __launch_bounds__(64 * rows_waves(BMN, MI)) void gemm_rows_kernel(Gem
   f32x4 v = join[block * 64 + lane];
 #pragma unroll
   for (int w = 1; w < NW; ++w) v += join[(w * MI * NB + block) * 64 + lane];
-  if (blocks < MI * NB) {
+  if (blocks < MI * NB) {  // the second term, as in gemm_tile
+    f32x4 u = join[(blocks + block) * 64 + lane];
 #pragma unroll
-    for (int w = 0; w < NW; ++w) v += join[(w * MI * NB + blocks + block) * 64 + lane];
+    for (int w = 1; w < NW; ++w) u += join[(w * MI * NB + blocks + block) * 64 + lane];
+    v += finite_or_zero(u);
   }
   const int m = block / NB * 16 + l, n = n0 + block % NB * 16 + g * 4;
   if (m >= p.m || n >= p.n || n + 3 < nt) return;

@@ -75,3 +75,27 @@ def test_dz_past_float16(order):
         size = torch.where(dz.isinf(), torch.zeros_like(dz), dz.abs())
         ref.close(dx, dz @ w.double().t(), (off + (2 * n + 8) * ref.u * size) @ w.double().abs().t(), torch.float16)
         ref.close(dw, x.double().t() @ dz, x.double().abs().t() @ (off + (2 * m + 8) * ref.u * size), torch.float16)
+
+
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("order", [0, 1])
+@pytest.mark.parametrize("activation", ["gelu", "silu"])
+def test_infinite_operands_of_a_gradient(activation, order, dtype):
+    """An infinity in x reaches dw's row, one in w dx's column, with the sign of dz; a NaN stays one."""
+    nn = _nn()
+    for m, n, k, _ in GRAD_SIZES:
+        g = torch.Generator().manual_seed(m * n)
+        x, w, dy = _matrix(g, m, k, dtype), _matrix(g, k, n, dtype), _matrix(g, m, n, dtype)
+        z = torch.rand(m, n, generator=g).to(dtype)  # the slope is above 0
+        dy[dy == 0] = 1
+        x[1, 2], x[3, 5], w[4, 6], w[6, 1], w[7, 7] = float("inf"), float("nan"), -float("inf"), float("nan"), float("inf")
+        dz = dy.double() * ref.slope(z.double(), activation)
+        args = dy.cuda(), x.cuda(), _ordered(w, order), z.cuda(), activation
+        _, dw, _ = nn.linear_grad(*args)
+        for how in ({}, {"want_dw": False, "tile": 4}, {"want_dw": False}, {"want_dw": False, "splits": 2}):
+            dx = nn.linear_grad(*args, **how)[0]
+            for got, want in ((dx, dz @ w.double().t()), (dw, x.double().t() @ dz)):
+                got = got.cpu().double()
+                assert torch.equal(got.isnan(), want.isnan()), (m, how)
+                assert torch.equal(got[want.isinf()], want[want.isinf()])
+                assert got[want.isfinite()].isfinite().all()
