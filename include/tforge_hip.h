@@ -257,8 +257,10 @@ int tf_registry_entry(int i, int *family, int *cfg7, char *name, int name_cap);
  * Matrices have their rows contiguous; *_ld is the distance between two rows in
  * elements (>= the row's length).  Any row length, distance and alignment of the
  * elements is accepted; 16-byte aligned rows run fastest.  Sizes are at most
- * 2^30.  Outputs and the workspace overlap nothing but where said.  A size of zero is a call without work, except that gradients summed
- * over no rows and products over no k are written as sums of nothing.
+ * 2^30.  Outputs and the workspace overlap nothing but where said.  A size of
+ * zero is a call without work, except that gradients summed over no rows and
+ * products over no k are written as sums of nothing, and the scales of rows
+ * without elements as those of zeros.
  * Arithmetic is float32 from the inputs on; every output is rounded once.
  * Sums are taken in a fixed order: equal calls give equal bits.
  * Arguments that cannot hold give TF_E_ARG before anything is enqueued. */

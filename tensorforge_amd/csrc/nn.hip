@@ -66,6 +66,14 @@ int hip(hipError_t e, const char *call) {
 
 // ---- norm ---------------------------------------------------------------------
 
+// The scales of rows without elements: quantised as they are, whose largest magnitude is
+// then the least that counts.
+hipError_t scales_of_nothing(float *scale, long long rows, hipStream_t stream) {
+  NormParams p;
+  p.scale = scale, p.rows = rows;
+  return launch_rms_norm(p, TF_T_F32, true, stream);
+}
+
 int rms_norm(const tf_rms_norm_args_t *a, hipStream_t stream) {
   const char *call = "tf_rms_norm";
   if (!a) return fail(TF_E_ARG, "tf_rms_norm: null arguments");
@@ -84,7 +92,8 @@ int rms_norm(const tf_rms_norm_args_t *a, hipStream_t stream) {
   c.matrix("y", a->y, a->y_ld, a->rows, a->d, a->y_type, true);
   c.vector("scale", a->scale, a->rows, TF_T_F32, a->y_type == TF_T_F8);
   if (!c.fine()) return fail(TF_E_ARG, c.wrong);
-  if (a->rows == 0 || a->d == 0) return TF_OK;
+  if (a->rows == 0) return TF_OK;
+  if (a->d == 0) return a->y_type == TF_T_F8 ? hip(scales_of_nothing(a->scale, a->rows, stream), call) : TF_OK;
   NormParams p;
   p.x = a->x, p.residual = a->residual, p.weight = a->weight, p.y = a->y, p.h = a->h, p.scale = a->scale;
   p.x_ld = a->x_ld, p.residual_ld = a->residual_ld, p.y_ld = a->y_ld, p.h_ld = a->h_ld, p.rows = a->rows;
@@ -101,9 +110,10 @@ int quantize_rows(const void *x, long long x_ld, long long rows, long long d, in
   c.size("d", d);
   c.matrix("x", x, x_ld, rows, d, type, true);
   c.matrix("y", y, y_ld, rows, d, TF_T_F8, true);
-  c.vector("scale", scale, rows, TF_T_F32, d > 0);
+  c.vector("scale", scale, rows, TF_T_F32, true);
   if (!c.fine()) return fail(TF_E_ARG, c.wrong);
-  if (rows == 0 || d == 0) return TF_OK;
+  if (rows == 0) return TF_OK;
+  if (d == 0) return hip(scales_of_nothing(scale, rows, stream), call);
   NormParams p;
   p.x = x, p.y = y, p.scale = scale, p.x_ld = x_ld, p.y_ld = y_ld, p.rows = rows, p.d = static_cast<int>(d);
   return hip(launch_rms_norm(p, type, true, stream), call);

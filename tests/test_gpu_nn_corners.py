@@ -99,3 +99,22 @@ def test_infinite_operands_of_a_gradient(activation, order, dtype):
                 assert torch.equal(got.isnan(), want.isnan()), (m, how)
                 assert torch.equal(got[want.isinf()], want[want.isinf()])
                 assert got[want.isfinite()].isfinite().all()
+
+
+def test_scales_of_rows_without_elements():
+    """Rows of no elements have the scale of zeros, and a product over no k of them is the bias."""
+    nn = _nn()
+    scale = torch.tensor(ref.TINY / ref.F8_MAX).cuda()
+    for dtype in (torch.float32, torch.bfloat16, torch.float16):
+        for rows in (1, 5, 9000):
+            torch.full((rows,), float("nan"), device="cuda")  # what the allocator may hand out next
+            q, s = nn.quantize_rows(torch.empty(rows, 0, dtype=dtype, device="cuda"))
+            assert q.shape == (rows, 0) and s.shape == (rows,) and (s == scale).all()
+            torch.full((rows,), float("nan"), device="cuda")
+            x = torch.empty(rows, 0, dtype=dtype, device="cuda")
+            _, s, h = nn.rms_norm(x, x[0], residual=x, quantize=True)
+            assert (s == scale).all() and h.shape == (rows, 0)
+    q, s = nn.quantize_rows(torch.empty(40, 0, device="cuda"))
+    wq, ws = nn.quantize_rows(torch.empty(24, 0, device="cuda"))
+    b = torch.randn(24, device="cuda")
+    assert torch.equal(nn.linear(q, wq.t(), b, x_scale=s, w_scale=ws), b.bfloat16().expand(40, 24))
