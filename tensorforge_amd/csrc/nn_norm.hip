@@ -408,7 +408,7 @@ void norm_grad_launch_as(const NormGradParams &p, dim3 grid, hipStream_t stream)
 }
 
 template <typename T>
-void norm_grad_launch(NormGradParams p, hipStream_t stream) {
+hipError_t norm_grad_launch(NormGradParams p, hipStream_t stream) {
   const long shares = norm_grad_shares(p.rows, p.d);
   if (shares == 1 && p.d >= 8 && p.d <= kLongest) p.shares = nullptr;
   const dim3 grid(static_cast<unsigned>(shares));
@@ -416,8 +416,10 @@ void norm_grad_launch(NormGradParams p, hipStream_t stream) {
     if (p.d < 8 || p.d > kLongest) rms_norm_grad_long_kernel<T><<<grid, 256, 0, stream>>>(p);
     else if (p.d % 8 == 0) norm_grad_launch_as<T, WHOLE>(p, grid, stream);
     else norm_grad_launch_as<T, TAIL>(p, grid, stream);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess || !p.shares) return e;
   }
-  if (p.shares || !shares) (void)launch_share_sum(p.shares, shares, p.d, p.dw, p.weight_type, stream);
+  return launch_share_sum(p.shares, shares, p.d, p.dw, p.weight_type, stream);
 }
 
 }  // namespace
@@ -451,10 +453,8 @@ hipError_t launch_rms_norm(const NormParams &p, int type, bool to_f8, hipStream_
 }
 
 hipError_t launch_rms_norm_grad(const NormGradParams &p, int type, hipStream_t stream) {
-  if (type == TYPE_F32) norm_grad_launch<float>(p, stream);
-  else if (type == TYPE_BF16) norm_grad_launch<bf16>(p, stream);
-  else norm_grad_launch<f16>(p, stream);
-  return hipGetLastError();
+  if (type == TYPE_F32) return norm_grad_launch<float>(p, stream);
+  return type == TYPE_BF16 ? norm_grad_launch<bf16>(p, stream) : norm_grad_launch<f16>(p, stream);
 }
 
 }  // namespace tfnn

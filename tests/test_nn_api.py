@@ -2,8 +2,10 @@
 what the C ABI and the Python functions refuse (before any device work)."""
 
 import ctypes
+import os
 import pathlib
 import subprocess
+import sys
 
 import pytest
 import torch
@@ -147,3 +149,67 @@ def test_python_refusals():
             (lambda: nn.linear_grad(w[:4], h, w, bias_dtype=torch.float64), TypeError, "bias_dtype is Double")]:
         with pytest.raises(error, match=words):
             call()
+
+
+# Stands in for HIP's launches in a process without a GPU: prints each launch's grid and block, refuses what HIP refuses
+# (2^32 threads or more along x) and the launch that FAIL_AT names, and keeps the last error as HIP does.
+STUB = """
+#include <stdio.h>
+#include <stdlib.h>
+#include <stddef.h>
+typedef struct { unsigned x, y, z; } dim3;
+static int last, launches;
+static dim3 grid, block;
+static size_t shared;
+static void *stream;
+int __hipPushCallConfiguration(dim3 g, dim3 b, size_t n, void *s) { grid = g; block = b; shared = n; stream = s; return 0; }
+int __hipPopCallConfiguration(dim3 *g, dim3 *b, size_t *n, void **s) { *g = grid; *b = block; *n = shared; *s = stream; return 0; }
+int hipLaunchKernel(const void *f, dim3 g, dim3 b, void **args, size_t n, void *s) {
+  const char *at = getenv("FAIL_AT");
+  int bad = (unsigned long long)g.x * b.x >> 32 || (unsigned long long)g.y * b.y >> 32 || (at && atoi(at) == launches);
+  fprintf(stderr, "launch %u %u %u %u\\n", g.x, g.y, b.x, b.y);
+  ++launches;
+  if (bad) last = 9;
+  return bad ? 9 : 0;
+}
+int hipGetLastError(void) { int e = last; last = 0; return e; }
+"""
+
+
+@pytest.fixture(scope="module")
+def without_gpu(tmp_path_factory):
+    """run(code, fail_at=None): code in a process with the stub before HIP; (its output, the launches)."""
+    at = tmp_path_factory.mktemp("stub")
+    (at / "stub.c").write_text(STUB)
+    subprocess.run(["gcc", "-shared", "-fPIC", str(at / "stub.c"), "-o", str(at / "stub.so")], check=True)
+
+    def run(code, fail_at=None):
+        preload = " ".join([str(at / "stub.so"), os.environ.get("LD_PRELOAD", "")]).strip()
+        env = {**os.environ, "LD_PRELOAD": preload, "HIP_VISIBLE_DEVICES": "-1", "ROCR_VISIBLE_DEVICES": "-1", "PYTHONPATH": str(_lib.PKG.parent)}
+        if fail_at is not None:
+            env["FAIL_AT"] = str(fail_at)
+        head = "import ctypes\nfrom tensorforge_amd import _lib\nlib, ref = _lib.lib(), ctypes.byref\n"
+        r = subprocess.run([sys.executable, "-c", head + code], env=env, capture_output=True, text=True)
+        assert r.returncode == 0, r.stdout + r.stderr
+        return r.stdout, [tuple(int(v) for v in l.split()[1:]) for l in r.stderr.splitlines() if l.startswith("launch ")]
+
+    return run
+
+
+NORM_GRAD = """
+d, rows = {d}, {rows}
+a = _lib.RmsNormGradArgs(dy=256, h=256, weight=256, dx=256, dweight=256, dy_ld=d, h_ld=d, dx_ld=d, rows=rows, d=d, type=1,
+                         weight_type=1, workspace=256, workspace_bytes=1 << 40)
+print(lib.tf_rms_norm_grad(ref(a), None))
+"""
+
+
+@pytest.mark.parametrize("rows,d", [(4, 64), (4000, 64), (4000, 4000), (5, 4), (70, 20000), (0, 64)])
+def test_failed_launches_of_the_norm_gradient(rows, d, without_gpu):
+    """Whichever of its launches fails, the call says so."""
+    code = NORM_GRAD.format(rows=rows, d=d)
+    out, launches = without_gpu(code)
+    assert out.split() == ["0"] and 1 <= len(launches) <= 2
+    for i in range(len(launches)):
+        out, _ = without_gpu(code, fail_at=i)
+        assert out.split() == ["-5"], i
