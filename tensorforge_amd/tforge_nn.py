@@ -16,13 +16,15 @@ current stream, and returns new tensors; nothing is synchronised, and a call may
 be captured in a HIP graph.  A tensor last written on another stream has to be
 ordered before the call as for torch's own operators.  Tensors with leading
 dimensions are taken as rows.  Where an input of rms_norm or linear requires a
-gradient, autograd runs the gradient calls.
+gradient, autograd runs the gradient calls, which have no gradient themselves: a
+second derivative raises RuntimeError.
 
 Bad arguments raise ValueError or TypeError before any work; errors of the
 library raise RuntimeError with its message.
 """
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from tensorforge_amd import _lib
 
@@ -82,6 +84,7 @@ class _RmsNorm(torch.autograd.Function):
         return y, h
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy, dh):
         h, weight = ctx.saved_tensors
         dy = torch.zeros_like(h) if dy is None else dy.contiguous()
@@ -137,6 +140,7 @@ class _Linear(torch.autograd.Function):
         return out, z
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy, _):
         x, w, z = ctx.saved_tensors
         activation, bias_dtype, tile, splits = ctx.how

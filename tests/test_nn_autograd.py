@@ -1,0 +1,74 @@
+"""How rms_norm and linear stand in autograd, without a GPU: the native layer is replaced by plain torch steps of
+the same contract (None where an input wants a gradient, results that record nothing)."""
+
+import pytest
+import torch
+
+import nn_reference as ref
+from tensorforge_amd import tforge_nn as nn
+
+NAMES = {v: k for k, v in nn.ACTIVATIONS.items()}
+
+
+class Plain:
+    """The native layer's calls in float64, in torch's operators."""
+
+    def rms_norm(self, x, weight, residual, eps, quantize):
+        if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, residual)):
+            return None
+        h = x if residual is None else x + residual.view_as(x)
+        y = h * (h.pow(2).mean(-1, keepdim=True) + eps).rsqrt() * weight
+        return y.detach(), (None if residual is None else h.detach())
+
+    def rms_norm_grad(self, dy, h, weight, eps, dh):
+        n = h.shape[-1]
+        dx, dw = ref.norm_grad(dy.reshape(-1, n), h.reshape(-1, n), weight, eps, None if dh is None else dh.reshape(-1, n))
+        return dx.view_as(h).detach(), dw.detach()
+
+    def linear(self, x, w, bias, act, residual, keep, x_scale, w_scale, out_dtype, tile, splits):
+        if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, w, bias, residual)):
+            return None
+        z = x @ w + (0 if bias is None else bias)
+        out = ref.act(z, NAMES[act])
+        out = (out if residual is None else out + residual.view_as(out)).detach()
+        return (out, z.detach()) if keep else out
+
+    def linear_grad(self, dy, x, w, z, act, bias_dtype, want_dx, want_dw, tile, splits):
+        k, n = w.shape
+        dz = (dy * ref.slope(z.view_as(dy), NAMES[act]) if act else dy).reshape(-1, n).detach()
+        return ((dz @ w.t()).view_as(x).detach() if want_dx else None, (x.reshape(-1, k).t() @ dz).detach() if want_dw else None,
+                dz.sum(0) if bias_dtype is not None else None)
+
+
+@pytest.fixture
+def plain(monkeypatch):
+    monkeypatch.setattr(nn, "_C", Plain())
+
+
+def _leaves(*shapes, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    return [torch.randn(s, generator=g, dtype=torch.float64).requires_grad_() for s in shapes]
+
+
+def _norm(x, w, r=None):
+    return ref.norm(x, w, r)[0]
+
+
+def test_first_order(plain):
+    x, w, r, w1, b = _leaves((6, 8), (8,), (6, 8), (8, 5), (5,))
+    f = lambda norm, linear: (linear(norm(x, w, r), w1, b).sin()).sum()  # noqa: E731
+    got = torch.autograd.grad(f(lambda *a: nn.rms_norm(*a)[0], lambda *a: nn.linear(*a, "gelu")), (x, w, r, w1, b))
+    want = torch.autograd.grad(f(_norm, lambda a, c, d: ref.act(a @ c + d, "gelu")), (x, w, r, w1, b))
+    for a, c in zip(got, want):
+        assert torch.allclose(a, c, rtol=1e-10)
+
+
+def test_second_order_is_refused(plain):
+    """A penalty on a gradient needs the gradient calls' own: an error, not a penalty without effect."""
+    x, w, w1, b = _leaves((6, 8), (8,), (8, 5), (5,))
+    for loss, of in ((nn.rms_norm(x, w)[0].sin().sum(), w), (nn.linear(x, w1, b, "silu").sin().sum(), w1),
+                     (nn.linear(x, w1, b).sin().sum(), w1)):
+        g, = torch.autograd.grad(loss, of, create_graph=True)
+        assert g.requires_grad
+        with pytest.raises(RuntimeError, match="once_differentiable"):
+            g.pow(2).sum().backward()
