@@ -46,10 +46,11 @@ const Tensor &tensor(PyObject *o, const char *name) {
 
 const Tensor *optional(PyObject *o, const char *name) { return o == Py_None ? nullptr : &tensor(o, name); }
 
+// In reverse mode, or in forward mode (a tangent, which no_grad does not hide).
 bool wants_grad(std::initializer_list<const Tensor *> all) {
-  if (!at::GradMode::is_enabled()) return false;
+  const bool reverse = at::GradMode::is_enabled();
   for (const Tensor *t : all)
-    if (t && t->requires_grad()) return true;
+    if (t && ((reverse && t->requires_grad()) || t->_fw_grad(0).defined())) return true;
   return false;
 }
 

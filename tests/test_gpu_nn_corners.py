@@ -118,3 +118,15 @@ def test_scales_of_rows_without_elements():
     wq, ws = nn.quantize_rows(torch.empty(24, 0, device="cuda"))
     b = torch.randn(24, device="cuda")
     assert torch.equal(nn.linear(q, wq.t(), b, x_scale=s, w_scale=ws), b.bfloat16().expand(40, 24))
+
+
+def test_forward_mode_is_refused():
+    """A tangent is not dropped in silence: the calls have no forward-mode derivative."""
+    import torch.autograd.forward_ad as fwd
+    nn = _nn()
+    x, w, v = (torch.ones(s, dtype=torch.bfloat16, device="cuda") for s in ((4, 8), (8, 8), (8,)))
+    with fwd.dual_level():
+        for call in (lambda t: nn.linear(t, w, None, "gelu"), lambda t: nn.rms_norm(t, v)):
+            for mode in (torch.enable_grad, torch.no_grad):
+                with mode(), pytest.raises((RuntimeError, NotImplementedError), match="jvp"):
+                    call(fwd.make_dual(x, x))

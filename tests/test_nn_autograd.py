@@ -72,3 +72,19 @@ def test_second_order_is_refused(plain):
         assert g.requires_grad
         with pytest.raises(RuntimeError, match="once_differentiable"):
             g.pow(2).sum().backward()
+
+
+def test_tangents_are_seen():
+    """The native layer hands a dual tensor to autograd, under no_grad too."""
+    import torch.autograd.forward_ad as fwd
+    x, w, v = (torch.ones(s, dtype=torch.bfloat16) for s in ((4, 8), (8, 8), (8,)))
+    with fwd.dual_level():
+        for at in (0, 1):
+            a, b = [x, w], [x, v]
+            a[at], b[at] = (fwd.make_dual(t[at], torch.ones_like(t[at])) for t in (a, b))
+            for mode in (torch.enable_grad, torch.no_grad):
+                with mode():
+                    assert nn._C.linear(*a, None, 0, None, False, None, None, None, 0, 0) is None
+                    assert nn._C.rms_norm(*b, None, 1e-6, False) is None
+        with pytest.raises(ValueError, match="no gradient"):
+            nn.rms_norm(*b, quantize=True)
