@@ -46,6 +46,7 @@ def half(p):
 class Served:
     """The block in 8 bits: weights laid out once, column by column with one scale each."""
 
+    @torch.no_grad()
     def __init__(self, p):
         self.norm, self.b1, self.b2 = p["norm"], p["b1"], p["b2"]
         self.w1, self.s1 = nn.quantize_rows(p["w1"].t().contiguous())

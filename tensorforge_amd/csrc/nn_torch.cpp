@@ -7,8 +7,8 @@
 // its arguments are positional: norm of one row of 2048 into 8 bits 18.0 us a call
 // with the same steps in Python (ctypes), 5.4 us here.
 //
-// Each function returns None where an input wants a gradient: tforge_nn.py then
-// goes through autograd.
+// Where an input wants a gradient, rms_norm and linear return None, and tforge_nn.py
+// goes through autograd; the calls without a gradient refuse.
 #include <ATen/ATen.h>
 #include <ATen/core/grad_mode.h>
 #include <ATen/hip/EmptyTensor.h>
@@ -52,6 +52,10 @@ bool wants_grad(std::initializer_list<const Tensor *> all) {
   for (const Tensor *t : all)
     if (t && ((reverse && t->requires_grad()) || t->_fw_grad(0).defined())) return true;
   return false;
+}
+
+void no_gradient(const char *call, std::initializer_list<const Tensor *> all) {
+  TORCH_CHECK_VALUE(!wants_grad(all), call, " has no gradient, and a tensor wants one: call it under torch.no_grad(), or on detached tensors");
 }
 
 void same_type(const Tensor &t, const char *name, ScalarType a, ScalarType b) {
@@ -214,6 +218,7 @@ PyObject *quantize_rows(PyObject *, PyObject *const *a, Py_ssize_t n) {
   count(n, 1);
   const Tensor &x = tensor(a[0], "x");
   float_type(x, "x");
+  no_gradient("quantize_rows", {&x});
   const Rows r = rows(x, "x");
   on_gpu(x, {});
   const On on(x);
@@ -231,6 +236,7 @@ PyObject *rms_norm_grad(PyObject *, PyObject *const *a, Py_ssize_t n) {
   const Tensor &dy = tensor(a[0], "dy"), &h = tensor(a[1], "h"), &weight = tensor(a[2], "weight");
   const Tensor *dh = optional(a[4], "dh");
   float_type(h, "h");
+  no_gradient("rms_norm_grad", {&dy, &h, &weight, dh});
   const ScalarType t = h.scalar_type();
   const Rows hr = rows(h, "h"), gr = rows_of(dy, "dy", hr.m, hr.n, t);
   tf_rms_norm_grad_args_t g{};
@@ -271,10 +277,8 @@ PyObject *linear(PyObject *, PyObject *const *a, Py_ssize_t n) {
     TORCH_CHECK_TYPE(half_type(to) && (f8 || to == t), "out_dtype is ", to,
                      f8 ? ", not BFloat16 or Half" : ": 16-bit products keep x's type");
   }
-  if (wants_grad({&x, &w, bias, residual})) {
-    TORCH_CHECK_VALUE(!f8, "8-bit products have no gradient: call linear under torch.no_grad()");
-    Py_RETURN_NONE;
-  }
+  if (f8) no_gradient("an 8-bit product", {&x, &w, bias, residual, xs, ws});
+  else if (wants_grad({&x, &w, bias, residual})) Py_RETURN_NONE;
   const Rows xr = rows(x, "x");
   const Weights wr = weights(w, xr.n, t);
   tf_linear_args_t g{};
@@ -320,6 +324,7 @@ PyObject *linear_grad(PyObject *, PyObject *const *a, Py_ssize_t n) {
   const Tensor *z = optional(a[3], "z");
   const ScalarType t = x.scalar_type();
   TORCH_CHECK_TYPE(half_type(t), "x is ", t, ", not BFloat16 or Half");
+  no_gradient("linear_grad", {&dy, &x, &w, z});
   const bool want_dx = a[6] == Py_True, want_dw = a[7] == Py_True;
   const Rows xr = rows(x, "x");
   const Weights wr = weights(w, xr.n, t);

@@ -17,7 +17,9 @@ be captured in a HIP graph.  A tensor last written on another stream has to be
 ordered before the call as for torch's own operators.  Tensors with leading
 dimensions are taken as rows.  Where an input of rms_norm or linear requires a
 gradient, autograd runs the gradient calls, which have no gradient themselves: a
-second derivative raises RuntimeError.
+second derivative raises RuntimeError.  Neither have the 8-bit results: with an input
+that requires a gradient, quantize_rows, rms_norm into 8 bits, 8-bit products and the
+gradient calls raise ValueError unless they run under torch.no_grad().
 
 Bad arguments raise ValueError or TypeError before any work; errors of the
 library raise RuntimeError with its message.
@@ -55,7 +57,7 @@ def rms_norm(x, weight, residual=None, eps=1e-6, quantize=False):
     if got is not None:
         return got
     if quantize:
-        raise ValueError("the 8-bit output has no gradient: call rms_norm under torch.no_grad()")
+        raise ValueError("the 8-bit output has no gradient: call rms_norm under torch.no_grad(), or on detached tensors")
     y, h = _RmsNorm.apply(x, weight, residual, eps)
     return y, (None if residual is None else h)
 

@@ -88,3 +88,22 @@ def test_tangents_are_seen():
                     assert nn._C.rms_norm(*b, None, 1e-6, False) is None
         with pytest.raises(ValueError, match="no gradient"):
             nn.rms_norm(*b, quantize=True)
+
+
+def test_calls_without_a_gradient_refuse():
+    """What cannot pass a gradient on says so where an input wants one, and takes it under no_grad (up to the missing GPU)."""
+    h, w, v, s = (torch.ones(n, dtype=torch.bfloat16) for n in ((4, 8), (8, 16), (8,), (4, 16)))
+    f8, w8 = h.to(ref.F8), w.t().contiguous().to(ref.F8).t()
+    one = torch.ones(4), torch.ones(16)
+    calls = [(lambda a: nn.quantize_rows(a), [h]), (lambda a, b, c: nn.rms_norm_grad(a, b, c), [h, h, v]),
+             (lambda a, b, c, d: nn.rms_norm_grad(a, b, c, dh=d), [h, h, v, h]),
+             (lambda a, b, c, d: nn.linear_grad(a, b, c, d, "gelu"), [s, h, w, s]),
+             (lambda a, b, c, d: nn.linear(f8, w8, a, "none", b, x_scale=c, w_scale=d), [one[1], s, *one]),
+             (lambda a, b, c: nn.rms_norm(a, b, c, quantize=True), [h, v, h])]
+    for call, tensors in calls:
+        for i in range(len(tensors)):
+            args = [t.clone().requires_grad_() if q == i else t for q, t in enumerate(tensors)]
+            with pytest.raises(ValueError, match="no gradient"):
+                call(*args)
+            with torch.no_grad(), pytest.raises(ValueError, match="not on a GPU"):
+                call(*args)
