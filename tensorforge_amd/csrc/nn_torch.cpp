@@ -277,6 +277,7 @@ PyObject *linear(PyObject *, PyObject *const *a, Py_ssize_t n) {
     TORCH_CHECK_TYPE(half_type(to) && (f8 || to == t), "out_dtype is ", to,
                      f8 ? ", not BFloat16 or Half" : ": 16-bit products keep x's type");
   }
+  TORCH_CHECK_VALUE(f8 || (!xs && !ws), "scales belong to 8-bit products");
   if (f8) no_gradient("an 8-bit product", {&x, &w, bias, residual, xs, ws});
   else if (wants_grad({&x, &w, bias, residual})) Py_RETURN_NONE;
   const Rows xr = rows(x, "x");
@@ -297,8 +298,6 @@ PyObject *linear(PyObject *, PyObject *const *a, Py_ssize_t n) {
     TORCH_CHECK_VALUE(xs->numel() == xr.m && xs->is_contiguous(), "x_scale is not a contiguous vector of ", xr.m);
     g.x_scale = xs->data_ptr<float>();
     g.w_scale = static_cast<const float *>(vector(*ws, "w_scale", wr.n, ScalarType::Float, ScalarType::Float));
-  } else {
-    TORCH_CHECK_VALUE(!xs && !ws, "scales belong to 8-bit products");
   }
   on_gpu(x, {&w, bias, residual, xs, ws});
   const On on(x);

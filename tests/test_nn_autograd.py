@@ -107,3 +107,26 @@ def test_calls_without_a_gradient_refuse():
                 call(*args)
             with torch.no_grad(), pytest.raises(ValueError, match="not on a GPU"):
                 call(*args)
+
+
+def test_refusals_with_a_gradient_wanted():
+    """The checks of the tensors hold for calls that go through autograd too."""
+    h, w, v = (torch.zeros(n, dtype=torch.bfloat16) for n in ((4, 8), (8, 16), (8,)))
+    one = torch.zeros(16)
+    for call, error, words in [
+            (lambda a: nn.linear(a, w, x_scale=one[:4]), ValueError, "scales belong"),
+            (lambda a: nn.linear(a, w, w_scale=one), ValueError, "scales belong"),
+            (lambda a: nn.linear(a, w, x_scale=one[:4], w_scale=one), ValueError, "scales belong"),
+            (lambda a: nn.linear(a, w, out_dtype=torch.float16), TypeError, "keep x's type"),
+            (lambda a: nn.linear(a, w.half()), TypeError, "w is Half"),
+            (lambda a: nn.linear(a, h), ValueError, "not 8 x n"),
+            (lambda a: nn.linear(a, w, v), ValueError, "bias is not"),
+            (lambda a: nn.linear(a, w, residual=h), ValueError, "residual is 4 x 8, not 4 x 16"),
+            (lambda a: nn.linear(a, w, activation="tanh"), ValueError, "not one of none, relu, gelu, silu"),
+            (lambda a: nn.linear(a, w, tile=9), ValueError, "not on a GPU"),
+            (lambda a: nn.rms_norm(a, v.half()), TypeError, "weight is Half"),
+            (lambda a: nn.rms_norm(a, one), ValueError, "not a contiguous vector of 8"),
+            (lambda a: nn.rms_norm(a, v, residual=w), ValueError, "residual is 8 x 16, not 4 x 8")]:
+        for a in (h, h.clone().requires_grad_()):
+            with pytest.raises(error, match=words):
+                call(a)
