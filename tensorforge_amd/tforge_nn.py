@@ -106,7 +106,7 @@ def linear(x, w, bias=None, activation="none", residual=None, keep=False, x_scal
     column, with x_scale (one a row) and w_scale (one a column), and out_dtype
     (bfloat16 unless given).  bias is of the output's type or float32.  activation:
     "none", "relu", "gelu" (by the normal distribution), "silu".  Returns out, or
-    (out, z) with keep=True.  tile and splits override the choice by sizes
+    (out, z) with keep=True; both are differentiable.  tile and splits override the choice by sizes
     (tf_linear_args_t in tforge_hip.h).
     """
     got = _C.linear(x, w, bias, _act(activation), residual, True if keep else False, x_scale, w_scale, out_dtype, tile,
@@ -136,17 +136,22 @@ class _Linear(torch.autograd.Function):
         out, z = got if keep or smooth else (got, None)
         ctx.save_for_backward(x, w, z if smooth else None)
         ctx.how = activation, None if bias is None else bias.dtype, tile, splits
-        if z is None or not keep:
-            return out, None
-        ctx.mark_non_differentiable(z)
-        return out, z
+        ctx.set_materialize_grads(False)
+        return out, z if keep else None
 
     @staticmethod
     @once_differentiable
-    def backward(ctx, dy, _):
+    def backward(ctx, dy, dz):
         x, w, z = ctx.saved_tensors
         activation, bias_dtype, tile, splits = ctx.how
         need = ctx.needs_input_grad
-        dy = dy.contiguous()
-        dx, dw, db = linear_grad(dy, x, w, z, activation, bias_dtype if need[2] else None, need[0], need[1], tile, splits)
-        return dx, dw, db, dy if need[3] else None, None, None, None, None
+
+        def grads(g, z, activation):
+            return linear_grad(g.contiguous(), x, w, z, activation, bias_dtype if need[2] else None, need[0], need[1], tile,
+                               splits)
+
+        # A gradient that reaches the kept z past the activation: its own products, added to the output's.
+        got = [] if dy is None else [grads(dy, z, activation)]
+        got += [] if dz is None else [grads(dz, None, "none")]
+        total = (None, None, None) if not got else got[0] if len(got) == 1 else [a if a is None else a + b for a, b in zip(*got)]
+        return (*total, dy if need[3] else None, None, None, None, None)

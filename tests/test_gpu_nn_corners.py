@@ -130,3 +130,20 @@ def test_forward_mode_is_refused():
             for mode in (torch.enable_grad, torch.no_grad):
                 with mode(), pytest.raises((RuntimeError, NotImplementedError), match="jvp"):
                     call(fwd.make_dual(x, x))
+
+
+@pytest.mark.parametrize("activation", ["none", "gelu"])
+def test_gradient_of_the_kept_pre_activation(activation):
+    nn = _nn()
+    g = torch.Generator().manual_seed(12)
+    x, w, gy, gz = (_matrix(g, *s, torch.float16, sc) for s, sc in (((30, 64), 1), ((64, 48), .125), ((30, 48), 1), ((30, 48), 1)))
+    b = torch.randn(48, generator=g)
+    leaves = [t.clone().cuda().requires_grad_() for t in (x, w, b)]
+    out, z = nn.linear(*leaves, activation, keep=True)
+    torch.autograd.backward([out, z], [gy.cuda(), gz.cuda()])
+    same = [t.clone().double().requires_grad_() for t in (x, w, b)]
+    zz = same[0] @ same[1] + same[2]
+    torch.autograd.backward([torch.nn.functional.gelu(zz) if activation == "gelu" else zz + 0, zz], [gy.double(), gz.double()])
+    for a, c in zip(leaves, same):
+        # z and dz are each rounded to 11 bits, then both gradients and their sum
+        assert float((a.grad.cpu().double() - c.grad).norm() / c.grad.norm()) < 5 * 2.0 ** -11

@@ -130,3 +130,20 @@ def test_refusals_with_a_gradient_wanted():
         for a in (h, h.clone().requires_grad_()):
             with pytest.raises(error, match=words):
                 call(a)
+
+
+@pytest.mark.parametrize("activation", ["none", "gelu"])
+@pytest.mark.parametrize("of", ["both", "out", "z"])
+def test_the_kept_pre_activation_is_differentiable(activation, of, plain):
+    """A loss on the kept z, alone or beside the output's, reaches x, w and the bias."""
+    leaves = _leaves((6, 8), (8, 5), (5,), (6, 5))
+
+    def loss(out, z):
+        return (out.sin().sum() if of != "z" else 0) + (z.pow(3).sum() if of != "out" else 0)
+
+    x, w, b, r = leaves
+    got = torch.autograd.grad(loss(*nn.linear(x, w, b, activation, r, keep=True)), leaves, allow_unused=True)
+    z = x @ w + b
+    want = torch.autograd.grad(loss(ref.act(z, activation) + r, z), leaves, allow_unused=True)
+    for a, c in zip(got, want):
+        assert (a is None) == (c is None) and (a is None or torch.allclose(a, c, rtol=1e-10))
