@@ -80,8 +80,8 @@ class _RmsNorm(torch.autograd.Function):
     def forward(ctx, x, weight, residual, eps):
         with torch.no_grad():
             y, h = rms_norm(x, weight, residual, eps)
-        ctx.eps, ctx.added = eps, residual is not None
-        ctx.save_for_backward(h if ctx.added else x, weight)
+        ctx.eps, ctx.added = eps, None if residual is None else residual.shape
+        ctx.save_for_backward(x if residual is None else h, weight)
         ctx.set_materialize_grads(False)
         return y, h
 
@@ -91,7 +91,10 @@ class _RmsNorm(torch.autograd.Function):
         h, weight = ctx.saved_tensors
         dy = torch.zeros_like(h) if dy is None else dy.contiguous()
         dx, dw = rms_norm_grad(dy, h, weight, ctx.eps, None if dh is None else dh.contiguous())
-        return dx, dw, dx if ctx.added else None, None
+        if ctx.added is None:
+            return dx, dw, None, None
+        # A view would be another tensor on dx's memory, and both could become a leaf's grad.
+        return dx, dw, dx if ctx.added == dx.shape else dx.reshape(ctx.added).clone(), None
 
 
 # ---- products ---------------------------------------------------------------------
@@ -136,6 +139,7 @@ class _Linear(torch.autograd.Function):
         out, z = got if keep or smooth else (got, None)
         ctx.save_for_backward(x, w, z if smooth else None)
         ctx.how = activation, None if bias is None else bias.dtype, tile, splits
+        ctx.added = None if residual is None else residual.shape
         ctx.set_materialize_grads(False)
         return out, z if keep else None
 
@@ -154,4 +158,4 @@ class _Linear(torch.autograd.Function):
         got = [] if dy is None else [grads(dy, z, activation)]
         got += [] if dz is None else [grads(dz, None, "none")]
         total = (None, None, None) if not got else got[0] if len(got) == 1 else [a if a is None else a + b for a, b in zip(*got)]
-        return (*total, dy if need[3] else None, None, None, None, None)
+        return (*total, dy.reshape(ctx.added) if need[3] and dy is not None else None, None, None, None, None)

@@ -147,3 +147,18 @@ def test_gradient_of_the_kept_pre_activation(activation):
     for a, c in zip(leaves, same):
         # z and dz are each rounded to 11 bits, then both gradients and their sum
         assert float((a.grad.cpu().double() - c.grad).norm() / c.grad.norm()) < 5 * 2.0 ** -11
+
+
+def test_a_residual_of_other_leading_dimensions():
+    nn = _nn()
+    g = torch.Generator().manual_seed(3)
+    x, r, w, v = (_matrix(g, *s, torch.bfloat16).cuda() for s in ((6, 64), (6, 64), (64, 64), (1, 64)))
+    grads = []
+    for shape in ((6, 64), (2, 3, 64)):
+        a, b = x.view(shape).clone().requires_grad_(), r.clone().requires_grad_()
+        y, h = nn.rms_norm(a, v[0], residual=b)
+        out = nn.linear(y, w, None, "gelu", b)
+        torch.autograd.backward([out, h], [torch.ones_like(out), torch.ones_like(h)])
+        assert a.grad.shape == a.shape and b.grad.shape == b.shape
+        grads.append((a.grad.view(6, 64), b.grad))
+    assert all(torch.equal(p, q) for p, q in zip(*grads))

@@ -147,3 +147,22 @@ def test_the_kept_pre_activation_is_differentiable(activation, of, plain):
     want = torch.autograd.grad(loss(ref.act(z, activation) + r, z), leaves, allow_unused=True)
     for a, c in zip(got, want):
         assert (a is None) == (c is None) and (a is None or torch.allclose(a, c, rtol=1e-10))
+
+
+@pytest.mark.parametrize("shape,other", [((2, 3, 8), (6, 8)), ((6, 8), (2, 3, 8)), ((8,), (1, 8)), ((1, 1, 8), (8,))])
+def test_a_residual_of_other_leading_dimensions(shape, other, plain):
+    """Leading dimensions are rows: the residual's gradient has the residual's own, and memory of its own."""
+    x, r, w, w1 = _leaves(shape, other, (8,), (8, 8))
+    for f, want in ((lambda: sum(t.sin().sum() for t in nn.rms_norm(x, w, r)),
+                     lambda: sum(t.sin().sum() for t in ref.norm(x.view(-1, 8), w, r.view(-1, 8)))),
+                    (lambda: nn.linear(x, w1, None, "gelu", r).sin().sum(),
+                     lambda: (ref.act(x.view(-1, 8) @ w1, "gelu") + r.view(-1, 8)).sin().sum())):
+        grads = []
+        for g in (f, want):
+            x.grad = r.grad = None
+            g().backward()
+            grads.append((x.grad, r.grad))
+            assert x.grad.shape == x.shape and r.grad.shape == r.shape
+            assert g is want or x.grad.data_ptr() != r.grad.data_ptr()
+        for a, c in zip(*grads):
+            assert torch.allclose(a, c, rtol=1e-10)
