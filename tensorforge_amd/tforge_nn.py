@@ -89,8 +89,10 @@ class _RmsNorm(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dy, dh):
         h, weight = ctx.saved_tensors
-        dy = torch.zeros_like(h) if dy is None else dy.contiguous()
-        dx, dw = rms_norm_grad(dy, h, weight, ctx.eps, None if dh is None else dh.contiguous())
+        if dy is None:  # h's alone, past the norm
+            dx, dw = dh, None
+        else:
+            dx, dw = rms_norm_grad(dy.contiguous(), h, weight, ctx.eps, None if dh is None else dh.contiguous())
         if ctx.added is None:
             return dx, dw, None, None
         # A view would be another tensor on dx's memory, and both could become a leaf's grad.

@@ -166,3 +166,14 @@ def test_a_residual_of_other_leading_dimensions(shape, other, plain):
             assert g is want or x.grad.data_ptr() != r.grad.data_ptr()
         for a, c in zip(*grads):
             assert torch.allclose(a, c, rtol=1e-10)
+
+
+def test_a_loss_on_h_alone(plain):
+    """The norm is not part of it: the gradients are h's, also where h holds an infinity."""
+    x, w, r = _leaves((4, 8), (8,), (4, 8))
+    with torch.no_grad():
+        x[1, 2] = float("inf")
+    _, h = nn.rms_norm(x, w, r)
+    gh = torch.arange(32.0, dtype=torch.float64).view(4, 8)
+    gx, gw, gr = torch.autograd.grad(h, (x, w, r), gh, allow_unused=True)
+    assert torch.equal(gx, gh) and torch.equal(gr, gh) and gw is None
