@@ -17,7 +17,7 @@
 namespace tfnn {
 namespace {
 
-// Row lengths: WHOLE, a multiple of 8; TAIL, at least 8; ANY (the long kernels).
+// Row lengths: WHOLE, a multiple of 8; TAIL, at least 8; ANY, shorter ones too.
 enum Length { WHOLE, TAIL, ANY };
 
 // 8 elements from c of a row of `length`; zeros past its end.
@@ -176,13 +176,13 @@ __global__ __launch_bounds__(256) void rms_norm_long_kernel(NormParams p) {
   float sum = 0.0f, top = 0.0f;
   for (int c = threadIdx.x * 8; c < p.d; c += NT * 8) {
     float v[8], u[8], w[8];
-    load8<ANY>(x, c, p.d, v);
+    load8<TAIL>(x, c, p.d, v);
     if (res) {
-      load8<ANY>(res, c, p.d, u);
+      load8<TAIL>(res, c, p.d, u);
 #pragma unroll
       for (int i = 0; i < 8; ++i) v[i] += u[i];
     }
-    load_weight8<ANY>(p, c, w);
+    load_weight8<TAIL>(p, c, w);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       sum = __builtin_fmaf(v[i], v[i], sum);
@@ -199,14 +199,14 @@ __global__ __launch_bounds__(256) void rms_norm_long_kernel(NormParams p) {
   }
   for (int c = threadIdx.x * 8; c < p.d; c += NT * 8) {
     float v[8], u[8], w[8];
-    load8<ANY>(x, c, p.d, v);
+    load8<TAIL>(x, c, p.d, v);
     if (res) {
-      load8<ANY>(res, c, p.d, u);
+      load8<TAIL>(res, c, p.d, u);
 #pragma unroll
       for (int i = 0; i < 8; ++i) v[i] += u[i];
       store8(static_cast<T *>(p.h) + row * p.h_ld + c, p.d - c, v);
     }
-    load_weight8<ANY>(p, c, w);
+    load_weight8<TAIL>(p, c, w);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       v[i] = v[i] * r * w[i];
@@ -330,9 +330,9 @@ __global__ __launch_bounds__(256) void rms_norm_grad_long_kernel(NormGradParams 
     float sum = 0.0f, dot = 0.0f;
     for (int c = threadIdx.x * 8; c < p.d; c += NT * 8) {
       float h[8], g[8], w[8];
-      load8<ANY>(hp, c, p.d, h);
-      load8<ANY>(gp, c, p.d, g);
-      load_weight8<ANY>(wp, c, w);
+      load8<TAIL>(hp, c, p.d, h);
+      load8<TAIL>(gp, c, p.d, g);
+      load_weight8<TAIL>(wp, c, w);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         sum = __builtin_fmaf(h[i], h[i], sum);
@@ -345,11 +345,11 @@ __global__ __launch_bounds__(256) void rms_norm_grad_long_kernel(NormGradParams 
     const float k = dot * r * r / static_cast<float>(p.d);
     for (int c = threadIdx.x * 8; c < p.d; c += NT * 8) {
       float h[8], g[8], w[8], u[8], s[8];
-      load8<ANY>(hp, c, p.d, h);
-      load8<ANY>(gp, c, p.d, g);
-      load_weight8<ANY>(wp, c, w);
-      if (p.dh) load8<ANY>(static_cast<const T *>(p.dh) + row * p.dh_ld, c, p.d, u);
-      if (!first) load8<ANY>(share, c, p.d, s);
+      load8<TAIL>(hp, c, p.d, h);
+      load8<TAIL>(gp, c, p.d, g);
+      load_weight8<TAIL>(wp, c, w);
+      if (p.dh) load8<TAIL>(static_cast<const T *>(p.dh) + row * p.dh_ld, c, p.d, u);
+      if (!first) load8<TAIL>(share, c, p.d, s);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         s[i] = __builtin_fmaf(g[i] * r, h[i], first ? 0.0f : s[i]);
@@ -374,12 +374,14 @@ constexpr long kNormGroups = 2048;
 // The register kernels hold up to 64 elements a thread.
 constexpr int kLongest = 16384;
 
+unsigned wave_groups(long rows) { return static_cast<unsigned>(std::min<long>((rows + 3) / 4, kNormGroups)); }
+
 int pieces(long d) { return static_cast<int>((d + 7) / 8); }
 
 template <typename T, typename O, Length L>
 void norm_launch_as(const NormParams &p, hipStream_t stream) {
   const int n = pieces(p.d);
-  const dim3 waves(static_cast<unsigned>(std::min<long>((p.rows + 3) / 4, kNormGroups)));
+  const dim3 waves(wave_groups(p.rows));
   const dim3 groups(static_cast<unsigned>(std::min<long>(p.rows, kNormGroups)));
   if (n <= 64) rms_norm_kernel<T, O, 64, 1, L><<<waves, 256, 0, stream>>>(p);
   else if (n <= 128) rms_norm_kernel<T, O, 64, 2, L><<<waves, 256, 0, stream>>>(p);
@@ -389,9 +391,13 @@ void norm_launch_as(const NormParams &p, hipStream_t stream) {
   else rms_norm_kernel<T, O, 256, 8, L><<<groups, 256, 0, stream>>>(p);
 }
 
+// A launch takes fewer than 2^32 threads.  Long rows come one a workgroup: 2^24 of them
+// would be 512 GB.  Rows under 8 elements take a wave each, of the same bounded number: one
+// a workgroup took 979 us for 1048576 x 4 bfloat16, this way 187 (and its gradient 791, 7535 so).
 template <typename T, typename O>
 void norm_launch(const NormParams &p, hipStream_t stream) {
-  if (p.d < 8 || p.d > kLongest) rms_norm_long_kernel<T, O><<<dim3(static_cast<unsigned>(p.rows)), 256, 0, stream>>>(p);
+  if (p.d > kLongest) rms_norm_long_kernel<T, O><<<dim3(static_cast<unsigned>(p.rows)), 256, 0, stream>>>(p);
+  else if (p.d < 8) rms_norm_kernel<T, O, 64, 1, ANY><<<dim3(wave_groups(p.rows)), 256, 0, stream>>>(p);
   else if (p.d % 8 == 0) norm_launch_as<T, O, WHOLE>(p, stream);
   else norm_launch_as<T, O, TAIL>(p, stream);
 }
@@ -410,10 +416,11 @@ void norm_grad_launch_as(const NormGradParams &p, dim3 grid, hipStream_t stream)
 template <typename T>
 hipError_t norm_grad_launch(NormGradParams p, hipStream_t stream) {
   const long shares = norm_grad_shares(p.rows, p.d);
-  if (shares == 1 && p.d >= 8 && p.d <= kLongest) p.shares = nullptr;
+  if (shares == 1 && p.d <= kLongest) p.shares = nullptr;
   const dim3 grid(static_cast<unsigned>(shares));
   if (shares) {
-    if (p.d < 8 || p.d > kLongest) rms_norm_grad_long_kernel<T><<<grid, 256, 0, stream>>>(p);
+    if (p.d > kLongest) rms_norm_grad_long_kernel<T><<<grid, 256, 0, stream>>>(p);
+    else if (p.d < 8) rms_norm_grad_kernel<T, 64, 1, ANY><<<grid, 64 * grad_rows(64, 1), 0, stream>>>(p);
     else if (p.d % 8 == 0) norm_grad_launch_as<T, WHOLE>(p, grid, stream);
     else norm_grad_launch_as<T, TAIL>(p, grid, stream);
     const hipError_t e = hipGetLastError();
@@ -432,10 +439,10 @@ hipError_t norm_grad_launch(NormGradParams p, hipStream_t stream) {
 // with it, 6.0 without; 2 x 4032 8.8 and 6.1).
 long norm_grad_shares(long rows, long d) {
   const int n = pieces(d);
-  const long at_a_time = d < 8 || n > 256 ? 1 : n <= 128 ? 4 : 2;  // grad_rows of the kernel that runs
+  const long at_a_time = n > 256 ? 1 : n <= 128 ? 4 : 2;  // grad_rows of the kernel that runs
   const long steps = n <= 256 ? 5 : n <= 512 ? 4 : n <= 1024 ? 2 : 1;
-  if (d >= 8 && d <= kLongest && rows <= steps * at_a_time) return rows > 0;
-  const long most = n <= 256 || d < 8 ? 512 : n <= 512 ? 768 : n <= 1024 ? 512 : 256;
+  if (d <= kLongest && rows <= steps * at_a_time) return rows > 0;
+  const long most = n <= 256 ? 512 : n <= 512 ? 768 : n <= 1024 ? 512 : 256;
   return std::min<long>((rows + at_a_time - 1) / at_a_time, most);
 }
 

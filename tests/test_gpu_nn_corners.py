@@ -162,3 +162,33 @@ def test_a_residual_of_other_leading_dimensions():
         assert a.grad.shape == a.shape and b.grad.shape == b.shape
         grads.append((a.grad.view(6, 64), b.grad))
     assert all(torch.equal(p, q) for p, q in zip(*grads))
+
+
+@pytest.mark.parametrize("d", [1, 4, 7])
+def test_many_short_rows(d):
+    """More rows than a launch has places for workgroups of one row each; every row's result."""
+    nn = _nn()
+    rows = (1 << 24) + 5
+    g = torch.Generator(device="cuda").manual_seed(d)
+    x = torch.randn(rows, d, generator=g, device="cuda").bfloat16()
+    w = 1 + 0.1 * torch.randn(d, generator=g, device="cuda")
+    with torch.no_grad():
+        f = x.float()
+        r = torch.rsqrt((f * f).mean(1, keepdim=True) + 1e-6)
+        want = f * r * w
+    y, _ = nn.rms_norm(x, w)
+    assert ((y.float() - want).abs() <= (ref.U[torch.bfloat16] + 64 * ref.u) * want.abs()).all()
+    q, s = nn.quantize_rows(x)
+    top = f.abs().amax(1).clamp_min(ref.TINY)
+    assert ((s * 448 - top).abs() <= 4 * ref.u * top).all()
+    # codes are off by half a spacing, 1/16 of the value at most, or of the smallest normal number
+    assert ((q.float() * s[:, None] - f).abs() <= 0.0626 * torch.maximum(f.abs(), s[:, None] * 2.0 ** -6)).all()
+    dy = torch.randn(rows, d, generator=g, device="cuda").bfloat16()
+    dx, dw = nn.rms_norm_grad(dy, x, w)
+    gw = dy.float() * w
+    size = r * (gw.abs() + (f * r).abs() * (gw * f * r).abs().mean(1, keepdim=True))
+    want = r * (gw - f * r * (gw * f * r).mean(1, keepdim=True))
+    assert ((dx.float() - want).abs() <= ref.U[torch.bfloat16] * want.abs() + 64 * ref.u * size + 2.0 ** -133).all()
+    want = (dy.double() * f * r).sum(0)
+    # 512 shares of 8192 rows each
+    assert ((dw - want).abs() <= 2 * (rows // 2048 + 64) * ref.u * (dy.double() * f * r).abs().sum(0)).all()

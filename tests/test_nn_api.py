@@ -151,23 +151,20 @@ def test_python_refusals():
             call()
 
 
-# Stands in for HIP's launches in a process without a GPU: prints each launch's grid and block, refuses what HIP refuses
-# (2^32 threads or more along x) and the launch that FAIL_AT names, and keeps the last error as HIP does.
+# Stands in for HIP's launches in a process without a GPU: refuses what HIP refuses (2^32 threads or more along a side)
+# and the launch that arm() names, and keeps the last error as HIP does.  arm() returns the launches since the last.
 STUB = """
-#include <stdio.h>
-#include <stdlib.h>
 #include <stddef.h>
 typedef struct { unsigned x, y, z; } dim3;
-static int last, launches;
+static int last, launches, fail = -1;
 static dim3 grid, block;
 static size_t shared;
 static void *stream;
+int arm(int fail_at) { int n = launches; launches = 0; last = 0; fail = fail_at; return n; }
 int __hipPushCallConfiguration(dim3 g, dim3 b, size_t n, void *s) { grid = g; block = b; shared = n; stream = s; return 0; }
 int __hipPopCallConfiguration(dim3 *g, dim3 *b, size_t *n, void **s) { *g = grid; *b = block; *n = shared; *s = stream; return 0; }
 int hipLaunchKernel(const void *f, dim3 g, dim3 b, void **args, size_t n, void *s) {
-  const char *at = getenv("FAIL_AT");
-  int bad = (unsigned long long)g.x * b.x >> 32 || (unsigned long long)g.y * b.y >> 32 || (at && atoi(at) == launches);
-  fprintf(stderr, "launch %u %u %u %u\\n", g.x, g.y, b.x, b.y);
+  int bad = (unsigned long long)g.x * b.x >> 32 || (unsigned long long)g.y * b.y >> 32 || launches == fail;
   ++launches;
   if (bad) last = 9;
   return bad ? 9 : 0;
@@ -175,41 +172,61 @@ int hipLaunchKernel(const void *f, dim3 g, dim3 b, void **args, size_t n, void *
 int hipGetLastError(void) { int e = last; last = 0; return e; }
 """
 
+HEAD = """
+import ctypes
+from tensorforge_amd import _lib
+lib, stub, ref = _lib.lib(), ctypes.CDLL(None), ctypes.byref
+
+def norm(d, rows, residual=0, y_type=1):
+    a = _lib.RmsNormArgs(x=256, weight=256, y=256, scale=256, residual=residual, h=residual, x_ld=d, y_ld=d, residual_ld=d, h_ld=d,
+                         rows=rows, d=d, type=1, weight_type=1, y_type=y_type)
+    return lib.tf_rms_norm(ref(a), None)
+
+def norm_grad(d, rows):
+    a = _lib.RmsNormGradArgs(dy=256, h=256, weight=256, dx=256, dweight=256, dy_ld=d, h_ld=d, dx_ld=d, rows=rows, d=d, type=1,
+                             weight_type=1, workspace=256, workspace_bytes=1 << 60)
+    return lib.tf_rms_norm_grad(ref(a), None)
+"""
+
 
 @pytest.fixture(scope="module")
 def without_gpu(tmp_path_factory):
-    """run(code, fail_at=None): code in a process with the stub before HIP; (its output, the launches)."""
+    """Runs code, after HEAD, in a process with the stub before HIP."""
     at = tmp_path_factory.mktemp("stub")
     (at / "stub.c").write_text(STUB)
     subprocess.run(["gcc", "-shared", "-fPIC", str(at / "stub.c"), "-o", str(at / "stub.so")], check=True)
+    preload = " ".join([str(at / "stub.so"), os.environ.get("LD_PRELOAD", "")]).strip()
+    env = {**os.environ, "LD_PRELOAD": preload, "HIP_VISIBLE_DEVICES": "-1", "ROCR_VISIBLE_DEVICES": "-1",
+           "PYTHONPATH": str(_lib.PKG.parent)}
 
-    def run(code, fail_at=None):
-        preload = " ".join([str(at / "stub.so"), os.environ.get("LD_PRELOAD", "")]).strip()
-        env = {**os.environ, "LD_PRELOAD": preload, "HIP_VISIBLE_DEVICES": "-1", "ROCR_VISIBLE_DEVICES": "-1", "PYTHONPATH": str(_lib.PKG.parent)}
-        if fail_at is not None:
-            env["FAIL_AT"] = str(fail_at)
-        head = "import ctypes\nfrom tensorforge_amd import _lib\nlib, ref = _lib.lib(), ctypes.byref\n"
-        r = subprocess.run([sys.executable, "-c", head + code], env=env, capture_output=True, text=True)
+    def run(code):
+        r = subprocess.run([sys.executable, "-c", HEAD + code], env=env, capture_output=True, text=True)
         assert r.returncode == 0, r.stdout + r.stderr
-        return r.stdout, [tuple(int(v) for v in l.split()[1:]) for l in r.stderr.splitlines() if l.startswith("launch ")]
 
     return run
 
 
-NORM_GRAD = """
-d, rows = {d}, {rows}
-a = _lib.RmsNormGradArgs(dy=256, h=256, weight=256, dx=256, dweight=256, dy_ld=d, h_ld=d, dx_ld=d, rows=rows, d=d, type=1,
-                         weight_type=1, workspace=256, workspace_bytes=1 << 40)
-print(lib.tf_rms_norm_grad(ref(a), None))
-"""
-
-
-@pytest.mark.parametrize("rows,d", [(4, 64), (4000, 64), (4000, 4000), (5, 4), (70, 20000), (0, 64)])
-def test_failed_launches_of_the_norm_gradient(rows, d, without_gpu):
+def test_failed_launches_of_the_norm_gradient(without_gpu):
     """Whichever of its launches fails, the call says so."""
-    code = NORM_GRAD.format(rows=rows, d=d)
-    out, launches = without_gpu(code)
-    assert out.split() == ["0"] and 1 <= len(launches) <= 2
-    for i in range(len(launches)):
-        out, _ = without_gpu(code, fail_at=i)
-        assert out.split() == ["-5"], i
+    without_gpu("""
+for rows, d in ((4, 64), (4000, 64), (4000, 4000), (5, 4), (70, 20000), (0, 64)):
+    stub.arm(-1)
+    assert norm_grad(d, rows) == 0
+    launches = stub.arm(-1)
+    assert 1 <= launches <= 2
+    for i in range(launches):
+        stub.arm(i)
+        assert norm_grad(d, rows) == -5, (rows, d, i)
+""")
+
+
+def test_norms_of_many_rows_launch(without_gpu):
+    """No launch has 2^32 threads, up to the largest sizes that fit a memory of 288 GB."""
+    without_gpu("""
+for rows, d in ((1 << 24, 4), (1 << 30, 1), (1 << 30, 7), (1 << 30, 0), (1 << 30, 64), (1 << 26, 2000), (1 << 22, 20000)):
+    for residual in (0, 256):
+        for y_type in (1, 3):
+            assert norm(d, rows, residual, y_type) == 0, (rows, d)
+    assert lib.tf_quantize_rows(256, d, rows, d, 1, 256, d, 256, None) == 0
+    assert norm_grad(d, rows) == 0, (rows, d)
+""")
