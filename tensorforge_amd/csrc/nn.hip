@@ -251,10 +251,16 @@ Plan plan_product(const Product &q, bool dma, int tile, int splits) {
   const bool amn = q.a.mn, bmn = q.b.mn;
   const int size = size_of(type);
   const long slabs = ceil_div(k, 128 / size);
-  const bool rows = m * terms <= 64 && !amn && (!bmn || n >= 32);
+  // A launch takes fewer than 2^32 threads.  (Through registers its grid may have two sides.)
+  const auto fits = [&](int t, long ranges) {
+    const long blocks = t == TILE_ROWS ? ceil_div(n, bmn ? 32 : 16) : ceil_div(m, tile_rows(t)) * ceil_div(n, tile_columns(t)) * ranges;
+    return blocks * tile_threads(t) < (1L << 32);
+  };
+  const bool rows = m * terms <= 64 && !amn && (!bmn || n >= 32) && fits(TILE_ROWS, 1);
   if (tile == TILE_ROWS && rows) return {TILE_ROWS, 1, 0};
   if (tile == TILE_ROWS || (!dma && tile != TILE_64) || (terms > 1 && tile == TILE_256)) tile = 0;
   splits = static_cast<int>(std::max<long>(0, std::min<long>(splits, std::max<long>(1, slabs))));
+  if (tile && dma && !fits(tile, std::max(1, splits))) tile = 0;
   Plan best{TILE_64, 1, 1e30};
   const double read = (static_cast<double>(m) + n) * k * terms * size / 8e6;
   if (rows && !tile) {
@@ -267,11 +273,12 @@ Plan plan_product(const Product &q, bool dma, int tile, int splits) {
   for (int t : {TILE_64, TILE_64x128, TILE_128, TILE_256}) {
     if (tile ? t != tile : (t != TILE_64 && !dma) || (t == TILE_256 && terms > 1)) continue;
     // Tiles mostly empty, and splits into more than four workgroups a CU, never win.
-    if (!tile && t != TILE_64 && (2 * m <= tile_rows(t) || 2 * n <= tile_columns(t))) continue;
+    if (!tile && t != TILE_64 && fits(TILE_64, 1) && (2 * m <= tile_rows(t) || 2 * n <= tile_columns(t))) continue;
     const long tiles = ceil_div(m, tile_rows(t)) * ceil_div(n, tile_columns(t));
     for (int s : {1, 2, 3, 4, 6, 8, 12, 16}) {
       if (s > 1 && (splits || s * 2 > slabs || tiles * s > 1024)) break;
       const int ranges = splits ? splits : s;
+      if (dma && !fits(t, ranges)) continue;
       const double us = predicted(m, n, slabs * terms, read, dma, size == 1, t, ranges);
       if (us < best.us) best = {t, ranges, us};
     }

@@ -145,6 +145,14 @@ __device__ __forceinline__ void store_as(void *out, int type, long i, float v) {
   else static_cast<f16 *>(out)[i] = static_cast<f16>(v);
 }
 
+// A launch takes fewer than 2^32 threads along a side: workgroups beyond 2^31 of them go
+// along y.  The last row of workgroups may have some too many.
+inline dim3 grid_of(long blocks, int threads) {
+  const long most = (1L << 31) / threads;
+  return blocks <= most ? dim3(static_cast<unsigned>(blocks)) : dim3(static_cast<unsigned>(most), static_cast<unsigned>((blocks + most - 1) / most));
+}
+__device__ __forceinline__ long block_of() { return blockIdx.x + static_cast<long>(blockIdx.y) * gridDim.x; }
+
 // Sum / maximum over groups of 64 lanes; every lane gets the result.
 __device__ __forceinline__ float wave_sum(float v) {
 #pragma unroll

@@ -604,7 +604,12 @@ __device__ __forceinline__ void gemm_tile(const GemmParams &p, int block, int bl
 template <typename T, typename O, bool AMN, bool BMN, int BM, int BN, int WM, int WN, int ST, bool DMA>
 __global__ __launch_bounds__(64 * WM *WN, DMA ? 1 : 3) void gemm_tile_kernel(GemmParams p) {
   __shared__ __align__(1024) char smem[tile_lds<BM, BN, ST>()];
-  gemm_tile<T, O, AMN, BMN, BM, BN, WM, WN, ST, DMA>(p, blockIdx.x, gridDim.x, (lds_char *)smem);
+  if constexpr (DMA) {
+    gemm_tile<T, O, AMN, BMN, BM, BN, WM, WN, ST, DMA>(p, blockIdx.x, gridDim.x, (lds_char *)smem);
+  } else {  // the one tile of odd operands: also where its grid has a second side
+    const int block = static_cast<int>(block_of()), blocks = p.tiles_m * p.tiles_n * p.splits;
+    if (block < blocks) gemm_tile<T, O, AMN, BMN, BM, BN, WM, WN, ST, DMA>(p, block, blocks, (lds_char *)smem);
+  }
 }
 
 // A small layer's two gradient products in one launch: dx (its left operand along

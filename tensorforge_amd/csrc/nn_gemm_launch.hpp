@@ -18,8 +18,9 @@ hipError_t launch_layout(const GemmParams &p, int tile, bool dma, hipStream_t st
       return hipGetLastError();
     }
   }
-  const dim3 grid(static_cast<unsigned>(p.tiles_m) * p.tiles_n * p.splits);
-  if (dma) {
+  const long blocks = static_cast<long>(p.tiles_m) * p.tiles_n * p.splits;
+  if (dma) {  // one-sided: plan_product leaves out what does not fit
+    const dim3 grid(static_cast<unsigned>(blocks));
     if (tile == TILE_256) gemm_wide_kernel<T, O, AMN, BMN><<<grid, 512, 0, stream>>>(p);
     else if (tile == TILE_128) gemm_tile_kernel<T, O, AMN, BMN, 128, 128, 2, 2, 2, true><<<grid, 256, 0, stream>>>(p);
     else if (tile == TILE_64x128) gemm_tile_kernel<T, O, AMN, BMN, 64, 128, 2, 2, 3, true><<<grid, 256, 0, stream>>>(p);
@@ -29,7 +30,7 @@ hipError_t launch_layout(const GemmParams &p, int tile, bool dma, hipStream_t st
     else if (grid.x <= 768) gemm_tile_kernel<T, O, AMN, BMN, 64, 64, 2, 2, 3, true><<<grid, 256, 0, stream>>>(p);
     else gemm_tile_kernel<T, O, AMN, BMN, 64, 64, 2, 2, 2, true><<<grid, 256, 0, stream>>>(p);
   } else {
-    gemm_tile_kernel<T, O, AMN, BMN, 64, 64, 2, 2, 2, false><<<grid, 256, 0, stream>>>(p);
+    gemm_tile_kernel<T, O, AMN, BMN, 64, 64, 2, 2, 2, false><<<grid_of(blocks, 256), 256, 0, stream>>>(p);
   }
   return hipGetLastError();
 }

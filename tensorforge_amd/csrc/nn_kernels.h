@@ -48,6 +48,7 @@ struct GemmParams {
 // operand along k only).
 enum Tile { TILE_256 = 1, TILE_128 = 2, TILE_64 = 3, TILE_ROWS = 4, TILE_64x128 = 5 };
 constexpr int tile_rows(int tile) { return tile == TILE_256 ? 256 : tile == TILE_128 ? 128 : 64; }
+constexpr int tile_threads(int tile) { return tile == TILE_256 ? 512 : tile == TILE_ROWS ? 1024 : 256; }  // at most
 constexpr int tile_columns(int tile) { return tile == TILE_64x128 ? 128 : tile_rows(tile); }
 
 // amn, bmn: the operand's own dimension (m, n) is contiguous, not k.

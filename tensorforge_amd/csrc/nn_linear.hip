@@ -13,8 +13,8 @@ namespace {
 // workgroups instead, behind a fence, the whole product took 22.9 us against 13.1: the caches'
 // write-back costs more than the launch.)
 template <typename O, int ACT>
-__device__ __forceinline__ void join_four(const GemmParams &p, int block) {
-  const long ld = (p.n + 3) & ~3, id = static_cast<long>(block) * 256 + threadIdx.x;
+__device__ __forceinline__ void join_four(const GemmParams &p, long block) {
+  const long ld = (p.n + 3L) & ~3L, id = block * 256 + threadIdx.x;
   const int m = static_cast<int>(id / (ld / 4)), n = static_cast<int>(id % (ld / 4)) * 4;
   if (m >= p.m) return;
   const float *part = p.parts + m * ld + n;
@@ -33,7 +33,7 @@ __device__ __forceinline__ void join_four(const GemmParams &p, int block) {
 }
 template <typename O, int ACT>
 __global__ __launch_bounds__(256) void gemm_join_kernel(GemmParams p) {
-  join_four<O, ACT>(p, blockIdx.x);
+  join_four<O, ACT>(p, block_of());
 }
 template <typename O>
 __global__ __launch_bounds__(256) void gemm_join_pair_kernel(GemmParams dx, GemmParams dw, int first) {
@@ -42,13 +42,11 @@ __global__ __launch_bounds__(256) void gemm_join_pair_kernel(GemmParams dx, Gemm
   else join_four<O, ACT_NONE>(dw, block - first);
 }
 
-unsigned join_blocks(const GemmParams &p) {
-  return static_cast<unsigned>((static_cast<long>(p.m) * ((p.n + 3) / 4) + 255) / 256);
-}
+long join_blocks(const GemmParams &p) { return (p.m * ((p.n + 3L) / 4) + 255) / 256; }
 
 template <typename O>
 void join(const GemmParams &p, hipStream_t stream) {
-  const dim3 grid(join_blocks(p));
+  const dim3 grid = grid_of(join_blocks(p), 256);
   if (p.act == ACT_RELU) gemm_join_kernel<O, ACT_RELU><<<grid, 256, 0, stream>>>(p);
   else if (p.act == ACT_GELU) gemm_join_kernel<O, ACT_GELU><<<grid, 256, 0, stream>>>(p);
   else if (p.act == ACT_SILU) gemm_join_kernel<O, ACT_SILU><<<grid, 256, 0, stream>>>(p);
@@ -58,9 +56,9 @@ void join(const GemmParams &p, hipStream_t stream) {
 // Copies to aligned lines, 16 bytes a thread.  Bound by memory: 7168 x 2107 and 8063 x 2107
 // bfloat16 23 us (64 MB read and written, 5.6 TB/s).
 template <typename T>
-__device__ __forceinline__ void pack_piece(const PackParams &p, int block) {
+__device__ __forceinline__ void pack_piece(const PackParams &p, long block) {
   constexpr int N = kPiece<T>;
-  long id = static_cast<long>(block) * 256 + threadIdx.x;
+  long id = block * 256 + threadIdx.x;
   const int q = id >= p.pieces[0];
   if (q) id -= p.pieces[0];
   if (id >= p.pieces[q]) return;
@@ -71,9 +69,9 @@ __device__ __forceinline__ void pack_piece(const PackParams &p, int block) {
 }
 template <typename T>
 __global__ __launch_bounds__(256) void pack_kernel(PackParams p) {
-  pack_piece<T>(p, blockIdx.x);
+  pack_piece<T>(p, block_of());
 }
-unsigned pack_blocks(const PackParams &p) { return static_cast<unsigned>((p.pieces[0] + p.pieces[1] + 255) / 256); }
+long pack_blocks(const PackParams &p) { return (p.pieces[0] + p.pieces[1] + 255) / 256; }
 
 // Without a branch, also where columns end inside a piece: 4096 x 8191 bfloat16 gelu 49 us
 // against 80 with one (4096 x 8192 44 either way).
@@ -94,12 +92,13 @@ constexpr float largest = __is_same(T, f16) ? 65504.0f : 0x1.fep127f;  // finite
 // 141 float16 19.6 us with 64, 8.8 with 32; of all up to 256 rows where that saves the sum's launch.
 template <typename T, int ACT, int CT>
 __global__ __launch_bounds__(256) void act_slope_kernel(SlopeParams p, PackParams pack, int blocks) {
-  if (static_cast<int>(blockIdx.x) >= blocks) {
-    pack_piece<T>(pack, blockIdx.x - blocks);
+  const long block = block_of();
+  if (block >= blocks) {
+    pack_piece<T>(pack, block - blocks);
     return;
   }
   constexpr int LANES = 256 / CT, COLS = CT * 8;
-  const int column_blocks = (p.n + COLS - 1) / COLS, bc = blockIdx.x % column_blocks, br = blockIdx.x / column_blocks;
+  const int column_blocks = (p.n + COLS - 1) / COLS, bc = static_cast<int>(block) % column_blocks, br = static_cast<int>(block) / column_blocks;
   const int c = bc * COLS + threadIdx.x % CT * 8, lane = threadIdx.x / CT, left = p.n - c, rows = p.rows;
   const long row0 = static_cast<long>(br) * rows;
   float sum[8];
@@ -159,7 +158,7 @@ template <typename T, int ACT>
 void slope(const SlopeParams &p, const PackParams &pack, hipStream_t stream) {
   const int columns = p.rows == SLOPE_WHOLE ? 32 : p.rows == SLOPE_FEW ? 128 : 256;
   const int blocks = (p.m + p.rows - 1) / p.rows * ((p.n + columns - 1) / columns);
-  const dim3 grid(blocks + pack_blocks(pack));
+  const dim3 grid = grid_of(blocks + pack_blocks(pack), 256);
   if (p.rows == SLOPE_WHOLE) act_slope_kernel<T, ACT, 4><<<grid, 256, 0, stream>>>(p, pack, blocks);
   else if (p.rows == SLOPE_FEW) act_slope_kernel<T, ACT, 16><<<grid, 256, 0, stream>>>(p, pack, blocks);
   else act_slope_kernel<T, ACT, 32><<<grid, 256, 0, stream>>>(p, pack, blocks);
@@ -176,7 +175,7 @@ void slope(const SlopeParams &p, const PackParams &pack, hipStream_t stream) {
 }  // namespace
 
 hipError_t launch_pack(const PackParams &p, int size, hipStream_t stream) {
-  const dim3 grid(pack_blocks(p));
+  const dim3 grid = grid_of(pack_blocks(p), 256);
   size == 1 ? pack_kernel<f8><<<grid, 256, 0, stream>>>(p) : pack_kernel<bf16><<<grid, 256, 0, stream>>>(p);
   return hipGetLastError();
 }
@@ -187,9 +186,10 @@ hipError_t launch_gemm_join(const GemmParams &p, int out_type, hipStream_t strea
 }
 
 hipError_t launch_gemm_join_pair(const GemmParams &dx, const GemmParams &dw, int out_type, hipStream_t stream) {
-  const unsigned first = dx.splits > 1 ? join_blocks(dx) : 0, second = dw.splits > 1 ? join_blocks(dw) : 0;
-  if (out_type == TYPE_BF16) gemm_join_pair_kernel<bf16><<<dim3(first + second), 256, 0, stream>>>(dx, dw, first);
-  else gemm_join_pair_kernel<f16><<<dim3(first + second), 256, 0, stream>>>(dx, dw, first);
+  const int first = dx.splits > 1 ? static_cast<int>(join_blocks(dx)) : 0;
+  const dim3 grid(static_cast<unsigned>(first + (dw.splits > 1 ? join_blocks(dw) : 0)));  // small (plan_pair)
+  if (out_type == TYPE_BF16) gemm_join_pair_kernel<bf16><<<grid, 256, 0, stream>>>(dx, dw, first);
+  else gemm_join_pair_kernel<f16><<<grid, 256, 0, stream>>>(dx, dw, first);
   return hipGetLastError();
 }
 

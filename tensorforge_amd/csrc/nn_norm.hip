@@ -365,7 +365,7 @@ __global__ __launch_bounds__(256) void rms_norm_grad_long_kernel(NormGradParams 
 
 __global__ __launch_bounds__(256) void share_sum_kernel(const float *shares, int count, int d, void *out, int type) {
   __shared__ float part[64][17];
-  share_sum(shares, count, d, out, type, blockIdx.x, part);
+  share_sum(shares, count, d, out, type, static_cast<int>(block_of()), part);
 }
 
 // Workgroups beyond this many would each take few rows for the weights they load.
@@ -447,8 +447,7 @@ long norm_grad_shares(long rows, long d) {
 }
 
 hipError_t launch_share_sum(const float *shares, long count, int d, void *out, int type, hipStream_t stream) {
-  share_sum_kernel<<<dim3(static_cast<unsigned>((d + 15) / 16)), 256, 0, stream>>>(shares, static_cast<int>(count), d, out,
-                                                                                  type);
+  share_sum_kernel<<<grid_of((d + 15L) / 16, 256), 256, 0, stream>>>(shares, static_cast<int>(count), d, out, type);
   return hipGetLastError();
 }
 

@@ -192,3 +192,43 @@ def test_many_short_rows(d):
     want = (dy.double() * f * r).sum(0)
     # 512 shares of 8192 rows each
     assert ((dw - want).abs() <= 2 * (rows // 2048 + 64) * ref.u * (dy.double() * f * r).abs().sum(0)).all()
+
+
+def _normal(seed, *shape, dtype=torch.bfloat16):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return torch.randn(shape, generator=g, device="cuda", dtype=dtype)
+
+
+def test_sums_of_many_columns():
+    """The shares' sums over more columns than one side of a launch has places for."""
+    nn = _nn()
+    d = (1 << 28) + 24
+    h, dy, w = _normal(1, 1, d), _normal(2, 1, d), torch.ones(d, dtype=torch.bfloat16, device="cuda")
+    dx, dw = nn.rms_norm_grad(dy, h, w)
+    r = torch.rsqrt(h.float().square().mean() + 1e-6)
+    want = dy[0].float() * h[0].float() * r
+    # the row's sum: 2^20 additions a thread and the joining, halved by its root
+    assert ((dw.float() - want).abs() <= (ref.U[torch.bfloat16] + (1 << 18) * ref.u) * want.abs()).all()
+    assert dx.isfinite().all()
+    del h, dx, dw, w, want
+    n = (1 << 29) + 8
+    dy = dy.new_empty(1, n).normal_()
+    x = torch.full((1, 1), 2.0, dtype=torch.bfloat16, device="cuda")
+    _, dw, db = nn.linear_grad(dy, x, torch.zeros(1, n, dtype=torch.bfloat16, device="cuda"), want_dx=False, bias_dtype=torch.bfloat16)
+    assert torch.equal(db, dy[0]) and torch.equal(dw, 2 * dy)
+
+
+@pytest.mark.parametrize("order", [0, 1])
+def test_few_rows_of_many_columns(order):
+    """More columns than the few-row kernel's launch has places for."""
+    nn = _nn()
+    for m, n, k in ((1, (1 << 27) + 8, 8), (3, (1 << 26) + 3, 7)):
+        x = _normal(m, m, k)
+        w = _normal(5, k, n) if order == 0 else _normal(5, n, k).t()
+        out = nn.linear(x, w)
+        want, size = 0, 0
+        for j in range(k):
+            term = x[:, j:j + 1].float() * w[j].float()
+            want, size = want + term, size + term.abs()
+        assert ((out.float() - want).abs() <= ref.U[torch.bfloat16] * want.abs() + 4 * (k + 4) * ref.u * size).all()
+        del w, out, want, size

@@ -186,6 +186,23 @@ def norm_grad(d, rows):
     a = _lib.RmsNormGradArgs(dy=256, h=256, weight=256, dx=256, dweight=256, dy_ld=d, h_ld=d, dx_ld=d, rows=rows, d=d, type=1,
                              weight_type=1, workspace=256, workspace_bytes=1 << 60)
     return lib.tf_rms_norm_grad(ref(a), None)
+
+def linear(m, n, k, order, type=1, **kw):
+    a = _lib.LinearArgs(x=256, w=256, out=256, x_scale=256 * (type == 3), w_scale=256 * (type == 3), x_ld=k, w_ld=k if order else n, out_ld=n,
+                        m=m, n=n, k=k, w_order=order, type=type, out_type=1, workspace=256, **kw)
+    size = ctypes.c_longlong()
+    assert lib.tf_linear_workspace(ref(a), ref(size)) == 0
+    a.workspace_bytes = size.value
+    return lib.tf_linear(ref(a), None)
+
+def linear_grad(m, n, k, order, act=0, **kw):
+    a = _lib.LinearGradArgs(dy=256, x=256, w=256, z=256, dx=256, dw=256, dbias=256, workspace=256, dy_ld=n, x_ld=k, z_ld=n,
+                            w_ld=k if order else n, dx_ld=k, dw_ld=k if order else n, m=m, n=n, k=k, w_order=order, type=1, bias_type=1,
+                            act=act, **kw)
+    size = ctypes.c_longlong()
+    assert lib.tf_linear_grad_workspace(ref(a), ref(size)) == 0
+    a.workspace_bytes = size.value
+    return lib.tf_linear_grad(ref(a), None)
 """
 
 
@@ -229,4 +246,22 @@ for rows, d in ((1 << 24, 4), (1 << 30, 1), (1 << 30, 7), (1 << 30, 0), (1 << 30
             assert norm(d, rows, residual, y_type) == 0, (rows, d)
     assert lib.tf_quantize_rows(256, d, rows, d, 1, 256, d, 256, None) == 0
     assert norm_grad(d, rows) == 0, (rows, d)
+""")
+
+
+def test_products_of_extreme_sizes_launch(without_gpu):
+    """One side as long as the header allows: no launch has 2^32 threads."""
+    without_gpu("""
+big = 1 << 30
+sizes = [(1, 1 << 26, 8), (16, 1 << 26, 64), (1, 1 << 27, 8), (64, 1 << 28, 8), (1, big, 1), (3, big, 7), (64, big, 64), (big, 1, 1),
+         (big, 9, 8), (big, 64, 64), (big, 64, 8), (big - 63, 8, 16), (100, 1 << 29, 8), (65, big, 9), (1 << 20, 1 << 16, 5), (1, 1, big)]
+for m, n, k in sizes:
+    for order in (0, 1):
+        for tile in (0, 1, 2, 3, 4, 5):
+            assert linear(m, n, k, order, tile=tile) == 0, (m, n, k, order, tile)
+        for act in (0, 1, 2):
+            assert linear_grad(m, n, k, order, act) == 0, (m, n, k, order, act)
+        assert linear_grad(m, n, k, order, 2, tile=3, splits=2) == 0, (m, n, k, order)
+    assert linear(m, n, k, 1, type=3) == 0 and linear(m, n, k, 1, type=3, tile=3, splits=2) == 0, (m, n, k)
+assert norm_grad(big, 1) == 0 and norm_grad(big, 2) == 0
 """)
