@@ -294,8 +294,11 @@ long long part_bytes(long m, long n, const Plan &plan) {
 // copied to aligned lines first (pack) where the faster kernels gain more than the
 // copy takes, about 3.7 us and 0.21 for its 1e6 bytes; results in rows off 16 bytes then
 // take 0.28 more for each 1e6 (fitted to the same products; the choices take 1.8% longer than
-// the best).  4095 x 4097 x 1023 bfloat16 110 us through registers, 62 with both copied; 777 x
+// the best).  Long matrices of lines far shorter than a cache line, whose copies would take many
+// times their memory (2^30 rows of one element 128 GB for 2), stay as they are.  4095 x 4097 x 1023 bfloat16 110 us through registers, 62 with both copied; 777 x
 // 1111 x 333 6.2 and 10.4.
+constexpr long long kCopies = 256 << 20;  // bytes any copies may have
+
 struct Choice {
   Plan plan;
   bool dma = false, pack_a = false, pack_b = false;
@@ -314,10 +317,11 @@ Choice choose(const Product &q, int tile, int splits, bool packing = true) {
   c.us = c.plan.us;
   if (!c.dma && packing && p.k > 0 && c.plan.tile != TILE_ROWS) {
     const long long copies = (da ? 0 : packed_bytes(q.a, size)) + (db ? 0 : packed_bytes(q.b, size));
+    const long long own = ((da ? 0 : q.a.lines * q.a.length) + (db ? 0 : q.b.lines * q.b.length)) * size;
     const auto fits = [&](const Operand &o) { return 256 * packed_ld(o, size) * size + 1024 < (1L << 31); };
     const Plan fast = plan_product(q, true, tile, splits);
     const double us = fast.us + 3.7 + copies * 0.21e-6 + (p.n % 8 ? 0.28e-6 * p.m * p.n : 0);
-    if (fits(q.a) && fits(q.b) && ((tile && tile != TILE_64 && tile != TILE_ROWS) || us < c.us)) {
+    if (fits(q.a) && fits(q.b) && copies <= std::max(4 * own, kCopies) && ((tile && tile != TILE_64 && tile != TILE_ROWS) || us < c.us)) {
       c.plan = fast;
       c.us = us;
       c.dma = true;

@@ -232,3 +232,12 @@ def test_few_rows_of_many_columns(order):
             want, size = want + term, size + term.abs()
         assert ((out.float() - want).abs() <= ref.U[torch.bfloat16] * want.abs() + 4 * (k + 4) * ref.u * size).all()
         del w, out, want, size
+
+
+def test_a_product_of_very_many_rows():
+    """More tiles than one side of a launch has places for: rows of one element, multiplied where they lie."""
+    nn = _nn()
+    m = 1 << 30
+    x = torch.empty(m, 1, dtype=torch.bfloat16, device="cuda").normal_()
+    out = nn.linear(x, torch.full((1, 1), 2.0, dtype=torch.bfloat16, device="cuda"), torch.zeros(1, device="cuda"), "none")
+    assert torch.equal(out, 2 * x)

@@ -265,3 +265,16 @@ for m, n, k in sizes:
     assert linear(m, n, k, 1, type=3) == 0 and linear(m, n, k, 1, type=3, tile=3, splits=2) == 0, (m, n, k)
 assert norm_grad(big, 1) == 0 and norm_grad(big, 2) == 0
 """)
+
+
+def test_copies_of_short_lines_stay_small():
+    """Aligned copies of odd operands take at most four times their memory, or 256 MB."""
+    lib, size = _lib.lib(), ctypes.c_longlong()
+    for m, n, k in ((1 << 30, 1, 1), (1 << 28, 64, 5), (1 << 26, 300, 3), (1 << 22, 4096, 1), (5, 1 << 28, 7), (4096, 4096, 5)):
+        for order in (0, 1):
+            for type_ in (1, 3)[:1 + order]:
+                for tile in (0, 2):
+                    a = _lib.LinearArgs(x=256, w=256, out=256, x_ld=k, w_ld=k if order else n, out_ld=n, m=m, n=n, k=k, w_order=order,
+                                        type=type_, out_type=1, tile=tile, splits=1)
+                    assert lib.tf_linear_workspace(ctypes.byref(a), ctypes.byref(size)) == 0
+                    assert size.value <= max(4 * (m + n) * k * 2, 256 << 20), (m, n, k, order, type_, tile)
