@@ -241,3 +241,31 @@ def test_a_product_of_very_many_rows():
     x = torch.empty(m, 1, dtype=torch.bfloat16, device="cuda").normal_()
     out = nn.linear(x, torch.full((1, 1), 2.0, dtype=torch.bfloat16, device="cuda"), torch.zeros(1, device="cuda"), "none")
     assert torch.equal(out, 2 * x)
+
+
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("activation", ["gelu", "silu"])
+def test_activations_of_every_value(activation, dtype):
+    """Every finite z: the value and the slope off by their rounding and 1e-5 of themselves (exponents of up to 126 halvings,
+    each rounded in float: 126 * ln 2 * 2^-24), 1e-6 where the slope crosses zero.  A factor below the smallest normal
+    number may be flushed to zero before z multiplies it."""
+    nn = _nn()
+    z = torch.arange(-32768, 32768, dtype=torch.int32).to(torch.int16).view(dtype)
+    z = z[z.isfinite()]
+    z = torch.cat([z, torch.zeros(-len(z) % 8, dtype=dtype)]).view(-1, 8)
+    zd = z.double()
+    eye = torch.eye(8, dtype=dtype).cuda()
+    out = nn.linear(z.cuda(), eye, None, activation)
+    flushed = lambda v: torch.finfo(torch.float32).tiny * (1 + v.abs().clamp_max(200))  # noqa: E731
+    want = ref.act(zd, activation)
+    ref.close(out, want, 1e-5 * want.abs() + flushed(zd), dtype)
+    dy = torch.ones_like(z)
+    _, _, db = nn.linear_grad(dy[:1].cuda(), dy[:1].cuda(), eye, z[:1].cuda(), activation, bias_dtype=torch.float32)
+    assert db.shape == (8,)
+    # dx of one row through the unit matrix: dz itself, in two terms
+    step = 2048
+    for at in range(0, len(z), step):
+        part = z[at:at + step]
+        dx, _, _ = nn.linear_grad(dy[at:at + step].cuda(), part.cuda(), eye, part.cuda(), activation, want_dw=False)
+        want = ref.slope(part.double(), activation)
+        ref.close(dx, want, 1e-5 * want.abs() + 1e-6 * (part.abs() < 3) + flushed(part.double()), dtype)
