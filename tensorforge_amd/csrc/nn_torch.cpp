@@ -142,7 +142,11 @@ Tensor fresh(const Tensor &like, at::IntArrayRef size, ScalarType type) {
   return at::detail::empty_cuda(size, type, like.device(), std::nullopt);
 }
 
-void check(int rc) { TORCH_CHECK(rc >= 0, tf_last_error()); }
+// What the library refuses is a ValueError, what HIP reports a RuntimeError.
+void check(int rc) {
+  TORCH_CHECK_VALUE(rc != TF_E_ARG, tf_last_error());
+  TORCH_CHECK(rc >= 0, tf_last_error());
+}
 
 PyObject *wrap(const Tensor *t) {
   if (!t) Py_RETURN_NONE;
@@ -158,10 +162,11 @@ PyObject *tuple(std::initializer_list<const Tensor *> all) {
 
 void count(Py_ssize_t got, Py_ssize_t want) { TORCH_CHECK_TYPE(got == want, "takes ", want, " arguments, got ", got); }
 
-long integer(PyObject *o) {
+int integer(PyObject *o, const char *name) {
   const long v = PyLong_AsLong(o);
   if (v == -1 && PyErr_Occurred()) throw python_error();
-  return v;
+  TORCH_CHECK_VALUE(v == static_cast<int>(v), name, " = ", v, " is out of range");
+  return static_cast<int>(v);
 }
 
 double number(PyObject *o) {
@@ -284,8 +289,8 @@ PyObject *linear(PyObject *, PyObject *const *a, Py_ssize_t n) {
   const Weights wr = weights(w, xr.n, t);
   tf_linear_args_t g{};
   g.x = xr.p, g.x_ld = xr.ld, g.m = xr.m, g.k = xr.n, g.w = wr.p, g.w_ld = wr.ld, g.n = wr.n, g.w_order = wr.order;
-  g.type = type_of(t), g.out_type = type_of(to), g.act = static_cast<int>(integer(a[3]));
-  g.tile = static_cast<int>(integer(a[9])), g.splits = static_cast<int>(integer(a[10]));
+  g.type = type_of(t), g.out_type = type_of(to), g.act = integer(a[3], "activation");
+  g.tile = integer(a[9], "tile"), g.splits = integer(a[10], "splits");
   if (bias) g.bias = vector(*bias, "bias", wr.n, to, ScalarType::Float), g.bias_type = type_of(bias->scalar_type());
   if (residual) {
     const Rows r = rows_of(*residual, "residual", xr.m, wr.n, to);
@@ -330,8 +335,8 @@ PyObject *linear_grad(PyObject *, PyObject *const *a, Py_ssize_t n) {
   const Rows gr = rows_of(dy, "dy", xr.m, wr.n, t);
   tf_linear_grad_args_t g{};
   g.dy = gr.p, g.dy_ld = gr.ld, g.x = xr.p, g.x_ld = xr.ld, g.w = wr.p, g.w_ld = wr.ld, g.w_order = wr.order;
-  g.m = xr.m, g.n = wr.n, g.k = xr.n, g.type = type_of(t), g.act = static_cast<int>(integer(a[4]));
-  g.tile = static_cast<int>(integer(a[8])), g.splits = static_cast<int>(integer(a[9]));
+  g.m = xr.m, g.n = wr.n, g.k = xr.n, g.type = type_of(t), g.act = integer(a[4], "activation");
+  g.tile = integer(a[8], "tile"), g.splits = integer(a[9], "splits");
   if (g.act) {
     TORCH_CHECK_VALUE(z, "an activation's gradient needs z: call linear with keep=True");
     const Rows r = rows_of(*z, "z", xr.m, wr.n, t);

@@ -269,3 +269,21 @@ def test_activations_of_every_value(activation, dtype):
         dx, _, _ = nn.linear_grad(dy[at:at + step].cuda(), part.cuda(), eye, part.cuda(), activation, want_dw=False)
         want = ref.slope(part.double(), activation)
         ref.close(dx, want, 1e-5 * want.abs() + 1e-6 * (part.abs() < 3) + flushed(part.double()), dtype)
+
+
+def test_bad_numbers_are_value_errors():
+    """What the library refuses, and numbers that its arguments do not hold, before any work."""
+    nn = _nn()
+    x, w, v = _normal(1, 4, 8), _normal(2, 8, 16), _normal(3, 8)
+    dy = _normal(4, 4, 16)
+    for call, words in (
+            (lambda: nn.linear(x, w, tile=9), "tile = 9"), (lambda: nn.linear(x, w, tile=1 << 32), "tile = 4294967296"),
+            (lambda: nn.linear(x, w, splits=-1), "splits = -1"), (lambda: nn.linear(x, w, splits=(1 << 32) + 2), "splits = 4294967298"),
+            (lambda: nn.linear_grad(dy, x, w, tile=-(1 << 40)), "tile = -1099511627776"),
+            (lambda: nn.linear_grad(dy, x, w, splits=65), "splits = 65"), (lambda: nn.rms_norm(x, v, eps=-1.0), "eps"),
+            (lambda: nn.rms_norm(x, v, eps=float("nan")), "eps"), (lambda: nn.rms_norm_grad(x, x, v, eps=-1e-3), "eps")):
+        with pytest.raises(ValueError, match=words):
+            call()
+    for call in (lambda: nn.linear(x, w, tile=1 << 70), lambda: nn.linear(x, w, tile="2"), lambda: nn.rms_norm(x, v, eps=None)):
+        with pytest.raises((TypeError, OverflowError)):
+            call()
