@@ -261,7 +261,10 @@ int tf_registry_entry(int i, int *family, int *cfg7, char *name, int name_cap);
  * zero is a call without work, except that gradients summed over no rows and
  * products over no k are written as sums of nothing, and the scales of rows
  * without elements as those of zeros.
- * Arithmetic is float32 from the inputs on; every output is rounded once.
+ * Arithmetic is float32 from the inputs on and every output is rounded once,
+ * but for two values that the products take in fewer bits: the gradients' dz
+ * (tf_linear_grad) and, inside the matrix instructions of 8-bit products, the
+ * products of eight neighbouring k (tf_linear).
  * Sums are taken in a fixed order: equal calls give equal bits.
  * Arguments that cannot hold give TF_E_ARG before anything is enqueued. */
 
@@ -352,9 +355,15 @@ typedef struct {
 int tf_linear_workspace(const tf_linear_args_t *args, long long *bytes);
 int tf_linear(const tf_linear_args_t *args, void *stream);
 
-/* tf_linear's gradient in 16 bits: dz = dy * act'(z) (rounded to `type` for the
- * products), dx = dz @ w^T, dw = x^T @ dz in w's memory order, dbias = sum over
- * rows of dz (before its rounding).  The residual's gradient is dy. */
+/* tf_linear's gradient in 16 bits: dz = dy * act'(z), dx = dz @ w^T, dw = x^T @ dz
+ * in w's memory order, dbias = sum over rows of dz.  The residual's gradient is dy.
+ *
+ * dbias sums dz in float32.  The products take it in `type`: exactly with
+ * TF_ACT_NONE and TF_ACT_RELU; with the smooth activations rounded, in one term, or
+ * in two (the value and what its rounding left, 16 bits more), as `terms` says.  In
+ * one term the products err by sqrt(2) of their own rounding; two take them twice
+ * as long.  By the sizes: two up to 1.4e8 multiply-adds (m * n * k), one above.  A
+ * dz past float16's largest value is an infinity in one term, itself in two. */
 typedef struct {
   const void *dy, *x, *w; /* m x n, m x k, k x n in either order                    */
   const void *z;          /* m x n: the kept pre-activation; NULL with TF_ACT_NONE  */
@@ -369,6 +378,8 @@ typedef struct {
   int bias_type; /* `type` or TF_T_F32                                              */
   int act;
   int tile, splits; /* both products', as tf_linear's                                */
+  int terms;     /* of dz in the products: 0 by the sizes, 1 or 2                   */
+  int reserved;  /* 0                                                               */
 } tf_linear_grad_args_t;
 /* As tf_linear_workspace; which of dx, dw and dbias are wanted counts too. */
 int tf_linear_grad_workspace(const tf_linear_grad_args_t *args, long long *bytes);

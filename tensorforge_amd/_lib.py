@@ -75,7 +75,7 @@ class LinearGradArgs(ctypes.Structure):
     _fields_ = [(f, ctypes.c_void_p) for f in ("dy", "x", "w", "z", "dx", "dw", "dbias", "workspace")] + \
                [(f, ctypes.c_longlong) for f in ("workspace_bytes", "dy_ld", "x_ld", "w_ld", "z_ld", "dx_ld", "dw_ld",
                                                  "m", "n", "k")] + \
-               [(f, ctypes.c_int) for f in ("w_order", "type", "bias_type", "act", "tile", "splits")]
+               [(f, ctypes.c_int) for f in ("w_order", "type", "bias_type", "act", "tile", "splits", "terms", "reserved")]
 
 
 # (name, restype, argtypes) of every exported function, in header order.

@@ -477,8 +477,8 @@ double plan_pair(GradPlan &g) {
   return best;
 }
 
-// Up to this many multiply-adds a product of the rounded dz is not taken alone:
-// what the rounding left goes in as a second term, into the same float sums.  A
+// Unless the caller says otherwise, up to this many multiply-adds a product of the rounded dz is
+// not taken alone: what the rounding left goes in as a second term, into the same float sums.  A
 // small gradient then errs by its own rounding only; larger ones, where a second
 // product would cost as much again, by sqrt(2) of it.  bfloat16 gelu, two terms here and
 // one just above: 512 x 512 x 520 14.0 us, x 544 11.0; 2048 x 256 x 264 17.1, x 280 15.0.
@@ -499,7 +499,7 @@ GradPlan plan_grad(const tf_linear_grad_args_t *a) {
     g.count = ceil_div(m, rows);
     g.shares = a->dbias && g.count > 1 ? round16(4 * g.count * a->n) : 0;
   };
-  g.terms = smooth && work <= kTwoTerms ? 2 : 1;
+  g.terms = !smooth ? 1 : a->terms ? a->terms : work <= kTwoTerms ? 2 : 1;
   const bool odd = !direct_loads(dy, 2);
   // A workgroup of dz takes all of up to 256 rows where that spares the bias gradient a
   // second launch; else 64, or 32 where that leaves CUs without work.
@@ -557,6 +557,7 @@ void check_grad_sizes(Checks &c, const tf_linear_grad_args_t *a) {
   c.size("n", a->n);
   c.size("k", a->k);
   check_choice(c, a->tile, a->splits);
+  c.one_of("terms", a->terms, {0, 1, 2});
 }
 
 int linear_grad_workspace(const tf_linear_grad_args_t *a, long long *bytes) {

@@ -320,10 +320,10 @@ PyObject *linear(PyObject *, PyObject *const *a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-// (dy, x, w, z, act, bias_dtype, want_dx, want_dw, tile, splits) -> (dx, dw, dbias)
+// (dy, x, w, z, act, bias_dtype, want_dx, want_dw, tile, splits, terms) -> (dx, dw, dbias)
 PyObject *linear_grad(PyObject *, PyObject *const *a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  count(n, 10);
+  count(n, 11);
   const Tensor &dy = tensor(a[0], "dy"), &x = tensor(a[1], "x"), &w = tensor(a[2], "w");
   const Tensor *z = optional(a[3], "z");
   const ScalarType t = x.scalar_type();
@@ -336,7 +336,7 @@ PyObject *linear_grad(PyObject *, PyObject *const *a, Py_ssize_t n) {
   tf_linear_grad_args_t g{};
   g.dy = gr.p, g.dy_ld = gr.ld, g.x = xr.p, g.x_ld = xr.ld, g.w = wr.p, g.w_ld = wr.ld, g.w_order = wr.order;
   g.m = xr.m, g.n = wr.n, g.k = xr.n, g.type = type_of(t), g.act = integer(a[4], "activation");
-  g.tile = integer(a[8], "tile"), g.splits = integer(a[9], "splits");
+  g.tile = integer(a[8], "tile"), g.splits = integer(a[9], "splits"), g.terms = integer(a[10], "terms");
   if (g.act) {
     TORCH_CHECK_VALUE(z, "an activation's gradient needs z: call linear with keep=True");
     const Rows r = rows_of(*z, "z", xr.m, wr.n, t);

@@ -103,7 +103,7 @@ class _RmsNorm(torch.autograd.Function):
 
 
 def linear(x, w, bias=None, activation="none", residual=None, keep=False, x_scale=None, w_scale=None, out_dtype=None,
-           tile=0, splits=0):
+           tile=0, splits=0, grad_terms=0):
     """z = x @ w + bias;  out = activation(z) + residual, rounded once.
 
     x (..., k) and w (k, n) are bfloat16 or float16; w may lie row by row or column by
@@ -112,35 +112,39 @@ def linear(x, w, bias=None, activation="none", residual=None, keep=False, x_scal
     (bfloat16 unless given).  bias is of the output's type or float32.  activation:
     "none", "relu", "gelu" (by the normal distribution), "silu".  Returns out, or
     (out, z) with keep=True; both are differentiable.  tile and splits override the choice by sizes
-    (tf_linear_args_t in tforge_hip.h).
+    (tf_linear_args_t in tforge_hip.h); grad_terms is linear_grad's terms under autograd.
     """
     got = _C.linear(x, w, bias, _act(activation), residual, True if keep else False, x_scale, w_scale, out_dtype, tile,
                     splits)
     if got is not None:
         return got
-    out, z = _Linear.apply(x, w, bias, residual, activation, keep, tile, splits)
+    out, z = _Linear.apply(x, w, bias, residual, activation, keep, tile, splits, grad_terms)
     return (out, z) if keep else out
 
 
-def linear_grad(dy, x, w, z=None, activation="none", bias_dtype=None, want_dx=True, want_dw=True, tile=0, splits=0):
+def linear_grad(dy, x, w, z=None, activation="none", bias_dtype=None, want_dx=True, want_dw=True, tile=0, splits=0,
+                terms=0):
     """(dx, dw, dbias) of linear from the gradient dy of its output and the kept pre-activation z.
 
     dw lies in memory as w does.  dbias comes in bias_dtype (x's type or float32), None
     without one; what is not wanted is None.  The residual's gradient is dy itself.
+    With gelu and silu the products take dz = dy * activation'(z) rounded to x's type
+    (terms=1, an error of sqrt(2) of the results' own rounding) or with what the rounding
+    left as a second term (terms=2, twice the time); 0 takes two up to 1.4e8 multiply-adds.
     """
     return _C.linear_grad(dy, x, w, z, _act(activation), bias_dtype, True if want_dx else False,
-                          True if want_dw else False, tile, splits)
+                          True if want_dw else False, tile, splits, terms)
 
 
 class _Linear(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, w, bias, residual, activation, keep, tile, splits):
+    def forward(ctx, x, w, bias, residual, activation, keep, tile, splits, terms):
         smooth = activation != "none"
         with torch.no_grad():
             got = linear(x, w, bias, activation, residual, keep=keep or smooth, tile=tile, splits=splits)
         out, z = got if keep or smooth else (got, None)
         ctx.save_for_backward(x, w, z if smooth else None)
-        ctx.how = activation, None if bias is None else bias.dtype, tile, splits
+        ctx.how = activation, None if bias is None else bias.dtype, tile, splits, terms
         ctx.added = None if residual is None else residual.shape
         ctx.set_materialize_grads(False)
         return out, z if keep else None
@@ -149,15 +153,15 @@ class _Linear(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dy, dz):
         x, w, z = ctx.saved_tensors
-        activation, bias_dtype, tile, splits = ctx.how
+        activation, bias_dtype, tile, splits, terms = ctx.how
         need = ctx.needs_input_grad
 
         def grads(g, z, activation):
             return linear_grad(g.contiguous(), x, w, z, activation, bias_dtype if need[2] else None, need[0], need[1], tile,
-                               splits)
+                               splits, terms)
 
         # A gradient that reaches the kept z past the activation: its own products, added to the output's.
         got = [] if dy is None else [grads(dy, z, activation)]
         got += [] if dz is None else [grads(dz, None, "none")]
         total = (None, None, None) if not got else got[0] if len(got) == 1 else [a if a is None else a + b for a, b in zip(*got)]
-        return (*total, dy.reshape(ctx.added) if need[3] and dy is not None else None, None, None, None, None)
+        return (*total, dy.reshape(ctx.added) if need[3] and dy is not None else None, None, None, None, None, None)

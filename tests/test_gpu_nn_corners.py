@@ -287,3 +287,32 @@ def test_bad_numbers_are_value_errors():
     for call in (lambda: nn.linear(x, w, tile=1 << 70), lambda: nn.linear(x, w, tile="2"), lambda: nn.rms_norm(x, v, eps=None)):
         with pytest.raises((TypeError, OverflowError)):
             call()
+
+
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("activation", ["gelu", "silu"])
+def test_terms_of_dz(activation, dtype):
+    """The caller's choice on both sides of the sizes': in two terms the products err by their own rounding (5% for few
+    elements, and the float sums' share), in one they are those of the rounded dz."""
+    nn = _nn()
+    for m, n, k in ((64, 72, 40), (130, 77, 65), (528, 528, 528), (700, 520, 515)):
+        for order in (0, 1):
+            g = torch.Generator().manual_seed(m + n)
+            dy, x, w, z = (_matrix(g, *s, dtype) for s in ((m, n), (m, k), (k, n), (m, n)))
+            args = dy.cuda(), x.cuda(), _ordered(w, order), z.cuda(), activation
+            dz = dy.double() * ref.slope(z.double(), activation)
+            got = {t: nn.linear_grad(*args, terms=t)[:2] for t in (0, 1, 2)}
+            for i, (a, b) in enumerate(((dz, w.double().t()), (x.double().t(), dz))):
+                want, own = a @ b, ((a @ b).to(dtype).double() - a @ b).norm()
+                assert float((got[2][i].cpu().double() - want).norm()) <= 1.05 * float(own) + 4e-6 * float(want.norm()), (m, n, k)
+                # sqrt(2) of the own rounding, and as much above one as 5% leaves
+                assert 1.05 * float(own) < float((got[1][i].cpu().double() - want).norm()) < 1.6 * float(own), (m, n, k)
+                assert torch.equal(got[0][i], got[2 if m * n * k <= 1.4e8 else 1][i])
+            leaves = [t.detach().requires_grad_() for t in args[1:3]]
+            out, zk = nn.linear(*leaves, None, activation, keep=True, grad_terms=2)
+            out.backward(args[0])
+            for a, b in zip(leaves, nn.linear_grad(args[0], *args[1:3], zk.detach(), activation, terms=2)):
+                assert torch.equal(a.grad, b)
+    for terms in (-1, 3):
+        with pytest.raises(ValueError, match="terms = "):
+            nn.linear_grad(*args, terms=terms)

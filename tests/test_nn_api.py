@@ -278,3 +278,10 @@ def test_copies_of_short_lines_stay_small():
                                         type=type_, out_type=1, tile=tile, splits=1)
                     assert lib.tf_linear_workspace(ctypes.byref(a), ctypes.byref(size)) == 0
                     assert size.value <= max(4 * (m + n) * k * 2, 256 << 20), (m, n, k, order, type_, tile)
+
+
+def test_terms_refusals():
+    base = dict(dy=256, x=256, w=256, dx=256, dw=256, dbias=256, workspace=256, workspace_bytes=1 << 30, dy_ld=32, x_ld=64,
+                w_ld=32, dx_ld=64, dw_ld=32, m=8, n=32, k=64, type=1, bias_type=1)
+    for terms in (-1, 3):
+        _refused(_lib.lib().tf_linear_grad, _lib.LinearGradArgs(**base, terms=terms), f"terms = {terms}")

@@ -33,7 +33,7 @@ class Plain:
         out = (out if residual is None else out + residual.view_as(out)).detach()
         return (out, z.detach()) if keep else out
 
-    def linear_grad(self, dy, x, w, z, act, bias_dtype, want_dx, want_dw, tile, splits):
+    def linear_grad(self, dy, x, w, z, act, bias_dtype, want_dx, want_dw, tile, splits, terms):
         k, n = w.shape
         dz = (dy * ref.slope(z.view_as(dy), NAMES[act]) if act else dy).reshape(-1, n).detach()
         return ((dz @ w.t()).view_as(x).detach() if want_dx else None, (x.reshape(-1, k).t() @ dz).detach() if want_dw else None,
