@@ -316,3 +316,29 @@ def test_terms_of_dz(activation, dtype):
     for terms in (-1, 3):
         with pytest.raises(ValueError, match="terms = "):
             nn.linear_grad(*args, terms=terms)
+
+
+@pytest.mark.parametrize("tile", [0, 1, 2, 3, 4, 5])
+def test_sums_of_8bit_products(tile):
+    """What the sums inside an 8-bit product lose, seen where the bias takes the exact sum away.  Eight neighbouring k are
+    aligned to the largest of their products and cut off 13 bits below it; the rest is float32 (one rounding for each eight
+    products, one for the bias).  Signs being random, the cuts' root mean square is under one cut a product."""
+    nn = _nn()
+    for k in (128, 1024, 4096):
+        g = torch.Generator().manual_seed(k)
+        x = (100 * torch.randn(1, k, generator=g)).clamp(-448, 448).to(ref.F8)
+        w = (100 * torch.randn(256, k, generator=g)).clamp(-448, 448).to(ref.F8)
+        products = x.float().double() * w.float().double()
+        want, size = products.sum(1), products.abs().sum(1)
+        cut = 2.0 ** -13 * products.abs().view(256, -1, 8).amax(2)
+        rows = 1 if tile in (0, 4) else 256
+        one = lambda n: torch.ones(n, device="cuda")  # noqa: E731
+        out = nn.linear(x.expand(rows, k).contiguous().cuda(), w.cuda().t(), (-want).float().cuda(), x_scale=one(rows), w_scale=one(256),
+                        tile=tile, splits=1)
+        off = out.cpu().double()
+        assert (off == off[:1]).all()
+        off = off[0]
+        rest = (k // 8 + 4) * ref.u * size
+        assert (off.abs() <= 1.01 * (8 * cut.sum(1) + rest)).all()
+        least = (8 * cut.square().sum(1)).mean().sqrt()
+        assert float(off.square().mean().sqrt()) <= 1.01 * float(least + rest.square().mean().sqrt()), k
