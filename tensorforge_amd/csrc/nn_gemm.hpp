@@ -102,7 +102,7 @@ __device__ __forceinline__ void load_to_lds(i32x4 resource, uint32_t offset, uin
       "buffer_load_dwordx4 %1, %2, 0 offen lds"
       :
       : "s"(lds), "v"(offset), "s"(resource)
-      : "memory");
+      : "memory", "m0");
 }
 
 constexpr uint32_t kNowhere = 0x80000000u;  // past every resource: reads zeros
