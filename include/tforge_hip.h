@@ -281,8 +281,9 @@ int tf_registry_entry(int i, int *family, int *cfg7, char *name, int name_cap);
 /* h = x + residual;  y = h / sqrt(mean(h^2) + eps) * weight, row by row, the norm
  * taken of the sum before h is rounded.  With y_type TF_T_F8 y is in 8 bits with
  * one scale a row: top = max(max|y|, 2^-100), scale = top/448, code = the value
- * nearest to y * (448 * (1/top)) (ties to even).  A row that holds an infinity or a
- * NaN gives NaN. */
+ * nearest to y * (448 * (1/top)) (ties to even).  In 8 bits a row that holds an
+ * infinity or a NaN stands for NaN throughout (codes times scale); in `type` its
+ * infinities give NaN and its finite values 0, a NaN gives NaN throughout. */
 typedef struct {
   const void *x, *residual; /* rows x d of `type`; residual may be NULL          */
   const void *weight;       /* d of weight_type                                  */

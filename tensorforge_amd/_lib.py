@@ -103,8 +103,8 @@ SIGNATURES = [
     ("tf_bench_samples", I, [P, ctypes.POINTER(ctypes.c_double), I]),
     ("tf_registry_size", I, []),
     ("tf_registry_entry", I, [I, ctypes.POINTER(I), ctypes.POINTER(I), ctypes.c_char_p, I]),
-    # The residual block's operators.  Their argument structs are passed as any
-    # pointer: tforge_nn packs them as bytes.
+    # The residual block's operators.  tforge_nn calls them from its native layer
+    # (_nn_torch); the structs above are for callers of the C ABI in Python.
     ("tf_rms_norm", I, [P, P]),
     ("tf_quantize_rows", I, [P, LL, LL, LL, I, P, LL, P, P]),
     ("tf_rms_norm_grad_workspace", I, [LL, LL, ctypes.POINTER(LL)]),

@@ -342,3 +342,52 @@ def test_sums_of_8bit_products(tile):
         assert (off.abs() <= 1.01 * (8 * cut.sum(1) + rest)).all()
         least = (8 * cut.square().sum(1)).mean().sqrt()
         assert float(off.square().mean().sqrt()) <= 1.01 * float(least + rest.square().mean().sqrt()), k
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("rows", [1, 6, 3000])
+def test_norms_in_place(rows, dtype):
+    """Through the C ABI: h over x or the residual, dx over dy or dh, at whole and odd lengths of every kernel."""
+    import ctypes
+
+    from tensorforge_amd import _lib
+    nn, lib = _nn(), _lib.lib()
+    stream = torch.cuda.current_stream().cuda_stream
+    code = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}[dtype]
+    for d in (5, 64, 333, 1024, 1111, 2056, 4100, 8193, 16387):
+        if rows * d > 8000000:
+            continue
+        x, r, dy, dh = (_normal(i, rows, d, dtype=torch.float32).to(dtype) for i in range(4))
+        w = 1 + 0.1 * _normal(9, d, dtype=torch.float32)
+        y, h = nn.rms_norm(x, w, r)
+        for over in (0, 1):
+            a, b, got = x.clone(), r.clone(), torch.empty_like(x)
+            args = _lib.RmsNormArgs(x=a.data_ptr(), residual=b.data_ptr(), weight=w.data_ptr(), y=got.data_ptr(),
+                                    h=(a, b)[over].data_ptr(), x_ld=d, residual_ld=d, y_ld=d, h_ld=d, rows=rows, d=d, type=code,
+                                    weight_type=0, y_type=code, eps=1e-6)
+            _lib.check(lib.tf_rms_norm(ctypes.byref(args), stream))
+            assert torch.equal(got, y) and torch.equal((a, b)[over], h) and torch.equal((a, b)[1 - over], (x, r)[1 - over]), (d, over)
+        dx, dw = nn.rms_norm_grad(dy, h, w, dh=dh)
+        space = torch.empty(1 << 26, dtype=torch.uint8, device="cuda")
+        for over in (0, 1):
+            a, b, got = dy.clone(), dh.clone(), torch.empty_like(w)
+            args = _lib.RmsNormGradArgs(dy=a.data_ptr(), h=h.data_ptr(), dh=b.data_ptr(), weight=w.data_ptr(), dx=(a, b)[over].data_ptr(),
+                                        dweight=got.data_ptr(), dy_ld=d, h_ld=d, dh_ld=d, dx_ld=d, rows=rows, d=d, type=code,
+                                        weight_type=0, eps=1e-6, workspace=space.data_ptr(), workspace_bytes=space.numel())
+            _lib.check(lib.tf_rms_norm_grad(ctypes.byref(args), stream))
+            assert torch.equal((a, b)[over], dx) and torch.equal(got, dw), (d, over)
+
+
+def test_rows_with_infinities():
+    nn = _nn()
+    inf, nan = float("inf"), float("nan")
+    for d in (6, 64, 1111, 20000):
+        x = torch.ones(4, d, device="cuda")
+        x[0, 3], x[1, 4], x[1, 5], x[2, 2] = inf, -inf, inf, nan
+        w = torch.ones(d, device="cuda")
+        y, _ = nn.rms_norm(x, w)
+        at = x[:2].isinf()
+        assert y[:2][at].isnan().all() and (y[:2][~at] == 0).all() and y[2].isnan().all() and y[3].isfinite().all()
+        for q, s in (nn.rms_norm(x, w, quantize=True)[:2], nn.quantize_rows(x)):
+            v = q.float() * s[:, None]
+            assert v[:3].isnan().all() and v[3].isfinite().all(), d
