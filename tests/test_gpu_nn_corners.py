@@ -391,3 +391,18 @@ def test_rows_with_infinities():
         for q, s in (nn.rms_norm(x, w, quantize=True)[:2], nn.quantize_rows(x)):
             v = q.float() * s[:, None]
             assert v[:3].isnan().all() and v[3].isfinite().all(), d
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_codes_are_those_of_the_formula(dtype):
+    """Bit by bit: scale = top/448, code = nearest(x * (448 * (1/top))), each step in float32."""
+    nn = _nn()
+    for rows, d in ((4000, 6), (3000, 64), (700, 1111), (300, 4096), (90, 20000)):
+        x = (_normal(d, rows, d, dtype=torch.float32) * torch.exp(_normal(7, rows, 1, dtype=torch.float32))).to(dtype)
+        x[1] = 0
+        q, s = nn.quantize_rows(x)
+        f = x.float()
+        top = f.abs().amax(1, keepdim=True).clamp_min(ref.TINY)
+        factor = ref.F8_MAX * (torch.ones_like(top) / top)
+        assert torch.equal(q.view(torch.uint8), (f * factor).to(ref.F8).view(torch.uint8)), (rows, d)
+        assert torch.equal(s, (top / torch.full_like(top, ref.F8_MAX))[:, 0])
