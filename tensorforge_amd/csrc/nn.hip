@@ -241,7 +241,8 @@ double predicted(double m, double n, double slabs, double read, bool dma, bool f
 // reads its columns' k at about 110 bytes a nanosecond and all rows' (from the caches) at
 // 45, fitted to 200 products of 1 to 64 rows.  Measured, bfloat16, us
 // (few-row / 64-tile), w 4096 x 4096 as n rows of k: 7.7 / 10.8 for 1 row, 9.8 / 11.1
-// for 16, 13.7 / 11.6 for 32; as k rows of n: 11.4 / 11.6, 13.4 / 12.2, 16.1 / 12.5.
+// for 16, 13.7 / 11.6 for 32; as k rows of n: 11.4 / 11.6, 13.4 / 12.2, 16.1 / 12.5 (w partly
+// in the caches; from memory alone 1 row takes 17.8 so, 7.7 on n rows of k).
 // A left operand of two terms counts as twice the rows here, as twice the slabs on the tiles.
 // Lines off four bytes take it longer (150 more): 5 x 4224 x 1022 5.3, x 1023 10.6 (8.1 on the
 // 64-tile); 4 x 5911 x 5281 40.8 and 21.8.

@@ -236,7 +236,8 @@ __device__ __forceinline__ void store_weight8(const NormGradParams &p, int c, co
 // The gradient's dx, and this workgroup's rows' share of dw, kept in registers over
 // its rows.  The shares are added by share_sum_kernel, in a fixed order.  Bound by
 // memory: 8192 x 4096 bfloat16 with dh 57 us, 51 and 5 for the sum (268 MB, 5.2 TB/s
-// in the first); 777 x 1111 float32 13 us, the two launches' latency.
+// in the first); 777 x 1111 float32 13 us: a workgroup's load, reduction
+// and stores one after the other 7, the sum's launch 4, the gap between them.
 template <typename T, int NT, int CH, Length L>
 __global__ __launch_bounds__(NT *grad_rows(NT, CH)) void rms_norm_grad_kernel(NormGradParams p) {
   constexpr int RPB = grad_rows(NT, CH), THREADS = NT * RPB;
@@ -320,7 +321,7 @@ __global__ __launch_bounds__(NT *grad_rows(NT, CH)) void rms_norm_grad_kernel(No
 
 // Rows longer than a workgroup's registers hold.  Workgroups own fixed rows; a
 // share of dw is added up in place, in memory, by the threads that own its columns: more
-// bytes than the rows themselves.  4096 x 32768 bfloat16 870 us (0.9 TB/s of the rows' bytes).
+// bytes than the rows themselves.  4096 x 32768 bfloat16 653 us (1.2 TB/s of the rows' bytes).
 template <typename T>
 __global__ __launch_bounds__(256) void rms_norm_grad_long_kernel(NormGradParams p) {
   constexpr int NT = 256;

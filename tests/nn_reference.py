@@ -5,8 +5,8 @@ Bounds: U[t] is the unit roundoff of the output's type; inner arithmetic is
 float32 (unit roundoff u = 2^-24) with sums of at most `terms` additions, each
 partial sum off by at most u, so a sum of products is off by at most
 2 * terms * u * sum|products| (one u a product, one an addition).  relu, gelu and
-silu have slopes of at most 1.13; the polynomial inside gelu is off by at most
-1.5e-7 (Abramowitz and Stegun 7.1.26), exponentials and reciprocals by a few u.
+silu have slopes of at most 1.13; the polynomial inside gelu's tail is off by at
+most 7e-7 of the tail, exponentials and reciprocals by a few u.
 """
 
 import math
