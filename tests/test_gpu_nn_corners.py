@@ -406,3 +406,22 @@ def test_codes_are_those_of_the_formula(dtype):
         factor = ref.F8_MAX * (torch.ones_like(top) / top)
         assert torch.equal(q.view(torch.uint8), (f * factor).to(ref.F8).view(torch.uint8)), (rows, d)
         assert torch.equal(s, (top / torch.full_like(top, ref.F8_MAX))[:, 0])
+
+
+@pytest.mark.parametrize("dtype", HALF)
+def test_8bit_products_of_few_k(dtype):
+    """Element by element within what tforge_hip.h says of 8-bit sums, where few products make that visible: for each
+    eight k 2^-10 of their largest product, then float32."""
+    nn = _nn()
+    for m, n, k in ((70, 61, 2), (33, 130, 8), (130, 40, 14), (5, 100, 30), (64, 64, 59), (3, 7, 130)):
+        g = torch.Generator().manual_seed(m + n + k)
+        q, s = nn.quantize_rows(_matrix(g, m, k, torch.float32).cuda())
+        wq, ws = nn.quantize_rows(_matrix(g, n, k, torch.float32).cuda())
+        b = torch.randn(n, generator=g)
+        x, w, scales = q.cpu().double(), wq.cpu().double(), s.cpu().double()[:, None] * ws.cpu().double()
+        cut = sum(2.0 ** -10 * (x[:, None, i:i + 8] * w[None, :, i:i + 8]).abs().amax(2) for i in range(0, k, 8))
+        z = (x @ w.t()) * scales + b.double()
+        off = (cut + (2 * k + 8) * ref.u * (x.abs() @ w.abs().t())) * scales + 4 * ref.u * (z.abs() + b.double().abs())
+        for tile, splits in ((0, 0), (1, 1), (2, 1), (3, 1), (3, 2), (4, 1), (5, 1)):
+            out = nn.linear(q, wq.t(), b.cuda(), x_scale=s, w_scale=ws, out_dtype=dtype, tile=tile, splits=splits)
+            ref.close(out, z, off, dtype)
