@@ -253,15 +253,14 @@ Plan plan_product(const Product &q, bool dma, int tile, int splits) {
   const int size = size_of(type);
   const long slabs = ceil_div(k, 128 / size);
   // A launch takes fewer than 2^32 threads.  (Through registers its grid may have two sides.)
-  const auto fits = [&](int t, long ranges) {
-    const long blocks = t == TILE_ROWS ? ceil_div(n, bmn ? 32 : 16) : ceil_div(m, tile_rows(t)) * ceil_div(n, tile_columns(t)) * ranges;
-    return blocks * tile_threads(t) < (1L << 32);
-  };
-  const bool rows = m * terms <= 64 && !amn && (!bmn || n >= 32) && fits(TILE_ROWS, 1);
+  const auto tiles_of = [&](int t) { return ceil_div(m, tile_rows(t)) * ceil_div(n, tile_columns(t)); };
+  const auto fits = [&](int t, long blocks) { return blocks * tile_threads(t) < (1L << 32); };
+  const bool rows = m * terms <= 64 && !amn && (!bmn || n >= 32) && fits(TILE_ROWS, ceil_div(n, bmn ? 32 : 16));
   if (tile == TILE_ROWS && rows) return {TILE_ROWS, 1, 0};
   if (tile == TILE_ROWS || (!dma && tile != TILE_64) || (terms > 1 && tile == TILE_256)) tile = 0;
   splits = static_cast<int>(std::max<long>(0, std::min<long>(splits, std::max<long>(1, slabs))));
-  if (tile && dma && !fits(tile, std::max(1, splits))) tile = 0;
+  if (m * ceil_div(n, 4) >= (1L << 31)) splits = 1;  // the join counts quads in 32 bits; so many need no split
+  if (tile && dma && !fits(tile, tiles_of(tile) * std::max(1, splits))) tile = 0;
   Plan best{TILE_64, 1, 1e30};
   const double read = (static_cast<double>(m) + n) * k * terms * size / 8e6;
   if (rows && !tile) {
@@ -274,12 +273,12 @@ Plan plan_product(const Product &q, bool dma, int tile, int splits) {
   for (int t : {TILE_64, TILE_64x128, TILE_128, TILE_256}) {
     if (tile ? t != tile : (t != TILE_64 && !dma) || (t == TILE_256 && terms > 1)) continue;
     // Tiles mostly empty, and splits into more than four workgroups a CU, never win.
-    if (!tile && t != TILE_64 && fits(TILE_64, 1) && (2 * m <= tile_rows(t) || 2 * n <= tile_columns(t))) continue;
-    const long tiles = ceil_div(m, tile_rows(t)) * ceil_div(n, tile_columns(t));
+    if (!tile && t != TILE_64 && (2 * m <= tile_rows(t) || 2 * n <= tile_columns(t)) && fits(TILE_64, tiles_of(TILE_64))) continue;
+    const long tiles = tiles_of(t);
     for (int s : {1, 2, 3, 4, 6, 8, 12, 16}) {
       if (s > 1 && (splits || s * 2 > slabs || tiles * s > 1024)) break;
       const int ranges = splits ? splits : s;
-      if (dma && !fits(t, ranges)) continue;
+      if (dma && !fits(t, tiles * ranges)) continue;
       const double us = predicted(m, n, slabs * terms, read, dma, size == 1, t, ranges);
       if (us < best.us) best = {t, ranges, us};
     }
@@ -518,7 +517,7 @@ GradPlan plan_grad(const tf_linear_grad_args_t *a) {
   g.dw.p.m = nk ? n : k, g.dw.p.n = nk ? k : n, g.dw.p.k = m, g.dw.p.out = a->dw, g.dw.p.ldo = a->dw_ld;
   if (g.terms == 2) {
     g.dx.p.terms = g.dw.p.terms = 2;
-    g.dx.p.a_term = (nk ? g.dw.p.a_term : g.dw.p.b_term) = g.dz / 2;
+    g.dx.p.a_term = (nk ? g.dw.p.a_term : g.dw.p.b_term) = -(g.dz / 2);  // what the rounding left lies behind
   }
   // One launch for both where it takes less; below 8 us two cannot.
   double pair = 1e30;
@@ -616,7 +615,7 @@ int linear_grad(const tf_linear_grad_args_t *a, hipStream_t stream) {
   if (e == hipSuccess && a->dbias && n && ((g.shares && !g.pair) || !m))
     e = launch_share_sum(shares, m ? g.count : 0, n, a->dbias, a->bias_type, stream);
   if (e != hipSuccess || !k) return hip(e, call);
-  if (g.own_dz) g.dx.a.p = (a->w_order ? g.dw.a.p : g.dw.b.p) = ws;
+  if (g.own_dz) g.dx.a.p = (a->w_order ? g.dw.a.p : g.dw.b.p) = g.terms == 2 ? ws + g.dz / 2 : ws;
   if (g.pair) {
     place(g.dx, {TILE_64, g.dx_splits, 0}, parts);
     place(g.dw, {TILE_64, g.dw_splits, 0}, parts + g.dx_parts);

@@ -39,7 +39,8 @@ struct GemmParams {
   int m = 0, n = 0, k = 0;
   int tiles_m = 0, tiles_n = 0, splits = 1;
   int act = 0, bias_f32 = 0;
-  int terms = 1;                // 2: a second term of A at a + a_term, or of B at b + b_term (bytes)
+  int terms = 1;                // 2: another term of A at a + a_term, or of B at b + b_term (bytes);
+                                // the first is what the other's rounding left
   long a_term = 0, b_term = 0;  // (all tiles but 256; few rows: of A, up to 32 rows)
 };
 

@@ -425,3 +425,24 @@ def test_8bit_products_of_few_k(dtype):
         for tile, splits in ((0, 0), (1, 1), (2, 1), (3, 1), (3, 2), (4, 1), (5, 1)):
             out = nn.linear(q, wq.t(), b.cuda(), x_scale=s, w_scale=ws, out_dtype=dtype, tile=tile, splits=splits)
             ref.close(out, z, off, dtype)
+
+
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("order", [0, 1])
+def test_infinite_operands_where_nothing_is_rounded(order, dtype):
+    """dz that is exact has a second term of zeros, and zero times infinity is no number: x's and w's infinities stay."""
+    nn = _nn()
+    for m, n, k, _ in GRAD_SIZES:
+        g = torch.Generator().manual_seed(m)
+        x, w, dy = _matrix(g, m, k, dtype), _matrix(g, k, n, dtype), _matrix(g, m, n, dtype)
+        dy[dy == 0] = 1
+        z = torch.zeros(m, n, dtype=dtype)  # the slope is 1/2
+        x[1, 2], x[3, 5], w[4, 6], w[6, 1] = float("inf"), -float("inf"), -float("inf"), float("inf")
+        dz = dy.double() / 2
+        args = dy.cuda(), x.cuda(), _ordered(w, order), z.cuda(), "gelu"
+        _, dw, _ = nn.linear_grad(*args, terms=2)
+        for how in ({}, {"want_dw": False, "tile": 4}, {"want_dw": False}, {"want_dw": False, "splits": 2}):
+            dx = nn.linear_grad(*args, **how, terms=2)[0]
+            for got, want in ((dx, dz @ w.double().t()), (dw, x.double().t() @ dz)):
+                got = got.cpu().double()
+                assert not got.isnan().any() and torch.equal(got[want.isinf()], want[want.isinf()]), (m, how)
