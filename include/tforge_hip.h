@@ -272,6 +272,7 @@ int tf_registry_entry(int i, int *family, int *cfg7, char *name, int name_cap);
 #define TF_T_BF16 1
 #define TF_T_F16 2
 #define TF_T_F8 3 /* OCP e4m3: 8 bits, largest value 448 */
+#define TF_T_I8 4 /* 8-bit integers (two's complement)    */
 
 #define TF_ACT_NONE 0
 #define TF_ACT_RELU 1 /* NaN stays, as in compiled programs */
@@ -281,7 +282,8 @@ int tf_registry_entry(int i, int *family, int *cfg7, char *name, int name_cap);
 /* h = x + residual;  y = h / sqrt(mean(h^2) + eps) * weight, row by row, the norm
  * taken of the sum before h is rounded.  With y_type TF_T_F8 y is in 8 bits with
  * one scale a row: top = max(max|y|, 2^-100), scale = top/448, code = the value
- * nearest to y * (448 * (1/top)) (ties to even).  In 8 bits a row that holds an
+ * nearest to y * (448 * (1/top)) (ties to even); with TF_T_I8 the same with 127 in
+ * 448's place, in integers of -127..127.  In 8 bits a row that holds an
  * infinity or a NaN stands for NaN throughout (codes times scale); in `type` its
  * infinities give NaN and its finite values 0, a NaN gives NaN throughout. */
 typedef struct {
@@ -290,12 +292,12 @@ typedef struct {
   void *y;                  /* rows x d of y_type                                */
   void *h;                  /* rows x d of `type`; NULL without a residual; may be
                                x or residual itself                               */
-  float *scale;             /* rows; TF_T_F8 only                                 */
+  float *scale;             /* rows; 8-bit y only                                 */
   long long x_ld, residual_ld, y_ld, h_ld;
   long long rows, d;
   int type;        /* TF_T_F32, TF_T_BF16, TF_T_F16                               */
   int weight_type; /* `type` or TF_T_F32                                          */
-  int y_type;      /* `type` or TF_T_F8                                           */
+  int y_type;      /* `type`, TF_T_F8 or TF_T_I8                                  */
   float eps;       /* >= 0                                                        */
 } tf_rms_norm_args_t;
 int tf_rms_norm(const tf_rms_norm_args_t *args, void *stream);
@@ -303,6 +305,10 @@ int tf_rms_norm(const tf_rms_norm_args_t *args, void *stream);
 /* x (rows x d of `type`) in 8 bits with one scale a row, as tf_rms_norm's. */
 int tf_quantize_rows(const void *x, long long x_ld, long long rows, long long d, int type, void *y, long long y_ld,
                      float *scale, void *stream);
+
+/* The same into y_type: TF_T_F8 or TF_T_I8. */
+int tf_quantize_rows_to(const void *x, long long x_ld, long long rows, long long d, int type, void *y, long long y_ld,
+                        int y_type, float *scale, void *stream);
 
 /* tf_rms_norm's gradient.  r = 1/sqrt(mean(h^2) + eps), xhat = h*r:
  *   dx = r*(dy*weight - xhat*mean(dy*weight*xhat)) + dh     (also the residual's)
@@ -325,10 +331,13 @@ int tf_rms_norm_grad_workspace(long long rows, long long d, long long *bytes);
 int tf_rms_norm_grad(const tf_rms_norm_grad_args_t *args, void *stream);
 
 /* z = x @ w + bias;  out = act(z) + residual.  x is m x k, w is k x n in either
- * memory order.  With type TF_T_F8 x has a scale a row and w a scale a column,
- * z = (x @ w) * x_scale[m] * w_scale[n] + bias, and w_order is 1.
+ * memory order.  With type TF_T_F8 or TF_T_I8 x has a scale a row and w a scale a
+ * column, z = (x @ w) * x_scale[m] * w_scale[n] + bias, and w_order is 1.
  *
- * Sums over k are float32.  In 8 bits the matrix instruction adds the products of
+ * Sums over k are float32; of TF_T_I8 they are 32-bit integers, exact, any codes
+ * of -128..127 allowed and k at most 131071, and are rounded to float32 before the
+ * scales: the same bits whatever the tile and the splits.
+ * In e4m3 the matrix instruction adds the products of
  * eight neighbouring k (0..7, 8..15, ...) first, aligned to the largest of the eight
  * and cut off 13 bits below it.  A sum of products of random signs is off by 1.5e-5
  * of itself by this, a 250th of bfloat16's rounding; where the sum cancels, by
@@ -337,7 +346,7 @@ typedef struct {
   const void *x, *w;
   const void *bias;     /* n of bias_type, or NULL                                  */
   const void *residual; /* m x n of out_type, or NULL                               */
-  const float *x_scale, *w_scale; /* TF_T_F8 only: m, n                             */
+  const float *x_scale, *w_scale; /* 8 bits only: m, n                              */
   void *out;            /* m x n of out_type                                        */
   void *z;              /* m x n of out_type: the pre-activation kept, or NULL      */
   void *workspace;      /* 16-byte aligned; with fewer bytes than tf_linear_workspace
@@ -347,8 +356,8 @@ typedef struct {
   long long x_ld, w_ld, residual_ld, out_ld, z_ld;
   long long m, n, k;
   int w_order;   /* 0: w lies as k rows of n, 1: as n rows of k                      */
-  int type;      /* TF_T_BF16, TF_T_F16, TF_T_F8                                     */
-  int out_type;  /* `type`; TF_T_BF16 or TF_T_F16 for TF_T_F8                        */
+  int type;      /* TF_T_BF16, TF_T_F16, TF_T_F8, TF_T_I8                            */
+  int out_type;  /* `type`; TF_T_BF16 or TF_T_F16 for 8 bits                         */
   int bias_type; /* out_type or TF_T_F32                                             */
   int act;       /* TF_ACT_*                                                         */
   int tile;      /* C tile: 0 by the sizes, 1: 256x256, 2: 128x128, 3: 64x64, 4: all of

@@ -107,6 +107,7 @@ SIGNATURES = [
     # (_nn_torch); the structs above are for callers of the C ABI in Python.
     ("tf_rms_norm", I, [P, P]),
     ("tf_quantize_rows", I, [P, LL, LL, LL, I, P, LL, P, P]),
+    ("tf_quantize_rows_to", I, [P, LL, LL, LL, I, P, LL, I, P, P]),
     ("tf_rms_norm_grad_workspace", I, [LL, LL, ctypes.POINTER(LL)]),
     ("tf_rms_norm_grad", I, [P, P]),
     ("tf_linear_workspace", I, [P, ctypes.POINTER(LL)]),

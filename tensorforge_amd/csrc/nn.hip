@@ -17,8 +17,10 @@ using namespace tfnn;
 namespace {
 
 constexpr long long kMostSize = 1LL << 30;
+constexpr long long kMostI8 = (1LL << 31) / (128 * 128) - 1;  // products of two codes in a 32-bit sum
 
-int size_of(int type) { return type == TF_T_F32 ? 4 : type == TF_T_F8 ? 1 : 2; }
+bool eight_bits(int type) { return type == TF_T_F8 || type == TF_T_I8; }
+int size_of(int type) { return type == TF_T_F32 ? 4 : eight_bits(type) ? 1 : 2; }
 
 // The first thing wrong with a call's arguments.  Messages are built only where
 // one is wanted: the checks of a good call cost some tens of nanoseconds.
@@ -68,10 +70,10 @@ int hip(hipError_t e, const char *call) {
 
 // The scales of rows without elements: quantised as they are, whose largest magnitude is
 // then the least that counts.
-hipError_t scales_of_nothing(float *scale, long long rows, hipStream_t stream) {
+hipError_t scales_of_nothing(float *scale, long long rows, int y_type, hipStream_t stream) {
   NormParams p;
   p.scale = scale, p.rows = rows;
-  return launch_rms_norm(p, TF_T_F32, true, stream);
+  return launch_rms_norm(p, TF_T_F32, y_type, stream);
 }
 
 int rms_norm(const tf_rms_norm_args_t *a, hipStream_t stream) {
@@ -80,7 +82,7 @@ int rms_norm(const tf_rms_norm_args_t *a, hipStream_t stream) {
   Checks c{call, {}};
   c.one_of("type", a->type, {TF_T_F32, TF_T_BF16, TF_T_F16});
   c.one_of("weight_type", a->weight_type, {a->type, TF_T_F32});
-  c.one_of("y_type", a->y_type, {a->type, TF_T_F8});
+  c.one_of("y_type", a->y_type, {a->type, TF_T_F8, TF_T_I8});
   c.size("rows", a->rows);
   c.size("d", a->d);
   c.need(a->eps >= 0, "eps is negative or not a number");
@@ -90,33 +92,33 @@ int rms_norm(const tf_rms_norm_args_t *a, hipStream_t stream) {
   c.need(a->residual || !a->h, "h without a residual: it would be x");
   c.vector("weight", a->weight, a->d, a->weight_type, true);
   c.matrix("y", a->y, a->y_ld, a->rows, a->d, a->y_type, true);
-  c.vector("scale", a->scale, a->rows, TF_T_F32, a->y_type == TF_T_F8);
+  c.vector("scale", a->scale, a->rows, TF_T_F32, eight_bits(a->y_type));
   if (!c.fine()) return fail(TF_E_ARG, c.wrong);
   if (a->rows == 0) return TF_OK;
-  if (a->d == 0) return a->y_type == TF_T_F8 ? hip(scales_of_nothing(a->scale, a->rows, stream), call) : TF_OK;
+  if (a->d == 0) return eight_bits(a->y_type) ? hip(scales_of_nothing(a->scale, a->rows, a->y_type, stream), call) : TF_OK;
   NormParams p;
   p.x = a->x, p.residual = a->residual, p.weight = a->weight, p.y = a->y, p.h = a->h, p.scale = a->scale;
   p.x_ld = a->x_ld, p.residual_ld = a->residual_ld, p.y_ld = a->y_ld, p.h_ld = a->h_ld, p.rows = a->rows;
   p.d = static_cast<int>(a->d), p.weight_type = a->weight_type, p.eps = a->eps;
-  return hip(launch_rms_norm(p, a->type, a->y_type == TF_T_F8, stream), call);
+  return hip(launch_rms_norm(p, a->type, a->y_type, stream), call);
 }
 
-int quantize_rows(const void *x, long long x_ld, long long rows, long long d, int type, void *y, long long y_ld,
-                  float *scale, hipStream_t stream) {
-  const char *call = "tf_quantize_rows";
+int quantize_rows(const char *call, const void *x, long long x_ld, long long rows, long long d, int type, void *y, long long y_ld,
+                  int y_type, float *scale, hipStream_t stream) {
   Checks c{call, {}};
   c.one_of("type", type, {TF_T_F32, TF_T_BF16, TF_T_F16});
+  c.one_of("y_type", y_type, {TF_T_F8, TF_T_I8});
   c.size("rows", rows);
   c.size("d", d);
   c.matrix("x", x, x_ld, rows, d, type, true);
-  c.matrix("y", y, y_ld, rows, d, TF_T_F8, true);
+  c.matrix("y", y, y_ld, rows, d, y_type, true);
   c.vector("scale", scale, rows, TF_T_F32, true);
   if (!c.fine()) return fail(TF_E_ARG, c.wrong);
   if (rows == 0) return TF_OK;
-  if (d == 0) return hip(scales_of_nothing(scale, rows, stream), call);
+  if (d == 0) return hip(scales_of_nothing(scale, rows, y_type, stream), call);
   NormParams p;
   p.x = x, p.y = y, p.scale = scale, p.x_ld = x_ld, p.y_ld = y_ld, p.rows = rows, p.d = static_cast<int>(d);
-  return hip(launch_rms_norm(p, type, true, stream), call);
+  return hip(launch_rms_norm(p, type, y_type, stream), call);
 }
 
 int rms_norm_grad(const tf_rms_norm_grad_args_t *a, hipStream_t stream) {
@@ -371,8 +373,9 @@ hipError_t run_product(Product &q, int tile, int splits, void *workspace, long l
   place(q, c.plan, workspace);
   e = q.type == TF_T_BF16  ? launch_gemm_bf16(q.p, q.a.mn, q.b.mn, c.plan.tile, c.dma, stream)
       : q.type == TF_T_F16 ? launch_gemm_f16(q.p, q.a.mn, q.b.mn, c.plan.tile, c.dma, stream)
-                           : launch_gemm_f8(q.p, q.out_type, c.plan.tile, c.dma, stream);
-  return e == hipSuccess && c.plan.splits > 1 ? launch_gemm_join(q.p, q.out_type, stream) : e;
+      : q.type == TF_T_F8  ? launch_gemm_f8(q.p, q.out_type, c.plan.tile, c.dma, stream)
+                           : launch_gemm_i8(q.p, q.out_type, c.plan.tile, c.dma, stream);
+  return e == hipSuccess && c.plan.splits > 1 ? launch_gemm_join(q.p, q.type, q.out_type, stream) : e;
 }
 
 void check_choice(Checks &c, int tile, int splits) {
@@ -381,12 +384,13 @@ void check_choice(Checks &c, int tile, int splits) {
 }
 
 void check_linear_sizes(Checks &c, const tf_linear_args_t *a) {
-  c.one_of("type", a->type, {TF_T_BF16, TF_T_F16, TF_T_F8});
-  if (a->type == TF_T_F8) c.one_of("out_type", a->out_type, {TF_T_BF16, TF_T_F16});
+  c.one_of("type", a->type, {TF_T_BF16, TF_T_F16, TF_T_F8, TF_T_I8});
+  if (eight_bits(a->type)) c.one_of("out_type", a->out_type, {TF_T_BF16, TF_T_F16});
   else c.one_of("out_type", a->out_type, {a->type});
   c.size("m", a->m);
   c.size("n", a->n);
   c.size("k", a->k);
+  c.need(a->type != TF_T_I8 || a->k <= kMostI8, "k = ", a->k, ": sums of more than ", kMostI8, " products of 8-bit integers pass 32 bits");
   check_choice(c, a->tile, a->splits);
 }
 
@@ -416,9 +420,9 @@ int linear(const tf_linear_args_t *a, hipStream_t stream) {
   if (!a) return fail(TF_E_ARG, "tf_linear: null arguments");
   Checks c{call, {}};
   check_linear_sizes(c, a);
-  const bool f8 = a->type == TF_T_F8;
+  const bool eight = eight_bits(a->type);
   c.one_of("w_order", a->w_order, {0, 1});
-  c.need(!f8 || a->w_order == 1, "8-bit weights lie as n rows of k (w_order 1)");
+  c.need(!eight || a->w_order == 1, "8-bit weights lie as n rows of k (w_order 1)");
   c.one_of("act", a->act, {TF_ACT_NONE, TF_ACT_RELU, TF_ACT_GELU, TF_ACT_SILU});
   if (a->bias) c.one_of("bias_type", a->bias_type, {a->out_type, TF_T_F32});
   c.matrix("x", a->x, a->x_ld, a->n ? a->m : 0, a->k, a->type, true);
@@ -428,9 +432,9 @@ int linear(const tf_linear_args_t *a, hipStream_t stream) {
   c.matrix("residual", a->residual, a->residual_ld, a->m, a->n, a->out_type, false);
   c.matrix("out", a->out, a->out_ld, a->m, a->n, a->out_type, true);
   c.matrix("z", a->z, a->z_ld, a->m, a->n, a->out_type, false);
-  c.vector("x_scale", a->x_scale, a->m, TF_T_F32, f8);
-  c.vector("w_scale", a->w_scale, a->n, TF_T_F32, f8);
-  c.need(f8 || (!a->x_scale && !a->w_scale), "scales belong to 8-bit products");
+  c.vector("x_scale", a->x_scale, a->m, TF_T_F32, eight);
+  c.vector("w_scale", a->w_scale, a->n, TF_T_F32, eight);
+  c.need(eight || (!a->x_scale && !a->w_scale), "scales belong to 8-bit products");
   if (a->workspace_bytes) c.workspace(a->workspace, a->workspace_bytes, 1);
   if (!c.fine()) return fail(TF_E_ARG, c.wrong);
   if (a->m == 0 || a->n == 0) return TF_OK;
@@ -649,7 +653,16 @@ int tf_rms_norm(const tf_rms_norm_args_t *args, void *stream) {
 
 int tf_quantize_rows(const void *x, long long x_ld, long long rows, long long d, int type, void *y, long long y_ld,
                      float *scale, void *stream) {
-  return guarded([&] { return quantize_rows(x, x_ld, rows, d, type, y, y_ld, scale, static_cast<hipStream_t>(stream)); });
+  return guarded([&] {
+    return quantize_rows("tf_quantize_rows", x, x_ld, rows, d, type, y, y_ld, TF_T_F8, scale, static_cast<hipStream_t>(stream));
+  });
+}
+
+int tf_quantize_rows_to(const void *x, long long x_ld, long long rows, long long d, int type, void *y, long long y_ld,
+                        int y_type, float *scale, void *stream) {
+  return guarded([&] {
+    return quantize_rows("tf_quantize_rows_to", x, x_ld, rows, d, type, y, y_ld, y_type, scale, static_cast<hipStream_t>(stream));
+  });
 }
 
 int tf_rms_norm_grad_workspace(long long rows, long long d, long long *bytes) {

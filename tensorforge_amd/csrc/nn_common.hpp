@@ -15,6 +15,9 @@ typedef _Float16 f16;
 struct f8 {  // OCP e4m3: largest value 448, no infinities
   uint8_t bits;
 };
+struct i8 {  // an 8-bit integer
+  int8_t bits;
+};
 
 template <typename T, int N>
 struct Vec {
@@ -207,10 +210,24 @@ __device__ __forceinline__ void share_sum(const float *shares, int count, int d,
   }
 }
 
-// The 8-bit code's scale: the row's largest magnitude over 448, taken as at
-// least 2^-100 so that a row of zeros keeps a finite factor.
-constexpr float kF8Max = 448.0f;
-constexpr float kF8Tiny = 0x1p-100f;
-__device__ __forceinline__ float f8_top(float top) { return top < kF8Tiny ? kF8Tiny : top; }
+// The 8-bit code's scale: the row's largest magnitude over the largest code (448, or
+// 127 as an integer), taken as at least 2^-100 so that a row of zeros keeps a finite factor.
+template <typename O>
+constexpr float kCodeMax = __is_same(O, i8) ? 127.0f : 448.0f;
+constexpr float kCodeTiny = 0x1p-100f;
+__device__ __forceinline__ float code_top(float top) { return top < kCodeTiny ? kCodeTiny : top; }
+
+// Four integers of up to 8 bits, nearest to v (ties to even), in one word.  Beside 1.5 * 2^23 a
+// float's spacing is 1, so the addition rounds and leaves the integer in the lowest byte.  (A NaN
+// leaves some code.)
+__device__ __forceinline__ uint32_t round_to_bytes(float a, float b, float c, float d) {
+  constexpr float kOne = 12582912.0f;
+  const auto bits = [](float v) {
+#pragma clang fp contract(off)  // v is rounded before: fused with v's last product, ties would fall otherwise than the formula's
+    return __builtin_bit_cast(uint32_t, v + kOne);
+  };
+  return __builtin_amdgcn_perm(__builtin_amdgcn_perm(bits(d), bits(c), 0x0c0c0400u), __builtin_amdgcn_perm(bits(b), bits(a), 0x0c0c0400u),
+                               0x05040100u);
+}
 
 }  // namespace tfnn

@@ -277,6 +277,39 @@ __device__ __forceinline__ f32x4 block_mma(f8, i32x4 a0, i32x4 a1, i32x4 b0, i32
   return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(b, a, c, 0, 0, 0, 0, 0, 0);
 }
 
+// 8-bit integers: sums of 32-bit integers, exact while k is at most 131071 (128 * 128 * k < 2^31).
+__device__ __forceinline__ i32x4 block_mma(i8, i32x4 a0, i32x4 a1, i32x4 b0, i32x4 b1, i32x4 c) {
+  c = __builtin_amdgcn_mfma_i32_16x16x64_i8(b0, a0, c, 0, 0, 0);
+  return __builtin_amdgcn_mfma_i32_16x16x64_i8(b1, a1, c, 0, 0, 0);
+}
+
+// A 16 x 16 block's four sums a lane, and one of them.
+template <typename T>
+struct SumsOf {
+  typedef f32x4 four;
+  typedef float one;
+};
+template <>
+struct SumsOf<i8> {
+  typedef i32x4 four;
+  typedef int one;
+};
+template <typename T>
+using sums4 = typename SumsOf<T>::four;
+
+// An 8-bit product's sum times its scales.  Of integers in three roundings everywhere: left to the
+// compiler, some kernels would fuse the last with the bias's addition and others not, and the
+// results' bits would depend on the tile.
+template <typename T>
+__device__ __forceinline__ float scaled(typename SumsOf<T>::one sum, float sa, float sb) {
+  if constexpr (__is_same(T, i8)) {
+#pragma clang fp contract(off)
+    return static_cast<float>(sum) * sa * sb;
+  } else {
+    return sum * sa * sb;
+  }
+}
+
 // What is not finite becomes finite, by one instruction (a NaN the least number).
 __device__ __forceinline__ f32x4 made_finite(f32x4 v) {
   constexpr float kMost = 0x1.fffffep127f;
@@ -300,8 +333,8 @@ __device__ __forceinline__ void load_some(const T *p, int left, float (&v)[N]) {
   }
 }
 // STREAM: past the caches, for results that would push the operands out of them.
-template <bool STREAM = false, int N, typename T>
-__device__ __forceinline__ void store_some(T *p, int left, const float (&v)[N]) {
+template <bool STREAM = false, int N, typename T, typename V>
+__device__ __forceinline__ void store_some(T *p, int left, const V (&v)[N]) {
   if (left >= N) {
     typename Vec<T, N>::loose u;
 #pragma unroll
@@ -375,21 +408,22 @@ __device__ __forceinline__ void write_patch(const GemmParams &p, int split, cons
   constexpr int LANES = COLS / 8, STEP = 64 / LANES;
   const int lane = threadIdx.x % 64, n = n0 + lane % LANES * 8, left = p.n - n;
   if (left <= 0 || n + 7 < nt) return;
-  const auto take = [&](int row, float (&v)[8]) {
+  typedef typename SumsOf<T>::one Sum;
+  const auto take = [&](int row, auto (&v)[8]) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const f32x4 u = __builtin_bit_cast(f32x4, lds_read16(patch + patch_at<COLS>(row, lane % LANES * 2 + h)));
+      const auto u = __builtin_bit_cast(sums4<T>, lds_read16(patch + patch_at<COLS>(row, lane % LANES * 2 + h)));
 #pragma unroll
       for (int i = 0; i < 4; ++i) v[h * 4 + i] = u[i];
     }
   };
-  if (p.splits > 1) {  // one range of k of several: float sums, joined by gemm_join_kernel
+  if (p.splits > 1) {  // one range of k of several: sums joined by gemm_join_kernel
     const long ld = (p.n + 3) & ~3;
-    float *part = p.parts + split * (p.m * ld);
+    Sum *part = reinterpret_cast<Sum *>(p.parts) + split * (p.m * ld);
     for (int row = lane / LANES; row < ROWS; row += STEP) {
       const int m = m0 + row;
       if (m >= p.m || m < mt) continue;
-      float v[8];
+      Sum v[8];
       take(row, v);
       store_some(part + m * ld + n, left, v);
     }
@@ -404,11 +438,14 @@ __device__ __forceinline__ void write_patch(const GemmParams &p, int split, cons
       const int m = m0 + row;
       if (m >= p.m || m < mt) continue;
       float v[8];
-      take(row, v);
       if constexpr (sizeof(T) == 1) {
+        Sum sums[8];
+        take(row, sums);
         const float sa = p.sa[m];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = v[i] * sa * sb[i];
+        for (int i = 0; i < 8; ++i) v[i] = scaled<T>(sums[i], sa, sb[i]);
+      } else {
+        take(row, v);
       }
       finish<O, act(), STREAM>(p, m, n, v, bias);
     }
@@ -491,11 +528,11 @@ __device__ __forceinline__ void gemm_tile(const GemmParams &p, int block, int bl
   FragReader<BMN> fb;
   fa.init(wm * (BM / WM));
   fb.init(wn * (BN / WN));
-  f32x4 acc[MI][NI];
+  sums4<T> acc[MI][NI];
 #pragma unroll
   for (int i = 0; i < MI; ++i)
 #pragma unroll
-    for (int j = 0; j < NI; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int j = 0; j < NI; ++j) acc[i][j] = sums4<T>{0, 0, 0, 0};
 
   const auto multiply = [&](const lds_char *slab) {
     i32x4 a[2][MI], b[2][NI];
@@ -584,11 +621,13 @@ __device__ __forceinline__ void gemm_tile(const GemmParams &p, int block, int bl
       }
     }
     wait_lds();
-    if (term + 1 < TERMS) {
+    if constexpr (TERMS > 1) {
+      if (term + 1 < TERMS) {
 #pragma unroll
-      for (int i = 0; i < MI; ++i)
+        for (int i = 0; i < MI; ++i)
 #pragma unroll
-        for (int j = 0; j < NI; ++j) acc[i][j] = made_finite(acc[i][j]);
+          for (int j = 0; j < NI; ++j) acc[i][j] = made_finite(acc[i][j]);
+      }
     }
   }
   barrier();  // the slabs' LDS is the patches' now
@@ -602,7 +641,7 @@ __device__ __forceinline__ void gemm_tile(const GemmParams &p, int block, int bl
     for (int i = 0; i < ROWS / 16; ++i)
 #pragma unroll
       for (int j = 0; j < NI; ++j)
-        *reinterpret_cast<__attribute__((address_space(3))) f32x4 *>(
+        *reinterpret_cast<__attribute__((address_space(3))) sums4<T> *>(
             patch + patch_at<COLS>(i * 16 + lane % 16, j * 4 + lane / 16)) = acc[h * (ROWS / 16) + i][j];
     wait_lds();
     write_patch<T, O, ROWS, COLS>(p, split, patch, m0 + wm * (BM / WM) + h * ROWS, n0 + wn * COLS, tm * BM, tn * BN);
@@ -689,11 +728,11 @@ __global__ __launch_bounds__(64 * rows_waves(BMN, MI)) void gemm_rows_kernel(Gem
 #pragma unroll
       for (int q = 0; q < 2; ++q) h.a[i][q] = *reinterpret_cast<const loose16 *>(a[i] + k0 + (q * 4 + g) * P);
   };
-  f32x4 acc[MI][NB];
+  sums4<T> acc[MI][NB];
 #pragma unroll
   for (int i = 0; i < MI; ++i)
 #pragma unroll
-    for (int j = 0; j < NB; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int j = 0; j < NB; ++j) acc[i][j] = sums4<T>{0, 0, 0, 0};
   lds_char *turn = (lds_char *)smem + wave * 4096;
   const auto multiply = [&](Held &h) {
     i32x4 bf[NB][2];
@@ -771,7 +810,7 @@ __global__ __launch_bounds__(64 * rows_waves(BMN, MI)) void gemm_rows_kernel(Gem
   }
   // The waves' sums, added in wave order.
   __syncthreads();
-  f32x4 *join = reinterpret_cast<f32x4 *>(smem);
+  sums4<T> *join = reinterpret_cast<sums4<T> *>(smem);
 #pragma unroll
   for (int i = 0; i < MI; ++i)
 #pragma unroll
@@ -780,13 +819,15 @@ __global__ __launch_bounds__(64 * rows_waves(BMN, MI)) void gemm_rows_kernel(Gem
   const int block = wave;
   const int blocks = MI > 1 && p.terms == 2 ? MI / 2 * NB : MI * NB;
   if (block >= blocks) return;
-  f32x4 v = join[block * 64 + lane];
+  sums4<T> v = join[block * 64 + lane];
 #pragma unroll
   for (int w = 1; w < NW; ++w) v += join[(w * MI * NB + block) * 64 + lane];
-  if (blocks < MI * NB) {  // the other term, as in gemm_tile
-    v = made_finite(v);
+  if constexpr (sizeof(T) == 2) {
+    if (blocks < MI * NB) {  // the other term, as in gemm_tile
+      v = made_finite(v);
 #pragma unroll
-    for (int w = 0; w < NW; ++w) v += join[(w * MI * NB + blocks + block) * 64 + lane];
+      for (int w = 0; w < NW; ++w) v += join[(w * MI * NB + blocks + block) * 64 + lane];
+    }
   }
   const int m = block / NB * 16 + l, n = n0 + block % NB * 16 + g * 4;
   if (m >= p.m || n >= p.n || n + 3 < nt) return;
@@ -797,7 +838,7 @@ __global__ __launch_bounds__(64 * rows_waves(BMN, MI)) void gemm_rows_kernel(Gem
     load_some(p.sb + n, p.n - n, sb);
     const float sa = p.sa[m];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) out[i] = v[i] * sa * sb[i];
+    for (int i = 0; i < 4; ++i) out[i] = scaled<T>(v[i], sa, sb[i]);
   } else {
 #pragma unroll
     for (int i = 0; i < 4; ++i) out[i] = v[i];

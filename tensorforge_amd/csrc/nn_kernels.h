@@ -7,7 +7,7 @@
 namespace tfnn {
 
 // The values of TF_T_* in tforge_hip.h.
-enum Type { TYPE_F32 = 0, TYPE_BF16 = 1, TYPE_F16 = 2, TYPE_F8 = 3 };
+enum Type { TYPE_F32 = 0, TYPE_BF16 = 1, TYPE_F16 = 2, TYPE_F8 = 3, TYPE_I8 = 4 };
 
 // *_ld: elements between two rows.
 struct NormParams {
@@ -34,7 +34,7 @@ struct GemmParams {
   const void *bias = nullptr, *residual = nullptr;
   const float *sa = nullptr, *sb = nullptr;  // 8 bits: scales of A's rows and B's columns
   void *out = nullptr, *z = nullptr;
-  float *parts = nullptr;  // splits > 1: splits x m x (n up to a multiple of 4)
+  float *parts = nullptr;  // splits > 1: splits x m x (n up to a multiple of 4); of 8-bit integers, integers
   long lda = 0, ldb = 0, ldr = 0, ldo = 0, ldz = 0;
   int m = 0, n = 0, k = 0;
   int tiles_m = 0, tiles_n = 0, splits = 1;
@@ -56,6 +56,7 @@ constexpr int tile_columns(int tile) { return tile == TILE_64x128 ? 128 : tile_r
 hipError_t launch_gemm_bf16(const GemmParams &p, bool amn, bool bmn, int tile, bool dma, hipStream_t stream);
 hipError_t launch_gemm_f16(const GemmParams &p, bool amn, bool bmn, int tile, bool dma, hipStream_t stream);
 hipError_t launch_gemm_f8(const GemmParams &p, int out_type, int tile, bool dma, hipStream_t stream);
+hipError_t launch_gemm_i8(const GemmParams &p, int out_type, int tile, bool dma, hipStream_t stream);
 // A sum of `count` shares of d floats, rounded to `type`; d = 0: none.
 struct ShareParams {
   const float *shares = nullptr;
@@ -77,8 +78,8 @@ struct PackParams {
 };
 hipError_t launch_pack(const PackParams &p, int size, hipStream_t stream);
 
-// out = epilogue(sum of the splits' parts).
-hipError_t launch_gemm_join(const GemmParams &p, int out_type, hipStream_t stream);
+// out = epilogue(sum of the splits' parts), which are those of a product of `type`.
+hipError_t launch_gemm_join(const GemmParams &p, int type, int out_type, hipStream_t stream);
 // The same of a pair's products, those that are split.
 hipError_t launch_gemm_join_pair(const GemmParams &dx, const GemmParams &dw, int out_type, hipStream_t stream);
 
@@ -99,7 +100,7 @@ hipError_t launch_act_slope(const SlopeParams &p, const PackParams &pack, int ty
 hipError_t launch_share_sum(const float *shares, long count, int d, void *out, int type, hipStream_t stream);
 
 long norm_grad_shares(long rows, long d);
-hipError_t launch_rms_norm(const NormParams &p, int type, bool to_f8, hipStream_t stream);
+hipError_t launch_rms_norm(const NormParams &p, int type, int y_type, hipStream_t stream);
 hipError_t launch_rms_norm_grad(const NormGradParams &p, int type, hipStream_t stream);
 
 }  // namespace tfnn

@@ -4,6 +4,7 @@
 #include "nn_gemm.hpp"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace tfnn {
 namespace {
@@ -12,47 +13,51 @@ namespace {
 // Bound by latency: 64 x 4096 of four parts 3.0-3.8 us.  (Joined by the last of a tile's
 // workgroups instead, behind a fence, the whole product took 22.9 us against 13.1: the caches'
 // write-back costs more than the launch.)
-template <typename O, int ACT>
+template <typename S, typename O, int ACT>
 __device__ __forceinline__ void join_four(const GemmParams &p, unsigned block) {
+  typedef typename Vec<S, 4>::type S4;  // the parts' type: float, or int
   // (plan_product splits no product of 2^31 quads or more.  A 64-bit division takes 0.3 us here.)
   const unsigned quads = (p.n + 3u) / 4, id = block * 256 + threadIdx.x;
   const int m = static_cast<int>(id / quads), n = static_cast<int>(id % quads) * 4;
   const long ld = 4L * quads;
   if (m >= p.m) return;
-  const float *part = p.parts + m * ld + n;
-  f32x4 sum = *reinterpret_cast<const f32x4 *>(part);
+  const S *part = reinterpret_cast<const S *>(p.parts) + m * ld + n;
+  S4 sum = *reinterpret_cast<const S4 *>(part);
 #pragma unroll 4
-  for (int s = 1; s < p.splits; ++s) sum += *reinterpret_cast<const f32x4 *>(part + s * (p.m * ld));
-  float v[4] = {sum.x, sum.y, sum.z, sum.w}, bias[4];
+  for (int s = 1; s < p.splits; ++s) sum += *reinterpret_cast<const S4 *>(part + s * (p.m * ld));
+  float v[4], bias[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = static_cast<float>(sum[i]);
   if (p.sa) {
+    typedef typename std::conditional<std::is_same<S, int>::value, i8, f8>::type T;
     float sb[4];
     load_some(p.sb + n, p.n - n, sb);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = v[i] * p.sa[m] * sb[i];
+    for (int i = 0; i < 4; ++i) v[i] = scaled<T>(sum[i], p.sa[m], sb[i]);
   }
   load_bias<O>(p, n, bias);
   finish<O, ACT>(p, m, n, v, bias);
 }
-template <typename O, int ACT>
+template <typename S, typename O, int ACT>
 __global__ __launch_bounds__(256) void gemm_join_kernel(GemmParams p) {
-  join_four<O, ACT>(p, blockIdx.x);
+  join_four<S, O, ACT>(p, blockIdx.x);
 }
 template <typename O>
 __global__ __launch_bounds__(256) void gemm_join_pair_kernel(GemmParams dx, GemmParams dw, unsigned first) {
   const unsigned block = blockIdx.x;
-  if (block < first) join_four<O, ACT_NONE>(dx, block);
-  else join_four<O, ACT_NONE>(dw, block - first);
+  if (block < first) join_four<float, O, ACT_NONE>(dx, block);
+  else join_four<float, O, ACT_NONE>(dw, block - first);
 }
 
 unsigned join_blocks(const GemmParams &p) { return static_cast<unsigned>((p.m * ((p.n + 3L) / 4) + 255) / 256); }
 
-template <typename O>
+template <typename S, typename O>
 void join(const GemmParams &p, hipStream_t stream) {
   const dim3 grid(join_blocks(p));
-  if (p.act == ACT_RELU) gemm_join_kernel<O, ACT_RELU><<<grid, 256, 0, stream>>>(p);
-  else if (p.act == ACT_GELU) gemm_join_kernel<O, ACT_GELU><<<grid, 256, 0, stream>>>(p);
-  else if (p.act == ACT_SILU) gemm_join_kernel<O, ACT_SILU><<<grid, 256, 0, stream>>>(p);
-  else gemm_join_kernel<O, ACT_NONE><<<grid, 256, 0, stream>>>(p);
+  if (p.act == ACT_RELU) gemm_join_kernel<S, O, ACT_RELU><<<grid, 256, 0, stream>>>(p);
+  else if (p.act == ACT_GELU) gemm_join_kernel<S, O, ACT_GELU><<<grid, 256, 0, stream>>>(p);
+  else if (p.act == ACT_SILU) gemm_join_kernel<S, O, ACT_SILU><<<grid, 256, 0, stream>>>(p);
+  else gemm_join_kernel<S, O, ACT_NONE><<<grid, 256, 0, stream>>>(p);
 }
 
 // Copies to aligned lines, 16 bytes a thread.  Bound by memory: 7168 x 2107 and 8063 x 2107
@@ -182,8 +187,9 @@ hipError_t launch_pack(const PackParams &p, int size, hipStream_t stream) {
   return hipGetLastError();
 }
 
-hipError_t launch_gemm_join(const GemmParams &p, int out_type, hipStream_t stream) {
-  out_type == TYPE_BF16 ? join<bf16>(p, stream) : join<f16>(p, stream);
+hipError_t launch_gemm_join(const GemmParams &p, int type, int out_type, hipStream_t stream) {
+  if (type == TYPE_I8) out_type == TYPE_BF16 ? join<int, bf16>(p, stream) : join<int, f16>(p, stream);
+  else out_type == TYPE_BF16 ? join<float, bf16>(p, stream) : join<float, f16>(p, stream);
   return hipGetLastError();
 }
 

@@ -1,8 +1,8 @@
 // Root-mean-square norm with the residual's addition, in the input's type or in
-// 8 bits with a scale a row, the row quantisation alone, and the norm's gradient.
+// 8 bits (e4m3 or integers) with a scale a row, the row quantisation alone, and the norm's gradient.
 //
 //   h = x + residual           r = 1/sqrt(mean(h^2) + eps)
-//   y = (h*r)*w                scale = max|y| / 448, code = nearest(y * (448 * (1/max|y|)))
+//   y = (h*r)*w                scale = max|y| / top, code = nearest(y * (top * (1/max|y|))), top 448 or 127
 //   g = dy*w, xhat = h*r       dx = r*(g - xhat*mean(g*xhat)) + dh,  dw = sum over rows of dy*xhat
 //
 // All of it is bound by memory.  A row stays in its threads' registers between
@@ -61,6 +61,18 @@ __device__ __forceinline__ void store8(f8 *p, int left, const float (&v)[8]) {
 #pragma unroll
     for (int i = 0; i < 8; ++i)
       if (i < left) p[i].bits = static_cast<uint8_t>((i < 4 ? lo : hi) >> (8 * (i & 3)));
+  }
+}
+
+__device__ __forceinline__ void store8(i8 *p, int left, const float (&v)[8]) {
+  const uint32_t lo = round_to_bytes(v[0], v[1], v[2], v[3]), hi = round_to_bytes(v[4], v[5], v[6], v[7]);
+  if (left >= 8) {
+    typedef uint32_t loose2 __attribute__((ext_vector_type(2), aligned(1)));
+    *reinterpret_cast<loose2 *>(p) = loose2{lo, hi};
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i < left) p[i].bits = static_cast<int8_t>((i < 4 ? lo : hi) >> (8 * (i & 3)));
   }
 }
 
@@ -151,9 +163,9 @@ __global__ __launch_bounds__(256) void rms_norm_kernel(NormParams p) {
     const float r = p.weight ? rsqrtf(sum / static_cast<float>(p.d) + p.eps) : 1.0f;
     float f = 1.0f;
     if constexpr (sizeof(O) == 1) {
-      const float most = f8_top(top * r);
-      f = kF8Max * (1.0f / most);
-      if (t == 0) p.scale[row] = most / kF8Max;
+      const float most = code_top(top * r);
+      f = kCodeMax<O> * (1.0f / most);
+      if (t == 0) p.scale[row] = most / kCodeMax<O>;
     }
     O *y = static_cast<O *>(p.y) + row * p.y_ld;
 #pragma unroll
@@ -197,9 +209,9 @@ __global__ __launch_bounds__(256) void rms_norm_long_kernel(NormParams p) {
   const float r = p.weight ? rsqrtf(sum / static_cast<float>(p.d) + p.eps) : 1.0f;
   float f = 1.0f;
   if constexpr (sizeof(O) == 1) {
-    const float most = f8_top(top * r);
-    f = kF8Max * (1.0f / most);
-    if (threadIdx.x == 0) p.scale[row] = most / kF8Max;
+    const float most = code_top(top * r);
+    f = kCodeMax<O> * (1.0f / most);
+    if (threadIdx.x == 0) p.scale[row] = most / kCodeMax<O>;
   }
   for (int c = threadIdx.x * 8; c < p.d; c += NT * 8) {
     float v[8], u[8], w[8];
@@ -456,11 +468,17 @@ hipError_t launch_share_sum(const float *shares, long count, int d, void *out, i
   return hipGetLastError();
 }
 
-hipError_t launch_rms_norm(const NormParams &p, int type, bool to_f8, hipStream_t stream) {
-  if (type == TYPE_F32) to_f8 ? norm_launch<float, f8>(p, stream) : norm_launch<float, float>(p, stream);
-  else if (type == TYPE_BF16) to_f8 ? norm_launch<bf16, f8>(p, stream) : norm_launch<bf16, bf16>(p, stream);
-  else to_f8 ? norm_launch<f16, f8>(p, stream) : norm_launch<f16, f16>(p, stream);
+template <typename T>
+hipError_t norm_launch_to(const NormParams &p, int y_type, hipStream_t stream) {
+  if (y_type == TYPE_F8) norm_launch<T, f8>(p, stream);
+  else if (y_type == TYPE_I8) norm_launch<T, i8>(p, stream);
+  else norm_launch<T, T>(p, stream);
   return hipGetLastError();
+}
+
+hipError_t launch_rms_norm(const NormParams &p, int type, int y_type, hipStream_t stream) {
+  if (type == TYPE_F32) return norm_launch_to<float>(p, y_type, stream);
+  return type == TYPE_BF16 ? norm_launch_to<bf16>(p, y_type, stream) : norm_launch_to<f16>(p, y_type, stream);
 }
 
 hipError_t launch_rms_norm_grad(const NormGradParams &p, int type, hipStream_t stream) {

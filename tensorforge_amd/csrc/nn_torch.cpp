@@ -33,6 +33,7 @@ int type_of(ScalarType t) {
     case ScalarType::BFloat16: return TF_T_BF16;
     case ScalarType::Half: return TF_T_F16;
     case ScalarType::Float8_e4m3fn: return TF_T_F8;
+    case ScalarType::Char: return TF_T_I8;
     default: return -1;
   }
 }
@@ -186,28 +187,40 @@ void float_type(const Tensor &x, const char *name) {
                    ", not Float, BFloat16 or Half");
 }
 
+// quantize: False, True (e4m3) or the 8-bit type.
+bool eight_bits(PyObject *o, ScalarType &to) {
+  if (o == Py_False) return false;
+  to = ScalarType::Float8_e4m3fn;
+  if (o == Py_True) return true;
+  TORCH_CHECK_TYPE(THPDtype_Check(o), "the 8-bit type is not a dtype");
+  to = reinterpret_cast<THPDtype *>(o)->scalar_type;
+  TORCH_CHECK_TYPE(to == ScalarType::Float8_e4m3fn || to == ScalarType::Char, "8-bit rows are Float8_e4m3fn or Char, not ", to);
+  return true;
+}
+
 // (x, weight, residual, eps, quantize) -> (y, h) or (q, scale, h)
 PyObject *rms_norm(PyObject *, PyObject *const *a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   count(n, 5);
   const Tensor &x = tensor(a[0], "x"), &weight = tensor(a[1], "weight");
   const Tensor *residual = optional(a[2], "residual");
-  const bool quantize = a[4] == Py_True;
   float_type(x, "x");
   const ScalarType t = x.scalar_type();
+  ScalarType to = t;
+  const bool quantize = eight_bits(a[4], to);
   if (wants_grad({&x, &weight, residual})) Py_RETURN_NONE;
   const Rows xr = rows(x, "x");
   tf_rms_norm_args_t g{};
   g.x = xr.p, g.x_ld = xr.ld, g.rows = xr.m, g.d = xr.n, g.eps = static_cast<float>(number(a[3]));
   g.weight = vector(weight, "weight", xr.n, t, ScalarType::Float);
-  g.type = type_of(t), g.weight_type = type_of(weight.scalar_type()), g.y_type = quantize ? TF_T_F8 : g.type;
+  g.type = type_of(t), g.weight_type = type_of(weight.scalar_type()), g.y_type = type_of(to);
   if (residual) {
     const Rows r = rows_of(*residual, "residual", xr.m, xr.n, t);
     g.residual = r.p, g.residual_ld = r.ld;
   }
   on_gpu(x, {&weight, residual});
   const On on(x);
-  Tensor y = fresh(x, x.sizes(), quantize ? ScalarType::Float8_e4m3fn : t), h, scale;
+  Tensor y = fresh(x, x.sizes(), to), h, scale;
   g.y = y.data_ptr(), g.y_ld = g.h_ld = xr.n;
   if (residual) h = fresh(x, x.sizes(), t), g.h = h.data_ptr();
   if (quantize) scale = fresh(x, x.sizes().slice(0, x.dim() - 1), ScalarType::Float), g.scale = scale.data_ptr<float>();
@@ -217,19 +230,22 @@ PyObject *rms_norm(PyObject *, PyObject *const *a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-// (x) -> (q, scale)
+// (x, dtype) -> (q, scale)
 PyObject *quantize_rows(PyObject *, PyObject *const *a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  count(n, 1);
+  count(n, 2);
   const Tensor &x = tensor(a[0], "x");
   float_type(x, "x");
+  ScalarType to = ScalarType::Float8_e4m3fn;
+  eight_bits(a[1], to);
   no_gradient("quantize_rows", {&x});
   const Rows r = rows(x, "x");
   on_gpu(x, {});
   const On on(x);
-  const Tensor q = fresh(x, x.sizes(), ScalarType::Float8_e4m3fn);
+  const Tensor q = fresh(x, x.sizes(), to);
   const Tensor scale = fresh(x, x.sizes().slice(0, x.dim() - 1), ScalarType::Float);
-  check(tf_quantize_rows(r.p, r.ld, r.m, r.n, type_of(x.scalar_type()), q.data_ptr(), r.n, scale.data_ptr<float>(), on.stream));
+  check(tf_quantize_rows_to(r.p, r.ld, r.m, r.n, type_of(x.scalar_type()), q.data_ptr(), r.n, type_of(to), scale.data_ptr<float>(),
+                            on.stream));
   return tuple({&q, &scale});
   END_HANDLE_TH_ERRORS
 }
@@ -273,17 +289,17 @@ PyObject *linear(PyObject *, PyObject *const *a, Py_ssize_t n) {
   const Tensor *xs = optional(a[6], "x_scale"), *ws = optional(a[7], "w_scale");
   const bool keep = a[5] == Py_True;
   const ScalarType t = x.scalar_type();
-  const bool f8 = t == ScalarType::Float8_e4m3fn;
-  TORCH_CHECK_TYPE(half_type(t) || f8, "x is ", t, ", not BFloat16, Half or Float8_e4m3fn");
-  ScalarType to = f8 ? ScalarType::BFloat16 : t;
+  const bool eight = t == ScalarType::Float8_e4m3fn || t == ScalarType::Char;
+  TORCH_CHECK_TYPE(half_type(t) || eight, "x is ", t, ", not BFloat16, Half, Float8_e4m3fn or Char");
+  ScalarType to = eight ? ScalarType::BFloat16 : t;
   if (a[8] != Py_None) {
     TORCH_CHECK_TYPE(THPDtype_Check(a[8]), "out_dtype is not a dtype");
     to = reinterpret_cast<THPDtype *>(a[8])->scalar_type;
-    TORCH_CHECK_TYPE(half_type(to) && (f8 || to == t), "out_dtype is ", to,
-                     f8 ? ", not BFloat16 or Half" : ": 16-bit products keep x's type");
+    TORCH_CHECK_TYPE(half_type(to) && (eight || to == t), "out_dtype is ", to,
+                     eight ? ", not BFloat16 or Half" : ": 16-bit products keep x's type");
   }
-  TORCH_CHECK_VALUE(f8 || (!xs && !ws), "scales belong to 8-bit products");
-  if (f8) no_gradient("an 8-bit product", {&x, &w, bias, residual, xs, ws});
+  TORCH_CHECK_VALUE(eight || (!xs && !ws), "scales belong to 8-bit products");
+  if (eight) no_gradient("an 8-bit product", {&x, &w, bias, residual, xs, ws});
   else if (wants_grad({&x, &w, bias, residual})) Py_RETURN_NONE;
   const Rows xr = rows(x, "x");
   const Weights wr = weights(w, xr.n, t);
@@ -296,7 +312,7 @@ PyObject *linear(PyObject *, PyObject *const *a, Py_ssize_t n) {
     const Rows r = rows_of(*residual, "residual", xr.m, wr.n, to);
     g.residual = r.p, g.residual_ld = r.ld;
   }
-  if (f8) {
+  if (eight) {
     TORCH_CHECK_VALUE(wr.order == 1, "8-bit weights have to lie column by column: pass weight.t() of an n x k weight");
     TORCH_CHECK_VALUE(xs && ws, "an 8-bit product needs x_scale and w_scale");
     same_type(*xs, "x_scale", ScalarType::Float, ScalarType::Float);

@@ -106,11 +106,11 @@ __global__ __launch_bounds__(512, 2) void gemm_wide_kernel(GemmParams p) {
   FragReader<BMN> fb;
   fa.init(wm * 128);
   fb.init(wn * 64);
-  f32x4 acc[8][4];
+  sums4<T> acc[8][4];
 #pragma unroll
   for (int i = 0; i < 8; ++i)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int j = 0; j < 4; ++j) acc[i][j] = sums4<T>{0, 0, 0, 0};
 
   // Slabs 0 and 1, but for slab 1's second half of A, which the first phase loads.
 #pragma unroll
@@ -191,7 +191,7 @@ __global__ __launch_bounds__(512, 2) void gemm_wide_kernel(GemmParams p) {
     for (int i = 0; i < 4; ++i)
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        *reinterpret_cast<__attribute__((address_space(3))) f32x4 *>(patch + patch_at<64>(i * 16 + lane % 16, j * 4 + lane / 16)) =
+        *reinterpret_cast<__attribute__((address_space(3))) sums4<T> *>(patch + patch_at<64>(i * 16 + lane % 16, j * 4 + lane / 16)) =
             acc[4 * h + i][j];
     wait_lds();
     write_patch<T, O, 64, 64, true>(p, split, patch, tm * 256 + wm * 128 + h * 64, tn * 256 + wn * 64, 0, 0);

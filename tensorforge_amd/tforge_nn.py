@@ -5,7 +5,8 @@ gradients.
 
     h, y = x + r, ...         y, h = rms_norm(x, weight, residual=r)
     8-bit rows with scales    q, s, h = rms_norm(x, weight, residual=r, quantize=True)
-                              q, s = quantize_rows(x)
+                              q, s = quantize_rows(x)   (e4m3; quantize=torch.int8 and
+                              quantize_rows(x, torch.int8): integers)
     act(x @ w + b) + r        out = linear(x, w, b, "gelu", r)
     8-bit product             out = linear(q, wq.t(), b, "gelu", r, x_scale=s, w_scale=ws)
     gradients                 dx, dweight = rms_norm_grad(dy, h, weight, dh=...)
@@ -46,14 +47,18 @@ def _act(activation):
 # ---- norm -----------------------------------------------------------------------
 
 
+def _eight_bits(quantize):
+    return quantize if isinstance(quantize, torch.dtype) else True if quantize else False
+
+
 def rms_norm(x, weight, residual=None, eps=1e-6, quantize=False):
     """h = x + residual;  y = h / sqrt(mean(h^2) + eps) * weight over the last dimension.
 
-    Returns (y, h), h None without a residual; with quantize=True (q, scale, h): y in
-    8 bits (float8_e4m3fn) with one scale a row, y ~ q * scale.  x is float32,
-    bfloat16 or float16, the weight of x's type or float32.
+    Returns (y, h), h None without a residual; with quantize=True or an 8-bit dtype
+    (q, scale, h): y in 8 bits (float8_e4m3fn, or int8) with one scale a row, y ~ q * scale.
+    x is float32, bfloat16 or float16, the weight of x's type or float32.
     """
-    got = _C.rms_norm(x, weight, residual, eps, True if quantize else False)
+    got = _C.rms_norm(x, weight, residual, eps, _eight_bits(quantize))
     if got is not None:
         return got
     if quantize:
@@ -62,9 +67,9 @@ def rms_norm(x, weight, residual=None, eps=1e-6, quantize=False):
     return y, (None if residual is None else h)
 
 
-def quantize_rows(x):
-    """(q, scale): x in 8 bits (float8_e4m3fn) with one float32 scale a row of the last dimension, x ~ q * scale."""
-    return _C.quantize_rows(x)
+def quantize_rows(x, dtype=torch.float8_e4m3fn):
+    """(q, scale): x in 8 bits (float8_e4m3fn or int8) with one float32 scale a row of the last dimension, x ~ q * scale."""
+    return _C.quantize_rows(x, dtype)
 
 
 def rms_norm_grad(dy, h, weight, eps=1e-6, dh=None):
@@ -107,9 +112,9 @@ def linear(x, w, bias=None, activation="none", residual=None, keep=False, x_scal
     """z = x @ w + bias;  out = activation(z) + residual, rounded once.
 
     x (..., k) and w (k, n) are bfloat16 or float16; w may lie row by row or column by
-    column (w = weight.t() of an n x k weight).  Or both are float8_e4m3fn, w column by
-    column, with x_scale (one a row) and w_scale (one a column), and out_dtype
-    (bfloat16 unless given).  bias is of the output's type or float32.  activation:
+    column (w = weight.t() of an n x k weight).  Or both are float8_e4m3fn, or both int8
+    (sums exact, k at most 131071), w column by column, with x_scale (one a row) and
+    w_scale (one a column), and out_dtype (bfloat16 unless given).  bias is of the output's type or float32.  activation:
     "none", "relu", "gelu" (by the normal distribution), "silu".  Returns out, or
     (out, z) with keep=True; both are differentiable.  tile and splits override the choice by sizes
     (tf_linear_args_t in tforge_hip.h); grad_terms is linear_grad's terms under autograd.
