@@ -310,6 +310,26 @@ int tf_quantize_rows(const void *x, long long x_ld, long long rows, long long d,
 int tf_quantize_rows_to(const void *x, long long x_ld, long long rows, long long d, int type, void *y, long long y_ld,
                         int y_type, float *scale, void *stream);
 
+/* Activations kept in 8 bits for a backward pass: rows x d values in groups of 32
+ * neighbours of a row, each value an integer of -127..127 times its group's unit, the
+ * least power of two (2^-126 at least) whose integers stay within 127 (nearest, ties
+ * to even).  In memory, 16-byte aligned, tf_keep8_bytes(rows, d) in all: rows x
+ * ceil(d/32) x 32 integers, zeros behind a row's end, then rows x ceil(d/32)
+ * bytes e, the unit being 2^(e-127).  A group that holds an infinity or a NaN has e =
+ * 255 and zeros, and stands for NaN throughout.
+ * positive: values above zero keep an integer of at least 1, so that relu's
+ * gradient from a pre-activation kept so is that of the pre-activation itself.
+ * tf_restore8 gives the values in `type`: exact in TF_T_F32 and TF_T_BF16; in
+ * TF_T_F16 rounded, past 65504 that. */
+int tf_keep8_bytes(long long rows, long long d, long long *bytes);
+int tf_keep8(const void *x, long long x_ld, long long rows, long long d, int type, int positive, void *kept, void *stream);
+int tf_restore8(const void *kept, long long rows, long long d, int type, void *x, long long x_ld, void *stream);
+
+/* Which operands of a gradient are kept in 8 bits (their *_ld does not count). */
+#define TF_KEPT_H 1 /* tf_rms_norm_grad's h        */
+#define TF_KEPT_X 1 /* tf_linear_grad's x          */
+#define TF_KEPT_Z 2 /* tf_linear_grad's z          */
+
 /* tf_rms_norm's gradient.  r = 1/sqrt(mean(h^2) + eps), xhat = h*r:
  *   dx = r*(dy*weight - xhat*mean(dy*weight*xhat)) + dh     (also the residual's)
  *   dweight = sum over rows of dy*xhat */
@@ -323,7 +343,7 @@ typedef struct {
   long long rows, d;
   int type, weight_type; /* as tf_rms_norm's                                        */
   float eps;
-  int reserved;    /* 0                                                             */
+  int kept;        /* 0, or TF_KEPT_H                                               */
   void *workspace; /* 16-byte aligned, tf_rms_norm_grad_workspace(rows, d) bytes    */
   long long workspace_bytes;
 } tf_rms_norm_grad_args_t;
@@ -395,7 +415,8 @@ typedef struct {
   int act;
   int tile, splits; /* both products', as tf_linear's                                */
   int terms;     /* of dz in the products: 0 by the sizes, 1 or 2                   */
-  int reserved;  /* 0                                                               */
+  int kept;      /* 0, or TF_KEPT_X, TF_KEPT_Z or both: x goes into its product
+                    rounded to `type`, z into the slope as it is                     */
 } tf_linear_grad_args_t;
 /* As tf_linear_workspace; which of dx, dw and dbias are wanted counts too. */
 int tf_linear_grad_workspace(const tf_linear_grad_args_t *args, long long *bytes);

@@ -59,7 +59,7 @@ class RmsNormGradArgs(ctypes.Structure):
     _fields_ = [(f, ctypes.c_void_p) for f in ("dy", "h", "dh", "weight", "dx", "dweight")] + \
                [(f, ctypes.c_longlong) for f in ("dy_ld", "h_ld", "dh_ld", "dx_ld", "rows", "d")] + \
                [("type", ctypes.c_int), ("weight_type", ctypes.c_int), ("eps", ctypes.c_float),
-                ("reserved", ctypes.c_int), ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_longlong)]
+                ("kept", ctypes.c_int), ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_longlong)]
 
 
 class LinearArgs(ctypes.Structure):
@@ -75,7 +75,7 @@ class LinearGradArgs(ctypes.Structure):
     _fields_ = [(f, ctypes.c_void_p) for f in ("dy", "x", "w", "z", "dx", "dw", "dbias", "workspace")] + \
                [(f, ctypes.c_longlong) for f in ("workspace_bytes", "dy_ld", "x_ld", "w_ld", "z_ld", "dx_ld", "dw_ld",
                                                  "m", "n", "k")] + \
-               [(f, ctypes.c_int) for f in ("w_order", "type", "bias_type", "act", "tile", "splits", "terms", "reserved")]
+               [(f, ctypes.c_int) for f in ("w_order", "type", "bias_type", "act", "tile", "splits", "terms", "kept")]
 
 
 # (name, restype, argtypes) of every exported function, in header order.
@@ -108,6 +108,9 @@ SIGNATURES = [
     ("tf_rms_norm", I, [P, P]),
     ("tf_quantize_rows", I, [P, LL, LL, LL, I, P, LL, P, P]),
     ("tf_quantize_rows_to", I, [P, LL, LL, LL, I, P, LL, I, P, P]),
+    ("tf_keep8_bytes", I, [LL, LL, ctypes.POINTER(LL)]),
+    ("tf_keep8", I, [P, LL, LL, LL, I, I, P, P]),
+    ("tf_restore8", I, [P, LL, LL, I, P, LL, P]),
     ("tf_rms_norm_grad_workspace", I, [LL, LL, ctypes.POINTER(LL)]),
     ("tf_rms_norm_grad", I, [P, P]),
     ("tf_linear_workspace", I, [P, ctypes.POINTER(LL)]),

@@ -56,6 +56,12 @@ struct Checks {
   void vector(const char *name, const void *p, long long n, int type, bool wanted) {
     matrix(name, p, n, 1, n, type, wanted);
   }
+  // Rows kept in 8 bits.
+  void kept(const char *name, const void *p, long long rows, long long d, bool wanted) {
+    if (!fine() || rows <= 0 || d <= 0) return;
+    need(p || !wanted, name, " is a null pointer");
+    need(reinterpret_cast<uintptr_t>(p) % 16 == 0, name, ", kept in 8 bits, is not 16-byte aligned");
+  }
   void workspace(const void *p, long long given, long long needed) {
     need(given >= needed, "the workspace has ", given, " bytes, ", needed, " are needed");
     need(needed == 0 || (p && reinterpret_cast<uintptr_t>(p) % 16 == 0), "the workspace is null or not 16-byte aligned");
@@ -130,8 +136,10 @@ int rms_norm_grad(const tf_rms_norm_grad_args_t *a, hipStream_t stream) {
   c.size("rows", a->rows);
   c.size("d", a->d);
   c.need(a->eps >= 0, "eps is negative or not a number");
+  c.one_of("kept", a->kept, {0, TF_KEPT_H});
   c.matrix("dy", a->dy, a->dy_ld, a->rows, a->d, a->type, true);
-  c.matrix("h", a->h, a->h_ld, a->rows, a->d, a->type, true);
+  if (a->kept) c.kept("h", a->h, a->rows, a->d, true);
+  else c.matrix("h", a->h, a->h_ld, a->rows, a->d, a->type, true);
   c.matrix("dh", a->dh, a->dh_ld, a->rows, a->d, a->type, false);
   c.vector("weight", a->weight, a->d, a->weight_type, true);
   c.matrix("dx", a->dx, a->dx_ld, a->rows, a->d, a->type, true);
@@ -140,6 +148,7 @@ int rms_norm_grad(const tf_rms_norm_grad_args_t *a, hipStream_t stream) {
   if (!c.fine()) return fail(TF_E_ARG, c.wrong);
   if (a->d == 0) return TF_OK;
   NormGradParams p;
+  p.kept = a->kept != 0;
   p.dy = a->dy, p.h = a->h, p.dh = a->dh, p.weight = a->weight, p.dx = a->dx, p.dw = a->dweight;
   p.shares = static_cast<float *>(a->workspace);
   p.dy_ld = a->dy_ld, p.h_ld = a->h_ld, p.dh_ld = a->dh_ld, p.dx_ld = a->dx_ld, p.rows = a->rows;
@@ -367,7 +376,7 @@ hipError_t run_product(Product &q, int tile, int splits, void *workspace, long l
     PackParams pack;
     if (c.pack_a) to += copy_of(q.a, size, to, pack);
     if (c.pack_b) copy_of(q.b, size, to, pack);
-    e = launch_pack(pack, size, stream);
+    e = launch_pack(pack, q.type, stream);
     if (e != hipSuccess) return e;
   }
   place(q, c.plan, workspace);
@@ -448,12 +457,12 @@ struct GradPlan {
   int terms = 1;         // of dz
   int rows = 0;          // of a workgroup of dz
   long dz_ld = 0, count = 1;                  // shares of the bias gradient
-  long long dz = 0, shares = 0, product = 0;  // bytes
+  long long dz = 0, shares = 0, x = 0, product = 0;  // bytes; x: restored from 8 bits
   bool pair = false;                          // both products in one launch, in these ranges of k,
   int dx_splits = 1, dw_splits = 1;           // and of `product`, the bytes of
   long long copies = 0, dx_parts = 0;         // aligned copies of w and x, and dx's parts
   Product dx, dw;
-  long long bytes() const { return dz + shares + product; }
+  long long bytes() const { return dz + shares + x + product; }
 };
 
 // Both products on 64 x 64 tiles in one launch (1148 x 848 x 209 bfloat16 silu 16.7 us, 35.8 in
@@ -516,7 +525,8 @@ GradPlan plan_grad(const tf_linear_grad_args_t *a) {
   };
   g.dx = {a->type, a->type, dz(false), nk ? Operand{a->w, a->w_ld, n, k, true, false} : Operand{a->w, a->w_ld, k, n, false, false}, {}};
   g.dx.p.m = m, g.dx.p.n = k, g.dx.p.k = n, g.dx.p.out = a->dx, g.dx.p.ldo = a->dx_ld;
-  const Operand x{a->x, a->x_ld, m, k, true, false};
+  Operand x{a->x, a->x_ld, m, k, true, false};
+  if (a->kept & TF_KEPT_X && a->dw) x.ld = packed_ld(x, 2), x.ours = true, g.x = packed_bytes(x, 2);
   g.dw = {a->type, a->type, nk ? dz(true) : x, nk ? x : dz(true), {}};
   g.dw.p.m = nk ? n : k, g.dw.p.n = nk ? k : n, g.dw.p.k = m, g.dw.p.out = a->dw, g.dw.p.ldo = a->dw_ld;
   if (g.terms == 2) {
@@ -528,7 +538,7 @@ GradPlan plan_grad(const tf_linear_grad_args_t *a) {
   long long copies = 0;
   if (!a->tile && !a->splits && a->dx && a->dw && m) {
     copies = (direct_loads(g.dx.b, 2) ? 0 : packed_bytes(g.dx.b, 2)) + (direct_loads(x, 2) ? 0 : packed_bytes(x, 2));
-    const bool more = !g.own_dz && !a->dbias && (odd || copies);  // a launch for the copies alone
+    const bool more = !g.own_dz && !a->dbias && (odd || copies || g.x);  // a launch for the copies alone
     pair = plan_pair(g) + (more ? 4 : 0) + copies * 0.21e-6;
   }
   if (pair > 8) {
@@ -562,6 +572,7 @@ void check_grad_sizes(Checks &c, const tf_linear_grad_args_t *a) {
   c.size("k", a->k);
   check_choice(c, a->tile, a->splits);
   c.one_of("terms", a->terms, {0, 1, 2});
+  c.one_of("kept", a->kept, {0, TF_KEPT_X, TF_KEPT_Z, TF_KEPT_X | TF_KEPT_Z});
 }
 
 int linear_grad_workspace(const tf_linear_grad_args_t *a, long long *bytes) {
@@ -581,8 +592,10 @@ int linear_grad(const tf_linear_grad_args_t *a, hipStream_t stream) {
   const long long wr = a->w_order ? a->n : a->k, wc = a->w_order ? a->k : a->n;
   if (a->dbias) c.one_of("bias_type", a->bias_type, {a->type, TF_T_F32});
   c.matrix("dy", a->dy, a->dy_ld, a->m, a->n, a->type, true);
-  c.matrix("z", a->z, a->z_ld, a->m, a->n, a->type, a->act != TF_ACT_NONE);
-  c.matrix("x", a->x, a->x_ld, a->m, a->k, a->type, a->dw != nullptr);
+  if (a->kept & TF_KEPT_Z) c.kept("z", a->z, a->m, a->n, a->act != TF_ACT_NONE);
+  else c.matrix("z", a->z, a->z_ld, a->m, a->n, a->type, a->act != TF_ACT_NONE);
+  if (a->kept & TF_KEPT_X) c.kept("x", a->x, a->m, a->k, a->dw != nullptr);
+  else c.matrix("x", a->x, a->x_ld, a->m, a->k, a->type, a->dw != nullptr);
   c.matrix("w", a->w, a->w_ld, wr, wc, a->type, a->dx != nullptr);
   c.matrix("dx", a->dx, a->dx_ld, a->m, a->k, a->type, false);
   c.matrix("dw", a->dw, a->dw_ld, wr, wc, a->type, false);
@@ -594,7 +607,8 @@ int linear_grad(const tf_linear_grad_args_t *a, hipStream_t stream) {
 
   char *ws = static_cast<char *>(a->workspace);
   float *shares = reinterpret_cast<float *>(ws + g.dz);
-  void *rest = ws + g.dz + g.shares;
+  char *const restored = ws + g.dz + g.shares;
+  void *rest = restored + g.x;
   const int m = static_cast<int>(a->m), n = static_cast<int>(a->n), k = static_cast<int>(a->k);
   char *const parts = static_cast<char *>(rest) + g.copies;
   hipError_t e = hipSuccess;
@@ -605,16 +619,24 @@ int linear_grad(const tf_linear_grad_args_t *a, hipStream_t stream) {
     if (!direct_loads(w, 2)) to += copy_of(w, 2, to, pack);
     if (!direct_loads(x, 2)) copy_of(x, 2, to, pack);
   }
+  if (g.x) {  // beside dz: x in 16 bits
+    Operand &x = a->w_order ? g.dw.b : g.dw.a;
+    const int i = pack.pieces[0] ? 1 : 0;
+    pack.from[i] = a->x, pack.rows[i] = m, pack.columns[i] = k, pack.kept[i] = true;
+    pack.to[i] = restored, pack.to_ld[i] = x.ld, pack.pieces[i] = x.lines * x.ld / 8;
+    x.p = restored;
+  }
   if (m && n && (g.own_dz || a->dbias)) {
     SlopeParams s{};
     s.rows = g.rows;
+    s.kept = (a->kept & TF_KEPT_Z) != 0;
     s.dy = a->dy, s.z = a->z, s.dy_ld = a->dy_ld, s.z_ld = a->z_ld, s.m = m, s.n = n, s.act = a->act;
     if (g.own_dz) s.dz = ws, s.dz_ld = g.dz_ld, s.lo = g.terms == 2 ? g.dz / 4 : 0;
     if (a->dbias && g.shares) s.shares = shares;
     if (a->dbias && !g.shares) s.sums = a->dbias, s.sums_type = a->bias_type;
     e = launch_act_slope(s, pack, a->type, stream);
-  } else if (g.copies) {
-    e = launch_pack(pack, 2, stream);
+  } else if (pack.pieces[0]) {
+    e = launch_pack(pack, a->type, stream);
   }
   if (e == hipSuccess && a->dbias && n && ((g.shares && !g.pair) || !m))
     e = launch_share_sum(shares, m ? g.count : 0, n, a->dbias, a->bias_type, stream);
@@ -679,6 +701,47 @@ int tf_rms_norm_grad_workspace(long long rows, long long d, long long *bytes) {
 
 int tf_rms_norm_grad(const tf_rms_norm_grad_args_t *args, void *stream) {
   return guarded([&] { return rms_norm_grad(args, static_cast<hipStream_t>(stream)); });
+}
+
+int tf_keep8_bytes(long long rows, long long d, long long *bytes) {
+  return guarded([&] {
+    Checks c{"tf_keep8_bytes", {}};
+    c.size("rows", rows);
+    c.size("d", d);
+    c.need(bytes != nullptr, "null arguments");
+    if (!c.fine()) return fail(TF_E_ARG, c.wrong);
+    *bytes = rows * ceil_div(d, 32) * 33;
+    return TF_OK;
+  });
+}
+
+int tf_keep8(const void *x, long long x_ld, long long rows, long long d, int type, int positive, void *kept, void *stream) {
+  return guarded([&] {
+    Checks c{"tf_keep8", {}};
+    c.one_of("type", type, {TF_T_F32, TF_T_BF16, TF_T_F16});
+    c.one_of("positive", positive, {0, 1});
+    c.size("rows", rows);
+    c.size("d", d);
+    c.matrix("x", x, x_ld, rows, d, type, true);
+    c.kept("kept", kept, rows, d, true);
+    if (!c.fine()) return fail(TF_E_ARG, c.wrong);
+    if (rows == 0 || d == 0) return TF_OK;
+    return hip(launch_keep(x, x_ld, rows, static_cast<int>(d), type, positive != 0, kept, static_cast<hipStream_t>(stream)), "tf_keep8");
+  });
+}
+
+int tf_restore8(const void *kept, long long rows, long long d, int type, void *x, long long x_ld, void *stream) {
+  return guarded([&] {
+    Checks c{"tf_restore8", {}};
+    c.one_of("type", type, {TF_T_F32, TF_T_BF16, TF_T_F16});
+    c.size("rows", rows);
+    c.size("d", d);
+    c.kept("kept", kept, rows, d, true);
+    c.matrix("x", x, x_ld, rows, d, type, true);
+    if (!c.fine()) return fail(TF_E_ARG, c.wrong);
+    if (rows == 0 || d == 0) return TF_OK;
+    return hip(launch_restore(kept, rows, static_cast<int>(d), type, x, x_ld, static_cast<hipStream_t>(stream)), "tf_restore8");
+  });
 }
 
 int tf_linear_workspace(const tf_linear_args_t *args, long long *bytes) {

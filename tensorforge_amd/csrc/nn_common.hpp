@@ -230,4 +230,60 @@ __device__ __forceinline__ uint32_t round_to_bytes(float a, float b, float c, fl
                                0x05040100u);
 }
 
+// ---- what is kept in 8 bits -----------------------------------------------------
+//
+// Rows in groups of 32 neighbours: a group's values are integers of -127..127 times its unit,
+// the least power of two (2^-126 at least) whose integers stay within 127.  rows x groups x 32
+// codes, zeros behind a row's end, then rows x groups exponents: the unit is 2^(exponent - 127),
+// a float of that exponent field.  A group with an infinity or a NaN has the exponent 255 (an
+// infinite unit) and codes 0, which make NaN.  A unit of two's power restores exactly: the
+// values need no more than bfloat16's bits.
+constexpr int kGroup = 32;
+
+struct Kept {
+  const uint8_t *codes = nullptr, *exponents = nullptr;
+  long groups = 0;  // of a row
+};
+__host__ __device__ inline Kept kept_at(const void *p, long rows, long d) {
+  const long groups = (d + kGroup - 1) / kGroup;
+  const uint8_t *codes = static_cast<const uint8_t *>(p);
+  return {codes, codes + rows * groups * kGroup, groups};
+}
+
+// The exponent for a group's largest magnitude (as bits, which order as magnitudes do, NaN above
+// all).  2^6 * 1.m of the unit below rounds past 127 from 1.m = 127.5/64 on: a carry from there.
+__device__ __forceinline__ uint32_t group_exponent(uint32_t top) {
+  const int e = static_cast<int>((top + 0x10000u) >> 23) - 6;
+  return top >= 0x7f800000u ? 255u : static_cast<uint32_t>(max(e, 1));
+}
+
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+
+__device__ __forceinline__ void restore_codes(u32x2 codes, uint32_t exponent, float (&v)[8]) {
+  const float unit = __builtin_bit_cast(float, exponent << 23);
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    v[i] = (static_cast<float>(((i < 4 ? codes.x : codes.y) ^ 0x80808080u) >> (8 * (i & 3)) & 255u) - 128.0f) * unit;
+}
+
+// 8 values from c (a multiple of 8) of a row; zeros past its last group.
+__device__ __forceinline__ void load_kept8(const Kept &k, long row, int c, float (&v)[8]) {
+  const long length = k.groups * kGroup, at = min(static_cast<long>(c), length - 8);
+  u32x2 codes = *reinterpret_cast<const u32x2 *>(k.codes + row * length + at);
+  uint32_t exponent = k.exponents[row * k.groups + at / kGroup];
+  if (c > at) codes = u32x2{0, 0}, exponent = 1;
+  restore_codes(codes, exponent, v);
+}
+
+// A kept value in T: past float16's largest it is that.
+template <typename T>
+__device__ __forceinline__ T kept_as(float v) {
+  if constexpr (__is_same(T, f16)) {
+    const float near = __builtin_fminf(__builtin_fmaxf(v, -65504.0f), 65504.0f);
+    return static_cast<T>(v != v ? v : near);
+  } else {
+    return static_cast<T>(v);
+  }
+}
+
 }  // namespace tfnn

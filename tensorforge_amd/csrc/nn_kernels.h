@@ -21,7 +21,8 @@ struct NormParams {
 };
 
 struct NormGradParams {
-  const void *dy, *h, *dh, *weight;
+  const void *dy, *h, *dh, *weight;  // h in `type`, or kept in 8 bits
+  bool kept;
   void *dx, *dw;
   float *shares;  // norm_grad_shares(rows, d) x d
   long dy_ld, h_ld, dh_ld, dx_ld, rows;
@@ -75,8 +76,9 @@ struct PackParams {
   long from_ld[2] = {}, to_ld[2] = {}, rows[2] = {};  // elements
   int columns[2] = {};
   long pieces[2] = {};  // rows x to_ld in pieces; 0: none
+  bool kept[2] = {};    // what is kept in 8 bits, restored in the copies' type
 };
-hipError_t launch_pack(const PackParams &p, int size, hipStream_t stream);
+hipError_t launch_pack(const PackParams &p, int type, hipStream_t stream);
 
 // out = epilogue(sum of the splits' parts), which are those of a product of `type`.
 hipError_t launch_gemm_join(const GemmParams &p, int type, int out_type, hipStream_t stream);
@@ -84,7 +86,8 @@ hipError_t launch_gemm_join(const GemmParams &p, int type, int out_type, hipStre
 hipError_t launch_gemm_join_pair(const GemmParams &dx, const GemmParams &dw, int out_type, hipStream_t stream);
 
 struct SlopeParams {
-  const void *dy, *z;
+  const void *dy, *z;  // z in `type`, or kept in 8 bits
+  bool kept;
   void *dz;       // m x dz_ld, columns from n on zero; null: sums alone
   long lo;        // not 0: what dz's rounding left, rounded, that many elements behind
   float *shares;  // ceil(m / rows) x n; null with one share, or without sums
@@ -98,6 +101,10 @@ enum SlopeRows { SLOPE_FEW = 32, SLOPE_MANY = 64, SLOPE_WHOLE = 256 };
 hipError_t launch_act_slope(const SlopeParams &p, const PackParams &pack, int type, hipStream_t stream);
 // out[0..d) = sum of `count` shares, in order, rounded to `type`.
 hipError_t launch_share_sum(const float *shares, long count, int d, void *out, int type, hipStream_t stream);
+
+// Rows into 8 bits in groups (nn_common.hpp) and back.  positive: values above zero keep a code above zero.
+hipError_t launch_keep(const void *x, long ld, long rows, int d, int type, bool positive, void *kept, hipStream_t stream);
+hipError_t launch_restore(const void *kept, long rows, int d, int type, void *x, long ld, hipStream_t stream);
 
 long norm_grad_shares(long rows, long d);
 hipError_t launch_rms_norm(const NormParams &p, int type, int y_type, hipStream_t stream);

@@ -62,7 +62,8 @@ void join(const GemmParams &p, hipStream_t stream) {
 
 // Copies to aligned lines, 16 bytes a thread.  Bound by memory: 7168 x 2107 and 8063 x 2107
 // bfloat16 23 us (64 MB read and written, 5.6 TB/s).
-template <typename T>
+// KEPT: some of it may be kept in 8 bits.
+template <typename T, bool KEPT = false>
 __device__ __forceinline__ void pack_piece(const PackParams &p, long block) {
   constexpr int N = kPiece<T>;
   long id = block * 256 + threadIdx.x;
@@ -71,12 +72,23 @@ __device__ __forceinline__ void pack_piece(const PackParams &p, long block) {
   if (id >= p.pieces[q]) return;
   const long per = p.to_ld[q] / N, row = id / per;
   const int c = static_cast<int>(id % per) * N;
+  if constexpr (KEPT) {
+    if (p.kept[q]) {
+      float u[8];
+      load_kept8(kept_at(p.from[q], p.rows[q], p.columns[q]), row, c, u);
+      typename Vec<T, 8>::type w;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) w[i] = kept_as<T>(u[i]);
+      *reinterpret_cast<typename Vec<T, 8>::type *>(static_cast<T *>(p.to[q]) + row * p.to_ld[q] + c) = w;
+      return;
+    }
+  }
   const i32x4 v = load_piece_any(static_cast<const T *>(p.from[q]) + row * p.from_ld[q], c, p.columns[q]);
   *reinterpret_cast<i32x4 *>(static_cast<T *>(p.to[q]) + row * p.to_ld[q] + c) = v;
 }
-template <typename T>
+template <typename T, bool KEPT>
 __global__ __launch_bounds__(256) void pack_kernel(PackParams p) {
-  pack_piece<T>(p, block_of());
+  pack_piece<T, KEPT>(p, block_of());
 }
 long pack_blocks(const PackParams &p) { return (p.pieces[0] + p.pieces[1] + 255) / 256; }
 
@@ -97,13 +109,14 @@ constexpr float largest = __is_same(T, f16) ? 65504.0f : 0x1.fep127f;  // finite
 // behind (gelu's slope is some 50 instructions an element): 4096 x 8192 bfloat16 gelu 44 us
 // with the sums (201 MB, 4.6 TB/s).  Workgroups of 32 rows where 64 leave CUs idle: 4736 x
 // 141 float16 19.6 us with 64, 8.8 with 32; of all up to 256 rows where that saves the sum's launch.
-template <typename T, int ACT, int CT>
+template <typename T, int ACT, int CT, bool KEPT>
 __global__ __launch_bounds__(256) void act_slope_kernel(SlopeParams p, PackParams pack, int blocks) {
   const long block = block_of();
   if (block >= blocks) {
-    pack_piece<T>(pack, block - blocks);
+    pack_piece<T, KEPT>(pack, block - blocks);
     return;
   }
+  const Kept kept = kept_at(p.z, p.m, p.n);
   constexpr int LANES = 256 / CT, COLS = CT * 8;
   const int column_blocks = (p.n + COLS - 1) / COLS, bc = static_cast<int>(block) % column_blocks, br = static_cast<int>(block) / column_blocks;
   const int c = bc * COLS + threadIdx.x % CT * 8, lane = threadIdx.x / CT, left = p.n - c, rows = p.rows;
@@ -119,7 +132,8 @@ __global__ __launch_bounds__(256) void act_slope_kernel(SlopeParams p, PackParam
       float g[8], z[8];
       load_slope8(static_cast<const T *>(p.dy) + row * p.dy_ld, c, p.n, g);
       if constexpr (ACT != ACT_NONE) {
-        load_slope8(static_cast<const T *>(p.z) + row * p.z_ld, c, p.n, z);
+        if (KEPT && p.kept) load_kept8(kept, row, c, z);
+        else load_slope8(static_cast<const T *>(p.z) + row * p.z_ld, c, p.n, z);
 #pragma unroll
         for (int i = 0; i < 8; ++i) g[i] *= act_slope<ACT>(z[i]);
       }
@@ -161,29 +175,36 @@ __global__ __launch_bounds__(256) void act_slope_kernel(SlopeParams p, PackParam
   else p.shares[static_cast<long>(br) * p.n + at] = v;
 }
 
-template <typename T, int ACT>
+template <typename T, int ACT, bool KEPT>
 void slope(const SlopeParams &p, const PackParams &pack, hipStream_t stream) {
   const int columns = p.rows == SLOPE_WHOLE ? 32 : p.rows == SLOPE_FEW ? 128 : 256;
   const int blocks = (p.m + p.rows - 1) / p.rows * ((p.n + columns - 1) / columns);
   const dim3 grid = grid_of(blocks + pack_blocks(pack), 256);
-  if (p.rows == SLOPE_WHOLE) act_slope_kernel<T, ACT, 4><<<grid, 256, 0, stream>>>(p, pack, blocks);
-  else if (p.rows == SLOPE_FEW) act_slope_kernel<T, ACT, 16><<<grid, 256, 0, stream>>>(p, pack, blocks);
-  else act_slope_kernel<T, ACT, 32><<<grid, 256, 0, stream>>>(p, pack, blocks);
+  if (p.rows == SLOPE_WHOLE) act_slope_kernel<T, ACT, 4, KEPT><<<grid, 256, 0, stream>>>(p, pack, blocks);
+  else if (p.rows == SLOPE_FEW) act_slope_kernel<T, ACT, 16, KEPT><<<grid, 256, 0, stream>>>(p, pack, blocks);
+  else act_slope_kernel<T, ACT, 32, KEPT><<<grid, 256, 0, stream>>>(p, pack, blocks);
 }
 
+template <typename T, bool KEPT>
+void slope(const SlopeParams &p, const PackParams &pack, hipStream_t stream) {
+  if (p.act == ACT_RELU) slope<T, ACT_RELU, KEPT>(p, pack, stream);
+  else if (p.act == ACT_GELU) slope<T, ACT_GELU, KEPT>(p, pack, stream);
+  else if (p.act == ACT_SILU) slope<T, ACT_SILU, KEPT>(p, pack, stream);
+  else slope<T, ACT_NONE, KEPT>(p, pack, stream);
+}
+bool some_kept(const PackParams &p) { return p.kept[0] || p.kept[1]; }
 template <typename T>
 void slope(const SlopeParams &p, const PackParams &pack, hipStream_t stream) {
-  if (p.act == ACT_RELU) slope<T, ACT_RELU>(p, pack, stream);
-  else if (p.act == ACT_GELU) slope<T, ACT_GELU>(p, pack, stream);
-  else if (p.act == ACT_SILU) slope<T, ACT_SILU>(p, pack, stream);
-  else slope<T, ACT_NONE>(p, pack, stream);
+  p.kept || some_kept(pack) ? slope<T, true>(p, pack, stream) : slope<T, false>(p, pack, stream);
 }
 
 }  // namespace
 
-hipError_t launch_pack(const PackParams &p, int size, hipStream_t stream) {
+hipError_t launch_pack(const PackParams &p, int type, hipStream_t stream) {
   const dim3 grid = grid_of(pack_blocks(p), 256);
-  size == 1 ? pack_kernel<f8><<<grid, 256, 0, stream>>>(p) : pack_kernel<bf16><<<grid, 256, 0, stream>>>(p);
+  if (some_kept(p)) type == TYPE_BF16 ? pack_kernel<bf16, true><<<grid, 256, 0, stream>>>(p) : pack_kernel<f16, true><<<grid, 256, 0, stream>>>(p);
+  else if (type == TYPE_F8 || type == TYPE_I8) pack_kernel<f8, false><<<grid, 256, 0, stream>>>(p);
+  else pack_kernel<bf16, false><<<grid, 256, 0, stream>>>(p);
   return hipGetLastError();
 }
 

@@ -245,14 +245,22 @@ __device__ __forceinline__ void store_weight8(const NormGradParams &p, int c, co
     if (c + i < p.d) store_as(p.dw, p.weight_type, c + i, v[i]);
 }
 
+// 8 elements of the norm's input, in T or kept in 8 bits.
+template <bool KEPT, Length L, typename T>
+__device__ __forceinline__ void load_h8(const NormGradParams &p, const Kept &kept, long row, int c, float (&v)[8]) {
+  if constexpr (KEPT) load_kept8(kept, row, c, v);
+  else load8<L>(static_cast<const T *>(p.h) + row * p.h_ld, c, p.d, v);
+}
+
 // The gradient's dx, and this workgroup's rows' share of dw, kept in registers over
 // its rows.  The shares are added by share_sum_kernel, in a fixed order.  Bound by
 // memory: 8192 x 4096 bfloat16 with dh 57 us, 51 and 5 for the sum (268 MB, 5.2 TB/s
 // in the first); 777 x 1111 float32 13 us: a workgroup's load, reduction
 // and stores one after the other 7, the sum's launch 4, the gap between them.
-template <typename T, int NT, int CH, Length L>
+template <typename T, int NT, int CH, Length L, bool KEPT>
 __global__ __launch_bounds__(NT *grad_rows(NT, CH)) void rms_norm_grad_kernel(NormGradParams p) {
   constexpr int RPB = grad_rows(NT, CH), THREADS = NT * RPB;
+  const Kept kept = kept_at(p.h, p.rows, p.d);
   const int t = threadIdx.x % NT, sub = threadIdx.x / NT;
   const NormParams wp{.weight = p.weight, .d = p.d, .weight_type = p.weight_type};
   float w[CH][8], dw[CH][8];
@@ -272,7 +280,7 @@ __global__ __launch_bounds__(NT *grad_rows(NT, CH)) void rms_norm_grad_kernel(No
     float h[CH][8], g[CH][8];
 #pragma unroll
     for (int j = 0; j < CH; ++j)
-      load8<L>(static_cast<const T *>(p.h) + row * p.h_ld, (j * NT + t) * 8, p.d, h[j]);
+      load_h8<KEPT, L, T>(p, kept, row, (j * NT + t) * 8, h[j]);
 #pragma unroll
     for (int j = 0; j < CH; ++j)
       load8<L>(static_cast<const T *>(p.dy) + row * p.dy_ld, (j * NT + t) * 8, p.d, g[j]);
@@ -334,20 +342,20 @@ __global__ __launch_bounds__(NT *grad_rows(NT, CH)) void rms_norm_grad_kernel(No
 // Rows longer than a workgroup's registers hold.  Workgroups own fixed rows; a
 // share of dw is added up in place, in memory, by the threads that own its columns: more
 // bytes than the rows themselves.  4096 x 32768 bfloat16 653 us (1.2 TB/s of the rows' bytes).
-template <typename T>
+template <typename T, bool KEPT>
 __global__ __launch_bounds__(256) void rms_norm_grad_long_kernel(NormGradParams p) {
   constexpr int NT = 256;
+  const Kept kept = kept_at(p.h, p.rows, p.d);
   const NormParams wp{.weight = p.weight, .d = p.d, .weight_type = p.weight_type};
   float *share = p.shares + static_cast<long>(blockIdx.x) * p.d;
   int turn = 0;
   bool first = true;
   for (long row = blockIdx.x; row < p.rows; row += gridDim.x) {
-    const T *hp = static_cast<const T *>(p.h) + row * p.h_ld;
     const T *gp = static_cast<const T *>(p.dy) + row * p.dy_ld;
     float sum = 0.0f, dot = 0.0f;
     for (int c = threadIdx.x * 8; c < p.d; c += NT * 8) {
       float h[8], g[8], w[8];
-      load8<TAIL>(hp, c, p.d, h);
+      load_h8<KEPT, TAIL, T>(p, kept, row, c, h);
       load8<TAIL>(gp, c, p.d, g);
       load_weight8<TAIL>(wp, c, w);
 #pragma unroll
@@ -362,7 +370,7 @@ __global__ __launch_bounds__(256) void rms_norm_grad_long_kernel(NormGradParams 
     const float k = dot * r * r / static_cast<float>(p.d);
     for (int c = threadIdx.x * 8; c < p.d; c += NT * 8) {
       float h[8], g[8], w[8], u[8], s[8];
-      load8<TAIL>(hp, c, p.d, h);
+      load_h8<KEPT, TAIL, T>(p, kept, row, c, h);
       load8<TAIL>(gp, c, p.d, g);
       load_weight8<TAIL>(wp, c, w);
       if (p.dh) load8<TAIL>(static_cast<const T *>(p.dh) + row * p.dh_ld, c, p.d, u);
@@ -419,27 +427,27 @@ void norm_launch(const NormParams &p, hipStream_t stream) {
   else norm_launch_as<T, O, TAIL>(p, stream);
 }
 
-template <typename T, Length L>
+template <typename T, Length L, bool KEPT>
 void norm_grad_launch_as(const NormGradParams &p, dim3 grid, hipStream_t stream) {
   const int n = pieces(p.d);
-  if (n <= 64) rms_norm_grad_kernel<T, 64, 1, L><<<grid, 64 * grad_rows(64, 1), 0, stream>>>(p);
-  else if (n <= 128) rms_norm_grad_kernel<T, 64, 2, L><<<grid, 64 * grad_rows(64, 2), 0, stream>>>(p);
-  else if (n <= 256) rms_norm_grad_kernel<T, 256, 1, L><<<grid, 256 * grad_rows(256, 1), 0, stream>>>(p);
-  else if (n <= 512) rms_norm_grad_kernel<T, 256, 2, L><<<grid, 256 * grad_rows(256, 2), 0, stream>>>(p);
-  else if (n <= 1024) rms_norm_grad_kernel<T, 256, 4, L><<<grid, 256 * grad_rows(256, 4), 0, stream>>>(p);
-  else rms_norm_grad_kernel<T, 256, 8, L><<<grid, 256 * grad_rows(256, 8), 0, stream>>>(p);
+  if (n <= 64) rms_norm_grad_kernel<T, 64, 1, L, KEPT><<<grid, 64 * grad_rows(64, 1), 0, stream>>>(p);
+  else if (n <= 128) rms_norm_grad_kernel<T, 64, 2, L, KEPT><<<grid, 64 * grad_rows(64, 2), 0, stream>>>(p);
+  else if (n <= 256) rms_norm_grad_kernel<T, 256, 1, L, KEPT><<<grid, 256 * grad_rows(256, 1), 0, stream>>>(p);
+  else if (n <= 512) rms_norm_grad_kernel<T, 256, 2, L, KEPT><<<grid, 256 * grad_rows(256, 2), 0, stream>>>(p);
+  else if (n <= 1024) rms_norm_grad_kernel<T, 256, 4, L, KEPT><<<grid, 256 * grad_rows(256, 4), 0, stream>>>(p);
+  else rms_norm_grad_kernel<T, 256, 8, L, KEPT><<<grid, 256 * grad_rows(256, 8), 0, stream>>>(p);
 }
 
-template <typename T>
+template <typename T, bool KEPT>
 hipError_t norm_grad_launch(NormGradParams p, hipStream_t stream) {
   const long shares = norm_grad_shares(p.rows, p.d);
   if (shares == 1 && p.d <= kLongest) p.shares = nullptr;
   const dim3 grid(static_cast<unsigned>(shares));
   if (shares) {
-    if (p.d > kLongest) rms_norm_grad_long_kernel<T><<<grid, 256, 0, stream>>>(p);
-    else if (p.d < 8) rms_norm_grad_kernel<T, 64, 1, ANY><<<grid, 64 * grad_rows(64, 1), 0, stream>>>(p);
-    else if (p.d % 8 == 0) norm_grad_launch_as<T, WHOLE>(p, grid, stream);
-    else norm_grad_launch_as<T, TAIL>(p, grid, stream);
+    if (p.d > kLongest) rms_norm_grad_long_kernel<T, KEPT><<<grid, 256, 0, stream>>>(p);
+    else if (p.d < 8) rms_norm_grad_kernel<T, 64, 1, ANY, KEPT><<<grid, 64 * grad_rows(64, 1), 0, stream>>>(p);
+    else if (p.d % 8 == 0) norm_grad_launch_as<T, WHOLE, KEPT>(p, grid, stream);
+    else norm_grad_launch_as<T, TAIL, KEPT>(p, grid, stream);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || !p.shares) return e;
   }
@@ -481,9 +489,14 @@ hipError_t launch_rms_norm(const NormParams &p, int type, int y_type, hipStream_
   return type == TYPE_BF16 ? norm_launch_to<bf16>(p, y_type, stream) : norm_launch_to<f16>(p, y_type, stream);
 }
 
+template <bool KEPT>
+hipError_t norm_grad_launch_of(const NormGradParams &p, int type, hipStream_t stream) {
+  if (type == TYPE_F32) return norm_grad_launch<float, KEPT>(p, stream);
+  return type == TYPE_BF16 ? norm_grad_launch<bf16, KEPT>(p, stream) : norm_grad_launch<f16, KEPT>(p, stream);
+}
+
 hipError_t launch_rms_norm_grad(const NormGradParams &p, int type, hipStream_t stream) {
-  if (type == TYPE_F32) return norm_grad_launch<float>(p, stream);
-  return type == TYPE_BF16 ? norm_grad_launch<bf16>(p, stream) : norm_grad_launch<f16>(p, stream);
+  return p.kept ? norm_grad_launch_of<true>(p, type, stream) : norm_grad_launch_of<false>(p, type, stream);
 }
 
 }  // namespace tfnn

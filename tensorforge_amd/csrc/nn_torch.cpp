@@ -250,27 +250,88 @@ PyObject *quantize_rows(PyObject *, PyObject *const *a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-// (dy, h, weight, eps, dh) -> (dx, dweight)
+// What rows x d values take in 8 bits, as one contiguous tensor of bytes.
+int64_t kept_bytes(int64_t m, int64_t n) {
+  long long bytes;
+  check(tf_keep8_bytes(m, n, &bytes));
+  return bytes;
+}
+void *kept_rows(const Tensor &t, const char *name, int64_t m, int64_t n) {
+  same_type(t, name, ScalarType::Byte, ScalarType::Byte);
+  const int64_t bytes = kept_bytes(m, n);
+  TORCH_CHECK_VALUE(t.is_contiguous() && t.numel() == bytes, name, ", ", m, " x ", n, " kept in 8 bits, is not ", bytes, " contiguous bytes");
+  return t.data_ptr();
+}
+
+// (x, positive) -> bytes
+PyObject *keep8(PyObject *, PyObject *const *a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  count(n, 2);
+  const Tensor &x = tensor(a[0], "x");
+  float_type(x, "x");
+  no_gradient("keep8", {&x});
+  const Rows r = rows(x, "x");
+  on_gpu(x, {});
+  const On on(x);
+  const Tensor kept = fresh(x, {kept_bytes(r.m, r.n)}, ScalarType::Byte);
+  check(tf_keep8(r.p, r.ld, r.m, r.n, type_of(x.scalar_type()), a[1] == Py_True, kept.data_ptr(), on.stream));
+  return wrap(&kept);
+  END_HANDLE_TH_ERRORS
+}
+
+// (bytes, shape, dtype) -> x
+PyObject *restore8(PyObject *, PyObject *const *a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  count(n, 3);
+  const Tensor &kept = tensor(a[0], "kept");
+  TORCH_CHECK_TYPE(PyTuple_Check(a[1]) && THPDtype_Check(a[2]), "shape is not a tuple, or dtype not a dtype");
+  c10::SmallVector<int64_t, 6> size;
+  int64_t m = 1;
+  const Py_ssize_t dims = PyTuple_GET_SIZE(a[1]);
+  TORCH_CHECK_VALUE(dims > 0, "the shape has no dimension");
+  for (Py_ssize_t i = 0; i < dims; ++i) {
+    const int64_t s = PyLong_AsLongLong(PyTuple_GET_ITEM(a[1], i));
+    if (s == -1 && PyErr_Occurred()) throw python_error();
+    TORCH_CHECK_VALUE(s >= 0 && s <= (1LL << 30) && (i + 1 == dims || s * m <= (1LL << 30)), "the shape's sizes are out of range");
+    size.push_back(s);
+    if (i + 1 < dims) m *= s;
+  }
+  const ScalarType t = reinterpret_cast<THPDtype *>(a[2])->scalar_type;
+  TORCH_CHECK_TYPE(t == ScalarType::Float || half_type(t), "what is kept is Float, BFloat16 or Half, not ", t);
+  const void *p = kept_rows(kept, "kept", m, size.back());
+  on_gpu(kept, {});
+  const On on(kept);
+  const Tensor x = fresh(kept, size, t);
+  check(tf_restore8(p, m, size.back(), type_of(t), x.data_ptr(), size.back(), on.stream));
+  return wrap(&x);
+  END_HANDLE_TH_ERRORS
+}
+
+// (dy, h, weight, eps, dh) -> (dx, dweight); h may be what keep8 gave.
 PyObject *rms_norm_grad(PyObject *, PyObject *const *a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   count(n, 5);
   const Tensor &dy = tensor(a[0], "dy"), &h = tensor(a[1], "h"), &weight = tensor(a[2], "weight");
   const Tensor *dh = optional(a[4], "dh");
-  float_type(h, "h");
+  const bool kept = h.scalar_type() == ScalarType::Byte;
+  if (kept) float_type(dy, "dy");
+  else float_type(h, "h");
   no_gradient("rms_norm_grad", {&dy, &h, &weight, dh});
-  const ScalarType t = h.scalar_type();
-  const Rows hr = rows(h, "h"), gr = rows_of(dy, "dy", hr.m, hr.n, t);
+  const ScalarType t = kept ? dy.scalar_type() : h.scalar_type();
+  Rows hr = rows(kept ? dy : h, "h");
+  const Rows gr = rows_of(dy, "dy", hr.m, hr.n, t);
+  if (kept) hr.p = kept_rows(h, "h", hr.m, hr.n);
   tf_rms_norm_grad_args_t g{};
   g.h = hr.p, g.h_ld = hr.ld, g.rows = hr.m, g.d = hr.n, g.dy = gr.p, g.dy_ld = gr.ld, g.eps = static_cast<float>(number(a[3]));
   g.weight = vector(weight, "weight", hr.n, t, ScalarType::Float);
-  g.type = type_of(t), g.weight_type = type_of(weight.scalar_type());
+  g.type = type_of(t), g.weight_type = type_of(weight.scalar_type()), g.kept = kept ? TF_KEPT_H : 0;
   if (dh) {
     const Rows r = rows_of(*dh, "dh", hr.m, hr.n, t);
     g.dh = r.p, g.dh_ld = r.ld;
   }
   on_gpu(h, {&dy, &weight, dh});
   const On on(h);
-  const Tensor dx = fresh(h, h.sizes(), t), dw = fresh(h, {hr.n}, weight.scalar_type());
+  const Tensor dx = fresh(h, kept ? dy.sizes() : h.sizes(), t), dw = fresh(h, {hr.n}, weight.scalar_type());
   g.dx = dx.data_ptr(), g.dx_ld = hr.n, g.dweight = dw.data_ptr();
   check(tf_rms_norm_grad_workspace(g.rows, g.d, &g.workspace_bytes));
   Tensor space;
@@ -336,17 +397,21 @@ PyObject *linear(PyObject *, PyObject *const *a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-// (dy, x, w, z, act, bias_dtype, want_dx, want_dw, tile, splits, terms) -> (dx, dw, dbias)
+// (dy, x, w, z, act, bias_dtype, want_dx, want_dw, tile, splits, terms) -> (dx, dw, dbias);
+// x and z may be what keep8 gave.
 PyObject *linear_grad(PyObject *, PyObject *const *a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   count(n, 11);
   const Tensor &dy = tensor(a[0], "dy"), &x = tensor(a[1], "x"), &w = tensor(a[2], "w");
   const Tensor *z = optional(a[3], "z");
-  const ScalarType t = x.scalar_type();
-  TORCH_CHECK_TYPE(half_type(t), "x is ", t, ", not BFloat16 or Half");
+  const bool kept = x.scalar_type() == ScalarType::Byte;
+  const ScalarType t = kept ? dy.scalar_type() : x.scalar_type();
+  TORCH_CHECK_TYPE(half_type(t), kept ? "dy is " : "x is ", t, ", not BFloat16 or Half");
   no_gradient("linear_grad", {&dy, &x, &w, z});
   const bool want_dx = a[6] == Py_True, want_dw = a[7] == Py_True;
-  const Rows xr = rows(x, "x");
+  TORCH_CHECK_VALUE(!kept || w.dim() == 2, "w is ", w.sizes(), ", not k x n");
+  Rows xr = kept ? Rows{nullptr, rows(dy, "dy").m, w.size(0), w.size(0)} : rows(x, "x");
+  if (kept) xr.p = kept_rows(x, "x", xr.m, xr.n);
   const Weights wr = weights(w, xr.n, t);
   const Rows gr = rows_of(dy, "dy", xr.m, wr.n, t);
   tf_linear_grad_args_t g{};
@@ -355,9 +420,14 @@ PyObject *linear_grad(PyObject *, PyObject *const *a, Py_ssize_t n) {
   g.tile = integer(a[8], "tile"), g.splits = integer(a[9], "splits"), g.terms = integer(a[10], "terms");
   if (g.act) {
     TORCH_CHECK_VALUE(z, "an activation's gradient needs z: call linear with keep=True");
-    const Rows r = rows_of(*z, "z", xr.m, wr.n, t);
-    g.z = r.p, g.z_ld = r.ld;
+    if (z->scalar_type() == ScalarType::Byte) {
+      g.z = kept_rows(*z, "z", xr.m, wr.n), g.kept = TF_KEPT_Z;
+    } else {
+      const Rows r = rows_of(*z, "z", xr.m, wr.n, t);
+      g.z = r.p, g.z_ld = r.ld;
+    }
   }
+  if (kept) g.kept |= TF_KEPT_X;
   ScalarType bt = t;
   const bool want_db = a[5] != Py_None;
   if (want_db) {
@@ -368,7 +438,7 @@ PyObject *linear_grad(PyObject *, PyObject *const *a, Py_ssize_t n) {
   on_gpu(x, {&dy, &w, z});
   const On on(x);
   Tensor dx, dw, db;
-  if (want_dx) dx = fresh(x, x.sizes(), t), g.dx = dx.data_ptr(), g.dx_ld = xr.n;
+  if (want_dx) dx = fresh(x, kept ? at::IntArrayRef(with_last(dy, xr.n)) : x.sizes(), t), g.dx = dx.data_ptr(), g.dx_ld = xr.n;
   if (want_dw) {
     dw = wr.order ? fresh(x, {wr.n, xr.n}, t).t() : fresh(x, {xr.n, wr.n}, t);
     g.dw = dw.data_ptr(), g.dw_ld = wr.order ? xr.n : wr.n;
@@ -384,6 +454,8 @@ PyObject *linear_grad(PyObject *, PyObject *const *a, Py_ssize_t n) {
 
 PyMethodDef methods[] = {
     {"rms_norm", reinterpret_cast<PyCFunction>(rms_norm), METH_FASTCALL, nullptr},
+    {"keep8", reinterpret_cast<PyCFunction>(keep8), METH_FASTCALL, nullptr},
+    {"restore8", reinterpret_cast<PyCFunction>(restore8), METH_FASTCALL, nullptr},
     {"quantize_rows", reinterpret_cast<PyCFunction>(quantize_rows), METH_FASTCALL, nullptr},
     {"rms_norm_grad", reinterpret_cast<PyCFunction>(rms_norm_grad), METH_FASTCALL, nullptr},
     {"linear", reinterpret_cast<PyCFunction>(linear), METH_FASTCALL, nullptr},

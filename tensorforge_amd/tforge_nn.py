@@ -9,6 +9,8 @@ gradients.
                               quantize_rows(x, torch.int8): integers)
     act(x @ w + b) + r        out = linear(x, w, b, "gelu", r)
     8-bit product             out = linear(q, wq.t(), b, "gelu", r, x_scale=s, w_scale=ws)
+    kept in 8 bits            x8 = keep8(x); x8.restore(); linear(..., keep8=True),
+                              rms_norm(..., keep8=True) for their gradients
     gradients                 dx, dweight = rms_norm_grad(dy, h, weight, dh=...)
                               dx, dw, dbias = linear_grad(dy, x, w, z, "gelu", bias_dtype=...)
 
@@ -20,7 +22,7 @@ dimensions are taken as rows.  Where an input of rms_norm or linear requires a
 gradient, autograd runs the gradient calls, which have no gradient themselves: a
 second derivative raises RuntimeError.  Neither have the 8-bit results: with an input
 that requires a gradient, quantize_rows, rms_norm into 8 bits, 8-bit products and the
-gradient calls raise ValueError unless they run under torch.no_grad().
+gradient calls raise ValueError unless they run under torch.no_grad(); so does keep8.
 
 Bad arguments raise ValueError or TypeError before any work; errors of the
 library raise RuntimeError with its message.
@@ -44,6 +46,51 @@ def _act(activation):
     return code
 
 
+# ---- activations kept in 8 bits -----------------------------------------------------
+
+
+class Kept8:
+    """A tensor of `shape` and `dtype` (float32, bfloat16 or float16) kept in 8 bits, its bytes in `data` (uint8, contiguous).
+
+    32 neighbours of a row of the last dimension share a unit, a power of two, and are integers of -127..127 times it;
+    tf_keep8 in tforge_hip.h describes the bytes.  linear_grad and rms_norm_grad take it as it is.
+    """
+
+    __slots__ = ("data", "shape", "dtype")
+
+    def __init__(self, data, shape, dtype):
+        self.data, self.shape, self.dtype = data, tuple(shape), dtype
+
+    def restore(self):
+        """The tensor, each value within half a unit of what it was."""
+        return _C.restore8(self.data, self.shape, self.dtype)
+
+    def __repr__(self):
+        return f"Kept8({self.shape}, {self.dtype})"
+
+
+def keep8(x, positive=False):
+    """x in 8 bits (Kept8), 33 bytes for 32 values.  positive: values above zero stay above zero, as relu's gradient needs."""
+    return Kept8(_C.keep8(x, True if positive else False), x.shape, x.dtype)
+
+
+def _kept(t, name, like, columns):
+    """What the native layer takes for an operand that may be kept in 8 bits."""
+    if isinstance(t, Kept8):
+        if t.dtype != like.dtype:
+            raise TypeError(f"{name} was {t.dtype}, not {like.dtype}")
+        if not t.shape or t.shape[-1] != columns:
+            raise ValueError(f"{name} was {t.shape}, not rows of {columns}")
+        return t.data
+    if isinstance(t, torch.Tensor) and t.dtype is torch.uint8:
+        raise TypeError(f"{name} is a tensor of bytes: what keep8 gave is passed as it is")
+    return t
+
+
+def _like(dx, x):
+    return dx.view(x.shape) if isinstance(x, Kept8) and dx is not None and dx.shape != x.shape else dx
+
+
 # ---- norm -----------------------------------------------------------------------
 
 
@@ -51,19 +98,20 @@ def _eight_bits(quantize):
     return quantize if isinstance(quantize, torch.dtype) else True if quantize else False
 
 
-def rms_norm(x, weight, residual=None, eps=1e-6, quantize=False):
+def rms_norm(x, weight, residual=None, eps=1e-6, quantize=False, keep8=False):
     """h = x + residual;  y = h / sqrt(mean(h^2) + eps) * weight over the last dimension.
 
     Returns (y, h), h None without a residual; with quantize=True or an 8-bit dtype
     (q, scale, h): y in 8 bits (float8_e4m3fn, or int8) with one scale a row, y ~ q * scale.
-    x is float32, bfloat16 or float16, the weight of x's type or float32.
+    x is float32, bfloat16 or float16, the weight of x's type or float32.  keep8: where the
+    result gets a gradient, h is kept for it in 8 bits (Kept8).
     """
     got = _C.rms_norm(x, weight, residual, eps, _eight_bits(quantize))
     if got is not None:
         return got
     if quantize:
         raise ValueError("the 8-bit output has no gradient: call rms_norm under torch.no_grad(), or on detached tensors")
-    y, h = _RmsNorm.apply(x, weight, residual, eps)
+    y, h = _RmsNorm.apply(x, weight, residual, eps, keep8)
     return y, (None if residual is None else h)
 
 
@@ -76,17 +124,34 @@ def rms_norm_grad(dy, h, weight, eps=1e-6, dh=None):
     """(dx, dweight) of rms_norm from the gradient dy of y and the norm's input h (x + residual).
 
     dh: the gradient that reaches h past the norm, added to dx; dx is the residual's gradient too.
+    h may be kept in 8 bits (Kept8).
     """
-    return _C.rms_norm_grad(dy, h, weight, eps, dh)
+    if isinstance(h, torch.Tensor) and h.dtype is not torch.uint8:
+        return _C.rms_norm_grad(dy, h, weight, eps, dh)
+    dx, dw = _C.rms_norm_grad(dy, _kept(h, "h", dy, dy.shape[-1] if dy.dim() else 0), weight, eps, dh)
+    return _like(dx, h), dw
+
+
+def _saved(t, keep, positive=False):
+    """What autograd saves of t: (t, None), or its bytes and what they stand for."""
+    if t is None or not keep:
+        return t, None
+    kept = keep8(t, positive)
+    return kept.data, (kept.shape, kept.dtype)
+
+
+def _again(t, kept):
+    return t if kept is None else Kept8(t, *kept)
 
 
 class _RmsNorm(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, residual, eps):
+    def forward(ctx, x, weight, residual, eps, keep):
         with torch.no_grad():
             y, h = rms_norm(x, weight, residual, eps)
+            saved, ctx.kept = _saved(x if residual is None else h, keep)
         ctx.eps, ctx.added = eps, None if residual is None else residual.shape
-        ctx.save_for_backward(x if residual is None else h, weight)
+        ctx.save_for_backward(saved, weight)
         ctx.set_materialize_grads(False)
         return y, h
 
@@ -94,21 +159,22 @@ class _RmsNorm(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dy, dh):
         h, weight = ctx.saved_tensors
+        h = _again(h, ctx.kept)
         if dy is None:  # h's alone, past the norm
             dx, dw = dh, None
         else:
             dx, dw = rms_norm_grad(dy.contiguous(), h, weight, ctx.eps, None if dh is None else dh.contiguous())
         if ctx.added is None:
-            return dx, dw, None, None
+            return dx, dw, None, None, None
         # A view would be another tensor on dx's memory, and both could become a leaf's grad.
-        return dx, dw, dx if ctx.added == dx.shape else dx.reshape(ctx.added).clone(), None
+        return dx, dw, dx if ctx.added == dx.shape else dx.reshape(ctx.added).clone(), None, None
 
 
 # ---- products ---------------------------------------------------------------------
 
 
 def linear(x, w, bias=None, activation="none", residual=None, keep=False, x_scale=None, w_scale=None, out_dtype=None,
-           tile=0, splits=0, grad_terms=0):
+           tile=0, splits=0, grad_terms=0, keep8=False):
     """z = x @ w + bias;  out = activation(z) + residual, rounded once.
 
     x (..., k) and w (k, n) are bfloat16 or float16; w may lie row by row or column by
@@ -118,12 +184,14 @@ def linear(x, w, bias=None, activation="none", residual=None, keep=False, x_scal
     "none", "relu", "gelu" (by the normal distribution), "silu".  Returns out, or
     (out, z) with keep=True; both are differentiable.  tile and splits override the choice by sizes
     (tf_linear_args_t in tforge_hip.h); grad_terms is linear_grad's terms under autograd.
+    keep8: where the result gets a gradient, x and the pre-activation are kept for it in
+    8 bits (Kept8), relu's with the sign of every value.
     """
     got = _C.linear(x, w, bias, _act(activation), residual, True if keep else False, x_scale, w_scale, out_dtype, tile,
                     splits)
     if got is not None:
         return got
-    out, z = _Linear.apply(x, w, bias, residual, activation, keep, tile, splits, grad_terms)
+    out, z = _Linear.apply(x, w, bias, residual, activation, keep, tile, splits, grad_terms, keep8)
     return (out, z) if keep else out
 
 
@@ -136,19 +204,27 @@ def linear_grad(dy, x, w, z=None, activation="none", bias_dtype=None, want_dx=Tr
     With gelu and silu the products take dz = dy * activation'(z) rounded to x's type
     (terms=1, an error of sqrt(2) of the results' own rounding) or with what the rounding
     left as a second term (terms=2, twice the time); 0 takes two up to 1.4e8 multiply-adds.
+    x and z may be kept in 8 bits (Kept8).
     """
-    return _C.linear_grad(dy, x, w, z, _act(activation), bias_dtype, True if want_dx else False,
-                          True if want_dw else False, tile, splits, terms)
+    bytes_x, bytes_z = x, z
+    if isinstance(w, torch.Tensor) and w.dim() == 2 and isinstance(dy, torch.Tensor):
+        bytes_x, bytes_z = _kept(x, "x", dy, w.shape[0]), _kept(z, "z", dy, w.shape[1])
+    dx, dw, dbias = _C.linear_grad(dy, bytes_x, w, bytes_z, _act(activation), bias_dtype, True if want_dx else False,
+                                   True if want_dw else False, tile, splits, terms)
+    return _like(dx, x), dw, dbias
 
 
 class _Linear(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, w, bias, residual, activation, keep, tile, splits, terms):
+    def forward(ctx, x, w, bias, residual, activation, keep, tile, splits, terms, keep8):
         smooth = activation != "none"
         with torch.no_grad():
             got = linear(x, w, bias, activation, residual, keep=keep or smooth, tile=tile, splits=splits)
-        out, z = got if keep or smooth else (got, None)
-        ctx.save_for_backward(x, w, z if smooth else None)
+            out, z = got if keep or smooth else (got, None)
+            saved_x, kept_x = _saved(x, keep8)
+            saved_z, kept_z = _saved(z if smooth else None, keep8, activation == "relu")
+        ctx.save_for_backward(saved_x, w, saved_z)
+        ctx.kept = kept_x, kept_z
         ctx.how = activation, None if bias is None else bias.dtype, tile, splits, terms
         ctx.added = None if residual is None else residual.shape
         ctx.set_materialize_grads(False)
@@ -158,6 +234,7 @@ class _Linear(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dy, dz):
         x, w, z = ctx.saved_tensors
+        x, z = _again(x, ctx.kept[0]), _again(z, ctx.kept[1])
         activation, bias_dtype, tile, splits, terms = ctx.how
         need = ctx.needs_input_grad
 
@@ -169,4 +246,5 @@ class _Linear(torch.autograd.Function):
         got = [] if dy is None else [grads(dy, z, activation)]
         got += [] if dz is None else [grads(dz, None, "none")]
         total = (None, None, None) if not got else got[0] if len(got) == 1 else [a if a is None else a + b for a, b in zip(*got)]
-        return (*total, dy.reshape(ctx.added) if need[3] and dy is not None else None, None, None, None, None, None)
+        return (*total, dy.reshape(ctx.added) if need[3] and dy is not None else None, None, None, None, None, None,
+                None)

@@ -86,3 +86,92 @@ for m, n, k in ((1, big, 1), (big, 1, 16), (64, big, 64), (1 << 20, 1 << 16, 5),
 for rows, d in ((1 << 24, 4), (big, 1), (big, 0), (1 << 22, 20000)):
     assert norm(d, rows, 256, 4) == 0 and lib.tf_quantize_rows_to(256, d, rows, d, 1, 256, d, 4, 256, None) == 0
 """)
+
+
+# ---- kept in 8 bits -------------------------------------------------------------
+
+
+def test_keep8_refusals():
+    lib, n = _lib.lib(), ctypes.c_longlong()
+    for rows, d, bytes_ in ((0, 5, 0), (5, 0, 0), (3, 1, 99), (3, 32, 99), (3, 33, 198), (1 << 30, 1 << 30, (1 << 55) * 33)):
+        assert lib.tf_keep8_bytes(rows, d, ctypes.byref(n)) == 0 and n.value == bytes_
+    _refused(lib.tf_keep8_bytes(-1, 5, ctypes.byref(n)), "rows = -1")
+    _refused(lib.tf_keep8_bytes(1, (1 << 30) + 1, ctypes.byref(n)), "d = 1073741825")
+    _refused(lib.tf_keep8_bytes(1, 1, None), "null")
+    _refused(lib.tf_keep8(256, 64, 4, 64, 3, 0, 256, None), "type = 3")
+    _refused(lib.tf_keep8(256, 63, 4, 64, 1, 0, 256, None), "x: 63 elements")
+    _refused(lib.tf_keep8(257, 64, 4, 64, 1, 0, 256, None), "x is not aligned")
+    _refused(lib.tf_keep8(256, 64, 4, 64, 1, 2, 256, None), "positive = 2")
+    _refused(lib.tf_keep8(256, 64, 4, 64, 1, 0, 264, None), "kept, kept in 8 bits, is not 16-byte aligned")
+    _refused(lib.tf_keep8(256, 64, 4, 64, 1, 0, None, None), "kept is a null pointer")
+    _refused(lib.tf_restore8(256, 4, 64, 4, 256, 64, None), "type = 4")
+    _refused(lib.tf_restore8(256, 4, 64, 1, 256, 32, None), "x: 32 elements")
+    _refused(lib.tf_restore8(None, 4, 64, 1, 256, 64, None), "kept is a null pointer")
+    assert lib.tf_keep8(None, 0, 0, 64, 1, 0, None, None) == lib.tf_restore8(None, 4, 0, 1, None, 0, None) == 0
+    base = dict(dy=256, x=256, w=256, z=256, dx=256, dw=256, workspace=256, workspace_bytes=1 << 30, dy_ld=32, w_ld=32, dx_ld=64,
+                dw_ld=32, m=8, n=32, k=64, type=1, bias_type=1, act=2)
+    for change, words in ((dict(kept=4), "kept = 4"), (dict(kept=3, x=264), "x, kept in 8 bits"), (dict(kept=3, z=0), "z is a null pointer"),
+                          (dict(kept=1), "z: 0 elements"), (dict(kept=2), "x: 0 elements"), (dict(kept=3, workspace_bytes=16), "are needed")):
+        _refused(lib.tf_linear_grad(ctypes.byref(_lib.LinearGradArgs(**{**base, **change})), None), words)
+    a = dict(dy=256, h=256, weight=256, dx=256, dweight=256, dy_ld=64, dx_ld=64, rows=4, d=64, type=1, weight_type=1, workspace=256,
+             workspace_bytes=1 << 20)
+    for change, words in ((dict(kept=2), "kept = 2"), (dict(kept=1, h=264), "h, kept in 8 bits"), (dict(kept=0), "h: 0 elements")):
+        _refused(lib.tf_rms_norm_grad(ctypes.byref(_lib.RmsNormGradArgs(**{**a, **change})), None), words)
+
+
+def test_kept_python_refusals():
+    h, w, v = (torch.zeros(n, dtype=torch.bfloat16) for n in ((4, 40), (40, 16), (40,)))
+    dy, half = torch.zeros(4, 16, dtype=torch.bfloat16), torch.zeros(4, 16, dtype=torch.float16)
+    kept = lambda m, n, t=torch.bfloat16, more=0: nn.Kept8(torch.zeros(m * (-(-n // 32)) * 33 + more, dtype=torch.uint8), (m, n), t)  # noqa: E731
+    for call, error, words in [
+            (lambda: nn.keep8(h), ValueError, "not on a GPU"),
+            (lambda: nn.keep8(h.int()), TypeError, "x is Int"),
+            (lambda: nn.keep8(h.t()), ValueError, "next to each other"),
+            (lambda: nn.keep8(h.clone().requires_grad_()), ValueError, "no gradient"),
+            (lambda: kept(4, 40).restore(), ValueError, "not on a GPU"),
+            (lambda: kept(4, 40, more=1).restore(), ValueError, "is not 264 contiguous bytes"),
+            (lambda: nn.Kept8(kept(4, 40).data, (4, 40), torch.int8).restore(), TypeError, "not Char"),
+            (lambda: nn.Kept8(kept(4, 40).data.char(), (4, 40), torch.bfloat16).restore(), TypeError, "kept is Char"),
+            (lambda: nn.Kept8(kept(4, 40).data, (-4, 40), torch.bfloat16).restore(), ValueError, "out of range"),
+            (lambda: nn.Kept8(kept(4, 40).data, (), torch.bfloat16).restore(), ValueError, "no dimension"),
+            (lambda: nn.linear_grad(dy, kept(4, 40), w), ValueError, "not on a GPU"),
+            (lambda: nn.linear_grad(dy, kept(4, 39), w), ValueError, "not rows of 40"),
+            (lambda: nn.linear_grad(dy, kept(5, 40), w), ValueError, "x, 4 x 40 kept in 8 bits"),
+            (lambda: nn.linear_grad(dy, kept(4, 40, torch.float16), w), TypeError, "x was torch.float16"),
+            (lambda: nn.linear_grad(half, kept(4, 40), w), TypeError, "x was torch.bfloat16"),
+            (lambda: nn.linear_grad(dy, kept(4, 40).data, w), TypeError, "a tensor of bytes"),
+            (lambda: nn.linear_grad(dy, h, w, kept(4, 17), "gelu"), ValueError, "not rows of 16"),
+            (lambda: nn.linear_grad(dy, kept(4, 40), w, None, "gelu"), ValueError, "keep=True"),
+            (lambda: nn.linear_grad(dy, kept(4, 40), w[0]), TypeError, "x is not a tensor"),
+            (lambda: nn.linear_grad(dy, kept(4, 40), w.clone().requires_grad_()), ValueError, "no gradient"),
+            (lambda: nn.rms_norm_grad(h, kept(4, 40), v), ValueError, "not on a GPU"),
+            (lambda: nn.rms_norm_grad(h, kept(4, 33), v), ValueError, "not rows of 40"),
+            (lambda: nn.rms_norm_grad(h, kept(3, 40), v), ValueError, "kept in 8 bits"),
+            (lambda: nn.rms_norm_grad(h.half(), kept(4, 40), v.half()), TypeError, "h was torch.bfloat16"),
+            (lambda: nn.rms_norm_grad(h, kept(4, 40).data, v), TypeError, "a tensor of bytes")]:
+        with pytest.raises(error, match=words):
+            call()
+
+
+def test_keeping_extreme_sizes_launches(without_gpu):  # noqa: F811
+    without_gpu("""
+big = 1 << 30
+for rows, d in ((1, big), (big, 1), (big, 33), (1 << 22, 20000), (1 << 15, big)):
+    for ld in (d, d + 8):
+        assert lib.tf_keep8(256, ld, rows, d, 1, 0, 256, None) == 0 and lib.tf_restore8(256, rows, d, 1, 256, ld, None) == 0, (rows, d)
+    if rows * d < 1 << 40:
+        a = _lib.RmsNormGradArgs(dy=256, h=256, weight=256, dx=256, dweight=256, dy_ld=d, dx_ld=d, rows=rows, d=d, type=1, weight_type=1,
+                                 workspace=256, workspace_bytes=1 << 60, kept=1)
+        assert lib.tf_rms_norm_grad(ref(a), None) == 0
+def grad8(m, n, k, order, act):
+    a = _lib.LinearGradArgs(dy=256, x=256, w=256, z=256, dx=256, dw=256, dbias=256, workspace=256, dy_ld=n, w_ld=k if order else n,
+                            dx_ld=k, dw_ld=k if order else n, m=m, n=n, k=k, w_order=order, type=1, bias_type=1, act=act, kept=3)
+    size = ctypes.c_longlong()
+    assert lib.tf_linear_grad_workspace(ref(a), ref(size)) == 0
+    a.workspace_bytes = size.value
+    return lib.tf_linear_grad(ref(a), None)
+for m, n, k in ((1, 1 << 26, 8), (64, big, 64), (big, 9, 8), (big, 1, 1), (1, 1, big), (64, 8, 1 << 27), (4096, 8, 1 << 22)):
+    for order in (0, 1):
+        for act in (0, 1, 2):
+            assert grad8(m, n, k, order, act) == 0, (m, n, k, order, act)
+""")
