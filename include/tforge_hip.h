@@ -25,7 +25,8 @@
  * Beside compiled programs the library has the operators of the residual MLP
  * block in 16 and 8 bits, for training and serving (no counterpart in the
  * reference): tf_rms_norm, tf_quantize_rows, tf_linear and the gradients
- * tf_rms_norm_grad and tf_linear_grad, at the end of this file.
+ * tf_rms_norm_grad and tf_linear_grad, what keeps activations in 8 bits for these
+ * (tf_keep8), and the loss over a vocabulary (tf_linear_xent), at the end of this file.
  */
 #ifndef TFORGE_HIP_H
 #define TFORGE_HIP_H
@@ -421,6 +422,60 @@ typedef struct {
 /* As tf_linear_workspace; which of dx, dw and dbias are wanted counts too. */
 int tf_linear_grad_workspace(const tf_linear_grad_args_t *args, long long *bytes);
 int tf_linear_grad(const tf_linear_grad_args_t *args, void *stream);
+
+/* The cross entropy of logits z = x @ w that are never in memory as a whole:
+ *   lse[m] = log(sum over n of exp(z[m][n])),  loss[m] = lse[m] - z[m][target[m]]
+ * w as tf_linear's.  A row whose target is `ignore` does not count: its loss is 0.  A
+ * target outside of 0..n-1 otherwise gives NaN.  Sums over k, logits, exponentials and
+ * their sums are float32; infinities and NaN follow the formulas. */
+typedef struct {
+  const void *x, *w;       /* m x k, k x n in either order                          */
+  const long long *target; /* m                                                     */
+  float *loss, *lse;       /* m                                                     */
+  float *sum, *mean, *count; /* one float each, or NULL: of the losses of the rows that
+                              count, and their number; a mean of no rows is 0       */
+  void *workspace;         /* 16-byte aligned, tf_linear_xent_workspace's bytes     */
+  long long workspace_bytes;
+  long long x_ld, w_ld;
+  long long m, n, k;       /* n >= 1                                                */
+  long long ignore;
+  int w_order, type;       /* type: TF_T_BF16, TF_T_F16                             */
+} tf_linear_xent_args_t;
+/* Bytes of workspace for these arguments, as tf_linear_workspace: 8 for each row and
+ * tile of columns, and aligned copies of odd operands. */
+int tf_linear_xent_workspace(const tf_linear_xent_args_t *args, long long *bytes);
+int tf_linear_xent(const tf_linear_xent_args_t *args, void *stream);
+
+/* Its gradient, from the dloss of every row (or one for all) and the kept lse:
+ *   dz[m][n] = (exp(z[m][n] - lse[m]) - [n == target[m]]) * dloss[m] / count
+ *   dx = dz @ w^T,  dw = x^T @ dz in w's memory order
+ * The logits are computed again, for a piece of the vocabulary at a time, and the
+ * products take dz in `type`, rounded once: one dloss for all rows is multiplied into
+ * their sums instead, and float16 has a unit that lets the largest dz reach 2^15.
+ * Sums are float32, over the pieces too.  A row that does not count
+ * has a dz of zeros whatever its x holds (dw is the product all the same: an x that is
+ * not finite gives NaN there). */
+typedef struct {
+  const void *x, *w;
+  const long long *target;
+  const float *lse;        /* m                                                     */
+  const float *dloss;      /* m with dloss_rows, else one                           */
+  const float *count;      /* one float, or NULL for 1: the mean's gradient takes
+                              tf_linear_xent's count                                */
+  void *dx, *dw;           /* each may be NULL: not wanted                          */
+  void *workspace;         /* 16-byte aligned, tf_linear_xent_grad_workspace's bytes */
+  long long workspace_bytes;
+  long long x_ld, w_ld, dx_ld, dw_ld;
+  long long m, n, k;
+  long long ignore;
+  int w_order, type;
+  int dloss_rows;          /* 0 or 1                                                */
+  int reserved;            /* 0                                                     */
+} tf_linear_xent_grad_args_t;
+/* A piece's dz of up to 512 MB (or 16384 columns), float32 sums of dx where there is
+ * more than one piece, parts of split products, aligned copies. */
+int tf_linear_xent_grad_workspace(const tf_linear_xent_grad_args_t *args, long long *bytes);
+int tf_linear_xent_grad(const tf_linear_xent_grad_args_t *args, void *stream);
 
 #ifdef __cplusplus
 }

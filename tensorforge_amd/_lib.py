@@ -78,6 +78,18 @@ class LinearGradArgs(ctypes.Structure):
                [(f, ctypes.c_int) for f in ("w_order", "type", "bias_type", "act", "tile", "splits", "terms", "kept")]
 
 
+class LinearXentArgs(ctypes.Structure):
+    _fields_ = [(f, ctypes.c_void_p) for f in ("x", "w", "target", "loss", "lse", "sum", "mean", "count", "workspace")] + \
+               [(f, ctypes.c_longlong) for f in ("workspace_bytes", "x_ld", "w_ld", "m", "n", "k", "ignore")] + \
+               [(f, ctypes.c_int) for f in ("w_order", "type")]
+
+
+class LinearXentGradArgs(ctypes.Structure):
+    _fields_ = [(f, ctypes.c_void_p) for f in ("x", "w", "target", "lse", "dloss", "count", "dx", "dw", "workspace")] + \
+               [(f, ctypes.c_longlong) for f in ("workspace_bytes", "x_ld", "w_ld", "dx_ld", "dw_ld", "m", "n", "k", "ignore")] + \
+               [(f, ctypes.c_int) for f in ("w_order", "type", "dloss_rows", "reserved")]
+
+
 # (name, restype, argtypes) of every exported function, in header order.
 P, I, LL, U = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_uint
 SIGNATURES = [
@@ -117,6 +129,10 @@ SIGNATURES = [
     ("tf_linear", I, [P, P]),
     ("tf_linear_grad_workspace", I, [P, ctypes.POINTER(LL)]),
     ("tf_linear_grad", I, [P, P]),
+    ("tf_linear_xent_workspace", I, [P, ctypes.POINTER(LL)]),
+    ("tf_linear_xent", I, [P, P]),
+    ("tf_linear_xent_grad_workspace", I, [P, ctypes.POINTER(LL)]),
+    ("tf_linear_xent_grad", I, [P, P]),
 ]
 
 _lib = None

@@ -507,8 +507,13 @@ template <int BM, int BN, int ST>
 constexpr int tile_lds() {
   return ST * (BM + BN) * 128;
 }
-template <typename T, typename O, bool AMN, bool BMN, int BM, int BN, int WM, int WN, int ST, bool DMA, int TERMS>
-__device__ __forceinline__ void gemm_tile(const GemmParams &p, int block, int blocks, lds_char *lds) {
+//
+// E: what becomes of the sums; Results writes them with bias, activation and residual.
+struct Results {
+  typedef GemmParams Params;
+};
+template <typename T, typename O, bool AMN, bool BMN, int BM, int BN, int WM, int WN, int ST, bool DMA, int TERMS, typename E = Results>
+__device__ __forceinline__ void gemm_tile(const typename E::Params &p, int block, int blocks, lds_char *lds) {
   constexpr int NW = WM * WN, MI = BM / WM / 16, NI = BN / WN / 16, STAGE = (BM + BN) * 128;
   const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(lds));
   int tm, tn, split;
@@ -634,17 +639,21 @@ __device__ __forceinline__ void gemm_tile(const GemmParams &p, int block, int bl
   constexpr int COLS = BN / WN, ROWS = BM / WM / ((BM / WM) * COLS > 4096 ? 2 : 1);  // 16 KiB a wave at most
   static_assert(NW * ROWS * COLS * 4 <= (DMA ? ST : 2) * STAGE, "the patches fit into the slabs' LDS");
   lds_char *patch = lds + wave * (ROWS * COLS * 4);
-  const int lane = threadIdx.x % 64;
+  if constexpr (__is_same(E, Results)) {
+    const int lane = threadIdx.x % 64;
 #pragma unroll
-  for (int h = 0; h < BM / WM / ROWS; ++h) {
+    for (int h = 0; h < BM / WM / ROWS; ++h) {
 #pragma unroll
-    for (int i = 0; i < ROWS / 16; ++i)
+      for (int i = 0; i < ROWS / 16; ++i)
 #pragma unroll
-      for (int j = 0; j < NI; ++j)
-        *reinterpret_cast<__attribute__((address_space(3))) sums4<T> *>(
-            patch + patch_at<COLS>(i * 16 + lane % 16, j * 4 + lane / 16)) = acc[h * (ROWS / 16) + i][j];
-    wait_lds();
-    write_patch<T, O, ROWS, COLS>(p, split, patch, m0 + wm * (BM / WM) + h * ROWS, n0 + wn * COLS, tm * BM, tn * BN);
+        for (int j = 0; j < NI; ++j)
+          *reinterpret_cast<__attribute__((address_space(3))) sums4<T> *>(
+              patch + patch_at<COLS>(i * 16 + lane % 16, j * 4 + lane / 16)) = acc[h * (ROWS / 16) + i][j];
+      wait_lds();
+      write_patch<T, O, ROWS, COLS>(p, split, patch, m0 + wm * (BM / WM) + h * ROWS, n0 + wn * COLS, tm * BM, tn * BN);
+    }
+  } else {
+    E::template finish<T, BM, BN, WM, WN, ROWS>(p, acc, split, lds, patch, m0, n0, wm, wn, tm, tn);
   }
 }
 

@@ -69,6 +69,32 @@ struct ShareParams {
 hipError_t launch_gemm_pair_bf16(const GemmParams &dx, bool bmn, const GemmParams &dw, const ShareParams &sum, hipStream_t stream);
 hipError_t launch_gemm_pair_f16(const GemmParams &dx, bool bmn, const GemmParams &dw, const ShareParams &sum, hipStream_t stream);
 
+// The products of the loss over a vocabulary and of its gradient.  The loss of row m is
+// lse[m] - logit(m, target[m]); a row whose target is `ignore` does not count, one whose
+// target is outside of the vocabulary is NaN.
+struct XentParams : GemmParams {
+  const long long *target = nullptr;
+  long long ignore = 0;
+  int vocabulary = 0, column0 = 0;  // all columns, and this piece's first
+  // XENT_STATS: of each row the largest logit of a tile's columns and the sum of exp(logit - largest), tiles_n x m
+  // pairs; and the target's logit.
+  float *stats = nullptr, *target_logit = nullptr;
+  // XENT_SLOPE: out = (exp(logit - lse) - [column is the target]) * unit, zeros up to a multiple of 8 columns.  One dloss
+  // for all rows: the unit is `power`, and dloss / count / power comes with XENT_SUM.  A row's own: dloss / count, in
+  // float16 times scale[0].
+  const float *lse = nullptr, *dloss = nullptr, *count = nullptr, *scale = nullptr;
+  float power = 1.0f;
+  int dloss_rows = 0;
+  // XENT_SUM: out = (product + sum) * dloss / count / power (scale[1] or 1 with a dloss a row), or the new sum; m x (n up to a
+  // multiple of 4) floats.
+  float *sum = nullptr;
+  int add = 0, last = 0;
+};
+enum XentProduct { XENT_STATS, XENT_SLOPE, XENT_SUM };
+// Tiles 256, 128 and 64.  XENT_STATS and XENT_SLOPE: amn false.
+hipError_t launch_xent_bf16(const XentParams &p, XentProduct what, bool amn, bool bmn, int tile, bool dma, hipStream_t stream);
+hipError_t launch_xent_f16(const XentParams &p, XentProduct what, bool amn, bool bmn, int tile, bool dma, hipStream_t stream);
+
 // Up to two matrices copied to rows of whole 16-byte pieces, zeros in the pad.
 struct PackParams {
   const void *from[2] = {};

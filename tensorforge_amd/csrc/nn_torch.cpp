@@ -452,8 +452,97 @@ PyObject *linear_grad(PyObject *, PyObject *const *a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// The targets of x's rows.
+const long long *targets(const Tensor &t, const Tensor &x) {
+  static_assert(sizeof(long long) == sizeof(int64_t), "targets are 64-bit");
+  same_type(t, "target", ScalarType::Long, ScalarType::Long);
+  TORCH_CHECK_VALUE(t.sizes() == x.sizes().slice(0, x.dim() - 1) && t.is_contiguous(), "target is not a contiguous tensor of ",
+                    x.sizes().slice(0, x.dim() - 1));
+  return reinterpret_cast<const long long *>(t.data_ptr<int64_t>());
+}
+
+long long integer64(PyObject *o) {
+  const long long v = PyLong_AsLongLong(o);
+  if (v == -1 && PyErr_Occurred()) throw python_error();
+  return v;
+}
+
+// (x, w, target, ignore, reduction) -> (loss, lse, count); reduction: 0 none, 1 sum, 2 mean
+PyObject *linear_xent(PyObject *, PyObject *const *a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  count(n, 5);
+  const Tensor &x = tensor(a[0], "x"), &w = tensor(a[1], "w"), &target = tensor(a[2], "target");
+  const ScalarType t = x.scalar_type();
+  TORCH_CHECK_TYPE(half_type(t), "x is ", t, ", not BFloat16 or Half");
+  const Rows xr = rows(x, "x");
+  const Weights wr = weights(w, xr.n, t);
+  tf_linear_xent_args_t g{};
+  g.target = targets(target, x);
+  const int reduction = integer(a[4], "reduction");
+  if (wants_grad({&x, &w})) Py_RETURN_NONE;
+  g.x = xr.p, g.x_ld = xr.ld, g.m = xr.m, g.k = xr.n, g.w = wr.p, g.w_ld = wr.ld, g.n = wr.n, g.w_order = wr.order;
+  g.type = type_of(t), g.ignore = integer64(a[3]);
+  on_gpu(x, {&w, &target});
+  const On on(x);
+  const at::IntArrayRef shape = x.sizes().slice(0, x.dim() - 1);
+  Tensor loss = fresh(x, shape, ScalarType::Float), lse = fresh(x, shape, ScalarType::Float), space, one, number;
+  g.loss = loss.data_ptr<float>(), g.lse = lse.data_ptr<float>();
+  if (reduction) one = fresh(x, {}, ScalarType::Float), (reduction == 1 ? g.sum : g.mean) = one.data_ptr<float>();
+  if (reduction == 2) number = fresh(x, {}, ScalarType::Float), g.count = number.data_ptr<float>();
+  check(tf_linear_xent_workspace(&g, &g.workspace_bytes));
+  if (g.workspace_bytes) space = fresh(x, {static_cast<int64_t>(g.workspace_bytes)}, ScalarType::Byte), g.workspace = space.data_ptr();
+  check(tf_linear_xent(&g, on.stream));
+  return tuple({reduction ? &one : &loss, &lse, reduction == 2 ? &number : nullptr});
+  END_HANDLE_TH_ERRORS
+}
+
+// (dloss, x, w, target, lse, count, ignore, want_dx, want_dw) -> (dx, dw)
+PyObject *linear_xent_grad(PyObject *, PyObject *const *a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  count(n, 9);
+  const Tensor &dloss = tensor(a[0], "dloss"), &x = tensor(a[1], "x"), &w = tensor(a[2], "w"), &target = tensor(a[3], "target");
+  const Tensor &lse = tensor(a[4], "lse"), *number = optional(a[5], "count");
+  const ScalarType t = x.scalar_type();
+  TORCH_CHECK_TYPE(half_type(t), "x is ", t, ", not BFloat16 or Half");
+  no_gradient("linear_cross_entropy_grad", {&dloss, &x, &w, &lse, number});
+  const bool want_dx = a[7] == Py_True, want_dw = a[8] == Py_True;
+  const Rows xr = rows(x, "x");
+  const Weights wr = weights(w, xr.n, t);
+  tf_linear_xent_grad_args_t g{};
+  g.target = targets(target, x);
+  const at::IntArrayRef shape = x.sizes().slice(0, x.dim() - 1);
+  same_type(lse, "lse", ScalarType::Float, ScalarType::Float);
+  TORCH_CHECK_VALUE(lse.sizes() == shape && lse.is_contiguous(), "lse is not a contiguous tensor of ", shape);
+  same_type(dloss, "dloss", ScalarType::Float, ScalarType::Float);
+  g.dloss_rows = dloss.dim() != 0 || shape.empty();
+  TORCH_CHECK_VALUE(dloss.dim() == 0 || (dloss.sizes() == shape && dloss.is_contiguous()), "dloss is not one number or a contiguous tensor of ", shape);
+  if (number) {
+    same_type(*number, "count", ScalarType::Float, ScalarType::Float);
+    TORCH_CHECK_VALUE(number->numel() == 1, "count is not one number");
+    g.count = number->data_ptr<float>();
+  }
+  g.lse = lse.data_ptr<float>(), g.dloss = dloss.data_ptr<float>();
+  g.x = xr.p, g.x_ld = xr.ld, g.m = xr.m, g.k = xr.n, g.w = wr.p, g.w_ld = wr.ld, g.n = wr.n, g.w_order = wr.order;
+  g.type = type_of(t), g.ignore = integer64(a[6]);
+  on_gpu(x, {&w, &target, &lse, &dloss, number});
+  const On on(x);
+  Tensor dx, dw, space;
+  if (want_dx) dx = fresh(x, x.sizes(), t), g.dx = dx.data_ptr(), g.dx_ld = xr.n;
+  if (want_dw) {
+    dw = wr.order ? fresh(x, {wr.n, xr.n}, t).t() : fresh(x, {xr.n, wr.n}, t);
+    g.dw = dw.data_ptr(), g.dw_ld = wr.order ? xr.n : wr.n;
+  }
+  check(tf_linear_xent_grad_workspace(&g, &g.workspace_bytes));
+  if (g.workspace_bytes) space = fresh(x, {static_cast<int64_t>(g.workspace_bytes)}, ScalarType::Byte), g.workspace = space.data_ptr();
+  check(tf_linear_xent_grad(&g, on.stream));
+  return tuple({want_dx ? &dx : nullptr, want_dw ? &dw : nullptr});
+  END_HANDLE_TH_ERRORS
+}
+
 PyMethodDef methods[] = {
     {"rms_norm", reinterpret_cast<PyCFunction>(rms_norm), METH_FASTCALL, nullptr},
+    {"linear_xent", reinterpret_cast<PyCFunction>(linear_xent), METH_FASTCALL, nullptr},
+    {"linear_xent_grad", reinterpret_cast<PyCFunction>(linear_xent_grad), METH_FASTCALL, nullptr},
     {"keep8", reinterpret_cast<PyCFunction>(keep8), METH_FASTCALL, nullptr},
     {"restore8", reinterpret_cast<PyCFunction>(restore8), METH_FASTCALL, nullptr},
     {"quantize_rows", reinterpret_cast<PyCFunction>(quantize_rows), METH_FASTCALL, nullptr},

@@ -85,11 +85,10 @@ struct WideLoader {
   }
 };
 
-template <typename T, typename O, bool AMN, bool BMN>
-__global__ __launch_bounds__(512, 2) void gemm_wide_kernel(GemmParams p) {
+constexpr int kWideLds = 2 * 2 * 256 * 128;
+template <typename T, typename O, bool AMN, bool BMN, typename E = Results>
+__device__ __forceinline__ void gemm_wide(const typename E::Params &p, lds_char *lds) {
   constexpr int STAGE = 2 * 256 * 128, HALF = 256 * 128;
-  __shared__ __align__(1024) char smem[2 * STAGE];
-  lds_char *lds = (lds_char *)smem;
   const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(lds));
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), wm = wave / 4, wn = wave % 4;
   int tm, tn, split;
@@ -183,19 +182,29 @@ __global__ __launch_bounds__(512, 2) void gemm_wide_kernel(GemmParams p) {
   barrier();
   // Through LDS (nn_gemm.hpp), 64 rows at a time.  Results of this size stream past
   // the caches: 8192^3 in bfloat16 1389 TFLOP/s without that, 1423 with it.
-  const int lane = threadIdx.x % 64;
   lds_char *patch = lds + wave * (64 * 64 * 4);
+  if constexpr (__is_same(E, Results)) {
+    const int lane = threadIdx.x % 64;
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
+    for (int h = 0; h < 2; ++h) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+      for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        *reinterpret_cast<__attribute__((address_space(3))) sums4<T> *>(patch + patch_at<64>(i * 16 + lane % 16, j * 4 + lane / 16)) =
-            acc[4 * h + i][j];
-    wait_lds();
-    write_patch<T, O, 64, 64, true>(p, split, patch, tm * 256 + wm * 128 + h * 64, tn * 256 + wn * 64, 0, 0);
+        for (int j = 0; j < 4; ++j)
+          *reinterpret_cast<__attribute__((address_space(3))) sums4<T> *>(patch + patch_at<64>(i * 16 + lane % 16, j * 4 + lane / 16)) =
+              acc[4 * h + i][j];
+      wait_lds();
+      write_patch<T, O, 64, 64, true>(p, split, patch, tm * 256 + wm * 128 + h * 64, tn * 256 + wn * 64, 0, 0);
+    }
+  } else {
+    E::template finish<T, 256, 256, 2, 4, 64>(p, acc, split, lds, patch, tm * 256, tn * 256, wm, wn, tm, tn);
   }
+}
+
+template <typename T, typename O, bool AMN, bool BMN>
+__global__ __launch_bounds__(512, 2) void gemm_wide_kernel(GemmParams p) {
+  __shared__ __align__(1024) char smem[kWideLds];
+  gemm_wide<T, O, AMN, BMN>(p, (lds_char *)smem);
 }
 
 }  // namespace tfnn

@@ -1,0 +1,242 @@
+// The products of the loss over a vocabulary: nn_gemm.hpp's and nn_wide.hpp's tiles with
+// epilogues of their own.  The logits stay in the accumulators; what leaves a tile is two floats a
+// row (the loss), or the logits' gradient in 16 bits (for one piece of the vocabulary).
+#pragma once
+
+#include "nn_gemm.hpp"
+#include "nn_wide.hpp"
+
+namespace tfnn {
+
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+
+// A lane holds of each 16 x 16 block the row lane % 16 and four columns from lane / 16 * 4.
+
+// The blocks reach memory by rows through the wave's patch of LDS (nn_gemm.hpp), ROWS at a
+// time: put(row, column, eight values), both from the wave's first.
+template <int ROWS, int MI, int NI, typename F>
+__device__ __forceinline__ void by_rows(const f32x4 (&acc)[MI][NI], lds_char *patch, F &&put) {
+  constexpr int COLS = NI * 16, LANES = COLS / 8;
+  const int lane = threadIdx.x % 64, c = lane % LANES;
+#pragma unroll
+  for (int h = 0; h < MI * 16 / ROWS; ++h) {
+#pragma unroll
+    for (int i = 0; i < ROWS / 16; ++i)
+#pragma unroll
+      for (int j = 0; j < NI; ++j)
+        *reinterpret_cast<__attribute__((address_space(3))) f32x4 *>(patch + patch_at<COLS>(i * 16 + lane % 16, j * 4 + lane / 16)) =
+            acc[h * (ROWS / 16) + i][j];
+    wait_lds();
+#pragma unroll 4
+    for (int row = lane / LANES; row < ROWS; row += 64 / LANES) {
+      float v[8];
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        const f32x4 u = __builtin_bit_cast(f32x4, lds_read16(patch + patch_at<COLS>(row, c * 2 + q)));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[q * 4 + i] = u[i];
+      }
+      put(h * ROWS + row, c * 8, v);
+    }
+  }
+}
+
+// Each row's largest logit of the tile's columns and the sum of exp(logit - largest): a lane's
+// own columns, the four lanes of a row, the waves side by side in LDS.
+struct Stats {
+  typedef XentParams Params;
+  template <typename T, int BM, int BN, int WM, int WN, int ROWS, int MI, int NI>
+  static __device__ __forceinline__ void finish(const XentParams &p, f32x4 (&acc)[MI][NI], int, lds_char *lds, lds_char *, int m0, int n0,
+                                                int wm, int wn, int tm, int tn) {
+    const int lane = threadIdx.x % 64, l = lane % 16, g = lane / 16, nw = n0 + wn * (BN / WN), nt = tn * BN;
+    auto *slots = reinterpret_cast<__attribute__((address_space(3))) f32x2 *>(lds);
+    const bool whole = nw >= nt && nw + NI * 16 <= p.n;
+#pragma unroll
+    for (int i = 0; i < MI; ++i) {
+      const int in_tile = wm * (BM / WM) + i * 16 + l, m = m0 + in_tile;
+      // The target's logit, by the one lane that holds it.
+      const long long target = m < p.m && m >= tm * BM ? p.target[m] : -1;
+      if (target >= max(nw, nt) && target < min(nw + NI * 16, p.n) && static_cast<int>(target - nw) / 4 % 4 == g) {
+        const int t = static_cast<int>(target - nw);
+        float v = 0.0f;
+#pragma unroll
+        for (int j = 0; j < NI; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (t / 16 == j && t % 4 == e) v = acc[i][j][e];
+        p.target_logit[m] = v;
+      }
+      if (!whole) {  // columns of another tile, or of none
+#pragma unroll
+        for (int j = 0; j < NI; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int n = nw + j * 16 + g * 4 + e;
+            if (n < nt || n >= p.n) acc[i][j][e] = -__builtin_inff();
+          }
+      }
+      float top = acc[i][0][0], sum = 0.0f;
+#pragma unroll
+      for (int j = 0; j < NI; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) top = __builtin_fmaxf(top, acc[i][j][e]);
+      top = __builtin_fmaxf(top, __shfl_xor(top, 16));
+      top = __builtin_fmaxf(top, __shfl_xor(top, 32));
+      const float from = top == -__builtin_inff() ? 0.0f : top;  // a NaN is in the sum
+#pragma unroll
+      for (int j = 0; j < NI; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sum += fast_exp2((acc[i][j][e] - from) * kLog2e);
+      sum += __shfl_xor(sum, 16);
+      sum += __shfl_xor(sum, 32);
+      if (g == 0) slots[wn * BM + in_tile] = f32x2{top, sum};
+    }
+    wait_lds();
+    barrier();
+    for (int r = threadIdx.x; r < BM; r += 64 * WM * WN) {
+      const int m = m0 + r;
+      if (m >= p.m || m < tm * BM) continue;
+      f32x2 s = slots[r];
+#pragma unroll
+      for (int w = 1; w < WN; ++w) {
+        const f32x2 o = slots[w * BM + r];
+        const float top = __builtin_fmaxf(s.x, o.x), from = top == -__builtin_inff() ? 0.0f : top;
+        s = f32x2{top, s.y * fast_exp2((s.x - from) * kLog2e) + o.y * fast_exp2((o.x - from) * kLog2e)};
+      }
+      reinterpret_cast<f32x2 *>(p.stats)[static_cast<long>(tn) * p.m + m] = s;
+    }
+  }
+};
+
+// What a finished sum of the gradient's products is multiplied by.
+__device__ __forceinline__ float sum_unit(const XentParams &p) {
+  if (p.dloss_rows) return p.scale ? p.scale[1] : 1.0f;
+  return *p.dloss / (p.count && *p.count > 0.0f ? *p.count : 1.0f) / p.power;
+}
+// Zeros stay (rows that do not count, where dloss is no number).
+__device__ __forceinline__ float in_unit(float v, float unit) { return v == 0.0f ? 0.0f : v * unit; }
+
+// The logits' gradient, in T: without dloss where that is one for all.  The target's -(1 - p), most of it,
+// then lies where T's spacing is least against it, and is exact while p is small.  8192 x 65536 x 2048 bfloat16:
+// dx and dw 0.0025 off 64 bits with dloss in it, 0.0017 without (their own rounding).
+struct Slope {
+  typedef XentParams Params;
+  template <typename T, int BM, int BN, int WM, int WN, int ROWS, int MI, int NI>
+  static __device__ __forceinline__ void finish(const XentParams &p, f32x4 (&acc)[MI][NI], int, lds_char *, lds_char *patch, int m0, int n0,
+                                                int wm, int wn, int tm, int tn) {
+    const int lane = threadIdx.x % 64, l = lane % 16, g = lane / 16, mw = m0 + wm * (BM / WM), nw = n0 + wn * (BN / WN);
+    const float unit = p.dloss_rows ? (p.scale ? p.scale[0] : 1.0f) / (p.count ? *p.count : 1.0f) : p.power;
+    const bool whole = nw + NI * 16 <= p.n;
+#pragma unroll
+    for (int i = 0; i < MI; ++i) {
+      const int m = min(mw + i * 16 + l, p.m - 1);  // rows past the last are not written
+      const long long target = p.target[m];
+      const bool dead = target == p.ignore;
+      const float lse = p.lse[m];
+      float d = p.dloss_rows ? p.dloss[m] * unit : unit;
+      const bool valid = target >= 0 && target < p.vocabulary;
+      if (!valid) d = __builtin_nanf("");
+      const long long from = valid ? target - p.column0 - nw : -1;
+      const int t = static_cast<int>(from);
+      const bool here = from >= 0 && from < NI * 16 && t / 4 % 4 == g;
+#pragma unroll
+      for (int j = 0; j < NI; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[i][j][e] = fast_exp2((acc[i][j][e] - lse) * kLog2e);
+      if (here) {
+#pragma unroll
+        for (int j = 0; j < NI; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (t / 16 == j && t % 4 == e) acc[i][j][e] -= 1.0f;
+      }
+#pragma unroll
+      for (int j = 0; j < NI; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const bool none = dead || (!whole && nw + j * 16 + g * 4 + e >= p.n);
+          acc[i][j][e] = none ? 0.0f : acc[i][j][e] * d;
+        }
+    }
+    const int end = (p.n + 7) & ~7;  // the next product reads whole pieces
+    T *out = static_cast<T *>(p.out);
+    by_rows<ROWS>(acc, patch, [&](int row, int column, const float (&v)[8]) {
+      const int m = mw + row, n = nw + column;
+      if (m >= p.m || m < tm * BM || n >= p.n || n + 7 < tn * BN) return;
+      T *to = out + m * p.ldo;
+      store_some(to + n, end - n, v);
+      for (int c = n + 8; n + 8 >= p.n && c < end; ++c) to[c] = static_cast<T>(0.0f);  // a tile moved back ends with n
+    });
+  }
+};
+
+// A product added to what earlier pieces left.
+struct Sum {
+  typedef XentParams Params;
+  template <typename T, int BM, int BN, int WM, int WN, int ROWS, int MI, int NI>
+  static __device__ __forceinline__ void finish(const XentParams &p, f32x4 (&acc)[MI][NI], int split, lds_char *, lds_char *patch, int m0,
+                                                int n0, int wm, int wn, int tm, int tn) {
+    const int mw = m0 + wm * (BM / WM), nw = n0 + wn * (BN / WN), nt = tn * BN;
+    const long ld = (p.n + 3) & ~3;
+    float *part = p.parts + split * (p.m * ld);
+    const float unit = sum_unit(p);
+    by_rows<ROWS>(acc, patch, [&](int row, int column, float (&v)[8]) {
+      const int m = mw + row, n = nw + column, left = p.n - n;
+      if (m >= p.m || m < tm * BM || left <= 0 || n + 7 < nt) return;
+      if (p.splits > 1) {
+        store_some(part + m * ld + n, left, v);
+        return;
+      }
+      if (p.add) {
+        float u[8];
+        load_some(p.sum + m * ld + n, left, u);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] += u[i];
+      }
+      if (p.last) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = in_unit(v[i], unit);
+        store_some(static_cast<T *>(p.out) + m * p.ldo + n, left, v);
+      } else if (n >= nt) {
+        store_some(p.sum + m * ld + n, left, v);
+      } else {  // a tile moved back: the columns before its own are another's sum
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (i < left && n + i >= nt) p.sum[m * ld + n + i] = v[i];
+      }
+    });
+  }
+};
+
+template <typename T, typename E, bool AMN, bool BMN, int BM, int WN, int ST, bool DMA>
+__global__ __launch_bounds__(256, DMA ? 1 : 3) void xent_tile_kernel(XentParams p) {
+  __shared__ __align__(1024) char smem[tile_lds<BM, BM, ST>()];
+  const int block = static_cast<int>(block_of()), blocks = p.tiles_m * p.tiles_n * p.splits;
+  if (block < blocks) gemm_tile<T, T, AMN, BMN, BM, BM, 2, WN, ST, DMA, 1, E>(p, block, blocks, (lds_char *)smem);
+}
+template <typename T, typename E, bool AMN, bool BMN>
+__global__ __launch_bounds__(512, 2) void xent_wide_kernel(XentParams p) {
+  __shared__ __align__(1024) char smem[kWideLds];
+  gemm_wide<T, T, AMN, BMN, E>(p, (lds_char *)smem);
+}
+
+template <typename T, typename E, bool AMN, bool BMN>
+hipError_t launch_xent_as(const XentParams &p, int tile, bool dma, hipStream_t stream) {
+  const long blocks = static_cast<long>(p.tiles_m) * p.tiles_n * p.splits;
+  const dim3 grid = grid_of(blocks, 256);
+  if (!dma) xent_tile_kernel<T, E, AMN, BMN, 64, 2, 2, false><<<grid, 256, 0, stream>>>(p);
+  else if (tile == TILE_256) xent_wide_kernel<T, E, AMN, BMN><<<dim3(static_cast<unsigned>(blocks)), 512, 0, stream>>>(p);
+  else if (tile == TILE_128) xent_tile_kernel<T, E, AMN, BMN, 128, 2, 2, true><<<grid, 256, 0, stream>>>(p);
+  else xent_tile_kernel<T, E, AMN, BMN, 64, 2, 3, true><<<grid, 256, 0, stream>>>(p);
+  return hipGetLastError();
+}
+
+template <typename T>
+hipError_t launch_xent(const XentParams &p, XentProduct what, bool amn, bool bmn, int tile, bool dma, hipStream_t stream) {
+  if (what == XENT_STATS) return bmn ? launch_xent_as<T, Stats, false, true>(p, tile, dma, stream) : launch_xent_as<T, Stats, false, false>(p, tile, dma, stream);
+  if (what == XENT_SLOPE) return bmn ? launch_xent_as<T, Slope, false, true>(p, tile, dma, stream) : launch_xent_as<T, Slope, false, false>(p, tile, dma, stream);
+  if (amn) return launch_xent_as<T, Sum, true, true>(p, tile, dma, stream);
+  return bmn ? launch_xent_as<T, Sum, false, true>(p, tile, dma, stream) : launch_xent_as<T, Sum, false, false>(p, tile, dma, stream);
+}
+
+}  // namespace tfnn

@@ -11,8 +11,10 @@ gradients.
     8-bit product             out = linear(q, wq.t(), b, "gelu", r, x_scale=s, w_scale=ws)
     kept in 8 bits            x8 = keep8(x); x8.restore(); linear(..., keep8=True),
                               rms_norm(..., keep8=True) for their gradients
+    loss over a vocabulary    loss = linear_cross_entropy(x, w, target)
     gradients                 dx, dweight = rms_norm_grad(dy, h, weight, dh=...)
                               dx, dw, dbias = linear_grad(dy, x, w, z, "gelu", bias_dtype=...)
+                              dx, dw = linear_cross_entropy_grad(dloss, x, w, target, lse)
 
 Every call enqueues kernels of libtforge_hip on the tensors' device and torch's
 current stream, and returns new tensors; nothing is synchronised, and a call may
@@ -28,8 +30,9 @@ Bad arguments raise ValueError or TypeError before any work; errors of the
 library raise RuntimeError with its message.
 """
 
+import functools
+
 import torch
-from torch.autograd.function import once_differentiable
 
 from tensorforge_amd import _lib
 
@@ -37,6 +40,31 @@ _lib.lib()  # the kernels; also the check that they are built
 from tensorforge_amd import _nn_torch as _C  # noqa: E402  (links libtforge_hip.so)
 
 ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "silu": 3}
+
+
+class _Refused(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, t):
+        return t.view_as(t)
+
+    @staticmethod
+    def backward(ctx, g):
+        raise RuntimeError("trying to differentiate twice: the gradient calls have no gradient (once_differentiable)")
+
+
+def _once_differentiable(backward):
+    """A backward whose results raise where a second derivative reaches them.  (torch's own decorator lets one through where the
+    incoming gradient is a constant: the loss itself, or a sum.)"""
+
+    @functools.wraps(backward)
+    def run(ctx, *grads):
+        with torch.no_grad():
+            got = backward(ctx, *grads)
+        if not torch.is_grad_enabled():
+            return got
+        return tuple(t if t is None else _Refused.apply(t.detach().requires_grad_()) for t in got)
+
+    return run
 
 
 def _act(activation):
@@ -156,7 +184,7 @@ class _RmsNorm(torch.autograd.Function):
         return y, h
 
     @staticmethod
-    @once_differentiable
+    @_once_differentiable
     def backward(ctx, dy, dh):
         h, weight = ctx.saved_tensors
         h = _again(h, ctx.kept)
@@ -231,7 +259,7 @@ class _Linear(torch.autograd.Function):
         return out, z if keep else None
 
     @staticmethod
-    @once_differentiable
+    @_once_differentiable
     def backward(ctx, dy, dz):
         x, w, z = ctx.saved_tensors
         x, z = _again(x, ctx.kept[0]), _again(z, ctx.kept[1])
@@ -248,3 +276,57 @@ class _Linear(torch.autograd.Function):
         total = (None, None, None) if not got else got[0] if len(got) == 1 else [a if a is None else a + b for a, b in zip(*got)]
         return (*total, dy.reshape(ctx.added) if need[3] and dy is not None else None, None, None, None, None, None,
                 None)
+
+
+# ---- the loss over a vocabulary -----------------------------------------------------
+
+REDUCTIONS = {"none": 0, "sum": 1, "mean": 2}
+
+
+def linear_cross_entropy(x, w, target, ignore_index=-100, reduction="mean", keep=False):
+    """The cross entropy of the logits x @ w with the classes target, without the logits in memory.
+
+    x (..., k) and w (k, n) are bfloat16 or float16, w row by row or column by column
+    (w = weight.t() of an n x k weight); target (...) is int64.  loss[i] = log(sum of
+    exp(logits[i])) - logits[i][target[i]] in float32.  Rows with the target ignore_index do not
+    count: their loss is 0, and the mean is over the others (0 if there are none).  Any other
+    target outside of 0..n-1 gives NaN.  reduction: "mean", "sum" or "none".  Returns the
+    loss, or (loss, lse, count) with keep=True: what linear_cross_entropy_grad takes.
+    """
+    code = REDUCTIONS.get(reduction)
+    if code is None:
+        raise ValueError(f"reduction {reduction!r} is not one of {', '.join(REDUCTIONS)}")
+    got = _C.linear_xent(x, w, target, ignore_index, code)
+    if got is None:
+        got = _LinearXent.apply(x, w, target, ignore_index, code)
+    return got if keep else got[0]
+
+
+def linear_cross_entropy_grad(dloss, x, w, target, lse, count=None, ignore_index=-100, want_dx=True, want_dw=True):
+    """(dx, dw) of linear_cross_entropy from the gradient dloss of its loss (one number, or one a row) and the kept lse.
+
+    count: the one kept with reduction="mean", whose gradient it then is.  dw lies in memory
+    as w does.  The products take the logits' gradient rounded to x's type.  What is not wanted is None.
+    """
+    return _C.linear_xent_grad(dloss, x, w, target, lse, count, ignore_index, True if want_dx else False, True if want_dw else False)
+
+
+class _LinearXent(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w, target, ignore, reduction):
+        with torch.no_grad():
+            loss, lse, count = _C.linear_xent(x, w, target, ignore, reduction)
+        ctx.save_for_backward(x, w, target, lse, count)
+        ctx.ignore = ignore
+        ctx.mark_non_differentiable(*(t for t in (lse, count) if t is not None))
+        ctx.set_materialize_grads(False)
+        return loss, lse, count
+
+    @staticmethod
+    @_once_differentiable
+    def backward(ctx, dloss, *_):
+        if dloss is None:
+            return None, None, None, None, None
+        x, w, target, lse, count = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        return (*linear_cross_entropy_grad(dloss.contiguous(), x, w, target, lse, count, ctx.ignore, need[0], need[1]), None, None, None)

@@ -175,3 +175,141 @@ for m, n, k in ((1, 1 << 26, 8), (64, big, 64), (big, 9, 8), (big, 1, 1), (1, 1,
         for act in (0, 1, 2):
             assert grad8(m, n, k, order, act) == 0, (m, n, k, order, act)
 """)
+
+
+# ---- the loss over a vocabulary ---------------------------------------------------
+
+
+def _xent(**kw):
+    base = dict(x=256, w=256, target=256, loss=256, lse=256, workspace=256, workspace_bytes=1 << 40, x_ld=64, w_ld=100, m=8, n=100, k=64,
+                ignore=-100, type=1)
+    return ctypes.byref(_lib.LinearXentArgs(**{**base, **kw}))
+
+
+def _xent_grad(**kw):
+    base = dict(x=256, w=256, target=256, lse=256, dloss=256, dx=256, dw=256, workspace=256, workspace_bytes=1 << 40, x_ld=64, w_ld=100,
+                dx_ld=64, dw_ld=100, m=8, n=100, k=64, ignore=-100, type=1, dloss_rows=1)
+    return ctypes.byref(_lib.LinearXentGradArgs(**{**base, **kw}))
+
+
+@pytest.mark.parametrize("change,words", [
+    (dict(type=0), "type = 0"), (dict(type=3), "type = 3"), (dict(w_order=2), "w_order = 2"), (dict(n=0), "no class"), (dict(m=-1), "m = -1"),
+    (dict(k=(1 << 30) + 1), "k = 1073741825"), (dict(x=0), "x is a null"), (dict(w=0), "w is a null"), (dict(target=0), "target is null"),
+    (dict(target=260), "target is null or not aligned"), (dict(loss=0), "loss is a null"), (dict(lse=0), "lse is a null"),
+    (dict(x_ld=63), "x: 63"), (dict(w_ld=99), "w: 99"), (dict(w_order=1, w_ld=63), "w: 63"), (dict(workspace=0), "workspace is null"),
+    (dict(workspace=264), "not 16-byte aligned"), (dict(workspace_bytes=16), "are needed"), (dict(x=257), "x is not aligned")])
+def test_xent_refusals(change, words):
+    _refused(_lib.lib().tf_linear_xent(_xent(**change), None), words)
+
+
+@pytest.mark.parametrize("change,words", [
+    (dict(type=4), "type = 4"), (dict(n=0), "no class"), (dict(dloss=0), "dloss is a null"), (dict(lse=0), "lse is a null"),
+    (dict(dloss_rows=2), "dloss_rows = 2"), (dict(target=0), "target is null"), (dict(dx_ld=63), "dx: 63"), (dict(dw_ld=99), "dw: 99"),
+    (dict(count=258), "count is not aligned"), (dict(workspace_bytes=16), "are needed"), (dict(m=(1 << 30) + 1), "m = 1073741825")])
+def test_xent_grad_refusals(change, words):
+    _refused(_lib.lib().tf_linear_xent_grad(_xent_grad(**change), None), words)
+    lib, n = _lib.lib(), ctypes.c_longlong()
+    assert lib.tf_linear_xent(None, None) == lib.tf_linear_xent_grad(None, None) == -4
+    assert lib.tf_linear_xent_workspace(None, ctypes.byref(n)) == lib.tf_linear_xent_grad_workspace(_xent_grad(), None) == -4
+
+
+def test_xent_python_refusals():
+    h, w, t = torch.zeros(4, 8, dtype=torch.bfloat16), torch.zeros(8, 16, dtype=torch.bfloat16), torch.zeros(4, dtype=torch.int64)
+    one, rows = torch.ones(()), torch.zeros(4)
+    for call, error, words in [
+            (lambda: nn.linear_cross_entropy(h, w, t), ValueError, "not on a GPU"),
+            (lambda: nn.linear_cross_entropy(h, w, t, reduction="max"), ValueError, "not one of none, sum, mean"),
+            (lambda: nn.linear_cross_entropy(h.float(), w.float(), t), TypeError, "x is Float"),
+            (lambda: nn.linear_cross_entropy(h, w.half(), t), TypeError, "w is Half"),
+            (lambda: nn.linear_cross_entropy(h, w, t.int()), TypeError, "target is Int"),
+            (lambda: nn.linear_cross_entropy(h, w, t[:3]), ValueError, "target is not"),
+            (lambda: nn.linear_cross_entropy(h, w, t[None]), ValueError, "target is not"),
+            (lambda: nn.linear_cross_entropy(h, w, t.repeat(2)[::2]), ValueError, "target is not"),
+            (lambda: nn.linear_cross_entropy(h, w[:4], t), ValueError, "not 8 x n"),
+            (lambda: nn.linear_cross_entropy(h, w[:, :0], t), ValueError, "not on a GPU|no class"),
+            (lambda: nn.linear_cross_entropy(h.clone().requires_grad_(), w, t), ValueError, "not on a GPU"),
+            (lambda: nn.linear_cross_entropy(h.clone().requires_grad_(), w, t[:3]), ValueError, "target is not"),
+            (lambda: nn.linear_cross_entropy_grad(one, h, w, t, rows), ValueError, "not on a GPU"),
+            (lambda: nn.linear_cross_entropy_grad(rows[:3], h, w, t, rows), ValueError, "dloss is not"),
+            (lambda: nn.linear_cross_entropy_grad(one.double(), h, w, t, rows), TypeError, "dloss is Double"),
+            (lambda: nn.linear_cross_entropy_grad(one, h, w, t, rows[:2]), ValueError, "lse is not"),
+            (lambda: nn.linear_cross_entropy_grad(one, h, w, t, rows, rows), ValueError, "count is not one"),
+            (lambda: nn.linear_cross_entropy_grad(one, h, w, t, rows.bfloat16()), TypeError, "lse is BFloat16"),
+            (lambda: nn.linear_cross_entropy_grad(one, h, w.clone().requires_grad_(), t, rows), ValueError, "no gradient")]:
+        with pytest.raises(error, match=words):
+            call()
+
+
+def test_xent_struct_layouts_match_c(tmp_path):
+    import subprocess
+    header = _lib.PKG.parent / "include" / "tforge_hip.h"
+    structs = {"tf_linear_xent_args_t": _lib.LinearXentArgs, "tf_linear_xent_grad_args_t": _lib.LinearXentGradArgs}
+    lines = ["#include <stdio.h>", "#include <stddef.h>", f'#include "{header}"', "int main(void) {"]
+    for cname, py in structs.items():
+        lines.append(f'  printf("%zu\\n", sizeof({cname}));')
+        lines += [f'  printf("%zu\\n", offsetof({cname}, {f}));' for f, _ in py._fields_]
+    (tmp_path / "sizes.c").write_text("\n".join(lines + ["  return 0;", "}"]))
+    subprocess.run(["gcc", str(tmp_path / "sizes.c"), "-o", str(tmp_path / "sizes")], check=True)
+    got = [int(v) for v in subprocess.run([str(tmp_path / "sizes")], capture_output=True, text=True).stdout.split()]
+    want = [v for py in structs.values() for v in [ctypes.sizeof(py)] + [getattr(py, f).offset for f, _ in py._fields_]]
+    assert got == want
+
+
+XENT = """
+def xent(m, n, k, order, type=1, fail=None):
+    a = _lib.LinearXentArgs(x=256, w=256, target=256, loss=256, lse=256, mean=256, count=256, workspace=256, x_ld=k, w_ld=k if order else n,
+                            m=m, n=n, k=k, w_order=order, type=type, ignore=-100)
+    size = ctypes.c_longlong()
+    assert lib.tf_linear_xent_workspace(ref(a), ref(size)) == 0
+    a.workspace_bytes = size.value
+    if fail is not None: stub.arm(fail)
+    return lib.tf_linear_xent(ref(a), None)
+def xent_grad(m, n, k, order, type=1, fail=None):
+    a = _lib.LinearXentGradArgs(x=256, w=256, target=256, lse=256, dloss=256, count=256, dx=256, dw=256, workspace=256, x_ld=k,
+                                w_ld=k if order else n, dx_ld=k, dw_ld=k if order else n, m=m, n=n, k=k, w_order=order, type=type, ignore=-100)
+    size = ctypes.c_longlong()
+    assert lib.tf_linear_xent_grad_workspace(ref(a), ref(size)) == 0
+    a.workspace_bytes = size.value
+    if fail is not None: stub.arm(fail)
+    return lib.tf_linear_xent_grad(ref(a), None)
+"""
+
+
+def test_failed_launches_of_the_loss(without_gpu):  # noqa: F811
+    """Whichever of its launches fails, the call says so."""
+    without_gpu(XENT + """
+for m, n, k in ((1, 5, 64), (70, 1001, 333), (4096, 4096, 4096), (20000, 40000, 72), (1, 70000, 2048)):
+    for order in (0, 1):
+        for type in (1, 2):
+            for call in (xent, xent_grad):
+                assert call(m, n, k, order, type, -1) == 0
+                for i in range(stub.arm(-1)):
+                    assert call(m, n, k, order, type, i) == -5, (call, m, n, k, order, i)
+""")
+
+
+def test_losses_of_extreme_sizes_launch(without_gpu):  # noqa: F811
+    """One side as long as memory may hold: no launch has 2^32 threads."""
+    without_gpu(XENT + """
+big = 1 << 30
+for m, n, k in ((1, big, 8), (big, 1, 1), (big, 9, 8), (1 << 24, 1 << 18, 64), (1 << 20, 1 << 20, 1000), (1, 1, big), (64, 1 << 28, 7), (0, 100, 64)):
+    for order in (0, 1):
+        for type in (1, 2):
+            assert xent(m, n, k, order, type) == 0, (m, n, k, order)
+            assert xent_grad(m, n, k, order, type) == 0, (m, n, k, order)
+""")
+
+
+def test_second_order_with_constant_gradients():
+    """A sum's gradient is a constant: a penalty on what it gives is refused all the same."""
+    from test_nn_autograd import Plain
+    plain, native = Plain(), nn._C
+    nn._C = plain
+    try:
+        x, w, w1 = (torch.randn(s, dtype=torch.float64, requires_grad=True) for s in ((6, 8), (8,), (8, 5)))
+        for loss, of in ((nn.rms_norm(x, w)[0].sum(), w), (nn.linear(x, w1, None, "gelu").sum(), w1), (nn.linear(x, w1).sum(), x)):
+            g, = torch.autograd.grad(loss, of, create_graph=True)
+            with pytest.raises(RuntimeError, match="twice"):
+                (loss.detach() + g.pow(2).sum()).backward()
+    finally:
+        nn._C = native
