@@ -8,7 +8,7 @@
 // with the same steps in Python (ctypes), 5.4 us here.
 //
 // Where an input wants a gradient, rms_norm and linear return None, and tforge_nn.py
-// goes through autograd; the calls without a gradient refuse.
+// goes through autograd; linear_xent's is here; the calls without a gradient refuse.
 #include <ATen/ATen.h>
 #include <ATen/core/grad_mode.h>
 #include <ATen/hip/EmptyTensor.h>
@@ -18,6 +18,8 @@
 #include <torch/csrc/DynamicTypes.h>
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include "tforge_hip.h"
@@ -467,54 +469,55 @@ long long integer64(PyObject *o) {
   return v;
 }
 
-// (x, w, target, ignore, reduction) -> (loss, lse, count); reduction: 0 none, 1 sum, 2 mean
-PyObject *linear_xent(PyObject *, PyObject *const *a, Py_ssize_t n) {
-  HANDLE_TH_ERRORS
-  count(n, 5);
-  const Tensor &x = tensor(a[0], "x"), &w = tensor(a[1], "w"), &target = tensor(a[2], "target");
+// The loss of checked operands, and what its gradient takes.
+struct Xent {
+  Tensor loss, lse, count;
+};
+void xent_operands(const Tensor &x, const Tensor &w, const Tensor &target, Rows &xr, Weights &wr) {
   const ScalarType t = x.scalar_type();
   TORCH_CHECK_TYPE(half_type(t), "x is ", t, ", not BFloat16 or Half");
-  const Rows xr = rows(x, "x");
-  const Weights wr = weights(w, xr.n, t);
+  xr = rows(x, "x");
+  wr = weights(w, xr.n, t);
+  targets(target, x);
+}
+
+// reduction: 0 none, 1 sum, 2 mean
+Xent xent(const Tensor &x, const Tensor &w, const Tensor &target, int64_t ignore, int64_t reduction) {
+  Rows xr;
+  Weights wr;
+  xent_operands(x, w, target, xr, wr);
   tf_linear_xent_args_t g{};
   g.target = targets(target, x);
-  const int reduction = integer(a[4], "reduction");
-  if (wants_grad({&x, &w})) Py_RETURN_NONE;
   g.x = xr.p, g.x_ld = xr.ld, g.m = xr.m, g.k = xr.n, g.w = wr.p, g.w_ld = wr.ld, g.n = wr.n, g.w_order = wr.order;
-  g.type = type_of(t), g.ignore = integer64(a[3]);
+  g.type = type_of(x.scalar_type()), g.ignore = ignore;
   on_gpu(x, {&w, &target});
   const On on(x);
   const at::IntArrayRef shape = x.sizes().slice(0, x.dim() - 1);
-  Tensor loss = fresh(x, shape, ScalarType::Float), lse = fresh(x, shape, ScalarType::Float), space, one, number;
-  g.loss = loss.data_ptr<float>(), g.lse = lse.data_ptr<float>();
+  Xent r{fresh(x, shape, ScalarType::Float), fresh(x, shape, ScalarType::Float), {}};
+  g.loss = r.loss.data_ptr<float>(), g.lse = r.lse.data_ptr<float>();
+  Tensor one, space;
   if (reduction) one = fresh(x, {}, ScalarType::Float), (reduction == 1 ? g.sum : g.mean) = one.data_ptr<float>();
-  if (reduction == 2) number = fresh(x, {}, ScalarType::Float), g.count = number.data_ptr<float>();
+  if (reduction == 2) r.count = fresh(x, {}, ScalarType::Float), g.count = r.count.data_ptr<float>();
   check(tf_linear_xent_workspace(&g, &g.workspace_bytes));
   if (g.workspace_bytes) space = fresh(x, {static_cast<int64_t>(g.workspace_bytes)}, ScalarType::Byte), g.workspace = space.data_ptr();
   check(tf_linear_xent(&g, on.stream));
-  return tuple({reduction ? &one : &loss, &lse, reduction == 2 ? &number : nullptr});
-  END_HANDLE_TH_ERRORS
+  if (reduction) r.loss = one;
+  return r;
 }
 
-// (dloss, x, w, target, lse, count, ignore, want_dx, want_dw) -> (dx, dw)
-PyObject *linear_xent_grad(PyObject *, PyObject *const *a, Py_ssize_t n) {
-  HANDLE_TH_ERRORS
-  count(n, 9);
-  const Tensor &dloss = tensor(a[0], "dloss"), &x = tensor(a[1], "x"), &w = tensor(a[2], "w"), &target = tensor(a[3], "target");
-  const Tensor &lse = tensor(a[4], "lse"), *number = optional(a[5], "count");
+std::pair<Tensor, Tensor> xent_grad(const Tensor &dloss, const Tensor &x, const Tensor &w, const Tensor &target, const Tensor &lse,
+                                    const Tensor *number, int64_t ignore, bool want_dx, bool want_dw) {
+  Rows xr;
+  Weights wr;
+  xent_operands(x, w, target, xr, wr);
   const ScalarType t = x.scalar_type();
-  TORCH_CHECK_TYPE(half_type(t), "x is ", t, ", not BFloat16 or Half");
-  no_gradient("linear_cross_entropy_grad", {&dloss, &x, &w, &lse, number});
-  const bool want_dx = a[7] == Py_True, want_dw = a[8] == Py_True;
-  const Rows xr = rows(x, "x");
-  const Weights wr = weights(w, xr.n, t);
   tf_linear_xent_grad_args_t g{};
   g.target = targets(target, x);
   const at::IntArrayRef shape = x.sizes().slice(0, x.dim() - 1);
   same_type(lse, "lse", ScalarType::Float, ScalarType::Float);
   TORCH_CHECK_VALUE(lse.sizes() == shape && lse.is_contiguous(), "lse is not a contiguous tensor of ", shape);
   same_type(dloss, "dloss", ScalarType::Float, ScalarType::Float);
-  g.dloss_rows = dloss.dim() != 0 || shape.empty();
+  g.dloss_rows = dloss.dim() != 0;
   TORCH_CHECK_VALUE(dloss.dim() == 0 || (dloss.sizes() == shape && dloss.is_contiguous()), "dloss is not one number or a contiguous tensor of ", shape);
   if (number) {
     same_type(*number, "count", ScalarType::Float, ScalarType::Float);
@@ -523,7 +526,7 @@ PyObject *linear_xent_grad(PyObject *, PyObject *const *a, Py_ssize_t n) {
   }
   g.lse = lse.data_ptr<float>(), g.dloss = dloss.data_ptr<float>();
   g.x = xr.p, g.x_ld = xr.ld, g.m = xr.m, g.k = xr.n, g.w = wr.p, g.w_ld = wr.ld, g.n = wr.n, g.w_order = wr.order;
-  g.type = type_of(t), g.ignore = integer64(a[6]);
+  g.type = type_of(t), g.ignore = ignore;
   on_gpu(x, {&w, &target, &lse, &dloss, number});
   const On on(x);
   Tensor dx, dw, space;
@@ -535,7 +538,70 @@ PyObject *linear_xent_grad(PyObject *, PyObject *const *a, Py_ssize_t n) {
   check(tf_linear_xent_grad_workspace(&g, &g.workspace_bytes));
   if (g.workspace_bytes) space = fresh(x, {static_cast<int64_t>(g.workspace_bytes)}, ScalarType::Byte), g.workspace = space.data_ptr();
   check(tf_linear_xent_grad(&g, on.stream));
-  return tuple({want_dx ? &dx : nullptr, want_dw ? &dw : nullptr});
+  return {dx, dw};
+}
+
+// The loss under autograd, natively: a step of a small classifier is bound by the host (61 x 1001 x
+// 333 102 us through a Python function, whose backward waits for the interpreter's lock).
+struct XentFunction : torch::autograd::Function<XentFunction> {
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext *ctx, const Tensor &x, const Tensor &w, const Tensor &target,
+                                                int64_t ignore, int64_t reduction) {
+    const at::AutoDispatchBelowADInplaceOrView below;
+    const Xent r = xent(x, w, target, ignore, reduction);
+    ctx->save_for_backward({x, w, target, r.lse, r.count});
+    ctx->saved_data["ignore"] = ignore;
+    if (r.count.defined()) ctx->mark_non_differentiable({r.lse, r.count});
+    else ctx->mark_non_differentiable({r.lse});
+    ctx->set_materialize_grads(false);
+    if (!r.count.defined()) return {r.loss, r.lse};
+    return {r.loss, r.lse, r.count};
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx, torch::autograd::variable_list grads) {
+    torch::autograd::variable_list all(5);
+    if (!grads[0].defined()) return all;
+    const auto saved = ctx->get_saved_variables();
+    const bool again = at::GradMode::is_enabled();
+    {
+      const at::NoGradGuard none;
+      std::tie(all[0], all[1]) = xent_grad(grads[0].contiguous(), saved[0], saved[1], saved[2], saved[3], saved[4].defined() ? &saved[4] : nullptr,
+                                           ctx->saved_data["ignore"].toInt(), ctx->needs_input_grad(0), ctx->needs_input_grad(1));
+    }
+    if (again) {  // what a second derivative reaches raises
+      const auto refuse = std::make_shared<torch::autograd::DelayedError>("trying to differentiate twice: the gradient calls have no gradient (once_differentiable)", 1);
+      for (Tensor &t : all)
+        if (t.defined()) t = (*refuse)({t.detach().set_requires_grad(true)})[0];
+    }
+    return all;
+  }
+};
+
+// (x, w, target, ignore, reduction) -> (loss, lse, count)
+PyObject *linear_xent(PyObject *, PyObject *const *a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  count(n, 5);
+  const Tensor &x = tensor(a[0], "x"), &w = tensor(a[1], "w"), &target = tensor(a[2], "target");
+  const int64_t ignore = integer64(a[3]), reduction = integer(a[4], "reduction");
+  if (wants_grad({&x, &w})) {
+    Rows xr;
+    Weights wr;
+    xent_operands(x, w, target, xr, wr);
+    const auto r = XentFunction::apply(x, w, target, ignore, reduction);
+    return tuple({&r[0], &r[1], r.size() > 2 ? &r[2] : nullptr});
+  }
+  const Xent r = xent(x, w, target, ignore, reduction);
+  return tuple({&r.loss, &r.lse, r.count.defined() ? &r.count : nullptr});
+  END_HANDLE_TH_ERRORS
+}
+
+// (dloss, x, w, target, lse, count, ignore, want_dx, want_dw) -> (dx, dw)
+PyObject *linear_xent_grad(PyObject *, PyObject *const *a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  count(n, 9);
+  const Tensor &dloss = tensor(a[0], "dloss"), &x = tensor(a[1], "x"), &w = tensor(a[2], "w"), &target = tensor(a[3], "target");
+  const Tensor &lse = tensor(a[4], "lse"), *number = optional(a[5], "count");
+  no_gradient("linear_cross_entropy_grad", {&dloss, &x, &w, &lse, number});
+  const auto [dx, dw] = xent_grad(dloss, x, w, target, lse, number, integer64(a[6]), a[7] == Py_True, a[8] == Py_True);
+  return tuple({dx.defined() ? &dx : nullptr, dw.defined() ? &dw : nullptr});
   END_HANDLE_TH_ERRORS
 }
 

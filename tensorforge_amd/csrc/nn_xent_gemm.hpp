@@ -41,8 +41,17 @@ __device__ __forceinline__ void by_rows(const f32x4 (&acc)[MI][NI], lds_char *pa
   }
 }
 
-// Each row's largest logit of the tile's columns and the sum of exp(logit - largest): a lane's
-// own columns, the four lanes of a row, the waves side by side in LDS.
+// Logarithms of sums are kept as pairs: t, and the sum of exp2(value * log2(e) - t).  t is the
+// largest value times log2(e), rounded: whatever it was rounded to, the pair stands for the sum.
+// -inf: no value yet.
+__device__ __forceinline__ float from_of(float t) { return t == -__builtin_inff() ? 0.0f : t; }
+__device__ __forceinline__ f32x2 joined(f32x2 a, f32x2 b) {
+  const float t = __builtin_fmaxf(a.x, b.x), from = from_of(t);
+  return f32x2{t, a.y * fast_exp2(a.x - from) + b.y * fast_exp2(b.x - from)};
+}
+
+// Each row's pair over the tile's columns: a lane's own columns, the four lanes of a row, the
+// waves side by side in LDS.
 struct Stats {
   typedef XentParams Params;
   template <typename T, int BM, int BN, int WM, int WN, int ROWS, int MI, int NI>
@@ -51,13 +60,17 @@ struct Stats {
     const int lane = threadIdx.x % 64, l = lane % 16, g = lane / 16, nw = n0 + wn * (BN / WN), nt = tn * BN;
     auto *slots = reinterpret_cast<__attribute__((address_space(3))) f32x2 *>(lds);
     const bool whole = nw >= nt && nw + NI * 16 <= p.n;
+    // The targets, all under way at once (one after the other: 8192 x 65536 x 2048 1.84 ms).
+    long long target[MI];
+#pragma unroll
+    for (int i = 0; i < MI; ++i) target[i] = p.target[min(m0 + wm * (BM / WM) + i * 16 + l, p.m - 1)];
 #pragma unroll
     for (int i = 0; i < MI; ++i) {
       const int in_tile = wm * (BM / WM) + i * 16 + l, m = m0 + in_tile;
       // The target's logit, by the one lane that holds it.
-      const long long target = m < p.m && m >= tm * BM ? p.target[m] : -1;
-      if (target >= max(nw, nt) && target < min(nw + NI * 16, p.n) && static_cast<int>(target - nw) / 4 % 4 == g) {
-        const int t = static_cast<int>(target - nw);
+      if (target[i] >= max(nw, nt) && target[i] < min(nw + NI * 16, p.n) && static_cast<int>(target[i] - nw) / 4 % 4 == g && m < p.m &&
+          m >= tm * BM) {
+        const int t = static_cast<int>(target[i] - nw);
         float v = 0.0f;
 #pragma unroll
         for (int j = 0; j < NI; ++j)
@@ -81,12 +94,12 @@ struct Stats {
 #pragma unroll
         for (int e = 0; e < 4; ++e) top = __builtin_fmaxf(top, acc[i][j][e]);
       top = __builtin_fmaxf(top, __shfl_xor(top, 16));
-      top = __builtin_fmaxf(top, __shfl_xor(top, 32));
-      const float from = top == -__builtin_inff() ? 0.0f : top;  // a NaN is in the sum
+      top = __builtin_fmaxf(top, __shfl_xor(top, 32)) * kLog2e;
+      const float from = from_of(top);  // a NaN is in the sum
 #pragma unroll
       for (int j = 0; j < NI; ++j)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) sum += fast_exp2((acc[i][j][e] - from) * kLog2e);
+        for (int e = 0; e < 4; ++e) sum += fast_exp2(__builtin_fmaf(acc[i][j][e], kLog2e, -from));
       sum += __shfl_xor(sum, 16);
       sum += __shfl_xor(sum, 32);
       if (g == 0) slots[wn * BM + in_tile] = f32x2{top, sum};
@@ -98,11 +111,7 @@ struct Stats {
       if (m >= p.m || m < tm * BM) continue;
       f32x2 s = slots[r];
 #pragma unroll
-      for (int w = 1; w < WN; ++w) {
-        const f32x2 o = slots[w * BM + r];
-        const float top = __builtin_fmaxf(s.x, o.x), from = top == -__builtin_inff() ? 0.0f : top;
-        s = f32x2{top, s.y * fast_exp2((s.x - from) * kLog2e) + o.y * fast_exp2((o.x - from) * kLog2e)};
-      }
+      for (int w = 1; w < WN; ++w) s = joined(s, slots[w * BM + r]);
       reinterpret_cast<f32x2 *>(p.stats)[static_cast<long>(tn) * p.m + m] = s;
     }
   }
@@ -127,36 +136,45 @@ struct Slope {
     const int lane = threadIdx.x % 64, l = lane % 16, g = lane / 16, mw = m0 + wm * (BM / WM), nw = n0 + wn * (BN / WN);
     const float unit = p.dloss_rows ? (p.scale ? p.scale[0] : 1.0f) / (p.count ? *p.count : 1.0f) : p.power;
     const bool whole = nw + NI * 16 <= p.n;
+    // What the rows need, all under way at once.  Rows past the last are not written.
+    long long target[MI];
+    float lse[MI], d[MI];
 #pragma unroll
     for (int i = 0; i < MI; ++i) {
-      const int m = min(mw + i * 16 + l, p.m - 1);  // rows past the last are not written
-      const long long target = p.target[m];
-      const bool dead = target == p.ignore;
-      const float lse = p.lse[m];
-      float d = p.dloss_rows ? p.dloss[m] * unit : unit;
-      const bool valid = target >= 0 && target < p.vocabulary;
-      if (!valid) d = __builtin_nanf("");
-      const long long from = valid ? target - p.column0 - nw : -1;
+      const int m = min(mw + i * 16 + l, p.m - 1);
+      target[i] = p.target[m];
+      lse[i] = p.lse[m] * kLog2e;
+      d[i] = p.dloss_rows ? p.dloss[m] * unit : unit;
+    }
+#pragma unroll
+    for (int i = 0; i < MI; ++i) {
+      const bool dead = target[i] == p.ignore, valid = target[i] >= 0 && target[i] < p.vocabulary;
+      if (!valid) d[i] = __builtin_nanf("");
+      const long long from = valid ? target[i] - p.column0 - nw : -1;
       const int t = static_cast<int>(from);
       const bool here = from >= 0 && from < NI * 16 && t / 4 % 4 == g;
 #pragma unroll
       for (int j = 0; j < NI; ++j)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) acc[i][j][e] = fast_exp2((acc[i][j][e] - lse) * kLog2e);
+        for (int e = 0; e < 4; ++e) acc[i][j][e] = fast_exp2(__builtin_fmaf(acc[i][j][e], kLog2e, -lse[i])) * d[i];
       if (here) {
 #pragma unroll
         for (int j = 0; j < NI; ++j)
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            if (t / 16 == j && t % 4 == e) acc[i][j][e] -= 1.0f;
+            if (t / 16 == j && t % 4 == e) acc[i][j][e] -= d[i];
       }
+      if (dead) {
 #pragma unroll
-      for (int j = 0; j < NI; ++j)
+        for (int j = 0; j < NI; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      }
+      if (!whole) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const bool none = dead || (!whole && nw + j * 16 + g * 4 + e >= p.n);
-          acc[i][j][e] = none ? 0.0f : acc[i][j][e] * d;
-        }
+        for (int j = 0; j < NI; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (nw + j * 16 + g * 4 + e >= p.n) acc[i][j][e] = 0.0f;
+      }
     }
     const int end = (p.n + 7) & ~7;  // the next product reads whole pieces
     T *out = static_cast<T *>(p.out);

@@ -297,8 +297,6 @@ def linear_cross_entropy(x, w, target, ignore_index=-100, reduction="mean", keep
     if code is None:
         raise ValueError(f"reduction {reduction!r} is not one of {', '.join(REDUCTIONS)}")
     got = _C.linear_xent(x, w, target, ignore_index, code)
-    if got is None:
-        got = _LinearXent.apply(x, w, target, ignore_index, code)
     return got if keep else got[0]
 
 
@@ -309,24 +307,3 @@ def linear_cross_entropy_grad(dloss, x, w, target, lse, count=None, ignore_index
     as w does.  The products take the logits' gradient rounded to x's type.  What is not wanted is None.
     """
     return _C.linear_xent_grad(dloss, x, w, target, lse, count, ignore_index, True if want_dx else False, True if want_dw else False)
-
-
-class _LinearXent(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, w, target, ignore, reduction):
-        with torch.no_grad():
-            loss, lse, count = _C.linear_xent(x, w, target, ignore, reduction)
-        ctx.save_for_backward(x, w, target, lse, count)
-        ctx.ignore = ignore
-        ctx.mark_non_differentiable(*(t for t in (lse, count) if t is not None))
-        ctx.set_materialize_grads(False)
-        return loss, lse, count
-
-    @staticmethod
-    @_once_differentiable
-    def backward(ctx, dloss, *_):
-        if dloss is None:
-            return None, None, None, None, None
-        x, w, target, lse, count = ctx.saved_tensors
-        need = ctx.needs_input_grad
-        return (*linear_cross_entropy_grad(dloss.contiguous(), x, w, target, lse, count, ctx.ignore, need[0], need[1]), None, None, None)
