@@ -450,7 +450,8 @@ int tf_linear_xent(const tf_linear_xent_args_t *args, void *stream);
  *   dz[m][n] = (exp(z[m][n] - lse[m]) - [n == target[m]]) * dloss[m] / count
  *   dx = dz @ w^T,  dw = x^T @ dz in w's memory order
  * The logits are computed again, for a piece of the vocabulary at a time, and the
- * products take dz in `type`, rounded once: one dloss for all rows is multiplied into
+ * products take dz in `type`: rounded once, up to 64 rows in two terms (the value and
+ * what its rounding left, 16 bits more).  One dloss for all rows is multiplied into
  * their sums instead, and float16 has a unit that lets the largest dz reach 2^15.
  * Sums are float32, over the pieces too.  A row that does not count
  * has a dz of zeros whatever its x holds (dw is the product all the same: an x that is

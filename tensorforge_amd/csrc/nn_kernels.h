@@ -85,6 +85,7 @@ struct XentParams : GemmParams {
   const float *lse = nullptr, *dloss = nullptr, *count = nullptr, *scale = nullptr;
   float power = 1.0f;
   int dloss_rows = 0;
+  long lo = 0;  // not 0: what dz's rounding left, rounded, that many elements behind
   // XENT_SUM: out = (product + sum) * dloss / count / power (scale[1] or 1 with a dloss a row), or the new sum; m x (n up to a
   // multiple of 4) floats.
   float *sum = nullptr;

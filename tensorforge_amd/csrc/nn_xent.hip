@@ -257,7 +257,13 @@ int loss(const tf_linear_xent_args_t *a, hipStream_t stream) {
 constexpr long long kPieceBytes = 512 << 20;
 constexpr long kLeastColumns = 16384;
 
+// Up to so many rows the products take what dz's rounding left as a second term, into the same sums:
+// they are bound by reading w and writing dw, and a class that few rows have would see dz's rounding
+// in its dw (2 x 59648 x 3436 bfloat16: dw 0.0003 off 64 bits in one term, its own rounding 0.00018).
+constexpr long kTwoTermRows = 64;
+
 struct GradPlan {
+  int terms = 1;
   long width = 0, pieces = 0, dz_ld = 0;
   Operand x, w;                      // as they lie, or their aligned copies
   bool copy_x = false, copy_w = false;
@@ -293,6 +299,10 @@ Piece piece_of(const GradPlan &g, const tf_linear_xent_grad_args_t *a, long n) {
   s.dx.p.m = m, s.dx.p.n = k, s.dx.p.k = static_cast<int>(n);
   s.dw = {a->type, a->type, nk ? dz_as(true) : x_as(true), nk ? x_as(true) : dz_as(true), {}, true};
   s.dw.p.m = static_cast<int>(nk ? n : k), s.dw.p.n = static_cast<int>(nk ? k : n), s.dw.p.k = m;
+  if (g.terms == 2) {  // what the rounding left lies behind, and comes first
+    s.dx.p.terms = s.dw.p.terms = 2;
+    s.dx.p.a_term = (nk ? s.dw.p.a_term : s.dw.p.b_term) = -(g.dz / 2);
+  }
   if (m) s.cz = choose(s.z, 0, 1, false), s.cdx = choose(s.dx, 0, 0, false);
   s.cdw = choose(s.dw, 0, 0, false);
   return s;
@@ -316,7 +326,8 @@ GradPlan plan_grad(const tf_linear_xent_grad_args_t *a) {
     if (g.copy_w) g.w.ld = packed_ld(g.w, 2), g.w.ours = true;
   }
   g.scale = a->type == TF_T_F16 && a->dloss_rows && m ? 16 : 0;
-  g.dz = round16(2 * m * g.dz_ld);
+  g.terms = m <= kTwoTermRows ? 2 : 1;
+  g.dz = round16(2 * m * g.dz_ld) * g.terms;
   g.sum = a->dx && g.pieces > 1 ? round16(4 * m * ((k + 3) & ~3L)) : 0;
   for (const long width : {g.width, n - (g.pieces - 1) * g.width}) {
     const Piece s = piece_of(g, a, width);
@@ -395,10 +406,11 @@ int grad(const tf_linear_xent_grad_args_t *a, hipStream_t stream) {
     Piece s = piece_of(g, a, n);
     const auto from_column = [&](const void *w, long ld) { return static_cast<const char *>(w) + 2 * column0 * (nk ? ld : 1); };
     s.z.b.p = s.dx.b.p = from_column(g.w.p, g.w.ld);
-    s.dx.a.p = (nk ? s.dw.a.p : s.dw.b.p) = dz;
+    s.dx.a.p = (nk ? s.dw.a.p : s.dw.b.p) = g.terms == 2 ? dz + g.dz / 2 : dz;
     if (a->m) {
       XentParams p = base;
       place_xent(p, s.z, s.cz, nullptr);
+      p.lo = g.terms == 2 ? g.dz / 4 : 0;
       p.out = dz, p.ldo = g.dz_ld, p.column0 = static_cast<int>(column0);
       e = launch_product(p, a->type, XENT_SLOPE, false, s.z.b.mn, s.cz, stream);
     }
