@@ -179,6 +179,7 @@ void check_sizes(Checks &c, int type, int w_order, long long m, long long n, lon
   c.size("n", n);
   c.size("k", k);
   c.need(n != 0, "n = 0: no class");
+  if (c.fine()) c.need(ceil_div(m, 64) * ceil_div(n, 64) < (1LL << 31), m, " rows of ", n, " classes are too many");
 }
 
 struct LossPlan {
@@ -217,6 +218,9 @@ int loss(const tf_linear_xent_args_t *a, hipStream_t stream) {
   if (a->m) c.need(a->target && reinterpret_cast<uintptr_t>(a->target) % 8 == 0, "target is null or not aligned");
   c.vector("lse", a->lse, a->m, TF_T_F32, true);
   c.vector("loss", a->loss, a->m, TF_T_F32, true);
+  c.vector("sum", a->sum, 1, TF_T_F32, false);
+  c.vector("mean", a->mean, 1, TF_T_F32, false);
+  c.vector("count", a->count, 1, TF_T_F32, false);
   if (!c.fine()) return fail(TF_E_ARG, c.wrong);
   LossPlan l = plan_loss(a);
   c.workspace(a->workspace, a->workspace_bytes, l.bytes());

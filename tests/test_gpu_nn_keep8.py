@@ -194,6 +194,22 @@ def test_linear_grad(activation, order, dtype):
                         dtype)
 
 
+@pytest.mark.parametrize("order", [0, 1])
+def test_gradients_of_no_rows(order):
+    nn = _nn()
+    w = torch.ones(40, 24, dtype=torch.bfloat16, device="cuda")
+    wc = w if order == 0 else w.t().contiguous().t()
+    empty = lambda n: torch.empty(0, n, dtype=torch.bfloat16, device="cuda")  # noqa: E731
+    dx, dw, db = nn.linear_grad(empty(24), nn.keep8(empty(40)), wc, nn.keep8(empty(24)), "gelu", torch.float32)
+    assert dx.shape == (0, 40) and (dw == 0).all() and dw.shape == (40, 24) and (db == 0).all()
+    dx, dw = nn.rms_norm_grad(empty(40), nn.keep8(empty(40)), torch.ones(40, device="cuda"))
+    assert dx.shape == (0, 40) and (dw == 0).all()
+    dy = torch.ones(3, 24, dtype=torch.bfloat16, device="cuda")
+    none = torch.empty(3, 0, dtype=torch.bfloat16, device="cuda")
+    dx, dw, db = nn.linear_grad(dy, nn.keep8(none), w[:0], nn.keep8(dy), "relu", torch.float32)
+    assert dx.shape == (3, 0) and dw.shape == (0, 24) and (db == 3).all()
+
+
 def test_large_linear_grad_is_that_of_the_restored():
     """Aligned sizes run the same products: the same bits."""
     nn = _nn()

@@ -390,3 +390,149 @@ def test_streams_and_graphs():
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(out, expected))
         step(*i)
+
+
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("m,n,k", [(1, 70, 64), (2, 4000, 136), (30, 1001, 77), (64, 520, 264)])
+def test_gradients_of_few_rows_round_once(m, n, k, dtype):
+    """Up to 64 rows dz goes in two terms: its rounding (2^-8 or 2^-11) squared is left beside the results' own."""
+    nn = _nn()
+    x, w, target, g = _data(m, n, k, dtype, ignored=0)
+    for order in (0, 1):
+        xc, wc, tc = x.cuda(), _ordered(w, order), target.cuda()
+        lse = nn.linear_cross_entropy(xc, wc, tc, reduction="none", keep=True)[1]
+        dloss = torch.randn(m, generator=g)
+        dx, dw = nn.linear_cross_entropy_grad(dloss.cuda(), xc, wc, tc, lse)
+        xd, wd = x.double(), w.double()
+        z = xd @ wd
+        p = torch.exp(z - torch.logsumexp(z, 1)[:, None])
+        p[torch.arange(m), target] -= 1
+        d = p * dloss.double()[:, None]
+        # dz's error: its second rounding, and what float32 loses of the logits, lse and the exponential (as _check_grad)
+        lost = 2 * (2 * k + 8) * ref.u * (xd.abs() @ wd.abs()) + ref.u * (2 * z.abs() + 144 + n / 4096 + 30)
+        small = 2.0 ** -39 * dloss.abs().max().double() if dtype == torch.float16 else 2.0 ** -133
+        off = (p.abs() + (p < 0)) * lost * dloss.double().abs()[:, None] + 2 * ref.U[dtype] ** 2 * d.abs() + small
+        ref.close(dx, d @ wd.t(), (off + (2 * n + 8) * ref.u * d.abs()) @ wd.abs().t(), dtype)
+        ref.close(dw, xd.t() @ d, xd.abs().t() @ (off + (2 * m + 8) * ref.u * d.abs()), dtype)
+
+
+def test_a_captured_step():
+    """Forward and backward through autograd in one graph, after a warm-up on another stream; replays with other inputs and eager
+    steps of other leaves between them."""
+    nn = _nn()
+    m, n, k = 96, 300, 64
+
+    def step(x, w, t):
+        loss = nn.linear_cross_entropy(x, w, t)
+        return (loss.detach(), *torch.autograd.grad(loss, (x, w)))
+
+    inputs = [[v.cuda() for v in _data(m, n, k, torch.bfloat16, seed=s)[:3]] for s in range(3)]
+    eager = [step(x.clone().requires_grad_(), w.clone().requires_grad_(), t) for x, w, t in inputs]
+    x, w, t = (v.clone() for v in inputs[0])
+    x.requires_grad_(), w.requires_grad_()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            step(x, w, t)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(x, w, t)
+    for (a, b, c), want in zip(inputs, eager):
+        with torch.no_grad():
+            x.copy_(a), w.copy_(b), t.copy_(c)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(out, want))
+        step(a.clone().requires_grad_(), b.clone().requires_grad_(), c)
+
+
+@pytest.mark.parametrize("order", [0, 1])
+def test_far_offsets(order):
+    """Weights of more than 2^31 elements: classes at both ends and around 2^31, in the loss and in dw."""
+    nn = _nn()
+    n, k = (1 << 20) + 40, 2056
+    w = torch.zeros((n, k) if order else (k, n), dtype=torch.bfloat16, device="cuda")
+    at = [0, 1, (1 << 31) // k - 1, (1 << 31) // k, (1 << 31) // k + 1, n // 2, n - 2, n - 1]
+    g = torch.Generator().manual_seed(1)
+    x = _matrix(g, 8, k, torch.bfloat16).cuda()
+    rows = _matrix(g, 8, k, torch.bfloat16, k ** -0.5).cuda()
+    for i, c in enumerate(at):
+        (w if order else w.t())[c] = rows[i]
+    wc = w.t() if order else w
+    target = torch.tensor(at, device="cuda")
+    loss, lse, _ = nn.linear_cross_entropy(x, wc, target, reduction="none", keep=True)
+    z = x.double() @ rows.double().t().contiguous()  # the other classes' logits are 0
+    want = torch.log(torch.exp(z).sum(1) + (n - 8))
+    assert ((lse.double() - want).abs() < 2e-5).all()
+    assert ((loss.double() - (want - z.diagonal())).abs() < 4e-5).all()
+    one = torch.ones(8, device="cuda")
+    dx, dw = nn.linear_cross_entropy_grad(one, x, wc, target, lse)
+    p = torch.exp(z - want[:, None]) - torch.eye(8, dtype=torch.float64, device="cuda")
+    full = p @ rows.double()
+    assert float((dx.double() - full).norm() / full.norm()) < 2.0 ** -8
+    part = p.t().contiguous() @ x.double()
+    cols = dw.t()[target].double()
+    assert float((cols - part).norm() / part.norm()) < 2.0 ** -8
+    other = torch.exp(-want) @ x.double()
+    for c in (2, (1 << 31) // k + 2, n - 3):
+        assert float((dw.t()[c].double() - other).norm() / other.norm()) < 2.0 ** -8
+    del w, wc, dw, dx
+    torch.cuda.empty_cache()
+
+
+def test_a_large_gradient_of_the_logits():
+    """A piece whose gradient of the logits holds more than 2^31 elements: the ends of the rows, and what they add to dw."""
+    nn = _nn()
+    m, n, k = 140000, 16384, 64
+    g = torch.Generator().manual_seed(2)
+    w = _matrix(g, k, n, torch.bfloat16, k ** -0.5).cuda()
+    x = torch.zeros(m, k, dtype=torch.bfloat16, device="cuda")
+    rows = torch.tensor([0, 1, (1 << 31) // n - 1, (1 << 31) // n, (1 << 31) // n + 1, m - 2, m - 1])
+    x[rows] = _matrix(g, len(rows), k, torch.bfloat16).cuda()
+    target = torch.full((m,), IGNORE, device="cuda")
+    target[rows] = torch.tensor([0, 5, 100, 8000, 16000, 16382, 16383], device="cuda")
+    loss, lse, _ = nn.linear_cross_entropy(x, w, target, reduction="none", keep=True)
+    dx, dw = nn.linear_cross_entropy_grad(torch.ones(m, device="cuda"), x, w, target, lse)
+    z = x[rows].double() @ w.double()
+    d = torch.exp(z - torch.logsumexp(z, 1)[:, None])
+    d[torch.arange(len(rows)), target[rows]] -= 1
+    full = d @ w.double().t().contiguous()
+    assert float((dx[rows].double() - full).norm() / full.norm()) < 2.0 ** -8
+    full = x[rows].double().t().contiguous() @ d
+    assert float((dw.double() - full).norm() / full.norm()) < 2.0 ** -8
+    dead = torch.ones(m, dtype=torch.bool, device="cuda")
+    dead[rows] = False
+    assert (dx[dead] == 0).all() and (loss[dead] == 0).all()
+    del dx, dw
+    torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("order", [0, 1])
+def test_operands_far_apart(order):
+    """Rows whose distance puts the last ones past 2^31 elements."""
+    nn = _nn()
+    m, n, k = (70, 300, 66) if order == 0 else (70, 69, 130)
+    x, w, target, g = _data(m, n, k, torch.bfloat16)
+    lines = w if order == 0 else w.t()
+    ld = (1 << 25) + 8
+    memory = torch.empty(70 * ld, dtype=torch.bfloat16, device="cuda")
+    xf = memory.as_strided((m, k), (ld, 1), 0)
+    wf = memory.as_strided(tuple(lines.shape), (ld, 1), 1024)
+    xf.copy_(x), wf.copy_(lines)
+    wc, tc = wf if order == 0 else wf.t(), target.cuda()
+    loss, lse, _ = nn.linear_cross_entropy(xf, wc, tc, reduction="none", keep=True)
+    z, want_lse = _check_loss(loss, lse, x, w, target)
+    dloss = torch.rand(m, generator=g)
+    dx, dw = nn.linear_cross_entropy_grad(dloss.cuda(), xf, wc, tc, lse)
+    _check_grad(dx, dw, dloss, x, w, target, z, want_lse, torch.bfloat16)
+    x8 = nn.keep8(xf)
+    assert torch.equal(x8.data, nn.keep8(x.cuda()).data)
+    dy = _matrix(g, m, n, torch.bfloat16).cuda()
+    got = nn.linear_grad(dy, x8, wc, None)
+    near = nn.linear_grad(dy, x8.restore(), _ordered(w, order), None)
+    for a, b in zip(got[:2], near[:2]):
+        assert float((a.double() - b.double()).norm() / b.double().norm()) < 2.0 ** -8
+    del memory, xf, wf
+    torch.cuda.empty_cache()

@@ -197,7 +197,8 @@ def _xent_grad(**kw):
     (dict(k=(1 << 30) + 1), "k = 1073741825"), (dict(x=0), "x is a null"), (dict(w=0), "w is a null"), (dict(target=0), "target is null"),
     (dict(target=260), "target is null or not aligned"), (dict(loss=0), "loss is a null"), (dict(lse=0), "lse is a null"),
     (dict(x_ld=63), "x: 63"), (dict(w_ld=99), "w: 99"), (dict(w_order=1, w_ld=63), "w: 63"), (dict(workspace=0), "workspace is null"),
-    (dict(workspace=264), "not 16-byte aligned"), (dict(workspace_bytes=16), "are needed"), (dict(x=257), "x is not aligned")])
+    (dict(workspace=264), "not 16-byte aligned"), (dict(sum=258), "sum is not aligned"), (dict(mean=258), "mean is not aligned"),
+    (dict(count=258), "count is not aligned"), (dict(m=1 << 30, n=1 << 27, w_ld=1 << 27), "are too many"), (dict(workspace_bytes=16), "are needed"), (dict(x=257), "x is not aligned")])
 def test_xent_refusals(change, words):
     _refused(_lib.lib().tf_linear_xent(_xent(**change), None), words)
 
