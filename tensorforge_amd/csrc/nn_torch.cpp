@@ -189,15 +189,20 @@ void float_type(const Tensor &x, const char *name) {
                    ", not Float, BFloat16 or Half");
 }
 
-// quantize: False, True (e4m3) or the 8-bit type.
-bool eight_bits(PyObject *o, ScalarType &to) {
-  if (o == Py_False) return false;
-  to = ScalarType::Float8_e4m3fn;
-  if (o == Py_True) return true;
+ScalarType eight_bits(PyObject *o) {
   TORCH_CHECK_TYPE(THPDtype_Check(o), "the 8-bit type is not a dtype");
-  to = reinterpret_cast<THPDtype *>(o)->scalar_type;
+  const ScalarType to = reinterpret_cast<THPDtype *>(o)->scalar_type;
   TORCH_CHECK_TYPE(to == ScalarType::Float8_e4m3fn || to == ScalarType::Char, "8-bit rows are Float8_e4m3fn or Char, not ", to);
-  return true;
+  return to;
+}
+// quantize: false, true (e4m3) or the 8-bit type.
+bool wants_eight_bits(PyObject *o, ScalarType &to) {
+  if (o == Py_False) return false;
+  if (THPDtype_Check(o)) return to = eight_bits(o), true;
+  const int truth = o == Py_True ? 1 : PyObject_IsTrue(o);
+  if (truth < 0) throw python_error();
+  if (truth) to = ScalarType::Float8_e4m3fn;
+  return truth != 0;
 }
 
 // (x, weight, residual, eps, quantize) -> (y, h) or (q, scale, h)
@@ -209,7 +214,7 @@ PyObject *rms_norm(PyObject *, PyObject *const *a, Py_ssize_t n) {
   float_type(x, "x");
   const ScalarType t = x.scalar_type();
   ScalarType to = t;
-  const bool quantize = eight_bits(a[4], to);
+  const bool quantize = wants_eight_bits(a[4], to);
   if (wants_grad({&x, &weight, residual})) Py_RETURN_NONE;
   const Rows xr = rows(x, "x");
   tf_rms_norm_args_t g{};
@@ -238,8 +243,7 @@ PyObject *quantize_rows(PyObject *, PyObject *const *a, Py_ssize_t n) {
   count(n, 2);
   const Tensor &x = tensor(a[0], "x");
   float_type(x, "x");
-  ScalarType to = ScalarType::Float8_e4m3fn;
-  eight_bits(a[1], to);
+  const ScalarType to = eight_bits(a[1]);
   no_gradient("quantize_rows", {&x});
   const Rows r = rows(x, "x");
   on_gpu(x, {});
@@ -309,13 +313,13 @@ PyObject *restore8(PyObject *, PyObject *const *a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-// (dy, h, weight, eps, dh) -> (dx, dweight); h may be what keep8 gave.
+// (dy, h, weight, eps, dh) -> (dx, dweight); kept: h is what keep8 gave.
+template <bool kept>
 PyObject *rms_norm_grad(PyObject *, PyObject *const *a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   count(n, 5);
   const Tensor &dy = tensor(a[0], "dy"), &h = tensor(a[1], "h"), &weight = tensor(a[2], "weight");
   const Tensor *dh = optional(a[4], "dh");
-  const bool kept = h.scalar_type() == ScalarType::Byte;
   if (kept) float_type(dy, "dy");
   else float_type(h, "h");
   no_gradient("rms_norm_grad", {&dy, &h, &weight, dh});
@@ -400,13 +404,14 @@ PyObject *linear(PyObject *, PyObject *const *a, Py_ssize_t n) {
 }
 
 // (dy, x, w, z, act, bias_dtype, want_dx, want_dw, tile, splits, terms) -> (dx, dw, dbias);
-// x and z may be what keep8 gave.
+// some_kept: x and z may be what keep8 gave, bytes.
+template <bool some_kept>
 PyObject *linear_grad(PyObject *, PyObject *const *a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   count(n, 11);
   const Tensor &dy = tensor(a[0], "dy"), &x = tensor(a[1], "x"), &w = tensor(a[2], "w");
   const Tensor *z = optional(a[3], "z");
-  const bool kept = x.scalar_type() == ScalarType::Byte;
+  const bool kept = some_kept && x.scalar_type() == ScalarType::Byte;
   const ScalarType t = kept ? dy.scalar_type() : x.scalar_type();
   TORCH_CHECK_TYPE(half_type(t), kept ? "dy is " : "x is ", t, ", not BFloat16 or Half");
   no_gradient("linear_grad", {&dy, &x, &w, z});
@@ -422,7 +427,7 @@ PyObject *linear_grad(PyObject *, PyObject *const *a, Py_ssize_t n) {
   g.tile = integer(a[8], "tile"), g.splits = integer(a[9], "splits"), g.terms = integer(a[10], "terms");
   if (g.act) {
     TORCH_CHECK_VALUE(z, "an activation's gradient needs z: call linear with keep=True");
-    if (z->scalar_type() == ScalarType::Byte) {
+    if (some_kept && z->scalar_type() == ScalarType::Byte) {
       g.z = kept_rows(*z, "z", xr.m, wr.n), g.kept = TF_KEPT_Z;
     } else {
       const Rows r = rows_of(*z, "z", xr.m, wr.n, t);
@@ -612,9 +617,11 @@ PyMethodDef methods[] = {
     {"keep8", reinterpret_cast<PyCFunction>(keep8), METH_FASTCALL, nullptr},
     {"restore8", reinterpret_cast<PyCFunction>(restore8), METH_FASTCALL, nullptr},
     {"quantize_rows", reinterpret_cast<PyCFunction>(quantize_rows), METH_FASTCALL, nullptr},
-    {"rms_norm_grad", reinterpret_cast<PyCFunction>(rms_norm_grad), METH_FASTCALL, nullptr},
+    {"rms_norm_grad", reinterpret_cast<PyCFunction>(rms_norm_grad<false>), METH_FASTCALL, nullptr},
+    {"rms_norm_grad8", reinterpret_cast<PyCFunction>(rms_norm_grad<true>), METH_FASTCALL, nullptr},
     {"linear", reinterpret_cast<PyCFunction>(linear), METH_FASTCALL, nullptr},
-    {"linear_grad", reinterpret_cast<PyCFunction>(linear_grad), METH_FASTCALL, nullptr},
+    {"linear_grad", reinterpret_cast<PyCFunction>(linear_grad<false>), METH_FASTCALL, nullptr},
+    {"linear_grad8", reinterpret_cast<PyCFunction>(linear_grad<true>), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_nn_torch", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -104,7 +104,7 @@ def keep8(x, positive=False):
 
 def _kept(t, name, like, columns):
     """What the native layer takes for an operand that may be kept in 8 bits."""
-    if isinstance(t, Kept8):
+    if type(t) is Kept8:
         if t.dtype != like.dtype:
             raise TypeError(f"{name} was {t.dtype}, not {like.dtype}")
         if not t.shape or t.shape[-1] != columns:
@@ -116,14 +116,10 @@ def _kept(t, name, like, columns):
 
 
 def _like(dx, x):
-    return dx.view(x.shape) if isinstance(x, Kept8) and dx is not None and dx.shape != x.shape else dx
+    return dx.view(x.shape) if type(x) is Kept8 and dx is not None and dx.shape != x.shape else dx
 
 
 # ---- norm -----------------------------------------------------------------------
-
-
-def _eight_bits(quantize):
-    return quantize if isinstance(quantize, torch.dtype) else True if quantize else False
 
 
 def rms_norm(x, weight, residual=None, eps=1e-6, quantize=False, keep8=False):
@@ -134,7 +130,7 @@ def rms_norm(x, weight, residual=None, eps=1e-6, quantize=False, keep8=False):
     x is float32, bfloat16 or float16, the weight of x's type or float32.  keep8: where the
     result gets a gradient, h is kept for it in 8 bits (Kept8).
     """
-    got = _C.rms_norm(x, weight, residual, eps, _eight_bits(quantize))
+    got = _C.rms_norm(x, weight, residual, eps, quantize)
     if got is not None:
         return got
     if quantize:
@@ -154,9 +150,9 @@ def rms_norm_grad(dy, h, weight, eps=1e-6, dh=None):
     dh: the gradient that reaches h past the norm, added to dx; dx is the residual's gradient too.
     h may be kept in 8 bits (Kept8).
     """
-    if isinstance(h, torch.Tensor) and h.dtype is not torch.uint8:
+    if type(h) is not Kept8:
         return _C.rms_norm_grad(dy, h, weight, eps, dh)
-    dx, dw = _C.rms_norm_grad(dy, _kept(h, "h", dy, dy.shape[-1] if dy.dim() else 0), weight, eps, dh)
+    dx, dw = _C.rms_norm_grad8(dy, _kept(h, "h", dy, dy.shape[-1] if dy.dim() else 0), weight, eps, dh)
     return _like(dx, h), dw
 
 
@@ -234,11 +230,13 @@ def linear_grad(dy, x, w, z=None, activation="none", bias_dtype=None, want_dx=Tr
     left as a second term (terms=2, twice the time); 0 takes two up to 1.4e8 multiply-adds.
     x and z may be kept in 8 bits (Kept8).
     """
-    bytes_x, bytes_z = x, z
-    if isinstance(w, torch.Tensor) and w.dim() == 2 and isinstance(dy, torch.Tensor):
-        bytes_x, bytes_z = _kept(x, "x", dy, w.shape[0]), _kept(z, "z", dy, w.shape[1])
-    dx, dw, dbias = _C.linear_grad(dy, bytes_x, w, bytes_z, _act(activation), bias_dtype, True if want_dx else False,
-                                   True if want_dw else False, tile, splits, terms)
+    if type(x) is not Kept8 and type(z) is not Kept8:
+        return _C.linear_grad(dy, x, w, z, _act(activation), bias_dtype, True if want_dx else False,
+                              True if want_dw else False, tile, splits, terms)
+    if w.dim() != 2:
+        raise ValueError(f"w is {tuple(w.shape)}, not k x n")
+    dx, dw, dbias = _C.linear_grad8(dy, _kept(x, "x", dy, w.shape[0]), w, _kept(z, "z", dy, w.shape[1]), _act(activation), bias_dtype,
+                                    True if want_dx else False, True if want_dw else False, tile, splits, terms)
     return _like(dx, x), dw, dbias
 
 

@@ -139,16 +139,18 @@ def test_kept_python_refusals():
             (lambda: nn.linear_grad(dy, kept(5, 40), w), ValueError, "x, 4 x 40 kept in 8 bits"),
             (lambda: nn.linear_grad(dy, kept(4, 40, torch.float16), w), TypeError, "x was torch.float16"),
             (lambda: nn.linear_grad(half, kept(4, 40), w), TypeError, "x was torch.bfloat16"),
-            (lambda: nn.linear_grad(dy, kept(4, 40).data, w), TypeError, "a tensor of bytes"),
+            (lambda: nn.linear_grad(dy, kept(4, 40).data, w), TypeError, "x is Byte"),
             (lambda: nn.linear_grad(dy, h, w, kept(4, 17), "gelu"), ValueError, "not rows of 16"),
             (lambda: nn.linear_grad(dy, kept(4, 40), w, None, "gelu"), ValueError, "keep=True"),
-            (lambda: nn.linear_grad(dy, kept(4, 40), w[0]), TypeError, "x is not a tensor"),
+            (lambda: nn.linear_grad(dy, kept(4, 40), w[0]), ValueError, "not k x n"),
+            (lambda: nn.linear_grad(dy, kept(4, 40), w, kept(4, 16).data, "gelu"), TypeError, "a tensor of bytes"),
+            (lambda: nn.linear_grad(dy, h, w, kept(4, 16).data, "gelu"), TypeError, "z is Byte"),
             (lambda: nn.linear_grad(dy, kept(4, 40), w.clone().requires_grad_()), ValueError, "no gradient"),
             (lambda: nn.rms_norm_grad(h, kept(4, 40), v), ValueError, "not on a GPU"),
             (lambda: nn.rms_norm_grad(h, kept(4, 33), v), ValueError, "not rows of 40"),
             (lambda: nn.rms_norm_grad(h, kept(3, 40), v), ValueError, "kept in 8 bits"),
             (lambda: nn.rms_norm_grad(h.half(), kept(4, 40), v.half()), TypeError, "h was torch.bfloat16"),
-            (lambda: nn.rms_norm_grad(h, kept(4, 40).data, v), TypeError, "a tensor of bytes")]:
+            (lambda: nn.rms_norm_grad(h, kept(4, 40).data, v), TypeError, "h is Byte")]:
         with pytest.raises(error, match=words):
             call()
 
