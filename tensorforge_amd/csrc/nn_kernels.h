@@ -90,6 +90,9 @@ struct XentParams : GemmParams {
   // multiple of 4) floats.
   float *sum = nullptr;
   int add = 0, last = 0;
+  // The rows are twice as many: of both terms of dz, the value's and then what its rounding left, whose products
+  // go to `parts` for the join to add.
+  int halves = 0;
 };
 enum XentProduct { XENT_STATS, XENT_SLOPE, XENT_SUM };
 // Tiles 256, 128 and 64.  XENT_STATS and XENT_SLOPE: amn false.

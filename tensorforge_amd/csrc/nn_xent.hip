@@ -130,14 +130,21 @@ __global__ __launch_bounds__(1024) void xent_scale_kernel(XentParams p, float *s
   scale[1] = __builtin_bit_cast(float, static_cast<uint32_t>(127 - up) << 23);
 }
 
-// Sum's epilogue for a product in ranges of k; four columns a thread.
+// Sum's epilogue for a product in ranges of k, or of both terms of dz; four columns a thread.
 template <typename T>
 __global__ __launch_bounds__(256) void xent_join_kernel(XentParams p) {
+  const int rows = p.halves ? p.m / 2 : p.m;
   const long quads = (p.n + 3L) / 4, id = block_of() * 256 + threadIdx.x, ld = quads * 4, m = id / quads, n = id % quads * 4;
-  if (m >= p.m) return;
-  const float *part = p.parts + m * ld + n;
-  f32x4 v = *reinterpret_cast<const f32x4 *>(part);
-  for (int s = 1; s < p.splits; ++s) v += *reinterpret_cast<const f32x4 *>(part + s * (p.m * ld));
+  if (m >= rows) return;
+  const auto added = [&](long row) {
+    const float *part = p.parts + row * ld + n;
+    f32x4 v = *reinterpret_cast<const f32x4 *>(part);
+#pragma unroll 4
+    for (int s = 1; s < p.splits; ++s) v += *reinterpret_cast<const f32x4 *>(part + s * (p.m * ld));
+    return v;
+  };
+  f32x4 v = added(m);
+  if (p.halves) v += made_finite(added(rows + m));  // as in gemm_tile
   f32x4 *sum = reinterpret_cast<f32x4 *>(p.sum + m * ld + n);
   if (p.add) v += *sum;
   if (!p.last) {
@@ -149,6 +156,88 @@ __global__ __launch_bounds__(256) void xent_join_kernel(XentParams p) {
 #pragma unroll
   for (int i = 0; i < 4; ++i)
     if (n + i < p.n) out[i] = static_cast<T>(in_unit(v[i], unit));
+}
+
+// The weights' gradient of up to 64 rows of x: out[r][c] = sum over m of R[m][r] * C[m][c], one of
+// both (dz) in two terms.  Bound by writing it.  A workgroup keeps COLUMNS columns of C as fragments in
+// LDS and its waves go down the rows, 16 at a time, R's fragments gathered as they lie (both
+// operands are small and come from the caches).  2 x 59648 x 3436 bfloat16 114 us (410 MB written, 3.6
+// TB/s) where 64 x 64 tiles took 421, 16 x 32000 x 4096 67 (121 on 128 x 128 tiles).
+struct OuterParams {
+  const void *r, *c;
+  long r_ld, c_ld, lo;  // lo: the second term's elements behind dz's
+  int k, rows, columns; // k: x's rows
+};
+template <typename T, bool TWO_R, int KS, int COLUMNS>
+__global__ __launch_bounds__(256) void xent_outer_kernel(OuterParams q, XentParams p) {
+  constexpr int BLOCKS = COLUMNS / 16, TC = TWO_R ? 1 : 2, TR = TWO_R ? 2 : 1;
+  __shared__ __align__(1024) char smem[BLOCKS * KS * TC * 1024 + 4 * 4096];
+  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, l = lane % 16, g = lane / 16;
+  lds_char *frags = (lds_char *)smem, *patch = frags + BLOCKS * KS * TC * 1024 + wave * 4096;
+  // Eight rows of x from 32 * ks + 8 * g on, of one column of its operand.
+  const auto gather = [&](const T *from, long ld, int ks) {
+    typename Vec<T, 8>::type v;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int m = ks * 32 + g * 8 + i;
+      const T e = from[min(m, q.k - 1) * ld];
+      v[i] = m < q.k ? e : static_cast<T>(0.0f);
+    }
+    return __builtin_bit_cast(i32x4, v);
+  };
+  const auto multiply = [&](const i32x4 (&a)[KS], const lds_char *at, f32x4 c) {
+    const i32x4 none = {0, 0, 0, 0};
+    return block_mma(T{}, a[0], KS > 1 ? a[KS - 1] : none, lds_read16(at), KS > 1 ? lds_read16(at + (KS - 1) * 1024) : none, c);
+  };
+  const int c0 = blockIdx.x * COLUMNS;
+  for (int f = wave; f < BLOCKS * TC * KS; f += 4) {
+    const int ks = f % KS, term = f / KS % TC, block = f / KS / TC;
+    const T *from = static_cast<const T *>(q.c) + term * q.lo + min(c0 + block * 16 + l, q.columns - 1);
+    *reinterpret_cast<__attribute__((address_space(3))) i32x4 *>(frags + f * 1024 + lane * 16) = gather(from, q.c_ld, ks);
+  }
+  __syncthreads();
+  const float unit = sum_unit(p);
+  const lds_char *mine = frags + lane * 16;
+  for (int r0 = (blockIdx.y * 4 + wave) * 16; r0 < q.rows; r0 += gridDim.y * 64) {
+    i32x4 a[TR][KS];
+#pragma unroll
+    for (int t = 0; t < TR; ++t)
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) a[t][ks] = gather(static_cast<const T *>(q.r) + t * q.lo + min(r0 + l, q.rows - 1), q.r_ld, ks);
+    for (int b = 0; b < BLOCKS; b += 4) {
+      if (c0 + b * 16 >= q.columns) break;
+      f32x4 acc[1][4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const lds_char *at = mine + (b + j) * (TC * KS * 1024);
+        // What the rounding left first, as in gemm_tile.
+        acc[0][j] = made_finite(multiply(a[TR - 1], at + (TC - 1) * KS * 1024, f32x4{0.0f, 0.0f, 0.0f, 0.0f}));
+        acc[0][j] = multiply(a[0], at, acc[0][j]);
+      }
+      by_rows<16>(acc, patch, [&](int row, int column, float (&v)[8]) {
+        const int r = r0 + row, c = c0 + b * 16 + column, left = q.columns - c;
+        if (r >= q.rows || left <= 0) return;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = in_unit(v[i], unit);
+        store_some(static_cast<T *>(p.out) + r * p.ldo + c, left, v);
+      });
+    }
+  }
+}
+
+template <typename T, bool TWO_R, int COLUMNS>
+void launch_outer_as(const OuterParams &q, const XentParams &p, hipStream_t stream) {
+  // As many workgroups down the rows as keep four on every CU.
+  const long across = (q.columns + COLUMNS - 1L) / COLUMNS, down = std::max(1L, std::min((1024 + across - 1) / across, (q.rows + 63L) / 64));
+  const dim3 grid(static_cast<unsigned>(across), static_cast<unsigned>(down));
+  if (q.k <= 32) xent_outer_kernel<T, TWO_R, 1, COLUMNS><<<grid, 256, 0, stream>>>(q, p);
+  else xent_outer_kernel<T, TWO_R, 2, COLUMNS><<<grid, 256, 0, stream>>>(q, p);
+}
+// 256 columns a workgroup, or 64 where that leaves CUs without one: 61 x 1001 x 333 float16 12.0 us with 256.
+template <typename T, bool TWO_R>
+void launch_outer(const OuterParams &q, const XentParams &p, hipStream_t stream) {
+  const bool few = ((q.columns + 255L) / 256) * ((q.rows + 63L) / 64) < 256;
+  few ? launch_outer_as<T, TWO_R, 64>(q, p, stream) : launch_outer_as<T, TWO_R, 256>(q, p, stream);
 }
 
 hipError_t launch_product(const XentParams &p, int type, XentProduct what, bool amn, bool bmn, const Choice &c, hipStream_t stream) {
@@ -264,6 +353,7 @@ constexpr long kLeastColumns = 16384;
 // Up to so many rows the products take what dz's rounding left as a second term, into the same sums:
 // they are bound by reading w and writing dw, and a class that few rows have would see dz's rounding
 // in its dw (2 x 59648 x 3436 bfloat16: dw 0.0003 off 64 bits in one term, its own rounding 0.00018).
+// dx takes the terms as so many rows more, which share one read of w, and dw has a kernel of its own.
 constexpr long kTwoTermRows = 64;
 
 struct GradPlan {
@@ -296,19 +386,20 @@ Piece piece_of(const GradPlan &g, const tf_linear_xent_grad_args_t *a, long n) {
     o.mn = mn;
     return o;
   };
-  const auto dz_as = [&](bool mn) { return Operand{nullptr, g.dz_ld, m, n, mn, true}; };
+  const int rows = m * g.terms;  // of dz
+  const auto dz_as = [&](bool mn) { return Operand{nullptr, g.dz_ld, mn ? m : rows, n, mn, true}; };
   s.z = {a->type, a->type, x_as(false), w_as(!nk), {}, true};
   s.z.p.m = m, s.z.p.n = static_cast<int>(n), s.z.p.k = k;
   s.dx = {a->type, a->type, dz_as(false), w_as(nk), {}, true};
-  s.dx.p.m = m, s.dx.p.n = k, s.dx.p.k = static_cast<int>(n);
+  s.dx.p.m = rows, s.dx.p.n = k, s.dx.p.k = static_cast<int>(n);
   s.dw = {a->type, a->type, nk ? dz_as(true) : x_as(true), nk ? x_as(true) : dz_as(true), {}, true};
   s.dw.p.m = static_cast<int>(nk ? n : k), s.dw.p.n = static_cast<int>(nk ? k : n), s.dw.p.k = m;
-  if (g.terms == 2) {  // what the rounding left lies behind, and comes first
-    s.dx.p.terms = s.dw.p.terms = 2;
-    s.dx.p.a_term = (nk ? s.dw.p.a_term : s.dw.p.b_term) = -(g.dz / 2);
-  }
   if (m) s.cz = choose(s.z, 0, 1, false), s.cdx = choose(s.dx, 0, 0, false);
-  s.cdw = choose(s.dw, 0, 0, false);
+  if (m && g.terms == 2) {
+    s.cdx.parts = round16(4LL * s.cdx.plan.splits * rows * ((k + 3) & ~3L));
+  } else {
+    s.cdw = choose(s.dw, 0, 0, false);
+  }
   return s;
 }
 
@@ -330,7 +421,7 @@ GradPlan plan_grad(const tf_linear_xent_grad_args_t *a) {
     if (g.copy_w) g.w.ld = packed_ld(g.w, 2), g.w.ours = true;
   }
   g.scale = a->type == TF_T_F16 && a->dloss_rows && m ? 16 : 0;
-  g.terms = m <= kTwoTermRows ? 2 : 1;
+  g.terms = m && m <= kTwoTermRows ? 2 : 1;
   g.dz = round16(2 * m * g.dz_ld) * g.terms;
   g.sum = a->dx && g.pieces > 1 ? round16(4 * m * ((k + 3) & ~3L)) : 0;
   for (const long width : {g.width, n - (g.pieces - 1) * g.width}) {
@@ -357,8 +448,8 @@ int grad_workspace(const tf_linear_xent_grad_args_t *a, long long *bytes) {
 hipError_t run_sum(XentParams p, Product &q, const Choice &c, int type, void *parts, hipStream_t stream) {
   place_xent(p, q, c, parts);
   hipError_t e = launch_product(p, type, XENT_SUM, q.a.mn, q.b.mn, c, stream);
-  if (e != hipSuccess || p.splits == 1) return e;
-  const dim3 grid = grid_of((p.m * ((p.n + 3L) / 4) + 255) / 256, 256);
+  if (e != hipSuccess || (p.splits == 1 && !p.halves)) return e;
+  const dim3 grid = grid_of(((p.halves ? p.m / 2 : p.m) * ((p.n + 3L) / 4) + 255) / 256, 256);
   type == TF_T_BF16 ? xent_join_kernel<bf16><<<grid, 256, 0, stream>>>(p) : xent_join_kernel<f16><<<grid, 256, 0, stream>>>(p);
   return hipGetLastError();
 }
@@ -410,16 +501,17 @@ int grad(const tf_linear_xent_grad_args_t *a, hipStream_t stream) {
     Piece s = piece_of(g, a, n);
     const auto from_column = [&](const void *w, long ld) { return static_cast<const char *>(w) + 2 * column0 * (nk ? ld : 1); };
     s.z.b.p = s.dx.b.p = from_column(g.w.p, g.w.ld);
-    s.dx.a.p = (nk ? s.dw.a.p : s.dw.b.p) = g.terms == 2 ? dz + g.dz / 2 : dz;
+    s.dx.a.p = (nk ? s.dw.a.p : s.dw.b.p) = dz;
     if (a->m) {
       XentParams p = base;
       place_xent(p, s.z, s.cz, nullptr);
-      p.lo = g.terms == 2 ? g.dz / 4 : 0;
+      p.lo = g.terms == 2 ? a->m * g.dz_ld : 0;
       p.out = dz, p.ldo = g.dz_ld, p.column0 = static_cast<int>(column0);
       e = launch_product(p, a->type, XENT_SLOPE, false, s.z.b.mn, s.cz, stream);
     }
     if (e == hipSuccess && a->dx && a->m) {
       XentParams p = base;
+      p.halves = g.terms == 2;
       p.sum = reinterpret_cast<float *>(sum), p.add = i > 0, p.last = i + 1 == g.pieces;
       s.dx.p.out = a->dx, s.dx.p.ldo = a->dx_ld;
       e = run_sum(p, s.dx, s.cdx, a->type, parts, stream);
@@ -428,7 +520,15 @@ int grad(const tf_linear_xent_grad_args_t *a, hipStream_t stream) {
       XentParams p = base;
       p.last = 1;
       s.dw.p.out = const_cast<char *>(from_column(a->dw, a->dw_ld)), s.dw.p.ldo = a->dw_ld;
-      e = run_sum(p, s.dw, s.cdw, a->type, parts, stream);
+      if (g.terms == 2) {
+        const OuterParams q{s.dw.a.p, s.dw.b.p, s.dw.a.ld, s.dw.b.ld, a->m * g.dz_ld, static_cast<int>(a->m), s.dw.p.m, s.dw.p.n};
+        p.out = s.dw.p.out, p.ldo = a->dw_ld;
+        if (a->type == TF_T_BF16) nk ? launch_outer<bf16, true>(q, p, stream) : launch_outer<bf16, false>(q, p, stream);
+        else nk ? launch_outer<f16, true>(q, p, stream) : launch_outer<f16, false>(q, p, stream);
+        e = hipGetLastError();
+      } else {
+        e = run_sum(p, s.dw, s.cdw, a->type, parts, stream);
+      }
     }
   }
   return hip(e, call);

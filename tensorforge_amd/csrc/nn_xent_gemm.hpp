@@ -212,7 +212,7 @@ struct Sum {
     by_rows<ROWS>(acc, patch, [&](int row, int column, float (&v)[8]) {
       const int m = mw + row, n = nw + column, left = p.n - n;
       if (m >= p.m || m < tm * BM || left <= 0 || n + 7 < nt) return;
-      if (p.splits > 1) {
+      if (p.splits > 1 || p.halves) {
         store_some(part + m * ld + n, left, v);
         return;
       }
@@ -237,11 +237,11 @@ struct Sum {
   }
 };
 
-template <typename T, typename E, bool AMN, bool BMN, int BM, int ST, bool DMA, int TERMS>
+template <typename T, typename E, bool AMN, bool BMN, int BM, int ST, bool DMA>
 __global__ __launch_bounds__(256, DMA ? 1 : 3) void xent_tile_kernel(XentParams p) {
   __shared__ __align__(1024) char smem[tile_lds<BM, BM, ST>()];
   const int block = static_cast<int>(block_of()), blocks = p.tiles_m * p.tiles_n * p.splits;
-  if (block < blocks) gemm_tile<T, T, AMN, BMN, BM, BM, 2, 2, ST, DMA, TERMS, E>(p, block, blocks, (lds_char *)smem);
+  if (block < blocks) gemm_tile<T, T, AMN, BMN, BM, BM, 2, 2, ST, DMA, 1, E>(p, block, blocks, (lds_char *)smem);
 }
 template <typename T, typename E, bool AMN, bool BMN>
 __global__ __launch_bounds__(512, 2) void xent_wide_kernel(XentParams p) {
@@ -249,27 +249,14 @@ __global__ __launch_bounds__(512, 2) void xent_wide_kernel(XentParams p) {
   gemm_wide<T, T, AMN, BMN, E>(p, (lds_char *)smem);
 }
 
-template <typename T, typename E, bool AMN, bool BMN, int TERMS>
-void launch_xent_tile(const XentParams &p, int tile, bool dma, hipStream_t stream) {
-  const dim3 grid = grid_of(static_cast<long>(p.tiles_m) * p.tiles_n * p.splits, 256);
-  if (!dma) xent_tile_kernel<T, E, AMN, BMN, 64, 2, false, TERMS><<<grid, 256, 0, stream>>>(p);
-  else if (tile == TILE_128) xent_tile_kernel<T, E, AMN, BMN, 128, 2, true, TERMS><<<grid, 256, 0, stream>>>(p);
-  else xent_tile_kernel<T, E, AMN, BMN, 64, 3, true, TERMS><<<grid, 256, 0, stream>>>(p);
-}
-
 template <typename T, typename E, bool AMN, bool BMN>
 hipError_t launch_xent_as(const XentParams &p, int tile, bool dma, hipStream_t stream) {
-  if (tile == TILE_256) {  // loads straight into LDS, one term
-    xent_wide_kernel<T, E, AMN, BMN><<<dim3(static_cast<unsigned>(p.tiles_m) * p.tiles_n * p.splits), 512, 0, stream>>>(p);
-    return hipGetLastError();
-  }
-  if constexpr (__is_same(E, Sum)) {
-    if (p.terms == 2) {
-      launch_xent_tile<T, E, AMN, BMN, 2>(p, tile, dma, stream);
-      return hipGetLastError();
-    }
-  }
-  launch_xent_tile<T, E, AMN, BMN, 1>(p, tile, dma, stream);
+  const long blocks = static_cast<long>(p.tiles_m) * p.tiles_n * p.splits;
+  const dim3 grid = grid_of(blocks, 256);
+  if (!dma) xent_tile_kernel<T, E, AMN, BMN, 64, 2, false><<<grid, 256, 0, stream>>>(p);
+  else if (tile == TILE_256) xent_wide_kernel<T, E, AMN, BMN><<<dim3(static_cast<unsigned>(blocks)), 512, 0, stream>>>(p);
+  else if (tile == TILE_128) xent_tile_kernel<T, E, AMN, BMN, 128, 2, true><<<grid, 256, 0, stream>>>(p);
+  else xent_tile_kernel<T, E, AMN, BMN, 64, 3, true><<<grid, 256, 0, stream>>>(p);
   return hipGetLastError();
 }
 
