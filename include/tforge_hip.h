@@ -473,7 +473,7 @@ typedef struct {
   int dloss_rows;          /* 0 or 1                                                */
   int reserved;            /* 0                                                     */
 } tf_linear_xent_grad_args_t;
-/* A piece's dz of up to 512 MB (or 16384 columns), float32 sums of dx where there is
+/* A piece's dz of up to 128 MB (or 8192 columns), float32 sums of dx where there is
  * more than one piece, parts of split products, aligned copies. */
 int tf_linear_xent_grad_workspace(const tf_linear_xent_grad_args_t *args, long long *bytes);
 int tf_linear_xent_grad(const tf_linear_xent_grad_args_t *args, void *stream);

@@ -41,8 +41,8 @@ __device__ __forceinline__ void write_totals(const RowsParams &p, float sum, flo
 }
 
 // R rows a workgroup, 1024/R threads a row that share the parts, kBatch of them under way at a
-// time.  One workgroup of all rows adds up the losses too.  Bound by latency: few rows take many
-// threads each (16 rows of 500 parts 7.2 us with 64 rows' places).
+// time.  One workgroup of all rows adds up the losses too.  Bound by latency: 16 rows of 500 parts
+// 4.2 us.
 template <int R>
 __global__ __launch_bounds__(1024) void xent_rows_kernel(RowsParams p) {
   constexpr int LANES = 1024 / R, kBatch = 8;
@@ -94,8 +94,9 @@ __global__ __launch_bounds__(1024) void xent_rows_kernel(RowsParams p) {
     write_totals(p, loss, counts);
   }
 }
-// Rows a workgroup: 16 as long as there are workgroups for all CUs, or one for all rows.
-constexpr int xent_rows(long m) { return m <= 16 || (m > 64 && m < 4096) ? 16 : 64; }
+// 16 rows a workgroup (with 64: 64 x 32000 12.3 us against 9.6 with the product, 1024 x 32000 33.8 and 33.0), but 64 where
+// that makes one workgroup of all and spares the totals' launch.
+bool one_group(long m, bool totals) { return m <= 16 || (m <= 64 && totals); }
 
 __global__ __launch_bounds__(1024) void xent_totals_kernel(RowsParams p) {
   __shared__ float sums[16];
@@ -314,6 +315,7 @@ int loss(const tf_linear_xent_args_t *a, hipStream_t stream) {
   LossPlan l = plan_loss(a);
   c.workspace(a->workspace, a->workspace_bytes, l.bytes());
   if (!c.fine()) return fail(TF_E_ARG, c.wrong);
+  const bool totals = a->sum || a->mean || a->count;
   char *ws = static_cast<char *>(a->workspace);
   RowsParams r{reinterpret_cast<float *>(ws), reinterpret_cast<float *>(ws + l.stats), a->target, a->ignore, a->lse, a->loss, a->sum, a->mean,
                a->count, static_cast<int>(a->m), static_cast<int>(a->n), 0};
@@ -331,12 +333,12 @@ int loss(const tf_linear_xent_args_t *a, hipStream_t stream) {
     if (e == hipSuccess) e = launch_product(p, a->type, XENT_STATS, false, l.q.b.mn, l.c, stream);
     r.parts = p.tiles_n;
     if (e == hipSuccess) {
-      if (xent_rows(a->m) == 16) xent_rows_kernel<16><<<grid_of((a->m + 15) / 16, 1024), 1024, 0, stream>>>(r);
+      if (a->m <= 16 || !one_group(a->m, totals)) xent_rows_kernel<16><<<grid_of((a->m + 15) / 16, 1024), 1024, 0, stream>>>(r);
       else xent_rows_kernel<64><<<grid_of((a->m + 63) / 64, 1024), 1024, 0, stream>>>(r);
       e = hipGetLastError();
     }
   }
-  if (e == hipSuccess && (a->sum || a->mean || a->count) && (a->m == 0 || a->m > 64)) {
+  if (e == hipSuccess && totals && (a->m == 0 || !one_group(a->m, totals))) {
     xent_totals_kernel<<<1, 1024, 0, stream>>>(r);
     e = hipGetLastError();
   }
@@ -346,9 +348,11 @@ int loss(const tf_linear_xent_args_t *a, hipStream_t stream) {
 // ---- its gradient ---------------------------------------------------------------
 
 // The vocabulary goes in pieces of equal width, multiples of 256, whose gradient of the logits takes up
-// to kPiece bytes, but at least kLeastColumns wide: dx's sums are read and written once a piece.
-constexpr long long kPieceBytes = 512 << 20;
-constexpr long kLeastColumns = 16384;
+// to kPieceBytes, but at least kLeastColumns wide: dx's sums are read and written once a piece.  us, bfloat16:
+// 8192 x 65536 x 2048 in pieces of 64 / 128 / 512 MB 5711 / 5321 / 5374, 65536 x 65536 x 1024 in
+// pieces of 4096 / 8192 / 16384 columns 23990 / 22980 / 22840.
+constexpr long long kPieceBytes = 128 << 20;
+constexpr long kLeastColumns = 8192;
 
 // Up to so many rows the products take what dz's rounding left as a second term, into the same sums:
 // they are bound by reading w and writing dw, and a class that few rows have would see dz's rounding

@@ -485,11 +485,11 @@ def test_far_offsets(order):
 def test_a_large_gradient_of_the_logits():
     """A piece whose gradient of the logits holds more than 2^31 elements: the ends of the rows, and what they add to dw."""
     nn = _nn()
-    m, n, k = 140000, 16384, 64
+    m, n, k = 270000, 16384, 64  # two pieces of 8192 classes
     g = torch.Generator().manual_seed(2)
     w = _matrix(g, k, n, torch.bfloat16, k ** -0.5).cuda()
     x = torch.zeros(m, k, dtype=torch.bfloat16, device="cuda")
-    rows = torch.tensor([0, 1, (1 << 31) // n - 1, (1 << 31) // n, (1 << 31) // n + 1, m - 2, m - 1])
+    rows = torch.tensor([0, 1, (1 << 31) // 8192 - 1, (1 << 31) // 8192, (1 << 31) // 8192 + 1, m - 2, m - 1])
     x[rows] = _matrix(g, len(rows), k, torch.bfloat16).cuda()
     target = torch.full((m,), IGNORE, device="cuda")
     target[rows] = torch.tensor([0, 5, 100, 8000, 16000, 16382, 16383], device="cuda")
