@@ -329,7 +329,7 @@ int tf_restore8(const void *kept, long long rows, long long d, int type, void *x
 /* Which operands of a gradient are kept in 8 bits (their *_ld does not count). */
 #define TF_KEPT_H 1 /* tf_rms_norm_grad's h        */
 #define TF_KEPT_X 1 /* tf_linear_grad's x          */
-#define TF_KEPT_Z 2 /* tf_linear_grad's z          */
+#define TF_KEPT_Z 2 /* tf_linear_grad's z, tf_linear's */
 
 /* tf_rms_norm's gradient.  r = 1/sqrt(mean(h^2) + eps), xhat = h*r:
  *   dx = r*(dy*weight - xhat*mean(dy*weight*xhat)) + dh     (also the residual's)
@@ -385,7 +385,9 @@ typedef struct {
                     up to 64 rows, k split over a workgroup's waves, 5: 64x128; one that
                     cannot run these operands gives way to the choice by sizes       */
   int splits;    /* ranges of k: 0 by the sizes, or 1..64                            */
-  int reserved;  /* 0                                                                */
+  int kept;      /* 0, or TF_KEPT_Z: z is written in 8 bits, as tf_keep8 of the z in
+                    out_type would (relu's with `positive`); not of 8-bit products,
+                    and the workspace has to be whole                                */
 } tf_linear_args_t;
 /* Bytes of workspace for these arguments: sizes, types, distances and the
  * alignment of x and w count, the memory is not touched. */

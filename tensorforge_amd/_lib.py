@@ -68,7 +68,7 @@ class LinearArgs(ctypes.Structure):
                [(f, ctypes.c_longlong) for f in ("workspace_bytes", "x_ld", "w_ld", "residual_ld", "out_ld", "z_ld",
                                                  "m", "n", "k")] + \
                [(f, ctypes.c_int) for f in ("w_order", "type", "out_type", "bias_type", "act", "tile", "splits",
-                                            "reserved")]
+                                            "kept")]
 
 
 class LinearGradArgs(ctypes.Structure):

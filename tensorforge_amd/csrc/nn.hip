@@ -100,6 +100,8 @@ void check_linear_sizes(Checks &c, const tf_linear_args_t *a) {
   c.size("m", a->m);
   c.size("n", a->n);
   c.size("k", a->k);
+  c.one_of("kept", a->kept, {0, TF_KEPT_Z});
+  c.need(!a->kept || !eight_bits(a->type), "8-bit products do not keep z in 8 bits");
   c.need(a->type != TF_T_I8 || a->k <= kMostI8, "k = ", a->k, ": sums of more than ", kMostI8, " products of 8-bit integers pass 32 bits");
   check_choice(c, a->tile, a->splits);
 }
@@ -116,12 +118,21 @@ Product product_of(const tf_linear_args_t *a) {
   return q;
 }
 
+// z kept in 8 bits: the bytes of the z in 16 that a product writes first where it cannot write the
+// codes itself (split, few rows, loads through registers).
+long long z_bytes(const tf_linear_args_t *a, const Choice &c) { return a->kept && !fused_z(c) ? round16(2 * a->m * a->n) : 0; }
+
 int linear_workspace(const tf_linear_args_t *a, long long *bytes) {
   if (!a || !bytes) return fail(TF_E_ARG, "tf_linear_workspace: null arguments");
   Checks c{"tf_linear_workspace", {}};
   check_linear_sizes(c, a);
   if (!c.fine()) return fail(TF_E_ARG, c.wrong);
-  *bytes = a->m && a->n ? choose(product_of(a), a->tile, a->splits).bytes() : 0;
+  if (a->m && a->n) {
+    const Choice plan = choose(product_of(a), a->tile, a->splits);
+    *bytes = plan.bytes() + z_bytes(a, plan);
+  } else {
+    *bytes = 0;
+  }
   return TF_OK;
 }
 
@@ -141,7 +152,8 @@ int linear(const tf_linear_args_t *a, hipStream_t stream) {
   c.vector("bias", a->bias, a->n, a->bias_type, false);
   c.matrix("residual", a->residual, a->residual_ld, a->m, a->n, a->out_type, false);
   c.matrix("out", a->out, a->out_ld, a->m, a->n, a->out_type, true);
-  c.matrix("z", a->z, a->z_ld, a->m, a->n, a->out_type, false);
+  if (a->kept) c.kept("z", a->z, a->m, a->n, true);
+  else c.matrix("z", a->z, a->z_ld, a->m, a->n, a->out_type, false);
   c.vector("x_scale", a->x_scale, a->m, TF_T_F32, eight);
   c.vector("w_scale", a->w_scale, a->n, TF_T_F32, eight);
   c.need(eight || (!a->x_scale && !a->w_scale), "scales belong to 8-bit products");
@@ -149,7 +161,17 @@ int linear(const tf_linear_args_t *a, hipStream_t stream) {
   if (!c.fine()) return fail(TF_E_ARG, c.wrong);
   if (a->m == 0 || a->n == 0) return TF_OK;
   Product q = product_of(a);
-  return hip(run_product(q, a->tile, a->splits, a->workspace, a->workspace_bytes, stream), call);
+  if (!a->kept) return hip(run_product(q, a->tile, a->splits, a->workspace, a->workspace_bytes, stream), call);
+  const Choice plan = choose(q, a->tile, a->splits);
+  const long long z16 = z_bytes(a, plan);
+  c.workspace(a->workspace, a->workspace_bytes, plan.bytes() + z16);
+  if (!c.fine()) return fail(TF_E_ARG, c.wrong);
+  char *ws = static_cast<char *>(a->workspace);
+  q.p.z = z16 ? ws + plan.bytes() : nullptr, q.p.ldz = a->n;
+  hipError_t e = run_product(q, a->tile, a->splits, ws, plan.bytes(), stream, z16 ? nullptr : a->z);
+  if (e == hipSuccess && z16)
+    e = launch_keep(ws + plan.bytes(), a->n, a->m, static_cast<int>(a->n), a->type, a->act == TF_ACT_RELU, a->z, stream);
+  return hip(e, call);
 }
 
 // How a gradient runs: the workspace's parts and the products.

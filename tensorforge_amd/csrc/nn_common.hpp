@@ -266,6 +266,28 @@ __device__ __forceinline__ void restore_codes(u32x2 codes, uint32_t exponent, fl
     v[i] = (static_cast<float>(((i < 4 ? codes.x : codes.y) ^ 0x80808080u) >> (8 * (i & 3)) & 255u) - 128.0f) * unit;
 }
 
+// The largest of four neighbouring lanes.
+__device__ __forceinline__ uint32_t quad_max(uint32_t v) {
+  v = max(v, static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(static_cast<int>(v), 0xb1, 0xf, 0xf, true)));  // lanes 1 0 3 2
+  return max(v, static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(static_cast<int>(v), 0x4e, 0xf, 0xf, true)));  // lanes 2 3 0 1
+}
+
+// The codes of a lane's 8 values; four neighbouring lanes hold a group, whose exponent each gets.
+__device__ __forceinline__ u32x2 group_codes(const float (&v)[8], bool positive, uint32_t &exponent) {
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) top = max(top, __builtin_bit_cast(uint32_t, v[i]) & 0x7fffffffu);
+  exponent = group_exponent(quad_max(top));
+  const float inverse = __builtin_bit_cast(float, (254u - min(exponent, 253u)) << 23);
+  float t[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    t[i] = v[i] * inverse;
+    if (positive && v[i] > 0.0f) t[i] = __builtin_fmaxf(t[i], 1.0f);
+  }
+  return exponent == 255 ? u32x2{0, 0} : u32x2{round_to_bytes(t[0], t[1], t[2], t[3]), round_to_bytes(t[4], t[5], t[6], t[7])};
+}
+
 // 8 values from c (a multiple of 8) of a row; zeros past its last group.
 __device__ __forceinline__ void load_kept8(const Kept &k, long row, int c, float (&v)[8]) {
   const long length = k.groups * kGroup, at = min(static_cast<long>(c), length - 8);

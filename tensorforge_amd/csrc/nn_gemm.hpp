@@ -399,6 +399,37 @@ __device__ __forceinline__ uint32_t patch_at(int row, int quad) {
   return row * (COLS * 4) + ((quad ^ (row & (COLS / 4 - 1))) << 4);
 }
 
+__device__ __forceinline__ void wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+
+// The blocks reach memory by rows through the wave's patch of LDS (nn_gemm.hpp), ROWS at a
+// time: put(row, column, eight values), both from the wave's first.
+template <int ROWS, int MI, int NI, typename F>
+__device__ __forceinline__ void by_rows(const f32x4 (&acc)[MI][NI], lds_char *patch, F &&put) {
+  constexpr int COLS = NI * 16, LANES = COLS / 8;
+  const int lane = threadIdx.x % 64, c = lane % LANES;
+#pragma unroll
+  for (int h = 0; h < MI * 16 / ROWS; ++h) {
+#pragma unroll
+    for (int i = 0; i < ROWS / 16; ++i)
+#pragma unroll
+      for (int j = 0; j < NI; ++j)
+        *reinterpret_cast<__attribute__((address_space(3))) f32x4 *>(patch + patch_at<COLS>(i * 16 + lane % 16, j * 4 + lane / 16)) =
+            acc[h * (ROWS / 16) + i][j];
+    wait_lds();
+#pragma unroll 4
+    for (int row = lane / LANES; row < ROWS; row += 64 / LANES) {
+      float v[8];
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        const f32x4 u = __builtin_bit_cast(f32x4, lds_read16(patch + patch_at<COLS>(row, c * 2 + q)));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[q * 4 + i] = u[i];
+      }
+      put(h * ROWS + row, c * 8, v);
+    }
+  }
+}
+
 // (m0, n0): the patch's place in C.  (mt, nt): the workgroup's own first row and
 // column; where its tile was moved back into the matrix, what lies before them is
 // another's (eight columns across nt are written by both, with the same values).
@@ -469,7 +500,6 @@ __device__ __forceinline__ void tile_of(const GemmParams &p, int id, int total, 
   tn = t / rows;
 }
 
-__device__ __forceinline__ void wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void wait_loads() {
   asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");

@@ -11,12 +11,6 @@ namespace {
 
 constexpr int kUnroll = 4;
 
-// The largest of four neighbouring lanes.
-__device__ __forceinline__ uint32_t quad_max(uint32_t v) {
-  v = max(v, static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(static_cast<int>(v), 0xb1, 0xf, 0xf, true)));  // lanes 1 0 3 2
-  return max(v, static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(static_cast<int>(v), 0x4e, 0xf, 0xf, true)));  // lanes 2 3 0 1
-}
-
 // Piece `id` of 8 elements: its row and its first element there.  FLAT: the rows follow each
 // other without gaps, whole groups each, and are one.
 template <bool FLAT>
@@ -56,18 +50,8 @@ __global__ __launch_bounds__(256) void keep_kernel(const T *x, long ld, int d, l
 #pragma unroll
   for (int u = 0; u < kUnroll; ++u) {
     const long id = first + u * 256;
-    uint32_t top = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) top = max(top, __builtin_bit_cast(uint32_t, v[u][i]) & 0x7fffffffu);
-    const uint32_t e = group_exponent(quad_max(top));
-    const float inverse = __builtin_bit_cast(float, (254u - min(e, 253u)) << 23);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float t = v[u][i] * inverse;
-      v[u][i] = positive && v[u][i] > 0.0f ? __builtin_fmaxf(t, 1.0f) : t;
-    }
-    u32x2 c = {round_to_bytes(v[u][0], v[u][1], v[u][2], v[u][3]), round_to_bytes(v[u][4], v[u][5], v[u][6], v[u][7])};
-    if (e == 255) c = u32x2{0, 0};
+    uint32_t e;
+    const u32x2 c = group_codes(v[u], positive, e);
     if (id >= all) continue;
     *reinterpret_cast<u32x2 *>(codes + id * 8) = c;
     if (threadIdx.x % 4 == 0) exponents[id / 4] = static_cast<uint8_t>(e);

@@ -69,6 +69,14 @@ struct ShareParams {
 hipError_t launch_gemm_pair_bf16(const GemmParams &dx, bool bmn, const GemmParams &dw, const ShareParams &sum, hipStream_t stream);
 hipError_t launch_gemm_pair_f16(const GemmParams &dx, bool bmn, const GemmParams &dw, const ShareParams &sum, hipStream_t stream);
 
+// A product that keeps z in 8 bits: rows of `groups` groups.
+struct KeptGemmParams : GemmParams {
+  unsigned char *codes = nullptr, *exponents = nullptr;
+  long groups = 0;
+};
+// All tiles but the few rows', unsplit, loads straight into LDS; z is null.
+hipError_t launch_gemm_kept(const KeptGemmParams &p, int type, bool bmn, int tile, hipStream_t stream);
+
 // The products of the loss over a vocabulary and of its gradient.  The loss of row m is
 // lse[m] - logit(m, target[m]); a row whose target is `ignore` does not count, one whose
 // target is outside of the vocabulary is NaN.

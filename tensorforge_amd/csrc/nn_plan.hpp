@@ -283,7 +283,10 @@ inline long long copy_of(Operand &o, int size, char *to, PackParams &pack) {
   return bytes;
 }
 
-inline hipError_t run_product(Product &q, int tile, int splits, void *workspace, long long bytes, hipStream_t stream) {
+// z, in 8 bits, where it is written with the product (fused_z), else null.
+inline bool fused_z(const Choice &c) { return c.dma && c.plan.splits == 1 && c.plan.tile != TILE_ROWS; }
+
+inline hipError_t run_product(Product &q, int tile, int splits, void *workspace, long long bytes, hipStream_t stream, void *z8 = nullptr) {
   const int size = size_of(q.type);
   Choice c = choose(q, tile, splits);
   if (c.bytes() > bytes) c = choose(q, tile, 1, false);
@@ -297,6 +300,13 @@ inline hipError_t run_product(Product &q, int tile, int splits, void *workspace,
     if (e != hipSuccess) return e;
   }
   place(q, c.plan, workspace);
+  if (z8) {
+    KeptGemmParams p;
+    static_cast<GemmParams &>(p) = q.p;
+    p.groups = ceil_div(p.n, 32);
+    p.codes = static_cast<unsigned char *>(z8), p.exponents = p.codes + p.m * p.groups * 32;
+    return launch_gemm_kept(p, q.type, q.b.mn, c.plan.tile, stream);
+  }
   e = q.type == TF_T_BF16  ? launch_gemm_bf16(q.p, q.a.mn, q.b.mn, c.plan.tile, c.dma, stream)
       : q.type == TF_T_F16 ? launch_gemm_f16(q.p, q.a.mn, q.b.mn, c.plan.tile, c.dma, stream)
       : q.type == TF_T_F8  ? launch_gemm_f8(q.p, q.out_type, c.plan.tile, c.dma, stream)

@@ -347,17 +347,19 @@ PyObject *rms_norm_grad(PyObject *, PyObject *const *a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-// (x, w, bias, act, residual, keep, x_scale, w_scale, out_dtype, tile, splits) -> out or (out, z)
+// (x, w, bias, act, residual, keep, x_scale, w_scale, out_dtype, tile, splits) -> out or (out, z);
+// kept: (out, z's bytes in 8 bits).
+template <bool kept>
 PyObject *linear(PyObject *, PyObject *const *a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   count(n, 11);
   const Tensor &x = tensor(a[0], "x"), &w = tensor(a[1], "w");
   const Tensor *bias = optional(a[2], "bias"), *residual = optional(a[4], "residual");
   const Tensor *xs = optional(a[6], "x_scale"), *ws = optional(a[7], "w_scale");
-  const bool keep = a[5] == Py_True;
+  const bool keep = kept || a[5] == Py_True;
   const ScalarType t = x.scalar_type();
   const bool eight = t == ScalarType::Float8_e4m3fn || t == ScalarType::Char;
-  TORCH_CHECK_TYPE(half_type(t) || eight, "x is ", t, ", not BFloat16, Half, Float8_e4m3fn or Char");
+  TORCH_CHECK_TYPE(half_type(t) || (eight && !kept), "x is ", t, ", not BFloat16, Half, Float8_e4m3fn or Char");
   ScalarType to = eight ? ScalarType::BFloat16 : t;
   if (a[8] != Py_None) {
     TORCH_CHECK_TYPE(THPDtype_Check(a[8]), "out_dtype is not a dtype");
@@ -392,7 +394,8 @@ PyObject *linear(PyObject *, PyObject *const *a, Py_ssize_t n) {
   const auto size = with_last(x, wr.n);
   Tensor out = fresh(x, size, to), z, space;
   g.out = out.data_ptr(), g.out_ld = g.z_ld = wr.n;
-  if (keep) z = fresh(x, size, to), g.z = z.data_ptr();
+  if (kept) z = fresh(x, {kept_bytes(xr.m, wr.n)}, ScalarType::Byte), g.z = z.data_ptr(), g.kept = TF_KEPT_Z;
+  else if (keep) z = fresh(x, size, to), g.z = z.data_ptr();
   check(tf_linear_workspace(&g, &g.workspace_bytes));
   if (g.workspace_bytes) {
     space = fresh(x, {static_cast<int64_t>(g.workspace_bytes)}, ScalarType::Byte);
@@ -619,7 +622,8 @@ PyMethodDef methods[] = {
     {"quantize_rows", reinterpret_cast<PyCFunction>(quantize_rows), METH_FASTCALL, nullptr},
     {"rms_norm_grad", reinterpret_cast<PyCFunction>(rms_norm_grad<false>), METH_FASTCALL, nullptr},
     {"rms_norm_grad8", reinterpret_cast<PyCFunction>(rms_norm_grad<true>), METH_FASTCALL, nullptr},
-    {"linear", reinterpret_cast<PyCFunction>(linear), METH_FASTCALL, nullptr},
+    {"linear", reinterpret_cast<PyCFunction>(linear<false>), METH_FASTCALL, nullptr},
+    {"linear_keep8", reinterpret_cast<PyCFunction>(linear<true>), METH_FASTCALL, nullptr},
     {"linear_grad", reinterpret_cast<PyCFunction>(linear_grad<false>), METH_FASTCALL, nullptr},
     {"linear_grad8", reinterpret_cast<PyCFunction>(linear_grad<true>), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};

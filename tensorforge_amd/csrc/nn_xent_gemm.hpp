@@ -12,35 +12,6 @@ typedef float f32x2 __attribute__((ext_vector_type(2)));
 
 // A lane holds of each 16 x 16 block the row lane % 16 and four columns from lane / 16 * 4.
 
-// The blocks reach memory by rows through the wave's patch of LDS (nn_gemm.hpp), ROWS at a
-// time: put(row, column, eight values), both from the wave's first.
-template <int ROWS, int MI, int NI, typename F>
-__device__ __forceinline__ void by_rows(const f32x4 (&acc)[MI][NI], lds_char *patch, F &&put) {
-  constexpr int COLS = NI * 16, LANES = COLS / 8;
-  const int lane = threadIdx.x % 64, c = lane % LANES;
-#pragma unroll
-  for (int h = 0; h < MI * 16 / ROWS; ++h) {
-#pragma unroll
-    for (int i = 0; i < ROWS / 16; ++i)
-#pragma unroll
-      for (int j = 0; j < NI; ++j)
-        *reinterpret_cast<__attribute__((address_space(3))) f32x4 *>(patch + patch_at<COLS>(i * 16 + lane % 16, j * 4 + lane / 16)) =
-            acc[h * (ROWS / 16) + i][j];
-    wait_lds();
-#pragma unroll 4
-    for (int row = lane / LANES; row < ROWS; row += 64 / LANES) {
-      float v[8];
-#pragma unroll
-      for (int q = 0; q < 2; ++q) {
-        const f32x4 u = __builtin_bit_cast(f32x4, lds_read16(patch + patch_at<COLS>(row, c * 2 + q)));
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[q * 4 + i] = u[i];
-      }
-      put(h * ROWS + row, c * 8, v);
-    }
-  }
-}
-
 // Logarithms of sums are kept as pairs: t, and the sum of exp2(value * log2(e) - t).  t is the
 // largest value times log2(e), rounded: whatever it was rounded to, the pair stands for the sum.
 // -inf: no value yet.

@@ -245,10 +245,14 @@ class _Linear(torch.autograd.Function):
     def forward(ctx, x, w, bias, residual, activation, keep, tile, splits, terms, keep8):
         smooth = activation != "none"
         with torch.no_grad():
-            got = linear(x, w, bias, activation, residual, keep=keep or smooth, tile=tile, splits=splits)
-            out, z = got if keep or smooth else (got, None)
+            if keep8 and smooth and not keep:  # z is written in 8 bits alone
+                out, saved_z = _C.linear_keep8(x, w, bias, _act(activation), residual, False, None, None, None, tile, splits)
+                z, kept_z = None, (out.shape, out.dtype)
+            else:
+                got = linear(x, w, bias, activation, residual, keep=keep or smooth, tile=tile, splits=splits)
+                out, z = got if keep or smooth else (got, None)
+                saved_z, kept_z = _saved(z if smooth else None, keep8, activation == "relu")
             saved_x, kept_x = _saved(x, keep8)
-            saved_z, kept_z = _saved(z if smooth else None, keep8, activation == "relu")
         ctx.save_for_backward(saved_x, w, saved_z)
         ctx.kept = kept_x, kept_z
         ctx.how = activation, None if bias is None else bias.dtype, tile, splits, terms

@@ -330,3 +330,42 @@ def test_workspaces_of_the_gradient():
         assert _lib.lib().tf_linear_grad(ctypes.byref(a), stream) == 0
         want = nn.linear_grad(dy, x8, w, z8, "gelu")
         assert torch.equal(dx, want[0]) and torch.equal(dw, want[1]) and (space[size.value:] == 0xaa).all()
+
+
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("order", [0, 1])
+@pytest.mark.parametrize("tile,splits", [(0, 0), (1, 1), (2, 1), (3, 1), (4, 1), (5, 1), (2, 2), (3, 3)])
+def test_products_that_keep_z(tile, splits, order, dtype):
+    """The product's result as without, and the bytes that keep8 gives of the kept z: written with the product or after it."""
+    nn = _nn()
+    for i, (m, n, k) in enumerate([(1, 1, 1), (2, 40, 64), (16, 96, 128), (70, 72, 200), (130, 136, 72), (300, 520, 136), (257, 1032, 264),
+                                   (65, 257, 77), (600, 200, 0)]):
+        g = torch.Generator().manual_seed(m + n + k)
+        x, w, r = _matrix(g, m, k, dtype), _matrix(g, k, n, dtype, max(k, 1) ** -0.5), _matrix(g, m, n, dtype)
+        if i == 4:
+            x[3, 5], x[100, 0] = float("inf"), float("nan")
+        b = torch.randn(n, generator=g).to(dtype if i % 2 else torch.float32).cuda()
+        wc = w.cuda() if order == 0 else w.t().contiguous().cuda().t()
+        for activation in ACTS:
+            args = (x.cuda(), wc, b if i != 2 else None, nn._act(activation), r.cuda() if i % 3 else None)
+            out, kept = nn._C.linear_keep8(*args, False, None, None, None, tile, splits)
+            want, z = nn._C.linear(*args, True, None, None, None, tile, splits)
+            assert torch.equal(out.isnan(), want.isnan()) and torch.equal(out.nan_to_num(), want.nan_to_num())
+            assert torch.equal(kept, nn.keep8(z, activation == "relu").data), (m, n, k, activation)
+
+
+def test_large_products_that_keep_z():
+    """Sizes that the choice by sizes gives to each tile, and the C call's refusal of less workspace than it asks for."""
+    from tensorforge_amd import _lib
+    nn = _nn()
+    g = torch.Generator().manual_seed(0)
+    for m, n, k in ((4096, 4096, 256), (1000, 4096, 512), (512, 1536, 768), (2048, 2048, 2048), (100, 4096, 4096), (40, 512, 4096), (700, 1001, 300)):
+        x, w, b = _matrix(g, m, k, torch.bfloat16).cuda(), _matrix(g, k, n, torch.bfloat16, k ** -0.5).cuda(), torch.randn(n, generator=g).cuda()
+        out, kept = nn._C.linear_keep8(x, w, b, 2, None, False, None, None, None, 0, 0)
+        want, z = nn.linear(x, w, b, "gelu", keep=True)
+        assert torch.equal(out, want) and torch.equal(kept, nn.keep8(z).data), (m, n, k)
+    a = _lib.LinearArgs(x=x.data_ptr(), w=w.data_ptr(), out=out.data_ptr(), z=kept.data_ptr(), x_ld=k, w_ld=n, out_ld=n, m=m, n=n, k=k, type=1,
+                        out_type=1, kept=2)
+    size = ctypes.c_longlong()
+    assert _lib.lib().tf_linear_workspace(ctypes.byref(a), ctypes.byref(size)) == 0 and size.value >= 2 * m * n
+    assert _lib.lib().tf_linear(ctypes.byref(a), torch.cuda.current_stream().cuda_stream) == -4

@@ -22,6 +22,10 @@ def _linear(**kw):
 
 
 @pytest.mark.parametrize("change,words", [
+    (dict(kept=1, type=1), "kept = 1"), (dict(kept=2, z=256), "do not keep z in 8 bits"),
+    (dict(kept=2, type=1, x_scale=0, w_scale=0, z=0), "z is a null pointer"),
+    (dict(kept=2, type=1, x_scale=0, w_scale=0, z=264), "z, kept in 8 bits, is not 16-byte"),
+    (dict(kept=2, type=1, x_scale=0, w_scale=0, z=256), "are needed"),
     (dict(k=131072, x_ld=131072, w_ld=131072), "k = 131072"), (dict(out_type=4), "out_type = 4"), (dict(out_type=0), "out_type = 0"),
     (dict(w_order=0), "8-bit weights"), (dict(x_scale=0), "x_scale is a null pointer"), (dict(w_scale=0), "w_scale is a null pointer"),
     (dict(x_ld=63), "x: 63 elements"), (dict(type=5), "type = 5"), (dict(bias=256, bias_type=4), "bias_type = 4"),
@@ -117,6 +121,30 @@ def test_keep8_refusals():
              workspace_bytes=1 << 20)
     for change, words in ((dict(kept=2), "kept = 2"), (dict(kept=1, h=264), "h, kept in 8 bits"), (dict(kept=0), "h: 0 elements")):
         _refused(lib.tf_rms_norm_grad(ctypes.byref(_lib.RmsNormGradArgs(**{**a, **change})), None), words)
+
+
+def test_products_that_keep_z_launch(without_gpu):  # noqa: F811
+    """Whichever of their launches fails, the call says so; no launch has 2^32 threads."""
+    without_gpu("""
+def kept(m, n, k, order, tile=0, splits=0, fail=-1):
+    a = _lib.LinearArgs(x=256, w=256, out=256, z=256, x_ld=k, w_ld=k if order else n, out_ld=n, m=m, n=n, k=k, w_order=order, type=1, out_type=1,
+                        workspace=256, tile=tile, splits=splits, kept=2, act=1)
+    size = ctypes.c_longlong()
+    assert lib.tf_linear_workspace(ref(a), ref(size)) == 0
+    a.workspace_bytes = size.value
+    stub.arm(fail)
+    return lib.tf_linear(ref(a), None)
+big = 1 << 30
+for order in (0, 1):
+    for m, n, k in ((big, 1, 1), (big, 64, 64), (1, big, 8), (64, 1 << 28, 7), (1 << 20, 1 << 16, 8)):
+        for tile in (0, 1, 2, 3, 4, 5):
+            assert kept(m, n, k, order, tile) == 0, (m, n, k, tile)
+    for m, n, k in ((4096, 4096, 512), (16, 512, 4096), (777, 1111, 333), (300, 300, 8000)):
+        for tile, splits in ((0, 0), (3, 2), (4, 1)):
+            assert kept(m, n, k, order, tile, splits) == 0
+            for i in range(stub.arm(-1)):
+                assert kept(m, n, k, order, tile, splits, i) == -5, (m, n, k, tile, i)
+""")
 
 
 def test_kept_python_refusals():
