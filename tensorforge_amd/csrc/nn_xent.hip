@@ -22,22 +22,24 @@ struct RowsParams {
   int m, n, parts;
 };
 
-// The sum of a workgroup's 1024 values in a fixed order, in the first thread.
-__device__ __forceinline__ float group_sum(float v, float *part) {
-  v = wave_sum(v);
+// The sum of a workgroup's 1024 values in a fixed order.
+template <typename S>
+__device__ __forceinline__ S group_sum(S v, S *part) {
+#pragma unroll
+  for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
   __syncthreads();
   if (threadIdx.x % 64 == 0) part[threadIdx.x / 64] = v;
   __syncthreads();
-  float s = 0.0f;
+  S s = 0;
   for (int i = 0; i < 16; ++i) s += part[i];
   return s;
 }
 
-__device__ __forceinline__ void write_totals(const RowsParams &p, float sum, float count) {
+__device__ __forceinline__ void write_totals(const RowsParams &p, double sum, double count) {
   if (threadIdx.x) return;
-  if (p.sum) *p.sum = sum;
-  if (p.count) *p.count = count;
-  if (p.mean) *p.mean = count > 0.0f ? sum / count : 0.0f;
+  if (p.sum) *p.sum = static_cast<float>(sum);
+  if (p.count) *p.count = static_cast<float>(count);
+  if (p.mean) *p.mean = count > 0.0 ? static_cast<float>(sum / count) : 0.0f;
 }
 
 // R rows a workgroup, 1024/R threads a row that share the parts, kBatch of them under way at a
@@ -79,13 +81,15 @@ __global__ __launch_bounds__(1024) void xent_rows_kernel(RowsParams p) {
   }
   float loss = 0.0f, counts = 0.0f;
   if (lane == 0 && m < p.m) {
-    const float lse = (s.x + __builtin_amdgcn_logf(s.y)) * 0.693147180559945309f;
+    constexpr float kLn2 = 0.693147180559945309f;
+    const float log_sum = log2f(s.y);
     const long long target = p.target[m];
     if (target != p.ignore) {
       counts = 1.0f;
-      loss = target >= 0 && target < p.n ? lse - p.target_logit[m] : __builtin_nanf("");
+      // Not lse - logit: large logits would leave their roundings where their difference is small.
+      loss = target >= 0 && target < p.n ? (__builtin_fmaf(-p.target_logit[m], kLog2e, s.x) + log_sum) * kLn2 : __builtin_nanf("");
     }
-    p.lse[m] = lse;
+    p.lse[m] = (s.x + log_sum) * kLn2;
     p.loss[m] = loss;
   }
   if (gridDim.x * gridDim.y == 1 && (p.sum || p.mean || p.count)) {
@@ -98,9 +102,10 @@ __global__ __launch_bounds__(1024) void xent_rows_kernel(RowsParams p) {
 // that makes one workgroup of all and spares the totals' launch.
 bool one_group(long m, bool totals) { return m <= 16 || (m <= 64 && totals); }
 
+// Sums of up to 2^30 rows: in 64 bits.
 __global__ __launch_bounds__(1024) void xent_totals_kernel(RowsParams p) {
-  __shared__ float sums[16];
-  float loss = 0.0f, counts = 0.0f;
+  __shared__ double sums[16];
+  double loss = 0.0, counts = 0.0;
   for (long m = threadIdx.x; m < p.m; m += 1024) {
     loss += p.loss[m];
     counts += p.target[m] != p.ignore;

@@ -536,3 +536,52 @@ def test_operands_far_apart(order):
         assert float((a.double() - b.double()).norm() / b.double().norm()) < 2.0 ** -8
     del memory, xf, wf
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("size", [1, 8, 60])
+def test_small_losses_of_large_logits(size):
+    """A row that is sure of its class: the loss is the sum of the others' exponentials, however large the logits are."""
+    nn = _nn()
+    m, n, k = 40, 300, 64
+    g = torch.Generator().manual_seed(size)
+    x, w = torch.zeros(m, k), torch.zeros(k, n)
+    x[:, 0], w[0] = size, 8.0  # exact logits of 8 * size for every class, beside
+    x[:, 1] = torch.arange(m) * 0.5
+    w[1, 7] = 1.0  # 0 to 19.5 more for the seventh
+    x[:, 2], w[2] = 0.25, torch.randint(-4, 5, (n,), generator=g).float()
+    x, w = x.bfloat16(), w.bfloat16()
+    z = x.double() @ w.double()
+    target = torch.full((m,), 7)
+    others = z - z[:, 7:8]
+    others[:, 7] = float("-inf")
+    want = torch.log1p(torch.exp(others).sum(1))
+    loss = nn.linear_cross_entropy(x.cuda(), w.cuda(), target.cuda(), reduction="none").cpu().double()
+    # sums of 300 exponentials in a tree, then a logarithm and a product: a few roundings of a value of 1 to 400
+    assert ((loss - want).abs() <= 16 * ref.u * (1 + want)).all(), (loss - want).abs().max()
+
+
+def test_totals_of_many_rows():
+    """Sums over rows that a float sum would lose parts of."""
+    nn = _nn()
+    m = 3_000_001
+    x = torch.zeros(m, 8, dtype=torch.bfloat16, device="cuda")
+    w = torch.zeros(8, 3, dtype=torch.bfloat16, device="cuda")
+    target = torch.zeros(m, dtype=torch.int64, device="cuda")
+    target[1::2] = IGNORE
+    mean, _, count = nn.linear_cross_entropy(x, w, target, keep=True)
+    total = nn.linear_cross_entropy(x, w, target, reduction="sum")
+    row = float(nn.linear_cross_entropy(x[0], w, target[0]))
+    assert float(count) == 1_500_001 and abs(float(mean) - row) <= 2 * ref.u * row and abs(float(total) - 1_500_001 * row) <= 4 * ref.u * 1_500_001 * row
+
+
+def test_forward_mode_is_refused():
+    import torch.autograd.forward_ad as fwd
+    nn = _nn()
+    x, w, target, g = _data(6, 40, 16, torch.bfloat16)
+    with fwd.dual_level():
+        for at in (0, 1):
+            a = [x.cuda(), w.cuda()]
+            a[at] = fwd.make_dual(a[at], torch.ones_like(a[at]))
+            for mode in (torch.enable_grad, torch.no_grad):
+                with mode(), pytest.raises((RuntimeError, NotImplementedError)):
+                    nn.linear_cross_entropy(*a, target.cuda())
