@@ -433,7 +433,9 @@ int tf_linear_grad(const tf_linear_grad_args_t *args, void *stream);
 typedef struct {
   const void *x, *w;       /* m x k, k x n in either order                          */
   const long long *target; /* m                                                     */
-  float *loss, *lse;       /* m                                                     */
+  float *loss;             /* m                                                     */
+  double *lse;             /* m; in 64 bits for the gradient: where a row is sure of its
+                              class, it takes a small difference of large numbers    */
   float *sum, *mean, *count; /* one float each, or NULL: of the losses of the rows that
                               count, and their number; a mean of no rows is 0       */
   void *workspace;         /* 16-byte aligned, tf_linear_xent_workspace's bytes     */
@@ -461,7 +463,7 @@ int tf_linear_xent(const tf_linear_xent_args_t *args, void *stream);
 typedef struct {
   const void *x, *w;
   const long long *target;
-  const float *lse;        /* m                                                     */
+  const double *lse;       /* m                                                     */
   const float *dloss;      /* m with dloss_rows, else one                           */
   const float *count;      /* one float, or NULL for 1: the mean's gradient takes
                               tf_linear_xent's count                                */

@@ -90,7 +90,8 @@ struct XentParams : GemmParams {
   // XENT_SLOPE: out = (exp(logit - lse) - [column is the target]) * unit, zeros up to a multiple of 8 columns.  One dloss
   // for all rows: the unit is `power`, and dloss / count / power comes with XENT_SUM.  A row's own: dloss / count, in
   // float16 times scale[0].
-  const float *lse = nullptr, *dloss = nullptr, *count = nullptr, *scale = nullptr;
+  const double *lse = nullptr;
+  const float *dloss = nullptr, *count = nullptr, *scale = nullptr;
   float power = 1.0f;
   int dloss_rows = 0;
   long lo = 0;  // not 0: what dz's rounding left, rounded, that many elements behind

@@ -501,8 +501,8 @@ Xent xent(const Tensor &x, const Tensor &w, const Tensor &target, int64_t ignore
   on_gpu(x, {&w, &target});
   const On on(x);
   const at::IntArrayRef shape = x.sizes().slice(0, x.dim() - 1);
-  Xent r{fresh(x, shape, ScalarType::Float), fresh(x, shape, ScalarType::Float), {}};
-  g.loss = r.loss.data_ptr<float>(), g.lse = r.lse.data_ptr<float>();
+  Xent r{fresh(x, shape, ScalarType::Float), fresh(x, shape, ScalarType::Double), {}};
+  g.loss = r.loss.data_ptr<float>(), g.lse = r.lse.data_ptr<double>();
   Tensor one, space;
   if (reduction) one = fresh(x, {}, ScalarType::Float), (reduction == 1 ? g.sum : g.mean) = one.data_ptr<float>();
   if (reduction == 2) r.count = fresh(x, {}, ScalarType::Float), g.count = r.count.data_ptr<float>();
@@ -522,7 +522,7 @@ std::pair<Tensor, Tensor> xent_grad(const Tensor &dloss, const Tensor &x, const 
   tf_linear_xent_grad_args_t g{};
   g.target = targets(target, x);
   const at::IntArrayRef shape = x.sizes().slice(0, x.dim() - 1);
-  same_type(lse, "lse", ScalarType::Float, ScalarType::Float);
+  same_type(lse, "lse", ScalarType::Double, ScalarType::Double);
   TORCH_CHECK_VALUE(lse.sizes() == shape && lse.is_contiguous(), "lse is not a contiguous tensor of ", shape);
   same_type(dloss, "dloss", ScalarType::Float, ScalarType::Float);
   g.dloss_rows = dloss.dim() != 0;
@@ -532,7 +532,7 @@ std::pair<Tensor, Tensor> xent_grad(const Tensor &dloss, const Tensor &x, const 
     TORCH_CHECK_VALUE(number->numel() == 1, "count is not one number");
     g.count = number->data_ptr<float>();
   }
-  g.lse = lse.data_ptr<float>(), g.dloss = dloss.data_ptr<float>();
+  g.lse = lse.data_ptr<double>(), g.dloss = dloss.data_ptr<float>();
   g.x = xr.p, g.x_ld = xr.ld, g.m = xr.m, g.k = xr.n, g.w = wr.p, g.w_ld = wr.ld, g.n = wr.n, g.w_order = wr.order;
   g.type = type_of(t), g.ignore = ignore;
   on_gpu(x, {&w, &target, &lse, &dloss, number});

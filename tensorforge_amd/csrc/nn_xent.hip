@@ -18,7 +18,8 @@ struct RowsParams {
   const float *stats, *target_logit;
   const long long *target;
   long long ignore;
-  float *lse, *loss, *sum, *mean, *count;
+  double *lse;
+  float *loss, *sum, *mean, *count;
   int m, n, parts;
 };
 
@@ -89,7 +90,7 @@ __global__ __launch_bounds__(1024) void xent_rows_kernel(RowsParams p) {
       // Not lse - logit: large logits would leave their roundings where their difference is small.
       loss = target >= 0 && target < p.n ? (__builtin_fmaf(-p.target_logit[m], kLog2e, s.x) + log_sum) * kLn2 : __builtin_nanf("");
     }
-    p.lse[m] = (s.x + log_sum) * kLn2;
+    p.lse[m] = (static_cast<double>(s.x) + log_sum) / kLog2e;
     p.loss[m] = loss;
   }
   if (gridDim.x * gridDim.y == 1 && (p.sum || p.mean || p.count)) {
@@ -311,7 +312,7 @@ int loss(const tf_linear_xent_args_t *a, hipStream_t stream) {
   c.matrix("x", a->x, a->x_ld, a->m, a->k, a->type, true);
   c.matrix("w", a->w, a->w_ld, a->m ? (a->w_order ? a->n : a->k) : 0, a->w_order ? a->k : a->n, a->type, true);
   if (a->m) c.need(a->target && reinterpret_cast<uintptr_t>(a->target) % 8 == 0, "target is null or not aligned");
-  c.vector("lse", a->lse, a->m, TF_T_F32, true);
+  if (a->m) c.need(a->lse && reinterpret_cast<uintptr_t>(a->lse) % 8 == 0, "lse is null or not aligned");
   c.vector("loss", a->loss, a->m, TF_T_F32, true);
   c.vector("sum", a->sum, 1, TF_T_F32, false);
   c.vector("mean", a->mean, 1, TF_T_F32, false);
@@ -473,7 +474,7 @@ int grad(const tf_linear_xent_grad_args_t *a, hipStream_t stream) {
   c.matrix("x", a->x, a->x_ld, a->m, a->k, a->type, true);
   c.matrix("w", a->w, a->w_ld, a->m ? (nk ? a->n : a->k) : 0, nk ? a->k : a->n, a->type, true);
   if (a->m) c.need(a->target && reinterpret_cast<uintptr_t>(a->target) % 8 == 0, "target is null or not aligned");
-  c.vector("lse", a->lse, a->m, TF_T_F32, true);
+  if (a->m) c.need(a->lse && reinterpret_cast<uintptr_t>(a->lse) % 8 == 0, "lse is null or not aligned");
   c.vector("dloss", a->dloss, a->m ? (a->dloss_rows ? a->m : 1) : 0, TF_T_F32, true);
   c.vector("count", a->count, 1, TF_T_F32, false);
   c.matrix("dx", a->dx, a->dx_ld, a->m, a->k, a->type, false);

@@ -109,12 +109,14 @@ struct Slope {
     const bool whole = nw + NI * 16 <= p.n;
     // What the rows need, all under way at once.  Rows past the last are not written.
     long long target[MI];
-    float lse[MI], d[MI];
+    float lse[MI], rest[MI], d[MI];  // lse * log2(e) in two floats: large logits keep what their differences are worth
 #pragma unroll
     for (int i = 0; i < MI; ++i) {
       const int m = min(mw + i * 16 + l, p.m - 1);
       target[i] = p.target[m];
-      lse[i] = p.lse[m] * kLog2e;
+      const double scaled = p.lse[m] * kLog2e;
+      lse[i] = static_cast<float>(scaled);
+      rest[i] = __builtin_fabsf(lse[i]) < __builtin_inff() ? static_cast<float>(scaled - lse[i]) : 0.0f;
       d[i] = p.dloss_rows ? p.dloss[m] * unit : unit;
     }
 #pragma unroll
@@ -127,7 +129,7 @@ struct Slope {
 #pragma unroll
       for (int j = 0; j < NI; ++j)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) acc[i][j][e] = fast_exp2(__builtin_fmaf(acc[i][j][e], kLog2e, -lse[i])) * d[i];
+        for (int e = 0; e < 4; ++e) acc[i][j][e] = fast_exp2(__builtin_fmaf(acc[i][j][e], kLog2e, -lse[i]) - rest[i]) * d[i];
       if (here) {
 #pragma unroll
         for (int j = 0; j < NI; ++j)

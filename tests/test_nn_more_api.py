@@ -225,7 +225,7 @@ def _xent_grad(**kw):
 @pytest.mark.parametrize("change,words", [
     (dict(type=0), "type = 0"), (dict(type=3), "type = 3"), (dict(w_order=2), "w_order = 2"), (dict(n=0), "no class"), (dict(m=-1), "m = -1"),
     (dict(k=(1 << 30) + 1), "k = 1073741825"), (dict(x=0), "x is a null"), (dict(w=0), "w is a null"), (dict(target=0), "target is null"),
-    (dict(target=260), "target is null or not aligned"), (dict(loss=0), "loss is a null"), (dict(lse=0), "lse is a null"),
+    (dict(target=260), "target is null or not aligned"), (dict(loss=0), "loss is a null"), (dict(lse=0), "lse is null"), (dict(lse=260), "lse is null or not aligned"),
     (dict(x_ld=63), "x: 63"), (dict(w_ld=99), "w: 99"), (dict(w_order=1, w_ld=63), "w: 63"), (dict(workspace=0), "workspace is null"),
     (dict(workspace=264), "not 16-byte aligned"), (dict(sum=258), "sum is not aligned"), (dict(mean=258), "mean is not aligned"),
     (dict(count=258), "count is not aligned"), (dict(m=1 << 30, n=1 << 27, w_ld=1 << 27), "are too many"), (dict(workspace_bytes=16), "are needed"), (dict(x=257), "x is not aligned")])
@@ -234,7 +234,7 @@ def test_xent_refusals(change, words):
 
 
 @pytest.mark.parametrize("change,words", [
-    (dict(type=4), "type = 4"), (dict(n=0), "no class"), (dict(dloss=0), "dloss is a null"), (dict(lse=0), "lse is a null"),
+    (dict(type=4), "type = 4"), (dict(n=0), "no class"), (dict(dloss=0), "dloss is a null"), (dict(lse=0), "lse is null"), (dict(lse=260), "lse is null or not aligned"),
     (dict(dloss_rows=2), "dloss_rows = 2"), (dict(target=0), "target is null"), (dict(dx_ld=63), "dx: 63"), (dict(dw_ld=99), "dw: 99"),
     (dict(count=258), "count is not aligned"), (dict(workspace_bytes=16), "are needed"), (dict(m=(1 << 30) + 1), "m = 1073741825")])
 def test_xent_grad_refusals(change, words):
@@ -246,7 +246,7 @@ def test_xent_grad_refusals(change, words):
 
 def test_xent_python_refusals():
     h, w, t = torch.zeros(4, 8, dtype=torch.bfloat16), torch.zeros(8, 16, dtype=torch.bfloat16), torch.zeros(4, dtype=torch.int64)
-    one, rows = torch.ones(()), torch.zeros(4)
+    one, dl, rows = torch.ones(()), torch.zeros(4), torch.zeros(4, dtype=torch.float64)
     for call, error, words in [
             (lambda: nn.linear_cross_entropy(h, w, t), ValueError, "not on a GPU"),
             (lambda: nn.linear_cross_entropy(h, w, t, reduction="max"), ValueError, "not one of none, sum, mean"),
@@ -261,11 +261,11 @@ def test_xent_python_refusals():
             (lambda: nn.linear_cross_entropy(h.clone().requires_grad_(), w, t), ValueError, "not on a GPU"),
             (lambda: nn.linear_cross_entropy(h.clone().requires_grad_(), w, t[:3]), ValueError, "target is not"),
             (lambda: nn.linear_cross_entropy_grad(one, h, w, t, rows), ValueError, "not on a GPU"),
-            (lambda: nn.linear_cross_entropy_grad(rows[:3], h, w, t, rows), ValueError, "dloss is not"),
+            (lambda: nn.linear_cross_entropy_grad(dl[:3], h, w, t, rows), ValueError, "dloss is not"),
             (lambda: nn.linear_cross_entropy_grad(one.double(), h, w, t, rows), TypeError, "dloss is Double"),
             (lambda: nn.linear_cross_entropy_grad(one, h, w, t, rows[:2]), ValueError, "lse is not"),
-            (lambda: nn.linear_cross_entropy_grad(one, h, w, t, rows, rows), ValueError, "count is not one"),
-            (lambda: nn.linear_cross_entropy_grad(one, h, w, t, rows.bfloat16()), TypeError, "lse is BFloat16"),
+            (lambda: nn.linear_cross_entropy_grad(one, h, w, t, rows, dl), ValueError, "count is not one"),
+            (lambda: nn.linear_cross_entropy_grad(one, h, w, t, dl), TypeError, "lse is Float"),
             (lambda: nn.linear_cross_entropy_grad(one, h, w.clone().requires_grad_(), t, rows), ValueError, "no gradient")]:
         with pytest.raises(error, match=words):
             call()
