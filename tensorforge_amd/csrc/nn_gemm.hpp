@@ -278,6 +278,8 @@ __device__ __forceinline__ f32x4 block_mma(f8, i32x4 a0, i32x4 a1, i32x4 b0, i32
 }
 
 // 8-bit integers: sums of 32-bit integers, exact while k is at most 131071 (128 * 128 * k < 2^31).
+// A loop of nothing but these reaches 3.9 POP/s at the power limit (e4m3's instruction 4.5, 32 x 32 x 32
+// blocks of integers 3.3), and the products stand so too: 8192^3 487 us, e4m3 404.
 __device__ __forceinline__ i32x4 block_mma(i8, i32x4 a0, i32x4 a1, i32x4 b0, i32x4 b1, i32x4 c) {
   c = __builtin_amdgcn_mfma_i32_16x16x64_i8(b0, a0, c, 0, 0, 0);
   return __builtin_amdgcn_mfma_i32_16x16x64_i8(b1, a1, c, 0, 0, 0);

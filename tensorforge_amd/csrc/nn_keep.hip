@@ -2,6 +2,7 @@
 //
 // Bound by memory: a thread takes 8 elements, four threads a group, whose largest
 // magnitude they find by two exchanges; kUnroll pieces a thread under way together.
+// 8192 x 8192 bfloat16 38 us there (5.3 TB/s) and 30 back (6.7), 70 for both in turn.
 #include "nn_common.hpp"
 
 #include <algorithm>
