@@ -87,6 +87,7 @@ struct Product {
   Operand a, b;
   GemmParams p;  // sizes, output and epilogue
   bool square = false;  // on the square tiles alone
+  bool logits = false;  // the loss's: statistics or dz leave a tile
 };
 
 inline long ceil_div(long a, long b) { return (a + b - 1) / b; }
@@ -141,7 +142,9 @@ constexpr TileCost kCostAny{3, 3.9, 0.55, 3.0, 0.28, 0.92, 1.09, 0.2, 2.5, 1.74,
 
 // Few slabs of LDS let five 64 x 64 tiles on a CU, from 768 on: 3.5, and a workgroup 0.46
 // and 0.22 a slab.  read: the operands' bytes at 8 TB/s.
-inline double predicted(double m, double n, double slabs, double read, bool dma, bool f8, int tile, int splits) {
+// logits: without a time for written results, which the large tiles' ends do not need there (8192 rows, 32768 classes and
+// k of 512, bfloat16, 128/256-tile: the loss 303 / 271, its gradient 1132 / 1035).
+inline double predicted(double m, double n, double slabs, double read, bool dma, bool f8, int tile, int splits, bool logits) {
   const TileCost &c = !dma ? kCostAny : tile == TILE_256 ? kCost256 : tile == TILE_128 ? kCost128 : tile == TILE_64 ? kCost64 : kCost64x128;
   const double each = std::ceil(slabs / splits), results = m * n / 1e6, most = c.most;
   const double w = std::ceil(m / tile_rows(tile)) * std::ceil(n / tile_columns(tile)) * splits / 256;  // workgroups a CU
@@ -160,7 +163,7 @@ inline double predicted(double m, double n, double slabs, double read, bool dma,
     }
   }
   us = std::max(us, 4.5 + read);
-  return splits > 1 ? us + c.join + c.join_part * splits * results : std::max(us, 4.5 + results * c.written);
+  return splits > 1 ? us + c.join + c.join_part * splits * results : std::max(us, logits ? 0.0 : 4.5 + results * c.written);
 }
 
 // The C tile and the ranges of k for a product of these sizes: the least
@@ -207,7 +210,7 @@ inline Plan plan_product(const Product &q, bool dma, int tile, int splits) {
       if (s > 1 && (splits || s * 2 > slabs || tiles * s > 1024)) break;
       const int ranges = splits ? splits : s;
       if (dma && !fits(t, tiles * ranges)) continue;
-      const double us = predicted(m, n, slabs * terms, read, dma, size == 1, t, ranges);
+      const double us = predicted(m, n, slabs * terms, read, dma, size == 1, t, ranges, q.logits);
       if (us < best.us) best = {t, ranges, us};
     }
   }

@@ -259,7 +259,7 @@ void place_xent(XentParams &p, Product &q, const Choice &c, void *parts) {
 }
 
 Product logits_of(const void *x, long x_ld, const void *w, long w_ld, int w_order, int type, long m, long n, long k) {
-  Product q{type, type, {}, {}, {}, true};
+  Product q{type, type, {}, {}, {}, true, true};
   q.a = {x, x_ld, m, k, false, false};
   q.b = w_order ? Operand{w, w_ld, n, k, false, false} : Operand{w, w_ld, k, n, true, false};
   q.p.m = static_cast<int>(m), q.p.n = static_cast<int>(n), q.p.k = static_cast<int>(k);
@@ -398,7 +398,7 @@ Piece piece_of(const GradPlan &g, const tf_linear_xent_grad_args_t *a, long n) {
   };
   const int rows = m * g.terms;  // of dz
   const auto dz_as = [&](bool mn) { return Operand{nullptr, g.dz_ld, mn ? m : rows, n, mn, true}; };
-  s.z = {a->type, a->type, x_as(false), w_as(!nk), {}, true};
+  s.z = {a->type, a->type, x_as(false), w_as(!nk), {}, true, true};
   s.z.p.m = m, s.z.p.n = static_cast<int>(n), s.z.p.k = k;
   s.dx = {a->type, a->type, dz_as(false), w_as(nk), {}, true};
   s.dx.p.m = rows, s.dx.p.n = k, s.dx.p.k = static_cast<int>(n);
