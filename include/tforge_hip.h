@@ -319,11 +319,15 @@ int tf_quantize_rows_to(const void *x, long long x_ld, long long rows, long long
  * bytes e, the unit being 2^(e-127).  A group that holds an infinity or a NaN has e =
  * 255 and zeros, and stands for NaN throughout.
  * positive: values above zero keep an integer of at least 1, so that relu's
- * gradient from a pre-activation kept so is that of the pre-activation itself.
+ * gradient from a pre-activation kept so is that of the pre-activation itself, where the
+ * group is finite.
+ * tf_keep8_masked: minus infinity is the integer -128 instead and counts for no unit.  It comes back
+ * as itself, with a slope of 0 under every activation, and its neighbours as without it.
  * tf_restore8 gives the values in `type`: exact in TF_T_F32 and TF_T_BF16; in
  * TF_T_F16 rounded, past 65504 that. */
 int tf_keep8_bytes(long long rows, long long d, long long *bytes);
 int tf_keep8(const void *x, long long x_ld, long long rows, long long d, int type, int positive, void *kept, void *stream);
+int tf_keep8_masked(const void *x, long long x_ld, long long rows, long long d, int type, int positive, void *kept, void *stream);
 int tf_restore8(const void *kept, long long rows, long long d, int type, void *x, long long x_ld, void *stream);
 
 /* Which operands of a gradient are kept in 8 bits (their *_ld does not count). */
@@ -385,8 +389,8 @@ typedef struct {
                     up to 64 rows, k split over a workgroup's waves, 5: 64x128; one that
                     cannot run these operands gives way to the choice by sizes       */
   int splits;    /* ranges of k: 0 by the sizes, or 1..64                            */
-  int kept;      /* 0, or TF_KEPT_Z: z is written in 8 bits, as tf_keep8 of the z in
-                    out_type would (relu's with `positive`); not of 8-bit products,
+  int kept;      /* 0, or TF_KEPT_Z: z is written in 8 bits, as tf_keep8_masked of the z
+                    in out_type would (relu's with `positive`); not of 8-bit products,
                     and the workspace has to be whole                                */
 } tf_linear_args_t;
 /* Bytes of workspace for these arguments: sizes, types, distances and the

@@ -122,6 +122,7 @@ SIGNATURES = [
     ("tf_quantize_rows_to", I, [P, LL, LL, LL, I, P, LL, I, P, P]),
     ("tf_keep8_bytes", I, [LL, LL, ctypes.POINTER(LL)]),
     ("tf_keep8", I, [P, LL, LL, LL, I, I, P, P]),
+    ("tf_keep8_masked", I, [P, LL, LL, LL, I, I, P, P]),
     ("tf_restore8", I, [P, LL, LL, I, P, LL, P]),
     ("tf_rms_norm_grad_workspace", I, [LL, LL, ctypes.POINTER(LL)]),
     ("tf_rms_norm_grad", I, [P, P]),

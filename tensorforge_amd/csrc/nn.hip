@@ -91,6 +91,22 @@ int rms_norm_grad(const tf_rms_norm_grad_args_t *a, hipStream_t stream) {
   return hip(launch_rms_norm_grad(p, a->type, stream), call);
 }
 
+// ---- kept in 8 bits ---------------------------------------------------------------
+
+int keep8(const char *call, const void *x, long long x_ld, long long rows, long long d, int type, int positive, bool masked, void *kept,
+          hipStream_t stream) {
+  Checks c{call, {}};
+  c.one_of("type", type, {TF_T_F32, TF_T_BF16, TF_T_F16});
+  c.one_of("positive", positive, {0, 1});
+  c.size("rows", rows);
+  c.size("d", d);
+  c.matrix("x", x, x_ld, rows, d, type, true);
+  c.kept("kept", kept, rows, d, true);
+  if (!c.fine()) return fail(TF_E_ARG, c.wrong);
+  if (rows == 0 || d == 0) return TF_OK;
+  return hip(launch_keep(x, x_ld, rows, static_cast<int>(d), type, positive != 0, masked, kept, stream), call);
+}
+
 // ---- products -------------------------------------------------------------------
 
 void check_linear_sizes(Checks &c, const tf_linear_args_t *a) {
@@ -170,7 +186,7 @@ int linear(const tf_linear_args_t *a, hipStream_t stream) {
   q.p.z = z16 ? ws + plan.bytes() : nullptr, q.p.ldz = a->n;
   hipError_t e = run_product(q, a->tile, a->splits, ws, plan.bytes(), stream, z16 ? nullptr : a->z);
   if (e == hipSuccess && z16)
-    e = launch_keep(ws + plan.bytes(), a->n, a->m, static_cast<int>(a->n), a->type, a->act == TF_ACT_RELU, a->z, stream);
+    e = launch_keep(ws + plan.bytes(), a->n, a->m, static_cast<int>(a->n), a->type, a->act == TF_ACT_RELU, true, a->z, stream);
   return hip(e, call);
 }
 
@@ -439,18 +455,11 @@ int tf_keep8_bytes(long long rows, long long d, long long *bytes) {
 }
 
 int tf_keep8(const void *x, long long x_ld, long long rows, long long d, int type, int positive, void *kept, void *stream) {
-  return guarded([&] {
-    Checks c{"tf_keep8", {}};
-    c.one_of("type", type, {TF_T_F32, TF_T_BF16, TF_T_F16});
-    c.one_of("positive", positive, {0, 1});
-    c.size("rows", rows);
-    c.size("d", d);
-    c.matrix("x", x, x_ld, rows, d, type, true);
-    c.kept("kept", kept, rows, d, true);
-    if (!c.fine()) return fail(TF_E_ARG, c.wrong);
-    if (rows == 0 || d == 0) return TF_OK;
-    return hip(launch_keep(x, x_ld, rows, static_cast<int>(d), type, positive != 0, kept, static_cast<hipStream_t>(stream)), "tf_keep8");
-  });
+  return guarded([&] { return keep8("tf_keep8", x, x_ld, rows, d, type, positive, false, kept, static_cast<hipStream_t>(stream)); });
+}
+
+int tf_keep8_masked(const void *x, long long x_ld, long long rows, long long d, int type, int positive, void *kept, void *stream) {
+  return guarded([&] { return keep8("tf_keep8_masked", x, x_ld, rows, d, type, positive, true, kept, static_cast<hipStream_t>(stream)); });
 }
 
 int tf_restore8(const void *kept, long long rows, long long d, int type, void *x, long long x_ld, void *stream) {

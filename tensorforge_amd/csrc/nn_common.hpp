@@ -236,8 +236,9 @@ __device__ __forceinline__ uint32_t round_to_bytes(float a, float b, float c, fl
 // the least power of two (2^-126 at least) whose integers stay within 127.  rows x groups x 32
 // codes, zeros behind a row's end, then rows x groups exponents: the unit is 2^(exponent - 127),
 // a float of that exponent field.  A group with an infinity or a NaN has the exponent 255 (an
-// infinite unit) and codes 0, which make NaN.  A unit of two's power restores exactly: the
-// values need no more than bfloat16's bits.
+// infinite unit) and codes 0, which make NaN.  `masked`: minus infinity is the code -128 instead and counts
+// for no unit, so that a hidden unit masked by its bias has a slope of 0 and leaves its neighbours
+// alone.  A unit of two's power restores exactly: the values need no more than bfloat16's bits.
 constexpr int kGroup = 32;
 
 struct Kept {
@@ -259,11 +260,19 @@ __device__ __forceinline__ uint32_t group_exponent(uint32_t top) {
 
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
-__device__ __forceinline__ void restore_codes(u32x2 codes, uint32_t exponent, float (&v)[8]) {
+// The values of 8 codes but for minus infinity's; whether there is one, which restore_masked then puts in.
+__device__ __forceinline__ bool restore_codes(u32x2 codes, uint32_t exponent, float (&v)[8]) {
   const float unit = __builtin_bit_cast(float, exponent << 23);
+  const u32x2 u = codes ^ 0x80808080u;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = (static_cast<float>((i < 4 ? u.x : u.y) >> (8 * (i & 3)) & 255u) - 128.0f) * unit;
+  const u32x2 zero = (u - 0x01010101u) & ~u;  // the lowest byte that is 0 leaves its highest bit
+  return (zero.x | zero.y) & 0x80808080u;
+}
+__device__ __forceinline__ void restore_masked(u32x2 codes, float (&v)[8]) {
 #pragma unroll
   for (int i = 0; i < 8; ++i)
-    v[i] = (static_cast<float>(((i < 4 ? codes.x : codes.y) ^ 0x80808080u) >> (8 * (i & 3)) & 255u) - 128.0f) * unit;
+    if (((i < 4 ? codes.x : codes.y) >> (8 * (i & 3)) & 255u) == 0x80u) v[i] = -__builtin_inff();
 }
 
 // The largest of four neighbouring lanes.
@@ -273,10 +282,17 @@ __device__ __forceinline__ uint32_t quad_max(uint32_t v) {
 }
 
 // The codes of a lane's 8 values; four neighbouring lanes hold a group, whose exponent each gets.
+template <bool MASKED>
 __device__ __forceinline__ u32x2 group_codes(const float (&v)[8], bool positive, uint32_t &exponent) {
   uint32_t top = 0;
 #pragma unroll
   for (int i = 0; i < 8; ++i) top = max(top, __builtin_bit_cast(uint32_t, v[i]) & 0x7fffffffu);
+  const bool infinite = MASKED && top == 0x7f800000u;  // seldom: the rest costs a branch a lane
+  if (infinite) {
+    top = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top = max(top, v[i] == -__builtin_inff() ? 0u : __builtin_bit_cast(uint32_t, v[i]) & 0x7fffffffu);
+  }
   exponent = group_exponent(quad_max(top));
   const float inverse = __builtin_bit_cast(float, (254u - min(exponent, 253u)) << 23);
   float t[8];
@@ -285,24 +301,34 @@ __device__ __forceinline__ u32x2 group_codes(const float (&v)[8], bool positive,
     t[i] = v[i] * inverse;
     if (positive && v[i] > 0.0f) t[i] = __builtin_fmaxf(t[i], 1.0f);
   }
+  if (infinite) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) t[i] = __builtin_fmaxf(t[i], -128.0f);  // minus infinity's code; others are -127.5 at least
+  }
   return exponent == 255 ? u32x2{0, 0} : u32x2{round_to_bytes(t[0], t[1], t[2], t[3]), round_to_bytes(t[4], t[5], t[6], t[7])};
 }
 
 // 8 values from c (a multiple of 8) of a row; zeros past its last group.
-__device__ __forceinline__ void load_kept8(const Kept &k, long row, int c, float (&v)[8]) {
+struct KeptCodes {
+  u32x2 codes;
+  uint32_t exponent;
+};
+__device__ __forceinline__ KeptCodes load_codes8(const Kept &k, long row, int c) {
   const long length = k.groups * kGroup, at = min(static_cast<long>(c), length - 8);
-  u32x2 codes = *reinterpret_cast<const u32x2 *>(k.codes + row * length + at);
-  uint32_t exponent = k.exponents[row * k.groups + at / kGroup];
-  if (c > at) codes = u32x2{0, 0}, exponent = 1;
-  restore_codes(codes, exponent, v);
+  const KeptCodes v = {*reinterpret_cast<const u32x2 *>(k.codes + row * length + at), k.exponents[row * k.groups + at / kGroup]};
+  return c > at ? KeptCodes{{0, 0}, 1} : v;
 }
+__device__ __forceinline__ void restore8(const KeptCodes &k, float (&v)[8]) {
+  if (restore_codes(k.codes, k.exponent, v)) restore_masked(k.codes, v);
+}
+__device__ __forceinline__ void load_kept8(const Kept &k, long row, int c, float (&v)[8]) { restore8(load_codes8(k, row, c), v); }
 
-// A kept value in T: past float16's largest it is that.
+// A kept value in T: a finite one past float16's largest is that.
 template <typename T>
 __device__ __forceinline__ T kept_as(float v) {
   if constexpr (__is_same(T, f16)) {
     const float near = __builtin_fminf(__builtin_fmaxf(v, -65504.0f), 65504.0f);
-    return static_cast<T>(v != v ? v : near);
+    return static_cast<T>(__builtin_fabsf(v) < __builtin_inff() ? near : v);
   } else {
     return static_cast<T>(v);
   }

@@ -8,7 +8,7 @@
 
 namespace tfnn {
 
-// out = act(z) + residual, and the codes of z rounded to T (as keep8 of a kept z would give them).  A
+// out = act(z) + residual, and the codes of z rounded to T (as keep8 of a kept z, masked, would give them).  A
 // group's columns are four lanes' of the patch: tiles start at multiples of 32.
 struct KeptResults {
   typedef KeptGemmParams Params;
@@ -30,7 +30,7 @@ struct KeptResults {
           z[i] = i < left ? static_cast<float>(static_cast<T>(v[i])) : 0.0f;
         }
         uint32_t exponent;
-        const u32x2 codes = group_codes(z, act() == ACT_RELU, exponent);
+        const u32x2 codes = group_codes<true>(z, act() == ACT_RELU, exponent);
         if (n < length) {
           *reinterpret_cast<u32x2 *>(p.codes + m * length + n) = codes;
           if (n % kGroup == 0) p.exponents[m * p.groups + n / kGroup] = static_cast<uint8_t>(exponent);

@@ -28,7 +28,7 @@ struct Place {
   }
 };
 
-template <typename T, bool FLAT>
+template <typename T, bool FLAT, bool MASKED>
 __global__ __launch_bounds__(256) void keep_kernel(const T *x, long ld, int d, long all, long pieces, bool positive, uint8_t *codes,
                                                    uint8_t *exponents) {
   constexpr int N = 16 / sizeof(T);
@@ -52,7 +52,7 @@ __global__ __launch_bounds__(256) void keep_kernel(const T *x, long ld, int d, l
   for (int u = 0; u < kUnroll; ++u) {
     const long id = first + u * 256;
     uint32_t e;
-    const u32x2 c = group_codes(v[u], positive, e);
+    const u32x2 c = group_codes<MASKED>(v[u], positive, e);
     if (id >= all) continue;
     *reinterpret_cast<u32x2 *>(codes + id * 8) = c;
     if (threadIdx.x % 4 == 0) exponents[id / 4] = static_cast<uint8_t>(e);
@@ -71,17 +71,23 @@ __global__ __launch_bounds__(256) void restore_kernel(T *x, long ld, int d, long
     c[u] = *reinterpret_cast<const u32x2 *>(codes + id * 8);
     e[u] = exponents[id / 4];
   }
+  float v[kUnroll][8];
+  bool masked = false;
+#pragma unroll
+  for (int u = 0; u < kUnroll; ++u) masked |= restore_codes(c[u], e[u], v[u]);
+  if (masked) {
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) restore_masked(c[u], v[u]);
+  }
 #pragma unroll
   for (int u = 0; u < kUnroll; ++u) {
     const long id = first + u * 256;
     if (id >= all) continue;
-    float v[8];
-    restore_codes(c[u], e[u], v);
     const Place<FLAT> at(id, pieces);
     T *to = FLAT ? x + id * 8 : x + at.row * ld + at.c;
     typename Vec<T, 8>::loose w;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) w[i] = kept_as<T>(v[i]);
+    for (int i = 0; i < 8; ++i) w[i] = kept_as<T>(v[u][i]);
     const int left = FLAT ? 8 : d - at.c;
     if (left >= 8) {
       *reinterpret_cast<typename Vec<T, 8>::loose *>(to) = w;
@@ -103,13 +109,18 @@ Sizes sizes_of(long ld, long rows, long d) {
   return {pieces, all, d % kGroup == 0 && (ld == d || rows == 1), grid_of((all + 256 * kUnroll - 1) / (256 * kUnroll), 256)};
 }
 
-template <typename T>
+template <typename T, bool MASKED>
 void keep(const void *x, long ld, long rows, int d, bool positive, const Kept &to, hipStream_t stream) {
   const Sizes s = sizes_of(ld, rows, d);
   const T *from = static_cast<const T *>(x);
   uint8_t *codes = const_cast<uint8_t *>(to.codes), *exponents = const_cast<uint8_t *>(to.exponents);
-  if (s.flat) keep_kernel<T, true><<<s.grid, 256, 0, stream>>>(from, ld, d, s.all, s.pieces, positive, codes, exponents);
-  else keep_kernel<T, false><<<s.grid, 256, 0, stream>>>(from, ld, d, s.all, s.pieces, positive, codes, exponents);
+  if (s.flat) keep_kernel<T, true, MASKED><<<s.grid, 256, 0, stream>>>(from, ld, d, s.all, s.pieces, positive, codes, exponents);
+  else keep_kernel<T, false, MASKED><<<s.grid, 256, 0, stream>>>(from, ld, d, s.all, s.pieces, positive, codes, exponents);
+}
+
+template <typename T>
+void keep(const void *x, long ld, long rows, int d, bool positive, bool masked, const Kept &to, hipStream_t stream) {
+  masked ? keep<T, true>(x, ld, rows, d, positive, to, stream) : keep<T, false>(x, ld, rows, d, positive, to, stream);
 }
 
 template <typename T>
@@ -122,11 +133,11 @@ void restore(const Kept &from, long rows, int d, void *x, long ld, hipStream_t s
 
 }  // namespace
 
-hipError_t launch_keep(const void *x, long ld, long rows, int d, int type, bool positive, void *kept, hipStream_t stream) {
+hipError_t launch_keep(const void *x, long ld, long rows, int d, int type, bool positive, bool masked, void *kept, hipStream_t stream) {
   const Kept to = kept_at(kept, rows, d);
-  if (type == TYPE_F32) keep<float>(x, ld, rows, d, positive, to, stream);
-  else if (type == TYPE_BF16) keep<bf16>(x, ld, rows, d, positive, to, stream);
-  else keep<f16>(x, ld, rows, d, positive, to, stream);
+  if (type == TYPE_F32) keep<float>(x, ld, rows, d, positive, masked, to, stream);
+  else if (type == TYPE_BF16) keep<bf16>(x, ld, rows, d, positive, masked, to, stream);
+  else keep<f16>(x, ld, rows, d, positive, masked, to, stream);
   return hipGetLastError();
 }
 

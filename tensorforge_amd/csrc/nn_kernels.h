@@ -141,8 +141,9 @@ hipError_t launch_act_slope(const SlopeParams &p, const PackParams &pack, int ty
 // out[0..d) = sum of `count` shares, in order, rounded to `type`.
 hipError_t launch_share_sum(const float *shares, long count, int d, void *out, int type, hipStream_t stream);
 
-// Rows into 8 bits in groups (nn_common.hpp) and back.  positive: values above zero keep a code above zero.
-hipError_t launch_keep(const void *x, long ld, long rows, int d, int type, bool positive, void *kept, hipStream_t stream);
+// Rows into 8 bits in groups (nn_common.hpp) and back.  positive: values above zero keep a code above zero; masked:
+// minus infinity is kept.
+hipError_t launch_keep(const void *x, long ld, long rows, int d, int type, bool positive, bool masked, void *kept, hipStream_t stream);
 hipError_t launch_restore(const void *kept, long rows, int d, int type, void *x, long ld, hipStream_t stream);
 
 long norm_grad_shares(long rows, long d);

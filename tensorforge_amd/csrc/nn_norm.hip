@@ -278,12 +278,19 @@ __global__ __launch_bounds__(NT *grad_rows(NT, CH)) void rms_norm_grad_kernel(No
     const bool past = row0 + sub >= p.rows;
     const long row = past ? p.rows - 1 : row0 + sub;
     float h[CH][8], g[CH][8];
+    KeptCodes codes[CH];
 #pragma unroll
-    for (int j = 0; j < CH; ++j)
-      load_h8<KEPT, L, T>(p, kept, row, (j * NT + t) * 8, h[j]);
+    for (int j = 0; j < CH; ++j) {
+      if constexpr (KEPT) codes[j] = load_codes8(kept, row, (j * NT + t) * 8);
+      else load8<L>(static_cast<const T *>(p.h) + row * p.h_ld, (j * NT + t) * 8, p.d, h[j]);
+    }
 #pragma unroll
     for (int j = 0; j < CH; ++j)
       load8<L>(static_cast<const T *>(p.dy) + row * p.dy_ld, (j * NT + t) * 8, p.d, g[j]);
+    if constexpr (KEPT) {
+#pragma unroll
+      for (int j = 0; j < CH; ++j) restore8(codes[j], h[j]);
+    }
     float sum = 0.0f, dot = 0.0f;
 #pragma unroll
     for (int j = 0; j < CH; ++j)

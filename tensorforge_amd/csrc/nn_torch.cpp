@@ -269,10 +269,10 @@ void *kept_rows(const Tensor &t, const char *name, int64_t m, int64_t n) {
   return t.data_ptr();
 }
 
-// (x, positive) -> bytes
+// (x, positive, masked) -> bytes
 PyObject *keep8(PyObject *, PyObject *const *a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  count(n, 2);
+  count(n, 3);
   const Tensor &x = tensor(a[0], "x");
   float_type(x, "x");
   no_gradient("keep8", {&x});
@@ -280,7 +280,8 @@ PyObject *keep8(PyObject *, PyObject *const *a, Py_ssize_t n) {
   on_gpu(x, {});
   const On on(x);
   const Tensor kept = fresh(x, {kept_bytes(r.m, r.n)}, ScalarType::Byte);
-  check(tf_keep8(r.p, r.ld, r.m, r.n, type_of(x.scalar_type()), a[1] == Py_True, kept.data_ptr(), on.stream));
+  const auto keep = a[2] == Py_True ? tf_keep8_masked : tf_keep8;
+  check(keep(r.p, r.ld, r.m, r.n, type_of(x.scalar_type()), a[1] == Py_True, kept.data_ptr(), on.stream));
   return wrap(&kept);
   END_HANDLE_TH_ERRORS
 }

@@ -97,9 +97,13 @@ class Kept8:
         return f"Kept8({self.shape}, {self.dtype})"
 
 
-def keep8(x, positive=False):
-    """x in 8 bits (Kept8), 33 bytes for 32 values.  positive: values above zero stay above zero, as relu's gradient needs."""
-    return Kept8(_C.keep8(x, True if positive else False), x.shape, x.dtype)
+def keep8(x, positive=False, masked=False):
+    """x in 8 bits (Kept8), 33 bytes for 32 values.  positive: values above zero stay above zero, as relu's gradient needs.
+
+    A group of 32 that holds an infinity or a NaN comes back as NaN.  masked: minus infinity does not count there; it
+    comes back as itself, and the values beside it as without it.
+    """
+    return Kept8(_C.keep8(x, True if positive else False, True if masked else False), x.shape, x.dtype)
 
 
 def _kept(t, name, like, columns):
@@ -160,7 +164,7 @@ def _saved(t, keep, positive=False):
     """What autograd saves of t: (t, None), or its bytes and what they stand for."""
     if t is None or not keep:
         return t, None
-    kept = keep8(t, positive)
+    kept = keep8(t, positive, masked=True)
     return kept.data, (kept.shape, kept.dtype)
 
 
@@ -209,7 +213,8 @@ def linear(x, w, bias=None, activation="none", residual=None, keep=False, x_scal
     (out, z) with keep=True; both are differentiable.  tile and splits override the choice by sizes
     (tf_linear_args_t in tforge_hip.h); grad_terms is linear_grad's terms under autograd.
     keep8: where the result gets a gradient, x and the pre-activation are kept for it in
-    8 bits (Kept8), relu's with the sign of every value.
+    8 bits (keep8, masked), relu's with the sign of every value.  A group of 32 neighbours with a NaN or plus infinity is
+    NaN in the gradient; minus infinity (a unit masked by its bias) has a slope of 0 and leaves the others alone.
     """
     got = _C.linear(x, w, bias, _act(activation), residual, True if keep else False, x_scale, w_scale, out_dtype, tile,
                     splits)

@@ -1,0 +1,139 @@
+"""Activations kept in 8 bits where their groups hold values that have no integer of their own."""
+
+import numpy as np
+import pytest
+import torch
+
+import nn_reference as ref
+
+pytestmark = pytest.mark.gpu
+
+HALF = [torch.bfloat16, torch.float16]
+DTYPES = [torch.float32, torch.bfloat16, torch.float16]
+KIND = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+INF = float("inf")
+
+
+def _nn():
+    from tensorforge_amd import tforge_nn
+    return tforge_nn
+
+
+def _same(a, b):
+    return torch.equal(a.isnan(), b.isnan()) and torch.equal(torch.where(a.isnan(), 0, a), torch.where(b.isnan(), 0, b))
+
+
+def _masked_bytes(x, positive):
+    """The definition with minus infinity as the integer -128, which counts for no unit; numpy, in 64 bits."""
+    rows, d = x.shape
+    groups = -(-d // 32)
+    v = np.zeros((rows, groups * 32))
+    v[:, :d] = x.double().numpy()
+    v = v.reshape(rows, groups, 32)
+    masked = v == -np.inf
+    v = np.where(masked, 0, v)
+    top = np.abs(v).max(2)
+    bad = ~np.isfinite(top)
+    mantissa, exponent = np.frexp(np.where(bad, 1.0, top))
+    e = np.where(top == 0, -126, np.maximum(np.where(mantissa * 128 < 127.5, exponent - 7, exponent - 6), -126))
+    codes = np.rint(np.ldexp(np.where(bad[..., None], 0, v), -e[..., None]))
+    if positive:
+        codes = np.where((v > 0) & (codes < 1), 1, codes)
+    codes = np.where(bad[..., None], 0, np.where(masked, -128, codes))
+    values = np.where(bad[..., None], np.nan, np.where(masked, -np.inf, np.ldexp(codes, e[..., None])))
+    return (torch.cat([torch.from_numpy(codes.astype(np.int8)).reshape(-1).view(torch.uint8),
+                       torch.from_numpy(np.where(bad, 255, e + 127).astype(np.uint8)).reshape(-1)]),
+            torch.from_numpy(values.reshape(rows, -1)[:, :d]))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("d", [1, 5, 32, 96, 100])
+def test_minus_infinity_is_kept(d, dtype):
+    """Alone, beside finite values (whose unit it does not change), beside plus infinity and NaN, a row and a group of it."""
+    nn = _nn()
+    g = torch.Generator().manual_seed(d)
+    x = torch.randn(9, d, generator=g) * torch.exp(2 * torch.randn(9, d, generator=g))
+    x[0, 0], x[1, ::3], x[2], x[3, :32] = -INF, -INF, -INF, -INF
+    x[4, -1] = -INF
+    if d > 4:
+        x[5, 1], x[5, 2] = -INF, INF
+        x[6, 3], x[6, 4] = float("nan"), -INF
+        x[7, 2] = INF
+    x = x.to(dtype)
+    for positive in (False, True):
+        want, values = _masked_bytes(x, positive)
+        kept = nn.keep8(x.cuda(), positive, masked=True)
+        assert torch.equal(kept.data.cpu(), want)
+        assert _same(kept.restore().cpu().double(), values.to(dtype).double())
+        wide = torch.full((9, d + 3), 7.0, dtype=dtype, device="cuda")
+        wide[:, 1:1 + d] = x.cuda()
+        assert torch.equal(nn.keep8(wide[:, 1:1 + d], positive, masked=True).data.cpu(), want)
+
+
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("activation", ["relu", "gelu", "silu"])
+@pytest.mark.parametrize("m,n,k", [(3, 40, 64), (70, 96, 64), (64, 77, 33), (300, 520, 136), (512, 512, 512)])
+def test_masked_units_have_a_gradient(m, n, k, activation, dtype):
+    """Hidden units that the bias masks with minus infinity (or, in float16, a number past its largest): the units beside them have
+    the gradient that they have from pre-activations kept in 16 bits, at the kept values; the masked ones none."""
+    nn = _nn()
+    g = torch.Generator().manual_seed(m + n)
+    x = torch.randn(m, k, generator=g).to(dtype).cuda()
+    w = (torch.randn(k, n, generator=g) * k ** -0.5).to(dtype).cuda()
+    dy = torch.randn(m, n, generator=g).to(dtype).cuda()
+    masked = torch.zeros(n, dtype=torch.bool)
+    masked[[0, 5, n - 1]] = True
+    b = torch.randn(n, generator=g)
+    b[masked] = -INF
+    if dtype == torch.float16:
+        b[5] = -1e5
+    leaves = [t.clone().requires_grad_() for t in (x, w, b.cuda())]
+    out = nn.linear(*leaves, activation, keep8=True)
+    got = torch.autograd.grad(out, leaves, dy)
+    with torch.no_grad():
+        plain, z = nn.linear(x, w, b.cuda(), activation, keep=True)
+        assert torch.equal(out, plain) and (out[:, masked.cuda()] == 0).all()
+        assert (z[:, masked.cuda()] == -INF).all() and z[:, ~masked.cuda()].isfinite().all()
+        x8, z8 = nn.keep8(x), nn.keep8(z, activation == "relu", masked=True)
+        back = z8.restore()
+        assert torch.equal(back == -INF, z == -INF) and (activation != "relu" or torch.equal(back > 0, z > 0))
+        groups = torch.nn.functional.pad(z.float().where(z > -INF, 0), (0, -n % 32)).view(m, -1, 32)
+        unit = torch.exp2((torch.floor(torch.log2(groups.abs().amax(2) / 127.5)) + 1).clamp_min(-126))
+        half = 0.5 * unit.repeat_interleave(32, 1)[:, :n]
+        fine = ~masked.cuda()
+        off = (back.float() - z.float()).abs()
+        # relu's smallest codes move a value by up to a whole unit
+        assert (off[:, fine] <= half[:, fine] * (2 if activation == "relu" else 1)).all()
+        want = nn.linear_grad(dy, x8.restore(), w, back, activation, torch.float32)
+    dx, dw, db = got
+    assert (dw[:, masked.cuda()] == 0).all() and (db[masked.cuda()] == 0).all()
+    xd, wd, zd, dyd = (t.cpu().double() for t in (x8.restore(), w, back, dy))
+    slope = torch.where(zd == -INF, torch.zeros_like(zd), ref.slope(zd.clamp_min(-1e4), activation))
+    dz = dyd * slope
+    off = 2e-6 * dyd.abs() * (zd > -INF)
+    rounded = off + (ref.U[dtype] * dz.abs() + ref.FLOOR[dtype])
+    size = dz.abs() + rounded
+    for one in (got, want):
+        ref.close(one[0], dz @ wd.t(), (rounded + (2 * n + 8) * ref.u * size) @ wd.abs().t(), dtype)
+        ref.close(one[1], xd.t() @ dz, xd.abs().t() @ (rounded + (2 * m + 8) * ref.u * size), dtype)
+        ref.close(one[2], dz.sum(0), (off + (2 * m + 8) * ref.u * size).sum(0), torch.float32)
+
+
+@pytest.mark.parametrize("dtype", HALF)
+def test_minus_infinity_in_kept_inputs(dtype):
+    """In a kept x or h it goes where it goes from 16 bits: into its own column of dw, its own row of the norm's gradient."""
+    nn = _nn()
+    g = torch.Generator().manual_seed(3)
+    x, dy = (torch.randn(40, c, generator=g).to(dtype) for c in (64, 72))
+    w = torch.randn(64, 72, generator=g).to(dtype).cuda()
+    x[7, 9] = -INF
+    x8 = nn.keep8(x.cuda(), masked=True)
+    a, b = nn.linear_grad(dy.cuda(), x8, w), nn.linear_grad(dy.cuda(), x8.restore(), w)
+    assert torch.equal(a[0], b[0]) and _same(a[1], b[1])
+    rows = torch.ones(64, dtype=torch.bool, device="cuda")
+    rows[9] = False
+    assert a[1][rows].isfinite().all() and not a[1][9].isfinite().any()
+    nw, dn = torch.ones(64, device="cuda"), torch.randn(40, 64, generator=g).to(dtype).cuda()
+    a, b = nn.rms_norm_grad(dn, x8, nw), nn.rms_norm_grad(dn, x8.restore(), nw)
+    assert _same(a[0], b[0]) and _same(a[1], b[1])
+    assert torch.equal(a[0].isnan().any(1).nonzero().flatten().cpu(), torch.tensor([7]))
