@@ -323,8 +323,9 @@ int tf_quantize_rows_to(const void *x, long long x_ld, long long rows, long long
  * group is finite.
  * tf_keep8_masked: minus infinity is the integer -128 instead and counts for no unit.  It comes back
  * as itself, with a slope of 0 under every activation, and its neighbours as without it.
- * tf_restore8 gives the values in `type`: exact in TF_T_F32 and TF_T_BF16; in
- * TF_T_F16 rounded, past 65504 that. */
+ * tf_restore8 gives the values in `type`: exact in TF_T_F32 and TF_T_BF16, in
+ * TF_T_F16 rounded; finite ones past the type's largest number (to which a group's largest
+ * value may have been rounded up) are that. */
 int tf_keep8_bytes(long long rows, long long d, long long *bytes);
 int tf_keep8(const void *x, long long x_ld, long long rows, long long d, int type, int positive, void *kept, void *stream);
 int tf_keep8_masked(const void *x, long long x_ld, long long rows, long long d, int type, int positive, void *kept, void *stream);

@@ -260,12 +260,19 @@ __device__ __forceinline__ uint32_t group_exponent(uint32_t top) {
 
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
-// The values of 8 codes but for minus infinity's; whether there is one, which restore_masked then puts in.
+// The values of 8 codes but for minus infinity's; whether there is one, which restore_masked then puts in.  A largest
+// value that was rounded up past T's numbers (64 units of 2^122) is T's largest (float16's: kept_as); a group that stands for NaN has no bound.
+template <typename T>
 __device__ __forceinline__ bool restore_codes(u32x2 codes, uint32_t exponent, float (&v)[8]) {
   const float unit = __builtin_bit_cast(float, exponent << 23);
+  const float most = exponent == 255 ? __builtin_nanf("") : __is_same(T, bf16) ? 0x1.fep127f : 0x1.fffffep127f;
   const u32x2 u = codes ^ 0x80808080u;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = (static_cast<float>((i < 4 ? u.x : u.y) >> (8 * (i & 3)) & 255u) - 128.0f) * unit;
+  for (int i = 0; i < 8; ++i) {
+    const float code = static_cast<float>((i < 4 ? u.x : u.y) >> (8 * (i & 3)) & 255u);
+    v[i] = (code - 128.0f) * unit;
+    if constexpr (!__is_same(T, f16)) v[i] = __builtin_amdgcn_fmed3f(v[i], -most, most);
+  }
   const u32x2 zero = (u - 0x01010101u) & ~u;  // the lowest byte that is 0 leaves its highest bit
   return (zero.x | zero.y) & 0x80808080u;
 }
@@ -318,10 +325,14 @@ __device__ __forceinline__ KeptCodes load_codes8(const Kept &k, long row, int c)
   const KeptCodes v = {*reinterpret_cast<const u32x2 *>(k.codes + row * length + at), k.exponents[row * k.groups + at / kGroup]};
   return c > at ? KeptCodes{{0, 0}, 1} : v;
 }
+template <typename T>
 __device__ __forceinline__ void restore8(const KeptCodes &k, float (&v)[8]) {
-  if (restore_codes(k.codes, k.exponent, v)) restore_masked(k.codes, v);
+  if (restore_codes<T>(k.codes, k.exponent, v)) restore_masked(k.codes, v);
 }
-__device__ __forceinline__ void load_kept8(const Kept &k, long row, int c, float (&v)[8]) { restore8(load_codes8(k, row, c), v); }
+template <typename T>
+__device__ __forceinline__ void load_kept8(const Kept &k, long row, int c, float (&v)[8]) {
+  restore8<T>(load_codes8(k, row, c), v);
+}
 
 // A kept value in T: a finite one past float16's largest is that.
 template <typename T>

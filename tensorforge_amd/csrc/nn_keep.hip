@@ -74,7 +74,7 @@ __global__ __launch_bounds__(256) void restore_kernel(T *x, long ld, int d, long
   float v[kUnroll][8];
   bool masked = false;
 #pragma unroll
-  for (int u = 0; u < kUnroll; ++u) masked |= restore_codes(c[u], e[u], v[u]);
+  for (int u = 0; u < kUnroll; ++u) masked |= restore_codes<T>(c[u], e[u], v[u]);
   if (masked) {
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) restore_masked(c[u], v[u]);

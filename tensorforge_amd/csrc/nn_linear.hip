@@ -75,7 +75,7 @@ __device__ __forceinline__ void pack_piece(const PackParams &p, long block) {
   if constexpr (KEPT) {
     if (p.kept[q]) {
       float u[8];
-      load_kept8(kept_at(p.from[q], p.rows[q], p.columns[q]), row, c, u);
+      load_kept8<T>(kept_at(p.from[q], p.rows[q], p.columns[q]), row, c, u);
       typename Vec<T, 8>::type w;
 #pragma unroll
       for (int i = 0; i < 8; ++i) w[i] = kept_as<T>(u[i]);
@@ -134,7 +134,7 @@ __global__ __launch_bounds__(256) void act_slope_kernel(SlopeParams p, PackParam
       float g[8], z[8];
       load_slope8(static_cast<const T *>(p.dy) + row * p.dy_ld, c, p.n, g);
       if constexpr (ACT != ACT_NONE) {
-        if (KEPT && p.kept) load_kept8(kept, row, c, z);
+        if (KEPT && p.kept) load_kept8<T>(kept, row, c, z);
         else load_slope8(static_cast<const T *>(p.z) + row * p.z_ld, c, p.n, z);
 #pragma unroll
         for (int i = 0; i < 8; ++i) g[i] *= act_slope<ACT>(z[i]);

@@ -248,7 +248,7 @@ __device__ __forceinline__ void store_weight8(const NormGradParams &p, int c, co
 // 8 elements of the norm's input, in T or kept in 8 bits (8192 x 4096 bfloat16 with dh 40 us against 51 in 16 bits).
 template <bool KEPT, Length L, typename T>
 __device__ __forceinline__ void load_h8(const NormGradParams &p, const Kept &kept, long row, int c, float (&v)[8]) {
-  if constexpr (KEPT) load_kept8(kept, row, c, v);
+  if constexpr (KEPT) load_kept8<T>(kept, row, c, v);
   else load8<L>(static_cast<const T *>(p.h) + row * p.h_ld, c, p.d, v);
 }
 
@@ -289,7 +289,7 @@ __global__ __launch_bounds__(NT *grad_rows(NT, CH)) void rms_norm_grad_kernel(No
       load8<L>(static_cast<const T *>(p.dy) + row * p.dy_ld, (j * NT + t) * 8, p.d, g[j]);
     if constexpr (KEPT) {
 #pragma unroll
-      for (int j = 0; j < CH; ++j) restore8(codes[j], h[j]);
+      for (int j = 0; j < CH; ++j) restore8<T>(codes[j], h[j]);
     }
     float sum = 0.0f, dot = 0.0f;
 #pragma unroll

@@ -137,3 +137,47 @@ def test_minus_infinity_in_kept_inputs(dtype):
     a, b = nn.rms_norm_grad(dn, x8, nw), nn.rms_norm_grad(dn, x8.restore(), nw)
     assert _same(a[0], b[0]) and _same(a[1], b[1])
     assert torch.equal(a[0].isnan().any(1).nonzero().flatten().cpu(), torch.tensor([7]))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("d", [32, 70])
+def test_finite_values_stay_finite(d, dtype):
+    """A group whose largest value rounds to 2^128 (or past 65504) comes back within half a unit, and not as an infinity."""
+    nn = _nn()
+    info = torch.finfo(dtype)
+    x = torch.zeros(6, d, dtype=dtype)
+    near = info.max * (1 - info.eps)
+    x[0, ::3], x[1, 1::2], x[2, 0], x[3, 5] = info.max, -info.max, info.max, near
+    x[4, 7], x[4, 8], x[4, 9] = -near, info.max / 2, -info.max / 3
+    x[5, 3], x[5, 4] = info.max, -INF
+    unit = 2.0 ** (122 if dtype != torch.float16 else 10)
+    for masked in (False, True):
+        back = nn.keep8(x.cuda(), masked=masked).restore().cpu()
+        rows = slice(0, 6 if masked else 5)
+        a, b = back[rows].double(), x[rows].double()
+        fine = b > -INF
+        assert a[fine].isfinite().all() and (a[fine] - b[fine]).abs().max() <= unit / 2
+        assert (a[~fine] == -INF).all()
+        assert back[0, 0] == info.max and back[1, 1] == -info.max
+    assert nn.keep8(x.cuda()).restore()[5, :32].isnan().all()
+
+
+@pytest.mark.parametrize("activation", ["relu", "gelu", "silu"])
+@pytest.mark.parametrize("m", [40, 300])
+def test_gradients_beside_the_largest_number(m, activation):
+    """bfloat16's largest number in a kept x that meets a gradient of zero adds nothing to dw; in a kept z it has a slope of 0 or 1."""
+    nn = _nn()
+    g = torch.Generator().manual_seed(m)
+    x, dy, z = (torch.randn(m, c, generator=g).bfloat16() for c in (64, 96, 96))
+    w = torch.randn(64, 96, generator=g).bfloat16().cuda()
+    top = torch.finfo(torch.bfloat16).max
+    x[3, 5], x[3, 40], dy[3] = top, -top, 0
+    z[7, 3], z[8, 40] = top, -top
+    z[7, :32], z[8, 32:64] = z[7, :32].sign() * top, z[8, 32:64].sign() * top  # the unit is 2^122: only zeros and these are held
+    x8, z8 = nn.keep8(x.cuda()), nn.keep8(z.cuda(), activation == "relu")
+    got = nn.linear_grad(dy.cuda(), x8, w, z8, activation, torch.float32)
+    want = nn.linear_grad(dy.cuda(), x8.restore(), w, z8.restore(), activation, torch.float32)
+    slope = (z8.restore() > 0).float()[7, :32].cpu()
+    assert torch.equal(slope, (z[7, :32] > 0).float())
+    for a, b in zip(got, want):
+        assert a.isfinite().all() and torch.equal(a, b)
