@@ -261,7 +261,8 @@ __device__ __forceinline__ uint32_t group_exponent(uint32_t top) {
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
 // The values of 8 codes but for minus infinity's; whether there is one, which restore_masked then puts in.  A largest
-// value that was rounded up past T's numbers (64 units of 2^122) is T's largest (float16's: kept_as); a group that stands for NaN has no bound.
+// value that was rounded up past T's numbers (64 units of 2^122) is T's largest (float16's, whose groups may be a wider type's: float32's, and then kept_as); a group that stands for NaN has
+// no bound.
 template <typename T>
 __device__ __forceinline__ bool restore_codes(u32x2 codes, uint32_t exponent, float (&v)[8]) {
   const float unit = __builtin_bit_cast(float, exponent << 23);
@@ -270,8 +271,7 @@ __device__ __forceinline__ bool restore_codes(u32x2 codes, uint32_t exponent, fl
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const float code = static_cast<float>((i < 4 ? u.x : u.y) >> (8 * (i & 3)) & 255u);
-    v[i] = (code - 128.0f) * unit;
-    if constexpr (!__is_same(T, f16)) v[i] = __builtin_amdgcn_fmed3f(v[i], -most, most);
+    v[i] = __builtin_amdgcn_fmed3f((code - 128.0f) * unit, -most, most);
   }
   const u32x2 zero = (u - 0x01010101u) & ~u;  // the lowest byte that is 0 leaves its highest bit
   return (zero.x | zero.y) & 0x80808080u;

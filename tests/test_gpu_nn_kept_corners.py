@@ -181,3 +181,27 @@ def test_gradients_beside_the_largest_number(m, activation):
     assert torch.equal(slope, (z[7, :32] > 0).float())
     for a, b in zip(got, want):
         assert a.isfinite().all() and torch.equal(a, b)
+
+
+def test_restored_in_another_type():
+    """The C call: what was kept from float32 or bfloat16, in any of the three types."""
+    from tensorforge_amd import _lib
+    nn = _nn()
+    top = torch.finfo(torch.float32).max
+    x = torch.zeros(5, 64)
+    x[0, 3], x[1, 4], x[2, 5], x[2, 6] = top, -top, -INF, 1.5
+    x[3, 7], x[3, 8] = 1e6, -7e4
+    x[4, 9], x[4, 40] = float("nan"), 3.0
+    for kind in (torch.float32, torch.bfloat16):
+        kept = nn.keep8(x.to(kind).cuda(), masked=True)
+        values = kept.restore().cpu()
+        for dtype in DTYPES:
+            out = torch.empty(5, 64, dtype=dtype, device="cuda")
+            assert _lib.lib().tf_restore8(kept.data.data_ptr(), 5, 64, KIND[dtype], out.data_ptr(), 64, torch.cuda.current_stream().cuda_stream) == 0
+            most = torch.finfo(dtype).max
+            want = torch.where(values > -INF, values.double().clamp(-most, most), values.double())
+            got = out.cpu().double()
+            # the largest of one type may be another's largest: both stand for 2^128
+            got, want = (torch.where(t.abs() > 3e38, torch.where(t.isinf(), t, t.sign() * 3e38), t) for t in (got, want))
+            assert _same(got, want), (kind, dtype)
+            assert out[0, 3].isfinite() and out[1, 4].isfinite() and out[2, 5] == -INF and out[4, :32].isnan().all()
