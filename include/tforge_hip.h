@@ -434,7 +434,9 @@ int tf_linear_grad(const tf_linear_grad_args_t *args, void *stream);
  *   lse[m] = log(sum over n of exp(z[m][n])),  loss[m] = lse[m] - z[m][target[m]]
  * w as tf_linear's.  A row whose target is `ignore` does not count: its loss is 0.  A
  * target outside of 0..n-1 otherwise gives NaN.  Sums over k, logits, exponentials and
- * their sums are float32; infinities and NaN follow the formulas. */
+ * their sums are float32.  A logit of minus infinity adds nothing.  A row with a logit of plus infinity or
+ * NaN is NaN, one whose logits are all minus infinity has that lse and a loss of NaN.  Exponents are taken in
+ * base 2, so that logits past 2.358e38 (2^128 / log2(e)) stand for these infinities. */
 typedef struct {
   const void *x, *w;       /* m x k, k x n in either order                          */
   const long long *target; /* m                                                     */

@@ -87,8 +87,9 @@ __global__ __launch_bounds__(1024) void xent_rows_kernel(RowsParams p) {
     const long long target = p.target[m];
     if (target != p.ignore) {
       counts = 1.0f;
-      // Not lse - logit: large logits would leave their roundings where their difference is small.
-      loss = target >= 0 && target < p.n ? (__builtin_fmaf(-p.target_logit[m], kLog2e, s.x) + log_sum) * kLn2 : __builtin_nanf("");
+      // Not lse - logit: large logits would leave their roundings where their difference is small.  A row without a
+      // logit that counts has none.
+      loss = target >= 0 && target < p.n && s.x != -__builtin_inff() ? (__builtin_fmaf(-p.target_logit[m], kLog2e, s.x) + log_sum) * kLn2 : __builtin_nanf("");
     }
     p.lse[m] = (static_cast<double>(s.x) + log_sum) / kLog2e;
     p.loss[m] = loss;

@@ -297,7 +297,8 @@ def linear_cross_entropy(x, w, target, ignore_index=-100, reduction="mean", keep
     (w = weight.t() of an n x k weight); target (...) is int64.  loss[i] = log(sum of
     exp(logits[i])) - logits[i][target[i]] in float32.  Rows with the target ignore_index do not
     count: their loss is 0, and the mean is over the others (0 if there are none).  Any other
-    target outside of 0..n-1 gives NaN.  reduction: "mean", "sum" or "none".  Returns the
+    target outside of 0..n-1 gives NaN, and so does a row with a logit of plus infinity or without one above minus
+    infinity (magnitudes past 2.358e38 count as these).  reduction: "mean", "sum" or "none".  Returns the
     loss, or (loss, lse, count) with keep=True: what linear_cross_entropy_grad takes (lse is
     float64: a row that is sure of its class takes small differences of it).
     """
