@@ -106,6 +106,12 @@ def keep8(x, positive=False, masked=False):
     return Kept8(_C.keep8(x, True if positive else False, True if masked else False), x.shape, x.dtype)
 
 
+def _tensor(t, name):
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} is not a tensor")
+    return t
+
+
 def _kept(t, name, like, columns):
     """What the native layer takes for an operand that may be kept in 8 bits."""
     if type(t) is Kept8:
@@ -156,7 +162,7 @@ def rms_norm_grad(dy, h, weight, eps=1e-6, dh=None):
     """
     if type(h) is not Kept8:
         return _C.rms_norm_grad(dy, h, weight, eps, dh)
-    dx, dw = _C.rms_norm_grad8(dy, _kept(h, "h", dy, dy.shape[-1] if dy.dim() else 0), weight, eps, dh)
+    dx, dw = _C.rms_norm_grad8(dy, _kept(h, "h", dy, dy.shape[-1] if _tensor(dy, "dy").dim() else 0), weight, eps, dh)
     return _like(dx, h), dw
 
 
@@ -238,7 +244,8 @@ def linear_grad(dy, x, w, z=None, activation="none", bias_dtype=None, want_dx=Tr
     if type(x) is not Kept8 and type(z) is not Kept8:
         return _C.linear_grad(dy, x, w, z, _act(activation), bias_dtype, True if want_dx else False,
                               True if want_dw else False, tile, splits, terms)
-    if w.dim() != 2:
+    _tensor(dy, "dy")
+    if _tensor(w, "w").dim() != 2:
         raise ValueError(f"w is {tuple(w.shape)}, not k x n")
     dx, dw, dbias = _C.linear_grad8(dy, _kept(x, "x", dy, w.shape[0]), w, _kept(z, "z", dy, w.shape[1]), _act(activation), bias_dtype,
                                     True if want_dx else False, True if want_dw else False, tile, splits, terms)

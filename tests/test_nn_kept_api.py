@@ -20,3 +20,24 @@ def test_masked_refusals():
         nn.keep8(x, masked=True)
     with pytest.raises(ValueError, match="no gradient"):
         nn.keep8(x.requires_grad_(), masked=True)
+
+
+def test_what_is_no_tensor_is_a_type_error():
+    """Beside kept activations as beside tensors."""
+    kept = lambda m, n: nn.Kept8(torch.zeros(m * (-(-n // 32)) * 33, dtype=torch.uint8), (m, n), torch.bfloat16)  # noqa: E731
+    dy, w, v = (torch.zeros(n, dtype=torch.bfloat16) for n in ((4, 16), (40, 16), (40,)))
+    for call, words in ((lambda: nn.linear_grad(None, kept(4, 40), w), "dy is not a tensor"),
+                        (lambda: nn.linear_grad([1.0], kept(4, 40), w), "dy is not a tensor"),
+                        (lambda: nn.linear_grad(dy, kept(4, 40), None), "w is not a tensor"),
+                        (lambda: nn.linear_grad(dy, None, w, kept(4, 16), "gelu"), "x is not a tensor"),
+                        (lambda: nn.linear_grad(kept(4, 16), kept(4, 40), w), "dy is not a tensor"),
+                        (lambda: nn.linear_grad(dy, kept(4, 40), kept(40, 16)), "w is not a tensor"),
+                        (lambda: nn.rms_norm_grad(None, kept(4, 40), v), "dy is not a tensor"),
+                        (lambda: nn.rms_norm_grad(kept(4, 40), kept(4, 40), v), "dy is not a tensor"),
+                        (lambda: nn.rms_norm_grad(torch.zeros(4, 40).bfloat16(), kept(4, 40), 1.0), "weight is not a tensor"),
+                        (lambda: nn.keep8([1.0, 2.0]), "x is not a tensor"),
+                        (lambda: nn.keep8(kept(4, 40)), "x is not a tensor"),
+                        (lambda: nn.linear(kept(4, 40), w), "x is not a tensor"),
+                        (lambda: nn.linear_cross_entropy(kept(4, 40), w, torch.zeros(4, dtype=torch.int64)), "x is not a tensor")):
+        with pytest.raises(TypeError, match=words):
+            call()
