@@ -49,3 +49,50 @@ def test_logits_at_the_ends_of_float32(classes, rows):
         loss, lse, _ = nn.linear_cross_entropy(x, w, target, reduction="none", keep=True)
         # row 0 meets the highest with a zero: 0 * infinity is NaN too
         assert loss[0].isfinite() == (highest < INF) and loss[1:].isnan().all() and lse[1:].isnan().all()
+
+
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("order", [0, 1])
+@pytest.mark.parametrize("m,n", [(64, 1_100_041), (33, 2_200_000)])
+def test_two_terms_over_several_pieces(m, n, order, dtype):
+    """Rows few enough for dz's second term and classes enough for two pieces, the last one narrower: dx's halves added up over the
+    pieces, dw from a column's offset.  Against float64; every result is rounded once (half a step at most), what dz's second
+    rounding and the float32 sums leave is a tenth of that in the norm."""
+    nn = _nn()
+    k = 64
+    g = torch.Generator(device="cuda").manual_seed(n)
+    x = torch.randn(m, k, generator=g, device="cuda").to(dtype)
+    w = (torch.randn((k, n) if order == 0 else (n, k), generator=g, device="cuda") * k ** -0.5).to(dtype)
+    wc = w if order == 0 else w.t()
+    width = -(-(-(-n // 2)) // 256) * 256  # of the first piece
+    target = torch.randint(0, n, (m,), generator=g, device="cuda")
+    target[:6] = torch.tensor([0, width - 1, width, width + 1, n - 1, IGNORE], device="cuda")
+    z = torch.matmul(x.double(), wc.double().contiguous())
+    lse = torch.logsumexp(z, 1)
+    loss, got_lse, _ = nn.linear_cross_entropy(x, wc, target, reduction="none", keep=True)
+    counts = target != IGNORE
+    at = target.clamp_min(0)
+    want = torch.where(counts, lse - z[torch.arange(m), at], torch.zeros_like(lse))
+    # k of 64: logits off by 2k + 8 roundings of their products at most; exponentials and their sum by 128 + n/4096 of them
+    off = ((2 * k + 8) * (x.double().abs() @ wc.double().abs().contiguous()).amax(1) + 150 + n / 4096 + 8 * lse.abs()) * ref.u
+    assert ((got_lse - lse).abs() <= off).all() and ((loss.double() - want).abs() <= 2 * off).all()
+    d = torch.exp(z - lse[:, None])
+    del z
+    d[torch.arange(m), at] -= 1
+    d *= counts[:, None]
+    for rows in (True, False):
+        # dloss large enough that float16 holds the other classes' gradients (1e-6 of it) as normal numbers
+        dloss = (torch.rand(m, generator=g, device="cuda") + 0.5) * 1024 if rows else torch.full((), 1024.0, device="cuda")
+        dz = d * dloss.double().reshape(-1, 1)
+        dx, dw = nn.linear_cross_entropy_grad(dloss, x, wc, target, got_lse)
+        full = torch.matmul(dz, wc.t().double().contiguous())
+        assert float((dx.double() - full).norm()) < 1.1 * ref.U[dtype] * float(full.norm())
+        assert (dx[5] == 0).all()
+        full = torch.matmul(x.t().double().contiguous(), dz)
+        off = dw.double() - full
+        assert float(off.norm()) < 1.1 * ref.U[dtype] * float(full.norm())
+        # and column by column: no column of another piece, none left out (float16: half a spacing of small numbers besides)
+        size = full.norm(dim=0)
+        assert bool((off.norm(dim=0) <= 2 * ref.U[dtype] * size + 2.0 ** -25 * k ** 0.5).all())
+        del full, off, dw, dx
+    torch.cuda.empty_cache()
