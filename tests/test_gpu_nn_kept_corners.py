@@ -210,3 +210,36 @@ def test_restored_in_another_type():
                 assert out[0, 3].isfinite() and out[1, 4].isfinite()
             else:
                 assert out[0, :32].isnan().all() and out[1, 4] == -INF
+
+
+@pytest.mark.parametrize("activation", ["none", "relu", "gelu", "silu"])
+@pytest.mark.parametrize("m,n,k", [(0, 40, 64), (5, 0, 64), (5, 40, 0), (1, 1, 1), (7, 33, 65), (130, 96, 64)])
+def test_autograd_of_every_size(m, n, k, activation):
+    """keep8 with and without the kept z's own loss, without rows, columns or a depth, on rows of leading dimensions: the gradients are
+    those of the gradient calls at the kept values."""
+    nn = _nn()
+    g = torch.Generator().manual_seed(m + n + k)
+    make = lambda *s: torch.randn(*s, generator=g).bfloat16().cuda()  # noqa: E731
+    x, w, b, r = make(1, m, k), make(k, n), make(n), make(m, n)
+    dy, dz = make(1, m, n), make(1, m, n)
+    for keep in (False, True):
+        leaves = [t.clone().requires_grad_() for t in (x, w, b, r)]
+        got = nn.linear(leaves[0], leaves[1], leaves[2], activation, leaves[3], keep=keep, keep8=True)
+        outs, ups = (list(got), [dy, dz]) if keep else ([got], [dy])
+        grads = torch.autograd.grad(outs, leaves, ups)
+        with torch.no_grad():
+            out, z = nn.linear(x, w, b, activation, r, keep=True)
+            assert torch.equal(outs[0], out) and (not keep or torch.equal(outs[1], z))
+            x8, z8 = nn.keep8(x, masked=True), nn.keep8(z, activation == "relu", masked=True)
+            want = nn.linear_grad(dy, x8, w, None if activation == "none" else z8, activation, torch.bfloat16)
+            if keep:
+                want = [p + q for p, q in zip(want, nn.linear_grad(dz, x8, w, bias_dtype=torch.bfloat16))]
+        for p, q in zip(grads, (*want, dy.view(m, n))):
+            assert torch.equal(p, q) and not p.isnan().any()
+    nw = torch.ones(k, device="cuda", requires_grad=True)
+    h = x.clone().requires_grad_()
+    y, _ = nn.rms_norm(h, nw, keep8=True)
+    a = torch.autograd.grad(y, [h, nw], make(1, m, k).mul_(0).add_(1))
+    with torch.no_grad():
+        c = nn.rms_norm_grad(torch.ones_like(x), nn.keep8(x), nw)
+    assert all(torch.equal(p, q) for p, q in zip(a, c))

@@ -96,3 +96,71 @@ def test_two_terms_over_several_pieces(m, n, order, dtype):
         assert bool((off.norm(dim=0) <= 2 * ref.U[dtype] * size + 2.0 ** -25 * k ** 0.5).all())
         del full, off, dw, dx
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
+@pytest.mark.parametrize("m,n,k", [(0, 5, 8), (5, 1, 8), (5, 7, 0), (1, 1, 1), (65, 3, 2)])
+def test_autograd_of_every_size(m, n, k, reduction):
+    """No rows, one class, no depth: as the gradient call; every row ignored gives zeros."""
+    nn = _nn()
+    g = torch.Generator().manual_seed(m + n + k)
+    x, w = torch.randn(m, k, generator=g).bfloat16().cuda(), torch.randn(n, k, generator=g).bfloat16().cuda()
+    for target in (torch.randint(0, n, (m,), generator=g).cuda(), torch.full((m,), IGNORE, device="cuda")):
+        leaves = [x.clone().requires_grad_(), w.clone().requires_grad_()]
+        loss = nn.linear_cross_entropy(leaves[0], leaves[1].t(), target, reduction=reduction)
+        up = torch.rand(loss.shape, generator=g).cuda()
+        got = torch.autograd.grad(loss, leaves, up)
+        with torch.no_grad():
+            again, lse, count = nn.linear_cross_entropy(x, w.t(), target, reduction=reduction, keep=True)
+            dx, dw = nn.linear_cross_entropy_grad(up, x, w.t(), target, lse, count)
+        assert torch.equal(loss, again) and torch.equal(got[0], dx) and torch.equal(got[1], dw.t())
+        want = torch.nn.functional.cross_entropy((x.double().cpu() @ w.double().cpu().t()), target.cpu(), reduction="none")
+        if reduction == "none":
+            assert ((loss.cpu().double() - want).abs() <= 1e-5 * (1 + want)).all()
+        assert all(t.isfinite().all() for t in got)
+        if m and target[0] == IGNORE:
+            assert (got[0] == 0).all() and (got[1] == 0).all() and (loss == 0).all()
+        if n == 1:
+            # The one class's pair is t, logit * log2(e) rounded, and exp2(logit * log2(e) - t): an exponent of at most u * |t| / 2
+            # (|t| < 16 here), an ulp of the exponential, one of the logarithm: 8u * ln 2 + 4u of 1, in p - 1 too; a row of dw
+            # adds m of them.
+            off = 12 * ref.u * (up.abs().sum().item() + 1)
+            assert (loss.abs() <= 12 * ref.u * max(1, m)).all() and (got[0].abs() <= off * w.float().abs().max()).all()
+            assert (got[1].abs() <= off * x.float().abs().max()).all()
+
+
+def test_calls_at_once_from_threads_and_streams():
+    """Steps through autograd from four threads on streams of their own give the bits of steps alone."""
+    import threading
+    nn = _nn()
+    shapes = [(33, 700, 64), (200, 520, 136), (65, 1001, 77), (16, 4000, 256)]
+    data = []
+    for i, (m, n, k) in enumerate(shapes):
+        g = torch.Generator().manual_seed(i)
+        data.append((torch.randn(m, k, generator=g).half().cuda(), (torch.randn(n, k, generator=g) * k ** -0.5).half().cuda(),
+                     torch.randint(0, n, (m,), generator=g).cuda(), torch.randn(k, generator=g).cuda()))
+
+    def step(x, w, t, nw):
+        a, b, c = (v.clone().requires_grad_() for v in (x, w, nw))
+        y, _ = nn.rms_norm(a, c, keep8=True)
+        loss = nn.linear_cross_entropy(nn.linear(y, b.t(), None, "gelu", keep8=True), torch.eye(w.shape[0], dtype=w.dtype, device="cuda"), t)
+        return (loss.detach(), *torch.autograd.grad(loss, (a, b, c)))
+
+    alone = [step(*d) for d in data]
+    torch.cuda.synchronize()
+    bad, streams = [], [torch.cuda.Stream() for _ in data]
+
+    def run(i):
+        with torch.cuda.stream(streams[i]):
+            for _ in range(8):
+                got = step(*data[i])
+                streams[i].synchronize()
+                if not all(torch.equal(p, q) for p, q in zip(got, alone[i])):
+                    bad.append(i)
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(len(data))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad
