@@ -84,8 +84,8 @@ struct XentParams : GemmParams {
   const long long *target = nullptr;
   long long ignore = 0;
   int vocabulary = 0, column0 = 0;  // all columns, and this piece's first
-  // XENT_STATS: of each row the largest logit of a tile's columns and the sum of exp(logit - largest), tiles_n x m
-  // pairs; and the target's logit.
+  // XENT_STATS: of each row and a tile's columns t, the largest logit times log2(e) as it was rounded, and the sum of
+  // exp2(logit * log2(e) - t): tiles_n x m pairs.  And the target's logit, as it is.
   float *stats = nullptr, *target_logit = nullptr;
   // XENT_SLOPE: out = (exp(logit - lse) - [column is the target]) * unit, zeros up to a multiple of 8 columns.  One dloss
   // for all rows: the unit is `power`, and dloss / count / power comes with XENT_SUM.  A row's own: dloss / count, in

@@ -286,7 +286,7 @@ inline long long copy_of(Operand &o, int size, char *to, PackParams &pack) {
   return bytes;
 }
 
-// z, in 8 bits, where it is written with the product (fused_z), else null.
+// Whether the product's own kernel can write z in 8 bits: unsplit, loads straight into LDS, more than a few rows.
 inline bool fused_z(const Choice &c) { return c.dma && c.plan.splits == 1 && c.plan.tile != TILE_ROWS; }
 
 inline hipError_t run_product(Product &q, int tile, int splits, void *workspace, long long bytes, hipStream_t stream, void *z8 = nullptr) {

@@ -235,7 +235,8 @@ __global__ __launch_bounds__(256) void xent_outer_kernel(OuterParams q, XentPara
 
 template <typename T, bool TWO_R, int COLUMNS>
 void launch_outer_as(const OuterParams &q, const XentParams &p, hipStream_t stream) {
-  // As many workgroups down the rows as keep four on every CU.
+  // As many workgroups down the rows as make four for each CU.  Of 64 columns they are there at once; of 256 their LDS (16 KB
+  // and 16 KB for each 32 rows of x and term of C) lets 2 to 5 be, and the others follow.
   const long across = (q.columns + COLUMNS - 1L) / COLUMNS, down = std::max(1L, std::min((1024 + across - 1) / across, (q.rows + 63L) / 64));
   const dim3 grid(static_cast<unsigned>(across), static_cast<unsigned>(down));
   if (q.k <= 32) xent_outer_kernel<T, TWO_R, 1, COLUMNS><<<grid, 256, 0, stream>>>(q, p);
