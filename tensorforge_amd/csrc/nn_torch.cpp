@@ -165,16 +165,9 @@ PyObject *tuple(std::initializer_list<const Tensor *> all) {
 
 void count(Py_ssize_t got, Py_ssize_t want) { TORCH_CHECK_TYPE(got == want, "takes ", want, " arguments, got ", got); }
 
-long long integer64(PyObject *o, const char *name) {
-  int past = 0;
-  const long long v = PyLong_AsLongLongAndOverflow(o, &past);
-  if (v == -1 && PyErr_Occurred()) throw python_error();
-  TORCH_CHECK_VALUE(!past, name, " is out of range");
-  return v;
-}
-
 int integer(PyObject *o, const char *name) {
-  const long long v = integer64(o, name);
+  const long v = PyLong_AsLong(o);
+  if (v == -1 && PyErr_Occurred()) throw python_error();
   TORCH_CHECK_VALUE(v == static_cast<int>(v), name, " = ", v, " is out of range");
   return static_cast<int>(v);
 }
@@ -304,7 +297,8 @@ PyObject *restore8(PyObject *, PyObject *const *a, Py_ssize_t n) {
   const Py_ssize_t dims = PyTuple_GET_SIZE(a[1]);
   TORCH_CHECK_VALUE(dims > 0, "the shape has no dimension");
   for (Py_ssize_t i = 0; i < dims; ++i) {
-    const int64_t s = integer64(PyTuple_GET_ITEM(a[1], i), "a size of the shape");
+    const int64_t s = PyLong_AsLongLong(PyTuple_GET_ITEM(a[1], i));
+    if (s == -1 && PyErr_Occurred()) throw python_error();
     TORCH_CHECK_VALUE(s >= 0 && s <= (1LL << 30) && (i + 1 == dims || s * m <= (1LL << 30)), "the shape's sizes are out of range");
     size.push_back(s);
     if (i + 1 < dims) m *= s;
@@ -478,6 +472,12 @@ const long long *targets(const Tensor &t, const Tensor &x) {
   return reinterpret_cast<const long long *>(t.data_ptr<int64_t>());
 }
 
+long long integer64(PyObject *o) {
+  const long long v = PyLong_AsLongLong(o);
+  if (v == -1 && PyErr_Occurred()) throw python_error();
+  return v;
+}
+
 // The loss of checked operands, and what its gradient takes.
 struct Xent {
   Tensor loss, lse, count;
@@ -589,7 +589,7 @@ PyObject *linear_xent(PyObject *, PyObject *const *a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   count(n, 5);
   const Tensor &x = tensor(a[0], "x"), &w = tensor(a[1], "w"), &target = tensor(a[2], "target");
-  const int64_t ignore = integer64(a[3], "ignore_index"), reduction = integer(a[4], "reduction");
+  const int64_t ignore = integer64(a[3]), reduction = integer(a[4], "reduction");
   if (wants_grad({&x, &w})) {
     Rows xr;
     Weights wr;
@@ -609,7 +609,7 @@ PyObject *linear_xent_grad(PyObject *, PyObject *const *a, Py_ssize_t n) {
   const Tensor &dloss = tensor(a[0], "dloss"), &x = tensor(a[1], "x"), &w = tensor(a[2], "w"), &target = tensor(a[3], "target");
   const Tensor &lse = tensor(a[4], "lse"), *number = optional(a[5], "count");
   no_gradient("linear_cross_entropy_grad", {&dloss, &x, &w, &lse, number});
-  const auto [dx, dw] = xent_grad(dloss, x, w, target, lse, number, integer64(a[6], "ignore_index"), a[7] == Py_True, a[8] == Py_True);
+  const auto [dx, dw] = xent_grad(dloss, x, w, target, lse, number, integer64(a[6]), a[7] == Py_True, a[8] == Py_True);
   return tuple({dx.defined() ? &dx : nullptr, dw.defined() ? &dw : nullptr});
   END_HANDLE_TH_ERRORS
 }

@@ -41,18 +41,3 @@ def test_what_is_no_tensor_is_a_type_error():
                         (lambda: nn.linear_cross_entropy(kept(4, 40), w, torch.zeros(4, dtype=torch.int64)), "x is not a tensor")):
         with pytest.raises(TypeError, match=words):
             call()
-
-
-def test_numbers_past_64_bits_are_value_errors():
-    x, w, t = torch.zeros(4, 8, dtype=torch.bfloat16), torch.zeros(8, 16, dtype=torch.bfloat16), torch.zeros(4, dtype=torch.int64)
-    rows, one = torch.zeros(4, dtype=torch.float64), torch.ones(())
-    for n in (1 << 63, 1 << 70, -(1 << 70)):
-        for call in (lambda: nn.linear_cross_entropy(x, w, t, ignore_index=n), lambda: nn.linear_cross_entropy_grad(one, x, w, t, rows, ignore_index=n),
-                     lambda: nn.linear(x, w, tile=n), lambda: nn.linear(x, w, splits=n), lambda: nn.linear_grad(torch.zeros(4, 16).bfloat16(), x, w, terms=n),
-                     lambda: nn.Kept8(torch.zeros(33, dtype=torch.uint8), (n, 1), torch.float16).restore()):
-            with pytest.raises(ValueError, match="out of range"):
-                call()
-    with pytest.raises(TypeError):
-        nn.linear_cross_entropy(x, w, t, ignore_index=1.5)
-    with pytest.raises(ValueError, match="not on a GPU"):
-        nn.linear_cross_entropy(x, w, t, ignore_index=-(1 << 63))
