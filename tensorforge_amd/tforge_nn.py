@@ -26,8 +26,8 @@ second derivative raises RuntimeError.  Neither have the 8-bit results: with an 
 that requires a gradient, quantize_rows, rms_norm into 8 bits, 8-bit products and the
 gradient calls raise ValueError unless they run under torch.no_grad(); so does keep8.
 
-Bad arguments raise ValueError or TypeError before any work; errors of the
-library raise RuntimeError with its message.
+Bad arguments raise ValueError or TypeError before any work (a number past 64 bits
+OverflowError); errors of the library raise RuntimeError with its message.
 """
 
 import functools
